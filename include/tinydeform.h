@@ -346,6 +346,59 @@ TD_API int td_test_peer_wait(void* control, int world, int rank, long long limit
                              size_t err_len);
 
 /*
+ * Softmax attention: the decoder layer's self attention (and any attention of queries over keys of another length).
+ *   out[b, i, h] = sum_j P_ij value[b, j, hk],  P_i = softmax over the open keys j of scale * query[b,i,h] . key[b,j,hk]
+ * with hk = h / (H / Hk). No counterpart in upstream, whose callers use torch for it.
+ *   query [B, Q, H, D], key and value [B, N, Hk, D]; strides: 9 element strides (batch, token, head of query, of key,
+ *   of value; the innermost stride is 1). H a multiple of Hk, D <= TD_MAX_HEAD_DIM.
+ *   attn_mask: NULL, or bytes, nonzero = query i may not use key j, at b * mask_strides[0] + h * mask_strides[1] +
+ *   i * mask_strides[2] + j (a stride of 0 shares the mask); key_padding_mask: NULL or [B, N], nonzero = no key there
+ *   (its key and value rows are not used at all, whatever they hold); causal: query i uses keys j <= i + (N - Q).
+ *   out [B, Q, H * D] (written; a query without any open key gets zeros).
+ *   lse: NULL, or [B, H, Qp] with Qp = Q rounded up to 128, float32 (float64 for TD_F64), written: the base-2
+ *   logarithm of each row's sum of exponentials, +infinity for rows without an open key and behind the last query.
+ *   scale > 0. workspace: td_attention_workspace_bytes(..., backward = 0) bytes, 16-byte aligned (NULL when 0).
+ *
+ * td_attention_backward: from the forward's inputs, its out and lse, and grad_out [B, Q, H * D], writes grad_query
+ * [B, Q, H, D], grad_key and grad_value [B, N, Hk, D] (dense). The probabilities are formed again from lse; sums over
+ * queries, keys and the heads of a group are taken in a fixed order (no atomics). workspace: as above with
+ * backward = 1. mask_b, mask_h: 1, or the mask's own batch and head counts (0 without an attn_mask).
+ */
+#define TD_MAX_HEAD_DIM 128
+TD_API size_t td_attention_workspace_bytes(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
+                                           int64_t D, int64_t mask_b, int64_t mask_h, int has_padding, int backward);
+TD_API int td_attention_forward(int dtype, const void* query, const void* key, const void* value,
+                                const int64_t* strides, const uint8_t* attn_mask, const int64_t* mask_strides,
+                                const uint8_t* key_padding_mask, void* out, void* lse, int64_t B, int64_t Q,
+                                int64_t N, int64_t H, int64_t Hk, int64_t D, double scale, int causal,
+                                void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
+TD_API int td_attention_backward(int dtype, const void* query, const void* key, const void* value,
+                                 const int64_t* strides, const uint8_t* attn_mask, const int64_t* mask_strides,
+                                 const uint8_t* key_padding_mask, const void* out, const void* lse,
+                                 const void* grad_out, void* grad_query, void* grad_key, void* grad_value, int64_t B,
+                                 int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, double scale, int causal,
+                                 void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
+
+/*
+ * Layer norm over the last dimension of x [rows, C], the residual added inside: s = x + residual (residual NULL: x),
+ * y = (s - mean(s)) / sqrt(var(s) + eps) * weight + bias (bias NULL: none). s is not rounded to the dtype; sums are
+ * float32 (float64 for TD_F64). mean, rstd: NULL, or [rows] in that type, written for the backward. 1 <= C <=
+ * TD_MAX_CHANNELS. No counterpart in upstream.
+ *
+ * td_layer_norm_backward: grad_x [rows, C] (the gradient of x and of residual alike), grad_weight and grad_bias [C]
+ * (either may be NULL), the column sums in a fixed order (no atomics). workspace:
+ * td_layer_norm_workspace_bytes(dtype, rows, C) bytes on the current device, 8-byte aligned.
+ */
+TD_API int td_layer_norm_forward(int dtype, const void* x, const void* residual, const void* weight,
+                                 const void* bias, void* y, void* mean, void* rstd, int64_t rows, int64_t C,
+                                 double eps, void* stream, char* err, size_t err_len);
+TD_API size_t td_layer_norm_workspace_bytes(int dtype, int64_t rows, int64_t C);
+TD_API int td_layer_norm_backward(int dtype, const void* grad_y, const void* x, const void* residual,
+                                  const void* weight, const void* mean, const void* rstd, void* grad_x,
+                                  void* grad_weight, void* grad_bias, int64_t rows, int64_t C, void* workspace,
+                                  size_t workspace_bytes, void* stream, char* err, size_t err_len);
+
+/*
  * Kernel policy for every later call in this process: TD_POLICY_BEST (default) uses the tcgen05 tensor-core
  * kernels wherever the shapes allow; TD_POLICY_CUDA_CORES keeps every call on the CUDA-core kernels (parity tests
  * run both). No counterpart in upstream, which has only CUDA-core kernels. Returns the previous policy.

@@ -21,6 +21,12 @@ Around the operator (additions; upstream has only the operator):
     pack_sampling_weights(offset_weight, offset_bias, attention_weight, attention_bias) -> the packed pair
 
 the whole MSDeformAttn layer (query -> offsets and softmaxed weights -> attention -> output_proj) in one library call.
+The rest of a decoder layer's attention half, forward and backward:
+
+    attention(query, key, value, key_padding_mask, attn_mask, causal, scale)   -> [B, Q, H * D]
+    layer_norm(x, weight, bias, residual, eps)                                -> x's shape
+
+the self attention among the queries, and the norm over a sublayer's result plus its residual.
 
 CPU tensors run ``ma_deform_attn_reference`` (as upstream does). CUDA tensors run only the native library; if it is
 missing, the call raises. Unlike upstream (inference only), this package's ``ma_deform_attn`` differentiates CUDA
@@ -33,11 +39,13 @@ import functools
 import torch
 
 from . import _native
-from .autograd import linear_train, ma_deform_attn_train, producer_train
-from .reference import deform_attn_layer_reference, ma_deform_attn_reference, sampling_producer_reference
+from .autograd import AttentionFunction, LayerNormFunction, linear_train, ma_deform_attn_train, producer_train
+from .reference import (attention_reference, deform_attn_layer_reference, layer_norm_reference,
+                        ma_deform_attn_reference, sampling_producer_reference)
 
 __all__ = ['ma_deform_attn', 'ma_deform_attn_reference', 'choose_mode', 'deform_attn_layer', 'sampling_producer',
-           'pack_sampling_weights', 'deform_attn_layer_reference', 'sampling_producer_reference']
+           'pack_sampling_weights', 'deform_attn_layer_reference', 'sampling_producer_reference', 'attention',
+           'attention_reference', 'layer_norm', 'layer_norm_reference']
 __version__ = '0.1.1+b200'
 
 MODES = ('auto', 'fused', 'project')
@@ -200,7 +208,8 @@ def sampling_producer(query, reference_points, spatial_shapes, n_heads, n_points
 
 def deform_attn_layer(query, reference_points, memory, spatial_shapes, level_start_index, n_heads, n_points,
                       sampling_weight, sampling_bias, value_weight, value_bias, output_weight=None, output_bias=None,
-                      value_padding_mask=None, mode='auto'):
+                      value_padding_mask=None, mode='auto', residual=None, norm_weight=None, norm_bias=None,
+                      norm_eps=1e-5):
     """One multi-scale deformable attention layer (the forward of Deformable-DETR's MSDeformAttn, whose core is
     ma_deform_attn): [B, Q, H * D], or [B, Q, C_out] with output_weight.
 
@@ -208,6 +217,9 @@ def deform_attn_layer(query, reference_points, memory, spatial_shapes, level_sta
     sampling_weight / sampling_bias: pack_sampling_weights of the offset and attention-weight projections;
     value_weight / value_bias: value_proj; output_weight / output_bias: output_proj (optional);
     value_padding_mask: bool [B, N], True = padded token. Same result as deform_attn_layer_reference.
+
+    norm_weight / norm_bias / norm_eps and residual (the layer's output shape): the decoder layer's norm behind the
+    attention, layer_norm(output, norm_weight, norm_bias, residual, norm_eps), as the call's last kernel.
 
     CUDA, mode 'project' (or 'auto' choosing it): three kernels in one library call (query projection, value
     projection, and the sampler computing the softmax and locations in its prologue), plus the output projection.
@@ -217,6 +229,13 @@ def deform_attn_layer(query, reference_points, memory, spatial_shapes, level_sta
         raise ValueError(f'mode must be one of {MODES}, got {mode!r}')
     if output_bias is not None and output_weight is None:
         raise ValueError('output_bias needs output_weight')
+    if norm_weight is None and (norm_bias is not None or residual is not None):
+        raise ValueError('norm_bias and residual need norm_weight')
+    if norm_weight is not None:
+        out = deform_attn_layer(query, reference_points, memory, spatial_shapes, level_start_index, n_heads, n_points,
+                                sampling_weight, sampling_bias, value_weight, value_bias, output_weight, output_bias,
+                                value_padding_mask, mode)
+        return layer_norm(out, norm_weight, norm_bias, residual, norm_eps)
     if not memory.is_cuda:
         return deform_attn_layer_reference(query, reference_points, memory, spatial_shapes, level_start_index,
                                            n_heads, n_points, sampling_weight, sampling_bias, value_weight,
@@ -236,3 +255,45 @@ def deform_attn_layer(query, reference_points, memory, spatial_shapes, level_sta
     return _native.layer_forward(query, reference_points, memory, spatial_shapes, level_start_index, n_heads,
                                  n_points, sampling_weight, sampling_bias, value_weight, value_bias, output_weight,
                                  output_bias, value_padding_mask, order=mode)
+
+
+def attention(query, key, value, key_padding_mask=None, attn_mask=None, causal=False, scale=None):
+    """Softmax attention: the self attention among a decoder's queries, or any attention over N keys; [B, Q, H * D].
+
+    query [B, Q, H, D]; key, value [B, N, Hk, D], H a multiple of Hk (query head h uses key head h // (H // Hk)),
+    D <= 128; float32, float16, bfloat16 or float64. Views of a packed projection are read in place.
+    key_padding_mask: bool [B, N], True = no key there (its rows may hold anything). attn_mask: bool [Q, N] or
+    [B or 1, H or 1, Q, N], True = query i may not use key j (DINO's denoising mask); what a blocked pair's key and
+    value hold must still be finite. causal: query i uses the keys up to i + N - Q. A query left without any key gets
+    zeros, and passes no gradient. scale: positive, 1 / sqrt(D) unless given.
+
+    CUDA tensors run this library's kernels, forward and backward (no probabilities are kept; sums run in float32,
+    float64 for float64; gradients are the same bits every time); CPU tensors run attention_reference. The backward
+    can be captured in a CUDA graph with the forward; as with every autograd backward under capture, no graph of the
+    same leaves that was built outside the capture may be alive then.
+    """
+    if scale is None:
+        scale = query.shape[-1] ** -0.5 if query.dim() == 4 and query.shape[-1] > 0 else 1.0
+    _native.check_attention(query, key, value, key_padding_mask, attn_mask, scale)
+    if not query.is_cuda:
+        return attention_reference(query, key, value, key_padding_mask, attn_mask, causal, scale)
+    _native.load()
+    if _wants_grad(query, key, value):
+        return AttentionFunction.apply(query, key, value, key_padding_mask, attn_mask, bool(causal), float(scale))
+    return _native.attention_forward(query, key, value, key_padding_mask, attn_mask, bool(causal), float(scale))[0]
+
+
+def layer_norm(x, weight, bias=None, residual=None, eps=1e-5):
+    """Layer norm of x + residual over the last dimension (up to 8192 wide), in x's shape and dtype.
+
+    The sum is not rounded before the norm, and the statistics are float32 (float64 for float64). CUDA tensors run
+    this library's kernels, forward and backward (the column sums of the weight's and bias's gradients in a fixed
+    order); CPU tensors run layer_norm_reference.
+    """
+    _native.check_layer_norm(x, weight, bias, residual, eps)
+    if not x.is_cuda:
+        return layer_norm_reference(x, weight, bias, residual, eps)
+    _native.load()
+    if _wants_grad(x, weight, bias, residual):
+        return LayerNormFunction.apply(x, weight, bias, residual, float(eps))
+    return _native.layer_norm_forward(x, weight, bias, residual, float(eps))[0]

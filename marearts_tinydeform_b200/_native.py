@@ -19,11 +19,23 @@ TD_F32, TD_F16, TD_BF16, TD_F64 = 0, 1, 2, 3
 DTYPE_CODE = {torch.float32: TD_F32, torch.float16: TD_F16, torch.bfloat16: TD_BF16, torch.float64: TD_F64}
 MAX_LEVEL_POINTS = 64
 MAX_CHANNELS = 8192
+MAX_HEAD_DIM = 128
+ATTN_ROW_PAD = 128  # rows of the attention's lse hold Q rounded up to this
 INT32_MAX = 2 ** 31 - 1
 
 # exported symbol -> (restype, argtypes); the list is also what tests check the .so against
 _i64, _vp, _ip, _sz, _cp = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_char_p
 SIGNATURES = {
+    'td_attention_workspace_bytes': (_sz, [_ip, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ip, _ip]),
+    'td_attention_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
+                                   _i64, ctypes.c_double, _ip, _vp, _sz, _vp, _cp, _sz]),
+    'td_attention_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
+                                    _i64, _i64, _i64, _i64, ctypes.c_double, _ip, _vp, _sz, _vp, _cp, _sz]),
+    'td_layer_norm_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp, _cp,
+                                    _sz]),
+    'td_layer_norm_workspace_bytes': (_sz, [_ip, _i64, _i64]),
+    'td_layer_norm_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp, _cp,
+                                     _sz]),
     'td_fused_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _cp, _sz]),
     'td_sample_forward': (_ip, [_ip, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
@@ -723,3 +735,182 @@ def linear_grad_weight(grad_out, x, with_bias=False):
         _call(lib.td_linear_grad_weight, code, _ptr(g), _ptr(xs), _ptr(grad_w), _ptr(grad_b), M, Nout, K, _ptr(ws),
               ws_bytes, _stream(x.device))
     return grad_w, grad_b
+
+
+def check_attention(query, key, value, key_padding_mask, attn_mask, scale):
+    """The attention's argument contract, on any device; returns B, Q, N, H, Hk, D."""
+    if query.dim() != 4 or key.dim() != 4 or value.dim() != 4:
+        raise RuntimeError('query must be [B, Q, H, D], key and value [B, N, Hk, D]')
+    B, Q, H, D = query.shape
+    N, Hk = key.shape[1], key.shape[2]
+    if key.shape[0] != B:
+        raise RuntimeError('batch size mismatch')
+    if key.shape[3] != D or value.shape != key.shape:
+        raise RuntimeError('key and value must be [B, N, Hk, D] with the head width of query')
+    if H <= 0 or Hk <= 0:
+        raise RuntimeError('need at least one head')
+    if H % Hk != 0:
+        raise RuntimeError('query heads must be a multiple of the key heads')
+    if not 1 <= D <= MAX_HEAD_DIM:
+        raise RuntimeError(f'head width must be between 1 and {MAX_HEAD_DIM}')
+    dt, dev = query.dtype, query.device
+    if dt not in DTYPE_CODE:
+        raise RuntimeError(f'unsupported dtype {dt}')
+    for t in (key, value):
+        if t.device != dev or t.dtype != dt:
+            raise RuntimeError('query, key and value must have the same device and dtype')
+    if key_padding_mask is not None:
+        if key_padding_mask.dtype not in (torch.bool, torch.uint8) or key_padding_mask.shape != (B, N):
+            raise RuntimeError('key_padding_mask must be a bool (or uint8) tensor [B, N]')
+        if key_padding_mask.device != dev:
+            raise RuntimeError('key_padding_mask must be on the device of query')
+    if attn_mask is not None:
+        if attn_mask.dtype not in (torch.bool, torch.uint8):
+            raise RuntimeError('attn_mask must be a bool (or uint8) tensor, nonzero = blocked')
+        shape = attn_mask.shape
+        if len(shape) not in (2, 4) or shape[-2:] != (Q, N) or \
+                (len(shape) == 4 and (shape[0] not in (1, B) or shape[1] not in (1, H))):
+            raise RuntimeError('attn_mask must be [Q, N] or [B or 1, H or 1, Q, N]')
+        if attn_mask.device != dev:
+            raise RuntimeError('attn_mask must be on the device of query')
+    if not (0 < scale < float('inf')):
+        raise RuntimeError('scale must be positive and finite')
+    return B, Q, N, H, Hk, D
+
+
+def _attention_operand(t):
+    """A [B, T, H, D] tensor the kernels can read in place (innermost stride 1, the other strides positive) or its
+    dense copy, and its three element strides."""
+    s = t.stride()
+    if t.numel() and (s[3] != 1 and t.shape[3] > 1 or min(s[:3]) <= 0):
+        t = t.contiguous()
+        s = t.stride()
+    return t, s[:3]
+
+
+_no_strides = (_i64 * 3)()
+
+
+def _attention_mask(attn_mask):
+    """The mask as bytes with unit key stride, its (batch, head, query) strides and its batch and head counts."""
+    if attn_mask is None:
+        return None, _no_strides, 0, 0
+    m = attn_mask if attn_mask.stride(-1) == 1 or attn_mask.shape[-1] == 1 else attn_mask.contiguous()
+    if m.dim() == 2:
+        return m, (_i64 * 3)(0, 0, m.stride(0)), 1, 1
+    nb, nh = m.shape[:2]
+    return m, (_i64 * 3)(m.stride(0) if nb > 1 else 0, m.stride(1) if nh > 1 else 0, m.stride(2)), nb, nh
+
+
+def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale, want_lse=False):
+    """(out [B, Q, H * D], lse or None) through td_attention_forward, for arguments check_attention has passed."""
+    lib = load()
+    if not query.is_cuda:
+        raise RuntimeError('inputs must be CUDA tensors')
+    B, Q, H, D = query.shape
+    N, Hk = key.shape[1], key.shape[2]
+    q, qs = _attention_operand(query)
+    k, ks = _attention_operand(key)
+    v, vs = _attention_operand(value)
+    m, ms, mb, mh = _attention_mask(attn_mask)
+    pad = None if key_padding_mask is None else key_padding_mask.contiguous()
+    dev = query.device
+    out = torch.empty((B, Q, H * D), dtype=query.dtype, device=dev)
+    lse = None
+    if want_lse:
+        acc = torch.float64 if query.dtype == torch.float64 else torch.float32
+        lse = torch.empty((B, H, -(-Q // ATTN_ROW_PAD) * ATTN_ROW_PAD), dtype=acc, device=dev)
+    if B * Q == 0:
+        return out, lse
+    code = DTYPE_CODE[query.dtype]
+    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, int(pad is not None), 0)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with torch.cuda.device(dev):
+        _call(lib.td_attention_forward, code, _ptr(q), _ptr(k), _ptr(v), (_i64 * 9)(*qs, *ks, *vs), _ptr(m), ms,
+              _ptr(pad), _ptr(out), _ptr(lse), B, Q, N, H, Hk, D, scale, int(causal), _ptr(ws), ws_bytes,
+              _stream(dev))
+    return out, lse
+
+
+def attention_backward(query, key, value, key_padding_mask, attn_mask, causal, scale, out, lse, grad_out):
+    """(grad_query, grad_key, grad_value) through td_attention_backward."""
+    lib = load()
+    B, Q, H, D = query.shape
+    N, Hk = key.shape[1], key.shape[2]
+    q, qs = _attention_operand(query)
+    k, ks = _attention_operand(key)
+    v, vs = _attention_operand(value)
+    m, ms, mb, mh = _attention_mask(attn_mask)
+    pad = None if key_padding_mask is None else key_padding_mask.contiguous()
+    g = grad_out.contiguous()
+    dev = query.device
+    grad_q = torch.empty((B, Q, H, D), dtype=q.dtype, device=dev)
+    grad_k = torch.empty((B, N, Hk, D), dtype=q.dtype, device=dev)
+    grad_v = torch.empty((B, N, Hk, D), dtype=q.dtype, device=dev)
+    code = DTYPE_CODE[q.dtype]
+    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, int(pad is not None), 1)
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+    with torch.cuda.device(dev):
+        _call(lib.td_attention_backward, code, _ptr(q), _ptr(k), _ptr(v), (_i64 * 9)(*qs, *ks, *vs), _ptr(m), ms,
+              _ptr(pad), _ptr(out), _ptr(lse), _ptr(g), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v), B, Q, N, H, Hk, D,
+              scale, int(causal), _ptr(ws), ws_bytes, _stream(dev))
+    return grad_q, grad_k, grad_v
+
+
+def check_layer_norm(x, weight, bias, residual, eps):
+    """The layer norm's argument contract, on any device."""
+    if x.dim() < 1:
+        raise RuntimeError('x must have at least one dimension')
+    C = x.shape[-1]
+    if not 1 <= C <= MAX_CHANNELS:
+        raise RuntimeError(f'channels must be between 1 and {MAX_CHANNELS}')
+    if x.dtype not in DTYPE_CODE:
+        raise RuntimeError(f'unsupported dtype {x.dtype}')
+    if weight.shape != (C,) or (bias is not None and bias.shape != (C,)):
+        raise RuntimeError('norm weight and bias must be [C] with C = the last dimension of the input')
+    if residual is not None and residual.shape != x.shape:
+        raise RuntimeError('residual must have the shape of the input')
+    for t in (weight, bias, residual):
+        if t is not None and (t.device != x.device or t.dtype != x.dtype):
+            raise RuntimeError('norm weight, bias and residual must have the device and dtype of the input')
+    if not (0 <= eps < float('inf')):
+        raise RuntimeError('eps must not be negative')
+
+
+def layer_norm_forward(x, weight, bias, residual, eps, want_stats=False):
+    """(y, mean, rstd) through td_layer_norm_forward (mean and rstd None unless want_stats), for arguments
+    check_layer_norm has passed."""
+    lib = load()
+    if not x.is_cuda:
+        raise RuntimeError('inputs must be CUDA tensors')
+    xs, w, b, r = _dense(x, weight, bias, residual)
+    C = x.shape[-1]
+    rows = xs.numel() // C
+    y = torch.empty_like(xs)
+    mean = rstd = None
+    if want_stats:
+        acc = torch.float64 if x.dtype == torch.float64 else torch.float32
+        mean, rstd = torch.empty((2, rows), dtype=acc, device=x.device)
+    if rows:
+        with torch.cuda.device(x.device):
+            _call(lib.td_layer_norm_forward, DTYPE_CODE[x.dtype], _ptr(xs), _ptr(r), _ptr(w), _ptr(b), _ptr(y),
+                  _ptr(mean), _ptr(rstd), rows, C, eps, _stream(x.device))
+    return y, mean, rstd
+
+
+def layer_norm_backward(grad_y, x, weight, residual, mean, rstd, want_weight=True, want_bias=True):
+    """(grad_x, grad_weight or None, grad_bias or None) through td_layer_norm_backward."""
+    lib = load()
+    g, xs, w, r = _dense(grad_y, x, weight, residual)
+    C = x.shape[-1]
+    rows = xs.numel() // C
+    code = DTYPE_CODE[x.dtype]
+    grad_x = torch.empty_like(xs)
+    grad_w = torch.empty((C,), dtype=x.dtype, device=x.device) if want_weight else None
+    grad_b = torch.empty((C,), dtype=x.dtype, device=x.device) if want_bias else None
+    with torch.cuda.device(x.device):
+        ws_bytes = lib.td_layer_norm_workspace_bytes(code, rows, C)
+        ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=x.device)
+        _call(lib.td_layer_norm_backward, code, _ptr(g), _ptr(xs), _ptr(r), _ptr(w), _ptr(mean), _ptr(rstd),
+              _ptr(grad_x), _ptr(grad_w), _ptr(grad_b), rows, C, _ptr(ws), ws_bytes, _stream(x.device))
+    return grad_x, grad_w, grad_b

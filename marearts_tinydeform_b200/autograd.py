@@ -21,10 +21,12 @@ LinearFunction is output_proj (y = x @ W^T + b) on the same kernels: td_linear f
 td_linear_grad_weight (with the bias gradient's column sums) backward. It is also the query projection of the
 sampling producer, whose own step (softmax over each row's L * P logits, offsets moving the reference points) is
 ProducerFunction: td_sampling_producer forward, td_sampling_producer_backward backward (gradients of the query
-projection's output and of the reference points).
+projection's output and of the reference points). AttentionFunction and LayerNormFunction are the rest of a decoder
+layer: the self attention among the queries, and the norm behind each attention.
 """
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -144,3 +146,47 @@ def producer_train(query, reference_points, spatial_shapes, heads, points, sampl
     """The differentiable sampling producer on CUDA: the query projection (LinearFunction), then ProducerFunction."""
     proj = LinearFunction.apply(query, sampling_weight, sampling_bias)
     return ProducerFunction.apply(proj, reference_points, spatial_shapes, heads, points)
+
+
+class AttentionFunction(torch.autograd.Function):
+    """Softmax attention on CUDA, differentiable in query, key and value: td_attention_forward, which also writes each
+    row's log-sum, and td_attention_backward, which forms the probabilities again from it."""
+
+    @staticmethod
+    def forward(ctx, query, key, value, key_padding_mask, attn_mask, causal, scale):
+        out, lse = _native.attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale,
+                                             want_lse=True)
+        ctx.save_for_backward(query, key, value, key_padding_mask, attn_mask, out, lse)
+        ctx.causal, ctx.scale = causal, scale
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out):
+        query, key, value, key_padding_mask, attn_mask, out, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = grad_out if grad_out.dtype == query.dtype else grad_out.to(query.dtype)
+        grads = _native.attention_backward(query, key, value, key_padding_mask, attn_mask, ctx.causal, ctx.scale, out,
+                                           lse, g)
+        return tuple(x if n else None for x, n in zip(grads, need)) + (None, None, None, None)
+
+
+class LayerNormFunction(torch.autograd.Function):
+    """Layer norm with the residual added inside on CUDA, differentiable in x, weight, bias and residual:
+    td_layer_norm_forward, which also writes each row's mean and reciprocal deviation, and td_layer_norm_backward. x
+    and residual have the same gradient; where both need it they get the same tensor."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, eps):
+        y, mean, rstd = _native.layer_norm_forward(x, weight, bias, residual, eps, want_stats=True)
+        ctx.save_for_backward(x, weight, residual, mean, rstd)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_y):
+        x, weight, residual, mean, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        g = grad_y if grad_y.dtype == x.dtype else grad_y.to(x.dtype)
+        grad_x, grad_w, grad_b = _native.layer_norm_backward(g, x, weight, residual, mean, rstd, need[1], need[2])
+        return (grad_x if need[0] else None, grad_w, grad_b, grad_x if need[3] else None, None)

@@ -6,9 +6,11 @@ ctypes (``_native.py``). It is rebuilt when any source under csrc/ or the public
     python -m marearts_tinydeform_b200.build [--force]
 """
 
+import concurrent.futures
 import os
 import subprocess
 import sys
+import tempfile
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
@@ -28,7 +30,7 @@ def _nvcc():
 
 
 def sources():
-    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(('.cu', '.cuh')))
+    return sorted(os.path.join(CSRC, f) for f in os.listdir(CSRC) if f.endswith(('.cu', '.cuh', '.h')))
 
 
 def stale(lib=LIB):
@@ -38,22 +40,30 @@ def stale(lib=LIB):
     return any(os.path.getmtime(p) > built for p in sources() + [HEADER, __file__])
 
 
+def _run(cmd):
+    print(' '.join(cmd), file=sys.stderr)
+    subprocess.run(cmd, check=True)
+
+
 def build(force=False, verbose=False, debug=False):
-    """Compile csrc/tinydeform.cu into _tinydeform.so (debug: the checked _tinydeform_debug.so, -DTD_DEBUG_BOUNDS) if
-    it is missing or stale; return the library path."""
+    """Compile every csrc/*.cu, each a translation unit of its own, side by side, and link them into _tinydeform.so
+    (debug: the checked _tinydeform_debug.so, -DTD_DEBUG_BOUNDS) if it is missing or stale; return the library path."""
     lib = DEBUG_LIB if debug else LIB
     if not force and not stale(lib):
         return lib
-    tmp = lib + '.tmp'
-    cmd = [_nvcc(), *ARCH, '-O3', '-lineinfo', '-std=c++17', '--expt-relaxed-constexpr',
-           '-Xcompiler', '-fPIC,-O3,-fvisibility=hidden', '-shared',
-           '-I' + os.path.join(ROOT, 'include'), os.path.join(CSRC, 'tinydeform.cu'), '-o', tmp]
+    flags = [*ARCH, '-O3', '-lineinfo', '-std=c++17', '--expt-relaxed-constexpr',
+             '-Xcompiler', '-fPIC,-O3,-fvisibility=hidden', '-I' + os.path.join(ROOT, 'include')]
     if debug:
-        cmd.insert(1, '-DTD_DEBUG_BOUNDS')
+        flags.insert(0, '-DTD_DEBUG_BOUNDS')
     if verbose:
-        cmd.insert(1, '-Xptxas=-v')
-    print(' '.join(cmd), file=sys.stderr)
-    subprocess.run(cmd, check=True)
+        flags.insert(0, '-Xptxas=-v')
+    with tempfile.TemporaryDirectory() as objects:
+        units = [p for p in sources() if p.endswith('.cu')]
+        outs = [os.path.join(objects, os.path.basename(p)[:-3] + '.o') for p in units]
+        with concurrent.futures.ThreadPoolExecutor(len(units)) as pool:
+            list(pool.map(_run, [[_nvcc(), *flags, '-c', p, '-o', o] for p, o in zip(units, outs)]))
+        tmp = lib + '.tmp'
+        _run([_nvcc(), *ARCH, '-shared', *outs, '-o', tmp])
     os.replace(tmp, lib)
     return lib
 

@@ -1,0 +1,418 @@
+// td_attention.cuh -- softmax attention with its backward pass: arguments shared by its kernels, and the CUDA-core
+// kernels, which take every type and head width up to 128.
+//
+//   S_ij = scale * q_i . k_j, over the keys j that query i may use;  L_i = log sum_j exp(S_ij)
+//   P_ij = exp(S_ij - L_i);  o_i = sum_j P_ij v_j
+//   backward, from do_i:  delta_i = do_i . o_i;  dP_ij = do_i . v_j;  dS_ij = P_ij (dP_ij - delta_i)
+//     dq_i = scale * sum_j dS_ij k_j;  dk_j = scale * sum_i dS_ij q_i;  dv_j = sum_i P_ij do_i
+//
+// The backward keeps no probabilities: it forms P again from S and L. A query that may use no key has o = 0, and its
+// L is stored as +infinity, which makes every P of its row exp(-infinity) = 0 in the backward, and so its gradients
+// zero. With fewer key heads than query heads, query head h reads key head h / (H / Hk), and dk, dv are summed over
+// the query heads of their group inside the kernel.
+//
+// Logarithms are base 2 in the kernels: c = scale * log2(e), lse = L * log2(e).
+//
+// CUDA-core kernels: 256 threads, a 16 x 16 grid of R x R register tiles. The tile of S (16 R x 16 R) is formed from
+// rows in shared memory, the online softmax's maximum and sum run in registers (16 lanes hold a row), and P goes
+// through shared memory for the product with the second operand, whose accumulator (16 R rows x DP columns) stays in
+// registers. Bound by the FMA units: an R x R tile needs 2 R vector loads for 4 R^2 FMAs (R = 4).
+#pragma once
+
+#include <type_traits>
+
+#include "td_common.cuh"
+#include "td_ptx.cuh"
+
+namespace td {
+
+constexpr int kAttnMaxHeadDim = 128;
+constexpr int kAttnRowPad = 128;  // lse and delta rows hold Q rounded up to this
+
+// Strides are in elements; the innermost stride of every tensor is 1.
+struct AttnArgs {
+    const void *q, *k, *v;
+    const void *out_in, *grad_out;  // backward: the forward's result and its gradient, [B, Q, H * D]
+    void* out;                      // forward: [B, Q, H * D]
+    void *grad_q, *grad_k, *grad_v; // backward: [B, Q, H, D], [B, N, Hk, D] twice
+    void* lse;                      // [B, H, Qp] in the accumulator type; forward: written unless null
+    void* delta;                    // backward workspace, [B, H, Qp]
+    long long q_b, q_t, q_h, k_b, k_t, k_h, v_b, v_t, v_h;
+    const uint8_t* mask;            // nonzero = blocked, at b * m_b + h * m_h + i * m_q + j; or null
+    long long m_b, m_h, m_q;
+    const uint8_t* padding;         // [B, N], nonzero = no key there; or null
+    int B, Q, N, H, Hk, D, Qp;
+    int causal;                     // key j is open to query i while j <= i + (N - Q)
+    double scale;
+};
+
+// Whether query i of head h may use key j (both inside their ranges).
+__device__ __forceinline__ bool attn_open(const AttnArgs& a, const uint8_t* mask_row, const uint8_t* pad, int i,
+                                          int j) {
+    if (a.causal && j > i + (a.N - a.Q)) return false;
+    if (pad != nullptr && pad[j] != 0) return false;
+    return mask_row == nullptr || mask_row[j] == 0;
+}
+
+template <typename A> __device__ __forceinline__ A attn_exp2(A x);
+template <> __device__ __forceinline__ float attn_exp2<float>(float x) { return exp2f(x); }
+template <> __device__ __forceinline__ double attn_exp2<double>(double x) { return exp2(x); }
+template <typename A> __device__ __forceinline__ A attn_log2(A x);
+template <> __device__ __forceinline__ float attn_log2<float>(float x) { return log2f(x); }
+template <> __device__ __forceinline__ double attn_log2<double>(double x) { return log2(x); }
+
+// ---- CUDA-core kernels --------------------------------------------------------------------------------------------
+
+template <typename A, int DP, int R>
+struct SimtTile {
+    static constexpr int kVN = 16 / int(sizeof(A));  // accumulators of a 16-byte load
+    static constexpr int kRows = 16 * R;
+    static constexpr int kLd = DP + kVN;              // row pitch of an operand tile
+    static constexpr int kLdP = kRows + kVN;          // row pitch of the P tile
+    static constexpr int kCols = DP / 16;             // accumulator columns a thread
+    static constexpr size_t kOperand = size_t(kRows) * kLd * sizeof(A);
+    static constexpr size_t kP = size_t(kRows) * kLdP * sizeof(A);
+};
+
+// Rows t0 .. t0 + kRows of a [tokens, D] slice into shared memory, widened; rows at or past n, padded rows and
+// columns past D are zero.
+template <typename T, typename A, int DP, int R>
+__device__ __forceinline__ void simt_load(A* dst, const T* src, long long stride, int t0, int n, int D,
+                                          const uint8_t* pad) {
+    using Tile = SimtTile<A, DP, R>;
+    for (int i = threadIdx.x; i < Tile::kRows * DP; i += 256) {
+        const int r = i / DP, c = i % DP;
+        A x = 0;
+        if (t0 + r < n && c < D && (pad == nullptr || pad[t0 + r] == 0)) x = to_acc(src[(t0 + r) * stride + c]);
+        dst[r * Tile::kLd + c] = x;
+    }
+}
+
+// s[r][c] = row (ty + 16 r) of x . row (tx + 16 c) of y
+template <typename A, int DP, int R>
+__device__ __forceinline__ void simt_dot(const A* x, const A* y, int ty, int tx, A (&s)[R][R]) {
+    using Tile = SimtTile<A, DP, R>;
+    constexpr int V = Tile::kVN;
+    struct alignas(16) Vec { A e[V]; };
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int c = 0; c < R; ++c) s[r][c] = 0;
+#pragma unroll 2
+    for (int k = 0; k < DP; k += V) {
+        Vec xv[R], yv[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            xv[r] = *reinterpret_cast<const Vec*>(x + (ty + 16 * r) * Tile::kLd + k);
+            yv[r] = *reinterpret_cast<const Vec*>(y + (tx + 16 * r) * Tile::kLd + k);
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int c = 0; c < R; ++c)
+#pragma unroll
+                for (int e = 0; e < V; ++e) s[r][c] += xv[r].e[e] * yv[c].e[e];
+    }
+}
+
+// o[r][c] += sum_j p[ty + 16 r][j] * y[j][tx + 16 c]
+template <typename A, int DP, int R>
+__device__ __forceinline__ void simt_accumulate(const A* p, const A* y, int ty, int tx,
+                                                A (&o)[R][SimtTile<A, DP, R>::kCols]) {
+    using Tile = SimtTile<A, DP, R>;
+    constexpr int V = Tile::kVN;
+    struct alignas(16) Vec { A e[V]; };
+#pragma unroll 2
+    for (int j = 0; j < Tile::kRows; j += V) {
+        Vec pv[R];
+#pragma unroll
+        for (int r = 0; r < R; ++r) pv[r] = *reinterpret_cast<const Vec*>(p + (ty + 16 * r) * Tile::kLdP + j);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+#pragma unroll
+            for (int c = 0; c < Tile::kCols; ++c) {
+                const A b = y[(j + e) * Tile::kLd + tx + 16 * c];
+#pragma unroll
+                for (int r = 0; r < R; ++r) o[r][c] += pv[r].e[e] * b;
+            }
+    }
+}
+
+// Sum or maximum over the 16 lanes that hold a row.
+template <typename A> __device__ __forceinline__ A row_sum(A v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+template <typename A> __device__ __forceinline__ A row_max(A v) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v = cmax(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+
+// The end of the keys that rows i < row_end may use: everything, or the causal edge of the last row.
+__device__ __forceinline__ int attn_key_end(const AttnArgs& a, int row_end) {
+    if (!a.causal) return a.N;
+    const int last = min(row_end, a.Q) + (a.N - a.Q);
+    return max(0, min(a.N, last));
+}
+
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(256) attn_simt_forward_kernel(const AttnArgs a) {
+    using A = typename Elem<T>::acc;
+    using Tile = SimtTile<A, DP, R>;
+    constexpr int M = Tile::kRows;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    A* qs = reinterpret_cast<A*>(smem_raw);
+    A* ks = qs + M * Tile::kLd;
+    A* vs = ks + M * Tile::kLd;
+    A* ps = vs + M * Tile::kLd;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int tiles = (a.Q + M - 1) / M;
+    const int i0 = blockIdx.x % tiles * M, bh = blockIdx.x / tiles, h = bh % a.H, b = bh / a.H;
+    const int hk = h / (a.H / a.Hk);
+    const A ninf = -A(INFINITY), c = A(a.scale * 1.4426950408889634);
+    const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
+    grid_dependency_wait();
+    launch_dependents();
+    simt_load<T, A, DP, R>(qs, static_cast<const T*>(a.q) + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+    A m[R], l[R], o[R][Tile::kCols];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        m[r] = ninf;
+        l[r] = 0;
+#pragma unroll
+        for (int x = 0; x < Tile::kCols; ++x) o[r][x] = 0;
+    }
+    const int key_end = attn_key_end(a, i0 + M);
+    for (int j0 = 0; j0 < key_end; j0 += M) {
+        __syncthreads();  // the tiles of the turn before have been read
+        simt_load<T, A, DP, R>(ks, static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, R>(vs, static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        __syncthreads();
+        A s[R][R];
+        simt_dot<A, DP, R>(qs, ks, ty, tx, s);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = i0 + ty + 16 * r;
+            A top = m[r];
+#pragma unroll
+            for (int x = 0; x < R; ++x) {
+                const int j = j0 + tx + 16 * x;
+                const bool open = i < a.Q && j < a.N &&
+                                  attn_open(a, mask == nullptr ? nullptr : mask + i * a.m_q, pad, i, j);
+                s[r][x] = open ? s[r][x] * c : ninf;
+                top = cmax(top, s[r][x]);
+            }
+            top = row_max(top);
+            const A ref = top == ninf ? A(0) : top;  // no key so far: exp2(-inf - 0) = 0
+            const A keep = attn_exp2<A>(m[r] - ref);
+            A sum = 0;
+#pragma unroll
+            for (int x = 0; x < R; ++x) {
+                s[r][x] = attn_exp2<A>(s[r][x] - ref);
+                sum += s[r][x];
+                ps[(ty + 16 * r) * Tile::kLdP + tx + 16 * x] = s[r][x];
+            }
+            l[r] = l[r] * keep + row_sum(sum);
+            m[r] = top;
+#pragma unroll
+            for (int x = 0; x < Tile::kCols; ++x) o[r][x] *= keep;
+        }
+        __syncwarp();  // a row's P is written and read by the same half warp
+        simt_accumulate<A, DP, R>(ps, vs, ty, tx, o);
+    }
+    T* out = static_cast<T*>(a.out);
+    A* lse = static_cast<A*>(a.lse);
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + ty + 16 * r;
+        const A inv = l[r] == A(0) ? A(0) : A(1) / l[r];
+        if (lse != nullptr && tx == 0 && i < a.Qp)
+            lse[(long long)bh * a.Qp + i] = i < a.Q && l[r] != A(0) ? m[r] + attn_log2<A>(l[r]) : A(INFINITY);
+        if (i >= a.Q) continue;
+#pragma unroll
+        for (int x = 0; x < Tile::kCols; ++x) {
+            const int d = tx + 16 * x;
+            if (d < a.D) out[(((long long)b * a.Q + i) * a.H + h) * a.D + d] = from_acc<T>(o[r][x] * inv);
+        }
+    }
+    // rows of lse that no tile covers
+    if (lse != nullptr && i0 + M >= a.Q)
+        for (int i = i0 + M + int(threadIdx.x); i < a.Qp; i += 256) lse[(long long)bh * a.Qp + i] = A(INFINITY);
+}
+
+// delta[b, h, i] = grad_out . out over a query's head; zero in the rows behind the last query. A warp per row.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
+    using A = typename Elem<T>::acc;
+    const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;  // (b * H + h) * Qp + i
+    const int lane = threadIdx.x % 32;
+    grid_dependency_wait();
+    launch_dependents();
+    if (row >= (long long)a.B * a.H * a.Qp) return;
+    const int i = int(row % a.Qp);
+    const long long bh = row / a.Qp;
+    A sum = 0;
+    if (i < a.Q) {
+        const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D;
+        const T* o = static_cast<const T*>(a.out_in) + at;
+        const T* g = static_cast<const T*>(a.grad_out) + at;
+        for (int d = lane; d < a.D; d += 32) sum += to_acc(o[d]) * to_acc(g[d]);
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    }
+    if (lane == 0) static_cast<A*>(a.delta)[row] = sum;
+}
+
+// The gradient of the keys and values (blocks below kv_blocks: one tile of keys of one key head, over the query heads
+// of its group and their query tiles) and of the queries (the other blocks: one tile of queries of one head).
+template <typename T, int DP, int R>
+__global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs a, int kv_blocks) {
+    using A = typename Elem<T>::acc;
+    using Tile = SimtTile<A, DP, R>;
+    constexpr int M = Tile::kRows;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    A* qs = reinterpret_cast<A*>(smem_raw);
+    A* gs = qs + M * Tile::kLd;
+    A* ks = gs + M * Tile::kLd;
+    A* vs = ks + M * Tile::kLd;
+    A* ps = vs + M * Tile::kLd;
+    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+    const int group = a.H / a.Hk;
+    const A c = A(a.scale * 1.4426950408889634), scale = A(a.scale);
+    const T* q = static_cast<const T*>(a.q);
+    const T* k = static_cast<const T*>(a.k);
+    const T* v = static_cast<const T*>(a.v);
+    const T* g = static_cast<const T*>(a.grad_out);
+    const A* lse = static_cast<const A*>(a.lse);
+    const A* delta = static_cast<const A*>(a.delta);
+    grid_dependency_wait();
+    launch_dependents();
+    if (int(blockIdx.x) < kv_blocks) {
+        const int tiles = (a.N + M - 1) / M;
+        const int j0 = blockIdx.x % tiles * M, hk = blockIdx.x / tiles % a.Hk, b = blockIdx.x / tiles / a.Hk;
+        const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
+        simt_load<T, A, DP, R>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, R>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        A dk[R][Tile::kCols], dv[R][Tile::kCols];
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int x = 0; x < Tile::kCols; ++x) dk[r][x] = dv[r][x] = 0;
+        // the first query that may use key j0
+        const int first = a.causal ? max(0, min(a.Q, j0 - (a.N - a.Q))) / M * M : 0;
+        for (int h = hk * group; h < (hk + 1) * group; ++h) {
+            const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
+            const A* lse_h = lse + ((long long)b * a.H + h) * a.Qp;
+            const A* delta_h = delta + ((long long)b * a.H + h) * a.Qp;
+            for (int i0 = first; i0 < a.Q; i0 += M) {
+                __syncthreads();
+                simt_load<T, A, DP, R>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+                simt_load<T, A, DP, R>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q,
+                                       a.D, nullptr);
+                __syncthreads();
+                A s[R][R], p[R][R];
+                simt_dot<A, DP, R>(ks, qs, ty, tx, s);
+#pragma unroll
+                for (int x = 0; x < R; ++x) {
+                    const int i = i0 + tx + 16 * x;
+                    const A li = i < a.Q ? lse_h[i] : A(INFINITY);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const int j = j0 + ty + 16 * r;
+                        const bool open = i < a.Q && j < a.N &&
+                                          attn_open(a, mask == nullptr ? nullptr : mask + i * a.m_q, pad, i, j);
+                        p[r][x] = open ? attn_exp2<A>(s[r][x] * c - li) : A(0);
+                        ps[(ty + 16 * r) * Tile::kLdP + tx + 16 * x] = p[r][x];
+                    }
+                }
+                __syncwarp();
+                simt_accumulate<A, DP, R>(ps, gs, ty, tx, dv);
+                simt_dot<A, DP, R>(vs, gs, ty, tx, s);
+                __syncwarp();
+#pragma unroll
+                for (int x = 0; x < R; ++x) {
+                    const int i = i0 + tx + 16 * x;
+                    const A di = i < a.Q ? delta_h[i] : A(0);
+#pragma unroll
+                    for (int r = 0; r < R; ++r)
+                        ps[(ty + 16 * r) * Tile::kLdP + tx + 16 * x] =
+                            p[r][x] == A(0) ? A(0) : p[r][x] * (s[r][x] - di);
+                }
+                __syncwarp();
+                simt_accumulate<A, DP, R>(ps, qs, ty, tx, dk);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int j = j0 + ty + 16 * r;
+            if (j >= a.N) continue;
+#pragma unroll
+            for (int x = 0; x < Tile::kCols; ++x) {
+                const int d = tx + 16 * x;
+                if (d >= a.D) continue;
+                const long long at = (((long long)b * a.N + j) * a.Hk + hk) * a.D + d;
+                static_cast<T*>(a.grad_k)[at] = from_acc<T>(dk[r][x] * scale);
+                static_cast<T*>(a.grad_v)[at] = from_acc<T>(dv[r][x]);
+            }
+        }
+        return;
+    }
+    const int blk = int(blockIdx.x) - kv_blocks;
+    const int tiles = (a.Q + M - 1) / M;
+    const int i0 = blk % tiles * M, h = blk / tiles % a.H, b = blk / tiles / a.H, hk = h / group;
+    const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
+    simt_load<T, A, DP, R>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+    simt_load<T, A, DP, R>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr);
+    A dq[R][Tile::kCols], li[R], di[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + ty + 16 * r;
+        const long long at = ((long long)b * a.H + h) * a.Qp + i;
+        li[r] = i < a.Q ? lse[at] : A(INFINITY);
+        di[r] = i < a.Q ? delta[at] : A(0);
+#pragma unroll
+        for (int x = 0; x < Tile::kCols; ++x) dq[r][x] = 0;
+    }
+    const int key_end = attn_key_end(a, i0 + M);
+    for (int j0 = 0; j0 < key_end; j0 += M) {
+        __syncthreads();
+        simt_load<T, A, DP, R>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, R>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        __syncthreads();
+        A s[R][R], dp[R][R];
+        simt_dot<A, DP, R>(qs, ks, ty, tx, s);
+        simt_dot<A, DP, R>(gs, vs, ty, tx, dp);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const int i = i0 + ty + 16 * r;
+#pragma unroll
+            for (int x = 0; x < R; ++x) {
+                const int j = j0 + tx + 16 * x;
+                const bool open = i < a.Q && j < a.N &&
+                                  attn_open(a, mask == nullptr ? nullptr : mask + i * a.m_q, pad, i, j);
+                ps[(ty + 16 * r) * Tile::kLdP + tx + 16 * x] =
+                    open ? attn_exp2<A>(s[r][x] * c - li[r]) * (dp[r][x] - di[r]) : A(0);
+            }
+        }
+        __syncwarp();
+        simt_accumulate<A, DP, R>(ps, ks, ty, tx, dq);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+        const int i = i0 + ty + 16 * r;
+        if (i >= a.Q) continue;
+#pragma unroll
+        for (int x = 0; x < Tile::kCols; ++x) {
+            const int d = tx + 16 * x;
+            if (d < a.D)
+                static_cast<T*>(a.grad_q)[(((long long)b * a.Q + i) * a.H + h) * a.D + d] =
+                    from_acc<T>(dq[r][x] * scale);
+        }
+    }
+}
+
+}  // namespace td

@@ -1,0 +1,288 @@
+// td_norm.cuh -- layer norm with the residual added inside, forward and backward.
+//
+//   s = x + residual;  mean = sum(s) / C;  rstd = 1 / sqrt(sum((s - mean)^2) / C + eps)
+//   y = (s - mean) * rstd * weight + bias
+//   backward, with z = (s - mean) * rstd and g = dy * weight:
+//     ds = rstd * (g - sum(g) / C - z * sum(g * z) / C)      (the gradient of x and of residual alike)
+//     dweight = sum over rows of dy * z,  dbias = sum over rows of dy
+//
+// Bound by memory: a row is read once, into registers, and every sum over it is taken there -- the variance from the
+// centred values, so rows far from zero lose nothing. s is not rounded to the input type: both passes form it from
+// x and residual in float32 (float64 for float64), as they do all sums.
+//
+// A group of G threads holds a row, EPT elements a thread (VEC = elements of a 16-byte vector, or 1 where C or an
+// address is not a multiple of it), and walks over rows blockIdx, blockIdx + gridDim, .., the next row's loads issued
+// before the present row's sums are taken. The backward's column sums stay in the group's registers over all of its
+// rows; the groups of a CTA add theirs in order through shared memory, each CTA stores one float32 partial row, and
+// norm_reduce_kernel adds those in a fixed order: no atomics, the same bits every time.
+#pragma once
+
+#include "td_common.cuh"
+#include "td_ptx.cuh"
+
+namespace td {
+
+constexpr int kNormThreads = 256;
+
+template <typename T>
+struct NormArgs {
+    using acc = typename Elem<T>::acc;
+    const T* x;
+    const T* residual;  // or null
+    const T* weight;
+    const T* bias;      // forward; or null
+    const T* grad_y;    // backward
+    T* out;             // forward: y; backward: the gradient of x
+    acc* mean;          // [rows], forward: written unless null; backward: read
+    acc* rstd;
+    acc* partial;       // backward: [gridDim][2][C] partial column sums
+    long long rows;
+    int C;
+    acc eps;
+};
+
+// A thread's EPT elements of a row as raw vectors: VEC-element vectors at group stride G.
+template <typename T, int VEC, int NV>
+struct RowRegs {
+    static constexpr bool kWide = VEC > 1;
+    uint4 wide[kWide ? NV : 1];
+    T one[kWide ? 1 : NV];
+
+    template <int G>
+    __device__ __forceinline__ void load(const T* __restrict__ p, int lane, int C) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (lane + i * G) * VEC;
+            if constexpr (kWide) {
+                wide[i] = c < C ? __ldg(reinterpret_cast<const uint4*>(p + c)) : make_uint4(0, 0, 0, 0);
+            } else {
+                one[i] = c < C ? p[c] : from_acc<T>(typename Elem<T>::acc(0));
+            }
+        }
+    }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (kWide) wide[i] = make_uint4(0, 0, 0, 0);
+            else one[i] = from_acc<T>(typename Elem<T>::acc(0));
+        }
+    }
+    __device__ __forceinline__ void widen(typename Elem<T>::acc* o) const {
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if constexpr (kWide) unpack16<T>(wide[i], o + i * VEC);
+            else o[i] = to_acc(one[i]);
+        }
+    }
+};
+
+template <typename T, int VEC, int NV, int G>
+__device__ __forceinline__ void store_row(T* __restrict__ p, const typename Elem<T>::acc* v, int lane, int C) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int c = (lane + i * G) * VEC;
+        if (c >= C) continue;
+        if constexpr (VEC > 1) store16<T>(p + c, v + i * VEC);
+        else p[c] = from_acc<T>(v[i]);
+    }
+}
+
+// Sum over the G threads of the calling group, the same bits in each (an xor butterfly, then the warps in order).
+// red: kNormThreads / 32 words a call; every thread of the CTA calls (G > 32: two CTA barriers).
+template <int G, typename A>
+__device__ __forceinline__ A group_sum(A v, A* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if constexpr (G > 32) {
+        const int warp = threadIdx.x >> 5;
+        __syncthreads();  // the words of the call before have been read
+        if ((threadIdx.x & 31) == 0) red[warp] = v;
+        __syncthreads();
+        const int first = warp / (G / 32) * (G / 32);
+        v = red[first];
+#pragma unroll
+        for (int i = 1; i < G / 32; ++i) v += red[first + i];
+    }
+    return v;
+}
+
+template <typename T, int VEC, int G, int EPT>
+__global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormArgs<T> a) {
+    using acc = typename Elem<T>::acc;
+    constexpr int NV = EPT / VEC, kGroups = kNormThreads / G;
+    __shared__ acc red[2 * kNormThreads / 32];
+    const int group = threadIdx.x / G, lane = threadIdx.x % G;
+    grid_dependency_wait();
+    launch_dependents();
+    RowRegs<T, VEC, NV> w, b, x, r;
+    w.template load<G>(a.weight, lane, a.C);
+    if (a.bias != nullptr) b.template load<G>(a.bias, lane, a.C);
+    else b.zero();
+    const acc inv = acc(1) / acc(a.C);
+    const long long step = (long long)gridDim.x * kGroups;
+    auto fetch = [&](long long row) {
+        if (row < a.rows) {
+            x.template load<G>(a.x + row * a.C, lane, a.C);
+            if (a.residual != nullptr) r.template load<G>(a.residual + row * a.C, lane, a.C);
+        } else {
+            x.zero();
+        }
+    };
+    r.zero();
+    long long row = (long long)blockIdx.x * kGroups + group;
+    fetch(row);
+    // every group takes the same number of turns, so that the CTA barriers of group_sum match
+    for (long long turn = (long long)blockIdx.x * kGroups; turn < a.rows; turn += step, row += step) {
+        acc s[EPT], t[EPT];
+        x.widen(s);
+        if (a.residual != nullptr) {
+            r.widen(t);
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) s[i] += t[i];
+        }
+        fetch(row + step);
+        acc sum = 0;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) sum += s[i];  // elements outside the row are zero
+        const acc mean = group_sum<G>(sum, red) * inv;
+        acc sq = 0;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            const int c = (lane + i / VEC * G) * VEC + i % VEC;
+            s[i] = c < a.C ? s[i] - mean : acc(0);
+            sq += s[i] * s[i];
+        }
+        const acc rstd = acc(1) / sqrt(group_sum<G>(sq, red + kNormThreads / 32) * inv + a.eps);
+        if (row < a.rows) {
+            if (a.mean != nullptr && lane == 0) {
+                a.mean[row] = mean;
+                a.rstd[row] = rstd;
+            }
+            acc u[EPT];
+            w.widen(t);
+            b.widen(u);
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) s[i] = s[i] * rstd * t[i] + u[i];
+            store_row<T, VEC, NV, G>(a.out + row * a.C, s, lane, a.C);
+        }
+    }
+}
+
+template <typename T, int VEC, int G, int EPT>
+__global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormArgs<T> a) {
+    using acc = typename Elem<T>::acc;
+    constexpr int NV = EPT / VEC, kGroups = kNormThreads / G;
+    constexpr int kCols = G * EPT;  // widest row of this form
+    __shared__ acc red[2 * kNormThreads / 32];
+    __shared__ acc cols[kGroups > 1 ? kCols : 1];
+    const int group = threadIdx.x / G, lane = threadIdx.x % G;
+    grid_dependency_wait();
+    launch_dependents();
+    RowRegs<T, VEC, NV> w, x, r, d;
+    w.template load<G>(a.weight, lane, a.C);
+    r.zero();
+    const acc inv = acc(1) / acc(a.C);
+    const long long step = (long long)gridDim.x * kGroups;
+    acc mean_n = 0, rstd_n = 0;
+    auto fetch = [&](long long row) {
+        if (row < a.rows) {
+            x.template load<G>(a.x + row * a.C, lane, a.C);
+            d.template load<G>(a.grad_y + row * a.C, lane, a.C);
+            if (a.residual != nullptr) r.template load<G>(a.residual + row * a.C, lane, a.C);
+            mean_n = a.mean[row];
+            rstd_n = a.rstd[row];
+        } else {  // adds nothing to the column sums
+            x.zero();
+            d.zero();
+            r.zero();
+            mean_n = rstd_n = 0;
+        }
+    };
+    acc dw[EPT], db[EPT];
+#pragma unroll
+    for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0;
+    long long row = (long long)blockIdx.x * kGroups + group;
+    fetch(row);
+    for (long long turn = (long long)blockIdx.x * kGroups; turn < a.rows; turn += step, row += step) {
+        acc z[EPT], g[EPT], t[EPT];
+        x.widen(z);
+        if (a.residual != nullptr) {
+            r.widen(t);
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) z[i] += t[i];
+        }
+        d.widen(g);
+        const acc mean = mean_n, rstd = rstd_n;
+        fetch(row + step);
+        w.widen(t);
+        acc sg = 0, sgz = 0;
+#pragma unroll
+        for (int i = 0; i < EPT; ++i) {
+            // outside the row g is zero (dy was loaded as zero), so z's value there counts for nothing
+            z[i] = (z[i] - mean) * rstd;
+            db[i] += g[i];
+            dw[i] += g[i] * z[i];
+            g[i] *= t[i];
+            sg += g[i];
+            sgz += g[i] * z[i];
+        }
+        sg = group_sum<G>(sg, red) * inv;
+        sgz = group_sum<G>(sgz, red + kNormThreads / 32) * inv;
+        if (row < a.rows) {
+#pragma unroll
+            for (int i = 0; i < EPT; ++i) g[i] = (g[i] - sg - z[i] * sgz) * rstd;
+            store_row<T, VEC, NV, G>(a.out + row * a.C, g, lane, a.C);
+        }
+    }
+    // the CTA's column sums: group 0's, + group 1's, .. in order
+    acc* part = a.partial + (long long)blockIdx.x * 2 * a.C;
+    auto add_up = [&](const acc(&v)[EPT], acc* out) {
+        for (int turn = 0; turn < kGroups; ++turn) {
+            if (group == turn) {
+#pragma unroll
+                for (int i = 0; i < EPT; ++i) {
+                    const int c = (lane + i / VEC * G) * VEC + i % VEC;
+                    acc sum = v[i];
+                    if constexpr (kGroups > 1) {
+                        if (turn > 0) sum += cols[c];
+                        cols[c] = sum;
+                    }
+                    if (turn == kGroups - 1 && c < a.C) out[c] = sum;
+                }
+            }
+            __syncthreads();
+        }
+    };
+    add_up(dw, part);
+    add_up(db, part + a.C);
+}
+
+// grad_weight and grad_bias from the CTAs' partial rows [parts][2][C]: each thread adds every kReduceRows-th row of
+// one column, then the threads of a column are added in order.
+constexpr int kReduceCols = 32, kReduceRows = 16;
+template <typename T>
+__global__ void __launch_bounds__(kReduceCols* kReduceRows)
+    norm_reduce_kernel(const typename Elem<T>::acc* __restrict__ partial, T* grad_weight, T* grad_bias, int parts,
+                       int C) {
+    using acc = typename Elem<T>::acc;
+    __shared__ acc sums[kReduceRows][kReduceCols];
+    const int tx = threadIdx.x % kReduceCols, ty = threadIdx.x / kReduceCols;
+    const int col = blockIdx.x * kReduceCols + tx;  // of 2 * C
+    grid_dependency_wait();
+    launch_dependents();
+    acc sum = 0;
+    if (col < 2 * C) {
+#pragma unroll 4
+        for (int p = ty; p < parts; p += kReduceRows) sum += partial[(long long)p * 2 * C + col];
+    }
+    sums[ty][tx] = sum;
+    __syncthreads();
+    if (ty == 0 && col < 2 * C) {
+#pragma unroll
+        for (int i = 1; i < kReduceRows; ++i) sum += sums[i][tx];
+        T* out = col < C ? grad_weight : grad_bias;
+        if (out != nullptr) out[col < C ? col : col - C] = from_acc<T>(sum);
+    }
+}
+
+}  // namespace td

@@ -30,6 +30,7 @@
 #include "td_sample_outproj.cuh"
 #include "td_peer_gather.cuh"
 #include "td_probe.cuh"
+#include "td_host.h"
 
 namespace td {
 namespace {
@@ -1087,6 +1088,45 @@ LayerWorkspace layer_workspace(size_t e, int order, int64_t B, int64_t Q, int64_
 
 using namespace td;
 
+namespace td {
+namespace host {
+
+int fail(char* err, size_t err_len, int code, const char* fmt, ...) {
+    if (err != nullptr && err_len > 0) {
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(err, err_len, fmt, ap);
+        va_end(ap);
+    }
+    return code;
+}
+
+int sm_count(int* out, char* err, size_t err_len) {
+    DeviceFacts f;
+    if (int rc = device_facts(&f, err, err_len)) return rc;
+    *out = f.sm_count;
+    return TD_OK;
+}
+
+bool best_policy() { return g_policy.load(std::memory_order_relaxed) == TD_POLICY_BEST; }
+void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
+
+CUresult encode_tiled_u16(CUtensorMap* map, uint32_t rank, const void* base, const uint64_t* dims,
+                          const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle) {
+    const cuuint32_t ones[5] = {1, 1, 1, 1, 1};
+    cuuint64_t d[5], st[5];
+    cuuint32_t bx[5];
+    for (uint32_t i = 0; i < rank; ++i) {
+        d[i] = dims[i];
+        bx[i] = box[i];
+        st[i] = i + 1 < rank ? strides[i] : 0;
+    }
+    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), d, st, bx, ones, swizzle);
+}
+
+}  // namespace host
+}  // namespace td
+
 extern "C" {
 
 int td_fused_forward(int dtype, const void* memory, const void* value_weight, const void* value_bias,
@@ -2011,7 +2051,10 @@ int td_device_error(int clear, unsigned int* code, char* err, size_t err_len) {
         const unsigned int zero = 0;
         e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
     }
+    unsigned int w = 0;
+    if (e == cudaSuccess) e = attention_device_error(clear, &w);
     if (e != cudaSuccess) return fail(err, err_len, TD_ERR_CUDA, "device error word: %s", cudaGetErrorString(e));
+    if (v == 0) v = w;
     if (code != nullptr) *code = v;
     return TD_OK;
 }

@@ -89,3 +89,38 @@ def deform_attn_layer_reference(query, reference_points, memory, spatial_shapes,
     out = ma_deform_attn_reference(memory, value_weight, value_bias, spatial_shapes, level_start_index, loc,
                                    attention, value_padding_mask)
     return out if output_weight is None else F.linear(out, output_weight, output_bias)
+
+
+def attention_reference(query, key, value, key_padding_mask=None, attn_mask=None, causal=False, scale=None):
+    """Softmax attention with torch operators; the definition ``attention`` follows (see there for the arguments).
+    Sums and probabilities are float32 for float16 / bfloat16 inputs, and the result is rounded once."""
+    B, Q, H, D = query.shape
+    N, Hk = key.shape[1:3]
+    acc = torch.float32 if query.dtype in (torch.float16, torch.bfloat16) else query.dtype
+    q, k, v = query.to(acc), key.to(acc), value.to(acc)
+    if key_padding_mask is not None:  # a padded key is not there at all, whatever its rows hold
+        gone = key_padding_mask.to(torch.bool)[:, :, None, None]
+        k, v = k.masked_fill(gone, 0), v.masked_fill(gone, 0)
+    if Hk != H:
+        k, v = k.repeat_interleave(H // Hk, 2), v.repeat_interleave(H // Hk, 2)
+    scores = torch.einsum('bihd,bjhd->bhij', q, k) * (D ** -0.5 if scale is None else scale)
+    blocked = torch.zeros((1, 1, Q, N), dtype=torch.bool, device=query.device)
+    if key_padding_mask is not None:
+        blocked = blocked | key_padding_mask.to(torch.bool)[:, None, None, :]
+    if attn_mask is not None:
+        blocked = blocked | attn_mask.to(torch.bool)
+    if causal:
+        blocked = blocked | torch.ones((Q, N), dtype=torch.bool, device=query.device).triu(N - Q + 1)
+    # rows without an open key: softmax over finite scores, then zeroed, so that their gradients are zeros too
+    empty = blocked.all(-1, keepdim=True)
+    scores = scores.masked_fill(blocked & ~empty, float('-inf'))
+    probs = scores.softmax(-1).masked_fill(empty | blocked, 0)
+    return torch.einsum('bhij,bjhd->bihd', probs, v).reshape(B, Q, H * D).to(query.dtype)
+
+
+def layer_norm_reference(x, weight, bias=None, residual=None, eps=1e-5):
+    """Layer norm over the last dimension with the residual added inside, with torch operators; the definition
+    ``layer_norm`` follows. float32 arithmetic for float16 / bfloat16 inputs, rounded once."""
+    acc = torch.float32 if x.dtype in (torch.float16, torch.bfloat16) else x.dtype
+    s = x.to(acc) if residual is None else x.to(acc) + residual.to(acc)
+    return F.layer_norm(s, s.shape[-1:], weight.to(acc), None if bias is None else bias.to(acc), eps).to(x.dtype)

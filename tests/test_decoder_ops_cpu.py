@@ -1,0 +1,132 @@
+"""attention and layer_norm without a GPU: the CPU path against float64, refusals, and the C ABI's argument checks."""
+
+import ctypes
+
+import pytest
+import torch
+
+from attention_oracle import attention_exact, check, layer_norm_exact
+from marearts_tinydeform_b200 import _native, attention, build, deform_attn_layer, layer_norm
+
+DTYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
+
+
+@pytest.fixture(scope='module')
+def lib():
+    build.build()
+    return _native.load()
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_attention_reference(dtype):
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(s, generator=g).to(dtype) for s in ((2, 9, 4, 16), (2, 12, 2, 16), (2, 12, 2, 16)))
+    grad = torch.randn((2, 9, 64), generator=g).to(dtype)
+    pad = torch.zeros((2, 12), dtype=torch.bool)
+    pad[1, 3:] = True
+    pairs = torch.rand((2, 1, 9, 12), generator=g) < 0.5
+    pairs[0, 0, 4] = True
+    for kw in (dict(), dict(key_padding_mask=pad), dict(attn_mask=pairs), dict(causal=True),
+               dict(key_padding_mask=pad, attn_mask=pairs, causal=True)):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+        out = attention(*leaves, **kw)
+        got = [out.detach()] + list(torch.autograd.grad(out, leaves, grad))
+        for i, (a, e) in enumerate(zip(got, attention_exact(q, k, v, grad=grad, **kw))):
+            check(a, e, f'{i} {list(kw)}')
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_layer_norm_reference(dtype):
+    g = torch.Generator().manual_seed(1)
+    x, r, dy = (torch.randn((6, 33), generator=g).to(dtype) for _ in range(3))
+    w, b = (torch.randn(33, generator=g).to(dtype) for _ in range(2))
+    leaves = [t.detach().requires_grad_() for t in (x, w, b, r)]
+    y = layer_norm(*leaves)
+    got = [y.detach()] + list(torch.autograd.grad(y, leaves, dy))
+    for a, e in zip(got, layer_norm_exact(x, w, b, r, grad=dy)):
+        check(a, e, 'layer norm')
+
+
+def test_attention_refusals():
+    q, k = torch.zeros(2, 3, 4, 8), torch.zeros(2, 5, 2, 8)
+    good = dict(query=q, key=k, value=k)
+    pad, pairs = torch.zeros(2, 5, dtype=torch.bool), torch.zeros(3, 5, dtype=torch.bool)
+    attention(**good, key_padding_mask=pad, attn_mask=pairs)
+    bad = [(dict(query=q[0]), 'query must be'), (dict(key=k[:1], value=k[:1]), 'batch size'),
+           (dict(value=k[:, :4]), 'key and value must be'), (dict(key=k[..., :4], value=k[..., :4]), 'key and value'),
+           (dict(key=torch.zeros(2, 5, 3, 8), value=torch.zeros(2, 5, 3, 8)), 'multiple of the key heads'),
+           (dict(key=k.double()), 'same device and dtype'), (dict(key_padding_mask=pad.float()), 'key_padding_mask'),
+           (dict(key_padding_mask=pad[:, :4]), 'key_padding_mask'), (dict(attn_mask=pairs.float()), 'attn_mask'),
+           (dict(attn_mask=pairs[:2]), 'attn_mask'), (dict(attn_mask=pairs.expand(3, 1, 3, 5)), 'attn_mask'),
+           (dict(scale=0.0), 'scale'), (dict(scale=float('nan')), 'scale'), (dict(scale=float('inf')), 'scale'),
+           (dict(query=torch.zeros(2, 3, 4, 129), key=torch.zeros(2, 5, 2, 129), value=torch.zeros(2, 5, 2, 129)),
+            'head width'),
+           (dict(query=q.int(), key=k.int(), value=k.int()), 'unsupported dtype'),
+           (dict(query=q.to('meta')), 'same device and dtype')]
+    for change, message in bad:
+        with pytest.raises(RuntimeError, match=message):
+            attention(**{**good, **change})
+
+
+def test_layer_norm_refusals():
+    x, w = torch.zeros(3, 8), torch.ones(8)
+    layer_norm(x, w)
+    for args, message in [((x, w[:7]), 'weight and bias'), ((x, w, w[:7]), 'weight and bias'),
+                          ((x, w, w, x[:2]), 'residual'), ((x, w.double()), 'device and dtype'),
+                          ((x, w, None, x.double()), 'device and dtype'), ((x, w, None, None, -1.0), 'eps'),
+                          ((x.int(), w), 'unsupported dtype'), ((torch.zeros(()), w), 'at least one dimension'),
+                          ((torch.zeros(2, 8193), torch.zeros(8193)), 'channels'),
+                          ((torch.zeros(2, 0), torch.zeros(0)), 'channels')]:
+        with pytest.raises(RuntimeError, match=message):
+            layer_norm(*args)
+    with pytest.raises(ValueError, match='need norm_weight'):
+        deform_attn_layer(*[None] * 11, residual=x)
+
+
+def call_attention(lib, dtype=_native.TD_F16, B=1, Q=4, N=5, H=2, Hk=1, D=32, scale=1.0, ptr=16, backward=False,
+                   ws=16, ws_bytes=1 << 20):
+    err = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p(ptr) if ptr else None
+    strides = (ctypes.c_int64 * 9)(*[1] * 9)
+    if backward:
+        rc = lib.td_attention_backward(dtype, p, p, p, strides, None, None, None, p, p, p, p, p, p, B, Q, N, H, Hk, D,
+                                       scale, 0, ctypes.c_void_p(ws), ws_bytes, None, err, 256)
+    else:
+        rc = lib.td_attention_forward(dtype, p, p, p, strides, None, None, None, p, p, B, Q, N, H, Hk, D, scale, 0,
+                                      ctypes.c_void_p(ws), ws_bytes, None, err, 256)
+    return rc, err.value.decode()
+
+
+@pytest.mark.parametrize('backward', (False, True))
+def test_attention_abi_refuses_before_any_launch(lib, backward):
+    for kw, message in [(dict(dtype=7), 'dtype'), (dict(B=-1), 'non-negative'), (dict(H=0), 'head'),
+                        (dict(H=3, Hk=2), 'multiple of the key heads'), (dict(D=0), 'head width'),
+                        (dict(D=129), 'head width'), (dict(scale=-1.0), 'scale'), (dict(scale=float('nan')), 'scale'),
+                        (dict(Q=2 ** 31), 'too many'), (dict(N=2 ** 31), 'too many'),
+                        (dict(B=2 ** 20, Q=2 ** 12), 'too many'), (dict(ptr=0), 'null tensor pointer')]:
+        rc, text = call_attention(lib, backward=backward, **kw)
+        assert rc == 1 and message in text, (kw, rc, text)
+    assert call_attention(lib, backward=backward, B=0, ptr=0) == (0, '')
+
+
+def test_attention_backward_needs_its_workspace(lib):
+    for kw in (dict(ws=0), dict(ws_bytes=8), dict(ws=24)):
+        rc, text = call_attention(lib, backward=True, **kw)
+        assert rc == 3 and 'workspace' in text
+
+
+def test_layer_norm_abi_refuses_before_any_launch(lib):
+    err = ctypes.create_string_buffer(256)
+    p = ctypes.c_void_p(16)
+
+    def forward(dtype=0, rows=4, C=8, eps=1e-5, x=p, mean=None):
+        return lib.td_layer_norm_forward(dtype, x, None, p, None, p, mean, None, rows, C, eps, None, err, 256)
+
+    assert forward(dtype=9) == 1 and forward(rows=-1) == 1 and forward(C=0) == 1 and forward(C=8193) == 1
+    assert forward(eps=-1.0) == 1 and forward(x=None) == 1 and forward(mean=p) == 1
+    assert forward(rows=0, x=None) == 0
+    assert lib.td_layer_norm_workspace_bytes(0, 4, 8) == 1 * 2 * 8 * 4
+    assert lib.td_layer_norm_workspace_bytes(9, 4, 8) == 0
+    rc = lib.td_layer_norm_backward(0, p, p, None, p, p, p, p, p, p, 4, 8, p, 3, None, err, 256)
+    # without a device the launch's own query fails first on some machines; either way nothing is launched
+    assert rc in (2, 3)
