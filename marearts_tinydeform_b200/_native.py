@@ -773,8 +773,8 @@ def check_attention(query, key, value, key_padding_mask, attn_mask, scale):
             raise RuntimeError('attn_mask must be [Q, N] or [B or 1, H or 1, Q, N]')
         if attn_mask.device != dev:
             raise RuntimeError('attn_mask must be on the device of query')
-    if not (0 < scale < float('inf')):
-        raise RuntimeError('scale must be positive and finite')
+    if not 1e-30 <= scale <= 1e30:
+        raise RuntimeError('scale must be between 1e-30 and 1e30')
     return B, Q, N, H, Hk, D
 
 

@@ -1,19 +1,7 @@
 // td_attention.cu -- the attention entry points of the C ABI: argument contract, kernel choice and launches.
-#include <cmath>
-
-#include "td_attention.cuh"
-#include "td_host.h"
+#include "td_attention_plan.h"
 
 namespace td {
-
-cudaError_t attention_device_error(int clear, unsigned int* code) {
-    cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
-    if (e == cudaSuccess && clear) {
-        const unsigned int zero = 0;
-        e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
-    }
-    return e;
-}
 
 namespace {
 
@@ -21,7 +9,44 @@ using host::fail;
 
 int64_t pad_rows(int64_t Q) { return (Q + kAttnRowPad - 1) / kAttnRowPad * kAttnRowPad; }
 size_t elem_bytes(int dtype) { return dtype == TD_F64 ? 8 : dtype == TD_F32 ? 4 : 2; }
-size_t acc_bytes(int dtype) { return dtype == TD_F64 ? 8 : 4; }
+
+// The parts of a call's workspace. The mask's bits and flags are laid out for 16-bit types only (the tensor-core
+// kernels read them); a mask shared by images or heads is packed once.
+AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t mb, int64_t mh,
+                             bool padding, bool backward) {
+    AttnWorkspace w = {};
+    auto take = [&](size_t bytes) {
+        const size_t at = w.total;
+        w.total += (bytes + 255) / 256 * 256;
+        return at;
+    };
+    if (backward) {
+        w.amax = take(2 * sizeof(unsigned int));
+        w.delta = take(size_t(B) * H * pad_rows(Q) * (dtype == TD_F64 ? 8 : 4));
+    }
+    if ((dtype == TD_F16 || dtype == TD_BF16) && (mb > 0 || padding)) {
+        w.images = padding ? B : mb;
+        w.heads = mb > 0 ? mh : 1;
+        w.rows = mb > 0 ? Q : 1;
+        w.words = 2 * ((N + 63) / 64);
+        const int64_t bh = w.images * w.heads, q_tiles = (w.rows + 127) / 128;
+        w.row_bits = take(size_t(bh) * w.rows * w.words * 4);
+        w.row_flags = take(size_t(bh) * q_tiles * (w.words / 2));
+        if (backward && mb > 0) {
+            w.col_words = 2 * ((Q + 63) / 64);
+            w.col_bits = take(size_t(mb) * mh * N * w.col_words * 4);
+            w.col_flags = take(size_t(mb) * mh * ((N + 127) / 128) * (w.col_words / 2));
+        }
+    }
+    return w;
+}
+
+int check_workspace(const void* workspace, size_t bytes, size_t need, char* err, size_t err_len) {
+    if (need == 0 || (workspace != nullptr && bytes >= need && (reinterpret_cast<uintptr_t>(workspace) & 15u) == 0))
+        return TD_OK;
+    return fail(err, err_len, TD_ERR_WORKSPACE, "workspace must be 16-byte aligned, of %zu bytes (got %zu)", need,
+                bytes);
+}
 
 int check_sizes(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, double scale, char* err,
                 size_t err_len) {
@@ -36,8 +61,8 @@ int check_sizes(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t H
     if (double(Q) > most || double(N) > most || double(B) * double(H) * double(pad_rows(Q)) > most ||
         double(B) * double(Hk) * double(pad_rows(N)) > most)
         return fail(err, err_len, TD_ERR_ARG, "too many (batch, token, head) rows");
-    if (!(scale > 0) || !std::isfinite(scale))
-        return fail(err, err_len, TD_ERR_ARG, "scale must be positive and finite");
+    if (!(scale >= 1e-30) || !(scale <= 1e30))  // so that the kernels' float32 multiples of it stay in range
+        return fail(err, err_len, TD_ERR_ARG, "scale must be between 1e-30 and 1e30");
     return TD_OK;
 }
 
@@ -93,7 +118,7 @@ int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_
     if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
     const long long rows = (long long)a.B * a.H * a.Qp;
     if (int rc = host::launch(err, err_len, "attn_delta_kernel", attn_delta_kernel<T>,
-                              dim3(unsigned((rows + 7) / 8)), dim3(256), 0, stream, true, a))
+                              dim3(unsigned((rows + 255) / 256)), dim3(256), 0, stream, true, a))
         return rc;
     const int kv_blocks = (a.N + Tile::kRows - 1) / Tile::kRows * a.B * a.Hk;
     const int q_blocks = (a.Q + Tile::kRows - 1) / Tile::kRows * a.B * a.H;
@@ -123,9 +148,8 @@ extern "C" {
 size_t td_attention_workspace_bytes(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D,
                                     int64_t mask_b, int64_t mask_h, int has_padding, int backward) {
     using namespace td;
-    (void)mask_b; (void)mask_h; (void)has_padding;
-    if (check_sizes(dtype, B, Q, N, H, Hk, D, 1.0, nullptr, 0) != TD_OK) return 0;
-    return backward ? size_t(B) * H * pad_rows(Q) * acc_bytes(dtype) : 0;
+    if (check_sizes(dtype, B, Q, N, H, Hk, D, 1.0, nullptr, 0) != TD_OK || B == 0 || Q == 0 || N == 0) return 0;
+    return attn_workspace(dtype, B, Q, N, H, mask_b, mask_h, has_padding != 0, backward != 0).total;
 }
 
 int td_attention_forward(int dtype, const void* query, const void* key, const void* value, const int64_t* strides,
@@ -139,12 +163,17 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
     if (query == nullptr || out == nullptr || strides == nullptr || (N > 0 && (key == nullptr || value == nullptr)) ||
         (attn_mask != nullptr && mask_strides == nullptr))
         return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
-    (void)workspace; (void)workspace_bytes;
+    const int64_t mb = attn_mask == nullptr ? 0 : mask_strides[0] != 0 ? B : 1;
+    const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
+    const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, mb, mh, key_padding_mask != nullptr, false);
+    if (int rc = check_workspace(workspace, workspace_bytes, N > 0 ? ws.total : 0, err, err_len)) return rc;
     AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
     a.out = out;
     a.lse = lse;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (N > 0 && attn_tc_fits(dtype, a))
+        return attn_tc_forward(dtype, a, ws, mb, mh, static_cast<unsigned char*>(workspace), s, err, err_len);
     switch (dtype) {
         case TD_F32: return forward<float>(a, s, err, err_len);
         case TD_F16: return forward<__half>(a, s, err, err_len);
@@ -175,10 +204,10 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
         lse == nullptr || grad_out == nullptr || grad_query == nullptr || grad_key == nullptr ||
         grad_value == nullptr || (attn_mask != nullptr && mask_strides == nullptr))
         return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
-    const size_t need = td_attention_workspace_bytes(dtype, B, Q, N, H, Hk, D, 0, 0, 0, 1);
-    if (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)
-        return fail(err, err_len, TD_ERR_WORKSPACE, "workspace must be 16-byte aligned, of %zu bytes (got %zu)", need,
-                    workspace_bytes);
+    const int64_t mb = attn_mask == nullptr ? 0 : mask_strides[0] != 0 ? B : 1;
+    const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
+    const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, mb, mh, key_padding_mask != nullptr, true);
+    if (int rc = check_workspace(workspace, workspace_bytes, ws.total, err, err_len)) return rc;
     AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
     a.out_in = out;
@@ -187,7 +216,9 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
     a.grad_q = grad_query;
     a.grad_k = grad_key;
     a.grad_v = grad_value;
-    a.delta = workspace;
+    a.delta = static_cast<unsigned char*>(workspace) + ws.delta;
+    if (attn_tc_fits(dtype, a))
+        return attn_tc_backward(dtype, a, ws, mb, mh, static_cast<unsigned char*>(workspace), s, err, err_len);
     switch (dtype) {
         case TD_F32: return backward<float>(a, s, err, err_len);
         case TD_F16: return backward<__half>(a, s, err, err_len);

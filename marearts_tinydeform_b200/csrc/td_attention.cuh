@@ -243,12 +243,12 @@ __global__ void __launch_bounds__(256) attn_simt_forward_kernel(const AttnArgs a
         for (int i = i0 + M + int(threadIdx.x); i < a.Qp; i += 256) lse[(long long)bh * a.Qp + i] = A(INFINITY);
 }
 
-// delta[b, h, i] = grad_out . out over a query's head; zero in the rows behind the last query. A warp per row.
+// delta[b, h, i] = grad_out . out over a query's head; zero in the rows behind the last query. A thread per row, adding
+// in simt_dot's order: where a query has one key only, its result is that key's value and dP - delta is exactly zero.
 template <typename T>
 __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     using A = typename Elem<T>::acc;
-    const long long row = (long long)blockIdx.x * 8 + threadIdx.x / 32;  // (b * H + h) * Qp + i
-    const int lane = threadIdx.x % 32;
+    const long long row = (long long)blockIdx.x * 256 + threadIdx.x;  // (b * H + h) * Qp + i
     grid_dependency_wait();
     launch_dependents();
     if (row >= (long long)a.B * a.H * a.Qp) return;
@@ -259,11 +259,9 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
         const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D;
         const T* o = static_cast<const T*>(a.out_in) + at;
         const T* g = static_cast<const T*>(a.grad_out) + at;
-        for (int d = lane; d < a.D; d += 32) sum += to_acc(o[d]) * to_acc(g[d]);
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        for (int d = 0; d < a.D; ++d) sum += to_acc(o[d]) * to_acc(g[d]);
     }
-    if (lane == 0) static_cast<A*>(a.delta)[row] = sum;
+    static_cast<A*>(a.delta)[row] = sum;
 }
 
 // The gradient of the keys and values (blocks below kv_blocks: one tile of keys of one key head, over the query heads

@@ -1,0 +1,191 @@
+// td_attention_tc.cu -- launches of the attention's tensor-core kernels: conditions, tensor maps, packed masks.
+#include "td_attention_plan.h"
+#include "td_attention_tc.cuh"
+
+namespace td {
+
+cudaError_t attention_tc_device_error(int clear, unsigned int* code) {
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
+    if (e == cudaSuccess && clear) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+    }
+    return e;
+}
+
+namespace {
+
+using host::fail;
+
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// A [B, T, heads, D] operand with its element strides, as the tensor maps see it.
+struct Operand {
+    const void* base;
+    int tokens, heads;
+    long long s_b, s_t, s_h;
+};
+
+Operand query_of(const AttnArgs& a) { return {a.q, a.Q, a.H, a.q_b, a.q_t, a.q_h}; }
+Operand key_of(const AttnArgs& a) { return {a.k, a.N, a.Hk, a.k_b, a.k_t, a.k_h}; }
+Operand value_of(const AttnArgs& a) { return {a.v, a.N, a.Hk, a.v_b, a.v_t, a.v_h}; }
+Operand grad_of(const AttnArgs& a) {
+    const long long row = (long long)a.H * a.D;
+    return {a.grad_out, a.Q, a.H, a.Q * row, row, a.D};
+}
+
+// The stride of a dimension of one element says nothing: any legal one will do.
+long long map_stride(long long stride, int size, const AttnArgs& a) { return size > 1 ? stride : (a.D + 7) / 8 * 8; }
+
+bool operand_fits(const Operand& o, const AttnArgs& a) {
+    const long long s[3] = {map_stride(o.s_t, o.tokens, a), map_stride(o.s_h, o.heads, a), map_stride(o.s_b, a.B, a)};
+    for (long long x : s)
+        if (x <= 0 || x % 8 != 0 || x >= (1LL << 38)) return false;
+    return aligned16(o.base);
+}
+
+// Boxes of 64 columns x `rows` tokens of one head of one image, 128-byte swizzle; what lies outside reads as zero.
+int make_map(CUtensorMap* map, const Operand& o, int rows, const AttnArgs& a, char* err, size_t err_len) {
+    const uint64_t dims[4] = {uint64_t(a.D), uint64_t(o.tokens), uint64_t(o.heads), uint64_t(a.B)};
+    const uint64_t strides[3] = {uint64_t(map_stride(o.s_t, o.tokens, a)) * 2,
+                                 uint64_t(map_stride(o.s_h, o.heads, a)) * 2,
+                                 uint64_t(map_stride(o.s_b, a.B, a)) * 2};
+    const uint32_t box[4] = {64, uint32_t(rows), 1, 1};
+    const CUresult r = host::encode_tiled_u16(map, 4, o.base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r == CUDA_SUCCESS) return TD_OK;
+    return fail(err, err_len, TD_ERR_CUDA, "cuTensorMapEncodeTiled (attention) failed (%d)", int(r));
+}
+
+// Packs the masks of a call (if any) and fills args' pointers and strides.
+int pack_masks(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, bool backward, unsigned char* workspace,
+               cudaStream_t stream, char* err, size_t err_len) {
+    const AttnArgs& a = t.a;
+    if (w.images == 0) return TD_OK;
+    PackArgs p = {};
+    p.mask = a.mask;
+    p.padding = a.padding;
+    p.m_b = a.m_b; p.m_h = a.m_h; p.m_q = a.m_q;
+    p.images = int(w.images); p.heads = int(w.heads); p.rows = int(w.rows); p.N = a.N;
+    p.words = int(w.words);
+    p.row_bits = reinterpret_cast<uint32_t*>(workspace + w.row_bits);
+    p.row_flags = workspace + w.row_flags;
+    const long long q_tiles = (w.rows + 127) / 128, k_tiles = (a.N + 127) / 128;
+    t.row_bits = p.row_bits;
+    t.row_flags = p.row_flags;
+    t.rb_q = mb > 0 ? w.words : 0;
+    t.rb_h = w.heads > 1 ? w.rows * w.words : 0;
+    t.rb_b = w.images > 1 ? w.heads * w.rows * w.words : 0;
+    t.rf_q = mb > 0 ? w.words / 2 : 0;
+    t.rf_h = w.heads > 1 ? q_tiles * (w.words / 2) : 0;
+    t.rf_b = w.images > 1 ? w.heads * q_tiles * (w.words / 2) : 0;
+    if (backward && mb > 0) {
+        p.mask_images = int(mb);
+        p.col_words = int(w.col_words);
+        p.col_bits = reinterpret_cast<uint32_t*>(workspace + w.col_bits);
+        p.col_flags = workspace + w.col_flags;
+        t.col_bits = p.col_bits;
+        t.col_flags = p.col_flags;
+        t.col_words = p.col_words;
+        t.col_tiles = p.col_words / 2;
+        t.cb_h = mh > 1 ? (long long)a.N * w.col_words : 0;
+        t.cb_b = mb > 1 ? mh * (long long)a.N * w.col_words : 0;
+        t.cf_h = mh > 1 ? k_tiles * t.col_tiles : 0;
+        t.cf_b = mb > 1 ? mh * k_tiles * t.col_tiles : 0;
+    }
+    const long long blocks = w.images * w.heads * q_tiles * k_tiles;
+    if (blocks > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "attn_mask is too large");
+    return host::launch(err, err_len, "attn_pack_kernel", attn_pack_kernel, dim3(unsigned(blocks)), dim3(256), 0,
+                        stream, true, p);
+}
+
+template <typename T, int DP>
+int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsigned char* workspace,
+            cudaStream_t stream, char* err, size_t err_len) {
+    const AttnArgs& a = t.a;
+    CUtensorMap q, k, v;
+    if (int rc = make_map(&q, query_of(a), kAttnBM, a, err, err_len)) return rc;
+    if (int rc = make_map(&k, key_of(a), kAttnBN, a, err, err_len)) return rc;
+    if (int rc = make_map(&v, value_of(a), kAttnBN, a, err, err_len)) return rc;
+    if (int rc = pack_masks(t, w, mb, mh, false, workspace, stream, err, err_len)) return rc;
+    auto kernel = attn_tc_forward_kernel<T, DP>;
+    constexpr size_t smem = AttnFwdLayout<DP>::kSmemBytes;
+    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    const unsigned grid = unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
+    return host::launch(err, err_len, "attn_tc_forward_kernel", kernel, dim3(grid), dim3(kAttnFwdThreads), smem, stream,
+                        true, q, k, v, t);
+}
+
+template <typename T, int DP>
+int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsigned char* workspace,
+             cudaStream_t stream, char* err, size_t err_len) {
+    const AttnArgs& a = t.a;
+    const Operand ops[4] = {query_of(a), grad_of(a), key_of(a), value_of(a)};
+    CUtensorMap fixed[4], tile[4];
+    for (int i = 0; i < 4; ++i) {
+        if (int rc = make_map(&fixed[i], ops[i], kAttnBM, a, err, err_len)) return rc;
+        if (int rc = make_map(&tile[i], ops[i], kAttnBN, a, err, err_len)) return rc;
+    }
+    if (int rc = pack_masks(t, w, mb, mh, true, workspace, stream, err, err_len)) return rc;
+    int lanes = 1;
+    while (lanes * 8 < a.D) lanes *= 2;
+    const int per_block = 256 / lanes;
+    const unsigned delta_blocks = unsigned(((long long)a.B * a.H * a.Qp + per_block - 1) / per_block);
+    unsigned blocks = delta_blocks;
+    unsigned int* amax = nullptr;
+    if constexpr (std::is_same<T, __half>::value) {
+        amax = reinterpret_cast<unsigned int*>(workspace + w.amax);
+        const cudaError_t e = cudaMemsetAsync(amax, 0, 2 * sizeof(unsigned int), stream);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            return fail(err, err_len, TD_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
+        }
+        blocks += unsigned(((long long)a.B * a.Hk * a.N + per_block - 1) / per_block);
+    }
+    if (int rc = host::launch(err, err_len, "attn_delta_tc_kernel", attn_delta_tc_kernel<T>, dim3(blocks), dim3(256), 0,
+                              stream, true, a, lanes, delta_blocks, amax))
+        return rc;
+    t.amax = amax;
+    t.kv_blocks = (a.N + kAttnBM - 1) / kAttnBM * a.B * a.Hk;
+    auto kernel = attn_tc_backward_kernel<T, DP>;
+    constexpr size_t smem = AttnBwdLayout<DP>::kSmemBytes;
+    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    const unsigned grid = unsigned(t.kv_blocks) + unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
+    return host::launch(err, err_len, "attn_tc_backward_kernel", kernel, dim3(grid), dim3(kAttnBwdThreads), smem, stream,
+                        true, fixed[0], fixed[1], fixed[2], fixed[3], tile[0], tile[1], tile[2], tile[3], t);
+}
+
+}  // namespace
+
+bool attn_tc_fits(int dtype, const AttnArgs& a) {
+    if ((dtype != TD_F16 && dtype != TD_BF16) || !host::best_policy()) return false;
+    if (a.D % 8 != 0 || a.N <= 32) return false;
+    if (!operand_fits(query_of(a), a) || !operand_fits(key_of(a), a) || !operand_fits(value_of(a), a)) return false;
+    if (!aligned16(a.lse)) return false;
+    if (a.grad_q == nullptr) return aligned16(a.out);
+    return operand_fits(grad_of(a), a) && aligned16(a.out_in) && aligned16(a.grad_q) && aligned16(a.grad_k) &&
+           aligned16(a.grad_v);
+}
+
+int attn_tc_forward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_t mb, int64_t mh,
+                    unsigned char* workspace, cudaStream_t stream, char* err, size_t err_len) {
+    AttnTcArgs t = {};
+    t.a = a;
+    if (dtype == TD_F16)
+        return a.D <= 64 ? forward<__half, 64>(t, w, mb, mh, workspace, stream, err, err_len)
+                         : forward<__half, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+    return a.D <= 64 ? forward<__nv_bfloat16, 64>(t, w, mb, mh, workspace, stream, err, err_len)
+                     : forward<__nv_bfloat16, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+}
+
+int attn_tc_backward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_t mb, int64_t mh,
+                     unsigned char* workspace, cudaStream_t stream, char* err, size_t err_len) {
+    AttnTcArgs t = {};
+    t.a = a;
+    if (dtype == TD_F16)
+        return a.D <= 64 ? backward<__half, 64>(t, w, mb, mh, workspace, stream, err, err_len)
+                         : backward<__half, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+    return a.D <= 64 ? backward<__nv_bfloat16, 64>(t, w, mb, mh, workspace, stream, err, err_len)
+                     : backward<__nv_bfloat16, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+}
+
+}  // namespace td

@@ -1,0 +1,958 @@
+// td_attention_tc.cuh -- attention on tcgen05 tensor cores, float16 and bfloat16 (the mathematics: td_attention.cuh).
+//
+// Every product is a tcgen05.mma of 128 rows (TMEM lanes) whose elementwise work one thread does per row:
+//   forward          S = Q K^T (lanes = queries), P = exp2 over it, O += P V
+//   queries' grad    S = Q K^T, dP = dO V^T (lanes = queries), dS = P (dP - delta), dQ += dS K
+//   keys' grad       S^T = K Q^T, dP^T = V dO^T (lanes = keys), dV += P^T dO, dK += dS^T Q
+// so a 128-row operand stays in shared memory (K-major), tiles of 64 rows of the other side stream through a ring of
+// TMA slots, and each streamed tile serves as a K-major operand of one product and as an MN-major operand of another.
+// P and dS are rounded to the input type and written back to TMEM over the scores they came from, as the A operand of
+// the next product: neither ever reaches shared memory. The two gradients are separate blocks of one launch, each of
+// which forms S and dP itself: 7 products instead of 5 and twice the exponentials, but every sum has one owner and one
+// order (no atomics, no float32 gradient in memory).
+//
+// Columns past D (D < DP) and rows past the last token are zero through the tensor maps' fill. Scores of closed pairs
+// are replaced by -infinity (P, dS by zero); tiles without an open pair are skipped by every role alike, from one
+// flag byte per tile (attn_pack_kernel), and tiles whose pairs are all open skip the tests. Rows of padded keys, which
+// may hold anything, are cleared in shared memory where they are summed over (V in the forward, K in the queries'
+// gradient): zero times infinity is no zero.
+//
+// The exponential bounds these kernels at D <= 64 (16 a cycle and SM against 8192 multiply-adds), so the forward
+// runs two CTAs an SM (256 TMEM columns each), the backward two elementwise warpgroups a CTA, each on its own
+// tile; in both the next tile's scores are being formed meanwhile.
+#pragma once
+
+#include <type_traits>
+
+#include "td_attention.cuh"
+#include "td_ptx.cuh"
+
+namespace td {
+
+struct AttnTcArgs {
+    AttnArgs a;
+    // forward and queries' gradient: open-pair bits (1 = open, N rounded up to 64 bits a row) and tile flags (bit 0:
+    // some pair open, bit 1: all open) per 128 queries x 64 keys, padding included; strides 0 where shared; or null
+    const uint32_t* row_bits;
+    const uint8_t* row_flags;
+    long long rb_b, rb_h, rb_q, rf_b, rf_h, rf_q;
+    // keys' gradient: the same per key over the queries (128 keys x 64 queries), padding not included; or null
+    const uint32_t* col_bits;
+    const uint8_t* col_flags;
+    long long cb_b, cb_h, cf_b, cf_h;
+    int col_words;              // words a key's row of col_bits has
+    int col_tiles;              // flags a row of col_flags has
+    const unsigned int* amax;   // float16 backward: bits of max|dO| and max|V|
+    int kv_blocks;              // backward: blocks of the keys' gradient, launched first
+};
+
+constexpr int kAttnBM = 128, kAttnBN = 64;
+
+// ---- PTX ----------------------------------------------------------------------------------------------------------
+// D[tmem] (+)= A[tmem] x B[smem desc]: A is 128 lanes x K packed 16-bit elements, two a column.
+__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                           uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+        ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
+          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
+          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 4-D tiled load of box (x, y, z, w), completing its bytes on the mbarrier (x * element size a multiple of 16 bytes).
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int x, int y, int z,
+                                            int w, uint64_t pol) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5, %6}], [%2], %7;"
+        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(bar)), "r"(x), "r"(y), "r"(z),
+          "r"(w), "l"(pol)
+        : "memory");
+}
+// Plain copy of `bytes` (a multiple of 16, both addresses 16-byte aligned) into shared memory.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+        ::"r"(smem_addr(dst)), "l"(reinterpret_cast<uint64_t>(src)), "r"(bytes), "r"(smem_addr(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Two floats rounded to T, lo in the low half.
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// All lanes of a warp wait; false in every lane if any gave up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int code) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
+}
+
+// Calls f(tile, all pairs open by the flags) for the tiles in [t0, t1) with an open pair, in order, in whole warps,
+// until f returns false. flags: one byte a tile, or null (every tile, all open).
+template <typename F>
+__device__ __forceinline__ bool for_tiles(int t0, int t1, const uint8_t* flags, F&& f) {
+    const int lane = threadIdx.x & 31;
+    for (int base = t0; base < t1; base += 32) {
+        const int t = base + lane;
+        const unsigned fl = t >= t1 ? 0u : flags != nullptr ? unsigned(__ldg(flags + t)) : 3u;
+        unsigned any = __ballot_sync(0xffffffffu, (fl & 1u) != 0);
+        const unsigned all = __ballot_sync(0xffffffffu, (fl & 2u) != 0);
+        while (any != 0) {
+            const int x = __ffs(int(any)) - 1;
+            any &= any - 1;
+            if (!f(base + x, ((all >> x) & 1u) != 0)) return false;
+        }
+    }
+    return true;
+}
+
+// Bits of [0, 64) below `n` (n may be negative or above 64).
+__device__ __forceinline__ unsigned long long bits_below(int n) {
+    return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
+}
+
+// Instruction descriptor: f32 accumulator, A K-major, B K-major or MN-major, 128 x N.
+template <typename T, bool B_MN>
+__device__ __forceinline__ constexpr uint32_t attn_idesc(int N) {
+    return idesc_f16(std::is_same<T, __nv_bfloat16>::value, 128, N) | (uint32_t(B_MN) << 16);
+}
+
+// MN-major operand made of boxes of 64 rows (of K) by 64 columns: next 8 K rows 1024 bytes on, next 64 columns
+// 64 * 128 bytes on.
+__device__ __forceinline__ uint64_t sdesc_mn64(uint32_t saddr) {
+    uint64_t d = sdesc_sw128(saddr);
+    d |= uint64_t(8192 >> 4) << 16;
+    return d;
+}
+
+// D = A x B^T over DP columns: A 128 rows, B 64 rows, both K-major in boxes of 64 columns.
+template <typename T, int DP>
+__device__ __forceinline__ void issue_scores(uint32_t d, uint32_t a_smem, uint32_t b_smem) {
+    constexpr uint32_t idesc = attn_idesc<T, false>(kAttnBN);
+#pragma unroll
+    for (int k = 0; k < DP / 16; ++k) {
+        const uint64_t da = sdesc_sw128(a_smem + (k / 4) * 16384) + uint64_t(2 * (k % 4));
+        const uint64_t db = sdesc_sw128(b_smem + (k / 4) * 8192) + uint64_t(2 * (k % 4));
+        mma_f16(d, da, db, idesc, k != 0);
+    }
+}
+
+// acc (+)= A x B: A 128 lanes x 64 packed elements in TMEM, B 64 rows x DP columns in shared memory.
+template <typename T, int DP>
+__device__ __forceinline__ void issue_product(uint32_t acc, uint32_t a_tmem, uint32_t b_smem, bool first) {
+    constexpr uint32_t idesc = attn_idesc<T, true>(DP);
+    const uint64_t db = sdesc_mn64(b_smem);
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        mma_f16_ts(acc, a_tmem + 8 * k, db + uint64_t(128 * k), idesc, !(first && k == 0));
+}
+
+// Clears the rows of padded keys in a slot's tile of 64 rows x DP columns (boxes of 64 rows x 128 bytes). One warp.
+template <int DP>
+__device__ __forceinline__ void clear_padded(unsigned char* tile, const uint8_t* pad, int j0, int N) {
+    const int lane = threadIdx.x & 31;
+    const bool p0 = j0 + lane < N && pad[j0 + lane] != 0, p1 = j0 + 32 + lane < N && pad[j0 + 32 + lane] != 0;
+    unsigned long long rows = (unsigned long long)__ballot_sync(0xffffffffu, p0) |
+                              (unsigned long long)__ballot_sync(0xffffffffu, p1) << 32;
+    while (rows != 0) {
+        const int r = __ffsll((long long)rows) - 1;
+        rows &= rows - 1;
+#pragma unroll
+        for (int box = 0; box < DP / 64; ++box)  // a whole 128-byte row: the swizzle only permutes inside it
+            *reinterpret_cast<uint32_t*>(tile + box * 8192 + r * 128 + lane * 4) = 0u;
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// ---- forward ------------------------------------------------------------------------------------------------------
+template <int DP>
+struct AttnFwdLayout {
+    static constexpr int kBoxes = DP / 64;
+    static constexpr uint32_t kQBytes = kAttnBM * 128 * kBoxes;
+    static constexpr uint32_t kTileBytes = kAttnBN * 128 * kBoxes;  // of K or of V
+    static constexpr int kStages = DP == 64 ? 4 : 2;                // two CTAs an SM
+    static constexpr uint32_t kStageBytes = 2 * kTileBytes;
+    static constexpr uint32_t kRing = kQBytes;
+    static constexpr uint32_t kBars = kRing + kStages * kStageBytes;
+    // qfull, kfull[S], vfull[S], ready[S], empty[S], sfull[2], pfull[2], done[2], finished
+    static constexpr int kNumBars = 1 + 4 * kStages + 7;
+    static constexpr uint32_t kSlot = kBars + kNumBars * 8;
+    static constexpr uint32_t kSmemBytes = kSlot + 16 + 1024;
+    static constexpr uint32_t kTmemCols = 256;  // two score tiles of 64, the output's DP
+    static_assert(128 + DP <= 256, "TMEM");
+    static_assert(2 * kSmemBytes <= 227 * 1024, "two CTAs an SM");
+};
+
+constexpr int kAttnFwdThreads = 256;  // producer, MMA, clearing, -, four softmax warps
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAttnFwdThreads, 2)
+    attn_tc_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
+                           const __grid_constant__ CUtensorMap map_v, const AttnTcArgs args) {
+    using Lay = AttnFwdLayout<DP>;
+    constexpr int S = Lay::kStages, KB = Lay::kBoxes;
+    const AttnArgs& a = args.a;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
+    uint64_t *kfull = qfull + 1, *vfull = kfull + S, *ready = vfull + S, *empty = ready + S, *sfull = empty + S,
+             *pfull = sfull + 2, *done = pfull + 2, *finished = done + 2;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Lay::kSlot);
+    auto k_tile = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes; };
+    auto v_tile = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes + Lay::kTileBytes; };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the last query tiles first: under the causal rule they are the longest
+    const int q_tiles = (a.Q + kAttnBM - 1) / kAttnBM;
+    const int bh = blockIdx.x % (a.B * a.H), qt = q_tiles - 1 - int(blockIdx.x) / (a.B * a.H);
+    const int h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk), i0 = qt * kAttnBM, off = a.N - a.Q;
+    const int tiles = (attn_key_end(a, i0 + kAttnBM) + kAttnBN - 1) / kAttnBN;
+    const uint8_t* flags = args.row_flags == nullptr
+                               ? nullptr
+                               : args.row_flags + b * args.rf_b + h * args.rf_h + qt * args.rf_q;
+    const bool clearing = a.padding != nullptr;
+
+    if (threadIdx.x == 0) {
+        mbar_init(qfull, KB);
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&kfull[s], KB);
+            mbar_init(&vfull[s], KB);
+            mbar_init(&ready[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&sfull[g], 1);
+            mbar_init(&pfull[g], 128);
+            mbar_init(&done[g], 1);
+        }
+        mbar_init(finished, 1);
+        mbar_fence_init();
+        tma_prefetch_desc(&map_q);
+        tma_prefetch_desc(&map_k);
+        tma_prefetch_desc(&map_v);
+    }
+    if (warp == 1) {
+        tmem_alloc(tmem_slot, Lay::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+    launch_dependents();
+
+    if (warp == 0) {
+        // a lane per box: TMA copies of one thread are served one after another, those of different threads overlap
+        const uint64_t pol = l2_evict_last();  // keys and values are read again by the other query tiles
+        if (lane < KB && tiles > 0) {
+            mbar_arrive_expect_tx(qfull, Lay::kQBytes / KB);
+            tma_load_4d(smem + lane * 16384, &map_q, qfull, 64 * lane, i0, h, b, l2_evict_first());
+        }
+        int n = 0;
+        for_tiles(0, tiles, flags, [&](int t, bool) {
+            const int s = n % S;
+            if (!warp_wait(&empty[s], uint32_t((n / S) & 1) ^ 1u, kErrSlotWait)) return false;
+            if (lane < 2 * KB) {
+                const int box = lane % KB;
+                uint64_t* bar = lane < KB ? &kfull[s] : &vfull[s];
+                mbar_arrive_expect_tx(bar, 8192u);
+                tma_load_4d((lane < KB ? k_tile(s) : v_tile(s)) + box * 8192, lane < KB ? &map_k : &map_v, bar,
+                            64 * box, t * kAttnBN, hk, b, pol);
+            }
+            __syncwarp();
+            ++n;
+            return true;
+        });
+        // no copy and no product is in flight when the CTA ends
+        for (int i = n > S ? n - S : 0; i < n; ++i)
+            if (!warp_wait(&empty[i % S], uint32_t((i / S) & 1), kErrSlotWait)) {
+                warp_wait(&kfull[i % S], uint32_t((i / S) & 1), kErrTmaWait);
+                warp_wait(&vfull[i % S], uint32_t((i / S) & 1), kErrTmaWait);
+            }
+    } else if (warp == 1) {
+        int n = 0;
+        bool ok = tiles == 0 || warp_wait(qfull, 0u, kErrTmaWait);
+        auto product = [&](int m) {  // O += P V of tile number m
+            const int s = m % S;
+            if (!warp_wait(clearing ? &ready[s] : &vfull[s], uint32_t((m / S) & 1), kErrTmaWait)) return false;
+            if (!warp_wait(&pfull[m & 1], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
+            tc_fence_after();
+            if (lane == 0) {
+                issue_product<T, DP>(tmem + 128, tmem + 64 * (m & 1), smem_addr(v_tile(s)), m == 0);
+                mma_commit(&empty[s]);
+                mma_commit(&done[m & 1]);
+            }
+            __syncwarp();
+            return true;
+        };
+        if (ok)
+            ok = for_tiles(0, tiles, flags, [&](int, bool) {
+                const int s = n % S;
+                if (!warp_wait(&kfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                tc_fence_after();
+                // the score buffer is free: P of tile n - 2 was read by a product issued before this one
+                if (lane == 0) {
+                    issue_scores<T, DP>(tmem + 64 * (n & 1), smem_addr(smem), smem_addr(k_tile(s)));
+                    mma_commit(&sfull[n & 1]);
+                }
+                __syncwarp();
+                ++n;
+                return n < 2 || product(n - 2);
+            });
+        if (ok && n > 0 && product(n - 1) && lane == 0) mma_commit(finished);
+    } else if (warp == 2) {
+        if (clearing) {
+            int n = 0;
+            const uint8_t* pad = a.padding + (long long)b * a.N;
+            for_tiles(0, tiles, flags, [&](int t, bool) {
+                const int s = n % S;
+                if (!warp_wait(&vfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                clear_padded<DP>(v_tile(s), pad, t * kAttnBN, a.N);
+                if (lane == 0) mbar_arrive(&ready[s]);
+                ++n;
+                return true;
+            });
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, i = i0 + quarter * 32 + lane;
+        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
+        const float c = float(a.scale * 1.4426950408889634);
+        // The reference of a row's exponentials follows its maximum only when that grew by more than 8 (base 2), so
+        // P stays below 2^8 and the output, in TMEM, is seldom rescaled.
+        const float slack = 8.0f / c;
+        const uint32_t* bits = args.row_bits == nullptr
+                                   ? nullptr
+                                   : args.row_bits + b * args.rb_b + h * args.rb_h + min(i, a.Q - 1) * args.rb_q;
+        float ref = -INFINITY, sum = 0.f;
+        int n = 0;
+        const bool ok = for_tiles(0, tiles, flags, [&](int t, bool all) {
+            const int j0 = t * kAttnBN;
+            const bool open = all && j0 + kAttnBN <= a.N && (!a.causal || j0 + kAttnBN - 1 <= i0 + off);
+            unsigned long long w = ~0ull;
+            if (!open) {
+                w = bits_below(a.N - j0);
+                if (a.causal) w &= bits_below(i + off - j0 + 1);
+                if (bits != nullptr) {
+                    const uint2 x = __ldg(reinterpret_cast<const uint2*>(bits + 2 * t));
+                    w &= (unsigned long long)x.y << 32 | x.x;
+                }
+            }
+            if (!warp_wait(&sfull[n & 1], uint32_t((n >> 1) & 1), kErrMmaWait)) return false;
+            tc_fence_after();
+            const uint32_t sc = lanes + 64 * (n & 1);
+            uint32_t v[2][32];
+            tmem_ld_32x32b_x32(sc, v[0]);
+            tmem_ld_32x32b_x32(sc + 32, v[1]);
+            tmem_ld_wait();
+            float top = -INFINITY;
+#pragma unroll
+            for (int g = 0; g < 2; ++g) {
+                if (!open) {
+                    const uint32_t wg = uint32_t(w >> (32 * g));
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (((wg >> x) & 1u) == 0) v[g][x] = 0xff800000u;  // -infinity
+                }
+#pragma unroll
+                for (int x = 0; x < 32; ++x) top = fmaxf(top, __uint_as_float(v[g][x]));
+            }
+            if (__any_sync(0xffffffffu, top > ref + slack)) {
+                const float next = fmaxf(ref, top);
+                const float keep = next == -INFINITY ? 1.f : ex2((ref - next) * c);
+                ref = next;
+                sum *= keep;
+                if (n > 0) {
+                    // the output so far is complete once the last product is (a barrier each for even and odd tiles:
+                    // a parity wait tells one phase from the next only, and not every phase is waited for)
+                    if (!warp_wait(&done[(n - 1) & 1], uint32_t(((n - 1) >> 1) & 1), kErrMmaWait)) return false;
+                    tc_fence_after();
+#pragma unroll 1
+                    for (int d = 0; d < DP; d += 32) {
+                        uint32_t o[32];
+                        tmem_ld_32x32b_x32(lanes + 128 + d, o);
+                        tmem_ld_wait();
+#pragma unroll
+                        for (int x = 0; x < 32; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * keep);
+                        tmem_st_32x32b_x32(lanes + 128 + d, o);
+                    }
+                }
+            }
+            const float shift = ref == -INFINITY ? 0.f : -ref * c;
+            uint32_t p[32];
+#pragma unroll
+            for (int x = 0; x < 32; ++x) {
+                const float p0 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16)]), c, shift));
+                const float p1 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16) + 1]), c, shift));
+                sum += p0 + p1;
+                p[x] = pack2<T>(p0, p1);
+            }
+            tmem_st_32x32b_x32(sc, p);
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&pfull[n & 1]);
+            ++n;
+            return true;
+        });
+        const bool got = ok && (n == 0 || warp_wait(finished, 0u, kErrMmaWait));
+        tc_fence_after();
+        if (got) {
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            T* out = static_cast<T*>(a.out) + (((long long)b * a.Q + i) * a.H + h) * a.D;
+#pragma unroll 1
+            for (int d = 0; d < DP && d < a.D; d += 32) {
+                uint32_t o[32];
+                __syncwarp();
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(lanes + 128 + d, o);
+                    tmem_ld_wait();
+                } else {
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+                }
+                if (i >= a.Q) continue;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (d + 8 * g >= a.D) break;  // D is a multiple of 8
+                    uint4 q;
+                    uint32_t* qw = &q.x;
+#pragma unroll
+                    for (int x = 0; x < 4; ++x)
+                        qw[x] = pack2<T>(__uint_as_float(o[8 * g + 2 * x]) * inv,
+                                         __uint_as_float(o[8 * g + 2 * x + 1]) * inv);
+                    *reinterpret_cast<uint4*>(out + d + 8 * g) = q;
+                }
+            }
+            if (a.lse != nullptr)  // Qp is a multiple of the tile
+                static_cast<float*>(a.lse)[(long long)bh * a.Qp + i] =
+                    i < a.Q && sum != 0.f ? fmaf(ref, c, log2f(sum)) : INFINITY;
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, Lay::kTmemCols);
+    }
+}
+
+// ---- backward -----------------------------------------------------------------------------------------------------
+template <int DP>
+struct AttnBwdLayout {
+    static constexpr int kBoxes = DP / 64;
+    static constexpr uint32_t kFixedBytes = kAttnBM * 128 * kBoxes;  // one resident operand
+    static constexpr uint32_t kTileBytes = kAttnBN * 128 * kBoxes;   // one streamed operand
+    static constexpr int kStages = 4;
+    static constexpr uint32_t kStageBytes = 2 * kTileBytes;
+    static constexpr uint32_t kRing = 2 * kFixedBytes;
+    static constexpr uint32_t kStats = kRing + kStages * kStageBytes;  // per stage: lse[64], delta[64]
+    static constexpr uint32_t kBars = kStats + kStages * 2 * kAttnBN * 4;
+    // fixed, full[S], ready[S], empty[S], sfull[2], pfull[2], finished
+    static constexpr int kNumBars = 1 + 3 * kStages + 5;
+    static constexpr uint32_t kSlot = kBars + kNumBars * 8;
+    static constexpr uint32_t kSmemBytes = kSlot + 16 + 1024;
+    static constexpr uint32_t kTmemCols = 512;  // per warpgroup S and dP of 64, then two accumulators of DP
+    static_assert(256 + 2 * DP <= 512, "TMEM");
+    static_assert(kSmemBytes <= 227 * 1024, "shared memory");
+};
+
+constexpr int kAttnBwdThreads = 384;  // producer, MMA, clearing, -, two elementwise warpgroups
+
+// float16 keeps P as 2^12 P (at most 4096, so that a row over many thousand keys stays above its smallest normal
+// number) and dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
+// gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs neither.
+constexpr float kHalfPShift = 12.f;
+
+__device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {
+    const float bound = 2.f * float(args.a.D) * __uint_as_float(args.amax[0]) * __uint_as_float(args.amax[1]);
+    if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
+    return exp2f(fminf(fmaxf(15.f - kHalfPShift - ceilf(log2f(bound)), -100.f), 100.f));
+}
+
+// One block of the keys' gradient (KEYS) or of the queries' gradient.
+template <typename T, int DP, bool KEYS>
+__device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fixed1, const CUtensorMap& map_fixed2,
+                                                       const CUtensorMap& map_b1, const CUtensorMap& map_b2,
+                                                       const AttnTcArgs& args, int block, unsigned char* smem,
+                                                       uint32_t tmem) {
+    using Lay = AttnBwdLayout<DP>;
+    constexpr int S = Lay::kStages, KB = Lay::kBoxes;
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const AttnArgs& a = args.a;
+    uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
+    uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + 2,
+             *finished = pfull + 2;
+    auto tile1 = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes; };
+    auto tile2 = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes + Lay::kTileBytes; };
+    auto stats = [&](int s) { return reinterpret_cast<float*>(smem + Lay::kStats) + s * 2 * kAttnBN; };
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, off = a.N - a.Q, group = a.H / a.Hk;
+    // the block's rows: keys r0 .. of key head hk, over the query heads h0 .. h1 and their query tiles; or queries
+    // r0 .. of head h0, over the key tiles
+    const int heads = KEYS ? a.Hk : a.H, rows = KEYS ? a.N : a.Q;
+    const int row_tiles = (rows + kAttnBM - 1) / kAttnBM;
+    const int bx = block % (a.B * heads);
+    // the longest blocks under the causal rule first: the first keys, the last queries
+    const int rt = KEYS ? block / (a.B * heads) : row_tiles - 1 - block / (a.B * heads);
+    const int head = bx % heads, b = bx / heads, r0 = rt * kAttnBM;
+    const int hk = KEYS ? head : head / group, h0 = KEYS ? head * group : head, h1 = KEYS ? h0 + group : h0 + 1;
+    const int t0 = KEYS && a.causal ? max(0, min(a.Q, r0 - off)) / kAttnBN : 0;
+    const int t1 = KEYS ? (a.Q + kAttnBN - 1) / kAttnBN
+                        : (attn_key_end(a, r0 + kAttnBM) + kAttnBN - 1) / kAttnBN;
+    const bool clearing = !KEYS && a.padding != nullptr;
+    auto each_tile = [&](auto&& f) {  // f(head, tile, all open by the flags)
+        for (int h = h0; h < h1; ++h) {
+            const uint8_t* flags = nullptr;
+            if (KEYS && args.col_flags != nullptr)
+                flags = args.col_flags + b * args.cf_b + h * args.cf_h + (long long)rt * args.col_tiles;
+            if (!KEYS && args.row_flags != nullptr)
+                flags = args.row_flags + b * args.rf_b + h * args.rf_h + rt * args.rf_q;
+            if (!for_tiles(t0, t1, flags, [&](int t, bool all) { return f(h, t, all); })) return false;
+        }
+        return true;
+    };
+
+    if (warp == 0) {
+        const uint64_t pol = l2_evict_last();
+        if (lane < 2 * KB) {
+            const int box = lane % KB;
+            mbar_arrive_expect_tx(fixed, 16384u);
+            tma_load_4d(smem + (lane / KB) * Lay::kFixedBytes + box * 16384, lane < KB ? &map_fixed1 : &map_fixed2,
+                        fixed, 64 * box, r0, head, b, pol);
+        }
+        int n = 0;
+        each_tile([&](int h, int t, bool) {
+            const int s = n % S;
+            if (!warp_wait(&empty[s], uint32_t((n / S) & 1) ^ 1u, kErrSlotWait)) return false;
+            if (lane < 2 * KB) {
+                const int box = lane % KB;
+                mbar_arrive_expect_tx(&full[s], 8192u);
+                tma_load_4d((lane < KB ? tile1(s) : tile2(s)) + box * 8192, lane < KB ? &map_b1 : &map_b2, &full[s],
+                            64 * box, t * kAttnBN, KEYS ? h : hk, b, pol);
+            } else if (KEYS && lane < 2 * KB + 2) {
+                const float* src = static_cast<const float*>(lane == 2 * KB ? a.lse : a.delta);
+                mbar_arrive_expect_tx(&full[s], kAttnBN * 4u);
+                bulk_load(stats(s) + (lane - 2 * KB) * kAttnBN,
+                          src + ((long long)b * a.H + h) * a.Qp + t * kAttnBN, kAttnBN * 4u, &full[s]);
+            }
+            __syncwarp();
+            ++n;
+            return true;
+        });
+        warp_wait(fixed, 0u, kErrTmaWait);
+        for (int i = n > S ? n - S : 0; i < n; ++i)
+            if (!warp_wait(&empty[i % S], uint32_t((i / S) & 1), kErrSlotWait))
+                warp_wait(&full[i % S], uint32_t((i / S) & 1), kErrTmaWait);
+    } else if (warp == 1) {
+        int n = 0;
+        bool ok = warp_wait(fixed, 0u, kErrTmaWait);
+        auto products = [&](int m) {  // the accumulators' part of tile number m
+            const int s = m % S;
+            const uint32_t sc = tmem + 128 * (m & 1);
+            if (!warp_wait(&pfull[m & 1], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
+            tc_fence_after();
+            if (lane == 0) {
+                if constexpr (KEYS)
+                    issue_product<T, DP>(tmem + 256 + DP, sc, smem_addr(tile2(s)), m == 0);  // dV += P^T dO
+                issue_product<T, DP>(tmem + 256, sc + 64, smem_addr(tile1(s)), m == 0);      // dK += dS^T Q, dQ += dS K
+                mma_commit(&empty[s]);
+            }
+            __syncwarp();
+            return true;
+        };
+        if (ok)
+            ok = each_tile([&](int, int, bool) {
+                const int s = n % S;
+                if (!warp_wait(clearing ? &ready[s] : &full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                tc_fence_after();
+                if (lane == 0) {
+                    const uint32_t sc = tmem + 128 * (n & 1);
+                    issue_scores<T, DP>(sc, smem_addr(smem), smem_addr(tile1(s)));
+                    issue_scores<T, DP>(sc + 64, smem_addr(smem + Lay::kFixedBytes), smem_addr(tile2(s)));
+                    mma_commit(&sfull[n & 1]);
+                }
+                __syncwarp();
+                ++n;
+                return n < 2 || products(n - 2);
+            });
+        if (ok && n > 0 && products(n - 1) && lane == 0) mma_commit(finished);
+    } else if (warp == 2) {
+        if (clearing) {
+            int n = 0;
+            const uint8_t* pad = a.padding + (long long)b * a.N;
+            each_tile([&](int, int t, bool) {
+                const int s = n % S;
+                if (!warp_wait(&full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                clear_padded<DP>(tile1(s), pad, t * kAttnBN, a.N);
+                if (lane == 0) mbar_arrive(&ready[s]);
+                ++n;
+                return true;
+            });
+        }
+    } else if (warp >= 4) {
+        const int quarter = warp & 3, wg = (warp - 4) >> 2, r = r0 + quarter * 32 + lane;
+        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), sc = lanes + 128 * wg;
+        const float c = float(a.scale * 1.4426950408889634);
+        const float ds_scale = kHalf ? attn_ds_scale(args) : 1.f;
+        const float p_shift = kHalf ? kHalfPShift : 0.f;
+        float row_lse = INFINITY, row_delta = 0.f;
+        if (!KEYS) {  // the rows' own statistics (the arrays hold Qp rows, a multiple of the tile)
+            const long long at = ((long long)b * a.H + h0) * a.Qp + r;
+            row_lse = static_cast<const float*>(a.lse)[at] - p_shift;
+            row_delta = static_cast<const float*>(a.delta)[at] * ds_scale;
+        }
+        int n = 0;
+        bool ok = each_tile([&](int h, int t, bool all) {
+            const int m = n++;
+            if ((m & 1) != wg) return true;
+            const int c0 = t * kAttnBN;  // the tile's first column: a query (KEYS) or a key
+            bool open = all;
+            unsigned long long w = ~0ull;
+            if constexpr (KEYS) {
+                open = open && (!a.causal || r0 + kAttnBM - 1 <= c0 + off);
+                if (!open) {
+                    if (a.causal) w &= ~bits_below(r - off - c0);
+                    if (args.col_bits != nullptr && r < a.N) {
+                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(
+                            args.col_bits + b * args.cb_b + h * args.cb_h + (long long)r * args.col_words + 2 * t));
+                        w &= (unsigned long long)x.y << 32 | x.x;
+                    }
+                }
+            } else {
+                open = open && c0 + kAttnBN <= a.N && (!a.causal || c0 + kAttnBN - 1 <= r0 + off);
+                if (!open) {
+                    w = bits_below(a.N - c0);
+                    if (a.causal) w &= bits_below(r + off - c0 + 1);
+                    if (args.row_bits != nullptr) {
+                        const uint2 x = __ldg(reinterpret_cast<const uint2*>(
+                            args.row_bits + b * args.rb_b + h * args.rb_h + min(r, a.Q - 1) * args.rb_q + 2 * t));
+                        w &= (unsigned long long)x.y << 32 | x.x;
+                    }
+                }
+            }
+            if (!warp_wait(&sfull[wg], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
+            if (KEYS && !warp_wait(&full[m % S], uint32_t((m / S) & 1), kErrTmaWait)) return false;  // the statistics
+            tc_fence_after();
+            const float* st = stats(m % S);
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                uint32_t s[32], d[32], p[16], e[16];
+                tmem_ld_32x32b_x32(sc + 32 * half, s);
+                tmem_ld_32x32b_x32(sc + 64 + 32 * half, d);
+                tmem_ld_wait();
+                const uint32_t wh = uint32_t(w >> (32 * half));
+#pragma unroll
+                for (int x = 0; x < 32; x += 4) {
+                    float4 ls = make_float4(row_lse, row_lse, row_lse, row_lse);
+                    float4 de = make_float4(row_delta, row_delta, row_delta, row_delta);
+                    if constexpr (KEYS) {
+                        ls = *reinterpret_cast<const float4*>(st + 32 * half + x);
+                        de = *reinterpret_cast<const float4*>(st + kAttnBN + 32 * half + x);
+                    }
+                    const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {de.x, de.y, de.z, de.w};
+                    float pv[4], ev[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        const float sv = __uint_as_float(s[x + y]), dp = __uint_as_float(d[x + y]);
+                        if constexpr (KEYS && kHalf) {
+                            pv[y] = ex2(fmaf(sv, c, kHalfPShift - lv[y]));
+                            ev[y] = pv[y] * ds_scale * (dp - dv[y]);
+                        } else if constexpr (kHalf) {
+                            pv[y] = ex2(fmaf(sv, c, -lv[y]));
+                            ev[y] = pv[y] * fmaf(dp, ds_scale, -dv[y]);
+                        } else {
+                            pv[y] = ex2(fmaf(sv, c, -lv[y]));
+                            ev[y] = pv[y] * (dp - dv[y]);
+                        }
+                        if (!open && ((wh >> (x + y)) & 1u) == 0) pv[y] = ev[y] = 0.f;
+                    }
+                    p[x / 2] = pack2<T>(pv[0], pv[1]);
+                    p[x / 2 + 1] = pack2<T>(pv[2], pv[3]);
+                    e[x / 2] = pack2<T>(ev[0], ev[1]);
+                    e[x / 2 + 1] = pack2<T>(ev[2], ev[3]);
+                }
+                if constexpr (KEYS) tmem_st_32x32b_x16(sc + 16 * half, p);
+                tmem_st_32x32b_x16(sc + 64 + 16 * half, e);
+            }
+            tmem_st_wait();
+            tc_fence_before();
+            mbar_arrive(&pfull[wg]);
+            return true;
+        });
+        ok = ok && (n == 0 || warp_wait(finished, 0u, kErrMmaWait));
+        tc_fence_after();
+        // the gradients' rows: a warpgroup an accumulator for the keys' block, else half of the columns each
+        if (ok) {
+            const bool is_v = KEYS && wg == 1;
+            const float k_scale = float(a.scale) / (kHalf ? exp2f(kHalfPShift) * ds_scale : 1.f);
+            const float f = is_v ? (kHalf ? exp2f(-kHalfPShift) : 1.f) : k_scale;
+            const bool gone = KEYS && a.padding != nullptr && r < a.N && a.padding[(long long)b * a.N + r] != 0;
+            T* out = KEYS ? static_cast<T*>(is_v ? a.grad_v : a.grad_k) + (((long long)b * a.N + r) * a.Hk + hk) * a.D
+                          : static_cast<T*>(a.grad_q) + (((long long)b * a.Q + r) * a.H + h0) * a.D;
+            const int d_first = KEYS ? 0 : 32 * wg, d_step = KEYS ? 32 : 64;
+#pragma unroll 1
+            for (int d = d_first; d < DP && d < a.D; d += d_step) {
+                uint32_t o[32];
+                __syncwarp();
+                if (n > 0) {
+                    tmem_ld_32x32b_x32(lanes + 256 + (is_v ? DP : 0) + d, o);
+                    tmem_ld_wait();
+                }
+                if (r >= rows) continue;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    if (d + 8 * g >= a.D) break;
+                    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+                    uint32_t* qw = &q.x;
+                    if (n > 0 && !gone) {
+#pragma unroll
+                        for (int x = 0; x < 4; ++x)
+                            qw[x] = pack2<T>(__uint_as_float(o[8 * g + 2 * x]) * f,
+                                             __uint_as_float(o[8 * g + 2 * x + 1]) * f);
+                    }
+                    *reinterpret_cast<uint4*>(out + d + 8 * g) = q;
+                }
+            }
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAttnBwdThreads, 1)
+    attn_tc_backward_kernel(const __grid_constant__ CUtensorMap q128, const __grid_constant__ CUtensorMap g128,
+                            const __grid_constant__ CUtensorMap k128, const __grid_constant__ CUtensorMap v128,
+                            const __grid_constant__ CUtensorMap q64, const __grid_constant__ CUtensorMap g64,
+                            const __grid_constant__ CUtensorMap k64, const __grid_constant__ CUtensorMap v64,
+                            const AttnTcArgs args) {
+    using Lay = AttnBwdLayout<DP>;
+    constexpr int S = Lay::kStages, KB = Lay::kBoxes;
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Lay::kSlot);
+    const bool keys = int(blockIdx.x) < args.kv_blocks;
+    if (threadIdx.x == 0) {
+        uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
+        uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + 2;
+        mbar_init(fixed, 2 * KB);
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 2 * KB + (keys ? 2 : 0));
+            mbar_init(&ready[s], 1);
+            mbar_init(&empty[s], 1);
+        }
+        for (int g = 0; g < 2; ++g) {
+            mbar_init(&sfull[g], 1);
+            mbar_init(&pfull[g], 128);
+        }
+        mbar_init(pfull + 2, 1);  // finished
+        mbar_fence_init();
+    }
+    if ((threadIdx.x >> 5) == 1) {
+        tmem_alloc(tmem_slot, Lay::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    grid_dependency_wait();
+    launch_dependents();
+    if (keys)
+        attn_tc_backward_block<T, DP, true>(k128, v128, q64, g64, args, int(blockIdx.x), smem, tmem);
+    else
+        attn_tc_backward_block<T, DP, false>(q128, g128, k64, v64, args, int(blockIdx.x) - args.kv_blocks, smem,
+                                             tmem);
+    tc_fence_before();
+    __syncthreads();
+    if ((threadIdx.x >> 5) == 1) {
+        tc_fence_after();
+        tmem_dealloc(tmem, Lay::kTmemCols);
+    }
+}
+
+// ---- what the kernels above are given ---------------------------------------------------------------------------
+// Open-pair bits and tile flags from the byte masks. A block takes 128 queries x 128 keys of one (image, head) of the
+// mask: a warp's ballot makes a row's word, and the words of 32 rows, transposed through shared memory, a key's.
+struct PackArgs {
+    const uint8_t* mask;     // as in AttnArgs; or null: one row per image, from the padding alone
+    const uint8_t* padding;
+    long long m_b, m_h, m_q;
+    uint32_t* row_bits;      // [images, heads, rows, words]
+    uint8_t* row_flags;      // [images, heads, row tiles of 128, tiles of 64 keys]
+    uint32_t* col_bits;      // [mask images, heads, N, q words], or null
+    uint8_t* col_flags;      // [mask images, heads, key tiles of 128, tiles of 64 queries]
+    int images, heads, rows, N;      // rows: Q, or 1 without a mask
+    int mask_images;                 // images the mask itself has (col_bits exist for these)
+    int words, col_words;            // 2 * ceil(N / 64), 2 * ceil(Q / 64)
+};
+
+__global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
+    __shared__ uint32_t pairs[128][4], all_rows[128][4];  // the mask's bits, and with the padding's
+    __shared__ uint32_t cols[128][4];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int q_tiles = (a.rows + 127) / 128, k_tiles = (a.N + 127) / 128;
+    int x = blockIdx.x;
+    const int kt = x % k_tiles;
+    x /= k_tiles;
+    const int qt = x % q_tiles;
+    x /= q_tiles;
+    const int h = x % a.heads, b = x / a.heads;
+    grid_dependency_wait();
+    launch_dependents();
+    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
+    const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
+    uint32_t padded[4];
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const int j = kt * 128 + 32 * w + lane;
+        padded[w] = __ballot_sync(0xffffffffu, j < a.N && (pad == nullptr || pad[j] == 0));
+    }
+    for (int r = warp; r < 128; r += 8) {
+        const int i = qt * 128 + r;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const int j = kt * 128 + 32 * w + lane;
+            const bool open = i < a.rows && j < a.N && (mask == nullptr || mask[i * a.m_q + j] == 0);
+            const uint32_t word = __ballot_sync(0xffffffffu, open);
+            if (lane == w) {
+                pairs[r][w] = word;
+                all_rows[r][w] = word & padded[w];
+            }
+        }
+    }
+    __syncthreads();
+    const long long bh = (long long)b * a.heads + h;
+    for (int e = threadIdx.x; e < 128 * 4; e += 256) {
+        const int i = qt * 128 + e / 4, w = kt * 4 + e % 4;
+        if (i < a.rows && w < a.words) a.row_bits[(bh * a.rows + i) * a.words + w] = all_rows[e / 4][e % 4];
+    }
+    if (warp < 2) {  // flags of the block's two 128 x 64 tiles
+        const int t = kt * 2 + warp;
+        uint32_t any = 0, every = 0xffffffffu;
+        for (int r = lane; r < 128; r += 32) {
+            const uint32_t w0 = all_rows[r][2 * warp], w1 = all_rows[r][2 * warp + 1];
+            any |= w0 | w1;
+            if (qt * 128 + r < a.rows) every &= w0 & w1;
+        }
+        const bool some = __any_sync(0xffffffffu, any != 0), full = __all_sync(0xffffffffu, every == 0xffffffffu);
+        const int tiles = a.words / 2;
+        if (lane == 0 && t < tiles) a.row_flags[(bh * q_tiles + qt) * tiles + t] = uint8_t(some) | uint8_t(full) << 1;
+    }
+    if (a.col_bits == nullptr || b >= a.mask_images) return;
+    for (int e = threadIdx.x; e < 128 * 4; e += 256) {
+        const int key = e % 128, qw = e / 128;
+        uint32_t word = 0;
+#pragma unroll 8
+        for (int r = 0; r < 32; ++r) word |= ((pairs[32 * qw + r][key / 32] >> (key % 32)) & 1u) << r;
+        cols[key][qw] = word;
+        const int j = kt * 128 + key, w = qt * 4 + qw;
+        if (j < a.N && w < a.col_words) a.col_bits[(bh * a.N + j) * a.col_words + w] = word;
+    }
+    __syncthreads();
+    if (warp < 2) {  // flags of the block's two tiles of 128 keys x 64 queries
+        const int t = qt * 2 + warp;
+        uint32_t any = 0, every = 0xffffffffu;
+        const int left = a.rows - (qt * 128 + 64 * warp);  // queries of this tile
+        const unsigned long long range = left >= 64 ? ~0ull : left <= 0 ? 0ull : (1ull << left) - 1ull;
+        for (int k = lane; k < 128; k += 32) {
+            const uint32_t w0 = cols[k][2 * warp], w1 = cols[k][2 * warp + 1];
+            any |= w0 | w1;
+            if (kt * 128 + k < a.N) every &= (w0 | ~uint32_t(range)) & (w1 | ~uint32_t(range >> 32));
+        }
+        const bool some = __any_sync(0xffffffffu, any != 0), full = __all_sync(0xffffffffu, every == 0xffffffffu);
+        const int tiles = a.col_words / 2;
+        if (lane == 0 && t < tiles) a.col_flags[(bh * k_tiles + kt) * tiles + t] = uint8_t(some) | uint8_t(full) << 1;
+    }
+}
+
+// delta as in attn_delta_kernel for 16-bit types with D a multiple of 8: 16-byte loads, `lanes` (a power of two, at
+// least D / 8) threads a row. float16: the blocks also take max|dO| over all rows, and the blocks behind delta_blocks
+// max|V| over the keys that are there, into amax (zeroed before; a maximum has no order).
+template <typename T>
+__global__ void __launch_bounds__(256) attn_delta_tc_kernel(const AttnArgs a, int lanes, unsigned delta_blocks,
+                                                            unsigned int* amax) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    const int sub = threadIdx.x % lanes, per_block = 256 / lanes;
+    const long long row = (long long)(blockIdx.x < delta_blocks ? blockIdx.x : blockIdx.x - delta_blocks) * per_block +
+                          threadIdx.x / lanes;
+    grid_dependency_wait();
+    launch_dependents();
+    float top = 0.f;
+    if (blockIdx.x < delta_blocks) {
+        const int i = int(row % a.Qp);
+        const long long bh = row / a.Qp;
+        const bool in = bh < (long long)a.B * a.H;
+        float sum = 0.f;
+        if (in && i < a.Q && sub * 8 < a.D) {
+            const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D + sub * 8;
+            float o[8], g[8];
+            load16<T>(static_cast<const T*>(a.out_in) + at, o);
+            load16<T>(static_cast<const T*>(a.grad_out) + at, g);
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                sum += o[x] * g[x];
+                if constexpr (kHalf) top = fmaxf(top, fabsf(g[x]));
+            }
+        }
+        for (int x = lanes / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+        if (in && sub == 0) static_cast<float*>(a.delta)[row] = sum;
+    } else if constexpr (kHalf) {
+        const long long tokens = (long long)a.B * a.N;  // row = (b * Hk + hk) * N + j
+        if (row < tokens * a.Hk && sub * 8 < a.D) {
+            const long long j = row % a.N, bh = row / a.N, b = bh / a.Hk;
+            if (a.padding == nullptr || a.padding[b * a.N + j] == 0) {
+                float v[8];
+                load16<T>(static_cast<const T*>(a.v) + b * a.v_b + bh % a.Hk * a.v_h + j * a.v_t + sub * 8, v);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(v[x]));
+            }
+        }
+    }
+    if constexpr (kHalf) {
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+        __shared__ float tops[8];
+        if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int x = 1; x < 8; ++x) top = fmaxf(top, tops[x]);
+            if (top > 0.f) atomicMax(amax + (blockIdx.x < delta_blocks ? 0 : 1), __float_as_uint(top));
+        }
+    }
+}
+
+}  // namespace td

@@ -62,7 +62,8 @@ int allow_smem(K kernel, size_t bytes, char* err, size_t err_len) {
 
 }  // namespace host
 
-// The device error words of the other translation units (each has its own copy of the word td_ptx.cuh declares).
-cudaError_t attention_device_error(int clear, unsigned int* code);
+// The device error word of td_attention_tc.cu (a translation unit has its own copy of the word td_ptx.cuh declares;
+// the kernels of the other units wait for nothing).
+cudaError_t attention_tc_device_error(int clear, unsigned int* code);
 
 }  // namespace td

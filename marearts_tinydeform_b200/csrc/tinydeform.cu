@@ -2052,7 +2052,7 @@ int td_device_error(int clear, unsigned int* code, char* err, size_t err_len) {
         e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
     }
     unsigned int w = 0;
-    if (e == cudaSuccess) e = attention_device_error(clear, &w);
+    if (e == cudaSuccess) e = attention_tc_device_error(clear, &w);
     if (e != cudaSuccess) return fail(err, err_len, TD_ERR_CUDA, "device error word: %s", cudaGetErrorString(e));
     if (v == 0) v = w;
     if (code != nullptr) *code = v;
