@@ -355,11 +355,13 @@ TD_API int td_test_peer_wait(void* control, int world, int rank, long long limit
  *   i * mask_strides[2] + j (a stride of 0 shares the mask); key_padding_mask: NULL or [B, N], nonzero = no key there
  *   (its key and value rows are not used at all, whatever they hold); causal: query i uses keys j <= i + (N - Q).
  *   out [B, Q, H * D] (written; a query without any open key gets zeros).
+ *   rest: NULL, or [B, Q, H * D] (16-bit types; otherwise ignored), written: what rounding took from out, which keeps
+ *   the backward's small differences exact.
  *   lse: NULL, or [B, H, Qp] with Qp = Q rounded up to 128, float32 (float64 for TD_F64), written: the base-2
  *   logarithm of each row's sum of exponentials, +infinity for rows without an open key and behind the last query.
  *   scale > 0. workspace: td_attention_workspace_bytes(..., backward = 0) bytes, 16-byte aligned (NULL when 0).
  *
- * td_attention_backward: from the forward's inputs, its out and lse, and grad_out [B, Q, H * D], writes grad_query
+ * td_attention_backward: from the forward's inputs, its out, rest (or NULL) and lse, and grad_out [B, Q, H * D], writes grad_query
  * [B, Q, H, D], grad_key and grad_value [B, N, Hk, D] (dense). The probabilities are formed again from lse; sums over
  * queries, keys and the heads of a group are taken in a fixed order (no atomics). workspace: as above with
  * backward = 1. mask_b, mask_h: 1, or the mask's own batch and head counts (0 without an attn_mask).
@@ -369,13 +371,13 @@ TD_API size_t td_attention_workspace_bytes(int dtype, int64_t B, int64_t Q, int6
                                            int64_t D, int64_t mask_b, int64_t mask_h, int has_padding, int backward);
 TD_API int td_attention_forward(int dtype, const void* query, const void* key, const void* value,
                                 const int64_t* strides, const uint8_t* attn_mask, const int64_t* mask_strides,
-                                const uint8_t* key_padding_mask, void* out, void* lse, int64_t B, int64_t Q,
-                                int64_t N, int64_t H, int64_t Hk, int64_t D, double scale, int causal,
+                                const uint8_t* key_padding_mask, void* out, void* rest, void* lse, int64_t B,
+                                int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, double scale, int causal,
                                 void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
 TD_API int td_attention_backward(int dtype, const void* query, const void* key, const void* value,
                                  const int64_t* strides, const uint8_t* attn_mask, const int64_t* mask_strides,
-                                 const uint8_t* key_padding_mask, const void* out, const void* lse,
-                                 const void* grad_out, void* grad_query, void* grad_key, void* grad_value, int64_t B,
+                                 const uint8_t* key_padding_mask, const void* out, const void* rest,
+                                 const void* lse, const void* grad_out, void* grad_query, void* grad_key, void* grad_value, int64_t B,
                                  int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, double scale, int causal,
                                  void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
 

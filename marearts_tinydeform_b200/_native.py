@@ -27,10 +27,10 @@ INT32_MAX = 2 ** 31 - 1
 _i64, _vp, _ip, _sz, _cp = ctypes.c_int64, ctypes.c_void_p, ctypes.c_int, ctypes.c_size_t, ctypes.c_char_p
 SIGNATURES = {
     'td_attention_workspace_bytes': (_sz, [_ip, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _ip, _ip]),
-    'td_attention_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64,
-                                   _i64, ctypes.c_double, _ip, _vp, _sz, _vp, _cp, _sz]),
-    'td_attention_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64,
-                                    _i64, _i64, _i64, _i64, ctypes.c_double, _ip, _vp, _sz, _vp, _cp, _sz]),
+    'td_attention_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
+                                   _i64, _i64, ctypes.c_double, _ip, _vp, _sz, _vp, _cp, _sz]),
+    'td_attention_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64,
+                                    _i64, _i64, _i64, _i64, _i64, ctypes.c_double, _ip, _vp, _sz, _vp, _cp, _sz]),
     'td_layer_norm_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, ctypes.c_double, _vp, _cp,
                                     _sz]),
     'td_layer_norm_workspace_bytes': (_sz, [_ip, _i64, _i64]),
@@ -802,8 +802,9 @@ def _attention_mask(attn_mask):
     return m, (_i64 * 3)(m.stride(0) if nb > 1 else 0, m.stride(1) if nh > 1 else 0, m.stride(2)), nb, nh
 
 
-def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale, want_lse=False):
-    """(out [B, Q, H * D], lse or None) through td_attention_forward, for arguments check_attention has passed."""
+def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale, for_backward=False):
+    """(out [B, Q, H * D], rest, lse) through td_attention_forward, for arguments check_attention has passed; rest (16-bit
+    types) and lse are None unless for_backward."""
     lib = load()
     if not query.is_cuda:
         raise RuntimeError('inputs must be CUDA tensors')
@@ -816,23 +817,25 @@ def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, sc
     pad = None if key_padding_mask is None else key_padding_mask.contiguous()
     dev = query.device
     out = torch.empty((B, Q, H * D), dtype=query.dtype, device=dev)
-    lse = None
-    if want_lse:
+    rest = lse = None
+    if for_backward:
+        if query.dtype in (torch.float16, torch.bfloat16):
+            rest = torch.empty_like(out)
         acc = torch.float64 if query.dtype == torch.float64 else torch.float32
         lse = torch.empty((B, H, -(-Q // ATTN_ROW_PAD) * ATTN_ROW_PAD), dtype=acc, device=dev)
     if B * Q == 0:
-        return out, lse
+        return out, rest, lse
     code = DTYPE_CODE[query.dtype]
     ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, int(pad is not None), 0)
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with torch.cuda.device(dev):
         _call(lib.td_attention_forward, code, _ptr(q), _ptr(k), _ptr(v), (_i64 * 9)(*qs, *ks, *vs), _ptr(m), ms,
-              _ptr(pad), _ptr(out), _ptr(lse), B, Q, N, H, Hk, D, scale, int(causal), _ptr(ws), ws_bytes,
+              _ptr(pad), _ptr(out), _ptr(rest), _ptr(lse), B, Q, N, H, Hk, D, scale, int(causal), _ptr(ws), ws_bytes,
               _stream(dev))
-    return out, lse
+    return out, rest, lse
 
 
-def attention_backward(query, key, value, key_padding_mask, attn_mask, causal, scale, out, lse, grad_out):
+def attention_backward(query, key, value, key_padding_mask, attn_mask, causal, scale, out, rest, lse, grad_out):
     """(grad_query, grad_key, grad_value) through td_attention_backward."""
     lib = load()
     B, Q, H, D = query.shape
@@ -852,8 +855,8 @@ def attention_backward(query, key, value, key_padding_mask, attn_mask, causal, s
     ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     with torch.cuda.device(dev):
         _call(lib.td_attention_backward, code, _ptr(q), _ptr(k), _ptr(v), (_i64 * 9)(*qs, *ks, *vs), _ptr(m), ms,
-              _ptr(pad), _ptr(out), _ptr(lse), _ptr(g), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v), B, Q, N, H, Hk, D,
-              scale, int(causal), _ptr(ws), ws_bytes, _stream(dev))
+              _ptr(pad), _ptr(out), _ptr(rest), _ptr(lse), _ptr(g), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v), B, Q, N,
+              H, Hk, D, scale, int(causal), _ptr(ws), ws_bytes, _stream(dev))
     return grad_q, grad_k, grad_v
 
 

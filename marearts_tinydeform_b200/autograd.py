@@ -150,24 +150,24 @@ def producer_train(query, reference_points, spatial_shapes, heads, points, sampl
 
 class AttentionFunction(torch.autograd.Function):
     """Softmax attention on CUDA, differentiable in query, key and value: td_attention_forward, which also writes each
-    row's log-sum, and td_attention_backward, which forms the probabilities again from it."""
+    row's log-sum (and, for 16-bit types, what the result's rounding took), and td_attention_backward, which forms the probabilities again from it."""
 
     @staticmethod
     def forward(ctx, query, key, value, key_padding_mask, attn_mask, causal, scale):
-        out, lse = _native.attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale,
-                                             want_lse=True)
-        ctx.save_for_backward(query, key, value, key_padding_mask, attn_mask, out, lse)
+        out, rest, lse = _native.attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale,
+                                                   for_backward=True)
+        ctx.save_for_backward(query, key, value, key_padding_mask, attn_mask, out, rest, lse)
         ctx.causal, ctx.scale = causal, scale
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out):
-        query, key, value, key_padding_mask, attn_mask, out, lse = ctx.saved_tensors
+        query, key, value, key_padding_mask, attn_mask, out, rest, lse = ctx.saved_tensors
         need = ctx.needs_input_grad
         g = grad_out if grad_out.dtype == query.dtype else grad_out.to(query.dtype)
         grads = _native.attention_backward(query, key, value, key_padding_mask, attn_mask, ctx.causal, ctx.scale, out,
-                                           lse, g)
+                                           rest, lse, g)
         return tuple(x if n else None for x, n in zip(grads, need)) + (None, None, None, None)
 
 

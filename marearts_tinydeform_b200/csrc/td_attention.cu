@@ -154,7 +154,7 @@ size_t td_attention_workspace_bytes(int dtype, int64_t B, int64_t Q, int64_t N, 
 
 int td_attention_forward(int dtype, const void* query, const void* key, const void* value, const int64_t* strides,
                          const uint8_t* attn_mask, const int64_t* mask_strides, const uint8_t* key_padding_mask,
-                         void* out, void* lse, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D,
+                         void* out, void* rest, void* lse, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D,
                          double scale, int causal, void* workspace, size_t workspace_bytes, void* stream, char* err,
                          size_t err_len) {
     using namespace td;
@@ -170,6 +170,7 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
     AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
     a.out = out;
+    a.rest = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
     a.lse = lse;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (N > 0 && attn_tc_fits(dtype, a))
@@ -184,7 +185,7 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
 
 int td_attention_backward(int dtype, const void* query, const void* key, const void* value, const int64_t* strides,
                           const uint8_t* attn_mask, const int64_t* mask_strides, const uint8_t* key_padding_mask,
-                          const void* out, const void* lse, const void* grad_out, void* grad_query, void* grad_key,
+                          const void* out, const void* rest, const void* lse, const void* grad_out, void* grad_query, void* grad_key,
                           void* grad_value, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D,
                           double scale, int causal, void* workspace, size_t workspace_bytes, void* stream, char* err,
                           size_t err_len) {
@@ -211,6 +212,7 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
     AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
     a.out_in = out;
+    a.rest_in = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
     a.lse = const_cast<void*>(lse);
     a.grad_out = grad_out;
     a.grad_q = grad_query;

@@ -11,6 +11,11 @@
 // zero. With fewer key heads than query heads, query head h reads key head h / (H / Hk), and dk, dv are summed over
 // the query heads of their group inside the kernel.
 //
+// delta is the one sum of the backward whose terms cancel: dP_ij - delta_i is small against either where a row has
+// few keys of weight, and a delta from the rounded result (and, on tensor cores, from rounded P) is off by as much as
+// the rounding of dS itself. A forward that a backward follows therefore keeps, for 16-bit types, what the rounding
+// took from each result as a second 16-bit tensor, and delta is formed from both.
+//
 // Logarithms are base 2 in the kernels: c = scale * log2(e), lse = L * log2(e).
 //
 // CUDA-core kernels: 256 threads, a 16 x 16 grid of R x R register tiles. The tile of S (16 R x 16 R) is formed from
@@ -33,7 +38,9 @@ constexpr int kAttnRowPad = 128;  // lse and delta rows hold Q rounded up to thi
 struct AttnArgs {
     const void *q, *k, *v;
     const void *out_in, *grad_out;  // backward: the forward's result and its gradient, [B, Q, H * D]
+    const void* rest_in;            // backward, 16-bit types: what rounding took from the result, or null
     void* out;                      // forward: [B, Q, H * D]
+    void* rest;                     // forward, 16-bit types: written unless null
     void *grad_q, *grad_k, *grad_v; // backward: [B, Q, H, D], [B, N, Hk, D] twice
     void* lse;                      // [B, H, Qp] in the accumulator type; forward: written unless null
     void* delta;                    // backward workspace, [B, H, Qp]
@@ -235,7 +242,11 @@ __global__ void __launch_bounds__(256) attn_simt_forward_kernel(const AttnArgs a
 #pragma unroll
         for (int x = 0; x < Tile::kCols; ++x) {
             const int d = tx + 16 * x;
-            if (d < a.D) out[(((long long)b * a.Q + i) * a.H + h) * a.D + d] = from_acc<T>(o[r][x] * inv);
+            if (d >= a.D) continue;
+            const long long at = (((long long)b * a.Q + i) * a.H + h) * a.D + d;
+            const T rounded = from_acc<T>(o[r][x] * inv);
+            out[at] = rounded;
+            if (a.rest != nullptr) static_cast<T*>(a.rest)[at] = from_acc<T>(o[r][x] * inv - to_acc(rounded));
         }
     }
     // rows of lse that no tile covers
@@ -259,7 +270,9 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
         const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D;
         const T* o = static_cast<const T*>(a.out_in) + at;
         const T* g = static_cast<const T*>(a.grad_out) + at;
-        for (int d = 0; d < a.D; ++d) sum += to_acc(o[d]) * to_acc(g[d]);
+        const T* rest = static_cast<const T*>(a.rest_in);
+        for (int d = 0; d < a.D; ++d)
+            sum += (rest == nullptr ? to_acc(o[d]) : to_acc(o[d]) + to_acc(rest[at + d])) * to_acc(g[d]);
     }
     static_cast<A*>(a.delta)[row] = sum;
 }

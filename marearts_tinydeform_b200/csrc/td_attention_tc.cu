@@ -98,7 +98,7 @@ int pack_masks(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, bo
                         stream, true, p);
 }
 
-template <typename T, int DP>
+template <typename T, int DP, bool EXACT>
 int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsigned char* workspace,
             cudaStream_t stream, char* err, size_t err_len) {
     const AttnArgs& a = t.a;
@@ -107,7 +107,7 @@ int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsig
     if (int rc = make_map(&k, key_of(a), kAttnBN, a, err, err_len)) return rc;
     if (int rc = make_map(&v, value_of(a), kAttnBN, a, err, err_len)) return rc;
     if (int rc = pack_masks(t, w, mb, mh, false, workspace, stream, err, err_len)) return rc;
-    auto kernel = attn_tc_forward_kernel<T, DP>;
+    auto kernel = attn_tc_forward_kernel<T, DP, EXACT>;
     constexpr size_t smem = AttnFwdLayout<DP>::kSmemBytes;
     if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
     const unsigned grid = unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
@@ -161,20 +161,25 @@ bool attn_tc_fits(int dtype, const AttnArgs& a) {
     if (a.D % 8 != 0 || a.N <= 32) return false;
     if (!operand_fits(query_of(a), a) || !operand_fits(key_of(a), a) || !operand_fits(value_of(a), a)) return false;
     if (!aligned16(a.lse)) return false;
-    if (a.grad_q == nullptr) return aligned16(a.out);
-    return operand_fits(grad_of(a), a) && aligned16(a.out_in) && aligned16(a.grad_q) && aligned16(a.grad_k) &&
-           aligned16(a.grad_v);
+    if (a.grad_q == nullptr) return aligned16(a.out) && aligned16(a.rest);
+    return operand_fits(grad_of(a), a) && aligned16(a.out_in) && a.rest_in != nullptr && aligned16(a.rest_in) &&
+           aligned16(a.grad_q) && aligned16(a.grad_k) && aligned16(a.grad_v);
 }
 
 int attn_tc_forward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_t mb, int64_t mh,
                     unsigned char* workspace, cudaStream_t stream, char* err, size_t err_len) {
     AttnTcArgs t = {};
     t.a = a;
-    if (dtype == TD_F16)
-        return a.D <= 64 ? forward<__half, 64>(t, w, mb, mh, workspace, stream, err, err_len)
-                         : forward<__half, 128>(t, w, mb, mh, workspace, stream, err, err_len);
-    return a.D <= 64 ? forward<__nv_bfloat16, 64>(t, w, mb, mh, workspace, stream, err, err_len)
-                     : forward<__nv_bfloat16, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+    auto go = [&](auto type, auto exact) {
+        using T = decltype(type);
+        constexpr bool E = decltype(exact)::value;
+        return a.D <= 64 ? forward<T, 64, E>(t, w, mb, mh, workspace, stream, err, err_len)
+                         : forward<T, 128, E>(t, w, mb, mh, workspace, stream, err, err_len);
+    };
+    auto pick = [&](auto type) {
+        return a.rest != nullptr ? go(type, std::true_type{}) : go(type, std::false_type{});
+    };
+    return dtype == TD_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
 }
 
 int attn_tc_backward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_t mb, int64_t mh,

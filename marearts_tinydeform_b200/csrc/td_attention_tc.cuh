@@ -116,6 +116,14 @@ template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, f
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t v);
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&v));
+}
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
+    return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
 // All lanes of a warp wait; false in every lane if any gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsigned int code) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, code));
@@ -220,7 +228,10 @@ struct AttnFwdLayout {
 
 constexpr int kAttnFwdThreads = 256;  // producer, MMA, clearing, -, four softmax warps
 
-template <typename T, int DP>
+// EXACT, for a forward that a backward follows: P is kept as two 16-bit parts, its rounding and what that took, which
+// both go through the product (one product more a tile), and the result's rounding is kept as well: see delta in
+// td_attention.cuh. Otherwise P is rounded once.
+template <typename T, int DP, bool EXACT>
 __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     attn_tc_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const AttnTcArgs args) {
@@ -315,6 +326,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             tc_fence_after();
             if (lane == 0) {
                 issue_product<T, DP>(tmem + 128, tmem + 64 * (m & 1), smem_addr(v_tile(s)), m == 0);
+                if constexpr (EXACT)
+                    issue_product<T, DP>(tmem + 128, tmem + 64 * (m & 1) + 32, smem_addr(v_tile(s)), false);
                 mma_commit(&empty[s]);
                 mma_commit(&done[m & 1]);
             }
@@ -421,8 +434,16 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 const float p1 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16) + 1]), c, shift));
                 sum += p0 + p1;
                 p[x] = pack2<T>(p0, p1);
+                if constexpr (EXACT) {  // v's two registers of this pair are free: they take the rest
+                    const float2 r = unpack2<T>(p[x]);
+                    v[x / 16][x % 16] = pack2<T>(p0 - r.x, p1 - r.y);
+                }
             }
             tmem_st_32x32b_x32(sc, p);
+            if constexpr (EXACT) {
+                tmem_st_32x32b_x16(sc + 32, v[0]);
+                tmem_st_32x32b_x16(sc + 48, v[1]);
+            }
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(&pfull[n & 1]);
@@ -433,7 +454,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         tc_fence_after();
         if (got) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            T* out = static_cast<T*>(a.out) + (((long long)b * a.Q + i) * a.H + h) * a.D;
+            const long long at = (((long long)b * a.Q + i) * a.H + h) * a.D;
 #pragma unroll 1
             for (int d = 0; d < DP && d < a.D; d += 32) {
                 uint32_t o[32];
@@ -449,13 +470,20 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     if (d + 8 * g >= a.D) break;  // D is a multiple of 8
-                    uint4 q;
-                    uint32_t* qw = &q.x;
+                    uint32_t q[4], rest[4];
 #pragma unroll
-                    for (int x = 0; x < 4; ++x)
-                        qw[x] = pack2<T>(__uint_as_float(o[8 * g + 2 * x]) * inv,
-                                         __uint_as_float(o[8 * g + 2 * x + 1]) * inv);
-                    *reinterpret_cast<uint4*>(out + d + 8 * g) = q;
+                    for (int x = 0; x < 4; ++x) {
+                        const float o0 = __uint_as_float(o[8 * g + 2 * x]) * inv;
+                        const float o1 = __uint_as_float(o[8 * g + 2 * x + 1]) * inv;
+                        q[x] = pack2<T>(o0, o1);
+                        const float2 r = unpack2<T>(q[x]);
+                        rest[x] = pack2<T>(o0 - r.x, o1 - r.y);
+                    }
+                    *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + d + 8 * g) =
+                        make_uint4(q[0], q[1], q[2], q[3]);
+                    if constexpr (EXACT)
+                        *reinterpret_cast<uint4*>(static_cast<T*>(a.rest) + at + d + 8 * g) =
+                            make_uint4(rest[0], rest[1], rest[2], rest[3]);
                 }
             }
             if (a.lse != nullptr)  // Qp is a multiple of the tile
@@ -919,12 +947,13 @@ __global__ void __launch_bounds__(256) attn_delta_tc_kernel(const AttnArgs a, in
         float sum = 0.f;
         if (in && i < a.Q && sub * 8 < a.D) {
             const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D + sub * 8;
-            float o[8], g[8];
+            float o[8], g[8], r[8];
             load16<T>(static_cast<const T*>(a.out_in) + at, o);
             load16<T>(static_cast<const T*>(a.grad_out) + at, g);
+            load16<T>(static_cast<const T*>(a.rest_in) + at, r);
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                sum += o[x] * g[x];
+                sum += (o[x] + r[x]) * g[x];
                 if constexpr (kHalf) top = fmaxf(top, fabsf(g[x]));
             }
         }
