@@ -389,7 +389,7 @@ TD_API int td_attention_backward(int dtype, const void* query, const void* key, 
  *
  * td_layer_norm_backward: grad_x [rows, C] (the gradient of x and of residual alike), grad_weight and grad_bias [C]
  * (either may be NULL), the column sums in a fixed order (no atomics). workspace:
- * td_layer_norm_workspace_bytes(dtype, rows, C) bytes on the current device, 8-byte aligned.
+ * td_layer_norm_workspace_bytes(dtype, rows, C) bytes, 8-byte aligned.
  */
 TD_API int td_layer_norm_forward(int dtype, const void* x, const void* residual, const void* weight,
                                  const void* bias, void* y, void* mean, void* rstd, int64_t rows, int64_t C,

@@ -789,6 +789,7 @@ def _attention_operand(t):
 
 
 _no_strides = (_i64 * 3)()
+_strides9, _strides3 = _i64 * 9, _i64 * 3
 
 
 def _attention_mask(attn_mask):
@@ -797,9 +798,29 @@ def _attention_mask(attn_mask):
         return None, _no_strides, 0, 0
     m = attn_mask if attn_mask.stride(-1) == 1 or attn_mask.shape[-1] == 1 else attn_mask.contiguous()
     if m.dim() == 2:
-        return m, (_i64 * 3)(0, 0, m.stride(0)), 1, 1
+        return m, _strides3(0, 0, m.stride(0)), 1, 1
     nb, nh = m.shape[:2]
-    return m, (_i64 * 3)(m.stride(0) if nb > 1 else 0, m.stride(1) if nh > 1 else 0, m.stride(2)), nb, nh
+    return m, _strides3(m.stride(0) if nb > 1 else 0, m.stride(1) if nh > 1 else 0, m.stride(2)), nb, nh
+
+
+# A decoder's calls are short next to what binding them costs on the host, so the calls below pass plain addresses,
+# take the stream as a number and enter the tensors' device only where it is not the current one.
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _launch(fn, device, *args):
+    """fn(*args, stream, err, err_len) on the device's current stream; raises its error."""
+    index = device.index
+    err = ctypes.create_string_buffer(512)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, stream, err, 512)
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, stream, err, 512)
+    if rc != 0:
+        raise RuntimeError(f'{fn.__name__} failed ({rc}): {err.value.decode(errors="replace")}')
 
 
 def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale, for_backward=False):
@@ -815,23 +836,22 @@ def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, sc
     v, vs = _attention_operand(value)
     m, ms, mb, mh = _attention_mask(attn_mask)
     pad = None if key_padding_mask is None else key_padding_mask.contiguous()
-    dev = query.device
-    out = torch.empty((B, Q, H * D), dtype=query.dtype, device=dev)
-    rest = lse = None
+    code = DTYPE_CODE[query.dtype]
+    out = query.new_empty((B, Q, H * D))
+    rest = lse = ws = None
     if for_backward:
-        if query.dtype in (torch.float16, torch.bfloat16):
-            rest = torch.empty_like(out)
-        acc = torch.float64 if query.dtype == torch.float64 else torch.float32
-        lse = torch.empty((B, H, -(-Q // ATTN_ROW_PAD) * ATTN_ROW_PAD), dtype=acc, device=dev)
+        if code == TD_F16 or code == TD_BF16:
+            rest = query.new_empty((B, Q, H * D))
+        acc = torch.float64 if code == TD_F64 else torch.float32
+        lse = query.new_empty((B, H, -(-Q // ATTN_ROW_PAD) * ATTN_ROW_PAD), dtype=acc)
     if B * Q == 0:
         return out, rest, lse
-    code = DTYPE_CODE[query.dtype]
-    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, int(pad is not None), 0)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with torch.cuda.device(dev):
-        _call(lib.td_attention_forward, code, _ptr(q), _ptr(k), _ptr(v), (_i64 * 9)(*qs, *ks, *vs), _ptr(m), ms,
-              _ptr(pad), _ptr(out), _ptr(rest), _ptr(lse), B, Q, N, H, Hk, D, scale, int(causal), _ptr(ws), ws_bytes,
-              _stream(dev))
+    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, pad is not None, 0)
+    if ws_bytes:
+        ws = query.new_empty((ws_bytes,), dtype=torch.uint8)
+    _launch(lib.td_attention_forward, query.device, code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _strides9(*qs, *ks, *vs), _address(m), ms, _address(pad), out.data_ptr(), _address(rest), _address(lse),
+            B, Q, N, H, Hk, D, scale, causal, _address(ws), ws_bytes)
     return out, rest, lse
 
 
@@ -846,17 +866,16 @@ def attention_backward(query, key, value, key_padding_mask, attn_mask, causal, s
     m, ms, mb, mh = _attention_mask(attn_mask)
     pad = None if key_padding_mask is None else key_padding_mask.contiguous()
     g = grad_out.contiguous()
-    dev = query.device
-    grad_q = torch.empty((B, Q, H, D), dtype=q.dtype, device=dev)
-    grad_k = torch.empty((B, N, Hk, D), dtype=q.dtype, device=dev)
-    grad_v = torch.empty((B, N, Hk, D), dtype=q.dtype, device=dev)
+    grad_q = q.new_empty((B, Q, H, D))
+    grad_k = q.new_empty((B, N, Hk, D))
+    grad_v = q.new_empty((B, N, Hk, D))
     code = DTYPE_CODE[q.dtype]
-    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, int(pad is not None), 1)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-    with torch.cuda.device(dev):
-        _call(lib.td_attention_backward, code, _ptr(q), _ptr(k), _ptr(v), (_i64 * 9)(*qs, *ks, *vs), _ptr(m), ms,
-              _ptr(pad), _ptr(out), _ptr(rest), _ptr(lse), _ptr(g), _ptr(grad_q), _ptr(grad_k), _ptr(grad_v), B, Q, N,
-              H, Hk, D, scale, int(causal), _ptr(ws), ws_bytes, _stream(dev))
+    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, pad is not None, 1)
+    ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    _launch(lib.td_attention_backward, query.device, code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+            _strides9(*qs, *ks, *vs), _address(m), ms, _address(pad), out.data_ptr(), _address(rest), lse.data_ptr(),
+            g.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(), B, Q, N, H, Hk, D, scale, causal,
+            _address(ws), ws_bytes)
     return grad_q, grad_k, grad_v
 
 
@@ -881,8 +900,8 @@ def check_layer_norm(x, weight, bias, residual, eps):
 
 
 def layer_norm_forward(x, weight, bias, residual, eps, want_stats=False):
-    """(y, mean, rstd) through td_layer_norm_forward (mean and rstd None unless want_stats), for arguments
-    check_layer_norm has passed."""
+    """(y, stats) through td_layer_norm_forward, for arguments check_layer_norm has passed; stats holds the rows' means,
+    then their reciprocal deviations, and is None unless want_stats."""
     lib = load()
     if not x.is_cuda:
         raise RuntimeError('inputs must be CUDA tensors')
@@ -890,18 +909,19 @@ def layer_norm_forward(x, weight, bias, residual, eps, want_stats=False):
     C = x.shape[-1]
     rows = xs.numel() // C
     y = torch.empty_like(xs)
-    mean = rstd = None
+    stats = mean = rstd = None
+    code = DTYPE_CODE[x.dtype]
     if want_stats:
-        acc = torch.float64 if x.dtype == torch.float64 else torch.float32
-        mean, rstd = torch.empty((2, rows), dtype=acc, device=x.device)
+        stats = xs.new_empty((2, rows), dtype=torch.float64 if code == TD_F64 else torch.float32)
+        mean = stats.data_ptr()
+        rstd = mean + rows * (8 if code == TD_F64 else 4)
     if rows:
-        with torch.cuda.device(x.device):
-            _call(lib.td_layer_norm_forward, DTYPE_CODE[x.dtype], _ptr(xs), _ptr(r), _ptr(w), _ptr(b), _ptr(y),
-                  _ptr(mean), _ptr(rstd), rows, C, eps, _stream(x.device))
-    return y, mean, rstd
+        _launch(lib.td_layer_norm_forward, x.device, code, xs.data_ptr(), _address(r), w.data_ptr(), _address(b),
+                y.data_ptr(), mean, rstd, rows, C, eps)
+    return y, stats
 
 
-def layer_norm_backward(grad_y, x, weight, residual, mean, rstd, want_weight=True, want_bias=True):
+def layer_norm_backward(grad_y, x, weight, residual, stats, want_weight=True, want_bias=True):
     """(grad_x, grad_weight or None, grad_bias or None) through td_layer_norm_backward."""
     lib = load()
     g, xs, w, r = _dense(grad_y, x, weight, residual)
@@ -909,11 +929,12 @@ def layer_norm_backward(grad_y, x, weight, residual, mean, rstd, want_weight=Tru
     rows = xs.numel() // C
     code = DTYPE_CODE[x.dtype]
     grad_x = torch.empty_like(xs)
-    grad_w = torch.empty((C,), dtype=x.dtype, device=x.device) if want_weight else None
-    grad_b = torch.empty((C,), dtype=x.dtype, device=x.device) if want_bias else None
-    with torch.cuda.device(x.device):
-        ws_bytes = lib.td_layer_norm_workspace_bytes(code, rows, C)
-        ws = torch.empty(max(ws_bytes, 1), dtype=torch.uint8, device=x.device)
-        _call(lib.td_layer_norm_backward, code, _ptr(g), _ptr(xs), _ptr(r), _ptr(w), _ptr(mean), _ptr(rstd),
-              _ptr(grad_x), _ptr(grad_w), _ptr(grad_b), rows, C, _ptr(ws), ws_bytes, _stream(x.device))
+    grad_w = w.new_empty((C,)) if want_weight else None
+    grad_b = w.new_empty((C,)) if want_bias else None
+    mean = stats.data_ptr()
+    ws_bytes = lib.td_layer_norm_workspace_bytes(code, rows, C)
+    ws = w.new_empty((max(ws_bytes, 1),), dtype=torch.uint8)
+    _launch(lib.td_layer_norm_backward, x.device, code, g.data_ptr(), xs.data_ptr(), _address(r), w.data_ptr(), mean,
+            mean + rows * (8 if code == TD_F64 else 4), grad_x.data_ptr(), _address(grad_w), _address(grad_b), rows, C,
+            ws.data_ptr(), ws_bytes)
     return grad_x, grad_w, grad_b

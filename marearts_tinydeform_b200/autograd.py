@@ -178,15 +178,15 @@ class LayerNormFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, residual, eps):
-        y, mean, rstd = _native.layer_norm_forward(x, weight, bias, residual, eps, want_stats=True)
-        ctx.save_for_backward(x, weight, residual, mean, rstd)
+        y, stats = _native.layer_norm_forward(x, weight, bias, residual, eps, want_stats=True)
+        ctx.save_for_backward(x, weight, residual, stats)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y):
-        x, weight, residual, mean, rstd = ctx.saved_tensors
+        x, weight, residual, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         g = grad_y if grad_y.dtype == x.dtype else grad_y.to(x.dtype)
-        grad_x, grad_w, grad_b = _native.layer_norm_backward(g, x, weight, residual, mean, rstd, need[1], need[2])
+        grad_x, grad_w, grad_b = _native.layer_norm_backward(g, x, weight, residual, stats, need[1], need[2])
         return (grad_x if need[0] else None, grad_w, grad_b, grad_x if need[3] else None, None)

@@ -1,4 +1,7 @@
 // td_attention.cu -- the attention entry points of the C ABI: argument contract, kernel choice and launches.
+#include <algorithm>
+#include <cstdlib>
+
 #include "td_attention_plan.h"
 
 namespace td {
@@ -10,21 +13,62 @@ using host::fail;
 int64_t pad_rows(int64_t Q) { return (Q + kAttnRowPad - 1) / kAttnRowPad * kAttnRowPad; }
 size_t elem_bytes(int dtype) { return dtype == TD_F64 ? 8 : dtype == TD_F32 ? 4 : 2; }
 
+// How a forward is split over the keys: splits CTAs of split_keys keys each (a multiple of `step`) for every one of
+// `blocks`, enough of them for `waves` CTAs an SM, but no split of fewer than `least` keys.
+void split_plan(int64_t blocks, int64_t N, int64_t waves, int64_t least, int64_t step, SplitArgs* p) {
+    int64_t splits = std::max<int64_t>(1, std::min((waves * kSms + blocks - 1) / blocks, N / least));
+    const int64_t keys = std::max((N + splits - 1) / splits, int64_t(1));  // one without any key, too
+    p->split_keys = int((keys + step - 1) / step * step);
+    p->splits = int(std::max<int64_t>(1, (N + p->split_keys - 1) / p->split_keys));
+}
+
+// The mma.sync split kernel's plan: the rows of a key head's group in tiles of 16.
+SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk) {
+    SplitArgs p = {};
+    p.row_tiles = int((H / Hk * Q + 15) / 16);
+    split_plan(B * Hk * p.row_tiles, N, 8, 256, 128, &p);
+    return p;
+}
+
+// The CUDA-core forward's register tile: 4 x 4, 2 x 2 for float64 (whose operand tiles take twice the bytes); one row
+// a thread for up to 16 queries, where most of a taller tile would be empty.
+template <typename T> constexpr int simt_r() { return std::is_same<T, double>::value ? 2 : 4; }
+
+// 16-bit calls of the usual widths come here only misaligned or short: they do without partials.
+SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t D) {
+    SplitArgs p = {};
+    const bool whole = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0;
+    const int rows = Q <= 16 ? 16 : 16 * (dtype == TD_F64 ? 2 : 4);
+    p.row_tiles = int((Q + rows - 1) / rows);
+    split_plan(B * H * p.row_tiles, N, 2, whole ? N + 1 : 128, 64, &p);
+    return p;
+}
+
 // The parts of a call's workspace. The mask's bits and flags are laid out for 16-bit types only (the tensor-core
-// kernels read them); a mask shared by images or heads is packed once.
-AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t mb, int64_t mh,
-                             bool padding, bool backward) {
+// kernels read them); a mask shared by images or heads is packed once. The partials of a split forward are sized for
+// whichever kernel takes the call.
+AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t mb,
+                             int64_t mh, bool padding, bool backward) {
     AttnWorkspace w = {};
     auto take = [&](size_t bytes) {
         const size_t at = w.total;
         w.total += (bytes + 255) / 256 * 256;
         return at;
     };
+    const size_t acc = dtype == TD_F64 ? 8 : 4;
+    const bool half = dtype == TD_F16 || dtype == TD_BF16;
     if (backward) {
         w.amax = take(2 * sizeof(unsigned int));
-        w.delta = take(size_t(B) * H * pad_rows(Q) * (dtype == TD_F64 ? 8 : 4));
+        w.delta = take(size_t(B) * H * pad_rows(Q) * acc);
+    } else {
+        int64_t splits = simt_split_plan(dtype, B, Q, N, H, D).splits;
+        if (half) splits = std::max<int64_t>(splits, mma_split_plan(B, Q, N, H, Hk).splits);
+        if (splits > 1) {
+            w.part_o = take(size_t(B) * H * Q * splits * D * acc);
+            w.part_ml = take(size_t(B) * H * Q * splits * 2 * acc);
+        }
     }
-    if ((dtype == TD_F16 || dtype == TD_BF16) && (mb > 0 || padding)) {
+    if (half && (mb > 0 || padding)) {
         w.images = padding ? B : mb;
         w.heads = mb > 0 ? mh : 1;
         w.rows = mb > 0 ? Q : 1;
@@ -94,26 +138,76 @@ int zero(void* p, size_t bytes, cudaStream_t stream, char* err, size_t err_len) 
     return fail(err, err_len, TD_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
 }
 
-// Register tile of the CUDA-core kernels: 4 x 4, 2 x 2 for float64 (whose operand tiles take twice the bytes).
-template <typename T> constexpr int simt_r() { return std::is_same<T, double>::value ? 2 : 4; }
+template <typename T>
+int combine(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
+    if (p.splits == 1) return TD_OK;
+    const long long rows = (long long)p.a.B * p.a.H * p.a.Q;
+    return host::launch(err, err_len, "attn_combine_kernel", attn_combine_kernel<T>, dim3(unsigned((rows + 3) / 4)),
+                        dim3(128), 0, stream, true, p);
+}
+
+template <typename T, int DP, int RM>
+int simt_forward_tile(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
+    constexpr int RN = simt_r<T>();
+    using Tile = SimtTile<typename Elem<T>::acc, DP, RM, RN>;
+    constexpr size_t smem = Tile::kRowBytes + 2 * Tile::kColBytes + Tile::kP;
+    auto kernel = attn_simt_forward_kernel<T, DP, RM, RN>;
+    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    const long long grid = (long long)p.splits * p.row_tiles * p.a.B * p.a.H;
+    if (int rc = host::launch(err, err_len, "attn_simt_forward_kernel", kernel, dim3(unsigned(grid)), dim3(256), smem,
+                              stream, true, p))
+        return rc;
+    return combine<T>(p, stream, err, err_len);
+}
 
 template <typename T, int DP>
-int simt_forward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
-    constexpr int R = simt_r<T>();
-    using Tile = SimtTile<typename Elem<T>::acc, DP, R>;
-    constexpr size_t smem = 3 * Tile::kOperand + Tile::kP;
-    auto kernel = attn_simt_forward_kernel<T, DP, R>;
-    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
-    const unsigned grid = unsigned((a.Q + Tile::kRows - 1) / Tile::kRows * a.B * a.H);
-    return host::launch(err, err_len, "attn_simt_forward_kernel", kernel, dim3(grid), dim3(256), smem, stream, true,
-                        a);
+int simt_forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned char* workspace, cudaStream_t stream,
+                 char* err, size_t err_len) {
+    SplitArgs p = simt_split_plan(dtype, a.B, a.Q, a.N, a.H, a.D);
+    p.a = a;
+    p.part_o = workspace + w.part_o;
+    p.part_ml = workspace + w.part_ml;
+    return a.Q <= 16 ? simt_forward_tile<T, DP, 1>(p, stream, err, err_len)
+                     : simt_forward_tile<T, DP, simt_r<T>()>(p, stream, err, err_len);
+}
+
+template <typename T, int DP, bool EXACT>
+int mma_split(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
+    const long long grid = (long long)p.splits * p.row_tiles * p.a.B * p.a.Hk;
+    if (int rc = host::launch(err, err_len, "attn_split_kernel", attn_split_kernel<T, DP, EXACT>,
+                              dim3(unsigned(grid)), dim3(kSplitWarps * 32), 0, stream, true, p))
+        return rc;
+    return combine<T>(p, stream, err, err_len);
+}
+
+template <typename T>
+int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* workspace, cudaStream_t stream,
+                      char* err, size_t err_len) {
+    SplitArgs p = mma_split_plan(a.B, a.Q, a.N, a.H, a.Hk);
+    p.a = a;
+    p.part_o = workspace + w.part_o;
+    p.part_ml = workspace + w.part_ml;
+    auto go = [&](auto exact) {
+        constexpr bool E = decltype(exact)::value;
+        if (a.D <= 32) return mma_split<T, 32, E>(p, stream, err, err_len);
+        if (a.D <= 64) return mma_split<T, 64, E>(p, stream, err, err_len);
+        return mma_split<T, 128, E>(p, stream, err, err_len);
+    };
+    return a.rest != nullptr ? go(std::true_type{}) : go(std::false_type{});
+}
+
+// Whether the split kernel takes a 16-bit forward that the tensor-core kernels could take as well.
+bool prefer_split(const AttnArgs& a) {
+    const char* e = getenv("ATTN_SPLIT");
+    if (e) return e[0] == '1';
+    return a.H / a.Hk * a.Q <= 16;
 }
 
 template <typename T, int DP>
 int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
     constexpr int R = simt_r<T>();
-    using Tile = SimtTile<typename Elem<T>::acc, DP, R>;
-    constexpr size_t smem = 4 * Tile::kOperand + Tile::kP;
+    using Tile = SimtTile<typename Elem<T>::acc, DP, R, R>;
+    constexpr size_t smem = 4 * Tile::kRowBytes + Tile::kP;
     auto kernel = attn_simt_backward_kernel<T, DP, R>;
     if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
     const long long rows = (long long)a.B * a.H * a.Qp;
@@ -127,10 +221,11 @@ int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_
 }
 
 template <typename T>
-int forward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
-    if (a.D <= 32) return simt_forward<T, 32>(a, stream, err, err_len);
-    if (a.D <= 64) return simt_forward<T, 64>(a, stream, err, err_len);
-    return simt_forward<T, 128>(a, stream, err, err_len);
+int forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned char* workspace, cudaStream_t stream,
+            char* err, size_t err_len) {
+    if (a.D <= 32) return simt_forward<T, 32>(a, dtype, w, workspace, stream, err, err_len);
+    if (a.D <= 64) return simt_forward<T, 64>(a, dtype, w, workspace, stream, err, err_len);
+    return simt_forward<T, 128>(a, dtype, w, workspace, stream, err, err_len);
 }
 
 template <typename T>
@@ -149,7 +244,7 @@ size_t td_attention_workspace_bytes(int dtype, int64_t B, int64_t Q, int64_t N, 
                                     int64_t mask_b, int64_t mask_h, int has_padding, int backward) {
     using namespace td;
     if (check_sizes(dtype, B, Q, N, H, Hk, D, 1.0, nullptr, 0) != TD_OK || B == 0 || Q == 0 || N == 0) return 0;
-    return attn_workspace(dtype, B, Q, N, H, mask_b, mask_h, has_padding != 0, backward != 0).total;
+    return attn_workspace(dtype, B, Q, N, H, Hk, D, mask_b, mask_h, has_padding != 0, backward != 0).total;
 }
 
 int td_attention_forward(int dtype, const void* query, const void* key, const void* value, const int64_t* strides,
@@ -165,7 +260,7 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
         return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
     const int64_t mb = attn_mask == nullptr ? 0 : mask_strides[0] != 0 ? B : 1;
     const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
-    const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, mb, mh, key_padding_mask != nullptr, false);
+    const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, Hk, D, mb, mh, key_padding_mask != nullptr, false);
     if (int rc = check_workspace(workspace, workspace_bytes, N > 0 ? ws.total : 0, err, err_len)) return rc;
     AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
@@ -173,13 +268,17 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
     a.rest = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
     a.lse = lse;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (N > 0 && attn_tc_fits(dtype, a))
-        return attn_tc_forward(dtype, a, ws, mb, mh, static_cast<unsigned char*>(workspace), s, err, err_len);
+    unsigned char* wp = static_cast<unsigned char*>(workspace);
+    if (N > 0 && attn_tc_fits(dtype, a)) {
+        if (!prefer_split(a)) return attn_tc_forward(dtype, a, ws, mb, mh, wp, s, err, err_len);
+        return dtype == TD_F16 ? mma_split_forward<__half>(a, ws, wp, s, err, err_len)
+                               : mma_split_forward<__nv_bfloat16>(a, ws, wp, s, err, err_len);
+    }
     switch (dtype) {
-        case TD_F32: return forward<float>(a, s, err, err_len);
-        case TD_F16: return forward<__half>(a, s, err, err_len);
-        case TD_BF16: return forward<__nv_bfloat16>(a, s, err, err_len);
-        default: return forward<double>(a, s, err, err_len);
+        case TD_F32: return forward<float>(a, dtype, ws, wp, s, err, err_len);
+        case TD_F16: return forward<__half>(a, dtype, ws, wp, s, err, err_len);
+        case TD_BF16: return forward<__nv_bfloat16>(a, dtype, ws, wp, s, err, err_len);
+        default: return forward<double>(a, dtype, ws, wp, s, err, err_len);
     }
 }
 
@@ -207,7 +306,7 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
         return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
     const int64_t mb = attn_mask == nullptr ? 0 : mask_strides[0] != 0 ? B : 1;
     const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
-    const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, mb, mh, key_padding_mask != nullptr, true);
+    const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, Hk, D, mb, mh, key_padding_mask != nullptr, true);
     if (int rc = check_workspace(workspace, workspace_bytes, ws.total, err, err_len)) return rc;
     AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);

@@ -18,7 +18,8 @@
 //
 // Logarithms are base 2 in the kernels: c = scale * log2(e), lse = L * log2(e).
 //
-// CUDA-core kernels: 256 threads, a 16 x 16 grid of R x R register tiles. The tile of S (16 R x 16 R) is formed from
+// CUDA-core kernels: 256 threads, a 16 x 16 grid of R x R register tiles (the forward takes 1 x R for few queries, and
+// is in td_attention_split.cuh). The tile of S (16 R x 16 R) is formed from
 // rows in shared memory, the online softmax's maximum and sum run in registers (16 lanes hold a row), and P goes
 // through shared memory for the product with the second operand, whose accumulator (16 R rows x DP columns) stays in
 // registers. Bound by the FMA units: an R x R tile needs 2 R vector loads for 4 R^2 FMAs (R = 4).
@@ -70,77 +71,78 @@ template <> __device__ __forceinline__ double attn_log2<double>(double x) { retu
 
 // ---- CUDA-core kernels --------------------------------------------------------------------------------------------
 
-template <typename A, int DP, int R>
+template <typename A, int DP, int RM, int RN>
 struct SimtTile {
     static constexpr int kVN = 16 / int(sizeof(A));  // accumulators of a 16-byte load
-    static constexpr int kRows = 16 * R;
+    static constexpr int kRows = 16 * RM, kCols = 16 * RN;  // of S
     static constexpr int kLd = DP + kVN;              // row pitch of an operand tile
-    static constexpr int kLdP = kRows + kVN;          // row pitch of the P tile
-    static constexpr int kCols = DP / 16;             // accumulator columns a thread
-    static constexpr size_t kOperand = size_t(kRows) * kLd * sizeof(A);
+    static constexpr int kLdP = kCols + kVN;          // row pitch of the P tile
+    static constexpr int kWidth = DP / 16;            // accumulator columns a thread
+    static constexpr size_t kRowBytes = size_t(kRows) * kLd * sizeof(A);  // an operand of S's rows
+    static constexpr size_t kColBytes = size_t(kCols) * kLd * sizeof(A);  // of its columns
     static constexpr size_t kP = size_t(kRows) * kLdP * sizeof(A);
 };
 
-// Rows t0 .. t0 + kRows of a [tokens, D] slice into shared memory, widened; rows at or past n, padded rows and
-// columns past D are zero.
-template <typename T, typename A, int DP, int R>
+// ROWS rows from t0 on of a [tokens, D] slice into shared memory, widened; rows at or past n, padded rows and columns
+// past D are zero.
+template <typename T, typename A, int DP, int ROWS>
 __device__ __forceinline__ void simt_load(A* dst, const T* src, long long stride, int t0, int n, int D,
                                           const uint8_t* pad) {
-    using Tile = SimtTile<A, DP, R>;
-    for (int i = threadIdx.x; i < Tile::kRows * DP; i += 256) {
+    constexpr int kLd = SimtTile<A, DP, 1, 1>::kLd;
+#pragma unroll 4
+    for (int i = threadIdx.x; i < ROWS * DP; i += 256) {
         const int r = i / DP, c = i % DP;
         A x = 0;
         if (t0 + r < n && c < D && (pad == nullptr || pad[t0 + r] == 0)) x = to_acc(src[(t0 + r) * stride + c]);
-        dst[r * Tile::kLd + c] = x;
+        dst[r * kLd + c] = x;
     }
 }
 
 // s[r][c] = row (ty + 16 r) of x . row (tx + 16 c) of y
-template <typename A, int DP, int R>
-__device__ __forceinline__ void simt_dot(const A* x, const A* y, int ty, int tx, A (&s)[R][R]) {
-    using Tile = SimtTile<A, DP, R>;
+template <typename A, int DP, int RM, int RN>
+__device__ __forceinline__ void simt_dot(const A* x, const A* y, int ty, int tx, A (&s)[RM][RN]) {
+    using Tile = SimtTile<A, DP, RM, RN>;
     constexpr int V = Tile::kVN;
     struct alignas(16) Vec { A e[V]; };
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int r = 0; r < RM; ++r)
 #pragma unroll
-        for (int c = 0; c < R; ++c) s[r][c] = 0;
+        for (int c = 0; c < RN; ++c) s[r][c] = 0;
 #pragma unroll 2
     for (int k = 0; k < DP; k += V) {
-        Vec xv[R], yv[R];
+        Vec xv[RM], yv[RN];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            xv[r] = *reinterpret_cast<const Vec*>(x + (ty + 16 * r) * Tile::kLd + k);
-            yv[r] = *reinterpret_cast<const Vec*>(y + (tx + 16 * r) * Tile::kLd + k);
-        }
+        for (int r = 0; r < RM; ++r) xv[r] = *reinterpret_cast<const Vec*>(x + (ty + 16 * r) * Tile::kLd + k);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+        for (int c = 0; c < RN; ++c) yv[c] = *reinterpret_cast<const Vec*>(y + (tx + 16 * c) * Tile::kLd + k);
 #pragma unroll
-            for (int c = 0; c < R; ++c)
+        for (int r = 0; r < RM; ++r)
+#pragma unroll
+            for (int c = 0; c < RN; ++c)
 #pragma unroll
                 for (int e = 0; e < V; ++e) s[r][c] += xv[r].e[e] * yv[c].e[e];
     }
 }
 
 // o[r][c] += sum_j p[ty + 16 r][j] * y[j][tx + 16 c]
-template <typename A, int DP, int R>
+template <typename A, int DP, int RM, int RN>
 __device__ __forceinline__ void simt_accumulate(const A* p, const A* y, int ty, int tx,
-                                                A (&o)[R][SimtTile<A, DP, R>::kCols]) {
-    using Tile = SimtTile<A, DP, R>;
+                                                A (&o)[RM][SimtTile<A, DP, RM, RN>::kWidth]) {
+    using Tile = SimtTile<A, DP, RM, RN>;
     constexpr int V = Tile::kVN;
     struct alignas(16) Vec { A e[V]; };
 #pragma unroll 2
-    for (int j = 0; j < Tile::kRows; j += V) {
-        Vec pv[R];
+    for (int j = 0; j < Tile::kCols; j += V) {
+        Vec pv[RM];
 #pragma unroll
-        for (int r = 0; r < R; ++r) pv[r] = *reinterpret_cast<const Vec*>(p + (ty + 16 * r) * Tile::kLdP + j);
+        for (int r = 0; r < RM; ++r) pv[r] = *reinterpret_cast<const Vec*>(p + (ty + 16 * r) * Tile::kLdP + j);
 #pragma unroll
         for (int e = 0; e < V; ++e)
 #pragma unroll
-            for (int c = 0; c < Tile::kCols; ++c) {
+            for (int c = 0; c < Tile::kWidth; ++c) {
                 const A b = y[(j + e) * Tile::kLd + tx + 16 * c];
 #pragma unroll
-                for (int r = 0; r < R; ++r) o[r][c] += pv[r].e[e] * b;
+                for (int r = 0; r < RM; ++r) o[r][c] += pv[r].e[e] * b;
             }
     }
 }
@@ -162,96 +164,6 @@ __device__ __forceinline__ int attn_key_end(const AttnArgs& a, int row_end) {
     if (!a.causal) return a.N;
     const int last = min(row_end, a.Q) + (a.N - a.Q);
     return max(0, min(a.N, last));
-}
-
-template <typename T, int DP, int R>
-__global__ void __launch_bounds__(256) attn_simt_forward_kernel(const AttnArgs a) {
-    using A = typename Elem<T>::acc;
-    using Tile = SimtTile<A, DP, R>;
-    constexpr int M = Tile::kRows;
-    extern __shared__ __align__(16) unsigned char smem_raw[];
-    A* qs = reinterpret_cast<A*>(smem_raw);
-    A* ks = qs + M * Tile::kLd;
-    A* vs = ks + M * Tile::kLd;
-    A* ps = vs + M * Tile::kLd;
-    const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-    const int tiles = (a.Q + M - 1) / M;
-    const int i0 = blockIdx.x % tiles * M, bh = blockIdx.x / tiles, h = bh % a.H, b = bh / a.H;
-    const int hk = h / (a.H / a.Hk);
-    const A ninf = -A(INFINITY), c = A(a.scale * 1.4426950408889634);
-    const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
-    const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
-    grid_dependency_wait();
-    launch_dependents();
-    simt_load<T, A, DP, R>(qs, static_cast<const T*>(a.q) + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
-    A m[R], l[R], o[R][Tile::kCols];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        m[r] = ninf;
-        l[r] = 0;
-#pragma unroll
-        for (int x = 0; x < Tile::kCols; ++x) o[r][x] = 0;
-    }
-    const int key_end = attn_key_end(a, i0 + M);
-    for (int j0 = 0; j0 < key_end; j0 += M) {
-        __syncthreads();  // the tiles of the turn before have been read
-        simt_load<T, A, DP, R>(ks, static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
-        simt_load<T, A, DP, R>(vs, static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
-        __syncthreads();
-        A s[R][R];
-        simt_dot<A, DP, R>(qs, ks, ty, tx, s);
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const int i = i0 + ty + 16 * r;
-            A top = m[r];
-#pragma unroll
-            for (int x = 0; x < R; ++x) {
-                const int j = j0 + tx + 16 * x;
-                const bool open = i < a.Q && j < a.N &&
-                                  attn_open(a, mask == nullptr ? nullptr : mask + i * a.m_q, pad, i, j);
-                s[r][x] = open ? s[r][x] * c : ninf;
-                top = cmax(top, s[r][x]);
-            }
-            top = row_max(top);
-            const A ref = top == ninf ? A(0) : top;  // no key so far: exp2(-inf - 0) = 0
-            const A keep = attn_exp2<A>(m[r] - ref);
-            A sum = 0;
-#pragma unroll
-            for (int x = 0; x < R; ++x) {
-                s[r][x] = attn_exp2<A>(s[r][x] - ref);
-                sum += s[r][x];
-                ps[(ty + 16 * r) * Tile::kLdP + tx + 16 * x] = s[r][x];
-            }
-            l[r] = l[r] * keep + row_sum(sum);
-            m[r] = top;
-#pragma unroll
-            for (int x = 0; x < Tile::kCols; ++x) o[r][x] *= keep;
-        }
-        __syncwarp();  // a row's P is written and read by the same half warp
-        simt_accumulate<A, DP, R>(ps, vs, ty, tx, o);
-    }
-    T* out = static_cast<T*>(a.out);
-    A* lse = static_cast<A*>(a.lse);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-        const int i = i0 + ty + 16 * r;
-        const A inv = l[r] == A(0) ? A(0) : A(1) / l[r];
-        if (lse != nullptr && tx == 0 && i < a.Qp)
-            lse[(long long)bh * a.Qp + i] = i < a.Q && l[r] != A(0) ? m[r] + attn_log2<A>(l[r]) : A(INFINITY);
-        if (i >= a.Q) continue;
-#pragma unroll
-        for (int x = 0; x < Tile::kCols; ++x) {
-            const int d = tx + 16 * x;
-            if (d >= a.D) continue;
-            const long long at = (((long long)b * a.Q + i) * a.H + h) * a.D + d;
-            const T rounded = from_acc<T>(o[r][x] * inv);
-            out[at] = rounded;
-            if (a.rest != nullptr) static_cast<T*>(a.rest)[at] = from_acc<T>(o[r][x] * inv - to_acc(rounded));
-        }
-    }
-    // rows of lse that no tile covers
-    if (lse != nullptr && i0 + M >= a.Q)
-        for (int i = i0 + M + int(threadIdx.x); i < a.Qp; i += 256) lse[(long long)bh * a.Qp + i] = A(INFINITY);
 }
 
 // delta[b, h, i] = grad_out . out over a query's head; zero in the rows behind the last query. A thread per row, adding
@@ -282,7 +194,7 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs a, int kv_blocks) {
     using A = typename Elem<T>::acc;
-    using Tile = SimtTile<A, DP, R>;
+    using Tile = SimtTile<A, DP, R, R>;
     constexpr int M = Tile::kRows;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     A* qs = reinterpret_cast<A*>(smem_raw);
@@ -305,13 +217,13 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
         const int tiles = (a.N + M - 1) / M;
         const int j0 = blockIdx.x % tiles * M, hk = blockIdx.x / tiles % a.Hk, b = blockIdx.x / tiles / a.Hk;
         const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
-        simt_load<T, A, DP, R>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
-        simt_load<T, A, DP, R>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
-        A dk[R][Tile::kCols], dv[R][Tile::kCols];
+        simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        A dk[R][Tile::kWidth], dv[R][Tile::kWidth];
 #pragma unroll
         for (int r = 0; r < R; ++r)
 #pragma unroll
-            for (int x = 0; x < Tile::kCols; ++x) dk[r][x] = dv[r][x] = 0;
+            for (int x = 0; x < Tile::kWidth; ++x) dk[r][x] = dv[r][x] = 0;
         // the first query that may use key j0
         const int first = a.causal ? max(0, min(a.Q, j0 - (a.N - a.Q))) / M * M : 0;
         for (int h = hk * group; h < (hk + 1) * group; ++h) {
@@ -320,12 +232,12 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
             const A* delta_h = delta + ((long long)b * a.H + h) * a.Qp;
             for (int i0 = first; i0 < a.Q; i0 += M) {
                 __syncthreads();
-                simt_load<T, A, DP, R>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
-                simt_load<T, A, DP, R>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q,
+                simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+                simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q,
                                        a.D, nullptr);
                 __syncthreads();
                 A s[R][R], p[R][R];
-                simt_dot<A, DP, R>(ks, qs, ty, tx, s);
+                simt_dot<A, DP, R, R>(ks, qs, ty, tx, s);
 #pragma unroll
                 for (int x = 0; x < R; ++x) {
                     const int i = i0 + tx + 16 * x;
@@ -340,8 +252,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
                     }
                 }
                 __syncwarp();
-                simt_accumulate<A, DP, R>(ps, gs, ty, tx, dv);
-                simt_dot<A, DP, R>(vs, gs, ty, tx, s);
+                simt_accumulate<A, DP, R, R>(ps, gs, ty, tx, dv);
+                simt_dot<A, DP, R, R>(vs, gs, ty, tx, s);
                 __syncwarp();
 #pragma unroll
                 for (int x = 0; x < R; ++x) {
@@ -353,7 +265,7 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
                             p[r][x] == A(0) ? A(0) : p[r][x] * (s[r][x] - di);
                 }
                 __syncwarp();
-                simt_accumulate<A, DP, R>(ps, qs, ty, tx, dk);
+                simt_accumulate<A, DP, R, R>(ps, qs, ty, tx, dk);
             }
         }
 #pragma unroll
@@ -361,7 +273,7 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
             const int j = j0 + ty + 16 * r;
             if (j >= a.N) continue;
 #pragma unroll
-            for (int x = 0; x < Tile::kCols; ++x) {
+            for (int x = 0; x < Tile::kWidth; ++x) {
                 const int d = tx + 16 * x;
                 if (d >= a.D) continue;
                 const long long at = (((long long)b * a.N + j) * a.Hk + hk) * a.D + d;
@@ -376,9 +288,9 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
     const int i0 = blk % tiles * M, h = blk / tiles % a.H, b = blk / tiles / a.H, hk = h / group;
     const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
-    simt_load<T, A, DP, R>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
-    simt_load<T, A, DP, R>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr);
-    A dq[R][Tile::kCols], li[R], di[R];
+    simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+    simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr);
+    A dq[R][Tile::kWidth], li[R], di[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = i0 + ty + 16 * r;
@@ -386,17 +298,17 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
         li[r] = i < a.Q ? lse[at] : A(INFINITY);
         di[r] = i < a.Q ? delta[at] : A(0);
 #pragma unroll
-        for (int x = 0; x < Tile::kCols; ++x) dq[r][x] = 0;
+        for (int x = 0; x < Tile::kWidth; ++x) dq[r][x] = 0;
     }
     const int key_end = attn_key_end(a, i0 + M);
     for (int j0 = 0; j0 < key_end; j0 += M) {
         __syncthreads();
-        simt_load<T, A, DP, R>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
-        simt_load<T, A, DP, R>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
         __syncthreads();
         A s[R][R], dp[R][R];
-        simt_dot<A, DP, R>(qs, ks, ty, tx, s);
-        simt_dot<A, DP, R>(gs, vs, ty, tx, dp);
+        simt_dot<A, DP, R, R>(qs, ks, ty, tx, s);
+        simt_dot<A, DP, R, R>(gs, vs, ty, tx, dp);
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             const int i = i0 + ty + 16 * r;
@@ -410,14 +322,14 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
             }
         }
         __syncwarp();
-        simt_accumulate<A, DP, R>(ps, ks, ty, tx, dq);
+        simt_accumulate<A, DP, R, R>(ps, ks, ty, tx, dq);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
         const int i = i0 + ty + 16 * r;
         if (i >= a.Q) continue;
 #pragma unroll
-        for (int x = 0; x < Tile::kCols; ++x) {
+        for (int x = 0; x < Tile::kWidth; ++x) {
             const int d = tx + 16 * x;
             if (d < a.D)
                 static_cast<T*>(a.grad_q)[(((long long)b * a.Q + i) * a.H + h) * a.D + d] =

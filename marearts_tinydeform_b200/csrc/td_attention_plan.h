@@ -2,14 +2,14 @@
 // tensor-core launches (td_attention_tc.cu) behind the entry points (td_attention.cu).
 #pragma once
 
-#include "td_attention.cuh"
+#include "td_attention_split.cuh"
 #include "td_host.h"
 
 namespace td {
 
 // Byte offsets into a call's workspace, and the sizes of the packed mask (rows = 1: from the padding alone).
 struct AttnWorkspace {
-    size_t amax, delta, row_bits, row_flags, col_bits, col_flags, total;
+    size_t part_o, part_ml, amax, delta, row_bits, row_flags, col_bits, col_flags, total;
     int64_t images, heads, rows, words, col_words;
 };
 

@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             tmem_ld_32x32b_x32(sc, v[0]);
             tmem_ld_32x32b_x32(sc + 32, v[1]);
             tmem_ld_wait();
-            float top = -INFINITY;
+            // four chains each for the maximum and the sum: one of 64 dependent steps would cost more than the work
+            float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int g = 0; g < 2; ++g) {
                 if (!open) {
@@ -403,8 +404,11 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                         if (((wg >> x) & 1u) == 0) v[g][x] = 0xff800000u;  // -infinity
                 }
 #pragma unroll
-                for (int x = 0; x < 32; ++x) top = fmaxf(top, __uint_as_float(v[g][x]));
+                for (int x = 0; x < 32; x += 2)
+                    tops[x / 2 % 4] = fmaxf(tops[x / 2 % 4],
+                                            fmaxf(__uint_as_float(v[g][x]), __uint_as_float(v[g][x + 1])));
             }
+            const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             if (__any_sync(0xffffffffu, top > ref + slack)) {
                 const float next = fmaxf(ref, top);
                 const float keep = next == -INFINITY ? 1.f : ex2((ref - next) * c);
@@ -428,17 +432,19 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             }
             const float shift = ref == -INFINITY ? 0.f : -ref * c;
             uint32_t p[32];
+            float sums[4] = {sum, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int x = 0; x < 32; ++x) {
                 const float p0 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16)]), c, shift));
                 const float p1 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16) + 1]), c, shift));
-                sum += p0 + p1;
+                sums[x % 4] += p0 + p1;
                 p[x] = pack2<T>(p0, p1);
                 if constexpr (EXACT) {  // v's two registers of this pair are free: they take the rest
                     const float2 r = unpack2<T>(p[x]);
                     v[x / 16][x % 16] = pack2<T>(p0 - r.x, p1 - r.y);
                 }
             }
+            sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
             tmem_st_32x32b_x32(sc, p);
             if constexpr (EXACT) {
                 tmem_st_32x32b_x16(sc + 32, v[0]);

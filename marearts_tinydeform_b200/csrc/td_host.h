@@ -11,12 +11,13 @@
 #include "../../include/tinydeform.h"
 
 namespace td {
+
+constexpr int kSms = 148;  // B200's, for plans that workspace sizes follow from
+
 namespace host {
 
 // Writes the printf-style message into err[0 .. err_len) and returns code.
 int fail(char* err, size_t err_len, int code, const char* fmt, ...);
-// TD_OK and the current device's SM count, or an error.
-int sm_count(int* out, char* err, size_t err_len);
 // Whether the kernel policy is TD_POLICY_BEST.
 bool best_policy();
 void count_launch();

@@ -27,9 +27,9 @@ int check_norm(int dtype, int64_t rows, int64_t C, double eps, char* err, size_t
 int groups_of(int64_t C) { return C <= 512 ? 8 : C <= 2048 ? 2 : 1; }
 
 // The CTAs of a launch: one wave, or fewer when there are fewer rows.
-int norm_grid(int64_t rows, int64_t C, int sms) {
+int norm_grid(int64_t rows, int64_t C) {
     const int64_t need = (rows + groups_of(C) - 1) / groups_of(C);
-    return int(std::min<int64_t>(need, int64_t(sms) * kNormCtasPerSm));
+    return int(std::min<int64_t>(need, int64_t(kSms) * kNormCtasPerSm));
 }
 
 template <typename T, int VEC, bool BWD>
@@ -67,8 +67,6 @@ template <typename T>
 int forward(const void* x, const void* residual, const void* weight, const void* bias, void* y, void* mean,
             void* rstd, int64_t rows, int64_t C, double eps, cudaStream_t stream, char* err, size_t err_len) {
     using acc = typename Elem<T>::acc;
-    int sms = 0;
-    if (int rc = host::sm_count(&sms, err, err_len)) return rc;
     NormArgs<T> a = {};
     a.x = static_cast<const T*>(x);
     a.residual = static_cast<const T*>(residual);
@@ -80,7 +78,7 @@ int forward(const void* x, const void* residual, const void* weight, const void*
     a.rows = rows;
     a.C = int(C);
     a.eps = acc(eps);
-    return pick_norm<T, false>(a, norm_grid(rows, C, sms), stream, err, err_len);
+    return pick_norm<T, false>(a, norm_grid(rows, C), stream, err, err_len);
 }
 
 template <typename T>
@@ -88,8 +86,6 @@ int backward(const void* grad_y, const void* x, const void* residual, const void
              const void* rstd, void* grad_x, void* grad_weight, void* grad_bias, int64_t rows, int64_t C,
              void* workspace, cudaStream_t stream, char* err, size_t err_len) {
     using acc = typename Elem<T>::acc;
-    int sms = 0;
-    if (int rc = host::sm_count(&sms, err, err_len)) return rc;
     NormArgs<T> a = {};
     a.x = static_cast<const T*>(x);
     a.residual = static_cast<const T*>(residual);
@@ -101,7 +97,7 @@ int backward(const void* grad_y, const void* x, const void* residual, const void
     a.partial = static_cast<acc*>(workspace);
     a.rows = rows;
     a.C = int(C);
-    const int grid = norm_grid(rows, C, sms);
+    const int grid = norm_grid(rows, C);
     if (int rc = pick_norm<T, true>(a, grid, stream, err, err_len)) return rc;
     return host::launch(err, err_len, "norm_reduce_kernel", norm_reduce_kernel<T>,
                         dim3(unsigned((2 * C + kReduceCols - 1) / kReduceCols)), dim3(kReduceCols * kReduceRows), 0,
@@ -134,10 +130,8 @@ int td_layer_norm_forward(int dtype, const void* x, const void* residual, const 
 
 size_t td_layer_norm_workspace_bytes(int dtype, int64_t rows, int64_t C) {
     using namespace td;
-    int sms = 0;
     if (dtype < TD_F32 || dtype > TD_F64 || rows <= 0 || C <= 0) return 0;
-    if (host::sm_count(&sms, nullptr, 0) != TD_OK) sms = 148;
-    return size_t(norm_grid(rows, C, sms)) * 2 * size_t(C) * (dtype == TD_F64 ? 8 : 4);
+    return size_t(norm_grid(rows, C)) * 2 * size_t(C) * (dtype == TD_F64 ? 8 : 4);
 }
 
 int td_layer_norm_backward(int dtype, const void* grad_y, const void* x, const void* residual, const void* weight,

@@ -1101,13 +1101,6 @@ int fail(char* err, size_t err_len, int code, const char* fmt, ...) {
     return code;
 }
 
-int sm_count(int* out, char* err, size_t err_len) {
-    DeviceFacts f;
-    if (int rc = device_facts(&f, err, err_len)) return rc;
-    *out = f.sm_count;
-    return TD_OK;
-}
-
 bool best_policy() { return g_policy.load(std::memory_order_relaxed) == TD_POLICY_BEST; }
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
