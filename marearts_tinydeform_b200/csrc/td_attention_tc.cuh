@@ -49,14 +49,37 @@ struct AttnTcArgs {
 constexpr int kAttnBM = 128, kAttnBN = 64;
 
 // ---- PTX ----------------------------------------------------------------------------------------------------------
-// D[tmem] (+)= A[tmem] x B[smem desc]: A is 128 lanes x K packed 16-bit elements, two a column.
-__device__ __forceinline__ void mma_f16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
-                                           uint32_t accumulate) {
+// The MMA warp stays converged: every lane forms the (equal) operands, which the compiler so keeps in uniform registers,
+// and the lane with `leader` set issues. Inside a branch that one lane takes, each descriptor would be moved there anew,
+// which cost more than the products: a tile's 16 took about 1100 cycles to issue.
+// D[tmem] (+)= A[smem desc] x B[smem desc]^T
+__device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
+                                       uint32_t idesc, uint32_t accumulate) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
         "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] x B[smem desc]: A is 128 lanes x K packed 16-bit elements, two a column.
+__device__ __forceinline__ void mma_ts(uint32_t leader, uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc,
+                                       uint32_t idesc, uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 q, %5, 0;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(leader)
+        : "memory");
+}
+__device__ __forceinline__ void commit(uint32_t leader, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\t"
+        "setp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}"
+        ::"r"(smem_addr(bar)), "r"(leader)
         : "memory");
 }
 
@@ -78,6 +101,11 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
           "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t* r) {
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
+                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
+                 : "memory");
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -103,6 +131,42 @@ __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two float32 operations in one instruction (sm_100): pairs in 64-bit registers.
+using F2 = unsigned long long;
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+    F2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ F2 f2(uint32_t lo, uint32_t hi) {
+    F2 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ void f2_split(F2 a, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a));
+}
+__device__ __forceinline__ F2 f2_fma(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ F2 f2_add(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ F2 f2_mul(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // Two floats rounded to T, lo in the low half.
@@ -169,24 +233,25 @@ __device__ __forceinline__ uint64_t sdesc_mn64(uint32_t saddr) {
 
 // D = A x B^T over DP columns: A 128 rows, B 64 rows, both K-major in boxes of 64 columns.
 template <typename T, int DP>
-__device__ __forceinline__ void issue_scores(uint32_t d, uint32_t a_smem, uint32_t b_smem) {
+__device__ __forceinline__ void issue_scores(uint32_t leader, uint32_t d, uint32_t a_smem, uint32_t b_smem) {
     constexpr uint32_t idesc = attn_idesc<T, false>(kAttnBN);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
         const uint64_t da = sdesc_sw128(a_smem + (k / 4) * 16384) + uint64_t(2 * (k % 4));
         const uint64_t db = sdesc_sw128(b_smem + (k / 4) * 8192) + uint64_t(2 * (k % 4));
-        mma_f16(d, da, db, idesc, k != 0);
+        mma_ss(leader, d, da, db, idesc, k != 0);
     }
 }
 
 // acc (+)= A x B: A 128 lanes x 64 packed elements in TMEM, B 64 rows x DP columns in shared memory.
 template <typename T, int DP>
-__device__ __forceinline__ void issue_product(uint32_t acc, uint32_t a_tmem, uint32_t b_smem, bool first) {
+__device__ __forceinline__ void issue_product(uint32_t leader, uint32_t acc, uint32_t a_tmem, uint32_t b_smem,
+                                              bool first) {
     constexpr uint32_t idesc = attn_idesc<T, true>(DP);
     const uint64_t db = sdesc_mn64(b_smem);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        mma_f16_ts(acc, a_tmem + 8 * k, db + uint64_t(128 * k), idesc, !(first && k == 0));
+        mma_ts(leader, acc, a_tmem + 8 * k, db + uint64_t(128 * k), idesc, !(first && k == 0));
 }
 
 // Clears the rows of padded keys in a slot's tile of 64 rows x DP columns (boxes of 64 rows x 128 bytes). One warp.
@@ -268,7 +333,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         }
         for (int g = 0; g < 2; ++g) {
             mbar_init(&sfull[g], 1);
-            mbar_init(&pfull[g], 128);
+            mbar_init(&pfull[g], 4);  // a warp of the four, not a thread: arrivals on one word are served in turn
             mbar_init(&done[g], 1);
         }
         mbar_init(finished, 1);
@@ -284,12 +349,13 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     grid_dependency_wait();
     launch_dependents();
 
     if (warp == 0) {
-        // a lane per box: TMA copies of one thread are served one after another, those of different threads overlap
+        // a lane per box of the ring: TMA copies of one thread are served one after another, those of different threads
+        // overlap
         const uint64_t pol = l2_evict_last();  // keys and values are read again by the other query tiles
         if (lane < KB && tiles > 0) {
             mbar_arrive_expect_tx(qfull, Lay::kQBytes / KB);
@@ -299,11 +365,11 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         for_tiles(0, tiles, flags, [&](int t, bool) {
             const int s = n % S;
             if (!warp_wait(&empty[s], uint32_t((n / S) & 1) ^ 1u, kErrSlotWait)) return false;
-            if (lane < 2 * KB) {
-                const int box = lane % KB;
-                uint64_t* bar = lane < KB ? &kfull[s] : &vfull[s];
+            const int job = lane - 2 * KB * s, box = job % KB;
+            if (job >= 0 && job < 2 * KB) {
+                uint64_t* bar = job < KB ? &kfull[s] : &vfull[s];
                 mbar_arrive_expect_tx(bar, 8192u);
-                tma_load_4d((lane < KB ? k_tile(s) : v_tile(s)) + box * 8192, lane < KB ? &map_k : &map_v, bar,
+                tma_load_4d((job < KB ? k_tile(s) : v_tile(s)) + box * 8192, job < KB ? &map_k : &map_v, bar,
                             64 * box, t * kAttnBN, hk, b, pol);
             }
             __syncwarp();
@@ -317,6 +383,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 warp_wait(&vfull[i % S], uint32_t((i / S) & 1), kErrTmaWait);
             }
     } else if (warp == 1) {
+        const uint32_t leader = lane == 0;
         int n = 0;
         bool ok = tiles == 0 || warp_wait(qfull, 0u, kErrTmaWait);
         auto product = [&](int m) {  // O += P V of tile number m
@@ -324,14 +391,11 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             if (!warp_wait(clearing ? &ready[s] : &vfull[s], uint32_t((m / S) & 1), kErrTmaWait)) return false;
             if (!warp_wait(&pfull[m & 1], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                issue_product<T, DP>(tmem + 128, tmem + 64 * (m & 1), smem_addr(v_tile(s)), m == 0);
-                if constexpr (EXACT)
-                    issue_product<T, DP>(tmem + 128, tmem + 64 * (m & 1) + 32, smem_addr(v_tile(s)), false);
-                mma_commit(&empty[s]);
-                mma_commit(&done[m & 1]);
-            }
-            __syncwarp();
+            issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (m & 1), smem_addr(v_tile(s)), m == 0);
+            if constexpr (EXACT)
+                issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (m & 1) + 32, smem_addr(v_tile(s)), false);
+            commit(leader, &empty[s]);
+            commit(leader, &done[m & 1]);
             return true;
         };
         if (ok)
@@ -340,15 +404,12 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 if (!warp_wait(&kfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
                 tc_fence_after();
                 // the score buffer is free: P of tile n - 2 was read by a product issued before this one
-                if (lane == 0) {
-                    issue_scores<T, DP>(tmem + 64 * (n & 1), smem_addr(smem), smem_addr(k_tile(s)));
-                    mma_commit(&sfull[n & 1]);
-                }
-                __syncwarp();
+                issue_scores<T, DP>(leader, tmem + 64 * (n & 1), smem_addr(smem), smem_addr(k_tile(s)));
+                commit(leader, &sfull[n & 1]);
                 ++n;
                 return n < 2 || product(n - 2);
             });
-        if (ok && n > 0 && product(n - 1) && lane == 0) mma_commit(finished);
+        if (ok && n > 0 && product(n - 1)) commit(leader, finished);
     } else if (warp == 2) {
         if (clearing) {
             int n = 0;
@@ -405,8 +466,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 }
 #pragma unroll
                 for (int x = 0; x < 32; x += 2)
-                    tops[x / 2 % 4] = fmaxf(tops[x / 2 % 4],
-                                            fmaxf(__uint_as_float(v[g][x]), __uint_as_float(v[g][x + 1])));
+                    tops[x / 2 % 4] = max3(tops[x / 2 % 4], __uint_as_float(v[g][x]), __uint_as_float(v[g][x + 1]));
             }
             const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
             if (__any_sync(0xffffffffu, top > ref + slack)) {
@@ -432,19 +492,25 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             }
             const float shift = ref == -INFINITY ? 0.f : -ref * c;
             uint32_t p[32];
-            float sums[4] = {sum, 0.f, 0.f, 0.f};
+            const F2 c2 = f2(c, c), shift2 = f2(shift, shift);
+            F2 sums[4] = {f2(sum, 0.f), 0ull, 0ull, 0ull};
 #pragma unroll
             for (int x = 0; x < 32; ++x) {
-                const float p0 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16)]), c, shift));
-                const float p1 = ex2(fmaf(__uint_as_float(v[x / 16][2 * (x % 16) + 1]), c, shift));
-                sums[x % 4] += p0 + p1;
+                float x0, x1;
+                f2_split(f2_fma(f2(v[x / 16][2 * (x % 16)], v[x / 16][2 * (x % 16) + 1]), c2, shift2), x0, x1);
+                const float p0 = ex2(x0), p1 = ex2(x1);
+                sums[x % 4] = f2_add(sums[x % 4], f2(p0, p1));
                 p[x] = pack2<T>(p0, p1);
                 if constexpr (EXACT) {  // v's two registers of this pair are free: they take the rest
                     const float2 r = unpack2<T>(p[x]);
                     v[x / 16][x % 16] = pack2<T>(p0 - r.x, p1 - r.y);
                 }
             }
-            sum = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            {
+                float s0, s1;
+                f2_split(f2_add(f2_add(sums[0], sums[1]), f2_add(sums[2], sums[3])), s0, s1);
+                sum = s0 + s1;
+            }
             tmem_st_32x32b_x32(sc, p);
             if constexpr (EXACT) {
                 tmem_st_32x32b_x16(sc + 32, v[0]);
@@ -452,7 +518,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             }
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&pfull[n & 1]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[n & 1]);
             ++n;
             return true;
         });
@@ -511,31 +578,83 @@ struct AttnBwdLayout {
     static constexpr int kBoxes = DP / 64;
     static constexpr uint32_t kFixedBytes = kAttnBM * 128 * kBoxes;  // one resident operand
     static constexpr uint32_t kTileBytes = kAttnBN * 128 * kBoxes;   // one streamed operand
-    static constexpr int kStages = 4;
+    // score buffers (S and dP, 64 columns each) and ring slots: with a buffer more than there are warpgroups, each finds
+    // its next tile's scores formed when it is done with one; wide heads' accumulators leave TMEM for two buffers
+    static constexpr int kBufs = DP == 64 ? 3 : 2;
+    static constexpr int kStages = DP == 64 ? 6 : 4;
+    static constexpr uint32_t kAcc = kBufs * 128;  // first accumulator's TMEM column
     static constexpr uint32_t kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kRing = 2 * kFixedBytes;
     static constexpr uint32_t kStats = kRing + kStages * kStageBytes;  // per stage: lse[64], delta[64]
     static constexpr uint32_t kBars = kStats + kStages * 2 * kAttnBN * 4;
-    // fixed, full[S], ready[S], empty[S], sfull[2], pfull[2], finished
-    static constexpr int kNumBars = 1 + 3 * kStages + 5;
+    // fixed, full[S], ready[S], empty[S], sfull[bufs], pfull[bufs], finished
+    static constexpr int kNumBars = 1 + 3 * kStages + 2 * kBufs + 1;
     static constexpr uint32_t kSlot = kBars + kNumBars * 8;
     static constexpr uint32_t kSmemBytes = kSlot + 16 + 1024;
-    static constexpr uint32_t kTmemCols = 512;  // per warpgroup S and dP of 64, then two accumulators of DP
-    static_assert(256 + 2 * DP <= 512, "TMEM");
+    static constexpr uint32_t kTmemCols = 512;
+    static_assert(kAcc + 2 * DP <= 512, "TMEM");
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
 constexpr int kAttnBwdThreads = 384;  // producer, MMA, clearing, -, two elementwise warpgroups
 
-// float16 keeps P as 2^12 P (at most 4096, so that a row over many thousand keys stays above its smallest normal
-// number) and dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
-// gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs neither.
-constexpr float kHalfPShift = 12.f;
-
+// float16 keeps dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
+// gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs no scale.
 __device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {
     const float bound = 2.f * float(args.a.D) * __uint_as_float(args.amax[0]) * __uint_as_float(args.amax[1]);
     if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
-    return exp2f(fminf(fmaxf(15.f - kHalfPShift - ceilf(log2f(bound)), -100.f), 100.f));
+    return exp2f(fminf(fmaxf(15.f - ceilf(log2f(bound)), -100.f), 100.f));
+}
+
+// P and dS of one row of a tile of 64 columns, from the scores at sc and sc + 64 to packed pairs in the same places. The
+// statistics are the row's own, or (KEYS) the columns', lse[64] and delta[64] at st. MASKED: w has a bit per open pair.
+template <typename T, bool KEYS, bool MASKED>
+__device__ __forceinline__ void elementwise(uint32_t sc, const float* st, float row_lse, float row_delta, float c,
+                                            float ds_scale, unsigned long long w) {
+    constexpr bool kHalf = std::is_same<T, __half>::value;
+    uint32_t s[2][16], d[2][16];
+    tmem_ld_32x32b_x16(sc, s[0]);
+    tmem_ld_32x32b_x16(sc + 64, d[0]);
+#pragma unroll
+    for (int part = 0; part < 4; ++part) {
+        tmem_ld_wait();
+        if (part < 3) {
+            tmem_ld_32x32b_x16(sc + 16 * (part + 1), s[(part + 1) & 1]);
+            tmem_ld_32x32b_x16(sc + 64 + 16 * (part + 1), d[(part + 1) & 1]);
+        }
+        uint32_t p[8], e[8];
+        const F2 nc = f2(-c, -c), minus = f2(-1.f, -1.f), scale = f2(ds_scale, ds_scale);
+        const uint32_t open = MASKED ? uint32_t(w >> (16 * part)) : 0u;
+#pragma unroll
+        for (int x = 0; x < 16; x += 4) {
+            F2 ls[2] = {f2(row_lse, row_lse), f2(row_lse, row_lse)};
+            F2 de[2] = {f2(row_delta, row_delta), f2(row_delta, row_delta)};
+            if constexpr (KEYS) {
+                const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(st + 16 * part + x);
+                const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(st + kAttnBN + 16 * part + x);
+                ls[0] = a.x; ls[1] = a.y; de[0] = b.x; de[1] = b.y;
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const int at = x + 2 * y;
+                // lse - c S, whose negative the exponential takes; dP - delta
+                float l0, l1, e0, e1;
+                f2_split(f2_fma(f2(s[part & 1][at], s[part & 1][at + 1]), nc, ls[y]), l0, l1);
+                float p0 = ex2(-l0), p1 = ex2(-l1);
+                F2 diff = f2_fma(de[y], minus, f2(d[part & 1][at], d[part & 1][at + 1]));
+                if constexpr (kHalf) diff = f2_mul(diff, scale);
+                f2_split(f2_mul(f2(p0, p1), diff), e0, e1);
+                if constexpr (MASKED) {
+                    if (((open >> at) & 1u) == 0) p0 = e0 = 0.f;
+                    if (((open >> (at + 1)) & 1u) == 0) p1 = e1 = 0.f;
+                }
+                p[at / 2] = pack2<T>(p0, p1);
+                e[at / 2] = pack2<T>(e0, e1);
+            }
+        }
+        if constexpr (KEYS) tmem_st_32x32b_x8(sc + 8 * part, p);
+        tmem_st_32x32b_x8(sc + 64 + 8 * part, e);
+    }
 }
 
 // One block of the keys' gradient (KEYS) or of the queries' gradient.
@@ -545,12 +664,12 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                                                        const AttnTcArgs& args, int block, unsigned char* smem,
                                                        uint32_t tmem) {
     using Lay = AttnBwdLayout<DP>;
-    constexpr int S = Lay::kStages, KB = Lay::kBoxes;
+    constexpr int S = Lay::kStages, KB = Lay::kBoxes, NB = Lay::kBufs;
     constexpr bool kHalf = std::is_same<T, __half>::value;
     const AttnArgs& a = args.a;
     uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
-    uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + 2,
-             *finished = pfull + 2;
+    uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + NB,
+             *finished = pfull + NB;
     auto tile1 = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes; };
     auto tile2 = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes + Lay::kTileBytes; };
     auto stats = [&](int s) { return reinterpret_cast<float*>(smem + Lay::kStats) + s * 2 * kAttnBN; };
@@ -593,15 +712,17 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         each_tile([&](int h, int t, bool) {
             const int s = n % S;
             if (!warp_wait(&empty[s], uint32_t((n / S) & 1) ^ 1u, kErrSlotWait)) return false;
-            if (lane < 2 * KB) {
-                const int box = lane % KB;
+            constexpr int kJobs = 2 * KB + (KEYS ? 2 : 0);
+            static_assert(kJobs * S <= 32, "a lane per copy of the ring");
+            const int job = lane - kJobs * s, box = job % KB;
+            if (job >= 0 && job < 2 * KB) {
                 mbar_arrive_expect_tx(&full[s], 8192u);
-                tma_load_4d((lane < KB ? tile1(s) : tile2(s)) + box * 8192, lane < KB ? &map_b1 : &map_b2, &full[s],
+                tma_load_4d((job < KB ? tile1(s) : tile2(s)) + box * 8192, job < KB ? &map_b1 : &map_b2, &full[s],
                             64 * box, t * kAttnBN, KEYS ? h : hk, b, pol);
-            } else if (KEYS && lane < 2 * KB + 2) {
-                const float* src = static_cast<const float*>(lane == 2 * KB ? a.lse : a.delta);
+            } else if (job >= 2 * KB && job < kJobs) {
+                const float* src = static_cast<const float*>(job == 2 * KB ? a.lse : a.delta);
                 mbar_arrive_expect_tx(&full[s], kAttnBN * 4u);
-                bulk_load(stats(s) + (lane - 2 * KB) * kAttnBN,
+                bulk_load(stats(s) + (job - 2 * KB) * kAttnBN,
                           src + ((long long)b * a.H + h) * a.Qp + t * kAttnBN, kAttnBN * 4u, &full[s]);
             }
             __syncwarp();
@@ -613,38 +734,37 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             if (!warp_wait(&empty[i % S], uint32_t((i / S) & 1), kErrSlotWait))
                 warp_wait(&full[i % S], uint32_t((i / S) & 1), kErrTmaWait);
     } else if (warp == 1) {
+        const uint32_t leader = lane == 0;
         int n = 0;
         bool ok = warp_wait(fixed, 0u, kErrTmaWait);
         auto products = [&](int m) {  // the accumulators' part of tile number m
-            const int s = m % S;
-            const uint32_t sc = tmem + 128 * (m & 1);
-            if (!warp_wait(&pfull[m & 1], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
+            const int s = m % S, u = m % NB;
+            const uint32_t sc = tmem + 128 * u;
+            if (!warp_wait(&pfull[u], uint32_t((m / NB) & 1), kErrMmaWait)) return false;
             tc_fence_after();
-            if (lane == 0) {
-                if constexpr (KEYS)
-                    issue_product<T, DP>(tmem + 256 + DP, sc, smem_addr(tile2(s)), m == 0);  // dV += P^T dO
-                issue_product<T, DP>(tmem + 256, sc + 64, smem_addr(tile1(s)), m == 0);      // dK += dS^T Q, dQ += dS K
-                mma_commit(&empty[s]);
-            }
-            __syncwarp();
+            if constexpr (KEYS)
+                issue_product<T, DP>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(s)), m == 0);  // dV += P^T dO
+            // dK += dS^T Q, dQ += dS K
+            issue_product<T, DP>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(s)), m == 0);
+            commit(leader, &empty[s]);
             return true;
         };
         if (ok)
             ok = each_tile([&](int, int, bool) {
-                const int s = n % S;
+                const int s = n % S, u = n % NB;
                 if (!warp_wait(clearing ? &ready[s] : &full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                // the buffer's P and dS before these were read by products issued before
+                if (n >= NB && !products(n - NB)) return false;
                 tc_fence_after();
-                if (lane == 0) {
-                    const uint32_t sc = tmem + 128 * (n & 1);
-                    issue_scores<T, DP>(sc, smem_addr(smem), smem_addr(tile1(s)));
-                    issue_scores<T, DP>(sc + 64, smem_addr(smem + Lay::kFixedBytes), smem_addr(tile2(s)));
-                    mma_commit(&sfull[n & 1]);
-                }
-                __syncwarp();
+                const uint32_t sc = tmem + 128 * u;
+                issue_scores<T, DP>(leader, sc, smem_addr(smem), smem_addr(tile1(s)));
+                issue_scores<T, DP>(leader, sc + 64, smem_addr(smem + Lay::kFixedBytes), smem_addr(tile2(s)));
+                commit(leader, &sfull[u]);
                 ++n;
-                return n < 2 || products(n - 2);
+                return true;
             });
-        if (ok && n > 0 && products(n - 1) && lane == 0) mma_commit(finished);
+        for (int m = max(0, n - NB); ok && m < n; ++m) ok = products(m);
+        if (ok && n > 0) commit(leader, finished);
     } else if (warp == 2) {
         if (clearing) {
             int n = 0;
@@ -660,15 +780,14 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         }
     } else if (warp >= 4) {
         const int quarter = warp & 3, wg = (warp - 4) >> 2, r = r0 + quarter * 32 + lane;
-        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16), sc = lanes + 128 * wg;
+        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
         const float c = float(a.scale * 1.4426950408889634);
         const float ds_scale = kHalf ? attn_ds_scale(args) : 1.f;
-        const float p_shift = kHalf ? kHalfPShift : 0.f;
         float row_lse = INFINITY, row_delta = 0.f;
         if (!KEYS) {  // the rows' own statistics (the arrays hold Qp rows, a multiple of the tile)
             const long long at = ((long long)b * a.H + h0) * a.Qp + r;
-            row_lse = static_cast<const float*>(a.lse)[at] - p_shift;
-            row_delta = static_cast<const float*>(a.delta)[at] * ds_scale;
+            row_lse = static_cast<const float*>(a.lse)[at];
+            row_delta = static_cast<const float*>(a.delta)[at];
         }
         int n = 0;
         bool ok = each_tile([&](int h, int t, bool all) {
@@ -699,53 +818,20 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                     }
                 }
             }
-            if (!warp_wait(&sfull[wg], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
+            const int u = m % NB;
             if (KEYS && !warp_wait(&full[m % S], uint32_t((m / S) & 1), kErrTmaWait)) return false;  // the statistics
+            if (!warp_wait(&sfull[u], uint32_t((m / NB) & 1), kErrMmaWait)) return false;
             tc_fence_after();
-            const float* st = stats(m % S);
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                uint32_t s[32], d[32], p[16], e[16];
-                tmem_ld_32x32b_x32(sc + 32 * half, s);
-                tmem_ld_32x32b_x32(sc + 64 + 32 * half, d);
-                tmem_ld_wait();
-                const uint32_t wh = uint32_t(w >> (32 * half));
-#pragma unroll
-                for (int x = 0; x < 32; x += 4) {
-                    float4 ls = make_float4(row_lse, row_lse, row_lse, row_lse);
-                    float4 de = make_float4(row_delta, row_delta, row_delta, row_delta);
-                    if constexpr (KEYS) {
-                        ls = *reinterpret_cast<const float4*>(st + 32 * half + x);
-                        de = *reinterpret_cast<const float4*>(st + kAttnBN + 32 * half + x);
-                    }
-                    const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {de.x, de.y, de.z, de.w};
-                    float pv[4], ev[4];
-#pragma unroll
-                    for (int y = 0; y < 4; ++y) {
-                        const float sv = __uint_as_float(s[x + y]), dp = __uint_as_float(d[x + y]);
-                        if constexpr (KEYS && kHalf) {
-                            pv[y] = ex2(fmaf(sv, c, kHalfPShift - lv[y]));
-                            ev[y] = pv[y] * ds_scale * (dp - dv[y]);
-                        } else if constexpr (kHalf) {
-                            pv[y] = ex2(fmaf(sv, c, -lv[y]));
-                            ev[y] = pv[y] * fmaf(dp, ds_scale, -dv[y]);
-                        } else {
-                            pv[y] = ex2(fmaf(sv, c, -lv[y]));
-                            ev[y] = pv[y] * (dp - dv[y]);
-                        }
-                        if (!open && ((wh >> (x + y)) & 1u) == 0) pv[y] = ev[y] = 0.f;
-                    }
-                    p[x / 2] = pack2<T>(pv[0], pv[1]);
-                    p[x / 2 + 1] = pack2<T>(pv[2], pv[3]);
-                    e[x / 2] = pack2<T>(ev[0], ev[1]);
-                    e[x / 2 + 1] = pack2<T>(ev[2], ev[3]);
-                }
-                if constexpr (KEYS) tmem_st_32x32b_x16(sc + 16 * half, p);
-                tmem_st_32x32b_x16(sc + 64 + 16 * half, e);
-            }
+            const uint32_t sc = lanes + 128 * u;
+            // 16 columns at a time, the next ones' loads in flight meanwhile; P and dS go where the first scores were
+            if (open)
+                elementwise<T, KEYS, false>(sc, stats(m % S), row_lse, row_delta, c, ds_scale, w);
+            else
+                elementwise<T, KEYS, true>(sc, stats(m % S), row_lse, row_delta, c, ds_scale, w);
             tmem_st_wait();
             tc_fence_before();
-            mbar_arrive(&pfull[wg]);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&pfull[u]);
             return true;
         });
         ok = ok && (n == 0 || warp_wait(finished, 0u, kErrMmaWait));
@@ -753,8 +839,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         // the gradients' rows: a warpgroup an accumulator for the keys' block, else half of the columns each
         if (ok) {
             const bool is_v = KEYS && wg == 1;
-            const float k_scale = float(a.scale) / (kHalf ? exp2f(kHalfPShift) * ds_scale : 1.f);
-            const float f = is_v ? (kHalf ? exp2f(-kHalfPShift) : 1.f) : k_scale;
+            const float f = is_v ? 1.f : float(a.scale) / ds_scale;
             const bool gone = KEYS && a.padding != nullptr && r < a.N && a.padding[(long long)b * a.N + r] != 0;
             T* out = KEYS ? static_cast<T*>(is_v ? a.grad_v : a.grad_k) + (((long long)b * a.N + r) * a.Hk + hk) * a.D
                           : static_cast<T*>(a.grad_q) + (((long long)b * a.Q + r) * a.H + h0) * a.D;
@@ -764,7 +849,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                 uint32_t o[32];
                 __syncwarp();
                 if (n > 0) {
-                    tmem_ld_32x32b_x32(lanes + 256 + (is_v ? DP : 0) + d, o);
+                    tmem_ld_32x32b_x32(lanes + Lay::kAcc + (is_v ? DP : 0) + d, o);
                     tmem_ld_wait();
                 }
                 if (r >= rows) continue;
@@ -794,25 +879,25 @@ __global__ void __launch_bounds__(kAttnBwdThreads, 1)
                             const __grid_constant__ CUtensorMap k64, const __grid_constant__ CUtensorMap v64,
                             const AttnTcArgs args) {
     using Lay = AttnBwdLayout<DP>;
-    constexpr int S = Lay::kStages, KB = Lay::kBoxes;
+    constexpr int S = Lay::kStages, KB = Lay::kBoxes, NB = Lay::kBufs;
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Lay::kSlot);
     const bool keys = int(blockIdx.x) < args.kv_blocks;
     if (threadIdx.x == 0) {
         uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
-        uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + 2;
+        uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + NB;
         mbar_init(fixed, 2 * KB);
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 2 * KB + (keys ? 2 : 0));
             mbar_init(&ready[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int g = 0; g < 2; ++g) {
+        for (int g = 0; g < NB; ++g) {
             mbar_init(&sfull[g], 1);
-            mbar_init(&pfull[g], 128);
+            mbar_init(&pfull[g], 4);  // a warp of the four, not a thread: arrivals on one word are served in turn
         }
-        mbar_init(pfull + 2, 1);  // finished
+        mbar_init(pfull + NB, 1);  // finished
         mbar_fence_init();
     }
     if ((threadIdx.x >> 5) == 1) {
@@ -822,7 +907,7 @@ __global__ void __launch_bounds__(kAttnBwdThreads, 1)
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     grid_dependency_wait();
     launch_dependents();
     if (keys)
