@@ -49,7 +49,7 @@ struct AttnTcArgs {
 constexpr int kAttnBM = 128, kAttnBN = 64;
 
 // ---- PTX ----------------------------------------------------------------------------------------------------------
-// The MMA warp stays converged: every lane forms the (equal) operands, which the compiler so keeps in uniform registers,
+// The MMA warps stay converged: every lane forms the (equal) operands, which the compiler so keeps in uniform registers,
 // and the lane with `leader` set issues. Inside a branch that one lane takes, each descriptor would be moved there anew,
 // which cost more than the products: a tile's 16 took about 1100 cycles to issue.
 // D[tmem] (+)= A[smem desc] x B[smem desc]^T
@@ -282,8 +282,8 @@ struct AttnFwdLayout {
     static constexpr uint32_t kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kRing = kQBytes;
     static constexpr uint32_t kBars = kRing + kStages * kStageBytes;
-    // qfull, kfull[S], vfull[S], ready[S], empty[S], sfull[2], pfull[2], done[2], finished
-    static constexpr int kNumBars = 1 + 4 * kStages + 7;
+    // qfull, kfull[S], vfull[S], empty[S], sfull[2], pfull[2], done[2], finished
+    static constexpr int kNumBars = 1 + 3 * kStages + 7;
     static constexpr uint32_t kSlot = kBars + kNumBars * 8;
     static constexpr uint32_t kSmemBytes = kSlot + 16 + 1024;
     static constexpr uint32_t kTmemCols = 256;  // two score tiles of 64, the output's DP
@@ -291,7 +291,7 @@ struct AttnFwdLayout {
     static_assert(2 * kSmemBytes <= 227 * 1024, "two CTAs an SM");
 };
 
-constexpr int kAttnFwdThreads = 256;  // producer, MMA, clearing, -, four softmax warps
+constexpr int kAttnFwdThreads = 224;  // loads, scores, products, four softmax warps
 
 // EXACT, for a forward that a backward follows: P is kept as two 16-bit parts, its rounding and what that took, which
 // both go through the product (one product more a tile), and the result's rounding is kept as well: see delta in
@@ -306,8 +306,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     uint64_t* qfull = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
-    uint64_t *kfull = qfull + 1, *vfull = kfull + S, *ready = vfull + S, *empty = ready + S, *sfull = empty + S,
-             *pfull = sfull + 2, *done = pfull + 2, *finished = done + 2;
+    uint64_t *kfull = qfull + 1, *vfull = kfull + S, *empty = vfull + S, *sfull = empty + S, *pfull = sfull + 2,
+             *done = pfull + 2, *finished = done + 2;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Lay::kSlot);
     auto k_tile = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes; };
     auto v_tile = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes + Lay::kTileBytes; };
@@ -321,14 +321,12 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     const uint8_t* flags = args.row_flags == nullptr
                                ? nullptr
                                : args.row_flags + b * args.rf_b + h * args.rf_h + qt * args.rf_q;
-    const bool clearing = a.padding != nullptr;
 
     if (threadIdx.x == 0) {
         mbar_init(qfull, KB);
         for (int s = 0; s < S; ++s) {
             mbar_init(&kfull[s], KB);
             mbar_init(&vfull[s], KB);
-            mbar_init(&ready[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int g = 0; g < 2; ++g) {
@@ -385,45 +383,38 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     } else if (warp == 1) {
         const uint32_t leader = lane == 0;
         int n = 0;
-        bool ok = tiles == 0 || warp_wait(qfull, 0u, kErrTmaWait);
-        auto product = [&](int m) {  // O += P V of tile number m
-            const int s = m % S;
-            if (!warp_wait(clearing ? &ready[s] : &vfull[s], uint32_t((m / S) & 1), kErrTmaWait)) return false;
-            if (!warp_wait(&pfull[m & 1], uint32_t((m >> 1) & 1), kErrMmaWait)) return false;
-            tc_fence_after();
-            issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (m & 1), smem_addr(v_tile(s)), m == 0);
-            if constexpr (EXACT)
-                issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (m & 1) + 32, smem_addr(v_tile(s)), false);
-            commit(leader, &empty[s]);
-            commit(leader, &done[m & 1]);
-            return true;
-        };
-        if (ok)
-            ok = for_tiles(0, tiles, flags, [&](int, bool) {
+        if (tiles == 0 || warp_wait(qfull, 0u, kErrTmaWait))
+            for_tiles(0, tiles, flags, [&](int, bool) {
                 const int s = n % S;
                 if (!warp_wait(&kfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                // the buffer's P before these scores has been read by its product
+                if (n >= 2 && !warp_wait(&done[n & 1], uint32_t((n / 2 - 1) & 1), kErrMmaWait)) return false;
                 tc_fence_after();
-                // the score buffer is free: P of tile n - 2 was read by a product issued before this one
                 issue_scores<T, DP>(leader, tmem + 64 * (n & 1), smem_addr(smem), smem_addr(k_tile(s)));
                 commit(leader, &sfull[n & 1]);
                 ++n;
-                return n < 2 || product(n - 2);
-            });
-        if (ok && n > 0 && product(n - 1)) commit(leader, finished);
-    } else if (warp == 2) {
-        if (clearing) {
-            int n = 0;
-            const uint8_t* pad = a.padding + (long long)b * a.N;
-            for_tiles(0, tiles, flags, [&](int t, bool) {
-                const int s = n % S;
-                if (!warp_wait(&vfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
-                clear_padded<DP>(v_tile(s), pad, t * kAttnBN, a.N);
-                if (lane == 0) mbar_arrive(&ready[s]);
-                ++n;
                 return true;
             });
-        }
-    } else if (warp >= 4) {
+    } else if (warp == 2) {
+        const uint32_t leader = lane == 0;
+        const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
+        int n = 0;
+        const bool ok = for_tiles(0, tiles, flags, [&](int t, bool all) {
+            const int s = n % S;
+            if (!warp_wait(&vfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+            if (pad != nullptr && !all) clear_padded<DP>(v_tile(s), pad, t * kAttnBN, a.N);
+            if (!warp_wait(&pfull[n & 1], uint32_t((n >> 1) & 1), kErrMmaWait)) return false;
+            tc_fence_after();
+            issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (n & 1), smem_addr(v_tile(s)), n == 0);
+            if constexpr (EXACT)
+                issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (n & 1) + 32, smem_addr(v_tile(s)), false);
+            commit(leader, &empty[s]);
+            commit(leader, &done[n & 1]);
+            ++n;
+            return true;
+        });
+        if (ok && n > 0) commit(leader, finished);
+    } else {
         const int quarter = warp & 3, i = i0 + quarter * 32 + lane;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
         const float c = float(a.scale * 1.4426950408889634);
@@ -587,8 +578,8 @@ struct AttnBwdLayout {
     static constexpr uint32_t kRing = 2 * kFixedBytes;
     static constexpr uint32_t kStats = kRing + kStages * kStageBytes;  // per stage: lse[64], delta[64]
     static constexpr uint32_t kBars = kStats + kStages * 2 * kAttnBN * 4;
-    // fixed, full[S], ready[S], empty[S], sfull[bufs], pfull[bufs], finished
-    static constexpr int kNumBars = 1 + 3 * kStages + 2 * kBufs + 1;
+    // fixed, full[S], empty[S], sfull[bufs], pfull[bufs], done[bufs], finished
+    static constexpr int kNumBars = 1 + 2 * kStages + 3 * kBufs + 1;
     static constexpr uint32_t kSlot = kBars + kNumBars * 8;
     static constexpr uint32_t kSmemBytes = kSlot + 16 + 1024;
     static constexpr uint32_t kTmemCols = 512;
@@ -596,7 +587,7 @@ struct AttnBwdLayout {
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-constexpr int kAttnBwdThreads = 384;  // producer, MMA, clearing, -, two elementwise warpgroups
+constexpr int kAttnBwdThreads = 384;  // loads, scores, products, -, two elementwise warpgroups
 
 // float16 keeps dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
 // gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs no scale.
@@ -668,8 +659,8 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
     constexpr bool kHalf = std::is_same<T, __half>::value;
     const AttnArgs& a = args.a;
     uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
-    uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + NB,
-             *finished = pfull + NB;
+    uint64_t *full = fixed + 1, *empty = full + S, *sfull = empty + S, *pfull = sfull + NB, *done = pfull + NB,
+             *finished = done + NB;
     auto tile1 = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes; };
     auto tile2 = [&](int s) { return smem + Lay::kRing + s * Lay::kStageBytes + Lay::kTileBytes; };
     auto stats = [&](int s) { return reinterpret_cast<float*>(smem + Lay::kStats) + s * 2 * kAttnBN; };
@@ -687,7 +678,6 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
     const int t0 = KEYS && a.causal ? max(0, min(a.Q, r0 - off)) / kAttnBN : 0;
     const int t1 = KEYS ? (a.Q + kAttnBN - 1) / kAttnBN
                         : (attn_key_end(a, r0 + kAttnBM) + kAttnBN - 1) / kAttnBN;
-    const bool clearing = !KEYS && a.padding != nullptr;
     auto each_tile = [&](auto&& f) {  // f(head, tile, all open by the flags)
         for (int h = h0; h < h1; ++h) {
             const uint8_t* flags = nullptr;
@@ -736,25 +726,12 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
     } else if (warp == 1) {
         const uint32_t leader = lane == 0;
         int n = 0;
-        bool ok = warp_wait(fixed, 0u, kErrTmaWait);
-        auto products = [&](int m) {  // the accumulators' part of tile number m
-            const int s = m % S, u = m % NB;
-            const uint32_t sc = tmem + 128 * u;
-            if (!warp_wait(&pfull[u], uint32_t((m / NB) & 1), kErrMmaWait)) return false;
-            tc_fence_after();
-            if constexpr (KEYS)
-                issue_product<T, DP>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(s)), m == 0);  // dV += P^T dO
-            // dK += dS^T Q, dQ += dS K
-            issue_product<T, DP>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(s)), m == 0);
-            commit(leader, &empty[s]);
-            return true;
-        };
-        if (ok)
-            ok = each_tile([&](int, int, bool) {
+        if (warp_wait(fixed, 0u, kErrTmaWait))
+            each_tile([&](int, int, bool) {
                 const int s = n % S, u = n % NB;
-                if (!warp_wait(clearing ? &ready[s] : &full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
-                // the buffer's P and dS before these were read by products issued before
-                if (n >= NB && !products(n - NB)) return false;
+                if (!warp_wait(&full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
+                // the buffer's P and dS before these scores have been read by their products
+                if (n >= NB && !warp_wait(&done[u], uint32_t((n / NB - 1) & 1), kErrMmaWait)) return false;
                 tc_fence_after();
                 const uint32_t sc = tmem + 128 * u;
                 issue_scores<T, DP>(leader, sc, smem_addr(smem), smem_addr(tile1(s)));
@@ -763,21 +740,27 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                 ++n;
                 return true;
             });
-        for (int m = max(0, n - NB); ok && m < n; ++m) ok = products(m);
-        if (ok && n > 0) commit(leader, finished);
     } else if (warp == 2) {
-        if (clearing) {
-            int n = 0;
-            const uint8_t* pad = a.padding + (long long)b * a.N;
-            each_tile([&](int, int t, bool) {
-                const int s = n % S;
-                if (!warp_wait(&full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
-                clear_padded<DP>(tile1(s), pad, t * kAttnBN, a.N);
-                if (lane == 0) mbar_arrive(&ready[s]);
-                ++n;
-                return true;
-            });
-        }
+        const uint32_t leader = lane == 0;
+        const uint8_t* pad = KEYS || a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
+        int n = 0;
+        const bool ok = each_tile([&](int, int t, bool all) {
+            const int s = n % S, u = n % NB;
+            const uint32_t sc = tmem + 128 * u;
+            if (!warp_wait(&pfull[u], uint32_t((n / NB) & 1), kErrMmaWait)) return false;
+            // (this tile's scores are formed: what they made of padded rows has been replaced)
+            if (pad != nullptr && !all) clear_padded<DP>(tile1(s), pad, t * kAttnBN, a.N);
+            tc_fence_after();
+            if constexpr (KEYS)
+                issue_product<T, DP>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(s)), n == 0);  // dV += P^T dO
+            // dK += dS^T Q, dQ += dS K
+            issue_product<T, DP>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(s)), n == 0);
+            commit(leader, &empty[s]);
+            commit(leader, &done[u]);
+            ++n;
+            return true;
+        });
+        if (ok && n > 0) commit(leader, finished);
     } else if (warp >= 4) {
         const int quarter = warp & 3, wg = (warp - 4) >> 2, r = r0 + quarter * 32 + lane;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
@@ -886,18 +869,18 @@ __global__ void __launch_bounds__(kAttnBwdThreads, 1)
     const bool keys = int(blockIdx.x) < args.kv_blocks;
     if (threadIdx.x == 0) {
         uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
-        uint64_t *full = fixed + 1, *ready = full + S, *empty = ready + S, *sfull = empty + S, *pfull = sfull + NB;
+        uint64_t *full = fixed + 1, *empty = full + S, *sfull = empty + S, *pfull = sfull + NB, *done = pfull + NB;
         mbar_init(fixed, 2 * KB);
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 2 * KB + (keys ? 2 : 0));
-            mbar_init(&ready[s], 1);
             mbar_init(&empty[s], 1);
         }
         for (int g = 0; g < NB; ++g) {
             mbar_init(&sfull[g], 1);
-            mbar_init(&pfull[g], 4);  // a warp of the four, not a thread: arrivals on one word are served in turn
+            mbar_init(&pfull[g], 4);  // as in the forward
+            mbar_init(&done[g], 1);
         }
-        mbar_init(pfull + NB, 1);  // finished
+        mbar_init(done + NB, 1);  // finished
         mbar_fence_init();
     }
     if ((threadIdx.x >> 5) == 1) {
