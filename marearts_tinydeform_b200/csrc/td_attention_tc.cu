@@ -44,14 +44,16 @@ bool operand_fits(const Operand& o, const AttnArgs& a) {
     return aligned16(o.base);
 }
 
-// Boxes of 64 columns x `rows` tokens of one head of one image, 128-byte swizzle; what lies outside reads as zero.
+// Boxes of min(DP, 64) columns x `rows` tokens of one head of one image; what lies outside reads as zero.
+template <int DP>
 int make_map(CUtensorMap* map, const Operand& o, int rows, const AttnArgs& a, char* err, size_t err_len) {
     const uint64_t dims[4] = {uint64_t(a.D), uint64_t(o.tokens), uint64_t(o.heads), uint64_t(a.B)};
     const uint64_t strides[3] = {uint64_t(map_stride(o.s_t, o.tokens, a)) * 2,
                                  uint64_t(map_stride(o.s_h, o.heads, a)) * 2,
                                  uint64_t(map_stride(o.s_b, a.B, a)) * 2};
-    const uint32_t box[4] = {64, uint32_t(rows), 1, 1};
-    const CUresult r = host::encode_tiled_u16(map, 4, o.base, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    const uint32_t box[4] = {uint32_t(AttnBox<DP>::kCols), uint32_t(rows), 1, 1};
+    const CUresult r = host::encode_tiled_u16(map, 4, o.base, dims, strides, box,
+                                              DP == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     if (r == CUDA_SUCCESS) return TD_OK;
     return fail(err, err_len, TD_ERR_CUDA, "cuTensorMapEncodeTiled (attention) failed (%d)", int(r));
 }
@@ -103,9 +105,9 @@ int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsig
             cudaStream_t stream, char* err, size_t err_len) {
     const AttnArgs& a = t.a;
     CUtensorMap q, k, v;
-    if (int rc = make_map(&q, query_of(a), kAttnBM, a, err, err_len)) return rc;
-    if (int rc = make_map(&k, key_of(a), kAttnBN, a, err, err_len)) return rc;
-    if (int rc = make_map(&v, value_of(a), kAttnBN, a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&q, query_of(a), kAttnBM, a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&k, key_of(a), kAttnBN, a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&v, value_of(a), kAttnBN, a, err, err_len)) return rc;
     if (int rc = pack_masks(t, w, mb, mh, false, workspace, stream, err, err_len)) return rc;
     auto kernel = attn_tc_forward_kernel<T, DP, EXACT>;
     constexpr size_t smem = AttnFwdLayout<DP>::kSmemBytes;
@@ -122,8 +124,8 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
     const Operand ops[4] = {query_of(a), grad_of(a), key_of(a), value_of(a)};
     CUtensorMap fixed[4], tile[4];
     for (int i = 0; i < 4; ++i) {
-        if (int rc = make_map(&fixed[i], ops[i], kAttnBM, a, err, err_len)) return rc;
-        if (int rc = make_map(&tile[i], ops[i], kAttnBN, a, err, err_len)) return rc;
+        if (int rc = make_map<DP>(&fixed[i], ops[i], kAttnBM, a, err, err_len)) return rc;
+        if (int rc = make_map<DP>(&tile[i], ops[i], kAttnBN, a, err, err_len)) return rc;
     }
     if (int rc = pack_masks(t, w, mb, mh, true, workspace, stream, err, err_len)) return rc;
     int lanes = 1;
@@ -173,8 +175,9 @@ int attn_tc_forward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_
     auto go = [&](auto type, auto exact) {
         using T = decltype(type);
         constexpr bool E = decltype(exact)::value;
-        return a.D <= 64 ? forward<T, 64, E>(t, w, mb, mh, workspace, stream, err, err_len)
-                         : forward<T, 128, E>(t, w, mb, mh, workspace, stream, err, err_len);
+        if (a.D <= 32) return forward<T, 32, E>(t, w, mb, mh, workspace, stream, err, err_len);
+        if (a.D <= 64) return forward<T, 64, E>(t, w, mb, mh, workspace, stream, err, err_len);
+        return forward<T, 128, E>(t, w, mb, mh, workspace, stream, err, err_len);
     };
     auto pick = [&](auto type) {
         return a.rest != nullptr ? go(type, std::true_type{}) : go(type, std::false_type{});
@@ -186,11 +189,13 @@ int attn_tc_backward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64
                      unsigned char* workspace, cudaStream_t stream, char* err, size_t err_len) {
     AttnTcArgs t = {};
     t.a = a;
-    if (dtype == TD_F16)
-        return a.D <= 64 ? backward<__half, 64>(t, w, mb, mh, workspace, stream, err, err_len)
-                         : backward<__half, 128>(t, w, mb, mh, workspace, stream, err, err_len);
-    return a.D <= 64 ? backward<__nv_bfloat16, 64>(t, w, mb, mh, workspace, stream, err, err_len)
-                     : backward<__nv_bfloat16, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+    auto go = [&](auto type) {
+        using T = decltype(type);
+        if (a.D <= 32) return backward<T, 32>(t, w, mb, mh, workspace, stream, err, err_len);
+        if (a.D <= 64) return backward<T, 64>(t, w, mb, mh, workspace, stream, err, err_len);
+        return backward<T, 128>(t, w, mb, mh, workspace, stream, err, err_len);
+    };
+    return dtype == TD_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
 
 }  // namespace td

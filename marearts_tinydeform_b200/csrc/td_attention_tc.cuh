@@ -48,6 +48,19 @@ struct AttnTcArgs {
 
 constexpr int kAttnBM = 128, kAttnBN = 64;
 
+// An operand tile in shared memory: boxes of min(DP, 64) columns, rows of 64 bytes (64-byte swizzle, DP = 32) or 128
+// bytes (128-byte swizzle), in atoms of 8 rows.
+template <int DP>
+struct AttnBox {
+    static constexpr int kCols = DP < 64 ? DP : 64;
+    static constexpr int kBoxes = DP / kCols;
+    static constexpr uint32_t kRow = kCols * 2;
+    static constexpr uint32_t kFixed = kAttnBM * kRow;  // a box of the resident operand
+    static constexpr uint32_t kTile = kAttnBN * kRow;   // a box of a streamed tile
+    static constexpr int kSteps = kCols / 16;           // K steps of a box
+    static_assert(DP == 32 || DP == 64 || DP == 128, "head width");
+};
+
 // ---- PTX ----------------------------------------------------------------------------------------------------------
 // The MMA warps stay converged: every lane forms the (equal) operands, which the compiler so keeps in uniform registers,
 // and the lane with `leader` set issues. Inside a branch that one lane takes, each descriptor would be moved there anew,
@@ -223,22 +236,33 @@ __device__ __forceinline__ constexpr uint32_t attn_idesc(int N) {
     return idesc_f16(std::is_same<T, __nv_bfloat16>::value, 128, N) | (uint32_t(B_MN) << 16);
 }
 
-// MN-major operand made of boxes of 64 rows (of K) by 64 columns: next 8 K rows 1024 bytes on, next 64 columns
-// 64 * 128 bytes on.
-__device__ __forceinline__ uint64_t sdesc_mn64(uint32_t saddr) {
-    uint64_t d = sdesc_sw128(saddr);
-    d |= uint64_t(8192 >> 4) << 16;
+// K-major operand: atoms of 8 rows stacked along M / N.
+template <int DP>
+__device__ __forceinline__ uint64_t sdesc_k(uint32_t saddr) {
+    if constexpr (DP >= 64) return sdesc_sw128(saddr);
+    uint64_t d = uint64_t((saddr & 0x3FFFFu) >> 4);
+    d |= uint64_t(512 >> 4) << 32;
+    d |= uint64_t(1) << 46;
+    d |= uint64_t(4) << 61;  // SWIZZLE_64B
     return d;
 }
 
-// D = A x B^T over DP columns: A 128 rows, B 64 rows, both K-major in boxes of 64 columns.
+// MN-major operand made of boxes of 64 rows (of K): the next 8 K rows an atom on, the next 64 columns a box on.
+template <int DP>
+__device__ __forceinline__ uint64_t sdesc_mn(uint32_t saddr) {
+    return sdesc_k<DP>(saddr) | uint64_t(AttnBox<DP>::kTile >> 4) << 16;
+}
+
+// D = A x B^T over DP columns: A 128 rows, B 64 rows, both K-major.
 template <typename T, int DP>
 __device__ __forceinline__ void issue_scores(uint32_t leader, uint32_t d, uint32_t a_smem, uint32_t b_smem) {
+    using Box = AttnBox<DP>;
     constexpr uint32_t idesc = attn_idesc<T, false>(kAttnBN);
 #pragma unroll
     for (int k = 0; k < DP / 16; ++k) {
-        const uint64_t da = sdesc_sw128(a_smem + (k / 4) * 16384) + uint64_t(2 * (k % 4));
-        const uint64_t db = sdesc_sw128(b_smem + (k / 4) * 8192) + uint64_t(2 * (k % 4));
+        const int box = k / Box::kSteps, step = k % Box::kSteps;
+        const uint64_t da = sdesc_k<DP>(a_smem + box * Box::kFixed) + uint64_t(2 * step);
+        const uint64_t db = sdesc_k<DP>(b_smem + box * Box::kTile) + uint64_t(2 * step);
         mma_ss(leader, d, da, db, idesc, k != 0);
     }
 }
@@ -248,13 +272,13 @@ template <typename T, int DP>
 __device__ __forceinline__ void issue_product(uint32_t leader, uint32_t acc, uint32_t a_tmem, uint32_t b_smem,
                                               bool first) {
     constexpr uint32_t idesc = attn_idesc<T, true>(DP);
-    const uint64_t db = sdesc_mn64(b_smem);
+    const uint64_t db = sdesc_mn<DP>(b_smem);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        mma_ts(leader, acc, a_tmem + 8 * k, db + uint64_t(128 * k), idesc, !(first && k == 0));
+        mma_ts(leader, acc, a_tmem + 8 * k, db + uint64_t(AttnBox<DP>::kRow * k), idesc, !(first && k == 0));
 }
 
-// Clears the rows of padded keys in a slot's tile of 64 rows x DP columns (boxes of 64 rows x 128 bytes). One warp.
+// Clears the rows of padded keys in a slot's tile of 64 rows x DP columns. One warp.
 template <int DP>
 __device__ __forceinline__ void clear_padded(unsigned char* tile, const uint8_t* pad, int j0, int N) {
     const int lane = threadIdx.x & 31;
@@ -265,8 +289,9 @@ __device__ __forceinline__ void clear_padded(unsigned char* tile, const uint8_t*
         const int r = __ffsll((long long)rows) - 1;
         rows &= rows - 1;
 #pragma unroll
-        for (int box = 0; box < DP / 64; ++box)  // a whole 128-byte row: the swizzle only permutes inside it
-            *reinterpret_cast<uint32_t*>(tile + box * 8192 + r * 128 + lane * 4) = 0u;
+        for (int box = 0; box < AttnBox<DP>::kBoxes; ++box)  // a whole row: the swizzle only permutes inside it
+            if (uint32_t(lane) * 4 < AttnBox<DP>::kRow)
+                *reinterpret_cast<uint32_t*>(tile + box * AttnBox<DP>::kTile + r * AttnBox<DP>::kRow + lane * 4) = 0u;
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -275,10 +300,10 @@ __device__ __forceinline__ void clear_padded(unsigned char* tile, const uint8_t*
 // ---- forward ------------------------------------------------------------------------------------------------------
 template <int DP>
 struct AttnFwdLayout {
-    static constexpr int kBoxes = DP / 64;
-    static constexpr uint32_t kQBytes = kAttnBM * 128 * kBoxes;
-    static constexpr uint32_t kTileBytes = kAttnBN * 128 * kBoxes;  // of K or of V
-    static constexpr int kStages = DP == 64 ? 4 : 2;                // two CTAs an SM
+    static constexpr int kBoxes = AttnBox<DP>::kBoxes;
+    static constexpr uint32_t kQBytes = AttnBox<DP>::kFixed * kBoxes;
+    static constexpr uint32_t kTileBytes = AttnBox<DP>::kTile * kBoxes;  // of K or of V
+    static constexpr int kStages = DP == 128 ? 2 : 4;                    // two CTAs an SM
     static constexpr uint32_t kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kRing = kQBytes;
     static constexpr uint32_t kBars = kRing + kStages * kStageBytes;
@@ -357,7 +382,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         const uint64_t pol = l2_evict_last();  // keys and values are read again by the other query tiles
         if (lane < KB && tiles > 0) {
             mbar_arrive_expect_tx(qfull, Lay::kQBytes / KB);
-            tma_load_4d(smem + lane * 16384, &map_q, qfull, 64 * lane, i0, h, b, l2_evict_first());
+            tma_load_4d(smem + lane * AttnBox<DP>::kFixed, &map_q, qfull, 64 * lane, i0, h, b, l2_evict_first());
         }
         int n = 0;
         for_tiles(0, tiles, flags, [&](int t, bool) {
@@ -366,8 +391,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             const int job = lane - 2 * KB * s, box = job % KB;
             if (job >= 0 && job < 2 * KB) {
                 uint64_t* bar = job < KB ? &kfull[s] : &vfull[s];
-                mbar_arrive_expect_tx(bar, 8192u);
-                tma_load_4d((job < KB ? k_tile(s) : v_tile(s)) + box * 8192, job < KB ? &map_k : &map_v, bar,
+                mbar_arrive_expect_tx(bar, AttnBox<DP>::kTile);
+                tma_load_4d((job < KB ? k_tile(s) : v_tile(s)) + box * AttnBox<DP>::kTile, job < KB ? &map_k : &map_v, bar,
                             64 * box, t * kAttnBN, hk, b, pol);
             }
             __syncwarp();
@@ -566,13 +591,13 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
 // ---- backward -----------------------------------------------------------------------------------------------------
 template <int DP>
 struct AttnBwdLayout {
-    static constexpr int kBoxes = DP / 64;
-    static constexpr uint32_t kFixedBytes = kAttnBM * 128 * kBoxes;  // one resident operand
-    static constexpr uint32_t kTileBytes = kAttnBN * 128 * kBoxes;   // one streamed operand
+    static constexpr int kBoxes = AttnBox<DP>::kBoxes;
+    static constexpr uint32_t kFixedBytes = AttnBox<DP>::kFixed * kBoxes;  // one resident operand
+    static constexpr uint32_t kTileBytes = AttnBox<DP>::kTile * kBoxes;    // one streamed operand
     // score buffers (S and dP, 64 columns each) and ring slots: with a buffer more than there are warpgroups, each finds
     // its next tile's scores formed when it is done with one; wide heads' accumulators leave TMEM for two buffers
-    static constexpr int kBufs = DP == 64 ? 3 : 2;
-    static constexpr int kStages = DP == 64 ? 6 : 4;
+    static constexpr int kBufs = DP == 128 ? 2 : 3;
+    static constexpr int kStages = DP == 128 ? 4 : 6;
     static constexpr uint32_t kAcc = kBufs * 128;  // first accumulator's TMEM column
     static constexpr uint32_t kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kRing = 2 * kFixedBytes;
@@ -694,8 +719,8 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         const uint64_t pol = l2_evict_last();
         if (lane < 2 * KB) {
             const int box = lane % KB;
-            mbar_arrive_expect_tx(fixed, 16384u);
-            tma_load_4d(smem + (lane / KB) * Lay::kFixedBytes + box * 16384, lane < KB ? &map_fixed1 : &map_fixed2,
+            mbar_arrive_expect_tx(fixed, AttnBox<DP>::kFixed);
+            tma_load_4d(smem + (lane / KB) * Lay::kFixedBytes + box * AttnBox<DP>::kFixed, lane < KB ? &map_fixed1 : &map_fixed2,
                         fixed, 64 * box, r0, head, b, pol);
         }
         int n = 0;
@@ -706,8 +731,8 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             static_assert(kJobs * S <= 32, "a lane per copy of the ring");
             const int job = lane - kJobs * s, box = job % KB;
             if (job >= 0 && job < 2 * KB) {
-                mbar_arrive_expect_tx(&full[s], 8192u);
-                tma_load_4d((job < KB ? tile1(s) : tile2(s)) + box * 8192, job < KB ? &map_b1 : &map_b2, &full[s],
+                mbar_arrive_expect_tx(&full[s], AttnBox<DP>::kTile);
+                tma_load_4d((job < KB ? tile1(s) : tile2(s)) + box * AttnBox<DP>::kTile, job < KB ? &map_b1 : &map_b2, &full[s],
                             64 * box, t * kAttnBN, KEYS ? h : hk, b, pol);
             } else if (job >= 2 * KB && job < kJobs) {
                 const float* src = static_cast<const float*>(job == 2 * KB ? a.lse : a.delta);
