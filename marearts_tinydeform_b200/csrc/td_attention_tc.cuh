@@ -210,10 +210,15 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, unsign
 // until f returns false. flags: one byte a tile, or null (every tile, all open).
 template <typename F>
 __device__ __forceinline__ bool for_tiles(int t0, int t1, const uint8_t* flags, F&& f) {
+    if (flags == nullptr) {
+        for (int t = t0; t < t1; ++t)
+            if (!f(t, true)) return false;
+        return true;
+    }
     const int lane = threadIdx.x & 31;
     for (int base = t0; base < t1; base += 32) {
         const int t = base + lane;
-        const unsigned fl = t >= t1 ? 0u : flags != nullptr ? unsigned(__ldg(flags + t)) : 3u;
+        const unsigned fl = t >= t1 ? 0u : unsigned(__ldg(flags + t));
         unsigned any = __ballot_sync(0xffffffffu, (fl & 1u) != 0);
         const unsigned all = __ballot_sync(0xffffffffu, (fl & 2u) != 0);
         while (any != 0) {
@@ -827,8 +832,8 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                 }
             }
             const int u = m % NB;
-            if (KEYS && !warp_wait(&full[m % S], uint32_t((m / S) & 1), kErrTmaWait)) return false;  // the statistics
             if (!warp_wait(&sfull[u], uint32_t((m / NB) & 1), kErrMmaWait)) return false;
+            if (KEYS && !warp_wait(&full[m % S], uint32_t((m / S) & 1), kErrTmaWait)) return false;  // the statistics
             tc_fence_after();
             const uint32_t sc = lanes + 128 * u;
             // 16 columns at a time, the next ones' loads in flight meanwhile; P and dS go where the first scores were
