@@ -230,6 +230,24 @@ __device__ __forceinline__ bool for_tiles(int t0, int t1, const uint8_t* flags, 
     return true;
 }
 
+// A place in a ring of N and the parity of its round, stepped instead of divided: on a warp alone on its scheduler every
+// instruction between two tiles shows.
+template <int N>
+struct Ring {
+    int at = 0;
+    uint32_t parity = 0;
+    __device__ __forceinline__ explicit Ring(int start = 0) : at(start) {}
+    template <int STEP = 1>
+    __device__ __forceinline__ void step() {
+        static_assert(STEP <= N, "at most a round");
+        at += STEP;
+        if (at >= N) {
+            at -= N;
+            parity ^= 1u;
+        }
+    }
+};
+
 // Bits of [0, 64) below `n` (n may be negative or above 64).
 __device__ __forceinline__ unsigned long long bits_below(int n) {
     return n <= 0 ? 0ull : n >= 64 ? ~0ull : (1ull << n) - 1ull;
@@ -390,9 +408,11 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             tma_load_4d(smem + lane * AttnBox<DP>::kFixed, &map_q, qfull, 64 * lane, i0, h, b, l2_evict_first());
         }
         int n = 0;
+        Ring<S> ring;
         for_tiles(0, tiles, flags, [&](int t, bool) {
-            const int s = n % S;
-            if (!warp_wait(&empty[s], uint32_t((n / S) & 1) ^ 1u, kErrSlotWait)) return false;
+            const int s = ring.at;
+            if (!warp_wait(&empty[s], ring.parity ^ 1u, kErrSlotWait)) return false;
+            ring.template step<>();
             const int job = lane - 2 * KB * s, box = job % KB;
             if (job >= 0 && job < 2 * KB) {
                 uint64_t* bar = job < KB ? &kfull[s] : &vfull[s];
@@ -412,38 +432,43 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             }
     } else if (warp == 1) {
         const uint32_t leader = lane == 0;
-        int n = 0;
+        Ring<S> ring;
+        Ring<2> buf;
         if (tiles == 0 || warp_wait(qfull, 0u, kErrTmaWait))
             for_tiles(0, tiles, flags, [&](int, bool) {
-                const int s = n % S;
-                if (!warp_wait(&kfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
-                // the buffer's P before these scores has been read by its product
-                if (n >= 2 && !warp_wait(&done[n & 1], uint32_t((n / 2 - 1) & 1), kErrMmaWait)) return false;
+                if (!warp_wait(&kfull[ring.at], ring.parity, kErrTmaWait)) return false;
+                // the buffer's P before these scores (none in the first round) has been read by its product
+                if (!warp_wait(&done[buf.at], buf.parity ^ 1u, kErrMmaWait)) return false;
                 tc_fence_after();
-                issue_scores<T, DP>(leader, tmem + 64 * (n & 1), smem_addr(smem), smem_addr(k_tile(s)));
-                commit(leader, &sfull[n & 1]);
-                ++n;
+                issue_scores<T, DP>(leader, tmem + 64 * buf.at, smem_addr(smem), smem_addr(k_tile(ring.at)));
+                commit(leader, &sfull[buf.at]);
+                ring.template step<>();
+                buf.template step<>();
                 return true;
             });
     } else if (warp == 2) {
         const uint32_t leader = lane == 0;
         const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
-        int n = 0;
+        bool first = true;
+        Ring<S> ring;
+        Ring<2> buf;
         const bool ok = for_tiles(0, tiles, flags, [&](int t, bool all) {
-            const int s = n % S;
-            if (!warp_wait(&vfull[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
-            if (pad != nullptr && !all) clear_padded<DP>(v_tile(s), pad, t * kAttnBN, a.N);
-            if (!warp_wait(&pfull[n & 1], uint32_t((n >> 1) & 1), kErrMmaWait)) return false;
+            unsigned char* v = v_tile(ring.at);
+            if (!warp_wait(&vfull[ring.at], ring.parity, kErrTmaWait)) return false;
+            if (pad != nullptr && !all) clear_padded<DP>(v, pad, t * kAttnBN, a.N);
+            if (!warp_wait(&pfull[buf.at], buf.parity, kErrMmaWait)) return false;
             tc_fence_after();
-            issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (n & 1), smem_addr(v_tile(s)), n == 0);
-            if constexpr (EXACT)
-                issue_product<T, DP>(leader, tmem + 128, tmem + 64 * (n & 1) + 32, smem_addr(v_tile(s)), false);
-            commit(leader, &empty[s]);
-            commit(leader, &done[n & 1]);
-            ++n;
+            const uint32_t p = tmem + 64 * buf.at;
+            issue_product<T, DP>(leader, tmem + 128, p, smem_addr(v), first);
+            if constexpr (EXACT) issue_product<T, DP>(leader, tmem + 128, p + 32, smem_addr(v), false);
+            commit(leader, &empty[ring.at]);
+            commit(leader, &done[buf.at]);
+            first = false;
+            ring.template step<>();
+            buf.template step<>();
             return true;
         });
-        if (ok && n > 0) commit(leader, finished);
+        if (ok && !first) commit(leader, finished);
     } else {
         const int quarter = warp & 3, i = i0 + quarter * 32 + lane;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
@@ -456,6 +481,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                                    : args.row_bits + b * args.rb_b + h * args.rb_h + min(i, a.Q - 1) * args.rb_q;
         float ref = -INFINITY, sum = 0.f;
         int n = 0;
+        Ring<2> buf;
         const bool ok = for_tiles(0, tiles, flags, [&](int t, bool all) {
             const int j0 = t * kAttnBN;
             const bool open = all && j0 + kAttnBN <= a.N && (!a.causal || j0 + kAttnBN - 1 <= i0 + off);
@@ -468,9 +494,9 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                     w &= (unsigned long long)x.y << 32 | x.x;
                 }
             }
-            if (!warp_wait(&sfull[n & 1], uint32_t((n >> 1) & 1), kErrMmaWait)) return false;
+            if (!warp_wait(&sfull[buf.at], buf.parity, kErrMmaWait)) return false;
             tc_fence_after();
-            const uint32_t sc = lanes + 64 * (n & 1);
+            const uint32_t sc = lanes + 64 * buf.at;
             uint32_t v[2][32];
             tmem_ld_32x32b_x32(sc, v[0]);
             tmem_ld_32x32b_x32(sc + 32, v[1]);
@@ -540,7 +566,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&pfull[n & 1]);
+            if (lane == 0) mbar_arrive(&pfull[buf.at]);
+            buf.template step<>();
             ++n;
             return true;
         });
@@ -729,9 +756,11 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                         fixed, 64 * box, r0, head, b, pol);
         }
         int n = 0;
+        Ring<S> ring;
         each_tile([&](int h, int t, bool) {
-            const int s = n % S;
-            if (!warp_wait(&empty[s], uint32_t((n / S) & 1) ^ 1u, kErrSlotWait)) return false;
+            const int s = ring.at;
+            if (!warp_wait(&empty[s], ring.parity ^ 1u, kErrSlotWait)) return false;
+            ring.template step<>();
             constexpr int kJobs = 2 * KB + (KEYS ? 2 : 0);
             static_assert(kJobs * S <= 32, "a lane per copy of the ring");
             const int job = lane - kJobs * s, box = job % KB;
@@ -755,42 +784,47 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                 warp_wait(&full[i % S], uint32_t((i / S) & 1), kErrTmaWait);
     } else if (warp == 1) {
         const uint32_t leader = lane == 0;
-        int n = 0;
+        Ring<S> ring;
+        Ring<NB> buf;
         if (warp_wait(fixed, 0u, kErrTmaWait))
             each_tile([&](int, int, bool) {
-                const int s = n % S, u = n % NB;
-                if (!warp_wait(&full[s], uint32_t((n / S) & 1), kErrTmaWait)) return false;
-                // the buffer's P and dS before these scores have been read by their products
-                if (n >= NB && !warp_wait(&done[u], uint32_t((n / NB - 1) & 1), kErrMmaWait)) return false;
+                if (!warp_wait(&full[ring.at], ring.parity, kErrTmaWait)) return false;
+                // the buffer's P and dS before these scores (none in the first round) have been read by their products
+                if (!warp_wait(&done[buf.at], buf.parity ^ 1u, kErrMmaWait)) return false;
                 tc_fence_after();
-                const uint32_t sc = tmem + 128 * u;
-                issue_scores<T, DP>(leader, sc, smem_addr(smem), smem_addr(tile1(s)));
-                issue_scores<T, DP>(leader, sc + 64, smem_addr(smem + Lay::kFixedBytes), smem_addr(tile2(s)));
-                commit(leader, &sfull[u]);
-                ++n;
+                const uint32_t sc = tmem + 128 * buf.at;
+                issue_scores<T, DP>(leader, sc, smem_addr(smem), smem_addr(tile1(ring.at)));
+                issue_scores<T, DP>(leader, sc + 64, smem_addr(smem + Lay::kFixedBytes), smem_addr(tile2(ring.at)));
+                commit(leader, &sfull[buf.at]);
+                if (lane == 0) mbar_arrive(&sfull[buf.at]);  // for the statistics, which this warp's wait has seen land
+                ring.template step<>();
+                buf.template step<>();
                 return true;
             });
     } else if (warp == 2) {
         const uint32_t leader = lane == 0;
         const uint8_t* pad = KEYS || a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
-        int n = 0;
+        bool first = true;
+        Ring<S> ring;
+        Ring<NB> buf;
         const bool ok = each_tile([&](int, int t, bool all) {
-            const int s = n % S, u = n % NB;
-            const uint32_t sc = tmem + 128 * u;
-            if (!warp_wait(&pfull[u], uint32_t((n / NB) & 1), kErrMmaWait)) return false;
+            const uint32_t sc = tmem + 128 * buf.at;
+            if (!warp_wait(&pfull[buf.at], buf.parity, kErrMmaWait)) return false;
             // (this tile's scores are formed: what they made of padded rows has been replaced)
-            if (pad != nullptr && !all) clear_padded<DP>(tile1(s), pad, t * kAttnBN, a.N);
+            if (pad != nullptr && !all) clear_padded<DP>(tile1(ring.at), pad, t * kAttnBN, a.N);
             tc_fence_after();
-            if constexpr (KEYS)
-                issue_product<T, DP>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(s)), n == 0);  // dV += P^T dO
+            if constexpr (KEYS)  // dV += P^T dO
+                issue_product<T, DP>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(ring.at)), first);
             // dK += dS^T Q, dQ += dS K
-            issue_product<T, DP>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(s)), n == 0);
-            commit(leader, &empty[s]);
-            commit(leader, &done[u]);
-            ++n;
+            issue_product<T, DP>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(ring.at)), first);
+            commit(leader, &empty[ring.at]);
+            commit(leader, &done[buf.at]);
+            first = false;
+            ring.template step<>();
+            buf.template step<>();
             return true;
         });
-        if (ok && n > 0) commit(leader, finished);
+        if (ok && !first) commit(leader, finished);
     } else if (warp >= 4) {
         const int quarter = warp & 3, wg = (warp - 4) >> 2, r = r0 + quarter * 32 + lane;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
@@ -802,10 +836,12 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             row_lse = static_cast<const float*>(a.lse)[at];
             row_delta = static_cast<const float*>(a.delta)[at];
         }
+        // this warpgroup takes every other tile
         int n = 0;
+        Ring<S> ring(wg);
+        Ring<NB> buf(wg);
         bool ok = each_tile([&](int h, int t, bool all) {
-            const int m = n++;
-            if ((m & 1) != wg) return true;
+            if ((n++ & 1) != wg) return true;
             const int c0 = t * kAttnBN;  // the tile's first column: a query (KEYS) or a key
             bool open = all;
             unsigned long long w = ~0ull;
@@ -831,20 +867,20 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                     }
                 }
             }
-            const int u = m % NB;
-            if (!warp_wait(&sfull[u], uint32_t((m / NB) & 1), kErrMmaWait)) return false;
-            if (KEYS && !warp_wait(&full[m % S], uint32_t((m / S) & 1), kErrTmaWait)) return false;  // the statistics
+            if (!warp_wait(&sfull[buf.at], buf.parity, kErrMmaWait)) return false;
             tc_fence_after();
-            const uint32_t sc = lanes + 128 * u;
+            const uint32_t sc = lanes + 128 * buf.at;
             // 16 columns at a time, the next ones' loads in flight meanwhile; P and dS go where the first scores were
             if (open)
-                elementwise<T, KEYS, false>(sc, stats(m % S), row_lse, row_delta, c, ds_scale, w);
+                elementwise<T, KEYS, false>(sc, stats(ring.at), row_lse, row_delta, c, ds_scale, w);
             else
-                elementwise<T, KEYS, true>(sc, stats(m % S), row_lse, row_delta, c, ds_scale, w);
+                elementwise<T, KEYS, true>(sc, stats(ring.at), row_lse, row_delta, c, ds_scale, w);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&pfull[u]);
+            if (lane == 0) mbar_arrive(&pfull[buf.at]);
+            ring.template step<2>();
+            buf.template step<2>();
             return true;
         });
         ok = ok && (n == 0 || warp_wait(finished, 0u, kErrMmaWait));
@@ -906,7 +942,7 @@ __global__ void __launch_bounds__(kAttnBwdThreads, 1)
             mbar_init(&empty[s], 1);
         }
         for (int g = 0; g < NB; ++g) {
-            mbar_init(&sfull[g], 1);
+            mbar_init(&sfull[g], 2);
             mbar_init(&pfull[g], 4);  // as in the forward
             mbar_init(&done[g], 1);
         }
