@@ -152,7 +152,7 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
     constexpr size_t smem = AttnBwdLayout<DP>::kSmemBytes;
     if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
     const unsigned grid = unsigned(t.kv_blocks) + unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
-    return host::launch(err, err_len, "attn_tc_backward_kernel", kernel, dim3(grid), dim3(kAttnBwdThreads), smem, stream,
+    return host::launch(err, err_len, "attn_tc_backward_kernel", kernel, dim3(grid), dim3(AttnBwdLayout<DP>::kThreads), smem, stream,
                         true, fixed[0], fixed[1], fixed[2], fixed[3], tile[0], tile[1], tile[2], tile[3], t);
 }
 

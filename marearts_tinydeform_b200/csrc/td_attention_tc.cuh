@@ -626,11 +626,16 @@ struct AttnBwdLayout {
     static constexpr int kBoxes = AttnBox<DP>::kBoxes;
     static constexpr uint32_t kFixedBytes = AttnBox<DP>::kFixed * kBoxes;  // one resident operand
     static constexpr uint32_t kTileBytes = AttnBox<DP>::kTile * kBoxes;    // one streamed operand
-    // score buffers (S and dP, 64 columns each) and ring slots: with a buffer more than there are warpgroups, each finds
-    // its next tile's scores formed when it is done with one; wide heads' accumulators leave TMEM for two buffers
+    // score buffers (S and dP, 64 columns each) and ring slots. A buffer goes from the scores' product through the
+    // elementwise work to the products that read P and dS, about 2000 cycles in all, so the tiles in flight set the pace:
+    // three where TMEM holds them, two beside the accumulators of wide heads
     static constexpr int kBufs = DP == 128 ? 2 : 3;
     static constexpr int kStages = DP == 128 ? 4 : 6;
     static constexpr uint32_t kAcc = kBufs * 128;  // first accumulator's TMEM column
+    // warpgroups of the elementwise work: three overlap their waits best where the products are short (encoder, D = 32:
+    // 498 us against 529 with two), two where those share the time (D = 64: 271 against 278)
+    static constexpr int kGroups = DP == 32 ? 3 : 2;
+    static constexpr int kThreads = 128 * (1 + kGroups);  // loads, scores, products, -, the warpgroups
     static constexpr uint32_t kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kRing = 2 * kFixedBytes;
     static constexpr uint32_t kStats = kRing + kStages * kStageBytes;  // per stage: lse[64], delta[64]
@@ -644,7 +649,6 @@ struct AttnBwdLayout {
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
-constexpr int kAttnBwdThreads = 384;  // loads, scores, products, -, two elementwise warpgroups
 
 // float16 keeps dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
 // gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs no scale.
@@ -836,12 +840,15 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             row_lse = static_cast<const float*>(a.lse)[at];
             row_delta = static_cast<const float*>(a.delta)[at];
         }
-        // this warpgroup takes every other tile
-        int n = 0;
+        // the warpgroups take the tiles in turn
+        constexpr int NG = Lay::kGroups;
+        int n = 0, turn = wg;
         Ring<S> ring(wg);
         Ring<NB> buf(wg);
         bool ok = each_tile([&](int h, int t, bool all) {
-            if ((n++ & 1) != wg) return true;
+            ++n;
+            if (turn-- != 0) return true;
+            turn = NG - 1;
             const int c0 = t * kAttnBN;  // the tile's first column: a query (KEYS) or a key
             bool open = all;
             unsigned long long w = ~0ull;
@@ -879,14 +886,14 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&pfull[buf.at]);
-            ring.template step<2>();
-            buf.template step<2>();
+            ring.template step<NG>();
+            buf.template step<NG>();
             return true;
         });
         ok = ok && (n == 0 || warp_wait(finished, 0u, kErrMmaWait));
         tc_fence_after();
         // the gradients' rows: a warpgroup an accumulator for the keys' block, else half of the columns each
-        if (ok) {
+        if (ok && wg < 2) {
             const bool is_v = KEYS && wg == 1;
             const float f = is_v ? 1.f : float(a.scale) / ds_scale;
             const bool gone = KEYS && a.padding != nullptr && r < a.N && a.padding[(long long)b * a.N + r] != 0;
@@ -921,7 +928,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAttnBwdThreads, 1)
+__global__ void __launch_bounds__(AttnBwdLayout<DP>::kThreads, 1)
     attn_tc_backward_kernel(const __grid_constant__ CUtensorMap q128, const __grid_constant__ CUtensorMap g128,
                             const __grid_constant__ CUtensorMap k128, const __grid_constant__ CUtensorMap v128,
                             const __grid_constant__ CUtensorMap q64, const __grid_constant__ CUtensorMap g64,
