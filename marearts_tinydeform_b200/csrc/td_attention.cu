@@ -1,6 +1,5 @@
 // td_attention.cu -- the attention entry points of the C ABI: argument contract, kernel choice and launches.
 #include <algorithm>
-#include <cstdlib>
 
 #include "td_attention_plan.h"
 
@@ -22,11 +21,13 @@ void split_plan(int64_t blocks, int64_t N, int64_t waves, int64_t least, int64_t
     p->splits = int(std::max<int64_t>(1, (N + p->split_keys - 1) / p->split_keys));
 }
 
-// The mma.sync split kernel's plan: the rows of a key head's group in tiles of 16.
-SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk) {
+// The mma.sync split kernel's plan: the rows of a key head's group in tiles of 16. One wave of long splits where every
+// image has all its keys; shorter ones where some have not, so that the CTAs of the full ones do not end last (8 images
+// of 22223 keys, the lengths falling to half: 48 us with 2, 42 with 6; all of them full: 43 and 43; one image: 12 and 17).
+SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, bool padding) {
     SplitArgs p = {};
     p.row_tiles = int((H / Hk * Q + 15) / 16);
-    split_plan(B * Hk * p.row_tiles, N, 8, 256, 128, &p);
+    split_plan(B * Hk * p.row_tiles, N, padding ? 6 : 2, 256, 128, &p);
     return p;
 }
 
@@ -62,7 +63,7 @@ AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t
         w.delta = take(size_t(B) * H * pad_rows(Q) * acc);
     } else {
         int64_t splits = simt_split_plan(dtype, B, Q, N, H, D).splits;
-        if (half) splits = std::max<int64_t>(splits, mma_split_plan(B, Q, N, H, Hk).splits);
+        if (half) splits = std::max<int64_t>(splits, mma_split_plan(B, Q, N, H, Hk, padding).splits);
         if (splits > 1) {
             w.part_o = take(size_t(B) * H * Q * splits * D * acc);
             w.part_ml = take(size_t(B) * H * Q * splits * 2 * acc);
@@ -142,8 +143,8 @@ template <typename T>
 int combine(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
     if (p.splits == 1) return TD_OK;
     const long long rows = (long long)p.a.B * p.a.H * p.a.Q;
-    return host::launch(err, err_len, "attn_combine_kernel", attn_combine_kernel<T>, dim3(unsigned((rows + 3) / 4)),
-                        dim3(128), 0, stream, true, p);
+    return host::launch(err, err_len, "attn_combine_kernel", attn_combine_kernel<T>, dim3(unsigned(rows)),
+                        dim3(kCombineWarps * 32), 0, stream, true, p);
 }
 
 template <typename T, int DP, int RM>
@@ -174,8 +175,11 @@ int simt_forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned 
 template <typename T, int DP, bool EXACT>
 int mma_split(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
     const long long grid = (long long)p.splits * p.row_tiles * p.a.B * p.a.Hk;
-    if (int rc = host::launch(err, err_len, "attn_split_kernel", attn_split_kernel<T, DP, EXACT>,
-                              dim3(unsigned(grid)), dim3(kSplitWarps * 32), 0, stream, true, p))
+    auto kernel = attn_split_kernel<T, DP, EXACT>;
+    constexpr size_t smem = SplitLayout<DP>::kSmem;
+    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    if (int rc = host::launch(err, err_len, "attn_split_kernel", kernel, dim3(unsigned(grid)),
+                              dim3(kSplitWarps * 32), smem, stream, true, p))
         return rc;
     return combine<T>(p, stream, err, err_len);
 }
@@ -183,7 +187,7 @@ int mma_split(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len
 template <typename T>
 int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* workspace, cudaStream_t stream,
                       char* err, size_t err_len) {
-    SplitArgs p = mma_split_plan(a.B, a.Q, a.N, a.H, a.Hk);
+    SplitArgs p = mma_split_plan(a.B, a.Q, a.N, a.H, a.Hk, a.padding != nullptr);
     p.a = a;
     p.part_o = workspace + w.part_o;
     p.part_ml = workspace + w.part_ml;
@@ -196,11 +200,19 @@ int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* 
     return a.rest != nullptr ? go(std::true_type{}) : go(std::false_type{});
 }
 
-// Whether the split kernel takes a 16-bit forward that the tensor-core kernels could take as well.
+// Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. In microseconds, as
+// measured on B200 over 1 to 16 images, 8 and 16 heads, D = 32, 64 and 128, 40 to 22223 keys and 1 to 300 queries:
+// the tensor-core kernel walks all keys of a 128-query tile in one CTA, about 10 ns a key (13 for wide heads) and wave of
+// 296 CTAs; the split kernel's time goes with its 16-row tiles times keys, behind about 7 for two launches. Below 1024
+// keys the two differ by little (300 keys, one query: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128). Where the
+// estimates are near each other so are the kernels (at most a fifth apart where the wrong one is taken).
 bool prefer_split(const AttnArgs& a) {
-    const char* e = getenv("ATTN_SPLIT");
-    if (e) return e[0] == '1';
-    return a.H / a.Hk * a.Q <= 16;
+    if (a.N < 1024) return false;
+    const double ctas = double((a.Q + 127) / 128) * a.B * a.H;
+    const double tiles = double((a.H / a.Hk * (long long)a.Q + 15) / 16) * a.B * a.Hk;
+    const double walk = 3.3 + 0.0103 * a.N * (a.D > 64 ? 1.25 : 1.0) * std::max(1.0, ctas / (2 * kSms));
+    const double split = 7.0 + tiles * a.N * (a.D <= 32 ? 5e-5 : a.D <= 64 ? 9e-5 : 1.8e-4);
+    return split < walk;
 }
 
 template <typename T, int DP>

@@ -6,12 +6,13 @@
 // sets and their order follow from the sizes alone, so the result is the same every time.
 //
 // Bound by reading K and V once, from HBM. A tile has 16 rows: the queries of a key head's whole group of query heads,
-// so shared keys are read once for all of them. Each warp streams its own keys straight from global memory into the
-// registers of mma.sync fragments, with 16-byte loads and no shared memory: the order of the summed index is free, so
-// a thread's 8 consecutive elements of a key row are two K steps' fragments (the queries are loaded in the same
-// order), and a thread's consecutive elements of a value row are the same column of as many 8-wide result tiles; the
-// pairs of keys that a value fragment packs are made with byte permutes. Tensor cores matter little here, but a
-// 16-row product on them costs what a one-row product on CUDA cores would.
+// so shared keys are read once for all of them. Each warp streams its own keys through a ring of its own in shared
+// memory (asynchronous 16-byte copies, two steps ahead, nothing shared between warps until the end) into mma.sync
+// fragments: the order of the summed index is free, so a thread's 8 consecutive elements of a key row are two K steps'
+// fragments (the queries are loaded in the same order), and a thread's consecutive elements of a value row are the
+// same column of as many 8-wide result tiles; the pairs of keys that a value fragment packs are made with byte
+// permutes. Tensor cores matter little here, but a 16-row product on them costs what a one-row product on CUDA cores
+// would.
 #pragma once
 
 #include "td_attention.cuh"
@@ -26,7 +27,27 @@ struct SplitArgs {
     void *part_o, *part_ml;
 };
 
-constexpr int kSplitWarps = 4;
+constexpr int kSplitWarps = 4, kSplitStages = 3;
+
+// A warp's ring slot: keys a step, K rows then V rows, padded so that rows fall on different banks.
+template <int DP>
+struct SplitLayout {
+    static constexpr int kKeys = DP == 128 ? 16 : 32;
+    static constexpr int kPitch = DP * 2 + 16;
+    static constexpr int kStage = 2 * kKeys * kPitch;
+    static constexpr int kJoin = kSplitWarps * 16 * (DP + 4) * 4;  // the warps' results take the ring's place
+    static constexpr int kRing = kSplitWarps * kSplitStages * kStage;
+    static constexpr size_t kSmem = kRing > kJoin ? kRing : kJoin;
+};
+
+// 16 bytes from global to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
 
 // The result's row `row` (of B * H * Q, head-major): o / l rounded, what the rounding took, and lse.
 template <typename T, typename A>
@@ -66,6 +87,12 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+__device__ __forceinline__ float fast_exp2(float x) {  // 2 ulp; P is rounded to 16 bits
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     const T v[2] = {from_acc<T>(lo), from_acc<T>(hi)};
     return *reinterpret_cast<const uint32_t*>(v);
@@ -75,13 +102,16 @@ template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, fl
 // heads x images, splits fastest.
 template <typename T, int DP, bool EXACT>
 __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const SplitArgs args) {
-    constexpr int kKeys = DP == 128 ? 16 : 32;      // keys a warp takes at a time
+    using Lay = SplitLayout<DP>;
+    constexpr int kKeys = Lay::kKeys;               // keys a warp takes at a time
     constexpr int kChunks = DP / 32;                // 16-byte pieces a thread has of a key row
     constexpr int kDims = DP / 8;                   // columns a thread has of a value row
     constexpr int kG = kKeys / 16;
     const AttnArgs& a = args.a;
-    __shared__ float sm_o[kSplitWarps][16][DP + 4];
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    float (*sm_o)[16][DP + 4] = reinterpret_cast<float (*)[16][DP + 4]>(smem_raw);
     __shared__ float sm_ml[kSplitWarps][16][2];
+    __shared__ uint32_t sm_live[kSplitWarps][kSplitStages];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     const int group = a.H / a.Hk, rows = group * a.Q;
     int x = blockIdx.x;
@@ -125,38 +155,74 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
 #pragma unroll
         for (int y = 0; y < 4; ++y) o[i][y] = 0.f;
 
-    for (int j0 = split * args.split_keys + warp * kKeys; j0 < end; j0 += kSplitWarps * kKeys) {
-        // a bit per key of the step: not behind the end, not padded
-        bool there = j0 + lane < end && lane < kKeys;
-        if (there && pad != nullptr) there = pad[j0 + lane] == 0;
-        const uint32_t live = __ballot_sync(0xffffffffu, there);
+    unsigned char* ring = smem_raw + warp * kSplitStages * Lay::kStage;
+    constexpr int kStep = kSplitWarps * kKeys, kPieces = DP / 8;  // 16-byte pieces of a row
+    const int first = split * args.split_keys + warp * kKeys;
+    const int steps = first < end ? (end - first + kStep - 1) / kStep : 0;
+    // a bit per key of a step: not behind the end, not padded; the padding's bytes are read a step before they are used
+    auto key_there = [&](int step) {
+        const int j = first + step * kStep + lane;
+        return step < steps && lane < kKeys && j < end && (pad == nullptr || __ldg(pad + j) == 0);
+    };
+    bool there = key_there(0);
+    // this lane's pieces: column c of rows r, r + kRowsPer, ..
+    constexpr int kRowsPer = 32 / kPieces;
+    const int pr = lane / kPieces, pc = lane % kPieces;
+    const bool col = 8 * pc < a.D;
+    const T* kl = kp + (long long)(first + pr) * a.k_t + (col ? 8 * pc : 0);
+    const T* vl = vp + (long long)(first + pr) * a.v_t + (col ? 8 * pc : 0);
+    const uint32_t dst = smem_addr(ring) + pr * Lay::kPitch + 16 * pc;
+    int fill = 0;  // the ring slot the next fetch goes to
+    auto fetch = [&](int step) {
+        if (step < steps) {
+            const uint32_t all = __ballot_sync(0xffffffffu, there), live = all >> pr;
+            there = key_there(step + 1);
+            if (lane == 0) sm_live[warp][fill] = all;
+            const uint32_t to = dst + fill * Lay::kStage;
+            fill = fill == kSplitStages - 1 ? 0 : fill + 1;
+#pragma unroll
+            for (int i = 0; i < kKeys / kRowsPer; ++i) {
+                const bool real = col && ((live >> (i * kRowsPer)) & 1u) != 0;
+                copy16(to + i * kRowsPer * Lay::kPitch, real ? kl + i * kRowsPer * a.k_t : kp, real);
+                copy16(to + (kKeys + i * kRowsPer) * Lay::kPitch, real ? vl + i * kRowsPer * a.v_t : vp, real);
+            }
+            kl += kStep * a.k_t;
+            vl += kStep * a.v_t;
+        }
+        copy_commit();
+    };
+    const bool both = rows - r0 > 8;  // whether the tile has rows 8 .. 15
+    int slot = 0;
+#pragma unroll
+    for (int step = 0; step < kSplitStages - 1; ++step) fetch(step);
+    for (int step = 0; step < steps; ++step) {
+        __syncwarp();  // the slot's last readers are done
+        fetch(step + kSplitStages - 1);
+        copy_wait<kSplitStages - 1>();
+        __syncwarp();
+        const int j0 = first + step * kStep;
+        const uint32_t live = sm_live[warp][slot];
+        const unsigned char* ks = ring + slot * Lay::kStage;
+        slot = slot == kSplitStages - 1 ? 0 : slot + 1;
         if (live == 0) continue;
+        const unsigned char* vs = ks + kKeys * Lay::kPitch;
         uint4 kv[2 * kG][kChunks];
         uint32_t vv[4 * kG][kDims / 2];
 #pragma unroll
-        for (int u = 0; u < 2 * kG; ++u) {  // keys g, g + 8, ..
-            const int key = 8 * u + g;
+        for (int u = 0; u < 2 * kG; ++u)  // keys g, g + 8, ..
 #pragma unroll
-            for (int k = 0; k < kChunks; ++k) {
-                kv[u][k] = make_uint4(0u, 0u, 0u, 0u);
-                if (((live >> key) & 1u) != 0 && 32 * k + 8 * t < a.D)
-                    kv[u][k] = __ldg(reinterpret_cast<const uint4*>(kp + (j0 + key) * a.k_t + 32 * k + 8 * t));
-            }
-        }
+            for (int k = 0; k < kChunks; ++k)
+                kv[u][k] = *reinterpret_cast<const uint4*>(ks + (8 * u + g) * Lay::kPitch + 64 * k + 16 * t);
 #pragma unroll
         for (int u = 0; u < 4 * kG; ++u) {  // keys 2 t, 2 t + 1, 2 t + 8, 2 t + 9 of each 16
             const int key = 16 * (u / 4) + 8 * ((u >> 1) & 1) + 2 * t + (u & 1);
-            const bool in = ((live >> key) & 1u) != 0;
-            const T* src = vp + (j0 + key) * a.v_t;
             if constexpr (DP == 32) {
-                uint2 w = make_uint2(0u, 0u);
-                if (in && 4 * g < a.D) w = __ldg(reinterpret_cast<const uint2*>(src + 4 * g));
+                const uint2 w = *reinterpret_cast<const uint2*>(vs + key * Lay::kPitch + 8 * g);
                 vv[u][0] = w.x; vv[u][1] = w.y;
             } else {
 #pragma unroll
                 for (int k = 0; k < DP / 64; ++k) {
-                    uint4 w = make_uint4(0u, 0u, 0u, 0u);
-                    if (in && 64 * k + 8 * g < a.D) w = __ldg(reinterpret_cast<const uint4*>(src + 64 * k + 8 * g));
+                    const uint4 w = *reinterpret_cast<const uint4*>(vs + key * Lay::kPitch + 128 * k + 16 * g);
                     vv[u][4 * k] = w.x; vv[u][4 * k + 1] = w.y; vv[u][4 * k + 2] = w.z; vv[u][4 * k + 3] = w.w;
                 }
             }
@@ -174,26 +240,32 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
                 mma_16816<T>(s[u], a1, kv[u][k].z, kv[u][k].w);
             }
         }
-        float top[2] = {m[0], m[1]};
+        const bool plain = live == (kKeys == 32 ? 0xffffffffu : (1u << kKeys) - 1u) && !a.causal && a.mask == nullptr;
+        float keep[2] = {1.f, 1.f}, ref[2] = {0.f, 0.f}, sum[2] = {0.f, 0.f};
 #pragma unroll
-        for (int u = 0; u < 2 * kG; ++u)
+        for (int e = 0; e < 2; ++e) {  // rows g, g + 8; element y of score tile u: key 8 u + 2 t + y
+            if (e == 1 && !both) continue;
+            float top = m[e];
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {  // row g + 8 (y / 2), key 8 u + 2 t + y % 2
-                const int key = 8 * u + 2 * t + (y & 1), e = y >> 1, j = j0 + key;
-                bool open = ((live >> key) & 1u) != 0;
-                if (a.causal) open = open && j <= qi[e] + off;
-                if (open && mask_row[e] != nullptr) open = mask_row[e][j] == 0;
-                s[u][y] = open ? s[u][y] * c : -INFINITY;
-                top[e] = fmaxf(top[e], s[u][y]);
-            }
-        float keep[2], ref[2], sum[2] = {0.f, 0.f};
+            for (int u = 0; u < 2 * kG; ++u)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 1));
-            top[e] = fmaxf(top[e], __shfl_xor_sync(0xffffffffu, top[e], 2));
-            ref[e] = top[e] == -INFINITY ? 0.f : top[e];
-            keep[e] = exp2f(m[e] - ref[e]);
-            m[e] = top[e];
+                for (int y = 0; y < 2; ++y) {
+                    float& sv = s[u][2 * e + y];
+                    sv *= c;
+                    if (!plain) {
+                        const int key = 8 * u + 2 * t + y, j = j0 + key;
+                        bool open = ((live >> key) & 1u) != 0;
+                        if (a.causal) open = open && j <= qi[e] + off;
+                        if (open && mask_row[e] != nullptr) open = mask_row[e][j] == 0;
+                        if (!open) sv = -INFINITY;
+                    }
+                    top = fmaxf(top, sv);
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            ref[e] = top == -INFINITY ? 0.f : top;
+            keep[e] = fast_exp2(m[e] - ref[e]);
+            m[e] = top;
         }
 #pragma unroll
         for (int i = 0; i < kDims; ++i) {
@@ -205,7 +277,10 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
 #pragma unroll
             for (int y = 0; y < 4; ++y) {  // fragment registers: rows g, g + 8 of keys 0 .. 7, then of 8 .. 15
                 const int u = 2 * w + (y >> 1), e = y & 1;
-                const float p0 = exp2f(s[u][2 * e] - ref[e]), p1 = exp2f(s[u][2 * e + 1] - ref[e]);
+                p[y] = 0u;
+                if constexpr (EXACT) rest[y] = 0u;
+                if (e == 1 && !both) continue;
+                const float p0 = fast_exp2(s[u][2 * e] - ref[e]), p1 = fast_exp2(s[u][2 * e + 1] - ref[e]);
                 sum[e] += p0 + p1;
                 p[y] = pack_pair<T>(p0, p1);
                 if constexpr (EXACT) {
@@ -231,6 +306,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
         for (int e = 0; e < 2; ++e) l[e] = l[e] * keep[e] + sum[e];
     }
     // the quads' sums, then the warps' partials through shared memory, joined in warp order
+    copy_wait<0>();
+    __syncthreads();  // the rings have been read
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         l[e] += __shfl_xor_sync(0xffffffffu, l[e], 1);
@@ -278,36 +355,44 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
     }
 }
 
-// Joins the partials of a row, a warp per row, in the order of the splits.
+// Joins the partials of a row, a block of 8 warps per row: warp w adds splits w, w + 8, .. (their loads in flight
+// together), then the warps' sums are added in order.
+constexpr int kCombineWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(128) attn_combine_kernel(const SplitArgs args) {
+__global__ void __launch_bounds__(kCombineWarps * 32) attn_combine_kernel(const SplitArgs args) {
     using A = typename Elem<T>::acc;
     const AttnArgs& a = args.a;
-    const long long row = (long long)blockIdx.x * 4 + threadIdx.x / 32;
-    const int lane = threadIdx.x % 32;
+    __shared__ A part[kCombineWarps][kAttnMaxHeadDim];
+    const long long row = blockIdx.x;
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
     grid_dependency_wait();
     launch_dependents();
-    if (row >= (long long)a.B * a.H * a.Q) return;
     const A* ml = static_cast<const A*>(args.part_ml) + row * args.splits * 2;
     const A* po = static_cast<const A*>(args.part_o) + row * args.splits * a.D;
-    A top = -A(INFINITY);
+    A top = -A(INFINITY), sum = 0;
     for (int s = lane; s < args.splits; s += 32) top = cmax(top, ml[2 * s]);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) top = cmax(top, __shfl_xor_sync(0xffffffffu, top, x));
     const A ref = top == -A(INFINITY) ? A(0) : top;
-    A sum = 0, o[kAttnMaxHeadDim / 32] = {};
-    for (int s = 0; s < args.splits; ++s) {
-        const A f = attn_exp2<A>(ml[2 * s] - ref);
-        sum += ml[2 * s + 1] * f;
+    for (int s = lane; s < args.splits; s += 32) sum += ml[2 * s + 1] * attn_exp2<A>(ml[2 * s] - ref);
 #pragma unroll
-        for (int x = 0; x < kAttnMaxHeadDim / 32; ++x)
-            if (lane + 32 * x < a.D) o[x] += po[(long long)s * a.D + lane + 32 * x] * f;
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    for (int d = lane; d < a.D; d += 32) {
+        A o = 0;
+#pragma unroll 4
+        for (int s = warp; s < args.splits; s += kCombineWarps)
+            o += po[(long long)s * a.D + d] * attn_exp2<A>(ml[2 * s] - ref);
+        part[warp][d] = o;
     }
+    __syncthreads();
     const A inv = sum == A(0) ? A(0) : A(1) / sum;
+    for (int d = threadIdx.x; d < a.D; d += kCombineWarps * 32) {
+        A o = 0;
 #pragma unroll
-    for (int x = 0; x < kAttnMaxHeadDim / 32; ++x)
-        if (lane + 32 * x < a.D) attn_store<T, A>(a, row, lane + 32 * x, o[x], inv);
-    if (lane == 0) attn_store_lse<A>(a, row, top, sum);
+        for (int w = 0; w < kCombineWarps; ++w) o += part[w][d];
+        attn_store<T, A>(a, row, d, o, inv);
+    }
+    if (threadIdx.x == 0) attn_store_lse<A>(a, row, top, sum);
 }
 
 // ---- CUDA-core forward: every type and head width (see td_attention.cuh) ------------------------------------------

@@ -1016,18 +1016,28 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
         const int j = kt * 128 + 32 * w + lane;
         padded[w] = __ballot_sync(0xffffffffu, j < a.N && (pad == nullptr || pad[j] == 0));
     }
-    for (int r = warp; r < 128; r += 8) {
-        const int i = qt * 128 + r;
+    // four rows a warp at a time, so that 16 loads are in flight
+    const int rows = min(128, a.rows - qt * 128);
+    for (int r0 = warp * 4; r0 < 128; r0 += 32) {
+        bool open[4][4];
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const int j = kt * 128 + 32 * w + lane;
-            const bool open = i < a.rows && j < a.N && (mask == nullptr || mask[i * a.m_q + j] == 0);
-            const uint32_t word = __ballot_sync(0xffffffffu, open);
-            if (lane == w) {
-                pairs[r][w] = word;
-                all_rows[r][w] = word & padded[w];
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const int j = kt * 128 + 32 * w + lane;
+                open[x][w] = r0 + x < rows && j < a.N &&
+                             (mask == nullptr || __ldg(mask + (long long)(qt * 128 + r0 + x) * a.m_q + j) == 0);
             }
-        }
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                const uint32_t word = __ballot_sync(0xffffffffu, open[x][w]);
+                if (lane == w) {
+                    pairs[r0 + x][w] = word;
+                    all_rows[r0 + x][w] = word & padded[w];
+                }
+            }
     }
     __syncthreads();
     const long long bh = (long long)b * a.heads + h;
