@@ -280,7 +280,7 @@ def attention(query, key, value, key_padding_mask=None, attn_mask=None, causal=F
     _native.load()
     if _wants_grad(query, key, value):
         return AttentionFunction.apply(query, key, value, key_padding_mask, attn_mask, bool(causal), float(scale))
-    return _native.attention_forward(query, key, value, key_padding_mask, attn_mask, bool(causal), float(scale))[0]
+    return _native.attention_forward(query, key, value, key_padding_mask, attn_mask, bool(causal), float(scale))
 
 
 def layer_norm(x, weight, bias=None, residual=None, eps=1e-5):

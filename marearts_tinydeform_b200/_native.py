@@ -8,6 +8,7 @@ device, so calls are stream-ordered and can be captured in CUDA graphs.
 """
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -823,9 +824,16 @@ def _launch(fn, device, *args):
         raise RuntimeError(f'{fn.__name__} failed ({rc}): {err.value.decode(errors="replace")}')
 
 
+@functools.lru_cache(maxsize=1024)
+def _attention_workspace(*sizes):
+    """td_attention_workspace_bytes (a function of the sizes alone)."""
+    return load().td_attention_workspace_bytes(*sizes)
+
+
 def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale, for_backward=False):
-    """(out [B, Q, H * D], rest, lse) through td_attention_forward, for arguments check_attention has passed; rest (16-bit
-    types) and lse are None unless for_backward."""
+    """td_attention_forward for arguments check_attention has passed: out [B, Q, H * D], or with for_backward (out,
+    tensors, sizes), which attention_backward takes beside the gradient: the tensors as the kernels read them, what
+    rounding took from out (16-bit types) and the rows' log-sums; strides and sizes."""
     lib = load()
     if not query.is_cuda:
         raise RuntimeError('inputs must be CUDA tensors')
@@ -837,6 +845,7 @@ def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, sc
     m, ms, mb, mh = _attention_mask(attn_mask)
     pad = None if key_padding_mask is None else key_padding_mask.contiguous()
     code = DTYPE_CODE[query.dtype]
+    strides = _strides9(*qs, *ks, *vs)
     out = query.new_empty((B, Q, H * D))
     rest = lse = ws = None
     if for_backward:
@@ -844,38 +853,32 @@ def attention_forward(query, key, value, key_padding_mask, attn_mask, causal, sc
             rest = query.new_empty((B, Q, H * D))
         acc = torch.float64 if code == TD_F64 else torch.float32
         lse = query.new_empty((B, H, -(-Q // ATTN_ROW_PAD) * ATTN_ROW_PAD), dtype=acc)
-    if B * Q == 0:
-        return out, rest, lse
-    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, pad is not None, 0)
-    if ws_bytes:
-        ws = query.new_empty((ws_bytes,), dtype=torch.uint8)
-    _launch(lib.td_attention_forward, query.device, code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            _strides9(*qs, *ks, *vs), _address(m), ms, _address(pad), out.data_ptr(), _address(rest), _address(lse),
-            B, Q, N, H, Hk, D, scale, causal, _address(ws), ws_bytes)
-    return out, rest, lse
+    if B * Q:
+        ws_bytes = _attention_workspace(code, B, Q, N, H, Hk, D, mb, mh, pad is not None, 0)
+        if ws_bytes:
+            ws = query.new_empty((ws_bytes,), dtype=torch.uint8)
+        _launch(lib.td_attention_forward, query.device, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides,
+                _address(m), ms, _address(pad), out.data_ptr(), _address(rest), _address(lse), B, Q, N, H, Hk, D,
+                scale, causal, _address(ws), ws_bytes)
+    if not for_backward:
+        return out
+    return out, (q, k, v, m, pad, out, rest, lse), (code, strides, ms, mb, mh, B, Q, N, H, Hk, D, scale, causal)
 
 
-def attention_backward(query, key, value, key_padding_mask, attn_mask, causal, scale, out, rest, lse, grad_out):
-    """(grad_query, grad_key, grad_value) through td_attention_backward."""
+def attention_backward(tensors, sizes, grad_out):
+    """(grad_query, grad_key, grad_value) through td_attention_backward, from what attention_forward returned."""
     lib = load()
-    B, Q, H, D = query.shape
-    N, Hk = key.shape[1], key.shape[2]
-    q, qs = _attention_operand(query)
-    k, ks = _attention_operand(key)
-    v, vs = _attention_operand(value)
-    m, ms, mb, mh = _attention_mask(attn_mask)
-    pad = None if key_padding_mask is None else key_padding_mask.contiguous()
+    q, k, v, m, pad, out, rest, lse = tensors
+    code, strides, ms, mb, mh, B, Q, N, H, Hk, D, scale, causal = sizes
     g = grad_out.contiguous()
     grad_q = q.new_empty((B, Q, H, D))
     grad_k = q.new_empty((B, N, Hk, D))
     grad_v = q.new_empty((B, N, Hk, D))
-    code = DTYPE_CODE[q.dtype]
-    ws_bytes = lib.td_attention_workspace_bytes(code, B, Q, N, H, Hk, D, mb, mh, pad is not None, 1)
+    ws_bytes = _attention_workspace(code, B, Q, N, H, Hk, D, mb, mh, pad is not None, 1)
     ws = q.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    _launch(lib.td_attention_backward, query.device, code, q.data_ptr(), k.data_ptr(), v.data_ptr(),
-            _strides9(*qs, *ks, *vs), _address(m), ms, _address(pad), out.data_ptr(), _address(rest), lse.data_ptr(),
-            g.data_ptr(), grad_q.data_ptr(), grad_k.data_ptr(), grad_v.data_ptr(), B, Q, N, H, Hk, D, scale, causal,
-            _address(ws), ws_bytes)
+    _launch(lib.td_attention_backward, q.device, code, q.data_ptr(), k.data_ptr(), v.data_ptr(), strides, _address(m),
+            ms, _address(pad), out.data_ptr(), _address(rest), lse.data_ptr(), g.data_ptr(), grad_q.data_ptr(),
+            grad_k.data_ptr(), grad_v.data_ptr(), B, Q, N, H, Hk, D, scale, causal, _address(ws), ws_bytes)
     return grad_q, grad_k, grad_v
 
 
@@ -921,6 +924,12 @@ def layer_norm_forward(x, weight, bias, residual, eps, want_stats=False):
     return y, stats
 
 
+@functools.lru_cache(maxsize=1024)
+def _layer_norm_workspace(*sizes):
+    """td_layer_norm_workspace_bytes (a function of the sizes alone)."""
+    return load().td_layer_norm_workspace_bytes(*sizes)
+
+
 def layer_norm_backward(grad_y, x, weight, residual, stats, want_weight=True, want_bias=True):
     """(grad_x, grad_weight or None, grad_bias or None) through td_layer_norm_backward."""
     lib = load()
@@ -932,7 +941,7 @@ def layer_norm_backward(grad_y, x, weight, residual, stats, want_weight=True, wa
     grad_w = w.new_empty((C,)) if want_weight else None
     grad_b = w.new_empty((C,)) if want_bias else None
     mean = stats.data_ptr()
-    ws_bytes = lib.td_layer_norm_workspace_bytes(code, rows, C)
+    ws_bytes = _layer_norm_workspace(code, rows, C)
     ws = w.new_empty((max(ws_bytes, 1),), dtype=torch.uint8)
     _launch(lib.td_layer_norm_backward, x.device, code, g.data_ptr(), xs.data_ptr(), _address(r), w.data_ptr(), mean,
             mean + rows * (8 if code == TD_F64 else 4), grad_x.data_ptr(), _address(grad_w), _address(grad_b), rows, C,

@@ -148,27 +148,39 @@ def producer_train(query, reference_points, spatial_shapes, heads, points, sampl
     return ProducerFunction.apply(proj, reference_points, spatial_shapes, heads, points)
 
 
+def _first_order(backward):
+    """once_differentiable, whose own bookkeeping is left out of an ordinary backward (one without create_graph)."""
+    guarded = once_differentiable(backward)
+
+    def run(ctx, grad):
+        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+
+    return run
+
+
 class AttentionFunction(torch.autograd.Function):
     """Softmax attention on CUDA, differentiable in query, key and value: td_attention_forward, which also writes each
-    row's log-sum (and, for 16-bit types, what the result's rounding took), and td_attention_backward, which forms the probabilities again from it."""
+    row's log-sum (and, for 16-bit types, what the result's rounding took), and td_attention_backward, which forms the
+    probabilities again from it."""
 
     @staticmethod
     def forward(ctx, query, key, value, key_padding_mask, attn_mask, causal, scale):
-        out, rest, lse = _native.attention_forward(query, key, value, key_padding_mask, attn_mask, causal, scale,
-                                                   for_backward=True)
-        ctx.save_for_backward(query, key, value, key_padding_mask, attn_mask, out, rest, lse)
-        ctx.causal, ctx.scale = causal, scale
+        out, tensors, ctx.sizes = _native.attention_forward(query, key, value, key_padding_mask, attn_mask, causal,
+                                                            scale, for_backward=True)
+        ctx.save_for_backward(*tensors)
         return out
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_out):
-        query, key, value, key_padding_mask, attn_mask, out, rest, lse = ctx.saved_tensors
+        tensors = ctx.saved_tensors
+        q = tensors[0]
+        g = grad_out if grad_out.dtype == q.dtype else grad_out.to(q.dtype)
+        grads = _native.attention_backward(tensors, ctx.sizes, g)
         need = ctx.needs_input_grad
-        g = grad_out if grad_out.dtype == query.dtype else grad_out.to(query.dtype)
-        grads = _native.attention_backward(query, key, value, key_padding_mask, attn_mask, ctx.causal, ctx.scale, out,
-                                           rest, lse, g)
-        return tuple(x if n else None for x, n in zip(grads, need)) + (None, None, None, None)
+        if not (need[0] and need[1] and need[2]):
+            grads = tuple(x if n else None for x, n in zip(grads, need))
+        return grads + (None, None, None, None)
 
 
 class LayerNormFunction(torch.autograd.Function):
@@ -183,7 +195,7 @@ class LayerNormFunction(torch.autograd.Function):
         return y
 
     @staticmethod
-    @once_differentiable
+    @_first_order
     def backward(ctx, grad_y):
         x, weight, residual, stats = ctx.saved_tensors
         need = ctx.needs_input_grad

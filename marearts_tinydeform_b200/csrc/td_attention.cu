@@ -59,7 +59,7 @@ AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t
     const size_t acc = dtype == TD_F64 ? 8 : 4;
     const bool half = dtype == TD_F16 || dtype == TD_BF16;
     if (backward) {
-        w.amax = take(2 * sizeof(unsigned int));
+        w.amax = take(2 * kSms * sizeof(float));
         w.delta = take(size_t(B) * H * pad_rows(Q) * acc);
     } else {
         int64_t splits = simt_split_plan(dtype, B, Q, N, H, D).splits;
@@ -152,8 +152,8 @@ int simt_forward_tile(const SplitArgs& p, cudaStream_t stream, char* err, size_t
     constexpr int RN = simt_r<T>();
     using Tile = SimtTile<typename Elem<T>::acc, DP, RM, RN>;
     constexpr size_t smem = Tile::kRowBytes + 2 * Tile::kColBytes + Tile::kP;
-    auto kernel = attn_simt_forward_kernel<T, DP, RM, RN>;
-    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    constexpr auto kernel = attn_simt_forward_kernel<T, DP, RM, RN>;
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     const long long grid = (long long)p.splits * p.row_tiles * p.a.B * p.a.H;
     if (int rc = host::launch(err, err_len, "attn_simt_forward_kernel", kernel, dim3(unsigned(grid)), dim3(256), smem,
                               stream, true, p))
@@ -175,9 +175,9 @@ int simt_forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned 
 template <typename T, int DP, bool EXACT>
 int mma_split(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
     const long long grid = (long long)p.splits * p.row_tiles * p.a.B * p.a.Hk;
-    auto kernel = attn_split_kernel<T, DP, EXACT>;
+    constexpr auto kernel = attn_split_kernel<T, DP, EXACT>;
     constexpr size_t smem = SplitLayout<DP>::kSmem;
-    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     if (int rc = host::launch(err, err_len, "attn_split_kernel", kernel, dim3(unsigned(grid)),
                               dim3(kSplitWarps * 32), smem, stream, true, p))
         return rc;
@@ -220,8 +220,8 @@ int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_
     constexpr int R = simt_r<T>();
     using Tile = SimtTile<typename Elem<T>::acc, DP, R, R>;
     constexpr size_t smem = 4 * Tile::kRowBytes + Tile::kP;
-    auto kernel = attn_simt_backward_kernel<T, DP, R>;
-    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    constexpr auto kernel = attn_simt_backward_kernel<T, DP, R>;
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     const long long rows = (long long)a.B * a.H * a.Qp;
     if (int rc = host::launch(err, err_len, "attn_delta_kernel", attn_delta_kernel<T>,
                               dim3(unsigned((rows + 255) / 256)), dim3(256), 0, stream, true, a))

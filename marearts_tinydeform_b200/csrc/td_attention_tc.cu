@@ -1,4 +1,6 @@
 // td_attention_tc.cu -- launches of the attention's tensor-core kernels: conditions, tensor maps, packed masks.
+#include <algorithm>
+
 #include "td_attention_plan.h"
 #include "td_attention_tc.cuh"
 
@@ -44,14 +46,15 @@ bool operand_fits(const Operand& o, const AttnArgs& a) {
     return aligned16(o.base);
 }
 
-// Boxes of min(DP, 64) columns x `rows` tokens of one head of one image; what lies outside reads as zero.
+// Boxes of min(DP, 64) columns x 64 tokens of one head of one image (a resident operand of 128 rows takes two, which lie
+// behind one another as one of 128 would); what lies outside reads as zero.
 template <int DP>
-int make_map(CUtensorMap* map, const Operand& o, int rows, const AttnArgs& a, char* err, size_t err_len) {
+int make_map(CUtensorMap* map, const Operand& o, const AttnArgs& a, char* err, size_t err_len) {
     const uint64_t dims[4] = {uint64_t(a.D), uint64_t(o.tokens), uint64_t(o.heads), uint64_t(a.B)};
     const uint64_t strides[3] = {uint64_t(map_stride(o.s_t, o.tokens, a)) * 2,
                                  uint64_t(map_stride(o.s_h, o.heads, a)) * 2,
                                  uint64_t(map_stride(o.s_b, a.B, a)) * 2};
-    const uint32_t box[4] = {uint32_t(AttnBox<DP>::kCols), uint32_t(rows), 1, 1};
+    const uint32_t box[4] = {uint32_t(AttnBox<DP>::kCols), uint32_t(kAttnBN), 1, 1};
     const CUresult r = host::encode_tiled_u16(map, 4, o.base, dims, strides, box,
                                               DP == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B);
     if (r == CUDA_SUCCESS) return TD_OK;
@@ -105,13 +108,13 @@ int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsig
             cudaStream_t stream, char* err, size_t err_len) {
     const AttnArgs& a = t.a;
     CUtensorMap q, k, v;
-    if (int rc = make_map<DP>(&q, query_of(a), kAttnBM, a, err, err_len)) return rc;
-    if (int rc = make_map<DP>(&k, key_of(a), kAttnBN, a, err, err_len)) return rc;
-    if (int rc = make_map<DP>(&v, value_of(a), kAttnBN, a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&q, query_of(a), a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&k, key_of(a), a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&v, value_of(a), a, err, err_len)) return rc;
     if (int rc = pack_masks(t, w, mb, mh, false, workspace, stream, err, err_len)) return rc;
-    auto kernel = attn_tc_forward_kernel<T, DP, EXACT>;
+    constexpr auto kernel = attn_tc_forward_kernel<T, DP, EXACT>;
     constexpr size_t smem = AttnFwdLayout<DP>::kSmemBytes;
-    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     const unsigned grid = unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
     return host::launch(err, err_len, "attn_tc_forward_kernel", kernel, dim3(grid), dim3(kAttnFwdThreads), smem, stream,
                         true, q, k, v, t);
@@ -121,39 +124,29 @@ template <typename T, int DP>
 int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsigned char* workspace,
              cudaStream_t stream, char* err, size_t err_len) {
     const AttnArgs& a = t.a;
-    const Operand ops[4] = {query_of(a), grad_of(a), key_of(a), value_of(a)};
-    CUtensorMap fixed[4], tile[4];
-    for (int i = 0; i < 4; ++i) {
-        if (int rc = make_map<DP>(&fixed[i], ops[i], kAttnBM, a, err, err_len)) return rc;
-        if (int rc = make_map<DP>(&tile[i], ops[i], kAttnBN, a, err, err_len)) return rc;
-    }
+    CUtensorMap q, g, k, v;
+    if (int rc = make_map<DP>(&q, query_of(a), a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&g, grad_of(a), a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&k, key_of(a), a, err, err_len)) return rc;
+    if (int rc = make_map<DP>(&v, value_of(a), a, err, err_len)) return rc;
     if (int rc = pack_masks(t, w, mb, mh, true, workspace, stream, err, err_len)) return rc;
     int lanes = 1;
     while (lanes * 8 < a.D) lanes *= 2;
-    const int per_block = 256 / lanes;
-    const unsigned delta_blocks = unsigned(((long long)a.B * a.H * a.Qp + per_block - 1) / per_block);
-    unsigned blocks = delta_blocks;
-    unsigned int* amax = nullptr;
-    if constexpr (std::is_same<T, __half>::value) {
-        amax = reinterpret_cast<unsigned int*>(workspace + w.amax);
-        const cudaError_t e = cudaMemsetAsync(amax, 0, 2 * sizeof(unsigned int), stream);
-        if (e != cudaSuccess) {
-            cudaGetLastError();
-            return fail(err, err_len, TD_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
-        }
-        blocks += unsigned(((long long)a.B * a.Hk * a.N + per_block - 1) / per_block);
-    }
-    if (int rc = host::launch(err, err_len, "attn_delta_tc_kernel", attn_delta_tc_kernel<T>, dim3(blocks), dim3(256), 0,
-                              stream, true, a, lanes, delta_blocks, amax))
+    const long long rows = std::max((long long)a.B * a.H * a.Qp, (long long)a.B * a.Hk * a.N);
+    const int per_block = kDeltaThreads / lanes;
+    const int blocks = int(std::min<long long>(kSms, (rows + per_block - 1) / per_block));
+    t.amax = reinterpret_cast<float*>(workspace + w.amax);
+    t.amax_parts = blocks;
+    if (int rc = host::launch(err, err_len, "attn_delta_tc_kernel", attn_delta_tc_kernel<T>, dim3(unsigned(blocks)),
+                              dim3(kDeltaThreads), 0, stream, true, a, lanes, t.amax))
         return rc;
-    t.amax = amax;
     t.kv_blocks = (a.N + kAttnBM - 1) / kAttnBM * a.B * a.Hk;
-    auto kernel = attn_tc_backward_kernel<T, DP>;
+    constexpr auto kernel = attn_tc_backward_kernel<T, DP>;
     constexpr size_t smem = AttnBwdLayout<DP>::kSmemBytes;
-    if (int rc = host::allow_smem(kernel, smem, err, err_len)) return rc;
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     const unsigned grid = unsigned(t.kv_blocks) + unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
     return host::launch(err, err_len, "attn_tc_backward_kernel", kernel, dim3(grid), dim3(AttnBwdLayout<DP>::kThreads), smem, stream,
-                        true, fixed[0], fixed[1], fixed[2], fixed[3], tile[0], tile[1], tile[2], tile[3], t);
+                        true, q, g, k, v, t);
 }
 
 }  // namespace

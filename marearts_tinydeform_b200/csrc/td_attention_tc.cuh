@@ -42,7 +42,8 @@ struct AttnTcArgs {
     long long cb_b, cb_h, cf_b, cf_h;
     int col_words;              // words a key's row of col_bits has
     int col_tiles;              // flags a row of col_flags has
-    const unsigned int* amax;   // float16 backward: bits of max|dO| and max|V|
+    float* amax;                // float16 backward: per block of the delta kernel max|dO|, then per block max|V|
+    int amax_parts;
     int kv_blocks;              // backward: blocks of the keys' gradient, launched first
 };
 
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                                : args.row_flags + b * args.rf_b + h * args.rf_h + qt * args.rf_q;
 
     if (threadIdx.x == 0) {
-        mbar_init(qfull, KB);
+        mbar_init(qfull, 2 * KB);
         for (int s = 0; s < S; ++s) {
             mbar_init(&kfull[s], KB);
             mbar_init(&vfull[s], KB);
@@ -403,9 +404,10 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         // a lane per box of the ring: TMA copies of one thread are served one after another, those of different threads
         // overlap
         const uint64_t pol = l2_evict_last();  // keys and values are read again by the other query tiles
-        if (lane < KB && tiles > 0) {
-            mbar_arrive_expect_tx(qfull, Lay::kQBytes / KB);
-            tma_load_4d(smem + lane * AttnBox<DP>::kFixed, &map_q, qfull, 64 * lane, i0, h, b, l2_evict_first());
+        if (lane < 2 * KB && tiles > 0) {  // the queries in halves of 64
+            mbar_arrive_expect_tx(qfull, AttnBox<DP>::kTile);
+            tma_load_4d(smem + lane * AttnBox<DP>::kTile, &map_q, qfull, 64 * (lane / 2), i0 + 64 * (lane % 2), h, b,
+                        l2_evict_first());
         }
         int n = 0;
         Ring<S> ring;
@@ -652,8 +654,18 @@ struct AttnBwdLayout {
 
 // float16 keeps dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
 // gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs no scale.
-__device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {
-    const float bound = 2.f * float(args.a.D) * __uint_as_float(args.amax[0]) * __uint_as_float(args.amax[1]);
+__device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {  // one warp
+    float g = 0.f, v = 0.f;
+    for (int i = threadIdx.x & 31; i < args.amax_parts; i += 32) {
+        g = fmaxf(g, args.amax[i]);
+        v = fmaxf(v, args.amax[args.amax_parts + i]);
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) {
+        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, x));
+        v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
+    }
+    const float bound = 2.f * float(args.a.D) * g * v;
     if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
     return exp2f(fminf(fmaxf(15.f - ceilf(log2f(bound)), -100.f), 100.f));
 }
@@ -753,11 +765,11 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
 
     if (warp == 0) {
         const uint64_t pol = l2_evict_last();
-        if (lane < 2 * KB) {
-            const int box = lane % KB;
-            mbar_arrive_expect_tx(fixed, AttnBox<DP>::kFixed);
-            tma_load_4d(smem + (lane / KB) * Lay::kFixedBytes + box * AttnBox<DP>::kFixed, lane < KB ? &map_fixed1 : &map_fixed2,
-                        fixed, 64 * box, r0, head, b, pol);
+        if (lane < 4 * KB) {  // the two resident operands, in halves of 64 rows
+            const int job = lane % (2 * KB), op = lane / (2 * KB);
+            mbar_arrive_expect_tx(fixed, AttnBox<DP>::kTile);
+            tma_load_4d(smem + op * Lay::kFixedBytes + job * AttnBox<DP>::kTile, op == 0 ? &map_fixed1 : &map_fixed2,
+                        fixed, 64 * (job / 2), r0 + 64 * (job % 2), head, b, pol);
         }
         int n = 0;
         Ring<S> ring;
@@ -929,10 +941,8 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
 
 template <typename T, int DP>
 __global__ void __launch_bounds__(AttnBwdLayout<DP>::kThreads, 1)
-    attn_tc_backward_kernel(const __grid_constant__ CUtensorMap q128, const __grid_constant__ CUtensorMap g128,
-                            const __grid_constant__ CUtensorMap k128, const __grid_constant__ CUtensorMap v128,
-                            const __grid_constant__ CUtensorMap q64, const __grid_constant__ CUtensorMap g64,
-                            const __grid_constant__ CUtensorMap k64, const __grid_constant__ CUtensorMap v64,
+    attn_tc_backward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_g,
+                            const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                             const AttnTcArgs args) {
     using Lay = AttnBwdLayout<DP>;
     constexpr int S = Lay::kStages, KB = Lay::kBoxes, NB = Lay::kBufs;
@@ -943,7 +953,7 @@ __global__ void __launch_bounds__(AttnBwdLayout<DP>::kThreads, 1)
     if (threadIdx.x == 0) {
         uint64_t* fixed = reinterpret_cast<uint64_t*>(smem + Lay::kBars);
         uint64_t *full = fixed + 1, *empty = full + S, *sfull = empty + S, *pfull = sfull + NB, *done = pfull + NB;
-        mbar_init(fixed, 2 * KB);
+        mbar_init(fixed, 4 * KB);
         for (int s = 0; s < S; ++s) {
             mbar_init(&full[s], 2 * KB + (keys ? 2 : 0));
             mbar_init(&empty[s], 1);
@@ -967,9 +977,9 @@ __global__ void __launch_bounds__(AttnBwdLayout<DP>::kThreads, 1)
     grid_dependency_wait();
     launch_dependents();
     if (keys)
-        attn_tc_backward_block<T, DP, true>(k128, v128, q64, g64, args, int(blockIdx.x), smem, tmem);
+        attn_tc_backward_block<T, DP, true>(map_k, map_v, map_q, map_g, args, int(blockIdx.x), smem, tmem);
     else
-        attn_tc_backward_block<T, DP, false>(q128, g128, k64, v64, args, int(blockIdx.x) - args.kv_blocks, smem,
+        attn_tc_backward_block<T, DP, false>(map_q, map_g, map_k, map_v, args, int(blockIdx.x) - args.kv_blocks, smem,
                                              tmem);
     tc_fence_before();
     __syncthreads();
@@ -1085,24 +1095,26 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
 }
 
 // delta as in attn_delta_kernel for 16-bit types with D a multiple of 8: 16-byte loads, `lanes` (a power of two, at
-// least D / 8) threads a row. float16: the blocks also take max|dO| over all rows, and the blocks behind delta_blocks
-// max|V| over the keys that are there, into amax (zeroed before; a maximum has no order).
+// least D / 8) threads a row, at most a CTA an SM walking over the rows. float16: each CTA also leaves max|dO| over its
+// rows and max|V| over its share of the keys that are there (a maximum of maxima has no order).
+constexpr int kDeltaThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(256) attn_delta_tc_kernel(const AttnArgs a, int lanes, unsigned delta_blocks,
-                                                            unsigned int* amax) {
+__global__ void __launch_bounds__(kDeltaThreads) attn_delta_tc_kernel(const AttnArgs a, int lanes, float* amax) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    const int sub = threadIdx.x % lanes, per_block = 256 / lanes;
-    const long long row = (long long)(blockIdx.x < delta_blocks ? blockIdx.x : blockIdx.x - delta_blocks) * per_block +
-                          threadIdx.x / lanes;
+    const int sub = threadIdx.x % lanes;
+    const long long step = (long long)gridDim.x * (kDeltaThreads / lanes);
+    const long long first = (long long)blockIdx.x * (kDeltaThreads / lanes) + threadIdx.x / lanes;
+    const bool col = sub * 8 < a.D;
     grid_dependency_wait();
     launch_dependents();
-    float top = 0.f;
-    if (blockIdx.x < delta_blocks) {
+    float top_g = 0.f, top_v = 0.f;
+    const long long rows = (long long)a.B * a.H * a.Qp;
+    // whole warps take the same number of turns (a warp holds whole rows)
+    for (long long row = first, warp0 = first - threadIdx.x % 32 / lanes; warp0 < rows; row += step, warp0 += step) {
         const int i = int(row % a.Qp);
         const long long bh = row / a.Qp;
-        const bool in = bh < (long long)a.B * a.H;
         float sum = 0.f;
-        if (in && i < a.Q && sub * 8 < a.D) {
+        if (row < rows && i < a.Q && col) {
             const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D + sub * 8;
             float o[8], g[8], r[8];
             load16<T>(static_cast<const T*>(a.out_in) + at, o);
@@ -1111,32 +1123,38 @@ __global__ void __launch_bounds__(256) attn_delta_tc_kernel(const AttnArgs a, in
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
                 sum += (o[x] + r[x]) * g[x];
-                if constexpr (kHalf) top = fmaxf(top, fabsf(g[x]));
+                if constexpr (kHalf) top_g = fmaxf(top_g, fabsf(g[x]));
             }
         }
         for (int x = lanes / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        if (in && sub == 0) static_cast<float*>(a.delta)[row] = sum;
-    } else if constexpr (kHalf) {
-        const long long tokens = (long long)a.B * a.N;  // row = (b * Hk + hk) * N + j
-        if (row < tokens * a.Hk && sub * 8 < a.D) {
-            const long long j = row % a.N, bh = row / a.N, b = bh / a.Hk;
-            if (a.padding == nullptr || a.padding[b * a.N + j] == 0) {
-                float v[8];
-                load16<T>(static_cast<const T*>(a.v) + b * a.v_b + bh % a.Hk * a.v_h + j * a.v_t + sub * 8, v);
-#pragma unroll
-                for (int x = 0; x < 8; ++x) top = fmaxf(top, fabsf(v[x]));
-            }
-        }
+        if (row < rows && sub == 0) static_cast<float*>(a.delta)[row] = sum;
     }
     if constexpr (kHalf) {
+        const long long keys = (long long)a.B * a.Hk * a.N;  // row = (b * Hk + hk) * N + j
+        for (long long row = first; row < keys && col; row += step) {
+            const long long j = row % a.N, bh = row / a.N, b = bh / a.Hk;
+            if (a.padding != nullptr && a.padding[b * a.N + j] != 0) continue;
+            float v[8];
+            load16<T>(static_cast<const T*>(a.v) + b * a.v_b + bh % a.Hk * a.v_h + j * a.v_t + sub * 8, v);
 #pragma unroll
-        for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-        __shared__ float tops[8];
-        if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+            for (int x = 0; x < 8; ++x) top_v = fmaxf(top_v, fabsf(v[x]));
+        }
+        __syncwarp();
+        __shared__ float tops[2][kDeltaThreads / 32];
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) {
+            top_g = fmaxf(top_g, __shfl_xor_sync(0xffffffffu, top_g, x));
+            top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, x));
+        }
+        if (threadIdx.x % 32 == 0) {
+            tops[0][threadIdx.x / 32] = top_g;
+            tops[1][threadIdx.x / 32] = top_v;
+        }
         __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int x = 1; x < 8; ++x) top = fmaxf(top, tops[x]);
-            if (top > 0.f) atomicMax(amax + (blockIdx.x < delta_blocks ? 0 : 1), __float_as_uint(top));
+        if (threadIdx.x < 2) {
+            float top = 0.f;
+            for (int x = 0; x < kDeltaThreads / 32; ++x) top = fmaxf(top, tops[threadIdx.x][x]);
+            amax[threadIdx.x * gridDim.x + blockIdx.x] = top;
         }
     }
 }

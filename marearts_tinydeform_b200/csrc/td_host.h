@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -50,15 +51,23 @@ int launch(char* err, size_t err_len, const char* what, K kernel, dim3 grid, dim
     return TD_OK;
 }
 
-// Raises the kernel's dynamic shared memory limit where it needs more than the 48 KB every kernel has. The attribute
-// is the device's, so it is set on every call (a host-side write, legal during capture).
-template <typename K>
-int allow_smem(K kernel, size_t bytes, char* err, size_t err_len) {
+// Raises a kernel's dynamic shared memory limit where it needs more than the 48 KB every kernel has: the attribute is the
+// device's, so once per kernel and device (a host-side write, legal during capture; two threads may both do it).
+template <auto Kernel>
+int allow_smem(size_t bytes, char* err, size_t err_len) {
+    static std::atomic<uint64_t> done{0};
     if (bytes <= 48 * 1024) return TD_OK;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
-    if (e == cudaSuccess) return TD_OK;
-    cudaGetLastError();
-    return fail(err, err_len, TD_ERR_CUDA, "shared memory limit of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1) != 0) return TD_OK;
+    if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return fail(err, err_len, TD_ERR_CUDA, "shared memory limit of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    }
+    if (dev < 64) done.fetch_or(uint64_t(1) << dev, std::memory_order_release);
+    return TD_OK;
 }
 
 }  // namespace host
