@@ -1,5 +1,6 @@
 // td_norm.cu -- the layer norm entry points of the C ABI: argument contract, kernel choice and launches.
 #include <algorithm>
+#include <type_traits>
 
 #include "td_host.h"
 #include "td_norm.cuh"
@@ -10,9 +11,6 @@ namespace {
 using host::fail;
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
-// CTAs an SM holds of either kernel (256 threads at up to 64 registers)
-constexpr int kNormCtasPerSm = 4;
 
 int check_norm(int dtype, int64_t rows, int64_t C, double eps, char* err, size_t err_len) {
     if (dtype < TD_F32 || dtype > TD_F64) return fail(err, err_len, TD_ERR_ARG, "unsupported dtype %d", dtype);
@@ -26,35 +24,43 @@ int check_norm(int dtype, int64_t rows, int64_t C, double eps, char* err, size_t
 // Rows a CTA holds at once: a warp a row up to 512 channels, 4 warps up to 2048, 8 above.
 int groups_of(int64_t C) { return C <= 512 ? 8 : C <= 2048 ? 2 : 1; }
 
-// The CTAs of a launch: one wave, or fewer when there are fewer rows.
-int norm_grid(int64_t rows, int64_t C) {
+// The CTAs of a launch with `per_sm` on each SM: one wave, or fewer when there are fewer rows.
+int norm_grid(int64_t rows, int64_t C, int per_sm) {
     const int64_t need = (rows + groups_of(C) - 1) / groups_of(C);
-    return int(std::min<int64_t>(need, int64_t(kSms) * kNormCtasPerSm));
+    return int(std::min<int64_t>(need, int64_t(kSms) * per_sm));
 }
+constexpr int kMostCtas = 3;  // of any backward form: the workspace's partial rows
 
 template <typename T, int VEC, bool BWD>
-int launch_norm(const NormArgs<T>& a, int grid, cudaStream_t stream, char* err, size_t err_len) {
-    auto go = [&](auto kernel) {
-        return host::launch(err, err_len, BWD ? "norm_backward_kernel" : "norm_forward_kernel", kernel,
-                            dim3(unsigned(grid)), dim3(kNormThreads), 0, stream, true, a);
+int launch_norm(const NormArgs<T>& a, int* grid, cudaStream_t stream, char* err, size_t err_len) {
+    auto go = [&](auto g, auto ept) {
+        constexpr int G = decltype(g)::value, EPT = decltype(ept)::value, kCtas = norm_ctas<T, VEC, EPT, BWD>();
+        static_assert(!BWD || kCtas <= kMostCtas, "workspace");
+        *grid = norm_grid(a.rows, a.C, kCtas);
+        if constexpr (BWD)
+            return host::launch(err, err_len, "norm_backward_kernel", norm_backward_kernel<T, VEC, G, EPT>,
+                                dim3(unsigned(*grid)), dim3(kNormThreads), 0, stream, true, a);
+        else
+            return host::launch(err, err_len, "norm_forward_kernel", norm_forward_kernel<T, VEC, G, EPT>,
+                                dim3(unsigned(*grid)), dim3(kNormThreads), 0, stream, true, a);
     };
-    if constexpr (BWD) {
-        if (a.C <= 256) return go(norm_backward_kernel<T, VEC, 32, 8>);
-        if (a.C <= 512) return go(norm_backward_kernel<T, VEC, 32, 16>);
-        if (a.C <= 2048) return go(norm_backward_kernel<T, VEC, 128, 16>);
-        if (a.C <= 4096) return go(norm_backward_kernel<T, VEC, 256, 16>);
-        return go(norm_backward_kernel<T, VEC, 256, 32>);
-    } else {
-        if (a.C <= 256) return go(norm_forward_kernel<T, VEC, 32, 8>);
-        if (a.C <= 512) return go(norm_forward_kernel<T, VEC, 32, 16>);
-        if (a.C <= 2048) return go(norm_forward_kernel<T, VEC, 128, 16>);
-        if (a.C <= 4096) return go(norm_forward_kernel<T, VEC, 256, 16>);
-        return go(norm_forward_kernel<T, VEC, 256, 32>);
-    }
+    using std::integral_constant;
+    const integral_constant<int, 32> warp;
+    const integral_constant<int, 128> four;
+    const integral_constant<int, 256> eight;
+    const integral_constant<int, 8> e8;
+    const integral_constant<int, 16> e16;
+    const integral_constant<int, 32> e32;
+    if (a.C <= 256) return go(warp, e8);
+    if (a.C <= 512) return go(warp, e16);
+    if (a.C <= 1024) return go(four, e8);
+    if (a.C <= 2048) return go(four, e16);
+    if (a.C <= 4096) return go(eight, e16);
+    return go(eight, e32);
 }
 
 template <typename T, bool BWD>
-int pick_norm(const NormArgs<T>& a, int grid, cudaStream_t stream, char* err, size_t err_len) {
+int pick_norm(const NormArgs<T>& a, int* grid, cudaStream_t stream, char* err, size_t err_len) {
     constexpr int V = Elem<T>::kVec;
     // 16-byte vectors where every row starts on a 16-byte boundary
     const bool wide = a.C % V == 0 && aligned16(a.x) && aligned16(a.residual) && aligned16(a.weight) &&
@@ -78,7 +84,8 @@ int forward(const void* x, const void* residual, const void* weight, const void*
     a.rows = rows;
     a.C = int(C);
     a.eps = acc(eps);
-    return pick_norm<T, false>(a, norm_grid(rows, C), stream, err, err_len);
+    int grid = 0;
+    return pick_norm<T, false>(a, &grid, stream, err, err_len);
 }
 
 template <typename T>
@@ -97,8 +104,8 @@ int backward(const void* grad_y, const void* x, const void* residual, const void
     a.partial = static_cast<acc*>(workspace);
     a.rows = rows;
     a.C = int(C);
-    const int grid = norm_grid(rows, C);
-    if (int rc = pick_norm<T, true>(a, grid, stream, err, err_len)) return rc;
+    int grid = 0;
+    if (int rc = pick_norm<T, true>(a, &grid, stream, err, err_len)) return rc;
     return host::launch(err, err_len, "norm_reduce_kernel", norm_reduce_kernel<T>,
                         dim3(unsigned((2 * C + kReduceCols - 1) / kReduceCols)), dim3(kReduceCols * kReduceRows), 0,
                         stream, true, static_cast<const acc*>(a.partial), static_cast<T*>(grad_weight),
@@ -131,7 +138,7 @@ int td_layer_norm_forward(int dtype, const void* x, const void* residual, const 
 size_t td_layer_norm_workspace_bytes(int dtype, int64_t rows, int64_t C) {
     using namespace td;
     if (dtype < TD_F32 || dtype > TD_F64 || rows <= 0 || C <= 0) return 0;
-    return size_t(norm_grid(rows, C)) * 2 * size_t(C) * (dtype == TD_F64 ? 8 : 4);
+    return size_t(norm_grid(rows, C, kMostCtas)) * 2 * size_t(C) * (dtype == TD_F64 ? 8 : 4);
 }
 
 int td_layer_norm_backward(int dtype, const void* grad_y, const void* x, const void* residual, const void* weight,

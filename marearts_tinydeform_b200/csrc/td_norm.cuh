@@ -87,30 +87,47 @@ __device__ __forceinline__ void store_row(T* __restrict__ p, const typename Elem
     }
 }
 
-// Sum over the G threads of the calling group, the same bits in each (an xor butterfly, then the warps in order).
-// red: kNormThreads / 32 words a call; every thread of the CTA calls (G > 32: two CTA barriers).
-template <int G, typename A>
-__device__ __forceinline__ A group_sum(A v, A* red) {
+// Sums of N values over the G threads of the calling group, the same bits in each (an xor butterfly, then the warps in
+// order). For G > 32 the warps meet at the group's own barrier, once a call: calls alternate between the two halves of
+// `red`, and whoever writes a half again has passed the barrier behind its last reading.
+template <int G, int N, typename A>
+__device__ __forceinline__ void group_sum(A (&v)[N], A (&red)[2][N][kNormThreads / 32], int& half) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    for (int n = 0; n < N; ++n)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
     if constexpr (G > 32) {
-        const int warp = threadIdx.x >> 5;
-        __syncthreads();  // the words of the call before have been read
-        if ((threadIdx.x & 31) == 0) red[warp] = v;
-        __syncthreads();
-        const int first = warp / (G / 32) * (G / 32);
-        v = red[first];
+        const int warp = threadIdx.x >> 5, first = warp / (G / 32) * (G / 32);
+        if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int i = 1; i < G / 32; ++i) v += red[first + i];
+            for (int n = 0; n < N; ++n) red[half][n][warp] = v[n];
+        }
+        named_barrier(1 + int(threadIdx.x) / G, G);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            v[n] = red[half][n][first];
+#pragma unroll
+            for (int i = 1; i < G / 32; ++i) v[n] += red[half][n][first + i];
+        }
+        half ^= 1;
     }
-    return v;
+}
+
+// CTAs an SM holds of a form, by the registers it needs; a launch has one wave of them, so that all end together.
+template <typename T, int VEC, int EPT, bool BWD>
+constexpr int norm_ctas() {
+    if (sizeof(T) == 8) return 1;
+    if (EPT == 8) return BWD ? (sizeof(T) == 2 && VEC > 1 ? 3 : 2) : VEC > 1 ? 4 : 3;
+    return EPT == 16 && !BWD ? 2 : 1;
 }
 
 template <typename T, int VEC, int G, int EPT>
-__global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, false>())
+    norm_forward_kernel(const NormArgs<T> a) {
     using acc = typename Elem<T>::acc;
     constexpr int NV = EPT / VEC, kGroups = kNormThreads / G;
-    __shared__ acc red[2 * kNormThreads / 32];
+    __shared__ acc red[2][1][kNormThreads / 32];
+    int half = 0;
     const int group = threadIdx.x / G, lane = threadIdx.x % G;
     grid_dependency_wait();
     launch_dependents();
@@ -131,8 +148,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormAr
     r.zero();
     long long row = (long long)blockIdx.x * kGroups + group;
     fetch(row);
-    // every group takes the same number of turns, so that the CTA barriers of group_sum match
-    for (long long turn = (long long)blockIdx.x * kGroups; turn < a.rows; turn += step, row += step) {
+    for (; row < a.rows; row += step) {
         acc s[EPT], t[EPT];
         x.widen(s);
         if (a.residual != nullptr) {
@@ -141,39 +157,40 @@ __global__ void __launch_bounds__(kNormThreads) norm_forward_kernel(const NormAr
             for (int i = 0; i < EPT; ++i) s[i] += t[i];
         }
         fetch(row + step);
-        acc sum = 0;
+        acc sum[1] = {0}, sq[1] = {0};
 #pragma unroll
-        for (int i = 0; i < EPT; ++i) sum += s[i];  // elements outside the row are zero
-        const acc mean = group_sum<G>(sum, red) * inv;
-        acc sq = 0;
+        for (int i = 0; i < EPT; ++i) sum[0] += s[i];  // elements outside the row are zero
+        group_sum<G>(sum, red, half);
+        const acc mean = sum[0] * inv;
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             const int c = (lane + i / VEC * G) * VEC + i % VEC;
             s[i] = c < a.C ? s[i] - mean : acc(0);
-            sq += s[i] * s[i];
+            sq[0] += s[i] * s[i];
         }
-        const acc rstd = acc(1) / sqrt(group_sum<G>(sq, red + kNormThreads / 32) * inv + a.eps);
-        if (row < a.rows) {
-            if (a.mean != nullptr && lane == 0) {
-                a.mean[row] = mean;
-                a.rstd[row] = rstd;
-            }
-            acc u[EPT];
-            w.widen(t);
-            b.widen(u);
+        group_sum<G>(sq, red, half);
+        const acc rstd = acc(1) / sqrt(sq[0] * inv + a.eps);
+        if (a.mean != nullptr && lane == 0) {
+            a.mean[row] = mean;
+            a.rstd[row] = rstd;
+        }
+        acc u[EPT];
+        w.widen(t);
+        b.widen(u);
 #pragma unroll
-            for (int i = 0; i < EPT; ++i) s[i] = s[i] * rstd * t[i] + u[i];
-            store_row<T, VEC, NV, G>(a.out + row * a.C, s, lane, a.C);
-        }
+        for (int i = 0; i < EPT; ++i) s[i] = s[i] * rstd * t[i] + u[i];
+        store_row<T, VEC, NV, G>(a.out + row * a.C, s, lane, a.C);
     }
 }
 
 template <typename T, int VEC, int G, int EPT>
-__global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormArgs<T> a) {
+__global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, true>())
+    norm_backward_kernel(const NormArgs<T> a) {
     using acc = typename Elem<T>::acc;
     constexpr int NV = EPT / VEC, kGroups = kNormThreads / G;
     constexpr int kCols = G * EPT;  // widest row of this form
-    __shared__ acc red[2 * kNormThreads / 32];
+    __shared__ acc red[2][2][kNormThreads / 32];
+    int half = 0;
     __shared__ acc cols[kGroups > 1 ? kCols : 1];
     const int group = threadIdx.x / G, lane = threadIdx.x % G;
     grid_dependency_wait();
@@ -203,7 +220,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
     for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0;
     long long row = (long long)blockIdx.x * kGroups + group;
     fetch(row);
-    for (long long turn = (long long)blockIdx.x * kGroups; turn < a.rows; turn += step, row += step) {
+    for (; row < a.rows; row += step) {
         acc z[EPT], g[EPT], t[EPT];
         x.widen(z);
         if (a.residual != nullptr) {
@@ -215,7 +232,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
         const acc mean = mean_n, rstd = rstd_n;
         fetch(row + step);
         w.widen(t);
-        acc sg = 0, sgz = 0;
+        acc sums[2] = {0, 0};  // of g and of g z
 #pragma unroll
         for (int i = 0; i < EPT; ++i) {
             // outside the row g is zero (dy was loaded as zero), so z's value there counts for nothing
@@ -223,16 +240,14 @@ __global__ void __launch_bounds__(kNormThreads) norm_backward_kernel(const NormA
             db[i] += g[i];
             dw[i] += g[i] * z[i];
             g[i] *= t[i];
-            sg += g[i];
-            sgz += g[i] * z[i];
+            sums[0] += g[i];
+            sums[1] += g[i] * z[i];
         }
-        sg = group_sum<G>(sg, red) * inv;
-        sgz = group_sum<G>(sgz, red + kNormThreads / 32) * inv;
-        if (row < a.rows) {
+        group_sum<G>(sums, red, half);
+        const acc sg = sums[0] * inv, sgz = sums[1] * inv;
 #pragma unroll
-            for (int i = 0; i < EPT; ++i) g[i] = (g[i] - sg - z[i] * sgz) * rstd;
-            store_row<T, VEC, NV, G>(a.out + row * a.C, g, lane, a.C);
-        }
+        for (int i = 0; i < EPT; ++i) g[i] = (g[i] - sg - z[i] * sgz) * rstd;
+        store_row<T, VEC, NV, G>(a.out + row * a.C, g, lane, a.C);
     }
     // the CTA's column sums: group 0's, + group 1's, .. in order
     acc* part = a.partial + (long long)blockIdx.x * 2 * a.C;
