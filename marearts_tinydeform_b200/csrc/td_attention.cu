@@ -111,11 +111,11 @@ int check_sizes(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t H
     return TD_OK;
 }
 
-AttnArgs make_args(const void* q, const void* k, const void* v, const int64_t* strides, const uint8_t* mask,
+AttnArgs make_args(int dtype, const void* q, const void* k, const void* v_, const int64_t* strides, const uint8_t* mask,
                    const int64_t* mask_strides, const uint8_t* padding, int64_t B, int64_t Q, int64_t N, int64_t H,
                    int64_t Hk, int64_t D, double scale, int causal) {
     AttnArgs a = {};
-    a.q = q; a.k = k; a.v = v;
+    a.q = q; a.k = k; a.v = v_;
     a.q_b = strides[0]; a.q_t = strides[1]; a.q_h = strides[2];
     a.k_b = strides[3]; a.k_t = strides[4]; a.k_h = strides[5];
     a.v_b = strides[6]; a.v_t = strides[7]; a.v_h = strides[8];
@@ -128,6 +128,14 @@ AttnArgs make_args(const void* q, const void* k, const void* v, const int64_t* s
     a.Qp = int(pad_rows(Q));
     a.causal = causal != 0;
     a.scale = scale;
+    const int64_t v = 16 / int64_t(elem_bytes(dtype));
+    auto whole = [&](const void* p, long long s_b, long long s_t, long long s_h) {
+        return D % v == 0 && s_b % v == 0 && s_t % v == 0 && s_h % v == 0 &&
+               (reinterpret_cast<uintptr_t>(p) & 15u) == 0;
+    };
+    a.vec_q = whole(q, a.q_b, a.q_t, a.q_h);
+    a.vec_k = whole(k, a.k_b, a.k_t, a.k_h);
+    a.vec_v = whole(v_, a.v_b, a.v_t, a.v_h);
     return a;
 }
 
@@ -274,7 +282,7 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
     const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
     const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, Hk, D, mb, mh, key_padding_mask != nullptr, false);
     if (int rc = check_workspace(workspace, workspace_bytes, N > 0 ? ws.total : 0, err, err_len)) return rc;
-    AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
+    AttnArgs a = make_args(dtype, query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
     a.out = out;
     a.rest = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
@@ -320,12 +328,13 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
     const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
     const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, Hk, D, mb, mh, key_padding_mask != nullptr, true);
     if (int rc = check_workspace(workspace, workspace_bytes, ws.total, err, err_len)) return rc;
-    AttnArgs a = make_args(query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
+    AttnArgs a = make_args(dtype, query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
                            scale, causal);
     a.out_in = out;
     a.rest_in = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
     a.lse = const_cast<void*>(lse);
     a.grad_out = grad_out;
+    a.vec_g = D % (16 / int64_t(elem_bytes(dtype))) == 0 && (reinterpret_cast<uintptr_t>(grad_out) & 15u) == 0;
     a.grad_q = grad_query;
     a.grad_k = grad_key;
     a.grad_v = grad_value;

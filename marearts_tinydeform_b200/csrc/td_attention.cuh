@@ -50,6 +50,7 @@ struct AttnArgs {
     long long m_b, m_h, m_q;
     const uint8_t* padding;         // [B, N], nonzero = no key there; or null
     int B, Q, N, H, Hk, D, Qp;
+    int vec_q, vec_k, vec_v, vec_g; // CUDA-core kernels: rows of q, k, v, grad_out are whole aligned 16-byte vectors
     int causal;                     // key j is open to query i while j <= i + (N - Q)
     double scale;
 };
@@ -84,11 +85,32 @@ struct SimtTile {
 };
 
 // ROWS rows from t0 on of a [tokens, D] slice into shared memory, widened; rows at or past n, padded rows and columns
-// past D are zero.
+// past D are zero. vec: rows are whole 16-byte vectors on 16-byte boundaries; all of a thread's loads are then in flight
+// together (one 64 x 64 tile in float32: 12.0 us with single elements).
 template <typename T, typename A, int DP, int ROWS>
 __device__ __forceinline__ void simt_load(A* dst, const T* src, long long stride, int t0, int n, int D,
-                                          const uint8_t* pad) {
+                                          const uint8_t* pad, bool vec) {
     constexpr int kLd = SimtTile<A, DP, 1, 1>::kLd;
+    if (vec) {
+        constexpr int V = Elem<T>::kVec, kPieces = DP / V, kTurns = (ROWS * kPieces + 255) / 256;
+        uint4 x[kTurns];
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+            const int i = int(threadIdx.x) + 256 * u, r = i / kPieces, c = i % kPieces * V;
+            x[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (i < ROWS * kPieces && t0 + r < n && c < D && (pad == nullptr || pad[t0 + r] == 0))
+                x[u] = __ldg(reinterpret_cast<const uint4*>(src + (t0 + r) * stride + c));
+        }
+#pragma unroll
+        for (int u = 0; u < kTurns; ++u) {
+            const int i = int(threadIdx.x) + 256 * u, r = i / kPieces, c = i % kPieces * V;
+            if (i >= ROWS * kPieces) continue;
+            struct alignas(16) Wide { A e[V]; } w;
+            unpack16<T>(x[u], w.e);
+            *reinterpret_cast<Wide*>(dst + r * kLd + c) = w;
+        }
+        return;
+    }
 #pragma unroll 4
     for (int i = threadIdx.x; i < ROWS * DP; i += 256) {
         const int r = i / DP, c = i % DP;
@@ -217,8 +239,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
         const int tiles = (a.N + M - 1) / M;
         const int j0 = blockIdx.x % tiles * M, hk = blockIdx.x / tiles % a.Hk, b = blockIdx.x / tiles / a.Hk;
         const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
-        simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
-        simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad, a.vec_k != 0);
+        simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad, a.vec_v != 0);
         A dk[R][Tile::kWidth], dv[R][Tile::kWidth];
 #pragma unroll
         for (int r = 0; r < R; ++r)
@@ -232,9 +254,9 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
             const A* delta_h = delta + ((long long)b * a.H + h) * a.Qp;
             for (int i0 = first; i0 < a.Q; i0 += M) {
                 __syncthreads();
-                simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+                simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr, a.vec_q != 0);
                 simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q,
-                                       a.D, nullptr);
+                                       a.D, nullptr, a.vec_g != 0);
                 __syncthreads();
                 A s[R][R], p[R][R];
                 simt_dot<A, DP, R, R>(ks, qs, ty, tx, s);
@@ -288,8 +310,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
     const int i0 = blk % tiles * M, h = blk / tiles % a.H, b = blk / tiles / a.H, hk = h / group;
     const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
-    simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
-    simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr);
+    simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr, a.vec_q != 0);
+    simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr, a.vec_g != 0);
     A dq[R][Tile::kWidth], li[R], di[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {
@@ -303,8 +325,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
     const int key_end = attn_key_end(a, i0 + M);
     for (int j0 = 0; j0 < key_end; j0 += M) {
         __syncthreads();
-        simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
-        simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad, a.vec_k != 0);
+        simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad, a.vec_v != 0);
         __syncthreads();
         A s[R][R], dp[R][R];
         simt_dot<A, DP, R, R>(qs, ks, ty, tx, s);

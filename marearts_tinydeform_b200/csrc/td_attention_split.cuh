@@ -418,7 +418,8 @@ __global__ void __launch_bounds__(256) attn_simt_forward_kernel(const SplitArgs 
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
     grid_dependency_wait();
     launch_dependents();
-    simt_load<T, A, DP, M>(qs, static_cast<const T*>(a.q) + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr);
+    simt_load<T, A, DP, M>(qs, static_cast<const T*>(a.q) + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr,
+                            a.vec_q != 0);
     A m[RM], l[RM], o[RM][Tile::kWidth];
 #pragma unroll
     for (int r = 0; r < RM; ++r) {
@@ -430,8 +431,10 @@ __global__ void __launch_bounds__(256) attn_simt_forward_kernel(const SplitArgs 
     const int key_end = min((long long)attn_key_end(a, i0 + M), (long long)(split + 1) * args.split_keys);
     for (int j0 = split * args.split_keys; j0 < key_end; j0 += KN) {
         __syncthreads();  // the tiles of the turn before have been read
-        simt_load<T, A, DP, KN>(ks, static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad);
-        simt_load<T, A, DP, KN>(vs, static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad);
+        simt_load<T, A, DP, KN>(ks, static_cast<const T*>(a.k) + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad,
+                                 a.vec_k != 0);
+        simt_load<T, A, DP, KN>(vs, static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad,
+                                 a.vec_v != 0);
         __syncthreads();
         A s[RM][RN];
         simt_dot<A, DP, RM, RN>(qs, ks, ty, tx, s);
