@@ -15,7 +15,7 @@ DTYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
 SHAPES = [(1, 1, 1, 1, 1, 32), (2, 7, 5, 4, 2, 16), (1, 300, 300, 8, 8, 32), (2, 129, 257, 4, 1, 64),
           (1, 128, 128, 2, 2, 128), (2, 200, 333, 6, 3, 24), (1, 130, 70, 2, 1, 20), (3, 2, 1000, 8, 4, 32),
           (1, 65, 1, 2, 2, 64), (2, 257, 129, 4, 2, 128), (2, 1, 2500, 4, 1, 64), (1, 9, 700, 3, 1, 96),
-          (1, 1, 4097, 16, 2, 128), (2, 448, 640, 2, 2, 40)]
+          (1, 1, 4097, 16, 2, 128), (2, 448, 640, 2, 2, 40), (2, 9, 1500, 6, 2, 32), (1, 40, 2100, 2, 2, 72)]
 MASKS = ('none', 'padding', 'pairs', 'pairs-all', 'causal', 'everything')
 NAMES = ('out', 'grad_query', 'grad_key', 'grad_value')
 
@@ -219,6 +219,18 @@ def test_offsets_beyond_32_bits(cuda):
         t.copy_(x)
     for name, got, want in zip(NAMES, run(q, k, v, ref[3]), run(*ref)):
         assert torch.equal(got, want), name
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_one_key_has_no_gradient_through_the_scores(cuda, dtype):
+    """The probability of an only key is one whatever the scores: gradients of query and key are exactly zero."""
+    for shape in ((2, 1, 1, 4, 2, 32), (1, 70, 1, 2, 2, 128), (3, 5, 1, 2, 1, 20)):
+        q, k, v, grad = inputs(shape, dtype, 13)
+        out, dq, dk, _ = run(q * 5, k, v, grad)
+        assert not dq.any() and not dk.any()
+        G = shape[3] // shape[4]
+        want = v.repeat_interleave(G, 2).expand(shape[0], shape[1], shape[3], shape[5]).reshape(out.shape)
+        assert torch.equal(out, want)
 
 
 def test_no_queries_no_keys(cuda):
