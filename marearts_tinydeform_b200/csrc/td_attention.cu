@@ -2,6 +2,7 @@
 #include <algorithm>
 
 #include "td_attention_plan.h"
+#include "td_attention_tf32.cuh"
 
 namespace td {
 
@@ -223,6 +224,48 @@ bool prefer_split(const AttnArgs& a) {
     return split < walk;
 }
 
+// float32 on tensor cores: rows of whole 16-byte vectors and at least 256 keys. Below, where a CTA has a few tiles, its
+// four warps' longer chains show (one head, 64 x 64: 12 us at D = 32 and 44 at D = 128 against 9 and 24 on CUDA cores;
+// 256 keys: 14 and 30 against 14 and 31; 4 x 1100 x 8 heads x 32: 152 against 233, the backward 445 against 699).
+bool tf32_fits(const AttnArgs& a) {
+    return host::best_policy() && a.N >= 256 && a.vec_q && a.vec_k && a.vec_v && (a.grad_q == nullptr || a.vec_g) &&
+           (reinterpret_cast<uintptr_t>(a.lse) & 15u) == 0;
+}
+
+template <int DP, int NT>
+int tf32_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* workspace, cudaStream_t stream, char* err,
+                 size_t err_len) {
+    using Lay = Tf32Layout<DP, NT>;
+    SplitArgs p = simt_split_plan(TD_F32, a.B, a.Q, a.N, a.H, a.D);
+    p.a = a;
+    p.part_o = workspace + w.part_o;
+    p.part_ml = workspace + w.part_ml;
+    constexpr auto kernel = attn_tf32_forward_kernel<DP, NT>;
+    constexpr size_t smem = (Lay::kFixed + 4 * Lay::kTile) * sizeof(float);
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
+    const long long grid = (long long)p.splits * p.row_tiles * a.B * a.H;
+    if (int rc = host::launch(err, err_len, "attn_tf32_forward_kernel", kernel, dim3(unsigned(grid)),
+                              dim3(kTf32Threads), smem, stream, true, p))
+        return rc;
+    return combine<float>(p, stream, err, err_len);
+}
+
+template <int DP, int NT>
+int tf32_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
+    using Lay = Tf32Layout<DP, NT>;
+    constexpr auto kernel = attn_tf32_backward_kernel<DP, NT>;
+    constexpr size_t smem = (2 * Lay::kFixed + 4 * Lay::kTile + 4 * NT) * sizeof(float);
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
+    const long long rows = (long long)a.B * a.H * a.Qp;
+    if (int rc = host::launch(err, err_len, "attn_delta_kernel", attn_delta_kernel<float>,
+                              dim3(unsigned((rows + 255) / 256)), dim3(256), 0, stream, true, a))
+        return rc;
+    const int kv_blocks = (a.N + kTf32Rows - 1) / kTf32Rows * a.B * a.Hk;
+    const int q_blocks = (a.Q + kTf32Rows - 1) / kTf32Rows * a.B * a.H;
+    return host::launch(err, err_len, "attn_tf32_backward_kernel", kernel, dim3(unsigned(kv_blocks) + q_blocks),
+                        dim3(kTf32Threads), smem, stream, true, a, kv_blocks);
+}
+
 template <typename T, int DP>
 int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
     constexpr int R = simt_r<T>();
@@ -243,6 +286,13 @@ int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_
 template <typename T>
 int forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned char* workspace, cudaStream_t stream,
             char* err, size_t err_len) {
+    if constexpr (std::is_same<T, float>::value) {
+        if (a.Q > 16 && tf32_fits(a)) {
+            if (a.D <= 32) return tf32_forward<32, 64>(a, w, workspace, stream, err, err_len);
+            if (a.D <= 64) return tf32_forward<64, 64>(a, w, workspace, stream, err, err_len);
+            return tf32_forward<128, 32>(a, w, workspace, stream, err, err_len);
+        }
+    }
     if (a.D <= 32) return simt_forward<T, 32>(a, dtype, w, workspace, stream, err, err_len);
     if (a.D <= 64) return simt_forward<T, 64>(a, dtype, w, workspace, stream, err, err_len);
     return simt_forward<T, 128>(a, dtype, w, workspace, stream, err, err_len);
@@ -250,6 +300,13 @@ int forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned char*
 
 template <typename T>
 int backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
+    if constexpr (std::is_same<T, float>::value) {
+        if (tf32_fits(a)) {
+            if (a.D <= 32) return tf32_backward<32, 64>(a, stream, err, err_len);
+            if (a.D <= 64) return tf32_backward<64, 32>(a, stream, err, err_len);
+            return tf32_backward<128, 32>(a, stream, err, err_len);
+        }
+    }
     if (a.D <= 32) return simt_backward<T, 32>(a, stream, err, err_len);
     if (a.D <= 64) return simt_backward<T, 64>(a, stream, err, err_len);
     return simt_backward<T, 128>(a, stream, err, err_len);

@@ -99,7 +99,7 @@ int pack_masks(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, bo
     }
     const long long blocks = w.images * w.heads * q_tiles * k_tiles;
     if (blocks > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "attn_mask is too large");
-    return host::launch(err, err_len, "attn_pack_kernel", attn_pack_kernel, dim3(unsigned(blocks)), dim3(256), 0,
+    return host::launch(err, err_len, "attn_pack_kernel", attn_pack_kernel, dim3(unsigned(blocks)), dim3(kPackThreads), 0,
                         stream, true, p);
 }
 

@@ -1005,7 +1005,8 @@ struct PackArgs {
     int words, col_words;            // 2 * ceil(N / 64), 2 * ceil(Q / 64)
 };
 
-__global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
+constexpr int kPackThreads = 512;
+__global__ void __launch_bounds__(kPackThreads) attn_pack_kernel(const PackArgs a) {
     __shared__ uint32_t pairs[128][4], all_rows[128][4];  // the mask's bits, and with the padding's
     __shared__ uint32_t cols[128][4];
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
@@ -1028,7 +1029,7 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
     }
     // four rows a warp at a time, so that 16 loads are in flight
     const int rows = min(128, a.rows - qt * 128);
-    for (int r0 = warp * 4; r0 < 128; r0 += 32) {
+    for (int r0 = warp * 4; r0 < 128; r0 += kPackThreads / 8) {
         bool open[4][4];
 #pragma unroll
         for (int x = 0; x < 4; ++x)
@@ -1051,7 +1052,7 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
     }
     __syncthreads();
     const long long bh = (long long)b * a.heads + h;
-    for (int e = threadIdx.x; e < 128 * 4; e += 256) {
+    for (int e = threadIdx.x; e < 128 * 4; e += kPackThreads) {
         const int i = qt * 128 + e / 4, w = kt * 4 + e % 4;
         if (i < a.rows && w < a.words) a.row_bits[(bh * a.rows + i) * a.words + w] = all_rows[e / 4][e % 4];
     }
@@ -1068,7 +1069,7 @@ __global__ void __launch_bounds__(256) attn_pack_kernel(const PackArgs a) {
         if (lane == 0 && t < tiles) a.row_flags[(bh * q_tiles + qt) * tiles + t] = uint8_t(some) | uint8_t(full) << 1;
     }
     if (a.col_bits == nullptr || b >= a.mask_images) return;
-    for (int e = threadIdx.x; e < 128 * 4; e += 256) {
+    for (int e = threadIdx.x; e < 128 * 4; e += kPackThreads) {
         const int key = e % 128, qw = e / 128;
         uint32_t word = 0;
 #pragma unroll 8

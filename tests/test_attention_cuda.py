@@ -15,7 +15,8 @@ DTYPES = (torch.float32, torch.float16, torch.bfloat16, torch.float64)
 SHAPES = [(1, 1, 1, 1, 1, 32), (2, 7, 5, 4, 2, 16), (1, 300, 300, 8, 8, 32), (2, 129, 257, 4, 1, 64),
           (1, 128, 128, 2, 2, 128), (2, 200, 333, 6, 3, 24), (1, 130, 70, 2, 1, 20), (3, 2, 1000, 8, 4, 32),
           (1, 65, 1, 2, 2, 64), (2, 257, 129, 4, 2, 128), (2, 1, 2500, 4, 1, 64), (1, 9, 700, 3, 1, 96),
-          (1, 1, 4097, 16, 2, 128), (2, 448, 640, 2, 2, 40), (2, 9, 1500, 6, 2, 32), (1, 40, 2100, 2, 2, 72)]
+          (1, 1, 4097, 16, 2, 128), (2, 448, 640, 2, 2, 40), (2, 9, 1500, 6, 2, 32), (1, 40, 2100, 2, 2, 72),
+          (2, 260, 300, 4, 2, 60), (1, 300, 390, 2, 1, 124)]
 MASKS = ('none', 'padding', 'pairs', 'pairs-all', 'causal', 'everything')
 NAMES = ('out', 'grad_query', 'grad_key', 'grad_value')
 
