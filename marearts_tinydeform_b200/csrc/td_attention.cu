@@ -24,7 +24,8 @@ void split_plan(int64_t blocks, int64_t N, int64_t waves, int64_t least, int64_t
 
 // The mma.sync split kernel's plan: the rows of a key head's group in tiles of 16. One wave of long splits where every
 // image has all its keys; shorter ones where some have not, so that the CTAs of the full ones do not end last (8 images
-// of 22223 keys, the lengths falling to half: 48 us with 2, 42 with 6; all of them full: 43 and 43; one image: 12 and 17).
+// of 22223 keys, the lengths falling to half: 48 us with 2, 42 with 6; all of them full: 43 and 43; one image: 12 and
+// 17).
 SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, bool padding) {
     SplitArgs p = {};
     p.row_tiles = int((H / Hk * Q + 15) / 16);
@@ -211,10 +212,10 @@ int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* 
 
 // Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. In microseconds, as
 // measured on B200 over 1 to 16 images, 8 and 16 heads, D = 32, 64 and 128, 40 to 22223 keys and 1 to 300 queries:
-// the tensor-core kernel walks all keys of a 128-query tile in one CTA, about 10 ns a key (13 for wide heads) and wave of
-// 296 CTAs; the split kernel's time goes with its 16-row tiles times keys, behind about 7 for two launches. Below 1024
-// keys the two differ by little (300 keys, one query: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128). Where the
-// estimates are near each other so are the kernels (at most a fifth apart where the wrong one is taken).
+// the tensor-core kernel walks all keys of a 128-query tile in one CTA, about 10 ns a key (13 for wide heads) and wave
+// of 296 CTAs; the split kernel's time goes with its 16-row tiles times keys, behind about 7 for two launches. Below
+// 1024 keys the two differ by little (300 keys, one query: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128).
+// Where the estimates are near each other so are the kernels (at most a fifth apart where the wrong one is taken).
 bool prefer_split(const AttnArgs& a) {
     if (a.N < 1024) return false;
     const double ctas = double((a.Q + 127) / 128) * a.B * a.H;
@@ -326,9 +327,9 @@ size_t td_attention_workspace_bytes(int dtype, int64_t B, int64_t Q, int64_t N, 
 
 int td_attention_forward(int dtype, const void* query, const void* key, const void* value, const int64_t* strides,
                          const uint8_t* attn_mask, const int64_t* mask_strides, const uint8_t* key_padding_mask,
-                         void* out, void* rest, void* lse, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D,
-                         double scale, int causal, void* workspace, size_t workspace_bytes, void* stream, char* err,
-                         size_t err_len) {
+                         void* out, void* rest, void* lse, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
+                         int64_t D, double scale, int causal, void* workspace, size_t workspace_bytes, void* stream,
+                         char* err, size_t err_len) {
     using namespace td;
     if (int rc = check_sizes(dtype, B, Q, N, H, Hk, D, scale, err, err_len)) return rc;
     if (B == 0 || Q == 0) return TD_OK;
@@ -339,8 +340,8 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
     const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
     const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, Hk, D, mb, mh, key_padding_mask != nullptr, false);
     if (int rc = check_workspace(workspace, workspace_bytes, N > 0 ? ws.total : 0, err, err_len)) return rc;
-    AttnArgs a = make_args(dtype, query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
-                           scale, causal);
+    AttnArgs a = make_args(dtype, query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H,
+                           Hk, D, scale, causal);
     a.out = out;
     a.rest = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
     a.lse = lse;
@@ -361,9 +362,9 @@ int td_attention_forward(int dtype, const void* query, const void* key, const vo
 
 int td_attention_backward(int dtype, const void* query, const void* key, const void* value, const int64_t* strides,
                           const uint8_t* attn_mask, const int64_t* mask_strides, const uint8_t* key_padding_mask,
-                          const void* out, const void* rest, const void* lse, const void* grad_out, void* grad_query, void* grad_key,
-                          void* grad_value, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D,
-                          double scale, int causal, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                          const void* out, const void* rest, const void* lse, const void* grad_out, void* grad_query,
+                          void* grad_key, void* grad_value, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
+                          int64_t D, double scale, int causal, void* workspace, size_t workspace_bytes, void* stream, char* err,
                           size_t err_len) {
     using namespace td;
     if (int rc = check_sizes(dtype, B, Q, N, H, Hk, D, scale, err, err_len)) return rc;
@@ -385,8 +386,8 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
     const int64_t mh = attn_mask == nullptr ? 0 : mask_strides[1] != 0 ? H : 1;
     const AttnWorkspace ws = attn_workspace(dtype, B, Q, N, H, Hk, D, mb, mh, key_padding_mask != nullptr, true);
     if (int rc = check_workspace(workspace, workspace_bytes, ws.total, err, err_len)) return rc;
-    AttnArgs a = make_args(dtype, query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H, Hk, D,
-                           scale, causal);
+    AttnArgs a = make_args(dtype, query, key, value, strides, attn_mask, mask_strides, key_padding_mask, B, Q, N, H,
+                           Hk, D, scale, causal);
     a.out_in = out;
     a.rest_in = dtype == TD_F16 || dtype == TD_BF16 ? rest : nullptr;
     a.lse = const_cast<void*>(lse);

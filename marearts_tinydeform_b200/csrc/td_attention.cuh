@@ -85,8 +85,8 @@ struct SimtTile {
 };
 
 // ROWS rows from t0 on of a [tokens, D] slice into shared memory, widened; rows at or past n, padded rows and columns
-// past D are zero. vec: rows are whole 16-byte vectors on 16-byte boundaries; all of a thread's loads are then in flight
-// together (one 64 x 64 tile in float32: 12.0 us with single elements).
+// past D are zero. vec: rows are whole 16-byte vectors on 16-byte boundaries; all of a thread's loads are then in
+// flight together (one 64 x 64 tile in float32: 12.0 us with single elements).
 template <typename T, typename A, int DP, int ROWS>
 __device__ __forceinline__ void simt_load(A* dst, const T* src, long long stride, int t0, int n, int D,
                                           const uint8_t* pad, bool vec) {
@@ -311,7 +311,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
     const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
     const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
     simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr, a.vec_q != 0);
-    simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr, a.vec_g != 0);
+    simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q, a.D, nullptr,
+                           a.vec_g != 0);
     A dq[R][Tile::kWidth], li[R], di[R];
 #pragma unroll
     for (int r = 0; r < R; ++r) {

@@ -12,7 +12,8 @@
 // fragments (the queries are loaded in the same order), and a thread's consecutive elements of a value row are the
 // same column of as many 8-wide result tiles; the pairs of keys that a value fragment packs are made with byte
 // permutes. Tensor cores matter little here, but a 16-row product on them costs what a one-row product on CUDA cores
-// would.
+// would. One query over 22223 keys, 8 images of 8 heads x 32 in bfloat16: 42 us (4.3 TB/s; 3.4 with lengths falling to
+// half), which the twelve warps' latency an SM sets, not the memory; loads straight into registers took 62.
 #pragma once
 
 #include "td_attention.cuh"
@@ -147,7 +148,7 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
     const T* vp = static_cast<const T*>(a.v) + b * a.v_b + hk * a.v_h;
     const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
     const int off = a.N - a.Q;
-    const int end = min(min(a.N, (split + 1) * args.split_keys), attn_key_end(a, a.Q));
+    const int end = int(min((long long)attn_key_end(a, a.Q), (split + 1LL) * args.split_keys));
 
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f}, o[kDims][4];
 #pragma unroll

@@ -46,8 +46,8 @@ bool operand_fits(const Operand& o, const AttnArgs& a) {
     return aligned16(o.base);
 }
 
-// Boxes of min(DP, 64) columns x 64 tokens of one head of one image (a resident operand of 128 rows takes two, which lie
-// behind one another as one of 128 would); what lies outside reads as zero.
+// Boxes of min(DP, 64) columns x 64 tokens of one head of one image (a resident operand of 128 rows takes two, which
+// lie behind one another as one of 128 would); what lies outside reads as zero.
 template <int DP>
 int make_map(CUtensorMap* map, const Operand& o, const AttnArgs& a, char* err, size_t err_len) {
     const uint64_t dims[4] = {uint64_t(a.D), uint64_t(o.tokens), uint64_t(o.heads), uint64_t(a.B)};
@@ -99,8 +99,8 @@ int pack_masks(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, bo
     }
     const long long blocks = w.images * w.heads * q_tiles * k_tiles;
     if (blocks > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "attn_mask is too large");
-    return host::launch(err, err_len, "attn_pack_kernel", attn_pack_kernel, dim3(unsigned(blocks)), dim3(kPackThreads), 0,
-                        stream, true, p);
+    return host::launch(err, err_len, "attn_pack_kernel", attn_pack_kernel, dim3(unsigned(blocks)),
+                        dim3(kPackThreads), 0, stream, true, p);
 }
 
 template <typename T, int DP, bool EXACT>
@@ -145,8 +145,8 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
     constexpr size_t smem = AttnBwdLayout<DP>::kSmemBytes;
     if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     const unsigned grid = unsigned(t.kv_blocks) + unsigned((a.Q + kAttnBM - 1) / kAttnBM) * unsigned(a.B * a.H);
-    return host::launch(err, err_len, "attn_tc_backward_kernel", kernel, dim3(grid), dim3(AttnBwdLayout<DP>::kThreads), smem, stream,
-                        true, q, g, k, v, t);
+    return host::launch(err, err_len, "attn_tc_backward_kernel", kernel, dim3(grid),
+                        dim3(AttnBwdLayout<DP>::kThreads), smem, stream, true, q, g, k, v, t);
 }
 
 }  // namespace
@@ -154,9 +154,9 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
 bool attn_tc_fits(int dtype, const AttnArgs& a) {
     if ((dtype != TD_F16 && dtype != TD_BF16) || !host::best_policy()) return false;
     if (a.D % 8 != 0) return false;
-    // One key, where the gradients of queries and keys are zero: the CUDA-core kernels form dP and delta in one order and
-    // find it so (3.5 us against 4.6). Up to 32 keys, the backward: sums of so few terms show each rounding of dS, which
-    // float32 throughout does without (8 images of 8 heads x 32, 32 keys: 9 us against 18).
+    // One key, where the gradients of queries and keys are zero: the CUDA-core kernels form dP and delta in one order
+    // and find it so (3.5 us against 4.6). Up to 32 keys, the backward: sums of so few terms show each rounding of dS,
+    // which float32 throughout does without (8 images of 8 heads x 32, 32 keys: 9 us against 18).
     if (a.N < (a.grad_q == nullptr ? 2 : 33)) return false;
     if (!operand_fits(query_of(a), a) || !operand_fits(key_of(a), a) || !operand_fits(value_of(a), a)) return false;
     if (!aligned16(a.lse)) return false;

@@ -6,10 +6,10 @@
 //   keys' grad       S^T = K Q^T, dP^T = V dO^T (lanes = keys), dV += P^T dO, dK += dS^T Q
 // so a 128-row operand stays in shared memory (K-major), tiles of 64 rows of the other side stream through a ring of
 // TMA slots, and each streamed tile serves as a K-major operand of one product and as an MN-major operand of another.
-// P and dS are rounded to the input type and written back to TMEM over the scores they came from, as the A operand of
-// the next product: neither ever reaches shared memory. The two gradients are separate blocks of one launch, each of
-// which forms S and dP itself: 7 products instead of 5 and twice the exponentials, but every sum has one owner and one
-// order (no atomics, no float32 gradient in memory).
+// P and dS are rounded to the input type (the products take 16 bits; their sums are float32) and written back to TMEM
+// over the scores they came from, as the A operand of the next product: neither ever reaches shared memory. The two
+// gradients are separate blocks of one launch, each of which forms S and dP itself: 7 products instead of 5 and twice
+// the exponentials, but every sum has one owner and one order (no atomics, no float32 gradient in memory).
 //
 // Columns past D (D < DP) and rows past the last token are zero through the tensor maps' fill. Scores of closed pairs
 // are replaced by -infinity (P, dS by zero); tiles without an open pair are skipped by every role alike, from one
@@ -17,9 +17,14 @@
 // may hold anything, are cleared in shared memory where they are summed over (V in the forward, K in the queries'
 // gradient): zero times infinity is no zero.
 //
-// The exponential bounds these kernels at D <= 64 (16 a cycle and SM against 8192 multiply-adds), so the forward
-// runs two CTAs an SM (256 TMEM columns each), the backward two elementwise warpgroups a CTA, each on its own
-// tile; in both the next tile's scores are being formed meanwhile.
+// What bounds them is the time a tile takes through its stations rather than any unit: barrier, product, commit and
+// TMEM latencies and, in the elementwise warps, instructions that wait for one another. So the forward runs two CTAs an
+// SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two or three elementwise warpgroups
+// over two or three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their
+// waits (encoder backward below: 827 to 598 us); everything between two tiles is kept short. Measured: 2 x 4096 tokens,
+// 16 / 4 heads x 64, causal, bfloat16: 112 us (615 TFLOP/s). 8400 tokens, 8 heads x 32: forward 226 us (319 TFLOP/s of
+// the 32-wide products; half the rate of the exponentials, 16 a cycle and SM), EXACT 294, backward 506 (357 TFLOP/s).
+// 2 x 2047, 8 / 2 heads x 128, causal, float16: EXACT 48, backward 151 us (286 TFLOP/s).
 #pragma once
 
 #include <type_traits>
@@ -63,9 +68,9 @@ struct AttnBox {
 };
 
 // ---- PTX ----------------------------------------------------------------------------------------------------------
-// The MMA warps stay converged: every lane forms the (equal) operands, which the compiler so keeps in uniform registers,
-// and the lane with `leader` set issues. Inside a branch that one lane takes, each descriptor would be moved there anew,
-// which cost more than the products: a tile's 16 took about 1100 cycles to issue.
+// The MMA warps stay converged: every lane forms the (equal) operands, which the compiler so keeps in uniform
+// registers, and the lane with `leader` set issues. Inside a branch that one lane takes, each descriptor would be moved
+// there anew, which cost more than the products: a tile's 16 took about 1100 cycles to issue.
 // D[tmem] (+)= A[smem desc] x B[smem desc]^T
 __device__ __forceinline__ void mma_ss(uint32_t leader, uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                        uint32_t idesc, uint32_t accumulate) {
@@ -231,8 +236,8 @@ __device__ __forceinline__ bool for_tiles(int t0, int t1, const uint8_t* flags, 
     return true;
 }
 
-// A place in a ring of N and the parity of its round, stepped instead of divided: on a warp alone on its scheduler every
-// instruction between two tiles shows.
+// A place in a ring of N and the parity of its round, stepped instead of divided: on a warp alone on its scheduler
+// every instruction between two tiles shows.
 template <int N>
 struct Ring {
     int at = 0;
@@ -419,8 +424,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             if (job >= 0 && job < 2 * KB) {
                 uint64_t* bar = job < KB ? &kfull[s] : &vfull[s];
                 mbar_arrive_expect_tx(bar, AttnBox<DP>::kTile);
-                tma_load_4d((job < KB ? k_tile(s) : v_tile(s)) + box * AttnBox<DP>::kTile, job < KB ? &map_k : &map_v, bar,
-                            64 * box, t * kAttnBN, hk, b, pol);
+                tma_load_4d((job < KB ? k_tile(s) : v_tile(s)) + box * AttnBox<DP>::kTile,
+                            job < KB ? &map_k : &map_v, bar, 64 * box, t * kAttnBN, hk, b, pol);
             }
             __syncwarp();
             ++n;
@@ -629,8 +634,8 @@ struct AttnBwdLayout {
     static constexpr uint32_t kFixedBytes = AttnBox<DP>::kFixed * kBoxes;  // one resident operand
     static constexpr uint32_t kTileBytes = AttnBox<DP>::kTile * kBoxes;    // one streamed operand
     // score buffers (S and dP, 64 columns each) and ring slots. A buffer goes from the scores' product through the
-    // elementwise work to the products that read P and dS, about 2000 cycles in all, so the tiles in flight set the pace:
-    // three where TMEM holds them, two beside the accumulators of wide heads
+    // elementwise work to the products that read P and dS, about 2000 cycles in all, so the tiles in flight set the
+    // pace: three where TMEM holds them, two beside the accumulators of wide heads
     static constexpr int kBufs = DP == 128 ? 2 : 3;
     static constexpr int kStages = DP == 128 ? 4 : 6;
     static constexpr uint32_t kAcc = kBufs * 128;  // first accumulator's TMEM column
@@ -670,8 +675,9 @@ __device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {  // one
     return exp2f(fminf(fmaxf(15.f - ceilf(log2f(bound)), -100.f), 100.f));
 }
 
-// P and dS of one row of a tile of 64 columns, from the scores at sc and sc + 64 to packed pairs in the same places. The
-// statistics are the row's own, or (KEYS) the columns', lse[64] and delta[64] at st. MASKED: w has a bit per open pair.
+// P and dS of one row of a tile of 64 columns, from the scores at sc and sc + 64 to packed pairs in the same places.
+// The statistics are the row's own, or (KEYS) the columns', lse[64] and delta[64] at st. MASKED: w has a bit per open
+// pair.
 template <typename T, bool KEYS, bool MASKED>
 __device__ __forceinline__ void elementwise(uint32_t sc, const float* st, float row_lse, float row_delta, float c,
                                             float ds_scale, unsigned long long w) {
@@ -782,8 +788,8 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             const int job = lane - kJobs * s, box = job % KB;
             if (job >= 0 && job < 2 * KB) {
                 mbar_arrive_expect_tx(&full[s], AttnBox<DP>::kTile);
-                tma_load_4d((job < KB ? tile1(s) : tile2(s)) + box * AttnBox<DP>::kTile, job < KB ? &map_b1 : &map_b2, &full[s],
-                            64 * box, t * kAttnBN, KEYS ? h : hk, b, pol);
+                tma_load_4d((job < KB ? tile1(s) : tile2(s)) + box * AttnBox<DP>::kTile,
+                            job < KB ? &map_b1 : &map_b2, &full[s], 64 * box, t * kAttnBN, KEYS ? h : hk, b, pol);
             } else if (job >= 2 * KB && job < kJobs) {
                 const float* src = static_cast<const float*>(job == 2 * KB ? a.lse : a.delta);
                 mbar_arrive_expect_tx(&full[s], kAttnBN * 4u);

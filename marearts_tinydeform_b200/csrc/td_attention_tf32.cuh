@@ -1,7 +1,7 @@
 // td_attention_tf32.cuh -- float32 attention on tensor cores: every product in three TF32 ones.
 //
-// x = hi + lo with hi = x cut to TF32's 11 bits (exact) and lo = x - hi, so a b ~ hi hi + hi lo + lo hi to about 21 bits,
-// as the library's float32 projections do. Tiles of 64 rows, four warps of 16, as mma.sync m16n8k8 fragments; the
+// x = hi + lo with hi = x cut to TF32's 11 bits (exact) and lo = x - hi, so a b ~ hi hi + hi lo + lo hi to about 21
+// bits, as the library's float32 projections do. Tiles of 64 rows, four warps of 16, as mma.sync m16n8k8 fragments; the
 // other side streams through two buffers of shared memory by asynchronous copies. What bounds it: the rate of these
 // products (about 38 TFLOP/s are left of three) and, with few tiles a CTA, one warp's chain of some 1500 instructions a
 // tile, 4.5 us. 8 heads x 32, 4 x 1100 tokens: forward 152 us (33 TFLOP/s), backward 445 us; 8 heads x 64, 4096 tokens:
@@ -170,7 +170,8 @@ __global__ void __launch_bounds__(kTf32Threads) attn_tf32_forward_kernel(const S
         __syncthreads();
         float s[NT / 8][4];
         tf32_scores<DP, NT>(qs + 16 * warp * Lay::kPitch, tile(buf, 0), g, t, s);
-        const bool plain = mask == nullptr && pad == nullptr && j0 + NT <= a.N && (!a.causal || j0 + NT - 1 <= i0 + off);
+        const bool plain = mask == nullptr && pad == nullptr && j0 + NT <= a.N &&
+                           (!a.causal || j0 + NT - 1 <= i0 + off);
         float keep[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

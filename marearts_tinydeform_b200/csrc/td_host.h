@@ -51,8 +51,8 @@ int launch(char* err, size_t err_len, const char* what, K kernel, dim3 grid, dim
     return TD_OK;
 }
 
-// Raises a kernel's dynamic shared memory limit where it needs more than the 48 KB every kernel has: the attribute is the
-// device's, so once per kernel and device (a host-side write, legal during capture; two threads may both do it).
+// Raises a kernel's dynamic shared memory limit where it needs more than the 48 KB every kernel has: the attribute is
+// the device's, so once per kernel and device (a host-side write, legal during capture; two threads may both do it).
 template <auto Kernel>
 int allow_smem(size_t bytes, char* err, size_t err_len) {
     static std::atomic<uint64_t> done{0};

@@ -89,11 +89,11 @@ def call_attention(lib, dtype=_native.TD_F16, B=1, Q=4, N=5, H=2, Hk=1, D=32, sc
     p = ctypes.c_void_p(ptr) if ptr else None
     strides = (ctypes.c_int64 * 9)(*[1] * 9)
     if backward:
-        rc = lib.td_attention_backward(dtype, p, p, p, strides, None, None, None, p, None, p, p, p, p, p, B, Q, N, H, Hk, D,
-                                       scale, 0, ctypes.c_void_p(ws), ws_bytes, None, err, 256)
+        rc = lib.td_attention_backward(dtype, p, p, p, strides, None, None, None, p, None, p, p, p, p, p, B, Q, N, H,
+                                       Hk, D, scale, 0, ctypes.c_void_p(ws), ws_bytes, None, err, 256)
     else:
-        rc = lib.td_attention_forward(dtype, p, p, p, strides, None, None, None, p, None, p, B, Q, N, H, Hk, D, scale, 0,
-                                      ctypes.c_void_p(ws), ws_bytes, None, err, 256)
+        rc = lib.td_attention_forward(dtype, p, p, p, strides, None, None, None, p, None, p, B, Q, N, H, Hk, D, scale,
+                                      0, ctypes.c_void_p(ws), ws_bytes, None, err, 256)
     return rc, err.value.decode()
 
 
