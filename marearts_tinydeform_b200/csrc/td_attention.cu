@@ -13,10 +13,9 @@ using host::fail;
 int64_t pad_rows(int64_t Q) { return (Q + kAttnRowPad - 1) / kAttnRowPad * kAttnRowPad; }
 size_t elem_bytes(int dtype) { return dtype == TD_F64 ? 8 : dtype == TD_F32 ? 4 : 2; }
 
-// How a forward is split over the keys: splits CTAs of split_keys keys each (a multiple of `step`) for every one of
-// `blocks`, enough of them for `waves` CTAs an SM, but no split of fewer than `least` keys.
-void split_plan(int64_t blocks, int64_t N, int64_t waves, int64_t least, int64_t step, SplitArgs* p) {
-    int64_t splits = std::max<int64_t>(1, std::min((waves * kSms + blocks - 1) / blocks, N / least));
+// How a forward is split over the keys: about `splits` CTAs of split_keys keys each, a multiple of `step`.
+void split_plan(int64_t N, int64_t splits, int64_t step, SplitArgs* p) {
+    splits = std::max<int64_t>(1, splits);
     const int64_t keys = std::max((N + splits - 1) / splits, int64_t(1));  // one without any key, too
     p->split_keys = int((keys + step - 1) / step * step);
     p->splits = int(std::max<int64_t>(1, (N + p->split_keys - 1) / p->split_keys));
@@ -25,11 +24,12 @@ void split_plan(int64_t blocks, int64_t N, int64_t waves, int64_t least, int64_t
 // The mma.sync split kernel's plan: the rows of a key head's group in tiles of 16. One wave of long splits where every
 // image has all its keys; shorter ones where some have not, so that the CTAs of the full ones do not end last (8 images
 // of 22223 keys, the lengths falling to half: 48 us with 2, 42 with 6; all of them full: 43 and 43; one image: 12 and
-// 17).
+// 17). No split of fewer than 256 keys, two of the kernel's tiles.
 SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, bool padding) {
     SplitArgs p = {};
     p.row_tiles = int((H / Hk * Q + 15) / 16);
-    split_plan(B * Hk * p.row_tiles, N, padding ? 6 : 2, 256, 128, &p);
+    const int64_t blocks = std::max(B * Hk * p.row_tiles, int64_t(1));
+    split_plan(N, std::min(((padding ? 6 : 2) * kSms + blocks - 1) / blocks, N / 256), 128, &p);
     return p;
 }
 
@@ -37,14 +37,35 @@ SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
 // a thread for up to 16 queries, where most of a taller tile would be empty.
 template <typename T> constexpr int simt_r() { return std::is_same<T, double>::value ? 2 : 4; }
 
-// 16-bit calls of the usual widths come here only misaligned or short: they do without partials.
+// The CUDA-core and the TF32 forward's plan: down to one tile of 64 keys a CTA, as long as all the CTAs are resident at
+// once, three an SM (float32, 8 heads of 32: 2 x 300 queries and keys 33 us in two splits, 24 in five; 2 x 64 on 200
+// keys 22 in one, 12 in four; 8 x 300 47 in one and 82 in two, which are more than a wave). 16-bit calls of the usual
+// widths come here only misaligned or short: they do without partials.
 SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t D) {
     SplitArgs p = {};
     const bool whole = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0;
     const int rows = Q <= 16 ? 16 : 16 * (dtype == TD_F64 ? 2 : 4);
     p.row_tiles = int((Q + rows - 1) / rows);
-    split_plan(B * H * p.row_tiles, N, 2, whole ? N + 1 : 128, 64, &p);
+    const int64_t blocks = std::max(B * H * p.row_tiles, int64_t(1));
+    split_plan(N, whole ? 1 : std::min(3 * kSms / blocks, (N + 63) / 64), 64, &p);
     return p;
+}
+
+// The backward: how many CTAs share the tiles that one tile of keys, or of queries, goes over, so that a few long ones
+// do not hold the others up: a key head's block goes over the queries of its whole group, and few queries make few
+// blocks. A CTA gets at most about the work of one of three on every SM, or, on tensor cores (one CTA an SM), of two;
+// but at least two tiles there, sixteen here, since partial sums and the launch that joins them cost about as much.
+// 16-bit causal 2 x 2047 x 8 heads (2 of keys) x 128: 150 us unsplit, 91; 1 query on 8400 keys x 8 heads x 32: 70 us
+// and 30, in float32 739 and 69; 2 x 300 queries on 8400 keys in float32: 961 and 516.
+void grad_splits(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t* k, int64_t* q) {
+    const bool tc = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0 && N > 32;  // (unless misaligned)
+    const int64_t rows = tc ? 128 : dtype == TD_F64 ? 32 : 64, cols = std::min<int64_t>(rows, 64);
+    auto tiles = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
+    const int64_t kc = H / Hk * tiles(Q, cols), qc = tiles(N, cols);
+    const int64_t work = B * (Hk * tiles(N, rows) * kc + H * tiles(Q, rows) * qc);
+    const int64_t chunk = std::max<int64_t>(tc ? 16 : 2, tiles(work, (tc ? 2 : 3) * kSms));
+    *k = std::max<int64_t>(1, (kc + chunk / 2) / chunk);
+    *q = std::max<int64_t>(1, (qc + chunk / 2) / chunk);
 }
 
 // The parts of a call's workspace. The mask's bits and flags are laid out for 16-bit types only (the tensor-core
@@ -63,9 +84,18 @@ AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t
     if (backward) {
         w.amax = take(2 * kSms * sizeof(float));
         w.delta = take(size_t(B) * H * pad_rows(Q) * acc);
+        int64_t k, q;
+        grad_splits(dtype, B, Q, N, H, Hk, D, &k, &q);
+        if (k > 1) {
+            w.part_k = take(size_t(B) * N * Hk * D * k * acc);
+            w.part_v = take(size_t(B) * N * Hk * D * k * acc);
+        }
+        if (q > 1) w.part_q = take(size_t(B) * Q * H * D * q * acc);
     } else {
         int64_t splits = simt_split_plan(dtype, B, Q, N, H, D).splits;
-        if (half) splits = std::max<int64_t>(splits, mma_split_plan(B, Q, N, H, Hk, padding).splits);
+        if (half)
+            splits = std::max({splits, int64_t(mma_split_plan(B, Q, N, H, Hk, padding).splits),
+                               attn_tc_splits(B, Q, N, H)});
         if (splits > 1) {
             w.part_o = take(size_t(B) * H * Q * splits * D * acc);
             w.part_ml = take(size_t(B) * H * Q * splits * 2 * acc);
@@ -149,14 +179,6 @@ int zero(void* p, size_t bytes, cudaStream_t stream, char* err, size_t err_len) 
     return fail(err, err_len, TD_ERR_CUDA, "memset: %s", cudaGetErrorString(e));
 }
 
-template <typename T>
-int combine(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
-    if (p.splits == 1) return TD_OK;
-    const long long rows = (long long)p.a.B * p.a.H * p.a.Q;
-    return host::launch(err, err_len, "attn_combine_kernel", attn_combine_kernel<T>, dim3(unsigned(rows)),
-                        dim3(kCombineWarps * 32), 0, stream, true, p);
-}
-
 template <typename T, int DP, int RM>
 int simt_forward_tile(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
     constexpr int RN = simt_r<T>();
@@ -210,18 +232,21 @@ int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* 
     return a.rest != nullptr ? go(std::true_type{}) : go(std::false_type{});
 }
 
-// Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. In microseconds, as
-// measured on B200 over 1 to 16 images, 8 and 16 heads, D = 32, 64 and 128, 40 to 22223 keys and 1 to 300 queries:
-// the tensor-core kernel walks all keys of a 128-query tile in one CTA, about 10 ns a key (13 for wide heads) and wave
-// of 296 CTAs; the split kernel's time goes with its 16-row tiles times keys, behind about 7 for two launches. Below
-// 1024 keys the two differ by little (300 keys, one query: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128).
-// Where the estimates are near each other so are the kernels (at most a fifth apart where the wrong one is taken).
+// Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. In microseconds, from
+// 216 calls of 1 to 8 images, 8 and 16 heads, D = 32, 64 and 128, 1024 to 22223 keys and 1 to 300 queries on B200: a
+// tensor-core CTA walks its keys at about 10 ns a key (13 for wide heads), and a launch that joins splits adds about 4;
+// the split kernel's time goes with its 16-row tiles times keys, behind about 6 for two launches. The faster kernel is
+// taken in all but a dozen of these calls, and the one taken is at most a quarter slower (64-wide heads, one query on
+// 22223 keys: 21 us against 17). Below 1024 keys the two differ by little (300 keys, one query: 6.3 against 5.0 at
+// D = 32, 7.6 against 9.7 at D = 128).
 bool prefer_split(const AttnArgs& a) {
     if (a.N < 1024) return false;
     const double ctas = double((a.Q + 127) / 128) * a.B * a.H;
     const double tiles = double((a.H / a.Hk * (long long)a.Q + 15) / 16) * a.B * a.Hk;
-    const double walk = 3.3 + 0.0103 * a.N * (a.D > 64 ? 1.25 : 1.0) * std::max(1.0, ctas / (2 * kSms));
-    const double split = 7.0 + tiles * a.N * (a.D <= 32 ? 5e-5 : a.D <= 64 ? 9e-5 : 1.8e-4);
+    const double splits = double(attn_tc_splits(a.B, a.Q, a.N, a.H));
+    const double walk = (splits > 1 ? 7.0 : 3.3) +
+                        0.0103 * a.N / splits * (a.D > 64 ? 1.25 : 1.0) * std::max(1.0, ctas / (2 * kSms));
+    const double split = 6.0 + tiles * a.N * (a.D <= 32 ? 3e-5 : a.D <= 64 ? 6e-5 : 1.2e-4);
     return split < walk;
 }
 
@@ -261,10 +286,12 @@ int tf32_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_
     if (int rc = host::launch(err, err_len, "attn_delta_kernel", attn_delta_kernel<float>,
                               dim3(unsigned((rows + 255) / 256)), dim3(256), 0, stream, true, a))
         return rc;
-    const int kv_blocks = (a.N + kTf32Rows - 1) / kTf32Rows * a.B * a.Hk;
-    const int q_blocks = (a.Q + kTf32Rows - 1) / kTf32Rows * a.B * a.H;
-    return host::launch(err, err_len, "attn_tf32_backward_kernel", kernel, dim3(unsigned(kv_blocks) + q_blocks),
-                        dim3(kTf32Threads), smem, stream, true, a, kv_blocks);
+    const int kv_blocks = (a.N + kTf32Rows - 1) / kTf32Rows * a.B * a.Hk * a.k_splits;
+    const int q_blocks = (a.Q + kTf32Rows - 1) / kTf32Rows * a.B * a.H * a.q_splits;
+    if (int rc = host::launch(err, err_len, "attn_tf32_backward_kernel", kernel, dim3(unsigned(kv_blocks) + q_blocks),
+                              dim3(kTf32Threads), smem, stream, true, a, kv_blocks))
+        return rc;
+    return join<float>(a, stream, err, err_len);
 }
 
 template <typename T, int DP>
@@ -278,10 +305,12 @@ int simt_backward(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_
     if (int rc = host::launch(err, err_len, "attn_delta_kernel", attn_delta_kernel<T>,
                               dim3(unsigned((rows + 255) / 256)), dim3(256), 0, stream, true, a))
         return rc;
-    const int kv_blocks = (a.N + Tile::kRows - 1) / Tile::kRows * a.B * a.Hk;
-    const int q_blocks = (a.Q + Tile::kRows - 1) / Tile::kRows * a.B * a.H;
-    return host::launch(err, err_len, "attn_simt_backward_kernel", kernel, dim3(unsigned(kv_blocks) + q_blocks),
-                        dim3(256), smem, stream, true, a, kv_blocks);
+    const int kv_blocks = (a.N + Tile::kRows - 1) / Tile::kRows * a.B * a.Hk * a.k_splits;
+    const int q_blocks = (a.Q + Tile::kRows - 1) / Tile::kRows * a.B * a.H * a.q_splits;
+    if (int rc = host::launch(err, err_len, "attn_simt_backward_kernel", kernel, dim3(unsigned(kv_blocks) + q_blocks),
+                              dim3(256), smem, stream, true, a, kv_blocks))
+        return rc;
+    return join<T>(a, stream, err, err_len);
 }
 
 template <typename T>
@@ -364,8 +393,8 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
                           const uint8_t* attn_mask, const int64_t* mask_strides, const uint8_t* key_padding_mask,
                           const void* out, const void* rest, const void* lse, const void* grad_out, void* grad_query,
                           void* grad_key, void* grad_value, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
-                          int64_t D, double scale, int causal, void* workspace, size_t workspace_bytes, void* stream, char* err,
-                          size_t err_len) {
+                          int64_t D, double scale, int causal, void* workspace, size_t workspace_bytes, void* stream,
+                          char* err, size_t err_len) {
     using namespace td;
     if (int rc = check_sizes(dtype, B, Q, N, H, Hk, D, scale, err, err_len)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
@@ -397,6 +426,13 @@ int td_attention_backward(int dtype, const void* query, const void* key, const v
     a.grad_k = grad_key;
     a.grad_v = grad_value;
     a.delta = static_cast<unsigned char*>(workspace) + ws.delta;
+    int64_t k_splits, q_splits;
+    grad_splits(dtype, B, Q, N, H, Hk, D, &k_splits, &q_splits);
+    a.k_splits = int(k_splits);
+    a.q_splits = int(q_splits);
+    a.part_k = static_cast<unsigned char*>(workspace) + ws.part_k;
+    a.part_v = static_cast<unsigned char*>(workspace) + ws.part_v;
+    a.part_q = static_cast<unsigned char*>(workspace) + ws.part_q;
     if (attn_tc_fits(dtype, a))
         return attn_tc_backward(dtype, a, ws, mb, mh, static_cast<unsigned char*>(workspace), s, err, err_len);
     switch (dtype) {

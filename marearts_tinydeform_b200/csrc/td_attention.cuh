@@ -50,6 +50,11 @@ struct AttnArgs {
     long long m_b, m_h, m_q;
     const uint8_t* padding;         // [B, N], nonzero = no key there; or null
     int B, Q, N, H, Hk, D, Qp;
+    // CUDA-core and TF32 backward: the query tiles of a tile of keys are shared by k_splits CTAs, the key tiles of a
+    // tile of queries by q_splits. With more than one, split s leaves its sums, in the accumulator type, at s times the
+    // size of the gradient in these, and attn_join_kernel adds them.
+    int k_splits, q_splits;
+    void *part_k, *part_v, *part_q;
     int vec_q, vec_k, vec_v, vec_g; // CUDA-core kernels: rows of q, k, v, grad_out are whole aligned 16-byte vectors
     int causal;                     // key j is open to query i while j <= i + (N - Q)
     double scale;
@@ -211,8 +216,39 @@ __global__ void __launch_bounds__(256) attn_delta_kernel(const AttnArgs a) {
     static_cast<A*>(a.delta)[row] = sum;
 }
 
+// What a backward CTA found for element `at` of a gradient of `size` elements.
+template <typename T, typename A>
+__device__ __forceinline__ void attn_put_grad(void* grad, void* part, int splits, int split, long long size,
+                                              long long at, A x) {
+    if (splits == 1) static_cast<T*>(grad)[at] = from_acc<T>(x);
+    else static_cast<A*>(part)[split * size + at] = x;
+}
+
+// Adds the splits of a gradient in their order, a thread per element: those of the keys, the values, then the queries
+// (without those that were not split).
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const AttnArgs a) {
+    using A = typename Elem<T>::acc;
+    const long long size_k = (long long)a.B * a.N * a.Hk * a.D, size_q = (long long)a.B * a.Q * a.H * a.D;
+    long long at = (long long)blockIdx.x * 256 + threadIdx.x;
+    grid_dependency_wait();
+    launch_dependents();
+    const bool keys = a.k_splits > 1 && at < 2 * size_k, values = keys && at >= size_k;
+    if (!keys && a.k_splits > 1) at -= 2 * size_k;
+    if (values) at -= size_k;
+    const long long size = keys ? size_k : size_q;
+    const int splits = keys ? a.k_splits : a.q_splits;
+    if (splits == 1 || at >= size) return;
+    const A* part = static_cast<const A*>(values ? a.part_v : keys ? a.part_k : a.part_q) + at;
+    A sum = 0;
+#pragma unroll 8
+    for (int s = 0; s < splits; ++s) sum += part[s * size];
+    static_cast<T*>(values ? a.grad_v : keys ? a.grad_k : a.grad_q)[at] = from_acc<T>(sum);
+}
+
 // The gradient of the keys and values (blocks below kv_blocks: one tile of keys of one key head, over the query heads
-// of its group and their query tiles) and of the queries (the other blocks: one tile of queries of one head).
+// of its group and their query tiles) and of the queries (the other blocks: one tile of queries of one head), the
+// splits of a tile beside each other.
 template <typename T, int DP, int R>
 __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs a, int kv_blocks) {
     using A = typename Elem<T>::acc;
@@ -236,8 +272,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
     grid_dependency_wait();
     launch_dependents();
     if (int(blockIdx.x) < kv_blocks) {
-        const int tiles = (a.N + M - 1) / M;
-        const int j0 = blockIdx.x % tiles * M, hk = blockIdx.x / tiles % a.Hk, b = blockIdx.x / tiles / a.Hk;
+        const int tiles = (a.N + M - 1) / M, split = blockIdx.x % a.k_splits, blk = blockIdx.x / a.k_splits;
+        const int j0 = blk % tiles * M, hk = blk / tiles % a.Hk, b = blk / tiles / a.Hk;
         const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
         simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad, a.vec_k != 0);
         simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad, a.vec_v != 0);
@@ -248,11 +284,17 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
             for (int x = 0; x < Tile::kWidth; ++x) dk[r][x] = dv[r][x] = 0;
         // the first query that may use key j0
         const int first = a.causal ? max(0, min(a.Q, j0 - (a.N - a.Q))) / M * M : 0;
-        for (int h = hk * group; h < (hk + 1) * group; ++h) {
+        const int cols = (a.Q - first + M - 1) / M;
+        int n = int((long long)cols * group * split / a.k_splits);
+        const int end = int((long long)cols * group * (split + 1) / a.k_splits);
+        while (n < end) {
+            const int h = hk * group + n / cols;
             const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
             const A* lse_h = lse + ((long long)b * a.H + h) * a.Qp;
             const A* delta_h = delta + ((long long)b * a.H + h) * a.Qp;
-            for (int i0 = first; i0 < a.Q; i0 += M) {
+            const int head_end = min(end, (n / cols + 1) * cols);
+            for (; n < head_end; ++n) {
+                const int i0 = first + n % cols * M;
                 __syncthreads();
                 simt_load<T, A, DP, M>(qs, q + b * a.q_b + h * a.q_h, a.q_t, i0, a.Q, a.D, nullptr, a.vec_q != 0);
                 simt_load<T, A, DP, M>(gs, g + ((long long)b * a.Q * a.H + h) * a.D, (long long)a.H * a.D, i0, a.Q,
@@ -299,13 +341,14 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
                 const int d = tx + 16 * x;
                 if (d >= a.D) continue;
                 const long long at = (((long long)b * a.N + j) * a.Hk + hk) * a.D + d;
-                static_cast<T*>(a.grad_k)[at] = from_acc<T>(dk[r][x] * scale);
-                static_cast<T*>(a.grad_v)[at] = from_acc<T>(dv[r][x]);
+                const long long size = (long long)a.B * a.N * a.Hk * a.D;
+                attn_put_grad<T, A>(a.grad_k, a.part_k, a.k_splits, split, size, at, dk[r][x] * scale);
+                attn_put_grad<T, A>(a.grad_v, a.part_v, a.k_splits, split, size, at, dv[r][x]);
             }
         }
         return;
     }
-    const int blk = int(blockIdx.x) - kv_blocks;
+    const int split = (int(blockIdx.x) - kv_blocks) % a.q_splits, blk = (int(blockIdx.x) - kv_blocks) / a.q_splits;
     const int tiles = (a.Q + M - 1) / M;
     const int i0 = blk % tiles * M, h = blk / tiles % a.H, b = blk / tiles / a.H, hk = h / group;
     const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + (long long)b * a.N;
@@ -323,8 +366,10 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
 #pragma unroll
         for (int x = 0; x < Tile::kWidth; ++x) dq[r][x] = 0;
     }
-    const int key_end = attn_key_end(a, i0 + M);
-    for (int j0 = 0; j0 < key_end; j0 += M) {
+    const int cols = (attn_key_end(a, i0 + M) + M - 1) / M;
+    const int end = int((long long)cols * (split + 1) / a.q_splits);
+    for (int n = int((long long)cols * split / a.q_splits); n < end; ++n) {
+        const int j0 = n * M;
         __syncthreads();
         simt_load<T, A, DP, M>(ks, k + b * a.k_b + hk * a.k_h, a.k_t, j0, a.N, a.D, pad, a.vec_k != 0);
         simt_load<T, A, DP, M>(vs, v + b * a.v_b + hk * a.v_h, a.v_t, j0, a.N, a.D, pad, a.vec_v != 0);
@@ -355,8 +400,8 @@ __global__ void __launch_bounds__(256) attn_simt_backward_kernel(const AttnArgs 
         for (int x = 0; x < Tile::kWidth; ++x) {
             const int d = tx + 16 * x;
             if (d < a.D)
-                static_cast<T*>(a.grad_q)[(((long long)b * a.Q + i) * a.H + h) * a.D + d] =
-                    from_acc<T>(dq[r][x] * scale);
+                attn_put_grad<T, A>(a.grad_q, a.part_q, a.q_splits, split, (long long)a.B * a.Q * a.H * a.D,
+                                    (((long long)b * a.Q + i) * a.H + h) * a.D + d, dq[r][x] * scale);
         }
     }
 }

@@ -356,18 +356,18 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
     }
 }
 
-// Joins the partials of a row, a block of 8 warps per row: warp w adds splits w, w + 8, .. (their loads in flight
-// together), then the warps' sums are added in order.
+// Joins the partials of a row by W of a block's 8 warps: warp w of a row adds splits w, w + W, .. (their loads in
+// flight together), then the warps' sums are added in order. Eight for few rows of many splits, one for many rows.
 constexpr int kCombineWarps = 8;
-template <typename T>
+template <typename T, int W>
 __global__ void __launch_bounds__(kCombineWarps * 32) attn_combine_kernel(const SplitArgs args) {
     using A = typename Elem<T>::acc;
     const AttnArgs& a = args.a;
-    __shared__ A part[kCombineWarps][kAttnMaxHeadDim];
-    const long long row = blockIdx.x;
-    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32 % W, lane = threadIdx.x % 32;
+    const long long row = (long long)blockIdx.x * (kCombineWarps / W) + threadIdx.x / (32 * W);
     grid_dependency_wait();
     launch_dependents();
+    if (row >= (long long)a.B * a.H * a.Q) return;  // whole warps, and whole blocks where they meet below
     const A* ml = static_cast<const A*>(args.part_ml) + row * args.splits * 2;
     const A* po = static_cast<const A*>(args.part_o) + row * args.splits * a.D;
     A top = -A(INFINITY), sum = 0;
@@ -378,22 +378,26 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_combine_kernel(const 
     for (int s = lane; s < args.splits; s += 32) sum += ml[2 * s + 1] * attn_exp2<A>(ml[2 * s] - ref);
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    const A inv = sum == A(0) ? A(0) : A(1) / sum;
+    __shared__ A part[W > 1 ? W : 1][W > 1 ? kAttnMaxHeadDim : 1];
     for (int d = lane; d < a.D; d += 32) {
         A o = 0;
 #pragma unroll 4
-        for (int s = warp; s < args.splits; s += kCombineWarps)
-            o += po[(long long)s * a.D + d] * attn_exp2<A>(ml[2 * s] - ref);
-        part[warp][d] = o;
+        for (int s = warp; s < args.splits; s += W) o += po[(long long)s * a.D + d] * attn_exp2<A>(ml[2 * s] - ref);
+        if constexpr (W > 1) part[warp][d] = o;
+        else attn_store<T, A>(a, row, d, o, inv);
     }
-    __syncthreads();
-    const A inv = sum == A(0) ? A(0) : A(1) / sum;
-    for (int d = threadIdx.x; d < a.D; d += kCombineWarps * 32) {
-        A o = 0;
+    if constexpr (W > 1) {
+        static_assert(W == kCombineWarps, "a row is a block");
+        __syncthreads();
+        for (int d = threadIdx.x; d < a.D; d += W * 32) {
+            A o = 0;
 #pragma unroll
-        for (int w = 0; w < kCombineWarps; ++w) o += part[w][d];
-        attn_store<T, A>(a, row, d, o, inv);
+            for (int w = 0; w < W; ++w) o += part[w][d];
+            attn_store<T, A>(a, row, d, o, inv);
+        }
     }
-    if (threadIdx.x == 0) attn_store_lse<A>(a, row, top, sum);
+    if (warp == 0 && lane == 0) attn_store_lse<A>(a, row, top, sum);
 }
 
 // ---- CUDA-core forward: every type and head width (see td_attention.cuh) ------------------------------------------

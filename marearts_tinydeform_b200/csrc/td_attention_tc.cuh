@@ -50,6 +50,10 @@ struct AttnTcArgs {
     float* amax;                // float16 backward: per block of the delta kernel max|dO|, then per block max|V|
     int amax_parts;
     int kv_blocks;              // backward: blocks of the keys' gradient, launched first
+    // forward: the key tiles of a query tile are shared by `splits` CTAs; with more than one these take their partial
+    // results, o [B * H * Q][splits][D] and (maximum, sum) [B * H * Q][splits][2], for attn_combine_kernel
+    int splits;
+    float *part_o, *part_ml;
 };
 
 constexpr int kAttnBM = 128, kAttnBN = 64;
@@ -369,9 +373,11 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     // the last query tiles first: under the causal rule they are the longest
     const int q_tiles = (a.Q + kAttnBM - 1) / kAttnBM;
-    const int bh = blockIdx.x % (a.B * a.H), qt = q_tiles - 1 - int(blockIdx.x) / (a.B * a.H);
+    const int bh = blockIdx.x % (a.B * a.H), split = blockIdx.x / (a.B * a.H) % args.splits;
+    const int qt = q_tiles - 1 - int(blockIdx.x / (a.B * a.H)) / args.splits;
     const int h = bh % a.H, b = bh / a.H, hk = h / (a.H / a.Hk), i0 = qt * kAttnBM, off = a.N - a.Q;
-    const int tiles = (attn_key_end(a, i0 + kAttnBM) + kAttnBN - 1) / kAttnBN;
+    const long long all_tiles = (attn_key_end(a, i0 + kAttnBM) + kAttnBN - 1) / kAttnBN;
+    const int t0 = int(all_tiles * split / args.splits), t1 = int(all_tiles * (split + 1) / args.splits);
     const uint8_t* flags = args.row_flags == nullptr
                                ? nullptr
                                : args.row_flags + b * args.rf_b + h * args.rf_h + qt * args.rf_q;
@@ -409,14 +415,14 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         // a lane per box of the ring: TMA copies of one thread are served one after another, those of different threads
         // overlap
         const uint64_t pol = l2_evict_last();  // keys and values are read again by the other query tiles
-        if (lane < 2 * KB && tiles > 0) {  // the queries in halves of 64
+        if (lane < 2 * KB && t1 > t0) {  // the queries in halves of 64
             mbar_arrive_expect_tx(qfull, AttnBox<DP>::kTile);
             tma_load_4d(smem + lane * AttnBox<DP>::kTile, &map_q, qfull, 64 * (lane / 2), i0 + 64 * (lane % 2), h, b,
                         l2_evict_first());
         }
         int n = 0;
         Ring<S> ring;
-        for_tiles(0, tiles, flags, [&](int t, bool) {
+        for_tiles(t0, t1, flags, [&](int t, bool) {
             const int s = ring.at;
             if (!warp_wait(&empty[s], ring.parity ^ 1u, kErrSlotWait)) return false;
             ring.template step<>();
@@ -441,8 +447,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         const uint32_t leader = lane == 0;
         Ring<S> ring;
         Ring<2> buf;
-        if (tiles == 0 || warp_wait(qfull, 0u, kErrTmaWait))
-            for_tiles(0, tiles, flags, [&](int, bool) {
+        if (t1 <= t0 || warp_wait(qfull, 0u, kErrTmaWait))
+            for_tiles(t0, t1, flags, [&](int, bool) {
                 if (!warp_wait(&kfull[ring.at], ring.parity, kErrTmaWait)) return false;
                 // the buffer's P before these scores (none in the first round) has been read by its product
                 if (!warp_wait(&done[buf.at], buf.parity ^ 1u, kErrMmaWait)) return false;
@@ -459,7 +465,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         bool first = true;
         Ring<S> ring;
         Ring<2> buf;
-        const bool ok = for_tiles(0, tiles, flags, [&](int t, bool all) {
+        const bool ok = for_tiles(t0, t1, flags, [&](int t, bool all) {
             unsigned char* v = v_tile(ring.at);
             if (!warp_wait(&vfull[ring.at], ring.parity, kErrTmaWait)) return false;
             if (pad != nullptr && !all) clear_padded<DP>(v, pad, t * kAttnBN, a.N);
@@ -489,7 +495,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         float ref = -INFINITY, sum = 0.f;
         int n = 0;
         Ring<2> buf;
-        const bool ok = for_tiles(0, tiles, flags, [&](int t, bool all) {
+        const bool ok = for_tiles(t0, t1, flags, [&](int t, bool all) {
             const int j0 = t * kAttnBN;
             const bool open = all && j0 + kAttnBN <= a.N && (!a.causal || j0 + kAttnBN - 1 <= i0 + off);
             unsigned long long w = ~0ull;
@@ -583,6 +589,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
         if (got) {
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             const long long at = (((long long)b * a.Q + i) * a.H + h) * a.D;
+            const long long place = ((long long)bh * a.Q + i) * args.splits + split;
 #pragma unroll 1
             for (int d = 0; d < DP && d < a.D; d += 32) {
                 uint32_t o[32];
@@ -598,6 +605,12 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     if (d + 8 * g >= a.D) break;  // D is a multiple of 8
+                    if (args.splits > 1) {
+                        uint4* part = reinterpret_cast<uint4*>(args.part_o + place * a.D + d + 8 * g);
+                        part[0] = make_uint4(o[8 * g], o[8 * g + 1], o[8 * g + 2], o[8 * g + 3]);
+                        part[1] = make_uint4(o[8 * g + 4], o[8 * g + 5], o[8 * g + 6], o[8 * g + 7]);
+                        continue;
+                    }
                     uint32_t q[4], rest[4];
 #pragma unroll
                     for (int x = 0; x < 4; ++x) {
@@ -614,7 +627,9 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                             make_uint4(rest[0], rest[1], rest[2], rest[3]);
                 }
             }
-            if (a.lse != nullptr)  // Qp is a multiple of the tile
+            if (args.splits > 1) {
+                if (i < a.Q) *reinterpret_cast<float2*>(args.part_ml + 2 * place) = make_float2(ref * c, sum);
+            } else if (a.lse != nullptr)  // Qp is a multiple of the tile
                 static_cast<float*>(a.lse)[(long long)bh * a.Qp + i] =
                     i < a.Q && sum != 0.f ? fmaf(ref, c, log2f(sum)) : INFINITY;
         }
@@ -749,22 +764,28 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
     // r0 .. of head h0, over the key tiles
     const int heads = KEYS ? a.Hk : a.H, rows = KEYS ? a.N : a.Q;
     const int row_tiles = (rows + kAttnBM - 1) / kAttnBM;
-    const int bx = block % (a.B * heads);
+    const int bx = block % (a.B * heads), splits = KEYS ? a.k_splits : a.q_splits;
+    const int split = block / (a.B * heads) % splits, tile = block / (a.B * heads) / splits;
     // the longest blocks under the causal rule first: the first keys, the last queries
-    const int rt = KEYS ? block / (a.B * heads) : row_tiles - 1 - block / (a.B * heads);
+    const int rt = KEYS ? tile : row_tiles - 1 - tile;
     const int head = bx % heads, b = bx / heads, r0 = rt * kAttnBM;
     const int hk = KEYS ? head : head / group, h0 = KEYS ? head * group : head, h1 = KEYS ? h0 + group : h0 + 1;
     const int t0 = KEYS && a.causal ? max(0, min(a.Q, r0 - off)) / kAttnBN : 0;
     const int t1 = KEYS ? (a.Q + kAttnBN - 1) / kAttnBN
                         : (attn_key_end(a, r0 + kAttnBM) + kAttnBN - 1) / kAttnBN;
+    // this split's tiles, counted over the heads
+    const long long work = (long long)(t1 - t0) * (h1 - h0);
+    const int from = int(work * split / splits), to = int(work * (split + 1) / splits);
     auto each_tile = [&](auto&& f) {  // f(head, tile, all open by the flags)
         for (int h = h0; h < h1; ++h) {
+            const int first = t0 - (h - h0) * (t1 - t0), lo = max(t0, first + from), hi = min(t1, first + to);
+            if (lo >= hi) continue;
             const uint8_t* flags = nullptr;
             if (KEYS && args.col_flags != nullptr)
                 flags = args.col_flags + b * args.cf_b + h * args.cf_h + (long long)rt * args.col_tiles;
             if (!KEYS && args.row_flags != nullptr)
                 flags = args.row_flags + b * args.rf_b + h * args.rf_h + rt * args.rf_q;
-            if (!for_tiles(t0, t1, flags, [&](int t, bool all) { return f(h, t, all); })) return false;
+            if (!for_tiles(lo, hi, flags, [&](int t, bool all) { return f(h, t, all); })) return false;
         }
         return true;
     };
@@ -915,8 +936,10 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             const bool is_v = KEYS && wg == 1;
             const float f = is_v ? 1.f : float(a.scale) / ds_scale;
             const bool gone = KEYS && a.padding != nullptr && r < a.N && a.padding[(long long)b * a.N + r] != 0;
-            T* out = KEYS ? static_cast<T*>(is_v ? a.grad_v : a.grad_k) + (((long long)b * a.N + r) * a.Hk + hk) * a.D
-                          : static_cast<T*>(a.grad_q) + (((long long)b * a.Q + r) * a.H + h0) * a.D;
+            const long long at = (((long long)b * rows + r) * heads + head) * a.D;
+            T* out = static_cast<T*>(KEYS ? (is_v ? a.grad_v : a.grad_k) : a.grad_q) + at;
+            float* part = static_cast<float*>(KEYS ? (is_v ? a.part_v : a.part_k) : a.part_q) +
+                          split * ((long long)a.B * rows * heads * a.D) + at;
             const int d_first = KEYS ? 0 : 32 * wg, d_step = KEYS ? 32 : 64;
 #pragma unroll 1
             for (int d = d_first; d < DP && d < a.D; d += d_step) {
@@ -930,6 +953,18 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
                     if (d + 8 * g >= a.D) break;
+                    if (splits > 1) {
+#pragma unroll
+                        for (int x = 0; x < 8; x += 4) {
+                            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+                            const uint32_t* z = o + 8 * g + x;
+                            if (n > 0 && !gone)
+                                y = make_float4(__uint_as_float(z[0]) * f, __uint_as_float(z[1]) * f,
+                                                __uint_as_float(z[2]) * f, __uint_as_float(z[3]) * f);
+                            *reinterpret_cast<float4*>(part + d + 8 * g + x) = y;
+                        }
+                        continue;
+                    }
                     uint4 q = make_uint4(0u, 0u, 0u, 0u);
                     uint32_t* qw = &q.x;
                     if (n > 0 && !gone) {

@@ -251,6 +251,8 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
     const float c = float(a.scale * 1.4426950408889634), scale = float(a.scale);
     const int heads = KEYS ? a.Hk : a.H, rows = KEYS ? a.N : a.Q;
     const int tiles = (rows + kTf32Rows - 1) / kTf32Rows;
+    const int splits = KEYS ? a.k_splits : a.q_splits, split = block % splits;
+    block /= splits;
     const int r0 = block % tiles * kTf32Rows, head = block / tiles % heads, b = block / tiles / heads;
     const int hk = KEYS ? head : head / group, h0 = KEYS ? head * group : head, h1 = KEYS ? h0 + group : h0 + 1;
     const float* q = static_cast<const float*>(a.q) + b * a.q_b;
@@ -300,10 +302,12 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
             acc[i][y] = 0.f;
             if constexpr (KEYS) acc2[i][y] = 0.f;
         }
-    const int cols = c1 > c0 ? (c1 - c0 + NT - 1) / NT : 0, total = cols * (h1 - h0);
-    if (total > 0) fetch(h0, c0, 0);
+    const int cols = c1 > c0 ? (c1 - c0 + NT - 1) / NT : 0;
+    const long long work = (long long)cols * (h1 - h0);
+    const int from = int(work * split / splits), total = int(work * (split + 1) / splits) - from;
+    int h = cols > 0 ? h0 + from / cols : h0, col = cols > 0 ? c0 + from % cols * NT : c0;
+    if (total > 0) fetch(h, col, 0);
     copy_commit();
-    int h = h0, col = c0;
     for (int n = 0; n < total; ++n) {
         const int buf = n & 1;
         int next_h = h, next = col + NT;
@@ -345,6 +349,7 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
         col = next;
     }
     copy_wait<0>();
+    const long long size = (long long)a.B * rows * heads * a.D;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
         if (row[e] >= rows) continue;
@@ -359,10 +364,11 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
                 if (d >= a.D) continue;
                 const float x = gone ? 0.f : acc[i][2 * e + y] * scale;
                 if constexpr (KEYS) {
-                    static_cast<float*>(a.grad_k)[at + d] = x;
-                    static_cast<float*>(a.grad_v)[at + d] = gone ? 0.f : acc2[i][2 * e + y];
+                    const float x2 = gone ? 0.f : acc2[i][2 * e + y];
+                    attn_put_grad<float>(a.grad_k, a.part_k, splits, split, size, at + d, x);
+                    attn_put_grad<float>(a.grad_v, a.part_v, splits, split, size, at + d, x2);
                 } else {
-                    static_cast<float*>(a.grad_q)[at + d] = x;
+                    attn_put_grad<float>(a.grad_q, a.part_q, splits, split, size, at + d, x);
                 }
             }
     }

@@ -66,6 +66,31 @@ def test_attention(cuda, dtype, shape, kind):
     assert _native.device_error() == 0
 
 
+# calls of few long rows of work: the forward shares a query tile's keys among CTAs (splits that end inside a tile, and
+# of which masks leave some nothing), the backward shares a tile's queries (those of a whole group, too) or keys
+@pytest.mark.parametrize('kind', MASKS)
+@pytest.mark.parametrize('shape', [(1, 140, 1700, 4, 2, 32), (2, 300, 2049, 2, 1, 128), (1, 1300, 100, 8, 1, 32),
+                                   (1, 3, 2600, 2, 2, 64), (1, 900, 20, 3, 1, 48)], ids=str)
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_shared_rows_of_work(cuda, dtype, shape, kind):
+    q, k, v, grad = inputs(shape, dtype, 21)
+    kw = masks(kind, shape, 21)
+    if kind in ('padding', 'pairs'):  # a whole split, and more, without a key
+        if kind == 'padding':
+            kw['key_padding_mask'][-1, shape[2] // 4:shape[2] * 3 // 4] = True
+        else:
+            kw['attn_mask'][:, :shape[2] * 2 // 3] = True
+    exact = attention_exact(q, k, v, grad=grad, **kw)
+    with torch.inference_mode():
+        check(attention(q, k, v, **kw), exact[0], 'out (inference)')
+    first = run(q, k, v, grad, **kw)
+    for name, got, want in zip(NAMES, first, exact):
+        check(got, want, name)
+    for name, got, again in zip(NAMES, first, run(q, k, v, grad, **kw)):
+        assert torch.equal(got, again), name
+    assert _native.device_error() == 0
+
+
 @pytest.mark.parametrize('dtype', (torch.float16, torch.bfloat16), ids=str)
 def test_cuda_core_kernels(policy, dtype):
     shape = (2, 150, 200, 4, 2, 64)
