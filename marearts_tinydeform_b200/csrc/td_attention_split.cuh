@@ -41,15 +41,6 @@ struct SplitLayout {
     static constexpr size_t kSmem = kRing > kJoin ? kRing : kJoin;
 };
 
-// 16 bytes from global to shared memory, or zeros.
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int LEFT> __device__ __forceinline__ void copy_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
-}
-
 // The result's row `row` (of B * H * Q, head-major): o / l rounded, what the rounding took, and lse.
 template <typename T, typename A>
 __device__ __forceinline__ void attn_store(const AttnArgs& a, long long row, int d, A o, A inv) {

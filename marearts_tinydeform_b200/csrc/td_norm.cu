@@ -37,10 +37,14 @@ int launch_norm(const NormArgs<T>& a, int* grid, cudaStream_t stream, char* err,
         constexpr int G = decltype(g)::value, EPT = decltype(ept)::value, kCtas = norm_ctas<T, VEC, EPT, BWD>();
         static_assert(!BWD || kCtas <= kMostCtas, "workspace");
         *grid = norm_grid(a.rows, a.C, kCtas);
-        if constexpr (BWD)
-            return host::launch(err, err_len, "norm_backward_kernel", norm_backward_kernel<T, VEC, G, EPT>,
-                                dim3(unsigned(*grid)), dim3(kNormThreads), 0, stream, true, a);
-        else
+        if constexpr (BWD) {
+            constexpr auto kernel = norm_backward_kernel<T, VEC, G, EPT>;
+            constexpr size_t smem = norm_smem<T, VEC, EPT>();
+            // (the kernel's static arrays count towards the 48 KB that need no raising)
+            if (int rc = host::allow_smem<kernel>(smem > 0 ? smem + 8192 : 0, err, err_len)) return rc;
+            return host::launch(err, err_len, "norm_backward_kernel", kernel, dim3(unsigned(*grid)),
+                                dim3(kNormThreads), smem, stream, true, a);
+        } else
             return host::launch(err, err_len, "norm_forward_kernel", norm_forward_kernel<T, VEC, G, EPT>,
                                 dim3(unsigned(*grid)), dim3(kNormThreads), 0, stream, true, a);
     };

@@ -12,11 +12,12 @@
 //
 // A group of G threads holds a row, EPT elements a thread (VEC = elements of a 16-byte vector, or 1 where C or an
 // address is not a multiple of it), and walks over rows blockIdx, blockIdx + gridDim, .., the next row's loads issued
-// before the present row's sums are taken. The backward's column sums stay in the group's registers over all of its
-// rows; the groups of a CTA add theirs in order through shared memory, each CTA stores one float32 partial row, and
-// norm_reduce_kernel adds those in a fixed order: no atomics, the same bits every time. 177784 rows x 256 in bfloat16:
-// forward 48.7 us (5.6 TB/s), backward with its reduction 85 us (4.3 TB/s; 24 warps an SM with a row ahead each); 8800
-// x 515 in float32, whose rows start anywhere, 13.5 and 19.5 us (4.0 and 3.7 TB/s).
+// before the present row's sums are taken (the backward, whose sums leave fewer warps an SM, has three rows ahead in
+// shared memory). The backward's column sums stay in the group's registers over all of its rows; the groups of a CTA
+// add theirs in order through shared memory, each CTA stores one float32 partial row, and norm_reduce_kernel adds those
+// in a fixed order: no atomics, the same bits every time. 177784 rows x 256 in bfloat16: forward 48.7 us (5.6 TB/s),
+// backward with its reduction 65.7 us (5.5 TB/s; 85 with one row ahead in registers, 75 with 4 CTAs an SM instead of
+// 3); 8800 x 515 in float32, whose rows start anywhere, 13.5 and 19.5 us (4.0 and 3.7 TB/s).
 #pragma once
 
 #include "td_common.cuh"
@@ -185,6 +186,18 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, false>())
     }
 }
 
+// Rows a backward group has in flight or at hand in shared memory: each thread copies its own vectors of them there
+// and reads them back, so no barrier is needed. 0 where rows go through registers, one ahead.
+template <typename T, int VEC, int EPT>
+constexpr int norm_stages() {
+    if (VEC == 1 || sizeof(T) == 8) return 0;
+    return EPT / VEC <= 4 ? 4 : 2;
+}
+template <typename T, int VEC, int EPT>
+constexpr size_t norm_smem() {
+    return size_t(norm_stages<T, VEC, EPT>()) * 3 * (EPT / VEC) * kNormThreads * 16;
+}
+
 template <typename T, int VEC, int G, int EPT>
 __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, true>())
     norm_backward_kernel(const NormArgs<T> a) {
@@ -202,6 +215,26 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, true>())
     r.zero();
     const acc inv = acc(1) / acc(a.C);
     const long long step = (long long)gridDim.x * kGroups;
+    constexpr int S = norm_stages<T, VEC, EPT>();
+    extern __shared__ __align__(16) unsigned char smem[];
+    auto place = [&](int stage, int which, int i) {
+        return smem + (((stage * 3 + which) * NV + i) * kNormThreads + threadIdx.x) * 16;
+    };
+    auto issue = [&](long long row, int stage) {
+        if (row < a.rows) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (lane + i * G) * VEC;
+                const long long at = c < a.C ? row * a.C + c : 0;
+                copy16(smem_addr(place(stage, 0, i)), a.x + at, c < a.C);
+                copy16(smem_addr(place(stage, 1, i)), a.grad_y + at, c < a.C);
+                if (a.residual != nullptr) copy16(smem_addr(place(stage, 2, i)), a.residual + at, c < a.C);
+            }
+        }
+        copy_commit();
+    };
+    // the statistics of the group's next 32 rows, a lane's each, so that their latency shows once in 32 rows
+    acc mean_l = 0, rstd_l = 0;
     acc mean_n = 0, rstd_n = 0;
     auto fetch = [&](long long row) {
         if (row < a.rows) {
@@ -221,9 +254,33 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, true>())
 #pragma unroll
     for (int i = 0; i < EPT; ++i) dw[i] = db[i] = 0;
     long long row = (long long)blockIdx.x * kGroups + group;
-    fetch(row);
-    for (; row < a.rows; row += step) {
+    if constexpr (S > 0) {
+#pragma unroll
+        for (int s = 0; s < S - 1; ++s) issue(row + s * step, s);
+    } else {
+        fetch(row);
+    }
+    int stage = 0;
+    for (int n = 0; row < a.rows; row += step, ++n) {
         acc z[EPT], g[EPT], t[EPT];
+        if constexpr (S > 0) {
+            if (n % 32 == 0) {
+                const long long mine = row + (threadIdx.x % 32) * step;
+                mean_l = mine < a.rows ? a.mean[mine] : acc(0);
+                rstd_l = mine < a.rows ? a.rstd[mine] : acc(0);
+            }
+            mean_n = __shfl_sync(0xffffffffu, mean_l, n % 32);
+            rstd_n = __shfl_sync(0xffffffffu, rstd_l, n % 32);
+            copy_wait<S - 2>();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                if constexpr (VEC > 1) {
+                    x.wide[i] = *reinterpret_cast<const uint4*>(place(stage, 0, i));
+                    d.wide[i] = *reinterpret_cast<const uint4*>(place(stage, 1, i));
+                    if (a.residual != nullptr) r.wide[i] = *reinterpret_cast<const uint4*>(place(stage, 2, i));
+                }
+            }
+        }
         x.widen(z);
         if (a.residual != nullptr) {
             r.widen(t);
@@ -232,7 +289,12 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, true>())
         }
         d.widen(g);
         const acc mean = mean_n, rstd = rstd_n;
-        fetch(row + step);
+        if constexpr (S > 0) {
+            issue(row + (S - 1) * step, stage == 0 ? S - 1 : stage - 1);
+            stage = stage == S - 1 ? 0 : stage + 1;
+        } else {
+            fetch(row + step);
+        }
         w.widen(t);
         acc sums[2] = {0, 0};  // of g and of g z
 #pragma unroll
@@ -251,6 +313,7 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, true>())
         for (int i = 0; i < EPT; ++i) g[i] = (g[i] - sg - z[i] * sgz) * rstd;
         store_row<T, VEC, NV, G>(a.out + row * a.C, g, lane, a.C);
     }
+    if constexpr (S > 0) copy_wait<0>();
     // the CTA's column sums: group 0's, + group 1's, .. in order
     acc* part = a.partial + (long long)blockIdx.x * 2 * a.C;
     auto add_up = [&](const acc(&v)[EPT], acc* out) {

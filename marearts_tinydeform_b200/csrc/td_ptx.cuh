@@ -288,6 +288,16 @@ __device__ __forceinline__ uint64_t sdesc_sw128(uint32_t saddr) {
     return d;
 }
 
+// ---- cp.async ------------------------------------------------------------------------------------------------
+// 16 bytes from global to shared memory, or zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool real) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT> __device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory");
+}
+
 // ---- tcgen05: TMEM -> registers -----------------------------------------------------------------------------
 // 32 lanes x 32 consecutive 32-bit columns: thread i of the warp gets row (lane base + i), columns [col, col + 32).
 __device__ __forceinline__ void tmem_ld_32x32b_x32(uint32_t taddr, uint32_t (&r)[32]) {
