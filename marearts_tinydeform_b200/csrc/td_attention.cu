@@ -38,9 +38,9 @@ SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
 template <typename T> constexpr int simt_r() { return std::is_same<T, double>::value ? 2 : 4; }
 
 // The CUDA-core and the TF32 forward's plan: down to one tile of 64 keys a CTA, as long as all the CTAs are resident at
-// once, three an SM (float32, 8 heads of 32: 2 x 300 queries and keys 33 us in two splits, 24 in five; 2 x 64 on 200
-// keys 22 in one, 12 in four; 8 x 300 47 in one and 82 in two, which are more than a wave). 16-bit calls of the usual
-// widths come here only misaligned or short: they do without partials.
+// once, three an SM (float32, 8 heads of 32: 2 x 64 queries on 200 keys 22 us in one split, 12 in four; 8 x 300 queries
+// and keys 47 in one and 82 in two, which are more than a wave). 16-bit calls of the usual widths come here only
+// misaligned or short: they do without partials.
 SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t D) {
     SplitArgs p = {};
     const bool whole = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0;
@@ -252,7 +252,7 @@ bool prefer_split(const AttnArgs& a) {
 
 // float32 on tensor cores: rows of whole 16-byte vectors and at least 256 keys. Below, where a CTA has a few tiles, its
 // four warps' longer chains show (one head, 64 x 64: 12 us at D = 32 and 44 at D = 128 against 9 and 24 on CUDA cores;
-// 256 keys: 14 and 30 against 14 and 31; 4 x 1100 x 8 heads x 32: 152 against 233, the backward 445 against 699).
+// 256 keys: 14 and 30 against 14 and 31; 4 x 1100 x 8 heads x 32: 209 against 233, the backward 493 against 699).
 bool tf32_fits(const AttnArgs& a) {
     return host::best_policy() && a.N >= 256 && a.vec_q && a.vec_k && a.vec_v && (a.grad_q == nullptr || a.vec_g) &&
            (reinterpret_cast<uintptr_t>(a.lse) & 15u) == 0;

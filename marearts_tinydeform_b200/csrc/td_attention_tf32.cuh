@@ -1,11 +1,16 @@
 // td_attention_tf32.cuh -- float32 attention on tensor cores: every product in three TF32 ones.
 //
-// x = hi + lo with hi = x cut to TF32's 11 bits (exact) and lo = x - hi, so a b ~ hi hi + hi lo + lo hi to about 21
-// bits, as the library's float32 projections do. Tiles of 64 rows, four warps of 16, as mma.sync m16n8k8 fragments; the
+// x = hi + lo with hi = x rounded to TF32's 11 bits and lo = x - hi (exact; the tensor core cuts it to 11 bits), so a b
+// ~ hi hi + hi lo + lo hi to about 22 bits. Tiles of 64 rows, four warps of 16, as mma.sync m16n8k8 fragments; the
 // other side streams through two buffers of shared memory by asynchronous copies. What bounds it: the rate of these
 // products (about 38 TFLOP/s are left of three) and, with few tiles a CTA, one warp's chain of some 1500 instructions a
-// tile, 4.5 us. 8 heads x 32, 4 x 1100 tokens: forward 152 us (33 TFLOP/s), backward 445 us; 8 heads x 64, 4096 tokens:
-// 950 and 2395 us; the CUDA-core kernels take 233, 699, 1293 and 3523.
+// tile. 8 heads x 32, 4 x 1100 tokens: forward 209 us (160 in one wave of four CTAs an SM with spills, but 18 instead
+// of 15 for 2 x 300), backward 493 us (three CTAs an SM; 533 with two, 626 with four); 8 heads x 64, 4096 tokens: 963
+// and 2495 us; the CUDA-core kernels take 233, 699, 1293 and 3523.
+//
+// Accuracy, relative to float64 over 2 x 1100 tokens x 8 heads x 32: 3.4e-7 forward, 5e-7 backward (float32 matrix
+// products of a library: 6.4e-7). With hi cut instead of rounded and one sum over all keys it was 8.6e-6, in
+// three quarters of the time.
 //
 // Fragments need no shuffles: the order of a summed index is free. For row . row products (S, dP) a thread's 4
 // consecutive elements of a row are its slots t, t + 4 of two K steps, in both operands. For P . rows products the
@@ -17,6 +22,8 @@
 namespace td {
 
 constexpr int kTf32Threads = 128, kTf32Rows = 64;
+// CTAs an SM holds, by registers and, for wide heads, shared memory.
+template <int DP, bool BWD> constexpr int kTf32Ctas = DP == 32 ? 3 : DP == 64 ? (BWD ? 3 : 2) : 1;
 
 template <int DP, int NT>
 struct Tf32Layout {
@@ -25,7 +32,7 @@ struct Tf32Layout {
 };
 
 __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
-    hi = __float_as_uint(x) & 0xffffe000u;
+    hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;
     lo = __float_as_uint(x - __uint_as_float(hi));
 }
 
@@ -36,17 +43,20 @@ __device__ __forceinline__ void mma_1688(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// d[i] += a b[i] for M independent tiles in three products each, the smallest first: one product of every tile before
-// the next of any, as each waits for the last into its tile.
+// big[i] + small[i] += a b[i] for M independent tiles in three products each: one product of every tile before the next
+// of any, as each waits for the last into its tile. The tensor core cuts its sums where float32 would round them, which
+// adds up in one direction: the two small products have sums of their own, where that does not show, and neither sum
+// lasts longer than a tile.
 template <int M>
-__device__ __forceinline__ void mma_split(float (*d)[4], const uint32_t (&ah)[4], const uint32_t (&al)[4],
-                                          const uint32_t (&bh)[M][2], const uint32_t (&bl)[M][2]) {
+__device__ __forceinline__ void mma_split(float (*big)[4], float (*small)[4], const uint32_t (&ah)[4],
+                                          const uint32_t (&al)[4], const uint32_t (&bh)[M][2],
+                                          const uint32_t (&bl)[M][2]) {
 #pragma unroll
-    for (int i = 0; i < M; ++i) mma_1688(d[i], al, bh[i][0], bh[i][1]);
+    for (int i = 0; i < M; ++i) mma_1688(small[i], al, bh[i][0], bh[i][1]);
 #pragma unroll
-    for (int i = 0; i < M; ++i) mma_1688(d[i], ah, bl[i][0], bl[i][1]);
+    for (int i = 0; i < M; ++i) mma_1688(big[i], ah, bh[i][0], bh[i][1]);
 #pragma unroll
-    for (int i = 0; i < M; ++i) mma_1688(d[i], ah, bh[i][0], bh[i][1]);
+    for (int i = 0; i < M; ++i) mma_1688(small[i], ah, bl[i][0], bl[i][1]);
 }
 
 // ROWS rows from t0 on of a [tokens, D] slice into shared memory (16-byte copies; rows past n, padded rows and columns
@@ -67,10 +77,11 @@ __device__ __forceinline__ void tf32_load(float* dst, const float* src, long lon
 template <int DP, int NT>
 __device__ __forceinline__ void tf32_scores(const float* a, const float* b, int g, int t, float (&s)[NT / 8][4]) {
     constexpr int kPitch = DP + 4;
+    float small[NT / 8][4];
 #pragma unroll
     for (int j = 0; j < NT / 8; ++j)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) s[j][y] = 0.f;
+        for (int y = 0; y < 4; ++y) s[j][y] = small[j][y] = 0.f;
 #pragma unroll 1
     for (int k = 0; k < DP; k += 16) {
         const float4 a0 = *reinterpret_cast<const float4*>(a + g * kPitch + k + 4 * t);
@@ -95,10 +106,14 @@ __device__ __forceinline__ void tf32_scores(const float* a, const float* b, int 
                 split_tf32(x.z, bh[1][j][0], bl[1][j][0]);
                 split_tf32(x.w, bh[1][j][1], bl[1][j][1]);
             }
-            mma_split<4>(s + j0, ah[0], al[0], bh[0], bl[0]);
-            mma_split<4>(s + j0, ah[1], al[1], bh[1], bl[1]);
+            mma_split<4>(s + j0, small + j0, ah[0], al[0], bh[0], bl[0]);
+            mma_split<4>(s + j0, small + j0, ah[1], al[1], bh[1], bl[1]);
         }
     }
+#pragma unroll
+    for (int j = 0; j < NT / 8; ++j)
+#pragma unroll
+        for (int y = 0; y < 4; ++y) s[j][y] += small[j][y];
 }
 
 // o[i] += p . rows of b, columns 8 i ..
@@ -107,29 +122,38 @@ __device__ __forceinline__ void tf32_product(const float (&p)[NT / 8][4], const 
                                              float (&o)[DP / 8][4]) {
     constexpr int kPitch = DP + 4;
 #pragma unroll
-    for (int j = 0; j < NT / 8; ++j) {
-        uint32_t ah[4], al[4];
-        split_tf32(p[j][0], ah[0], al[0]);
-        split_tf32(p[j][2], ah[1], al[1]);
-        split_tf32(p[j][1], ah[2], al[2]);
-        split_tf32(p[j][3], ah[3], al[3]);
-        const float* rows = b + (8 * j + 2 * t) * kPitch + g;
+    for (int i0 = 0; i0 < DP / 8; i0 += 4) {
+        float big[4][4], small[4][4];
 #pragma unroll
-        for (int i0 = 0; i0 < DP / 8; i0 += 4) {
-            uint32_t bh[4][2], bl[4][2];
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) big[i][y] = small[i][y] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NT / 8; ++j) {
+            uint32_t ah[4], al[4], bh[4][2], bl[4][2];
+            split_tf32(p[j][0], ah[0], al[0]);
+            split_tf32(p[j][2], ah[1], al[1]);
+            split_tf32(p[j][1], ah[2], al[2]);
+            split_tf32(p[j][3], ah[3], al[3]);
+            const float* rows = b + (8 * j + 2 * t) * kPitch + g;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 split_tf32(rows[8 * (i0 + i)], bh[i][0], bl[i][0]);
                 split_tf32(rows[kPitch + 8 * (i0 + i)], bh[i][1], bl[i][1]);
             }
-            mma_split<4>(o + i0, ah, al, bh, bl);
+            mma_split<4>(big, small, ah, al, bh, bl);
         }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) o[i0 + i][y] += big[i][y] + small[i][y];
     }
 }
 
 // A block takes 64 queries of one head and the keys of one split. grid as attn_simt_forward_kernel's.
 template <int DP, int NT>
-__global__ void __launch_bounds__(kTf32Threads) attn_tf32_forward_kernel(const SplitArgs args) {
+__global__ void __launch_bounds__(kTf32Threads, kTf32Ctas<DP, false>)
+    attn_tf32_forward_kernel(const SplitArgs args) {
     using Lay = Tf32Layout<DP, NT>;
     const AttnArgs& a = args.a;
     extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -375,7 +399,8 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
 }
 
 template <int DP, int NT>
-__global__ void __launch_bounds__(kTf32Threads) attn_tf32_backward_kernel(const AttnArgs a, int kv_blocks) {
+__global__ void __launch_bounds__(kTf32Threads, kTf32Ctas<DP, true>)
+    attn_tf32_backward_kernel(const AttnArgs a, int kv_blocks) {
     extern __shared__ __align__(16) unsigned char smem_raw[];
     float* smem = reinterpret_cast<float*>(smem_raw);
     grid_dependency_wait();
