@@ -38,9 +38,8 @@ SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk,
 template <typename T> constexpr int simt_r() { return std::is_same<T, double>::value ? 2 : 4; }
 
 // The CUDA-core and the TF32 forward's plan: down to one tile of 64 keys a CTA, as long as all the CTAs are resident at
-// once, three an SM (float32, 8 heads of 32: 2 x 64 queries on 200 keys 22 us in one split, 12 in four; 8 x 300 queries
-// and keys 47 in one and 82 in two, which are more than a wave). 16-bit calls of the usual widths come here only
-// misaligned or short: they do without partials.
+// once, three an SM (float32, 8 heads of 32, 2 x 64 queries on 200 keys: 22 us in one split, 12 in four). 16-bit calls
+// of the usual widths come here only misaligned or short: they do without partials.
 SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t D) {
     SplitArgs p = {};
     const bool whole = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0;
@@ -56,7 +55,7 @@ SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H,
 // blocks. A CTA gets at most about the work of one of three on every SM, or, on tensor cores (one CTA an SM), of two;
 // but at least two tiles there, sixteen here, since partial sums and the launch that joins them cost about as much.
 // 16-bit causal 2 x 2047 x 8 heads (2 of keys) x 128: 150 us unsplit, 91; 1 query on 8400 keys x 8 heads x 32: 70 us
-// and 30, in float32 739 and 69; 2 x 300 queries on 8400 keys in float32: 961 and 516.
+// and 30, in float32 739 and 79; 2 x 300 queries on 8400 keys in float32: 961 and 545.
 void grad_splits(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t* k, int64_t* q) {
     const bool tc = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0 && N > 32;  // (unless misaligned)
     const int64_t rows = tc ? 128 : dtype == TD_F64 ? 32 : 64, cols = std::min<int64_t>(rows, 64);

@@ -9,7 +9,8 @@
 // P and dS are rounded to the input type (the products take 16 bits; their sums are float32) and written back to TMEM
 // over the scores they came from, as the A operand of the next product: neither ever reaches shared memory. The two
 // gradients are separate blocks of one launch, each of which forms S and dP itself: 7 products instead of 5 and twice
-// the exponentials, but every sum has one owner and one order (no atomics, no float32 gradient in memory).
+// the exponentials, but every sum has one owner and one order (no atomics, and no float32 gradient in memory but where
+// a few long rows of work are shared by several CTAs, whose partial sums are then joined in order).
 //
 // Columns past D (D < DP) and rows past the last token are zero through the tensor maps' fill. Scores of closed pairs
 // are replaced by -infinity (P, dS by zero); tiles without an open pair are skipped by every role alike, from one
@@ -22,9 +23,9 @@
 // SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two or three elementwise warpgroups
 // over two or three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their
 // waits (encoder backward below: 827 to 598 us); everything between two tiles is kept short. Measured: 2 x 4096 tokens,
-// 16 / 4 heads x 64, causal, bfloat16: 112 us (615 TFLOP/s). 8400 tokens, 8 heads x 32: forward 226 us (319 TFLOP/s of
-// the 32-wide products; half the rate of the exponentials, 16 a cycle and SM), EXACT 294, backward 506 (357 TFLOP/s).
-// 2 x 2047, 8 / 2 heads x 128, causal, float16: EXACT 48, backward 151 us (286 TFLOP/s).
+// 16 / 4 heads x 64, causal, bfloat16: 115 us (597 TFLOP/s). 8400 tokens, 8 heads x 32: forward 230 us (314 TFLOP/s of
+// the 32-wide products; half the rate of the exponentials, 16 a cycle and SM), EXACT 300, backward 489 (369 TFLOP/s).
+// 2 x 2047, 8 / 2 heads x 128, causal, float16: EXACT 49, backward 95 us (452 TFLOP/s).
 #pragma once
 
 #include <type_traits>
