@@ -203,10 +203,10 @@ int simt_forward(const AttnArgs& a, int dtype, const AttnWorkspace& w, unsigned 
                      : simt_forward_tile<T, DP, simt_r<T>()>(p, stream, err, err_len);
 }
 
-template <typename T, int DP, bool EXACT>
+template <typename T, int DP>
 int mma_split(const SplitArgs& p, cudaStream_t stream, char* err, size_t err_len) {
     const long long grid = (long long)p.splits * p.row_tiles * p.a.B * p.a.Hk;
-    constexpr auto kernel = attn_split_kernel<T, DP, EXACT>;
+    constexpr auto kernel = attn_split_kernel<T, DP>;
     constexpr size_t smem = SplitLayout<DP>::kSmem;
     if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     if (int rc = host::launch(err, err_len, "attn_split_kernel", kernel, dim3(unsigned(grid)),
@@ -222,22 +222,18 @@ int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* 
     p.a = a;
     p.part_o = workspace + w.part_o;
     p.part_ml = workspace + w.part_ml;
-    auto go = [&](auto exact) {
-        constexpr bool E = decltype(exact)::value;
-        if (a.D <= 32) return mma_split<T, 32, E>(p, stream, err, err_len);
-        if (a.D <= 64) return mma_split<T, 64, E>(p, stream, err, err_len);
-        return mma_split<T, 128, E>(p, stream, err, err_len);
-    };
-    return a.rest != nullptr ? go(std::true_type{}) : go(std::false_type{});
+    if (a.D <= 32) return mma_split<T, 32>(p, stream, err, err_len);
+    if (a.D <= 64) return mma_split<T, 64>(p, stream, err, err_len);
+    return mma_split<T, 128>(p, stream, err, err_len);
 }
 
-// Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. In microseconds, from
-// 216 calls of 1 to 8 images, 8 and 16 heads, D = 32, 64 and 128, 1024 to 22223 keys and 1 to 300 queries on B200: a
-// tensor-core CTA walks its keys at about 10 ns a key (13 for wide heads), and a launch that joins splits adds about 4;
-// the split kernel's time goes with its 16-row tiles times keys, behind about 6 for two launches. The faster kernel is
-// taken in all but a dozen of these calls, and the one taken is at most a quarter slower (64-wide heads, one query on
-// 22223 keys: 21 us against 17). Below 1024 keys the two differ by little (300 keys, one query: 6.3 against 5.0 at
-// D = 32, 7.6 against 9.7 at D = 128).
+// Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. A tensor-core CTA's
+// time goes with its keys, and a launch that joins splits adds to it; the split kernel's goes with its 16-row tiles times
+// keys, behind two launches. The constants stand for both, fitted to the choice rather than the times: of 432 calls of 1
+// to 8 images, 8 and 16 heads, D = 32, 64 and 128, 1024 to 22223 keys and 1 to 300 queries on B200, the slower kernel is
+// taken by more than 2 % in 24, at worst 1.37 times as slow (64-wide heads, 2 images, one query on 22223 keys: 32 us
+// against 24), and all of them together lose 0.7 % to the faster one each time. Below 1024 keys the two differ by little
+// (300 keys, one query, P in one part: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128).
 bool prefer_split(const AttnArgs& a) {
     if (a.N < 1024) return false;
     const double ctas = double((a.Q + 127) / 128) * a.B * a.H;

@@ -12,8 +12,9 @@
 // fragments (the queries are loaded in the same order), and a thread's consecutive elements of a value row are the
 // same column of as many 8-wide result tiles; the pairs of keys that a value fragment packs are made with byte
 // permutes. Tensor cores matter little here, but a 16-row product on them costs what a one-row product on CUDA cores
-// would. One query over 22223 keys, 8 images of 8 heads x 32 in bfloat16: 42 us (4.3 TB/s; 3.4 with lengths falling to
-// half), which the twelve warps' latency an SM sets, not the memory; loads straight into registers took 62.
+// would. One query over 22223 keys, 8 images of 8 heads x 32 in bfloat16, lengths falling to half: 45 us (3.2 TB/s),
+// which the latency of the twelve warps an SM sets, not the memory; loads straight into registers took 62 with P in one
+// part, where these took 41.
 #pragma once
 
 #include "td_attention.cuh"
@@ -79,7 +80,7 @@ __device__ __forceinline__ void mma_16816<__nv_bfloat16>(float (&d)[4], const ui
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ float fast_exp2(float x) {  // 2 ulp; P is rounded to 16 bits
+__device__ __forceinline__ float fast_exp2(float x) {  // 2 ulp
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
@@ -90,9 +91,10 @@ template <typename T> __device__ __forceinline__ uint32_t pack_pair(float lo, fl
     return *reinterpret_cast<const uint32_t*>(v);
 }
 
-// DP: 32, 64 or 128, D <= DP a multiple of 8; EXACT as in attn_tc_forward_kernel. grid: splits x row tiles x key
-// heads x images, splits fastest.
-template <typename T, int DP, bool EXACT>
+// DP: 32, 64 or 128, D <= DP a multiple of 8. P goes through its product in two 16-bit parts, as in
+// attn_tc_forward_kernel: two more products on data at hand, next to what the keys' way here takes. grid: splits x row
+// tiles x key heads x images, splits fastest.
+template <typename T, int DP>
 __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const SplitArgs args) {
     using Lay = SplitLayout<DP>;
     constexpr int kKeys = Lay::kKeys;               // keys a warp takes at a time
@@ -270,15 +272,13 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
             for (int y = 0; y < 4; ++y) {  // fragment registers: rows g, g + 8 of keys 0 .. 7, then of 8 .. 15
                 const int u = 2 * w + (y >> 1), e = y & 1;
                 p[y] = 0u;
-                if constexpr (EXACT) rest[y] = 0u;
+                rest[y] = 0u;
                 if (e == 1 && !both) continue;
                 const float p0 = fast_exp2(s[u][2 * e] - ref[e]), p1 = fast_exp2(s[u][2 * e + 1] - ref[e]);
                 sum[e] += p0 + p1;
                 p[y] = pack_pair<T>(p0, p1);
-                if constexpr (EXACT) {
-                    const T* r = reinterpret_cast<const T*>(&p[y]);
-                    rest[y] = pack_pair<T>(p0 - to_acc(r[0]), p1 - to_acc(r[1]));
-                }
+                const T* r = reinterpret_cast<const T*>(&p[y]);
+                rest[y] = pack_pair<T>(p0 - to_acc(r[0]), p1 - to_acc(r[1]));
             }
 #pragma unroll
             for (int i = 0; i < kDims; i += 2) {
@@ -288,10 +288,8 @@ __global__ void __launch_bounds__(kSplitWarps * 32) attn_split_kernel(const Spli
                 const uint32_t b2 = __byte_perm(v0, v1, 0x7632), b3 = __byte_perm(v2, v3, 0x7632);
                 mma_16816<T>(o[i], p, b0, b1);
                 mma_16816<T>(o[i + 1], p, b2, b3);
-                if constexpr (EXACT) {
-                    mma_16816<T>(o[i], rest, b0, b1);
-                    mma_16816<T>(o[i + 1], rest, b2, b3);
-                }
+                mma_16816<T>(o[i], rest, b0, b1);
+                mma_16816<T>(o[i + 1], rest, b2, b3);
             }
         }
 #pragma unroll

@@ -103,7 +103,7 @@ int pack_masks(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, bo
                         dim3(kPackThreads), 0, stream, true, p);
 }
 
-template <typename T, int DP, bool EXACT>
+template <typename T, int DP>
 int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsigned char* workspace,
             cudaStream_t stream, char* err, size_t err_len) {
     const AttnArgs& a = t.a;
@@ -112,7 +112,7 @@ int forward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsig
     if (int rc = make_map<DP>(&k, key_of(a), a, err, err_len)) return rc;
     if (int rc = make_map<DP>(&v, value_of(a), a, err, err_len)) return rc;
     if (int rc = pack_masks(t, w, mb, mh, false, workspace, stream, err, err_len)) return rc;
-    constexpr auto kernel = attn_tc_forward_kernel<T, DP, EXACT>;
+    constexpr auto kernel = attn_tc_forward_kernel<T, DP>;
     constexpr size_t smem = AttnFwdLayout<DP>::kSmemBytes;
     if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     t.splits = int(attn_tc_splits(a.B, a.Q, a.N, a.H));
@@ -191,17 +191,13 @@ int attn_tc_forward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_
                     unsigned char* workspace, cudaStream_t stream, char* err, size_t err_len) {
     AttnTcArgs t = {};
     t.a = a;
-    auto go = [&](auto type, auto exact) {
+    auto go = [&](auto type) {
         using T = decltype(type);
-        constexpr bool E = decltype(exact)::value;
-        if (a.D <= 32) return forward<T, 32, E>(t, w, mb, mh, workspace, stream, err, err_len);
-        if (a.D <= 64) return forward<T, 64, E>(t, w, mb, mh, workspace, stream, err, err_len);
-        return forward<T, 128, E>(t, w, mb, mh, workspace, stream, err, err_len);
+        if (a.D <= 32) return forward<T, 32>(t, w, mb, mh, workspace, stream, err, err_len);
+        if (a.D <= 64) return forward<T, 64>(t, w, mb, mh, workspace, stream, err, err_len);
+        return forward<T, 128>(t, w, mb, mh, workspace, stream, err, err_len);
     };
-    auto pick = [&](auto type) {
-        return a.rest != nullptr ? go(type, std::true_type{}) : go(type, std::false_type{});
-    };
-    return dtype == TD_F16 ? pick(__half{}) : pick(__nv_bfloat16{});
+    return dtype == TD_F16 ? go(__half{}) : go(__nv_bfloat16{});
 }
 
 int attn_tc_backward(int dtype, const AttnArgs& a, const AttnWorkspace& w, int64_t mb, int64_t mh,

@@ -6,8 +6,9 @@
 //   keys' grad       S^T = K Q^T, dP^T = V dO^T (lanes = keys), dV += P^T dO, dK += dS^T Q
 // so a 128-row operand stays in shared memory (K-major), tiles of 64 rows of the other side stream through a ring of
 // TMA slots, and each streamed tile serves as a K-major operand of one product and as an MN-major operand of another.
-// P and dS are rounded to the input type (the products take 16 bits; their sums are float32) and written back to TMEM
-// over the scores they came from, as the A operand of the next product: neither ever reaches shared memory. The two
+// P and dS are written back to TMEM over the scores they came from, as the A operand of the next product: neither ever
+// reaches shared memory. Products take 16 bits: the forward gives P in two parts, the backward rounds P and dS once.
+// Sums are float32. The two
 // gradients are separate blocks of one launch, each of which forms S and dP itself: 7 products instead of 5 and twice
 // the exponentials, but every sum has one owner and one order (no atomics, and no float32 gradient in memory but where
 // a few long rows of work are shared by several CTAs, whose partial sums are then joined in order).
@@ -23,9 +24,9 @@
 // SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two or three elementwise warpgroups
 // over two or three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their
 // waits (encoder backward below: 827 to 598 us); everything between two tiles is kept short. Measured: 2 x 4096 tokens,
-// 16 / 4 heads x 64, causal, bfloat16: 115 us (597 TFLOP/s). 8400 tokens, 8 heads x 32: forward 230 us (314 TFLOP/s of
-// the 32-wide products; half the rate of the exponentials, 16 a cycle and SM), EXACT 300, backward 489 (369 TFLOP/s).
-// 2 x 2047, 8 / 2 heads x 128, causal, float16: EXACT 49, backward 95 us (452 TFLOP/s).
+// 16 / 4 heads x 64, causal, bfloat16: 146 us (472 TFLOP/s). 8400 tokens, 8 heads x 32: forward 300 us, backward 489
+// (369 TFLOP/s).
+// 2 x 2047, 8 / 2 heads x 128, causal, float16: forward 49, backward 95 us (452 TFLOP/s).
 #pragma once
 
 #include <type_traits>
@@ -352,10 +353,10 @@ struct AttnFwdLayout {
 
 constexpr int kAttnFwdThreads = 224;  // loads, scores, products, four softmax warps
 
-// EXACT, for a forward that a backward follows: P is kept as two 16-bit parts, its rounding and what that took, which
-// both go through the product (one product more a tile), and the result's rounding is kept as well: see delta in
-// td_attention.cuh. Otherwise P is rounded once.
-template <typename T, int DP, bool EXACT>
+// P is kept as two 16-bit parts, its rounding and what that took, which both go through the product (one product more a
+// tile), so that the result's own rounding is the only one; a forward that a backward follows keeps what that one took
+// as well (see delta in td_attention.cuh). P rounded once would put the result 1.3 to 1.4 times as far from float64.
+template <typename T, int DP>
 __global__ void __launch_bounds__(kAttnFwdThreads, 2)
     attn_tc_forward_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
                            const __grid_constant__ CUtensorMap map_v, const AttnTcArgs args) {
@@ -474,7 +475,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             tc_fence_after();
             const uint32_t p = tmem + 64 * buf.at;
             issue_product<T, DP>(leader, tmem + 128, p, smem_addr(v), first);
-            if constexpr (EXACT) issue_product<T, DP>(leader, tmem + 128, p + 32, smem_addr(v), false);
+            issue_product<T, DP>(leader, tmem + 128, p + 32, smem_addr(v), false);
             commit(leader, &empty[ring.at]);
             commit(leader, &done[buf.at]);
             first = false;
@@ -562,10 +563,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 const float p0 = ex2(x0), p1 = ex2(x1);
                 sums[x % 4] = f2_add(sums[x % 4], f2(p0, p1));
                 p[x] = pack2<T>(p0, p1);
-                if constexpr (EXACT) {  // v's two registers of this pair are free: they take the rest
-                    const float2 r = unpack2<T>(p[x]);
-                    v[x / 16][x % 16] = pack2<T>(p0 - r.x, p1 - r.y);
-                }
+                const float2 r = unpack2<T>(p[x]);  // v's two registers of this pair are free: they take the rest
+                v[x / 16][x % 16] = pack2<T>(p0 - r.x, p1 - r.y);
             }
             {
                 float s0, s1;
@@ -573,10 +572,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 sum = s0 + s1;
             }
             tmem_st_32x32b_x32(sc, p);
-            if constexpr (EXACT) {
-                tmem_st_32x32b_x16(sc + 32, v[0]);
-                tmem_st_32x32b_x16(sc + 48, v[1]);
-            }
+            tmem_st_32x32b_x16(sc + 32, v[0]);
+            tmem_st_32x32b_x16(sc + 48, v[1]);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -623,7 +620,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                     }
                     *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + at + d + 8 * g) =
                         make_uint4(q[0], q[1], q[2], q[3]);
-                    if constexpr (EXACT)
+                    if (a.rest != nullptr)
                         *reinterpret_cast<uint4*>(static_cast<T*>(a.rest) + at + d + 8 * g) =
                             make_uint4(rest[0], rest[1], rest[2], rest[3]);
                 }

@@ -1,0 +1,68 @@
+"""16-bit attention on the GPU, over whole results: what is left besides the result's own rounding.
+
+Element by element a bound has to allow for every term of a sum at its worst, and cannot tell a factor that was rounded
+to 16 bits from one that was not. Over a whole result the roundings add up as a random walk does, and can. The measure
+is the result's distance from float64, in units of the distance that rounding float64's result to the type leaves (a
+step of relative size u = finfo.eps / 2 is off by 0.29 u to 0.58 u in the mean square, as the mantissa has it).
+
+What else is allowed. A factor kept in two 16-bit parts is off by u^2. Scores and sums are float32: D <= 128 products and
+scores of a few units make 2^-19 of a probability; a tensor core cuts its running sum by up to 2^-24 for every 16 terms,
+in one direction: 2^-16 over 4200 terms. Against u = 2^-11 that is u / 32, or u / 16 with as much again for the row's
+statistics, so at most (u / 16) / (0.29 u) = 0.22 of the measure where it all adds up in line with the rounding. One
+factor rounded once to 16 bits adds about 0.4 u at random instead: sqrt(2) of the measure or nearly so."""
+
+import pytest
+import torch
+
+from attention_oracle import U, attention_exact
+from marearts_tinydeform_b200 import _native, attention
+from test_attention_cuda import inputs, masks
+
+pytestmark = pytest.mark.gpu
+
+HALVES = (torch.float16, torch.bfloat16)
+LIMIT = 1.22
+# B, Q, N, H, Hk, D: a decoder's, a tile or two with every width, shared heads, keys split among CTAs (tensor cores),
+# one and few queries (the split kernel), an odd width (CUDA cores)
+SHAPES = [(1, 300, 300, 8, 8, 32), (2, 520, 640, 4, 2, 64), (1, 300, 515, 4, 2, 128), (2, 200, 333, 6, 3, 24),
+          (1, 300, 4200, 4, 4, 32), (2, 1, 2500, 8, 4, 64), (4, 9, 1500, 6, 2, 32), (2, 3, 4200, 8, 2, 128),
+          (1, 90, 150, 4, 4, 20)]
+
+
+def off(got, exact, dtype):
+    """The measure above; a result of zeros that should be zeros is off by nothing."""
+    own = (exact.to(dtype).double() - exact).norm()
+    return 0.0 if own == 0 and not (got.double() != exact).any() else ((got.double() - exact).norm() / own).item()
+
+
+@pytest.mark.parametrize('kind', ('none', 'pairs', 'causal', 'padding'))
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_only_the_result_is_rounded(cuda, dtype, shape, kind):
+    q, k, v, _ = inputs(shape, dtype, 41)
+    kw = masks(kind, shape, 41)
+    exact = attention_exact(q, k, v, **kw)[0][0]
+    with torch.inference_mode():
+        found = off(attention(q, k, v, **kw), exact, dtype)
+    assert found < LIMIT, found
+    trained = attention(*(t.detach().requires_grad_() for t in (q, k, v)), **kw).detach()
+    assert off(trained, exact, dtype) < LIMIT
+
+
+@pytest.mark.parametrize('kind', ('none', 'pairs', 'causal', 'padding'))
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_rest_is_what_rounding_took(cuda, dtype, shape, kind):
+    """The forward that a backward follows leaves its result in two 16-bit parts: together within u / 16 of float64 (by
+    the same count as above), where the result alone is at 0.29 u at best."""
+    q, k, v, _ = inputs(shape, dtype, 42)
+    kw = masks(kind, shape, 42)
+    _, tensors, _ = _native.attention_forward(q, k, v, kw['key_padding_mask'], kw['attn_mask'], kw['causal'],
+                                              shape[5] ** -0.5, for_backward=True)
+    out, rest = tensors[5], tensors[6]
+    exact = attention_exact(q, k, v, **kw)[0][0]
+    if not exact.any():
+        assert not out.any() and not rest.any()
+        return
+    assert (out.double() + rest.double() - exact).norm() / exact.norm() < U[dtype] / 16
+    assert (out.double() - exact).norm() / exact.norm() > U[dtype] / 4
