@@ -7,8 +7,10 @@
 // so a 128-row operand stays in shared memory (K-major), tiles of 64 rows of the other side stream through a ring of
 // TMA slots, and each streamed tile serves as a K-major operand of one product and as an MN-major operand of another.
 // P and dS are written back to TMEM over the scores they came from, as the A operand of the next product: neither ever
-// reaches shared memory. Products take 16 bits: the forward gives P in two parts, the backward rounds P and dS once.
-// Sums are float32. The two
+// reaches shared memory. The products take 16 bits, so both are kept in two parts, a rounding and what that took (in the
+// room that float32 scores leave), and each part goes through the product: with float32 sums, the results' own roundings
+// are the only ones to 16 bits. P and dS rounded once put the gradients 1.4 times as far from float64, in three quarters
+// of the time (encoder backward below: 489 us; grouped: 96). The two
 // gradients are separate blocks of one launch, each of which forms S and dP itself: 7 products instead of 5 and twice
 // the exponentials, but every sum has one owner and one order (no atomics, and no float32 gradient in memory but where
 // a few long rows of work are shared by several CTAs, whose partial sums are then joined in order).
@@ -24,9 +26,9 @@
 // SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two or three elementwise warpgroups
 // over two or three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their
 // waits (encoder backward below: 827 to 598 us); everything between two tiles is kept short. Measured: 2 x 4096 tokens,
-// 16 / 4 heads x 64, causal, bfloat16: 146 us (472 TFLOP/s). 8400 tokens, 8 heads x 32: forward 300 us, backward 489
-// (369 TFLOP/s).
-// 2 x 2047, 8 / 2 heads x 128, causal, float16: forward 49, backward 95 us (452 TFLOP/s).
+// 16 / 4 heads x 64, causal, bfloat16: 146 us (472 TFLOP/s). 8400 tokens, 8 heads x 32: forward 300 us, backward 677
+// (267 TFLOP/s).
+// 2 x 2047, 8 / 2 heads x 128, causal, float16: forward 49, backward 126 us (343 TFLOP/s).
 #pragma once
 
 #include <type_traits>
@@ -127,11 +129,6 @@ __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_
           "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_st_32x32b_x8(uint32_t taddr, const uint32_t* r) {
-    asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};"
-                 ::"r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(taddr)
-                 : "memory");
-}
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // 4-D tiled load of box (x, y, z, w), completing its bytes on the mbarrier (x * element size a multiple of 16 bytes).
@@ -211,6 +208,14 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
 }
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t v) {
     return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+}
+
+// Two floats in two 16-bit parts: their roundings, and the rounding of what those took.
+template <typename T>
+__device__ __forceinline__ void pack_parts(float x0, float x1, uint32_t& part, uint32_t& rest) {
+    part = pack2<T>(x0, x1);
+    const float2 r = unpack2<T>(part);
+    rest = pack2<T>(x0 - r.x, x1 - r.y);
 }
 
 // All lanes of a warp wait; false in every lane if any gave up.
@@ -302,15 +307,16 @@ __device__ __forceinline__ void issue_scores(uint32_t leader, uint32_t d, uint32
     }
 }
 
-// acc (+)= A x B: A 128 lanes x 64 packed elements in TMEM, B 64 rows x DP columns in shared memory.
-template <typename T, int DP>
+// acc (+)= A x B: A 128 lanes x 64 packed elements in TMEM, 16 of them every STEP columns, B 64 rows x DP columns in
+// shared memory.
+template <typename T, int DP, int STEP>
 __device__ __forceinline__ void issue_product(uint32_t leader, uint32_t acc, uint32_t a_tmem, uint32_t b_smem,
                                               bool first) {
     constexpr uint32_t idesc = attn_idesc<T, true>(DP);
     const uint64_t db = sdesc_mn<DP>(b_smem);
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-        mma_ts(leader, acc, a_tmem + 8 * k, db + uint64_t(AttnBox<DP>::kRow * k), idesc, !(first && k == 0));
+        mma_ts(leader, acc, a_tmem + STEP * k, db + uint64_t(AttnBox<DP>::kRow * k), idesc, !(first && k == 0));
 }
 
 // Clears the rows of padded keys in a slot's tile of 64 rows x DP columns. One warp.
@@ -474,8 +480,8 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
             if (!warp_wait(&pfull[buf.at], buf.parity, kErrMmaWait)) return false;
             tc_fence_after();
             const uint32_t p = tmem + 64 * buf.at;
-            issue_product<T, DP>(leader, tmem + 128, p, smem_addr(v), first);
-            issue_product<T, DP>(leader, tmem + 128, p + 32, smem_addr(v), false);
+            issue_product<T, DP, 8>(leader, tmem + 128, p, smem_addr(v), first);
+            issue_product<T, DP, 8>(leader, tmem + 128, p + 32, smem_addr(v), false);
             commit(leader, &empty[ring.at]);
             commit(leader, &done[buf.at]);
             first = false;
@@ -562,9 +568,7 @@ __global__ void __launch_bounds__(kAttnFwdThreads, 2)
                 f2_split(f2_fma(f2(v[x / 16][2 * (x % 16)], v[x / 16][2 * (x % 16) + 1]), c2, shift2), x0, x1);
                 const float p0 = ex2(x0), p1 = ex2(x1);
                 sums[x % 4] = f2_add(sums[x % 4], f2(p0, p1));
-                p[x] = pack2<T>(p0, p1);
-                const float2 r = unpack2<T>(p[x]);  // v's two registers of this pair are free: they take the rest
-                v[x / 16][x % 16] = pack2<T>(p0 - r.x, p1 - r.y);
+                pack_parts<T>(p0, p1, p[x], v[x / 16][x % 16]);  // (v's two registers of this pair are free)
             }
             {
                 float s0, s1;
@@ -688,9 +692,9 @@ __device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {  // one
     return exp2f(fminf(fmaxf(15.f - ceilf(log2f(bound)), -100.f), 100.f));
 }
 
-// P and dS of one row of a tile of 64 columns, from the scores at sc and sc + 64 to packed pairs in the same places.
-// The statistics are the row's own, or (KEYS) the columns', lse[64] and delta[64] at st. MASKED: w has a bit per open
-// pair.
+// P and dS of one row of a tile of 64 columns, from the scores at sc and sc + 64 to packed pairs in the same places: of
+// every 16 columns, 8 for the roundings, then 8 for what they took. The statistics are the row's own, or (KEYS) the
+// columns', lse[64] and delta[64] at st. MASKED: w has a bit per open pair.
 template <typename T, bool KEYS, bool MASKED>
 __device__ __forceinline__ void elementwise(uint32_t sc, const float* st, float row_lse, float row_delta, float c,
                                             float ds_scale, unsigned long long w) {
@@ -705,7 +709,7 @@ __device__ __forceinline__ void elementwise(uint32_t sc, const float* st, float 
             tmem_ld_32x32b_x16(sc + 16 * (part + 1), s[(part + 1) & 1]);
             tmem_ld_32x32b_x16(sc + 64 + 16 * (part + 1), d[(part + 1) & 1]);
         }
-        uint32_t p[8], e[8];
+        uint32_t p[16], e[16];  // the roundings, then what they took
         const F2 nc = f2(-c, -c), minus = f2(-1.f, -1.f), scale = f2(ds_scale, ds_scale);
         const uint32_t open = MASKED ? uint32_t(w >> (16 * part)) : 0u;
 #pragma unroll
@@ -731,12 +735,12 @@ __device__ __forceinline__ void elementwise(uint32_t sc, const float* st, float 
                     if (((open >> at) & 1u) == 0) p0 = e0 = 0.f;
                     if (((open >> (at + 1)) & 1u) == 0) p1 = e1 = 0.f;
                 }
-                p[at / 2] = pack2<T>(p0, p1);
-                e[at / 2] = pack2<T>(e0, e1);
+                if constexpr (KEYS) pack_parts<T>(p0, p1, p[at / 2], p[8 + at / 2]);
+                pack_parts<T>(e0, e1, e[at / 2], e[8 + at / 2]);
             }
         }
-        if constexpr (KEYS) tmem_st_32x32b_x8(sc + 8 * part, p);
-        tmem_st_32x32b_x8(sc + 64 + 8 * part, e);
+        if constexpr (KEYS) tmem_st_32x32b_x16(sc + 16 * part, p);
+        tmem_st_32x32b_x16(sc + 64 + 16 * part, e);
     }
 }
 
@@ -854,10 +858,13 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             // (this tile's scores are formed: what they made of padded rows has been replaced)
             if (pad != nullptr && !all) clear_padded<DP>(tile1(ring.at), pad, t * kAttnBN, a.N);
             tc_fence_after();
-            if constexpr (KEYS)  // dV += P^T dO
-                issue_product<T, DP>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(ring.at)), first);
+            if constexpr (KEYS) {  // dV += P^T dO
+                issue_product<T, DP, 16>(leader, tmem + Lay::kAcc + DP, sc, smem_addr(tile2(ring.at)), first);
+                issue_product<T, DP, 16>(leader, tmem + Lay::kAcc + DP, sc + 8, smem_addr(tile2(ring.at)), false);
+            }
             // dK += dS^T Q, dQ += dS K
-            issue_product<T, DP>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(ring.at)), first);
+            issue_product<T, DP, 16>(leader, tmem + Lay::kAcc, sc + 64, smem_addr(tile1(ring.at)), first);
+            issue_product<T, DP, 16>(leader, tmem + Lay::kAcc, sc + 72, smem_addr(tile1(ring.at)), false);
             commit(leader, &empty[ring.at]);
             commit(leader, &done[buf.at]);
             first = false;

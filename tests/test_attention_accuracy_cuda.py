@@ -16,7 +16,7 @@ import torch
 
 from attention_oracle import U, attention_exact
 from marearts_tinydeform_b200 import _native, attention
-from test_attention_cuda import inputs, masks
+from test_attention_cuda import NAMES, inputs, masks, run
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,14 @@ def test_rest_is_what_rounding_took(cuda, dtype, shape, kind):
         return
     assert (out.double() + rest.double() - exact).norm() / exact.norm() < U[dtype] / 16
     assert (out.double() - exact).norm() / exact.norm() > U[dtype] / 4
+
+
+@pytest.mark.parametrize('kind', ('none', 'pairs', 'causal', 'padding'))
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_only_the_gradients_are_rounded(cuda, dtype, shape, kind):
+    q, k, v, grad = inputs(shape, dtype, 43)
+    kw = masks(kind, shape, 43)
+    for name, got, want in zip(NAMES, run(q, k, v, grad, **kw), attention_exact(q, k, v, grad=grad, **kw)):
+        found = off(got, want[0], dtype)
+        assert found < LIMIT, (name, found)
