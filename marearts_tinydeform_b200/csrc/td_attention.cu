@@ -81,7 +81,10 @@ AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t
     const size_t acc = dtype == TD_F64 ? 8 : 4;
     const bool half = dtype == TD_F16 || dtype == TD_BF16;
     if (backward) {
-        w.amax = take(2 * kSms * sizeof(float));
+        if (dtype == TD_F16) {
+            w.amax = take(2 * size_t(B) * Hk * attn_delta_parts(B * Hk) * sizeof(float));
+            w.row_g = take(size_t(B) * H * pad_rows(Q) * sizeof(float));
+        }
         w.delta = take(size_t(B) * H * pad_rows(Q) * acc);
         int64_t k, q;
         grad_splits(dtype, B, Q, N, H, Hk, D, &k, &q);
@@ -228,12 +231,12 @@ int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* 
 }
 
 // Whether the split kernel takes a 16-bit forward that the tensor-core kernel could take as well. A tensor-core CTA's
-// time goes with its keys, and a launch that joins splits adds to it; the split kernel's goes with its 16-row tiles times
-// keys, behind two launches. The constants stand for both, fitted to the choice rather than the times: of 432 calls of 1
-// to 8 images, 8 and 16 heads, D = 32, 64 and 128, 1024 to 22223 keys and 1 to 300 queries on B200, the slower kernel is
-// taken by more than 2 % in 24, at worst 1.37 times as slow (64-wide heads, 2 images, one query on 22223 keys: 32 us
-// against 24), and all of them together lose 0.7 % to the faster one each time. Below 1024 keys the two differ by little
-// (300 keys, one query, P in one part: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128).
+// time goes with its keys, and a launch that joins splits adds to it; the split kernel's goes with its 16-row tiles
+// times keys, behind two launches. The constants stand for both, fitted to the choice rather than the times: of 432
+// calls of 1 to 8 images, 8 and 16 heads, D = 32, 64 and 128, 1024 to 22223 keys and 1 to 300 queries on B200, the
+// slower kernel is taken by more than 2 % in 24, at worst 1.37 times as slow (64-wide heads, 2 images, one query on
+// 22223 keys: 32 us against 24), and all of them together lose 0.7 % to the faster one each time. Below 1024 keys the
+// two differ by little (300 keys, one query, P in one part: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128).
 bool prefer_split(const AttnArgs& a) {
     if (a.N < 1024) return false;
     const double ctas = double((a.Q + 127) / 128) * a.B * a.H;

@@ -11,10 +11,10 @@
 // zero. With fewer key heads than query heads, query head h reads key head h / (H / Hk), and dk, dv are summed over
 // the query heads of their group inside the kernel.
 //
-// delta is the one sum of the backward whose terms cancel: dP_ij - delta_i is small against either where a row has
-// few keys of weight, and a delta from the rounded result is off by as much as a rounding of dS itself would be. A
-// forward that a backward follows therefore keeps, for 16-bit types, what the rounding took from each result as a second
-// 16-bit tensor, and delta is formed from both.
+// delta is the one sum of the backward whose terms cancel: dP_ij - delta_i is small against either where a row has few
+// keys of weight, and a delta from the rounded result is off by as much as a rounding of dS itself would be. A forward
+// that a backward follows therefore keeps, for 16-bit types, what the rounding took from each result as a second 16-bit
+// tensor, and delta is formed from both.
 //
 // Logarithms are base 2 in the kernels: c = scale * log2(e), lse = L * log2(e).
 //

@@ -142,13 +142,16 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
     if (int rc = pack_masks(t, w, mb, mh, true, workspace, stream, err, err_len)) return rc;
     int lanes = 1;
     while (lanes * 8 < a.D) lanes *= 2;
-    const long long rows = std::max((long long)a.B * a.H * a.Qp, (long long)a.B * a.Hk * a.N);
-    const int per_block = kDeltaThreads / lanes;
-    const int blocks = int(std::min<long long>(kSms, (rows + per_block - 1) / per_block));
-    t.amax = reinterpret_cast<float*>(workspace + w.amax);
-    t.amax_parts = blocks;
-    if (int rc = host::launch(err, err_len, "attn_delta_tc_kernel", attn_delta_tc_kernel<T>, dim3(unsigned(blocks)),
-                              dim3(kDeltaThreads), 0, stream, true, a, lanes, t.amax))
+    const long long rows = std::max((long long)(a.H / a.Hk) * a.Qp, (long long)a.N);
+    const int per_block = kDeltaThreads / lanes, pairs = a.B * a.Hk;
+    float* row_g = reinterpret_cast<float*>(workspace + w.row_g);
+    float* amax = reinterpret_cast<float*>(workspace + w.amax);
+    t.row_g = row_g;
+    t.amax = amax;
+    t.amax_parts = int(std::min<long long>(attn_delta_parts(pairs), (rows + per_block - 1) / per_block));
+    if (int rc = host::launch(err, err_len, "attn_delta_tc_kernel", attn_delta_tc_kernel<T>,
+                              dim3(unsigned(pairs) * unsigned(t.amax_parts)), dim3(kDeltaThreads), 0, stream, true, a,
+                              lanes, t.amax_parts, row_g, amax))
         return rc;
     t.kv_blocks = (a.N + kAttnBM - 1) / kAttnBM * a.B * a.Hk * a.k_splits;
     constexpr auto kernel = attn_tc_backward_kernel<T, DP>;

@@ -5,15 +5,15 @@
 //   queries' grad    S = Q K^T, dP = dO V^T (lanes = queries), dS = P (dP - delta), dQ += dS K
 //   keys' grad       S^T = K Q^T, dP^T = V dO^T (lanes = keys), dV += P^T dO, dK += dS^T Q
 // so a 128-row operand stays in shared memory (K-major), tiles of 64 rows of the other side stream through a ring of
-// TMA slots, and each streamed tile serves as a K-major operand of one product and as an MN-major operand of another.
-// P and dS are written back to TMEM over the scores they came from, as the A operand of the next product: neither ever
-// reaches shared memory. The products take 16 bits, so both are kept in two parts, a rounding and what that took (in the
-// room that float32 scores leave), and each part goes through the product: with float32 sums, the results' own roundings
-// are the only ones to 16 bits. P and dS rounded once put the gradients 1.4 times as far from float64, in three quarters
-// of the time (encoder backward below: 489 us; grouped: 96). The two
-// gradients are separate blocks of one launch, each of which forms S and dP itself: 7 products instead of 5 and twice
-// the exponentials, but every sum has one owner and one order (no atomics, and no float32 gradient in memory but where
-// a few long rows of work are shared by several CTAs, whose partial sums are then joined in order).
+// TMA slots, and each streamed tile serves as a K-major operand of one product and as an MN-major operand of another. P
+// and dS are written back to TMEM over the scores they came from, as the A operand of the next product: neither ever
+// reaches shared memory. The products take 16 bits, so both are kept in two parts, a rounding and what that took (in
+// the room that float32 scores leave), and each part goes through the product: with float32 sums, the results' own
+// roundings are the only ones to 16 bits. P and dS rounded once put the gradients 1.4 times as far from float64, in
+// three quarters of the time (encoder backward below: 489 us; grouped: 96). The two gradients are separate blocks of
+// one launch, each of which forms S and dP itself: 7 products instead of 5 and twice the exponentials, but every sum
+// has one owner and one order (no atomics, and no float32 gradient in memory but where a few long rows of work are
+// shared by several CTAs, whose partial sums are then joined in order).
 //
 // Columns past D (D < DP) and rows past the last token are zero through the tensor maps' fill. Scores of closed pairs
 // are replaced by -infinity (P, dS by zero); tiles without an open pair are skipped by every role alike, from one
@@ -51,7 +51,9 @@ struct AttnTcArgs {
     long long cb_b, cb_h, cf_b, cf_h;
     int col_words;              // words a key's row of col_bits has
     int col_tiles;              // flags a row of col_flags has
-    float* amax;                // float16 backward: per block of the delta kernel max|dO|, then per block max|V|
+    // float16 backward: |dO|^2 of every row [B, H, Qp]; of each (image, key head) and block of the delta kernel the
+    // largest |dO|^2, then the same of |V|^2 [2][B, Hk, amax_parts]
+    const float *row_g, *amax;
     int amax_parts;
     int kv_blocks;              // backward: blocks of the keys' gradient, launched first
     // forward: the key tiles of a query tile are shared by `splits` CTAs; with more than one these take their partial
@@ -674,22 +676,28 @@ struct AttnBwdLayout {
 };
 
 
-// float16 keeps dS times a power of two that makes its bound, 2 D max|dO| max|V|, at most 2^15: it cannot overflow, and
-// gradients far below or above one lose nothing. bfloat16 has float32's exponents and needs no scale.
-__device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args) {  // one warp
-    float g = 0.f, v = 0.f;
+// float16 keeps dS times a power of two that makes its bound 2^15 or little less, so that dS cannot overflow and is a
+// normal number down to 2^-29 of the bound. |dS_ij| <= P_ij |dO_i| (|v_j| + |o_i|) <= 2 |dO_i| max|v|, the maximum over
+// the keys of the (image, key head). A row of the queries' gradient is a lane's own and has a scale of its own, row_g
+// being its |dO_i|^2. The keys' gradient sums over queries, so there one scale holds for the (image, key head), from
+// the largest |dO_i|. bfloat16 has float32's exponents and needs no scale.
+template <bool KEYS>
+__device__ __forceinline__ float attn_ds_scale(const AttnTcArgs& args, int bhk, float row_g) {  // one warp
+    const float* amax = args.amax + (long long)bhk * args.amax_parts;
+    const long long values = (long long)args.a.B * args.a.Hk * args.amax_parts;
+    float g = KEYS ? 0.f : row_g, v = 0.f;
     for (int i = threadIdx.x & 31; i < args.amax_parts; i += 32) {
-        g = fmaxf(g, args.amax[i]);
-        v = fmaxf(v, args.amax[args.amax_parts + i]);
+        if (KEYS) g = fmaxf(g, amax[i]);
+        v = fmaxf(v, amax[values + i]);
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) {
-        g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, x));
+        if (KEYS) g = fmaxf(g, __shfl_xor_sync(0xffffffffu, g, x));
         v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, x));
     }
-    const float bound = 2.f * float(args.a.D) * g * v;
-    if (!(bound > 0.f) || !(bound < INFINITY)) return 1.f;
-    return exp2f(fminf(fmaxf(15.f - ceilf(log2f(bound)), -100.f), 100.f));
+    const float square = g * v;  // of finite float16 numbers: 2^-96 .. 2^78, or zero
+    if (!(square > 0.f) || !(square < INFINITY)) return 1.f;
+    return exp2f(14.f - ceilf(0.5f * log2f(square)));
 }
 
 // P and dS of one row of a tile of 64 columns, from the scores at sc and sc + 64 to packed pairs in the same places: of
@@ -877,13 +885,14 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         const int quarter = warp & 3, wg = (warp - 4) >> 2, r = r0 + quarter * 32 + lane;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16);
         const float c = float(a.scale * 1.4426950408889634);
-        const float ds_scale = kHalf ? attn_ds_scale(args) : 1.f;
-        float row_lse = INFINITY, row_delta = 0.f;
+        float row_lse = INFINITY, row_delta = 0.f, row_g = 0.f;
         if (!KEYS) {  // the rows' own statistics (the arrays hold Qp rows, a multiple of the tile)
             const long long at = ((long long)b * a.H + h0) * a.Qp + r;
             row_lse = static_cast<const float*>(a.lse)[at];
             row_delta = static_cast<const float*>(a.delta)[at];
+            if constexpr (kHalf) row_g = args.row_g[at];
         }
+        const float ds_scale = kHalf ? attn_ds_scale<KEYS>(args, b * a.Hk + hk, row_g) : 1.f;
         // the warpgroups take the tiles in turn
         constexpr int NG = Lay::kGroups;
         int n = 0, turn = wg;
@@ -1142,51 +1151,63 @@ __global__ void __launch_bounds__(kPackThreads) attn_pack_kernel(const PackArgs 
 }
 
 // delta as in attn_delta_kernel for 16-bit types with D a multiple of 8: 16-byte loads, `lanes` (a power of two, at
-// least D / 8) threads a row, at most a CTA an SM walking over the rows. float16: each CTA also leaves max|dO| over its
-// rows and max|V| over its share of the keys that are there (a maximum of maxima has no order).
+// least D / 8) threads a row, `parts` CTAs for the rows of each (image, key head), its whole group of query heads.
+// float16: row_g takes each row's |dO|^2, amax the largest of them in the CTA's rows and the largest |V|^2 in its share
+// of the keys that are there (a maximum of maxima has no order).
 constexpr int kDeltaThreads = 512;
 template <typename T>
-__global__ void __launch_bounds__(kDeltaThreads) attn_delta_tc_kernel(const AttnArgs a, int lanes, float* amax) {
+__global__ void __launch_bounds__(kDeltaThreads)
+    attn_delta_tc_kernel(const AttnArgs a, int lanes, int parts, float* row_g, float* amax) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
-    const int sub = threadIdx.x % lanes;
-    const long long step = (long long)gridDim.x * (kDeltaThreads / lanes);
-    const long long first = (long long)blockIdx.x * (kDeltaThreads / lanes) + threadIdx.x / lanes;
+    const int sub = threadIdx.x % lanes, bhk = blockIdx.x / parts, part = blockIdx.x % parts;
+    const long long step = (long long)parts * (kDeltaThreads / lanes);
+    const long long first = (long long)part * (kDeltaThreads / lanes) + threadIdx.x / lanes;
     const bool col = sub * 8 < a.D;
     grid_dependency_wait();
     launch_dependents();
     float top_g = 0.f, top_v = 0.f;
-    const long long rows = (long long)a.B * a.H * a.Qp;
+    const long long rows = (long long)(a.H / a.Hk) * a.Qp;  // of (image, key head) bhk, which lie together
     // whole warps take the same number of turns (a warp holds whole rows)
-    for (long long row = first, warp0 = first - threadIdx.x % 32 / lanes; warp0 < rows; row += step, warp0 += step) {
+    for (long long r = first, warp0 = first - threadIdx.x % 32 / lanes; warp0 < rows; r += step, warp0 += step) {
+        const long long row = bhk * rows + r, bh = row / a.Qp;
         const int i = int(row % a.Qp);
-        const long long bh = row / a.Qp;
-        float sum = 0.f;
-        if (row < rows && i < a.Q && col) {
+        float sum = 0.f, square = 0.f;
+        if (r < rows && i < a.Q && col) {
             const long long at = ((bh / a.H * a.Q + i) * a.H + bh % a.H) * a.D + sub * 8;
-            float o[8], g[8], r[8];
+            float o[8], g[8], e[8];
             load16<T>(static_cast<const T*>(a.out_in) + at, o);
             load16<T>(static_cast<const T*>(a.grad_out) + at, g);
-            load16<T>(static_cast<const T*>(a.rest_in) + at, r);
+            load16<T>(static_cast<const T*>(a.rest_in) + at, e);
 #pragma unroll
             for (int x = 0; x < 8; ++x) {
-                sum += (o[x] + r[x]) * g[x];
-                if constexpr (kHalf) top_g = fmaxf(top_g, fabsf(g[x]));
+                sum += (o[x] + e[x]) * g[x];
+                if constexpr (kHalf) square += g[x] * g[x];
             }
         }
-        for (int x = lanes / 2; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
-        if (row < rows && sub == 0) static_cast<float*>(a.delta)[row] = sum;
+        for (int x = lanes / 2; x > 0; x >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, x);
+            if constexpr (kHalf) square += __shfl_xor_sync(0xffffffffu, square, x);
+        }
+        top_g = fmaxf(top_g, square);
+        if (r < rows && sub == 0) {
+            static_cast<float*>(a.delta)[row] = sum;
+            if constexpr (kHalf) row_g[row] = square;
+        }
     }
     if constexpr (kHalf) {
-        const long long keys = (long long)a.B * a.Hk * a.N;  // row = (b * Hk + hk) * N + j
-        for (long long row = first; row < keys && col; row += step) {
-            const long long j = row % a.N, bh = row / a.N, b = bh / a.Hk;
-            if (a.padding != nullptr && a.padding[b * a.N + j] != 0) continue;
-            float v[8];
-            load16<T>(static_cast<const T*>(a.v) + b * a.v_b + bh % a.Hk * a.v_h + j * a.v_t + sub * 8, v);
+        const long long b = bhk / a.Hk;
+        const T* values = static_cast<const T*>(a.v) + b * a.v_b + bhk % a.Hk * a.v_h + sub * 8;
+        const uint8_t* pad = a.padding == nullptr ? nullptr : a.padding + b * a.N;
+        for (long long j = first, warp0 = first - threadIdx.x % 32 / lanes; warp0 < a.N; j += step, warp0 += step) {
+            float v[8], square = 0.f;
+            if (j < a.N && col && (pad == nullptr || pad[j] == 0)) {
+                load16<T>(values + j * a.v_t, v);
 #pragma unroll
-            for (int x = 0; x < 8; ++x) top_v = fmaxf(top_v, fabsf(v[x]));
+                for (int x = 0; x < 8; ++x) square += v[x] * v[x];
+            }
+            for (int x = lanes / 2; x > 0; x >>= 1) square += __shfl_xor_sync(0xffffffffu, square, x);
+            top_v = fmaxf(top_v, square);
         }
-        __syncwarp();
         __shared__ float tops[2][kDeltaThreads / 32];
 #pragma unroll
         for (int x = 16; x > 0; x >>= 1) {
@@ -1201,7 +1222,7 @@ __global__ void __launch_bounds__(kDeltaThreads) attn_delta_tc_kernel(const Attn
         if (threadIdx.x < 2) {
             float top = 0.f;
             for (int x = 0; x < kDeltaThreads / 32; ++x) top = fmaxf(top, tops[threadIdx.x][x]);
-            amax[threadIdx.x * gridDim.x + blockIdx.x] = top;
+            amax[(long long)threadIdx.x * gridDim.x + blockIdx.x] = top;
         }
     }
 }

@@ -77,3 +77,32 @@ def test_only_the_gradients_are_rounded(cuda, dtype, shape, kind):
     for name, got, want in zip(NAMES, run(q, k, v, grad, **kw), attention_exact(q, k, v, grad=grad, **kw)):
         found = off(got, want[0], dtype)
         assert found < LIMIT, (name, found)
+
+
+@pytest.mark.parametrize('shape', [(2, 300, 1100, 4, 4, 32), (3, 260, 300, 4, 2, 64), (2, 140, 400, 2, 1, 128),
+                                   (2, 300, 4200, 2, 2, 32)], ids=str)
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_gradients_of_mixed_size(cuda, dtype, shape):
+    """A row, a head and an image whose incoming gradients are 2^12 times the others', and an image with a value 2^8 times
+    the others: the small rows' gradients are as good as if they were alone."""
+    q, k, v, grad = inputs(shape, dtype, 44)
+    B, Q, N, H, Hk, D = shape
+    grad = (grad / 2).view(B, Q, H, D).clone()
+    small_q = torch.ones((B, Q, H), dtype=torch.bool, device='cuda')
+    small_k = torch.ones((B, N, Hk), dtype=torch.bool, device='cuda')
+    small_q[0, 5], small_k[0] = False, False  # a row, which every key of its image has a share of
+    small_q[1, :, H - 1], small_k[1, :, Hk - 1] = False, False  # a head
+    if B > 2:
+        small_q[2], small_k[2] = False, False  # an image
+    grad = torch.where(small_q[..., None], grad, grad.float().mul(2.0 ** 12).clamp(-30000, 30000).to(dtype))
+    for spread in (1.0, 2.0 ** 8):
+        v = v.clone()
+        v[0, N // 2] *= spread
+        got = run(q, k, v, grad.view(B, Q, H * D))
+        want = attention_exact(q, k, v, grad=grad.view(B, Q, H * D))
+        for name, a, (b, _), small in zip(NAMES[1:], got[1:], want[1:], (small_q, small_k, small_k)):
+            if small.any():
+                found = off(a[small], b[small], dtype)
+                assert found < LIMIT, (name, spread, found)
+            found = off(a, b, dtype)
+            assert found < LIMIT, (name, spread, found)
