@@ -84,6 +84,7 @@ AttnWorkspace attn_workspace(int dtype, int64_t B, int64_t Q, int64_t N, int64_t
         if (dtype == TD_F16) {
             w.amax = take(2 * size_t(B) * Hk * attn_delta_parts(B * Hk) * sizeof(float));
             w.row_g = take(size_t(B) * H * pad_rows(Q) * sizeof(float));
+            w.keys_lse = take(size_t(B) * H * pad_rows(Q) * sizeof(float));
         }
         w.delta = take(size_t(B) * H * pad_rows(Q) * acc);
         int64_t k, q;

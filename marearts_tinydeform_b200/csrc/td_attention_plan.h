@@ -9,7 +9,8 @@ namespace td {
 
 // Byte offsets into a call's workspace, and the sizes of the packed mask (rows = 1: from the padding alone).
 struct AttnWorkspace {
-    size_t part_o, part_ml, part_k, part_v, part_q, amax, row_g, delta, row_bits, row_flags, col_bits, col_flags, total;
+    size_t part_o, part_ml, part_k, part_v, part_q, amax, row_g, keys_lse, delta, row_bits, row_flags, col_bits, col_flags,
+        total;
     int64_t images, heads, rows, words, col_words;
 };
 

@@ -146,12 +146,14 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
     const int per_block = kDeltaThreads / lanes, pairs = a.B * a.Hk;
     float* row_g = reinterpret_cast<float*>(workspace + w.row_g);
     float* amax = reinterpret_cast<float*>(workspace + w.amax);
+    float* keys_lse = reinterpret_cast<float*>(workspace + w.keys_lse);
+    t.keys_lse = attn_p_bits<T>() != 0 ? keys_lse : static_cast<const float*>(a.lse);
     t.row_g = row_g;
     t.amax = amax;
     t.amax_parts = int(std::min<long long>(attn_delta_parts(pairs), (rows + per_block - 1) / per_block));
     if (int rc = host::launch(err, err_len, "attn_delta_tc_kernel", attn_delta_tc_kernel<T>,
                               dim3(unsigned(pairs) * unsigned(t.amax_parts)), dim3(kDeltaThreads), 0, stream, true, a,
-                              lanes, t.amax_parts, row_g, amax))
+                              lanes, t.amax_parts, keys_lse, row_g, amax))
         return rc;
     t.kv_blocks = (a.N + kAttnBM - 1) / kAttnBM * a.B * a.Hk * a.k_splits;
     constexpr auto kernel = attn_tc_backward_kernel<T, DP>;

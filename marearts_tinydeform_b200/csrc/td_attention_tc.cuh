@@ -55,6 +55,7 @@ struct AttnTcArgs {
     // largest |dO|^2, then the same of |V|^2 [2][B, Hk, amax_parts]
     const float *row_g, *amax;
     int amax_parts;
+    const float* keys_lse;      // backward: lse as the keys' blocks take it (see attn_p_bits)
     int kv_blocks;              // backward: blocks of the keys' gradient, launched first
     // forward: the key tiles of a query tile are shared by `splits` CTAs; with more than one these take their partial
     // results, o [B * H * Q][splits][D] and (maximum, sum) [B * H * Q][splits][2], for attn_combine_kernel
@@ -676,6 +677,11 @@ struct AttnBwdLayout {
 };
 
 
+// A key's P may be about 1 / N for every query, from some 16000 keys on below float16's normal numbers. So the keys'
+// gradient in float16 keeps it times 2^15 (P is at most one), from an lse that is 15 less, and divides dV by that.
+// bfloat16 has float32's exponents.
+template <typename T> constexpr int attn_p_bits() { return std::is_same<T, __half>::value ? 15 : 0; }
+
 // float16 keeps dS times a power of two that makes its bound 2^15 or little less, so that dS cannot overflow and is a
 // normal number down to 2^-29 of the bound. |dS_ij| <= P_ij |dO_i| (|v_j| + |o_i|) <= 2 |dO_i| max|v|, the maximum over
 // the keys of the (image, key head). A row of the queries' gradient is a lane's own and has a scale of its own, row_g
@@ -822,7 +828,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
                 tma_load_4d((job < KB ? tile1(s) : tile2(s)) + box * AttnBox<DP>::kTile,
                             job < KB ? &map_b1 : &map_b2, &full[s], 64 * box, t * kAttnBN, KEYS ? h : hk, b, pol);
             } else if (job >= 2 * KB && job < kJobs) {
-                const float* src = static_cast<const float*>(job == 2 * KB ? a.lse : a.delta);
+                const float* src = job == 2 * KB ? args.keys_lse : static_cast<const float*>(a.delta);
                 mbar_arrive_expect_tx(&full[s], kAttnBN * 4u);
                 bulk_load(stats(s) + (job - 2 * KB) * kAttnBN,
                           src + ((long long)b * a.H + h) * a.Qp + t * kAttnBN, kAttnBN * 4u, &full[s]);
@@ -893,6 +899,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             if constexpr (kHalf) row_g = args.row_g[at];
         }
         const float ds_scale = kHalf ? attn_ds_scale<KEYS>(args, b * a.Hk + hk, row_g) : 1.f;
+        constexpr float kP = float(1 << (KEYS ? attn_p_bits<T>() : 0));  // what P is kept times
         // the warpgroups take the tiles in turn
         constexpr int NG = Lay::kGroups;
         int n = 0, turn = wg;
@@ -932,9 +939,9 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             const uint32_t sc = lanes + 128 * buf.at;
             // 16 columns at a time, the next ones' loads in flight meanwhile; P and dS go where the first scores were
             if (open)
-                elementwise<T, KEYS, false>(sc, stats(ring.at), row_lse, row_delta, c, ds_scale, w);
+                elementwise<T, KEYS, false>(sc, stats(ring.at), row_lse, row_delta, c, ds_scale / kP, w);
             else
-                elementwise<T, KEYS, true>(sc, stats(ring.at), row_lse, row_delta, c, ds_scale, w);
+                elementwise<T, KEYS, true>(sc, stats(ring.at), row_lse, row_delta, c, ds_scale / kP, w);
             tmem_st_wait();
             tc_fence_before();
             __syncwarp();
@@ -948,7 +955,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         // the gradients' rows: a warpgroup an accumulator for the keys' block, else half of the columns each
         if (ok && wg < 2) {
             const bool is_v = KEYS && wg == 1;
-            const float f = is_v ? 1.f : float(a.scale) / ds_scale;
+            const float f = is_v ? 1.f / kP : float(a.scale) / ds_scale;
             const bool gone = KEYS && a.padding != nullptr && r < a.N && a.padding[(long long)b * a.N + r] != 0;
             const long long at = (((long long)b * rows + r) * heads + head) * a.D;
             T* out = static_cast<T*>(KEYS ? (is_v ? a.grad_v : a.grad_k) : a.grad_q) + at;
@@ -1152,12 +1159,12 @@ __global__ void __launch_bounds__(kPackThreads) attn_pack_kernel(const PackArgs 
 
 // delta as in attn_delta_kernel for 16-bit types with D a multiple of 8: 16-byte loads, `lanes` (a power of two, at
 // least D / 8) threads a row, `parts` CTAs for the rows of each (image, key head), its whole group of query heads.
-// float16: row_g takes each row's |dO|^2, amax the largest of them in the CTA's rows and the largest |V|^2 in its share
-// of the keys that are there (a maximum of maxima has no order).
+// float16: keys_lse takes lse less attn_p_bits, row_g each row's |dO|^2, amax the largest of them in the CTA's rows and
+// the largest |V|^2 in its share of the keys that are there (a maximum of maxima has no order).
 constexpr int kDeltaThreads = 512;
 template <typename T>
 __global__ void __launch_bounds__(kDeltaThreads)
-    attn_delta_tc_kernel(const AttnArgs a, int lanes, int parts, float* row_g, float* amax) {
+    attn_delta_tc_kernel(const AttnArgs a, int lanes, int parts, float* keys_lse, float* row_g, float* amax) {
     constexpr bool kHalf = std::is_same<T, __half>::value;
     const int sub = threadIdx.x % lanes, bhk = blockIdx.x / parts, part = blockIdx.x % parts;
     const long long step = (long long)parts * (kDeltaThreads / lanes);
@@ -1191,7 +1198,10 @@ __global__ void __launch_bounds__(kDeltaThreads)
         top_g = fmaxf(top_g, square);
         if (r < rows && sub == 0) {
             static_cast<float*>(a.delta)[row] = sum;
-            if constexpr (kHalf) row_g[row] = square;
+            if constexpr (kHalf) {
+                row_g[row] = square;
+                keys_lse[row] = static_cast<const float*>(a.lse)[row] - float(attn_p_bits<T>());
+            }
         }
     }
     if constexpr (kHalf) {

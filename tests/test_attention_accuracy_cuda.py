@@ -106,3 +106,13 @@ def test_gradients_of_mixed_size(cuda, dtype, shape):
                 assert found < LIMIT, (name, spread, found)
             found = off(a, b, dtype)
             assert found < LIMIT, (name, spread, found)
+
+
+@pytest.mark.parametrize('shape', [(1, 500, 20000, 1, 1, 32), (1, 300, 60000, 1, 1, 64)], ids=str)
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_gradients_over_very_long_keys(cuda, dtype, shape):
+    """Probabilities near float16's smallest normal number and below (1 / 60000 = 1.7e-5 against 6.1e-5)."""
+    q, k, v, grad = inputs(shape, dtype, 45)
+    for name, got, want in zip(NAMES, run(q, k, v, grad * 40), attention_exact(q, k, v, grad=grad * 40)):
+        found = off(got, want[0], dtype)
+        assert found < LIMIT, (name, found)
