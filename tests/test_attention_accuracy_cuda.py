@@ -14,7 +14,7 @@ factor rounded once to 16 bits adds about 0.4 u at random instead: sqrt(2) of th
 import pytest
 import torch
 
-from attention_oracle import U, attention_exact
+from attention_oracle import U, attention_exact, blocked_pairs
 from marearts_tinydeform_b200 import _native, attention
 from test_attention_cuda import NAMES, inputs, masks, run
 
@@ -116,3 +116,35 @@ def test_gradients_over_very_long_keys(cuda, dtype, shape):
     for name, got, want in zip(NAMES, run(q, k, v, grad * 40), attention_exact(q, k, v, grad=grad * 40)):
         found = off(got, want[0], dtype)
         assert found < LIMIT, (name, found)
+
+
+@pytest.mark.parametrize('kind', ('none', 'pairs', 'causal'))
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_gradients_behind_large_results(cuda, dtype, shape, kind):
+    """Values around 16 that differ by about one: what is left of dP - delta is a sixteenth of either, so that a delta from
+    rounded results, without what rounding took from them, puts the queries' gradient 20 to 120 times as far off as its
+    own rounding does.
+
+    What is allowed follows the result's error into them. A result that is off by a relative x moves delta_i by at most
+    t_i = x sum|do_i o_i|, and with it dq_i by scale t_i sum_j P_ij k_j and dk_j by scale sum_i P_ij t_i q_i. Here x is
+    u^2 for the result's two parts, u^2 for those of P, and the tensor core's cuts of a sum of values that all have one
+    sign: 2^-24 of it for each of two groups of 8 in the 16 terms of a product, so N 2^-24 / 8 for one part of P (the other
+    adds u of that)."""
+    q, k, v, grad = inputs(shape, dtype, 46)
+    v = v + 16
+    kw = masks(kind, shape, 46)
+    B, Q, N, H, Hk, D = shape
+    x, G, scale = 2 * U[dtype] ** 2 + N * 2.0 ** -24 / 8 * (1 + U[dtype]), H // Hk, D ** -0.5
+    exact = attention_exact(q, k, v, grad=grad, **kw)
+    wide_q, wide_k = q.double().transpose(1, 2), k.double().transpose(1, 2).repeat_interleave(G, 1)
+    scores = (wide_q @ wide_k.transpose(2, 3) * scale).masked_fill(
+        blocked_pairs(B, Q, N, kw['key_padding_mask'], kw['attn_mask'], kw['causal'], q.device), -float('inf'))
+    p = scores.softmax(3).nan_to_num(0.0)
+    t = x * (grad.double() * exact[0][0]).abs().view(B, Q, H, D).sum(3).transpose(1, 2)[..., None]
+    moved = {'grad_query': scale * t * (p @ wide_k),
+             'grad_key': scale * (p.transpose(2, 3) @ (t * wide_q.abs())).view(B, Hk, G, N, D).sum(2)}
+    for name, got, (want, _) in zip(NAMES, run(q, k, v, grad, **kw), exact):
+        own, found = (want.to(dtype).double() - want).norm().item(), off(got, want, dtype)
+        allowed = moved[name].norm().item() / own if name in moved and own > 0 else 0.0
+        assert found < LIMIT + allowed, (name, found, allowed)
