@@ -296,3 +296,38 @@ def test_float32_is_float32_over_long_keys(cuda, shape):
         want = want[0] if isinstance(want, tuple) else want
         error = float((got.double() - want).norm() / want.norm())
         assert error < 2.0 ** -19, (name, error)
+
+
+@pytest.mark.parametrize('causal', (False, True))
+@pytest.mark.parametrize('padded', (False, True))
+@pytest.mark.parametrize('shape', [(2, 150, 210, 4, 2, 32), (3, 3, 1500, 2, 1, 64)], ids=str)
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_mask_layouts(cuda, dtype, shape, padded, causal):
+    """Masks shared by images or heads, expanded, sliced, transposed and of any nonzero bytes, against the same pairs
+    written out as a dense [B, H, Q, N] mask: the same bits."""
+    B, Q, N, H, _, _ = shape
+    q, k, v, grad = inputs(shape, dtype, 51)
+    g = torch.Generator(device='cuda').manual_seed(52)
+    kw = dict(causal=causal, key_padding_mask=masks('padding', shape, 51)['key_padding_mask'] if padded else None)
+
+    def some(*s):
+        m = torch.rand(s, generator=g, device='cuda') < 0.5
+        m[..., N // 3:N // 3 + 140] = True
+        return m
+
+    wide = some(B, H, Q + 3, N + 13)
+    layouts = {'[Q, N]': some(Q, N), '[1, 1, Q, N]': some(1, 1, Q, N), '[B, 1, Q, N]': some(B, 1, Q, N),
+               '[1, H, Q, N]': some(1, H, Q, N), 'images expanded': some(1, H, Q, N).expand(B, H, Q, N),
+               'heads expanded': some(B, 1, Q, N).expand(B, H, Q, N), 'both expanded': some(Q, N).expand(B, H, Q, N),
+               'queries expanded': some(B, H, 1, N).expand(B, H, Q, N), 'one row for all': some(1, N).expand(Q, N),
+               'sliced': wide[:, :, 2:Q + 2, 5:N + 5], 'sliced [Q, N]': wide[0, 0, 2:Q + 2, 5:N + 5],
+               'every other image': some(2 * B, H, Q, N)[::2], 'heads innermost': some(B, Q, H, N).transpose(1, 2),
+               'transposed': some(B, H, Q, N).transpose(2, 3).contiguous().transpose(2, 3),
+               'keys expanded': (torch.rand((Q, 1), generator=g, device='cuda') < 0.3).expand(Q, N)}
+    for name, m in layouts.items():
+        dense = m.expand(B, H, Q, N).contiguous()
+        want = run(q, k, v, grad, attn_mask=dense, **kw)
+        any_byte = m.to(torch.uint8) * 2 if m.dim() == 2 else torch.where(m, 255, 0).to(torch.uint8)
+        for form in (m, any_byte):
+            for part, a, b in zip(NAMES, run(q, k, v, grad, attn_mask=form, **kw), want):
+                assert torch.equal(a, b), (name, form.dtype, part)
