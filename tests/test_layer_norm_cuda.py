@@ -195,3 +195,50 @@ def test_decoder_layer(cuda, dtype):
     with torch.inference_mode():
         assert torch.equal(decoder_layer(p, attention, layer_norm, library_cross).isfinite().all(),
                            torch.tensor(True, device='cuda'))
+
+
+def library_cross_at(tgt, p):
+    """library_cross with sampling locations and weights that pass no gradient."""
+    return deform_attn_layer(tgt.detach(), p['ref'], p['memory'], p['shapes'], p['starts'], p['H'], p['P'], p['sw'],
+                             p['sb'], p['vw'], p['vb'], output_weight=p['ow'], residual=tgt, norm_weight=p['n2_w'],
+                             norm_bias=p['n2_b'])
+
+
+def reference_cross_at(tgt, p):
+    out = deform_attn_layer_reference(tgt.detach(), p['ref'], p['memory'], p['shapes'], p['starts'], p['H'], p['P'],
+                                      p['sw'], p['sb'], p['vw'], p['vb'], p['ow'])
+    return layer_norm_reference(out, p['n2_w'], p['n2_b'], tgt)
+
+
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_decoder_layer_with_fixed_locations(cuda, dtype):
+    """The decoder layer's gradients where nothing jumps: the sampling locations pass none, so that no sample's slope
+    changes at a pixel's border, and every gradient is held to the count of roundings alone (as above: twenty of half a
+    step on the way there and back, and 12 for a sample moved by a rounded location)."""
+    H, P, C = 8, 4, 256
+    args = make_layer(2, 90, C, H, C // H, C, [(12, 10), (6, 5)], P, ref_dim=4, dtype=dtype, seed=23)
+    q, ref, mem, shapes, starts, sw, sb, vw, vb = [None if t is None else t.cuda() for t in args]
+    g = torch.Generator(device='cuda').manual_seed(24)
+
+    def normal(*s, std):
+        return (torch.randn(s, generator=g, device='cuda') * std).to(dtype)
+
+    mask = torch.zeros((90, 90), dtype=torch.bool, device='cuda')
+    mask[30:, :30] = True
+    p = dict(query=q, qkv_w=normal(3 * C, C, std=C ** -0.5), H=H, P=P, mask=mask, ref=ref, memory=mem, shapes=shapes,
+             starts=starts, sw=sw, sb=sb, vw=vw, vb=vb, ow=normal(C, C, std=C ** -0.5), n1_w=1 + normal(C, std=0.1),
+             n1_b=normal(C, std=0.1), n2_w=1 + normal(C, std=0.1), n2_b=normal(C, std=0.1))
+    names = ('query', 'qkv_w', 'memory', 'vw', 'ow', 'n1_w', 'n1_b', 'n2_w', 'n2_b')
+    grad = normal(2, 90, C, std=0.1)
+
+    def both(p, *parts):
+        p = dict(p, **{n: p[n].detach().requires_grad_() for n in names})
+        out = decoder_layer(p, *parts)
+        return [out.detach()] + list(torch.autograd.grad(out, [p[n] for n in names], grad.to(out.dtype)))
+
+    wide = {n: t.double() if torch.is_tensor(t) and t.is_floating_point() else t for n, t in p.items()}
+    want = both(wide, attention_reference, layer_norm_reference, reference_cross_at)
+    got = both(p, attention, layer_norm, library_cross_at)
+    for name, a, b in zip(('out', *names), got, want):
+        rel = ((a.double() - b).norm() / b.norm()).item()
+        assert rel <= 32 * U[dtype] + 2e-6 * (dtype == torch.float32) + 1e-13, f'{name}: {rel}'
