@@ -73,8 +73,8 @@ __device__ __forceinline__ void tf32_load(float* dst, const float* src, long lon
     }
 }
 
-// s[j] (+)= rows g, g + 8 of a . rows 8 j .. of b.
-template <int DP, int NT>
+// s[j] = rows g, g + 8 of a . rows 8 j .. of b. CHECK: infinities come out as float32 has them.
+template <int DP, int NT, bool CHECK>
 __device__ __forceinline__ void tf32_scores(const float* a, const float* b, int g, int t, float (&s)[NT / 8][4]) {
     constexpr int kPitch = DP + 4;
     float small[NT / 8][4];
@@ -110,10 +110,28 @@ __device__ __forceinline__ void tf32_scores(const float* a, const float* b, int 
             mma_split<4>(s + j0, small + j0, ah[1], al[1], bh[1], bl[1]);
         }
     }
+    bool bad = false;
 #pragma unroll
     for (int j = 0; j < NT / 8; ++j)
 #pragma unroll
-        for (int y = 0; y < 4; ++y) s[j][y] += small[j][y];
+        for (int y = 0; y < 4; ++y) {
+            s[j][y] += small[j][y];
+            if (CHECK) bad = bad || s[j][y] != s[j][y];
+        }
+    // An infinity (or a number that TF32 rounds to one) has no low part, inf - inf, and its products with a low part of
+    // zero are none either. A warp that found one forms its scores in plain float32.
+    if (!CHECK || !__any_sync(0xffffffffu, bad)) return;
+    float plain[NT / 2];  // in local memory, so that this seldom taken way is short
+#pragma unroll 1
+    for (int i = 0; i < NT / 2; ++i) {
+        const float *x = a + (g + 8 * (i >> 1 & 1)) * kPitch, *z = b + (8 * (i >> 2) + 2 * t + (i & 1)) * kPitch;
+        float sum = 0.f;
+#pragma unroll 1
+        for (int k = 0; k < DP; ++k) sum = fmaf(x[k], z[k], sum);
+        plain[i] = sum;
+    }
+#pragma unroll
+    for (int i = 0; i < NT / 2; ++i) s[i / 4][i % 4] = plain[i];
 }
 
 // o[i] += p . rows of b, columns 8 i ..
@@ -193,7 +211,7 @@ __global__ void __launch_bounds__(kTf32Threads, kTf32Ctas<DP, false>)
         copy_wait<1>();
         __syncthreads();
         float s[NT / 8][4];
-        tf32_scores<DP, NT>(qs + 16 * warp * Lay::kPitch, tile(buf, 0), g, t, s);
+        tf32_scores<DP, NT, true>(qs + 16 * warp * Lay::kPitch, tile(buf, 0), g, t, s);
         const bool plain = mask == nullptr && pad == nullptr && j0 + NT <= a.N &&
                            (!a.causal || j0 + NT - 1 <= i0 + off);
         float keep[2];
@@ -344,8 +362,8 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
         copy_wait<1>();
         __syncthreads();
         float p[NT / 8][4], s[NT / 8][4];
-        tf32_scores<DP, NT>(fix1 + 16 * warp * Lay::kPitch, tile(buf, 0), g, t, p);
-        tf32_scores<DP, NT>(fix2 + 16 * warp * Lay::kPitch, tile(buf, 1), g, t, s);
+        tf32_scores<DP, NT, true>(fix1 + 16 * warp * Lay::kPitch, tile(buf, 0), g, t, p);
+        tf32_scores<DP, NT, false>(fix2 + 16 * warp * Lay::kPitch, tile(buf, 1), g, t, s);
         const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
         const bool plain = mask == nullptr && (KEYS || pad == nullptr) && (KEYS || col + NT <= a.N) &&
                            (!a.causal || (KEYS ? r0 + kTf32Rows - 1 <= col + off : col + NT - 1 <= r0 + off));

@@ -140,6 +140,23 @@ def test_padded_keys_may_hold_anything(cuda, dtype, Q):
             assert torch.equal(got, ref), f'{name} with {junk} in padded rows'
 
 
+@pytest.mark.parametrize('shape', [(1, 40, 300, 2, 2, 32), (2, 70, 333, 4, 2, 64), (1, 20, 270, 1, 1, 128),
+                                   (1, 33, 90, 2, 2, 32), (1, 5, 700, 2, 1, 64), (1, 130, 1700, 2, 1, 24)], ids=str)
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_keys_at_infinity(cuda, dtype, shape):
+    """A key whose score is minus infinity for every query has no probability: results are those of a call that pads it."""
+    q, k, v, _ = inputs(shape, dtype, 14)
+    q[..., 0] = q[..., 0].abs() + 0.25
+    pad = torch.zeros((shape[0], shape[2]), dtype=torch.bool, device='cuda')
+    for j in (0, 7, shape[2] // 2, shape[2] - 1):
+        k[:, j, :, 0] = -float('inf')
+        pad[:, j] = True
+    exact = attention_exact(q, k, v, key_padding_mask=pad)[0]
+    with torch.inference_mode():
+        check(attention(q, k, v), exact, 'out (inference)')
+    check(attention(*(t.detach().requires_grad_() for t in (q, k, v))).detach(), exact, 'out')
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_rows_without_keys_are_zero(cuda, dtype):
     shape = (2, 131, 90, 4, 4, 32)
