@@ -265,7 +265,8 @@ def attention(query, key, value, key_padding_mask=None, attn_mask=None, causal=F
     key_padding_mask: bool [B, N], True = no key there (its rows may hold anything). attn_mask: bool [Q, N] or
     [B or 1, H or 1, Q, N], True = query i may not use key j (DINO's denoising mask); what a blocked pair's key and
     value hold must still be finite. causal: query i uses the keys up to i + N - Q. A query left without any key gets
-    zeros, and passes no gradient. scale: positive, 1 / sqrt(D) unless given.
+    zeros, and passes no gradient. scale: positive, 1 / sqrt(D) unless given. An infinite key that makes a score minus
+    infinity has no probability there; an infinite value or any NaN makes what uses it infinite or NaN.
 
     CUDA tensors run this library's kernels, forward and backward (no probabilities are kept; sums run in float32,
     float64 for float64; gradients are the same bits every time); CPU tensors run attention_reference. The backward

@@ -913,8 +913,10 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
             bool open = all;
             unsigned long long w = ~0ull;
             if constexpr (KEYS) {
-                open = open && (!a.causal || r0 + kAttnBM - 1 <= c0 + off);
+                // (the queries behind the last, which are zeros, do not count: an infinite key makes NaN of them)
+                open = open && c0 + kAttnBN <= a.Q && (!a.causal || r0 + kAttnBM - 1 <= c0 + off);
                 if (!open) {
+                    w = bits_below(a.Q - c0);
                     if (a.causal) w &= ~bits_below(r - off - c0);
                     if (args.col_bits != nullptr && r < a.N) {
                         const uint2 x = __ldg(reinterpret_cast<const uint2*>(

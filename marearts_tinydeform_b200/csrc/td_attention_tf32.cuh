@@ -365,7 +365,8 @@ __device__ __forceinline__ void attn_tf32_backward_block(const AttnArgs& a, int 
         tf32_scores<DP, NT, true>(fix1 + 16 * warp * Lay::kPitch, tile(buf, 0), g, t, p);
         tf32_scores<DP, NT, false>(fix2 + 16 * warp * Lay::kPitch, tile(buf, 1), g, t, s);
         const uint8_t* mask = a.mask == nullptr ? nullptr : a.mask + b * a.m_b + h * a.m_h;
-        const bool plain = mask == nullptr && (KEYS || pad == nullptr) && (KEYS || col + NT <= a.N) &&
+        // (the queries behind the last, which are zeros, do not count: an infinite key makes NaN of them)
+        const bool plain = mask == nullptr && (KEYS || pad == nullptr) && col + NT <= (KEYS ? a.Q : a.N) &&
                            (!a.causal || (KEYS ? r0 + kTf32Rows - 1 <= col + off : col + NT - 1 <= r0 + off));
         const float* st = stats + 2 * buf * NT;
 #pragma unroll

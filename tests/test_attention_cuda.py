@@ -157,6 +157,28 @@ def test_keys_at_infinity(cuda, dtype, shape):
     check(attention(*(t.detach().requires_grad_() for t in (q, k, v))).detach(), exact, 'out')
 
 
+@pytest.mark.parametrize('causal', (False, True))
+@pytest.mark.parametrize('shape', [(1, 40, 300, 2, 2, 32), (2, 70, 333, 4, 2, 64), (1, 20, 270, 1, 1, 128),
+                                   (1, 33, 90, 2, 2, 32), (1, 5, 700, 2, 1, 64), (1, 130, 1700, 2, 1, 24),
+                                   (2, 40, 20, 2, 2, 32)], ids=str)
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_gradients_with_keys_at_infinity(cuda, dtype, shape, causal):
+    """Such keys' gradients are zero and they take no part in the others', but for the queries' in the infinite column
+    (zero times infinity)."""
+    q, k, v, grad = inputs(shape, dtype, 15)
+    q[..., 0] = q[..., 0].abs() + 0.25
+    pad = torch.zeros((shape[0], shape[2]), dtype=torch.bool, device='cuda')
+    for j in (0, 7, shape[2] // 2, shape[2] - 1):
+        k[:, j, :, 0] = -float('inf')
+        pad[:, j] = True
+    exact = attention_exact(q, k, v, key_padding_mask=pad, grad=grad, causal=causal)
+    got = run(q, k, v, grad, causal=causal)
+    B, Q, H, D = q.shape
+    exact[1], got[1] = [t.view(B, Q, H, D)[..., 1:] for t in exact[1]], got[1][..., 1:]
+    for name, a, b in zip(NAMES, got, exact):
+        check(a, b, name)
+
+
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_rows_without_keys_are_zero(cuda, dtype):
     shape = (2, 131, 90, 4, 4, 32)
