@@ -84,6 +84,36 @@ def test_rows_far_from_zero_and_constant_rows(cuda, dtype):
     assert all(torch.isfinite(t).all() for t in run(flat, w, b, None, dy))
 
 
+@pytest.mark.parametrize('C', (7, 256, 300, 515, 1024, 2048, 4099, 8192))
+@pytest.mark.parametrize('dtype, far', [(torch.float32, 1e4), (torch.float32, -3e5), (torch.float64, 1e9),
+                                        (torch.float16, 1e3), (torch.bfloat16, 1e3)], ids=str)
+def test_rows_very_far_from_zero(cuda, dtype, far, C):
+    """Offsets thousands of deviations wide. Each centred value is a difference of near numbers and exact, so their sums
+    err by (C + 32) e of the centred values and not of the offset, and z by that; only the saved mean, which the backward
+    subtracts, is rounded to e of the offset (e: half a step of the accumulators' type)."""
+    x, w, b, _, dy = inputs(40, C, dtype, 6)
+    x = (x.double() * max(1.0, abs(far) * U[dtype] * 8) + far).to(dtype)  # a few steps of the type wide at least
+    e, u = U[torch.float64 if dtype == torch.float64 else torch.float32], U[dtype]
+    s, wd, d = x.double(), w.double(), dy.double()
+    mean = s.mean(1, keepdim=True)
+    c = s - mean
+    c = c - c.mean(1, keepdim=True)  # (float64 itself loses some of such a mean)
+    rstd = 1 / torch.sqrt((c ** 2).mean(1, keepdim=True) + 1e-5)
+    z, g = c * rstd, (C + 32) * e
+    z_err = g * (c.abs().mean(1, keepdim=True) * rstd + z.abs()) + 4 * e * z.abs()
+    y = z * wd + b.double()
+    got = run(x, w, b, None, dy)
+    check(got[0], (y, (u + 4 * e) * y.abs() + z_err * wd.abs() + 4 * e * (z * wd).abs()), 'y')
+    z_err = z_err + 1.01 * e * mean.abs() * rstd
+    h = d * wd
+    a1, a2 = h.abs().mean(1, keepdim=True), (h * z).abs().mean(1, keepdim=True)
+    dx = rstd * (h - h.mean(1, keepdim=True) - z * (h * z).mean(1, keepdim=True))
+    check(got[1], (dx, u * dx.abs() + rstd * (8 * g * (h.abs() + a1 + z.abs() * a2) + z_err * a2
+                                              + z.abs() * (h.abs() * z_err).mean(1, keepdim=True))), 'grad_x')
+    dw = (d * z).sum(0)
+    check(got[2], (dw, u * dw.abs() + (40 + 32) * e * (d * z).abs().sum(0) + (d.abs() * z_err).sum(0)), 'grad_weight')
+
+
 def test_same_bits_every_time(cuda):
     x, w, b, r, dy = inputs(9000, 256, torch.float16, 3)
     first = run(x, w, b, r, dy)
