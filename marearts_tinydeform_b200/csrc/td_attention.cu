@@ -57,7 +57,7 @@ SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H,
 // 16-bit causal 2 x 2047 x 8 heads (2 of keys) x 128: 150 us unsplit, 91; 1 query on 8400 keys x 8 heads x 32: 70 us
 // and 30, in float32 739 and 79; 2 x 300 queries on 8400 keys in float32: 961 and 545.
 void grad_splits(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t* k, int64_t* q) {
-    const bool tc = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0 && N > 32;  // (unless misaligned)
+    const bool tc = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0 && N > 1;  // (unless misaligned)
     const int64_t rows = tc ? 128 : dtype == TD_F64 ? 32 : 64, cols = std::min<int64_t>(rows, 64);
     auto tiles = [](int64_t n, int64_t of) { return (n + of - 1) / of; };
     const int64_t kc = H / Hk * tiles(Q, cols), qc = tiles(N, cols);

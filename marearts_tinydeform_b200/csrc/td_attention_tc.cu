@@ -182,9 +182,8 @@ bool attn_tc_fits(int dtype, const AttnArgs& a) {
     if ((dtype != TD_F16 && dtype != TD_BF16) || !host::best_policy()) return false;
     if (a.D % 8 != 0) return false;
     // One key, where the gradients of queries and keys are zero: the CUDA-core kernels form dP and delta in one order
-    // and find it so (3.5 us against 4.6). Up to 32 keys, the backward, whose tiles of 64 are mostly empty (8 images of
-    // 8 heads x 32, 32 keys: 9 us against 18).
-    if (a.N < (a.grad_q == nullptr ? 2 : 33)) return false;
+    // and find it so (8 images of 8 heads x 32, 32 queries: 7.7 us forward against 4.6).
+    if (a.N < 2) return false;
     if (!operand_fits(query_of(a), a) || !operand_fits(key_of(a), a) || !operand_fits(value_of(a), a)) return false;
     if (!aligned16(a.lse)) return false;
     if (a.grad_q == nullptr) return aligned16(a.out) && aligned16(a.rest);

@@ -148,3 +148,32 @@ def test_gradients_behind_large_results(cuda, dtype, shape, kind):
         own, found = (want.to(dtype).double() - want).norm().item(), off(got, want, dtype)
         allowed = moved[name].norm().item() / own if name in moved and own > 0 else 0.0
         assert found < LIMIT + allowed, (name, found, allowed)
+
+
+@pytest.mark.parametrize('kind', ('none', 'pairs', 'causal'))
+@pytest.mark.parametrize('N', (2, 3, 5, 8, 17, 32, 33))
+@pytest.mark.parametrize('D', (16, 32, 64, 128))
+@pytest.mark.parametrize('dtype', HALVES, ids=str)
+def test_gradients_of_few_keys(cuda, dtype, D, N, kind):
+    """Sums of few terms, where a factor rounded to 16 bits would show in each. Where one key has all the weight, what is
+    left of dP - delta is small against both and off by what test_gradients_behind_large_results counts: a few u^2 of
+    sum|do_i v_j| for each pair, in proportion to its probability."""
+    shape = (2, 150, N, 4, 2, D)
+    q, k, v, grad = inputs(shape, dtype, 47)
+    kw = masks(kind, shape, 47)
+    B, Q, _, H, Hk, _ = shape
+    exact = attention_exact(q, k, v, grad=grad, **kw)
+    G, scale, x = H // Hk, D ** -0.5, 4 * U[dtype] ** 2 + 16 * 2.0 ** -24
+    wide_q, wide_k, wide_v = (t.double().transpose(1, 2) for t in (q, k, v))
+    wide_k, wide_v = wide_k.repeat_interleave(G, 1), wide_v.repeat_interleave(G, 1)
+    scores = (wide_q @ wide_k.transpose(2, 3) * scale).masked_fill(
+        blocked_pairs(B, Q, N, kw['key_padding_mask'], kw['attn_mask'], kw['causal'], q.device), -float('inf'))
+    p = scores.softmax(3).nan_to_num(0.0)
+    do = grad.double().view(B, Q, H, D).transpose(1, 2)
+    t = x * p * (do.abs() @ wide_v.abs().transpose(2, 3)).amax(3, keepdim=True)
+    moved = {'grad_query': scale * (t @ wide_k.abs()),
+             'grad_key': scale * (t.transpose(2, 3) @ wide_q.abs()).view(B, Hk, G, N, D).sum(2)}
+    for name, got, (want, _) in zip(NAMES, run(q, k, v, grad, **kw), exact):
+        own, found = (want.to(dtype).double() - want).norm().item(), off(got, want, dtype)
+        allowed = moved[name].norm().item() / own if name in moved and own > 0 else 0.0
+        assert found < LIMIT + allowed, (name, found, allowed)
