@@ -23,7 +23,7 @@
 //
 // What bounds them is the time a tile takes through its stations rather than any unit: barrier, product, commit and
 // TMEM latencies and, in the elementwise warps, instructions that wait for one another. So the forward runs two CTAs an
-// SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two or three elementwise warpgroups
+// SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two elementwise warpgroups
 // over two or three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their
 // waits (encoder backward below: 827 to 598 us); everything between two tiles is kept short. Measured: 2 x 4096 tokens,
 // 16 / 4 heads x 64, causal, bfloat16: 146 us (472 TFLOP/s). 8400 tokens, 8 heads x 32: forward 300 us, backward 677
@@ -659,9 +659,7 @@ struct AttnBwdLayout {
     static constexpr int kBufs = DP == 128 ? 2 : 3;
     static constexpr int kStages = DP == 128 ? 4 : 6;
     static constexpr uint32_t kAcc = kBufs * 128;  // first accumulator's TMEM column
-    // warpgroups of the elementwise work: three overlap their waits best where the products are short (encoder, D = 32:
-    // 498 us against 529 with two), two where those share the time (D = 64: 271 against 278)
-    static constexpr int kGroups = DP == 32 ? 3 : 2;
+    static constexpr int kGroups = 2;  // warpgroups of the elementwise work (encoder with three: 676 us against 677)
     static constexpr int kThreads = 128 * (1 + kGroups);  // loads, scores, products, -, the warpgroups
     static constexpr uint32_t kStageBytes = 2 * kTileBytes;
     static constexpr uint32_t kRing = 2 * kFixedBytes;
@@ -955,7 +953,7 @@ __device__ __forceinline__ void attn_tc_backward_block(const CUtensorMap& map_fi
         ok = ok && (n == 0 || warp_wait(finished, 0u, kErrMmaWait));
         tc_fence_after();
         // the gradients' rows: a warpgroup an accumulator for the keys' block, else half of the columns each
-        if (ok && wg < 2) {
+        if (ok) {
             const bool is_v = KEYS && wg == 1;
             const float f = is_v ? 1.f / kP : float(a.scale) / ds_scale;
             const bool gone = KEYS && a.padding != nullptr && r < a.N && a.padding[(long long)b * a.N + r] != 0;
