@@ -287,9 +287,9 @@ def attention(query, key, value, key_padding_mask=None, attn_mask=None, causal=F
 def layer_norm(x, weight, bias=None, residual=None, eps=1e-5):
     """Layer norm of x + residual over the last dimension (up to 8192 wide), in x's shape and dtype.
 
-    The sum is not rounded before the norm, and the statistics are float32 (float64 for float64). CUDA tensors run
-    this library's kernels, forward and backward (the column sums of the weight's and bias's gradients in a fixed
-    order); CPU tensors run layer_norm_reference.
+    weight, bias and residual have x's dtype and device. The sum is not rounded before the norm, and the statistics are
+    float32 (float64 for float64). CUDA tensors run this library's kernels, forward and backward (the column sums of the
+    weight's and bias's gradients in a fixed order); CPU tensors run layer_norm_reference.
     """
     _native.check_layer_norm(x, weight, bias, residual, eps)
     if not x.is_cuda:

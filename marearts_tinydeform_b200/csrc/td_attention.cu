@@ -23,7 +23,7 @@ void split_plan(int64_t N, int64_t splits, int64_t step, SplitArgs* p) {
 
 // The mma.sync split kernel's plan: the rows of a key head's group in tiles of 16. One wave of long splits where every
 // image has all its keys; shorter ones where some have not, so that the CTAs of the full ones do not end last (8 images
-// of 22223 keys, the lengths falling to half: 48 us with 2, 42 with 6; all of them full: 43 and 43; one image: 12 and
+// of 22223 keys, the lengths falling to half: 51 us with 2, 44 with 6; without padding: 47 and 45; one image: 13 and
 // 17). No split of fewer than 256 keys, two of the kernel's tiles.
 SplitArgs mma_split_plan(int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, bool padding) {
     SplitArgs p = {};
@@ -54,8 +54,8 @@ SplitArgs simt_split_plan(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H,
 // do not hold the others up: a key head's block goes over the queries of its whole group, and few queries make few
 // blocks. A CTA gets at most about the work of one of three on every SM, or, on tensor cores (one CTA an SM), of two;
 // but at least two tiles there, sixteen here, since partial sums and the launch that joins them cost about as much.
-// 16-bit causal 2 x 2047 x 8 heads (2 of keys) x 128: 150 us unsplit, 91; 1 query on 8400 keys x 8 heads x 32: 70 us
-// and 30, in float32 739 and 79; 2 x 300 queries on 8400 keys in float32: 961 and 545.
+// 16-bit causal 2 x 2047 x 8 heads (2 of keys) x 128: 183 us unsplit, 125; 1 query on 8400 keys x 8 heads x 32: 90 us
+// and 36, in float32 798 and 80; 2 x 300 queries on 8400 keys in float32: 1044 and 577.
 void grad_splits(int dtype, int64_t B, int64_t Q, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t* k, int64_t* q) {
     const bool tc = (dtype == TD_F16 || dtype == TD_BF16) && D % 8 == 0 && N > 1;  // (unless misaligned)
     const int64_t rows = tc ? 128 : dtype == TD_F64 ? 32 : 64, cols = std::min<int64_t>(rows, 64);
@@ -237,7 +237,7 @@ int mma_split_forward(const AttnArgs& a, const AttnWorkspace& w, unsigned char* 
 // calls of 1 to 8 images, 8 and 16 heads, D = 32, 64 and 128, 1024 to 22223 keys and 1 to 300 queries on B200, the
 // slower kernel is taken by more than 2 % in 24, at worst 1.37 times as slow (64-wide heads, 2 images, one query on
 // 22223 keys: 32 us against 24), and all of them together lose 0.7 % to the faster one each time. Below 1024 keys the
-// two differ by little (300 keys, one query, P in one part: 6.3 against 5.0 at D = 32, 7.6 against 9.7 at D = 128).
+// two differ by little (300 keys, one query: 7.8 on tensor cores against 5.4 at D = 32, 9.8 against 9.4 at D = 128).
 bool prefer_split(const AttnArgs& a) {
     if (a.N < 1024) return false;
     const double ctas = double((a.Q + 127) / 128) * a.B * a.H;
@@ -251,7 +251,7 @@ bool prefer_split(const AttnArgs& a) {
 
 // float32 on tensor cores: rows of whole 16-byte vectors and at least 256 keys. Below, where a CTA has a few tiles, its
 // four warps' longer chains show (one head, 64 x 64: 12 us at D = 32 and 44 at D = 128 against 9 and 24 on CUDA cores;
-// 256 keys: 14 and 30 against 14 and 31; 4 x 1100 x 8 heads x 32: 209 against 233, the backward 493 against 699).
+// 256 keys: 14 and 30 against 14 and 31; 4 x 1100 x 8 heads x 32: 216 against 234, the backward 527 against 708).
 bool tf32_fits(const AttnArgs& a) {
     return host::best_policy() && a.N >= 256 && a.vec_q && a.vec_k && a.vec_v && (a.grad_q == nullptr || a.vec_g) &&
            (reinterpret_cast<uintptr_t>(a.lse) & 15u) == 0;

@@ -9,8 +9,8 @@ namespace td {
 
 // Byte offsets into a call's workspace, and the sizes of the packed mask (rows = 1: from the padding alone).
 struct AttnWorkspace {
-    size_t part_o, part_ml, part_k, part_v, part_q, amax, row_g, keys_lse, delta, row_bits, row_flags, col_bits, col_flags,
-        total;
+    size_t part_o, part_ml, part_k, part_v, part_q, amax, row_g, keys_lse, delta;
+    size_t row_bits, row_flags, col_bits, col_flags, total;
     int64_t images, heads, rows, words, col_words;
 };
 
@@ -36,7 +36,8 @@ int join(const AttnArgs& a, cudaStream_t stream, char* err, size_t err_len) {
                         dim3(256), 0, stream, true, a);
 }
 
-// CTAs of the tensor-core backward's delta kernel for each of `pairs` (image, key head) pairs, at most: two an SM in all.
+// CTAs of the tensor-core backward's delta kernel for each of `pairs` (image, key head) pairs, at most: two an SM in
+// all.
 inline int64_t attn_delta_parts(int64_t pairs) { return pairs < 2 * kSms ? 2 * kSms / pairs : 1; }
 // How many CTAs share the keys of a query tile in the tensor-core forward.
 int64_t attn_tc_splits(int64_t B, int64_t Q, int64_t N, int64_t H);

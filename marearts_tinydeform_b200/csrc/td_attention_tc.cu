@@ -169,9 +169,9 @@ int backward(AttnTcArgs& t, const AttnWorkspace& w, int64_t mb, int64_t mh, unsi
 
 }  // namespace
 
-// One wave of two CTAs an SM (300 queries on 8400 keys, 8 heads of 32: 51 us unsplit, 22 in 12 splits; 2 images 92 and
-// 30), of at least 512 keys a split and where two splits save more than joining them costs (1024 keys: 15 us against
-// 18; 1600: 18 against 14).
+// One wave of two CTAs an SM (300 queries on 8400 keys, 8 heads of 32: 112 us unsplit, 23 in 12 splits; 2 images 112
+// and 35), of at least 512 keys a split and where two splits save more than joining them costs for any number of images
+// (1024 keys: 16.6 us unsplit, in two 13.5 for one image and 19.3 for four; 1600 keys: 24 and 15).
 int64_t attn_tc_splits(int64_t B, int64_t Q, int64_t N, int64_t H) {
     const int64_t ctas = (Q + kAttnBM - 1) / kAttnBM * B * H;
     if (N < 1536 || ctas == 0) return 1;

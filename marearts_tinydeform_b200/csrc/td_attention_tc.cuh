@@ -23,12 +23,13 @@
 //
 // What bounds them is the time a tile takes through its stations rather than any unit: barrier, product, commit and
 // TMEM latencies and, in the elementwise warps, instructions that wait for one another. So the forward runs two CTAs an
-// SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two elementwise warpgroups
-// over two or three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their
-// waits (encoder backward below: 827 to 598 us); everything between two tiles is kept short. Measured: 2 x 4096 tokens,
-// 16 / 4 heads x 64, causal, bfloat16: 146 us (472 TFLOP/s). 8400 tokens, 8 heads x 32: forward 300 us, backward 677
-// (267 TFLOP/s).
-// 2 x 2047, 8 / 2 heads x 128, causal, float16: forward 49, backward 126 us (343 TFLOP/s).
+// SM (256 TMEM columns each) with the next scores formed meanwhile, the backward two elementwise warpgroups over two or
+// three score buffers; products of scores and of P, dS are issued by a warp each, which overlaps their waits (827 to
+// 598 us for the encoder's backward, with P and dS in one part); everything between two tiles is kept short. Measured:
+// 2 x 4096 tokens, 16 / 4 heads x 64, causal, bfloat16: 146 us (472 TFLOP/s; issue slots 51 % busy, the tcgen05 pipe 58
+// %). 8400 tokens, 8 heads x 32 (the encoder's): forward 300 us, backward 675 (268 TFLOP/s of the products that P and
+// dS in one part would take; issue slots 55 %, the pipe 59 %). 2 x 2047, 8 / 2 heads x 128, causal, float16: forward 49
+// us, backward 125 (343 TFLOP/s; 33 and 61 %).
 #pragma once
 
 #include <type_traits>

@@ -4,9 +4,10 @@
 // ~ hi hi + hi lo + lo hi to about 22 bits. Tiles of 64 rows, four warps of 16, as mma.sync m16n8k8 fragments; the
 // other side streams through two buffers of shared memory by asynchronous copies. What bounds it: the rate of these
 // products (about 38 TFLOP/s are left of three) and, with few tiles a CTA, one warp's chain of some 1500 instructions a
-// tile. 8 heads x 32, 4 x 1100 tokens: forward 209 us (160 in one wave of four CTAs an SM with spills, but 18 instead
-// of 15 for 2 x 300), backward 493 us (three CTAs an SM; 533 with two, 626 with four); 8 heads x 64, 4096 tokens: 963
-// and 2495 us; the CUDA-core kernels take 233, 699, 1293 and 3523.
+// tile. 8 heads x 32, 4 x 1100 tokens: forward 216 us (a quarter less in one wave of four CTAs an SM with spills, but
+// 18 instead of 15 for 2 x 300), backward 527 us (three CTAs an SM; a tenth more with two, a quarter with four); 8
+// heads x 64, 4096 tokens: 980 and 2500 to 2650 us; the CUDA-core kernels take 234, 708, 1293 and 3517. The mma.sync
+// pipe is 38 % (forward) and 44 % (backward) busy, the issue slots 43 and 40 %; waits on fixed latencies come first.
 //
 // Accuracy, relative to float64 over 2 x 1100 tokens x 8 heads x 32: 3.4e-7 forward, 5e-7 backward (float32 matrix
 // products of a library: 6.4e-7). With hi cut instead of rounded and one sum over all keys it was 8.6e-6, in

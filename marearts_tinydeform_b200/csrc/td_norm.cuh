@@ -9,7 +9,7 @@
 // Bound by memory: a row is read once, into registers, and every sum over it is taken there -- the variance from the
 // centred values. Where a row's mean is more than its deviation, the centred values are summed once more, so that what
 // the first sum lost of large values does not move the row: one far from zero is normed as well as one at zero, but for
-// its mean's rounding where the backward reads it. (Every row summed so: 54.6 us for the 48.7 below.) s is not rounded
+// its mean's rounding where the backward reads it. (Every row summed so: 54.6 us for the 49.4 below.) s is not rounded
 // to the input type: both passes form it from x and residual in float32 (float64 for float64), as they do all sums.
 //
 // A group of G threads holds a row, EPT elements a thread (VEC = elements of a 16-byte vector, or 1 where C or an
@@ -17,9 +17,9 @@
 // before the present row's sums are taken (the backward, whose sums leave fewer warps an SM, has three rows ahead in
 // shared memory). The backward's column sums stay in the group's registers over all of its rows; the groups of a CTA
 // add theirs in order through shared memory, each CTA stores one float32 partial row, and norm_reduce_kernel adds those
-// in a fixed order: no atomics, the same bits every time. 177784 rows x 256 in bfloat16: forward 48.7 us (5.6 TB/s),
+// in a fixed order: no atomics, the same bits every time. 177784 rows x 256 in bfloat16: forward 49.4 us (5.5 TB/s),
 // backward with its reduction 65.7 us (5.5 TB/s; 85 with one row ahead in registers, 75 with 4 CTAs an SM instead of
-// 3); 8800 x 515 in float32, whose rows start anywhere, 13.5 and 19.5 us (4.0 and 3.7 TB/s).
+// 3); 8800 x 515 in float32, whose rows start anywhere, 14.3 and 19.6 us (3.8 and 3.7 TB/s).
 #pragma once
 
 #include "td_common.cuh"

@@ -5,11 +5,11 @@ to 16 bits from one that was not. Over a whole result the roundings add up as a 
 is the result's distance from float64, in units of the distance that rounding float64's result to the type leaves (a
 step of relative size u = finfo.eps / 2 is off by 0.29 u to 0.58 u in the mean square, as the mantissa has it).
 
-What else is allowed. A factor kept in two 16-bit parts is off by u^2. Scores and sums are float32: D <= 128 products and
-scores of a few units make 2^-19 of a probability; a tensor core cuts its running sum by up to 2^-24 for every 16 terms,
-in one direction: 2^-16 over 4200 terms. Against u = 2^-11 that is u / 32, or u / 16 with as much again for the row's
-statistics, so at most (u / 16) / (0.29 u) = 0.22 of the measure where it all adds up in line with the rounding. One
-factor rounded once to 16 bits adds about 0.4 u at random instead: sqrt(2) of the measure or nearly so."""
+What else is allowed. A factor kept in two 16-bit parts is off by u^2. Scores and sums are float32: D <= 128 products
+and scores of a few units make 2^-19 of a probability; a tensor core cuts its running sum by up to 2^-24 for every 8
+terms, in one direction: 2^-15 over 4200 terms. Against u = 2^-11 that is u / 16, so at most (u / 16) / (0.29 u) = 0.22
+of the measure where it all adds up in line with the rounding. One factor rounded once to 16 bits adds about 0.4 u at
+random instead: sqrt(2) of the measure or nearly so."""
 
 import pytest
 import torch
@@ -83,8 +83,8 @@ def test_only_the_gradients_are_rounded(cuda, dtype, shape, kind):
                                    (2, 300, 4200, 2, 2, 32)], ids=str)
 @pytest.mark.parametrize('dtype', HALVES, ids=str)
 def test_gradients_of_mixed_size(cuda, dtype, shape):
-    """A row, a head and an image whose incoming gradients are 2^12 times the others', and an image with a value 2^8 times
-    the others: the small rows' gradients are as good as if they were alone."""
+    """A row, a head and an image whose incoming gradients are 2^12 times the others', and an image with a value 2^8
+    times the others: the small rows' gradients are as good as if they were alone."""
     q, k, v, grad = inputs(shape, dtype, 44)
     B, Q, N, H, Hk, D = shape
     grad = (grad / 2).view(B, Q, H, D).clone()
@@ -122,15 +122,15 @@ def test_gradients_over_very_long_keys(cuda, dtype, shape):
 @pytest.mark.parametrize('shape', SHAPES, ids=str)
 @pytest.mark.parametrize('dtype', HALVES, ids=str)
 def test_gradients_behind_large_results(cuda, dtype, shape, kind):
-    """Values around 16 that differ by about one: what is left of dP - delta is a sixteenth of either, so that a delta from
-    rounded results, without what rounding took from them, puts the queries' gradient 20 to 120 times as far off as its
-    own rounding does.
+    """Values around 16 that differ by about one: what is left of dP - delta is a sixteenth of either, so that a delta
+    from rounded results, without what rounding took from them, puts the queries' gradient 20 to 120 times as far off as
+    its own rounding does.
 
     What is allowed follows the result's error into them. A result that is off by a relative x moves delta_i by at most
     t_i = x sum|do_i o_i|, and with it dq_i by scale t_i sum_j P_ij k_j and dk_j by scale sum_i P_ij t_i q_i. Here x is
     u^2 for the result's two parts, u^2 for those of P, and the tensor core's cuts of a sum of values that all have one
-    sign: 2^-24 of it for each of two groups of 8 in the 16 terms of a product, so N 2^-24 / 8 for one part of P (the other
-    adds u of that)."""
+    sign: 2^-24 of it for each of two groups of 8 in the 16 terms of a product, so N 2^-24 / 8 for one part of P (the
+    other adds u of that)."""
     q, k, v, grad = inputs(shape, dtype, 46)
     v = v + 16
     kw = masks(kind, shape, 46)
@@ -155,8 +155,8 @@ def test_gradients_behind_large_results(cuda, dtype, shape, kind):
 @pytest.mark.parametrize('D', (16, 32, 64, 128))
 @pytest.mark.parametrize('dtype', HALVES, ids=str)
 def test_gradients_of_few_keys(cuda, dtype, D, N, kind):
-    """Sums of few terms, where a factor rounded to 16 bits would show in each. Where one key has all the weight, what is
-    left of dP - delta is small against both and off by what test_gradients_behind_large_results counts: a few u^2 of
+    """Sums of few terms, where a factor rounded to 16 bits would show in each. Where one key has all the weight, what
+    is left of dP - delta is small against both and off by what test_gradients_behind_large_results counts: a few u^2 of
     sum|do_i v_j| for each pair, in proportion to its probability."""
     shape = (2, 150, N, 4, 2, D)
     q, k, v, grad = inputs(shape, dtype, 47)

@@ -144,7 +144,8 @@ def test_padded_keys_may_hold_anything(cuda, dtype, Q):
                                    (1, 33, 90, 2, 2, 32), (1, 5, 700, 2, 1, 64), (1, 130, 1700, 2, 1, 24)], ids=str)
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_keys_at_infinity(cuda, dtype, shape):
-    """A key whose score is minus infinity for every query has no probability: results are those of a call that pads it."""
+    """A key whose score is minus infinity for every query has no probability: results are those of a call that pads
+    it."""
     q, k, v, _ = inputs(shape, dtype, 14)
     q[..., 0] = q[..., 0].abs() + 0.25
     pad = torch.zeros((shape[0], shape[2]), dtype=torch.bool, device='cuda')

@@ -88,8 +88,8 @@ def test_rows_far_from_zero_and_constant_rows(cuda, dtype):
 @pytest.mark.parametrize('dtype, far', [(torch.float32, 1e4), (torch.float32, -3e5), (torch.float64, 1e9),
                                         (torch.float16, 1e3), (torch.bfloat16, 1e3)], ids=str)
 def test_rows_very_far_from_zero(cuda, dtype, far, C):
-    """Offsets thousands of deviations wide. Each centred value is a difference of near numbers and exact, so their sums
-    err by (C + 32) e of the centred values and not of the offset, and z by that; only the saved mean, which the backward
+    """Offsets thousands of deviations wide. Each centred value is a difference of near numbers and exact, so their
+    sums err by (C + 32) e of the centred values and not of the offset, and z by that; only the saved mean, which the backward
     subtracts, is rounded to e of the offset (e: half a step of the accumulators' type)."""
     x, w, b, _, dy = inputs(40, C, dtype, 6)
     x = (x.double() * max(1.0, abs(far) * U[dtype] * 8) + far).to(dtype)  # a few steps of the type wide at least
