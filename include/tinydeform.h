@@ -401,6 +401,71 @@ TD_API int td_layer_norm_backward(int dtype, const void* grad_y, const void* x, 
                                   size_t workspace_bytes, void* stream, char* err, size_t err_len);
 
 /*
+ * Root-mean-square norm over the last dimension of x [rows, C], the residual added inside: s = x + residual (residual
+ * NULL: x), y = s / sqrt(mean(s^2) + eps) * weight. s is not rounded before the norm; sums are float32 (float64 for
+ * TD_F64). total: NULL, or [rows, C], written with s. rstd: NULL, or [rows] in float32 (float64), written for the
+ * backward. q: NULL, or (then y is NULL, and dtype is not TD_F64) the result in 8 bits as td_fp8_quantize writes it
+ * from y before its rounding: rows q_pitch = C rounded up to 16 apart, with scale [rows, ceil(C / 128)].
+ * 1 <= C <= TD_MAX_CHANNELS. No counterpart in upstream.
+ *
+ * td_rms_norm_backward: from grad_y and grad_total (NULL: none), grad_x [rows, C] (the gradient of x and of residual
+ * alike) and grad_weight [C] (may be NULL), the column sums in a fixed order (no atomics). workspace:
+ * td_rms_norm_workspace_bytes(dtype, rows, C) bytes, 8-byte aligned.
+ */
+TD_API int td_rms_norm_forward(int dtype, const void* x, const void* residual, const void* weight, void* y,
+                               void* total, void* q, int64_t q_pitch, float* scale, void* rstd, int64_t rows,
+                               int64_t C, double eps, void* stream, char* err, size_t err_len);
+TD_API size_t td_rms_norm_workspace_bytes(int dtype, int64_t rows, int64_t C);
+TD_API int td_rms_norm_backward(int dtype, const void* grad_y, const void* grad_total, const void* x,
+                                const void* residual, const void* weight, const void* rstd, void* grad_x,
+                                void* grad_weight, int64_t rows, int64_t C, void* workspace, size_t workspace_bytes,
+                                void* stream, char* err, size_t err_len);
+
+/*
+ * 8-bit floating point (e4m3) with a scale for each block of 128. A block's scale is 2^e, e the smallest integer
+ * >= -126 with (largest finite magnitude) * 2^-e <= 448; its values are v * 2^-e rounded to nearest, ties to even; an
+ * infinity or NaN becomes NaN. No counterpart in upstream.
+ *
+ * td_fp8_quantize: x [M, K] (TD_F32, TD_F16 or TD_BF16) into q, rows q_pitch = K rounded up to 16 bytes apart (16-byte
+ * aligned; what lies behind K is written as zeros), in blocks of 1 x 128 with scale [M, ceil(K / 128)], or, with
+ * tiles, of 128 x 128 with scale [ceil(M / 128), ceil(K / 128)].
+ * td_fp8_dequantize: out [M, K] of `dtype` = q * scale, rows of q q_pitch >= K bytes apart.
+ *
+ * td_fp8_linear: out [M, N] = activation(x weight^T + bias) on 8-bit operands: the products of each block of 128 along
+ * K are summed in float32, times the blocks' scales, which may be any float32 values whose products stay in range.
+ *   x: [M, K] of x_dtype, quantised by the call (blocks of 1 x 128), or TD_E4M3 with rows x_pitch bytes apart and
+ *   x_scale [M, ceil(K / 128)]; weight [N, K] e4m3, rows w_pitch apart, in blocks of 128 x 128 with w_scale
+ *   [ceil(N / 128), ceil(K / 128)]; bias [N] of bias_dtype or NULL; activation: enum td_activation;
+ *   out: [M, N] of out_dtype, or TD_E4M3 as td_fp8_quantize writes it (out_pitch, out_scale [M, ceil(N / 128)]).
+ *   workspace: td_fp8_linear_workspace_bytes(x_dtype, M, K, N) bytes.
+ * td_fp8_linear_backward: gradients of y = Q(x) Qw(weight)^T + bias, Q and Qw the roundings to 8 bits above, whose own
+ * derivative counts as 1. x (rows x_pitch apart) and x_scale: what td_fp8_quantize gave for the forward, the only copy
+ * of the input that is kept. weight [N, K] of dtype.
+ *   grad_x = Q(grad_out) Qw(weight); grad_weight = Qc(grad_out)^T Qc(x), Qc: blocks of 128 rows of one column;
+ *   grad_bias = sum over rows of grad_out (not rounded before). Each may be NULL. Sums are taken in a fixed order.
+ *   workspace: td_fp8_linear_backward_workspace_bytes(M, K, N, whether each is wanted) bytes.
+ * 0 <= M < 2^31, 1 <= K, N <= TD_MAX_FP8_WIDTH.
+ */
+#define TD_E4M3 4 /* a dtype of the td_fp8_* calls alone */
+#define TD_MAX_FP8_WIDTH 65536
+enum td_activation { TD_ACT_NONE = 0, TD_ACT_RELU = 1, TD_ACT_GELU = 2, TD_ACT_SILU = 3 };
+TD_API int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* scale, int64_t M, int64_t K,
+                           int tiles, void* stream, char* err, size_t err_len);
+TD_API int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* scale, void* out, int64_t M,
+                             int64_t K, int tiles, void* stream, char* err, size_t err_len);
+TD_API size_t td_fp8_linear_workspace_bytes(int x_dtype, int64_t M, int64_t K, int64_t N);
+TD_API int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_scale, const void* weight,
+                         int64_t w_pitch, const float* w_scale, int bias_dtype, const void* bias, int activation,
+                         int out_dtype, void* out, int64_t out_pitch, float* out_scale, int64_t M, int64_t K,
+                         int64_t N, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
+TD_API size_t td_fp8_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int want_input, int want_weight,
+                                                     int want_bias);
+TD_API int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64_t x_pitch,
+                                  const float* x_scale, const void* weight, void* grad_x, void* grad_weight,
+                                  void* grad_bias, int64_t M, int64_t K, int64_t N, void* workspace,
+                                  size_t workspace_bytes, void* stream, char* err, size_t err_len);
+
+/*
  * Kernel policy for every later call in this process: TD_POLICY_BEST (default) uses the tcgen05 tensor-core
  * kernels wherever the shapes allow; TD_POLICY_CUDA_CORES keeps every call on the CUDA-core kernels (parity tests
  * run both). No counterpart in upstream, which has only CUDA-core kernels. Returns the previous policy.

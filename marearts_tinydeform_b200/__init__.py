@@ -26,6 +26,13 @@ The rest of a decoder layer's attention half, forward and backward:
     attention(query, key, value, key_padding_mask, attn_mask, causal, scale)   -> [B, Q, H * D]
     layer_norm(x, weight, bias, residual, eps)                                -> x's shape
 
+and its feed-forward half, with products in 8-bit floating point (e4m3, a scale for each block of 128), forward and
+backward:
+
+    rms_norm(x, weight, residual, eps, return_sum, quantize)                   -> x's shape, or 8-bit (data, scale)
+    linear_fp8(x, weight, bias, activation, quantize, dtype)                   -> [..., N], or 8-bit (data, scale)
+    quantize_fp8(x), quantize_weight_fp8(weight), dequantize_fp8(data, scale, dtype)
+
 the self attention among the queries, and the norm over a sublayer's result plus its residual.
 
 CPU tensors run ``ma_deform_attn_reference`` (as upstream does). CUDA tensors run only the native library; if it is
@@ -39,13 +46,18 @@ import functools
 import torch
 
 from . import _native
-from .autograd import AttentionFunction, LayerNormFunction, linear_train, ma_deform_attn_train, producer_train
-from .reference import (attention_reference, deform_attn_layer_reference, layer_norm_reference,
-                        ma_deform_attn_reference, sampling_producer_reference)
+from .autograd import (AttentionFunction, LayerNormFunction, LinearFp8Function, RmsNormFunction, linear_train,
+                       ma_deform_attn_train, producer_train)
+from .reference import (attention_reference, deform_attn_layer_reference, dequantize_fp8_reference,
+                        layer_norm_reference, linear_fp8_reference, ma_deform_attn_reference,
+                        quantize_fp8_reference, quantize_weight_fp8_reference, rms_norm_reference,
+                        sampling_producer_reference)
 
 __all__ = ['ma_deform_attn', 'ma_deform_attn_reference', 'choose_mode', 'deform_attn_layer', 'sampling_producer',
            'pack_sampling_weights', 'deform_attn_layer_reference', 'sampling_producer_reference', 'attention',
-           'attention_reference', 'layer_norm', 'layer_norm_reference']
+           'attention_reference', 'layer_norm', 'layer_norm_reference', 'rms_norm', 'rms_norm_reference',
+           'linear_fp8', 'linear_fp8_reference', 'quantize_fp8', 'quantize_fp8_reference', 'quantize_weight_fp8',
+           'quantize_weight_fp8_reference', 'dequantize_fp8', 'dequantize_fp8_reference']
 __version__ = '0.1.1+b200'
 
 MODES = ('auto', 'fused', 'project')
@@ -298,3 +310,95 @@ def layer_norm(x, weight, bias=None, residual=None, eps=1e-5):
     if _wants_grad(x, weight, bias, residual):
         return LayerNormFunction.apply(x, weight, bias, residual, float(eps))
     return _native.layer_norm_forward(x, weight, bias, residual, float(eps))[0]
+
+
+def rms_norm(x, weight, residual=None, eps=1e-6, return_sum=False, quantize=False):
+    """Root-mean-square norm of s = x + residual over the last dimension (up to 8192 wide): s / sqrt(mean(s^2) + eps)
+    * weight, in x's shape and dtype.
+
+    weight and residual have x's dtype and device. s is not rounded before the norm, and the mean is float32 (float64
+    for float64). return_sum: the pair (result, s), s being what the next layer adds to. quantize: the result in 8 bits,
+    as a pair (data, scale) like quantize_fp8's, rounded once; for calls without gradients, not for float64. CUDA
+    tensors run this library's kernels, forward and backward (the weight's gradient summed in a fixed order); CPU
+    tensors run rms_norm_reference.
+    """
+    _native.check_rms_norm(x, weight, residual, eps, quantize)
+    grad = _wants_grad(x, weight, residual)
+    if grad and quantize:
+        raise RuntimeError('an 8-bit result has no gradient: leave quantize off, or run under torch.no_grad()')
+    if not x.is_cuda:
+        return rms_norm_reference(x, weight, residual, eps, return_sum, quantize)
+    _native.load()
+    if grad:
+        return RmsNormFunction.apply(x, weight, residual, float(eps), bool(return_sum))
+    y, total, _ = _native.rms_norm_forward(x, weight, residual, float(eps), return_sum, quantize)
+    return (y, total) if return_sum else y
+
+
+def quantize_fp8(x):
+    """x [..., K] in 8 bits (e4m3), a scale for each 128 values along the last dimension: the pair (data, scale) of
+    float8_e4m3fn [..., K] and float32 [..., ceil(K / 128)]; x is about data * scale.
+
+    x: float32, float16 or bfloat16, up to 65536 wide. Scales are powers of two, the smallest that bring a block's
+    largest finite magnitude to at most 448 (e4m3's largest); values are rounded to nearest, ties to even; infinities
+    and NaN become NaN. data's rows start 16 bytes apart or a multiple of that, so it is a view where K is not one.
+    """
+    _native.check_fp8_source(x)
+    x = x.detach()
+    return _native.fp8_quantize(x) if x.is_cuda else quantize_fp8_reference(x)
+
+
+def quantize_weight_fp8(weight):
+    """A weight [N, K] in 8 bits as linear_fp8 takes it, to be laid out once: (data, scale) as quantize_fp8's, with a
+    scale for each block of 128 x 128, float32 [ceil(N / 128), ceil(K / 128)]."""
+    _native.check_fp8_source(weight, 'weight')
+    if weight.dim() != 2 or not 1 <= weight.shape[0] <= _native.MAX_FP8_WIDTH:
+        raise RuntimeError(f'weight must be [N, K], both between 1 and {_native.MAX_FP8_WIDTH}')
+    weight = weight.detach()
+    return _native.fp8_quantize(weight, tiles=True) if weight.is_cuda else quantize_weight_fp8_reference(weight)
+
+
+def dequantize_fp8(data, scale, dtype):
+    """data * scale in `dtype` (float32, float16 or bfloat16): what quantize_fp8's pair, or quantize_weight_fp8's, stands
+    for. bfloat16 and float32 hold the values of this package's own pairs exactly."""
+    tiles = isinstance(data, torch.Tensor) and isinstance(scale, torch.Tensor) and data.dim() == 2 and \
+        scale.dim() == 2 and scale.shape[0] != data.shape[0]
+    _native.check_fp8_pair((data, scale), 'the input', tiles)
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise RuntimeError('dtype must be float32, float16 or bfloat16')
+    if not data.is_cuda:
+        return dequantize_fp8_reference(data, scale, dtype)
+    return _native.fp8_dequantize(data, scale, dtype, tiles)
+
+
+def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None):
+    """activation(x @ weight.T + bias) with both operands in 8 bits (e4m3), over the last dimension of x; [..., N].
+
+    x: float32, float16 or bfloat16 [..., K] (quantised by the call as quantize_fp8 does), or a pair (data, scale).
+    weight: a pair from quantize_weight_fp8 (or any other such pair: scales may be any float32 numbers, as long as the
+    product of a scale of x and one of weight is one too), or a floating [N, K] of x's dtype, laid out by the call.
+    bias: [N], floating. activation: None, 'relu', 'gelu' (with erf) or 'silu'. dtype: the result's, x's unless given
+    (needed where x is a pair). quantize: the result in 8 bits instead, a pair that the next product takes. The
+    products of a block are summed in float32, then scaled, and the result is rounded once.
+
+    Training: where x (floating), weight (floating) or bias requires grad, the backward runs too, with the input kept
+    for it only in 8 bits; no activation, quantize or other dtype then. With Q the roundings to 8 bits, whose own
+    derivative counts as 1: grad_x = Q(g) Q(weight), grad_weight = Q(g)^T Q(Q(x)), the last two in blocks of 128 rows,
+    grad_bias = the sum of g. Sums are taken in a fixed order. CUDA tensors run this library's kernels; CPU tensors
+    linear_fp8_reference.
+    """
+    tensors = [t for t in (x, weight, bias) if isinstance(t, torch.Tensor)]
+    grad = _wants_grad(*tensors)
+    dtype = _native.check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad)
+    cuda = (x if isinstance(x, torch.Tensor) else x[0]).is_cuda
+    if cuda:
+        _native.load()
+    if grad:
+        return LinearFp8Function.apply(x, weight, bias)
+    if isinstance(weight, torch.Tensor):
+        weight = quantize_weight_fp8(weight)
+    if cuda:
+        return _native.linear_fp8_forward(x, weight, bias, activation, quantize, dtype)
+    if isinstance(x, torch.Tensor):
+        x = quantize_fp8_reference(x)
+    return linear_fp8_reference(x, weight, bias, activation, quantize, dtype)

@@ -16,11 +16,14 @@ import torch
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, '_tinydeform.so')
 
-TD_F32, TD_F16, TD_BF16, TD_F64 = 0, 1, 2, 3
+TD_F32, TD_F16, TD_BF16, TD_F64, TD_E4M3 = 0, 1, 2, 3, 4
 DTYPE_CODE = {torch.float32: TD_F32, torch.float16: TD_F16, torch.bfloat16: TD_BF16, torch.float64: TD_F64}
 MAX_LEVEL_POINTS = 64
 MAX_CHANNELS = 8192
 MAX_HEAD_DIM = 128
+MAX_FP8_WIDTH = 65536
+FP8_BLOCK = 128  # values that share a scale, along an axis
+ACTIVATION_CODE = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
 ATTN_ROW_PAD = 128  # rows of the attention's lse hold Q rounded up to this
 INT32_MAX = 2 ** 31 - 1
 
@@ -37,6 +40,18 @@ SIGNATURES = {
     'td_layer_norm_workspace_bytes': (_sz, [_ip, _i64, _i64]),
     'td_layer_norm_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp, _cp,
                                      _sz]),
+    'td_rms_norm_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, ctypes.c_double, _vp,
+                                  _cp, _sz]),
+    'td_rms_norm_workspace_bytes': (_sz, [_ip, _i64, _i64]),
+    'td_rms_norm_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp, _cp, _sz]),
+    'td_fp8_quantize': (_ip, [_ip, _vp, _vp, _i64, _vp, _i64, _i64, _ip, _vp, _cp, _sz]),
+    'td_fp8_dequantize': (_ip, [_ip, _vp, _i64, _vp, _vp, _i64, _i64, _ip, _vp, _cp, _sz]),
+    'td_fp8_linear_workspace_bytes': (_sz, [_ip, _i64, _i64, _i64]),
+    'td_fp8_linear': (_ip, [_ip, _vp, _i64, _vp, _vp, _i64, _vp, _ip, _vp, _ip, _ip, _vp, _i64, _vp, _i64, _i64, _i64,
+                            _vp, _sz, _vp, _cp, _sz]),
+    'td_fp8_linear_backward_workspace_bytes': (_sz, [_i64, _i64, _i64, _ip, _ip, _ip]),
+    'td_fp8_linear_backward': (_ip, [_ip, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp,
+                                     _cp, _sz]),
     'td_fused_forward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
                                _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _vp, _cp, _sz]),
     'td_sample_forward': (_ip, [_ip, _vp, _i64, _vp, _vp, _vp, _vp, _vp,
@@ -946,4 +961,268 @@ def layer_norm_backward(grad_y, x, weight, residual, stats, want_weight=True, wa
     _launch(lib.td_layer_norm_backward, x.device, code, g.data_ptr(), xs.data_ptr(), _address(r), w.data_ptr(), mean,
             mean + rows * (8 if code == TD_F64 else 4), grad_x.data_ptr(), _address(grad_w), _address(grad_b), rows, C,
             ws.data_ptr(), ws_bytes)
+    return grad_x, grad_w, grad_b
+
+
+# ---- root-mean-square norm and products in 8-bit floating point ------------------------------------------------------
+
+FP8 = torch.float8_e4m3fn
+_FP8_SOURCES = (torch.float32, torch.float16, torch.bfloat16)
+
+
+def check_rms_norm(x, weight, residual, eps, quantize):
+    """The root-mean-square norm's argument contract, on any device."""
+    check_layer_norm(x, weight, None, residual, eps)
+    if quantize and x.dtype not in _FP8_SOURCES:
+        raise RuntimeError('an 8-bit result needs float32, float16 or bfloat16 inputs')
+
+
+def _fp8_empty(like, lead, width):
+    """Uninitialised 8-bit rows and their scales: data [*lead, width] with rows a multiple of 16 bytes apart, that
+    distance, and scale [*lead, ceil(width / 128)]."""
+    pitch = -(-width // 16) * 16
+    data = like.new_empty((*lead, pitch), dtype=FP8)
+    scale = like.new_empty((*lead, -(-width // FP8_BLOCK)), dtype=torch.float32)
+    return data if pitch == width else data[..., :width], pitch, scale
+
+
+def rms_norm_forward(x, weight, residual, eps, return_sum, quantize, want_rstd=False):
+    """(y, sum or None, rstd or None) through td_rms_norm_forward, for arguments check_rms_norm has passed; y is a pair
+    (data, scale) with quantize."""
+    lib = load()
+    if not x.is_cuda:
+        raise RuntimeError('inputs must be CUDA tensors')
+    xs, w, r = _dense(x, weight, residual)
+    C = x.shape[-1]
+    rows = xs.numel() // C
+    code = DTYPE_CODE[x.dtype]
+    total = torch.empty_like(xs) if return_sum else None
+    rstd = xs.new_empty((rows,), dtype=torch.float64 if code == TD_F64 else torch.float32) if want_rstd else None
+    if quantize:
+        data, pitch, scale = _fp8_empty(xs, xs.shape[:-1], C)
+        y, out, q, sc = (data, scale), None, data.data_ptr(), scale.data_ptr()
+    else:
+        y = torch.empty_like(xs)
+        out, q, pitch, sc = y.data_ptr(), None, 0, None
+    if rows:
+        _launch(lib.td_rms_norm_forward, x.device, code, xs.data_ptr(), _address(r), w.data_ptr(), out,
+                _address(total), q, pitch, sc, _address(rstd), rows, C, eps)
+    return y, total, rstd
+
+
+@functools.lru_cache(maxsize=1024)
+def _rms_norm_workspace(*sizes):
+    """td_rms_norm_workspace_bytes (a function of the sizes alone)."""
+    return load().td_rms_norm_workspace_bytes(*sizes)
+
+
+def rms_norm_backward(grad_y, grad_sum, x, weight, residual, rstd, want_weight=True):
+    """(grad_x, grad_weight or None) through td_rms_norm_backward; grad_sum may be None."""
+    lib = load()
+    g, gs, xs, w, r = _dense(grad_y, grad_sum, x, weight, residual)
+    C = x.shape[-1]
+    rows = xs.numel() // C
+    code = DTYPE_CODE[x.dtype]
+    grad_x = torch.empty_like(xs)
+    grad_w = w.new_empty((C,)) if want_weight else None
+    ws_bytes = _rms_norm_workspace(code, rows, C)
+    ws = w.new_empty((max(ws_bytes, 1),), dtype=torch.uint8)
+    _launch(lib.td_rms_norm_backward, x.device, code, g.data_ptr(), _address(gs), xs.data_ptr(), _address(r),
+            w.data_ptr(), rstd.data_ptr(), grad_x.data_ptr(), _address(grad_w), rows, C, ws.data_ptr(), ws_bytes)
+    return grad_x, grad_w
+
+
+def check_fp8_source(x, what='x'):
+    """A tensor that can be quantised: float32, float16 or bfloat16, its last dimension 1 to MAX_FP8_WIDTH wide."""
+    if x.dim() < 1:
+        raise RuntimeError(f'{what} must have at least one dimension')
+    if x.dtype not in _FP8_SOURCES:
+        raise RuntimeError(f'{what} must be float32, float16 or bfloat16, not {x.dtype}')
+    if not 1 <= x.shape[-1] <= MAX_FP8_WIDTH:
+        raise RuntimeError(f'the last dimension of {what} must be between 1 and {MAX_FP8_WIDTH}')
+
+
+def check_fp8_pair(pair, what, tiles):
+    """A pair (data, scale): e4m3 data [..., K] with float32 scales [..., ceil(K / 128)], or, with tiles, data [N, K]
+    with scales [ceil(N / 128), ceil(K / 128)]. Returns it."""
+    if not (isinstance(pair, (tuple, list)) and len(pair) == 2 and all(isinstance(t, torch.Tensor) for t in pair)):
+        raise RuntimeError(f'{what} must be a tensor, or a pair (data, scale) of tensors')
+    data, scale = pair
+    if data.dtype != FP8 or scale.dtype != torch.float32:
+        raise RuntimeError(f'{what} in 8 bits must be float8_e4m3fn data with float32 scales')
+    if data.device != scale.device:
+        raise RuntimeError(f'data and scale of {what} must be on the same device')
+    if data.dim() < (2 if tiles else 1) or (tiles and data.dim() != 2):
+        raise RuntimeError(f'data of {what} must be [N, K]' if tiles else f'{what} must have at least one dimension')
+    if not 1 <= data.shape[-1] <= MAX_FP8_WIDTH or (tiles and not 1 <= data.shape[0] <= MAX_FP8_WIDTH):
+        raise RuntimeError(f'widths of {what} must be between 1 and {MAX_FP8_WIDTH}')
+    want = tuple(data.shape[:-1]) + (-(-data.shape[-1] // FP8_BLOCK),)
+    if tiles:
+        want = (-(-data.shape[0] // FP8_BLOCK), want[1])
+    if tuple(scale.shape) != want:
+        raise RuntimeError(f'the scales of {what} must be of shape {list(want)}, not {list(scale.shape)}')
+    return data, scale
+
+
+def _fp8_rows(data):
+    """8-bit data [..., K] as rows an equal number of bytes apart, starting on 16-byte boundaries (a copy where they are
+    not), and that distance."""
+    K = data.shape[-1]
+    pitch, span = None, None
+    good = data.stride(-1) == 1 or K == 1
+    for size, stride in zip(reversed(data.shape[:-1]), reversed(data.stride()[:-1])):
+        if size == 1:
+            continue
+        if pitch is None:
+            pitch, span = stride, stride
+        good = good and stride == span
+        span *= size
+    if pitch is None:
+        pitch = -(-K // 16) * 16
+    if good and pitch >= K and pitch % 16 == 0 and data.data_ptr() % 16 == 0:
+        return data, pitch
+    pitch = -(-K // 16) * 16
+    rows = data.new_zeros((*data.shape[:-1], pitch), dtype=torch.uint8)
+    rows[..., :K] = data.view(torch.uint8)
+    return rows, pitch
+
+
+def _fp8_weight(pair):
+    data, scale = pair
+    data, pitch = _fp8_rows(data)
+    return data, pitch, scale if scale.is_contiguous() else scale.contiguous()
+
+
+def fp8_quantize(x, tiles=False):
+    """(data, scale) through td_fp8_quantize: x [..., K] in blocks of 1 x 128, or, with tiles, x [N, K] in blocks of
+    128 x 128."""
+    lib = load()
+    if not x.is_cuda:
+        raise RuntimeError('inputs must be CUDA tensors')
+    xs = x.contiguous()
+    K = x.shape[-1]
+    M = xs.numel() // K
+    data, pitch, scale = _fp8_empty(xs, xs.shape[:-1], K)
+    if tiles:
+        scale = xs.new_empty((-(-M // FP8_BLOCK), -(-K // FP8_BLOCK)), dtype=torch.float32)
+    if M:
+        _launch(lib.td_fp8_quantize, x.device, DTYPE_CODE[x.dtype], xs.data_ptr(), data.data_ptr(), pitch,
+                scale.data_ptr(), M, K, tiles)
+    return data, scale
+
+
+def fp8_dequantize(data, scale, dtype, tiles):
+    """data * scale in `dtype` through td_fp8_dequantize."""
+    lib = load()
+    if not data.is_cuda:
+        raise RuntimeError('inputs must be CUDA tensors')
+    q, pitch = _fp8_rows(data)
+    sc = scale.contiguous()
+    K = data.shape[-1]
+    out = data.new_empty(data.shape, dtype=dtype)
+    M = out.numel() // K
+    if M:
+        _launch(lib.td_fp8_dequantize, data.device, DTYPE_CODE[dtype], q.data_ptr(), pitch, sc.data_ptr(),
+                out.data_ptr(), M, K, tiles)
+    return out
+
+
+def check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad):
+    """The 8-bit product's argument contract, on any device; x and weight are tensors or pairs. Returns the output's
+    dtype. grad: gradients are wanted."""
+    x_pair, w_pair = not isinstance(x, torch.Tensor), not isinstance(weight, torch.Tensor)
+    if x_pair:
+        check_fp8_pair(x, 'x', tiles=False)
+    else:
+        check_fp8_source(x)
+    if w_pair:
+        check_fp8_pair(weight, 'weight', tiles=True)
+    else:
+        check_fp8_source(weight, 'weight')
+        if weight.dim() != 2 or not 1 <= weight.shape[0] <= MAX_FP8_WIDTH:
+            raise RuntimeError(f'weight must be [N, K], both between 1 and {MAX_FP8_WIDTH}')
+    data, wide = (x[0] if x_pair else x), (weight[0] if w_pair else weight)
+    if wide.shape[1] != data.shape[-1]:
+        raise RuntimeError('weight must be [N, K] with K = the last dimension of x')
+    if data.numel() // data.shape[-1] > INT32_MAX:
+        raise RuntimeError('too many rows')
+    if not x_pair and not w_pair and x.dtype != weight.dtype:
+        raise RuntimeError('a floating weight must have the dtype of x')
+    if bias is not None and (bias.shape != (wide.shape[0],) or bias.dtype not in _FP8_SOURCES):
+        raise RuntimeError('bias must be [N], float32, float16 or bfloat16')
+    for t in (wide, bias):
+        if t is not None and t.device != data.device:
+            raise RuntimeError('x, weight and bias must be on the same device')
+    if activation not in ACTIVATION_CODE:
+        raise ValueError(f'activation must be one of {tuple(ACTIVATION_CODE)}, got {activation!r}')
+    if quantize and dtype is not None:
+        raise RuntimeError('an 8-bit result has no dtype to choose')
+    if dtype is not None and dtype not in _FP8_SOURCES:
+        raise RuntimeError('dtype must be float32, float16 or bfloat16')
+    if dtype is None and not quantize:
+        if x_pair:
+            raise RuntimeError('x in 8 bits needs the dtype of the result (or quantize)')
+        dtype = x.dtype
+    if grad:
+        if x_pair or w_pair:
+            raise RuntimeError('gradients need x and weight in a floating dtype: what is in 8 bits has none')
+        if activation is not None or quantize or dtype != x.dtype:
+            raise RuntimeError('gradients go through the plain product: no activation, quantize or other dtype')
+        if bias is not None and bias.dtype != x.dtype:
+            raise RuntimeError('for gradients the bias must have the dtype of x')
+    return dtype
+
+
+def linear_fp8_forward(x, weight, bias, activation, quantize, dtype):
+    """td_fp8_linear for arguments check_linear_fp8 has passed; x may be a pair, weight is one."""
+    lib = load()
+    w, w_pitch, w_scale = _fp8_weight(weight)
+    if isinstance(x, torch.Tensor):
+        data, x_scale, x_pitch, code = x.contiguous(), None, 0, DTYPE_CODE[x.dtype]
+        shape = x.shape
+    else:
+        shape, code = x[0].shape, TD_E4M3
+        data, x_pitch = _fp8_rows(x[0])
+        x_scale = x[1].contiguous()
+    if not data.is_cuda:
+        raise RuntimeError('inputs must be CUDA tensors')
+    K, N = shape[-1], weight[0].shape[0]
+    lead = tuple(shape[:-1])
+    M = 1
+    for n in lead:
+        M *= n
+    b = None if bias is None else bias.contiguous()
+    if quantize:
+        out, out_pitch, out_scale = _fp8_empty(data, lead, N)
+        result, out_code = (out, out_scale), TD_E4M3
+    else:
+        out = result = data.new_empty((*lead, N), dtype=dtype)
+        out_pitch, out_scale, out_code = 0, None, DTYPE_CODE[dtype]
+    if M:
+        ws_bytes = lib.td_fp8_linear_workspace_bytes(code, M, K, N)
+        ws = data.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+        _launch(lib.td_fp8_linear, data.device, code, data.data_ptr(), x_pitch, _address(x_scale), w.data_ptr(),
+                w_pitch, w_scale.data_ptr(), 0 if b is None else DTYPE_CODE[b.dtype], _address(b),
+                ACTIVATION_CODE[activation], out_code, out.data_ptr(), out_pitch, _address(out_scale), M, K, N,
+                _address(ws), ws_bytes)
+    return result
+
+
+def linear_fp8_backward(grad_out, x8, weight, want_x, want_w, want_b):
+    """(grad_x, grad_weight, grad_bias), None where not wanted, through td_fp8_linear_backward; x8: the pair that the
+    forward's input was quantised to."""
+    lib = load()
+    g, w = _dense(grad_out, weight)
+    data, pitch = _fp8_rows(x8[0])
+    scale = x8[1]
+    N, K = weight.shape
+    M = g.numel() // N
+    grad_x = g.new_empty((*g.shape[:-1], K)) if want_x else None
+    grad_w = g.new_empty((N, K)) if want_w else None
+    grad_b = g.new_empty((N,)) if want_b else None
+    ws_bytes = lib.td_fp8_linear_backward_workspace_bytes(M, K, N, want_x, want_w, want_b)
+    ws = g.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
+    _launch(lib.td_fp8_linear_backward, g.device, DTYPE_CODE[g.dtype], g.data_ptr(), data.data_ptr(), pitch,
+            scale.data_ptr(), w.data_ptr(), _address(grad_x), _address(grad_w), _address(grad_b), M, K, N,
+            _address(ws), ws_bytes)
     return grad_x, grad_w, grad_b

@@ -28,7 +28,7 @@ layer: the self attention among the queries, and the norm behind each attention.
 import torch
 from torch.autograd.function import once_differentiable
 
-from . import _native
+from . import _native, reference
 
 
 class MaDeformAttnFunction(torch.autograd.Function):
@@ -152,8 +152,8 @@ def _first_order(backward):
     """once_differentiable, whose own bookkeeping is left out of an ordinary backward (one without create_graph)."""
     guarded = once_differentiable(backward)
 
-    def run(ctx, grad):
-        return guarded(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
 
     return run
 
@@ -202,3 +202,53 @@ class LayerNormFunction(torch.autograd.Function):
         g = grad_y if grad_y.dtype == x.dtype else grad_y.to(x.dtype)
         grad_x, grad_w, grad_b = _native.layer_norm_backward(g, x, weight, residual, stats, need[1], need[2])
         return (grad_x if need[0] else None, grad_w, grad_b, grad_x if need[3] else None, None)
+
+
+class RmsNormFunction(torch.autograd.Function):
+    """Root-mean-square norm with the residual added inside on CUDA, differentiable in x, weight and residual, with the
+    sum as a second output if asked: td_rms_norm_forward, which also writes each row's reciprocal norm, and
+    td_rms_norm_backward. x and residual have the same gradient; where both need it they get the same tensor."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps, return_sum):
+        y, total, rstd = _native.rms_norm_forward(x, weight, residual, eps, return_sum, False, want_rstd=True)
+        ctx.save_for_backward(x, weight, residual, rstd)
+        ctx.set_materialize_grads(False)
+        return (y, total) if return_sum else y
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, grad_y, grad_sum=None):
+        x, weight, residual, rstd = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if grad_y is None and grad_sum is None:
+            return None, None, None, None, None
+        if grad_y is None:  # the sum alone was used
+            grad_x = grad_sum.to(x.dtype)
+            return grad_x if need[0] else None, None, grad_x if need[2] else None, None, None
+        g, gs = (None if t is None else t.to(x.dtype) for t in (grad_y, grad_sum))
+        grad_x, grad_w = _native.rms_norm_backward(g, gs, x, weight, residual, rstd, need[1])
+        return grad_x if need[0] else None, grad_w, grad_x if need[2] else None, None, None
+
+
+class LinearFp8Function(torch.autograd.Function):
+    """The 8-bit product, differentiable in x, weight and bias, on CUDA and (with torch operators) on the CPU. The
+    input is kept as its 8-bit copy alone; the weight, which the caller keeps anyway, is laid out again."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        if x.is_cuda:
+            x8, w8 = _native.fp8_quantize(x), _native.fp8_quantize(weight, tiles=True)
+            y = _native.linear_fp8_forward(x8, w8, bias, None, False, x.dtype)
+        else:
+            x8, w8 = reference.quantize_fp8_reference(x), reference.quantize_weight_fp8_reference(weight)
+            y = reference.linear_fp8_reference(x8, w8, bias, dtype=x.dtype)
+        ctx.save_for_backward(*x8, weight)
+        return y
+
+    @staticmethod
+    @_first_order
+    def backward(ctx, grad_y):
+        data, scale, weight = ctx.saved_tensors
+        run = _native.linear_fp8_backward if data.is_cuda else reference.linear_fp8_backward_reference
+        return run(grad_y.to(weight.dtype), (data, scale), weight, *ctx.needs_input_grad)

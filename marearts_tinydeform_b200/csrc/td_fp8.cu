@@ -1,0 +1,374 @@
+// td_fp8.cu -- the 8-bit entry points of the C ABI (quantising, products, their backward): argument contract, kernel
+// choice, workspaces and launches.
+#include <algorithm>
+#include <type_traits>
+
+#include "td_fp8.cuh"
+#include "td_fp8_simt.cuh"
+#include "td_host.h"
+
+namespace td {
+
+cudaError_t fp8_device_error(int clear, unsigned int* code) {
+    cudaError_t e = cudaMemcpyFromSymbol(code, g_device_error, sizeof(*code));
+    if (e == cudaSuccess && clear) {
+        const unsigned int zero = 0;
+        e = cudaMemcpyToSymbol(g_device_error, &zero, sizeof(zero));
+    }
+    return e;
+}
+
+namespace {
+
+using host::fail;
+
+bool aligned(const void* p, uintptr_t n) { return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0; }
+int64_t up(int64_t v, int64_t n) { return (v + n - 1) / n * n; }
+int64_t blocks_of(int64_t v) { return (v + kBlock8 - 1) / kBlock8; }
+bool wide_type(int dtype) { return dtype >= TD_F32 && dtype <= TD_BF16; }
+size_t type_bytes(int dtype) { return dtype == TD_F32 ? 4 : dtype == TD_E4M3 ? 1 : 2; }
+
+// Calls f with a value of the C++ type of a floating dtype.
+template <typename F>
+int by_type(int dtype, F f) {
+    switch (dtype) {
+        case TD_F32: return f(float());
+        case TD_F16: return f(__half());
+        default: return f(__nv_bfloat16());
+    }
+}
+
+int check_sizes(int64_t M, int64_t K, int64_t N, char* err, size_t err_len) {
+    if (M < 0 || M > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "rows must be between 0 and 2^31 - 1");
+    if (K < 1 || K > TD_MAX_FP8_WIDTH || N < 1 || N > TD_MAX_FP8_WIDTH)
+        return fail(err, err_len, TD_ERR_ARG, "widths must be between 1 and %d", TD_MAX_FP8_WIDTH);
+    return TD_OK;
+}
+
+// 8-bit rows that this library writes: 16-byte aligned, `width` rounded up to 16 apart.
+int check_written(const void* q, int64_t pitch, int64_t width, const float* scale, char* err, size_t err_len) {
+    if (q == nullptr || scale == nullptr) return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
+    if (pitch != up(width, 16) || !aligned(q, 16))
+        return fail(err, err_len, TD_ERR_ARG, "8-bit rows must be 16-byte aligned, their width rounded up to 16 apart");
+    return TD_OK;
+}
+
+// A workspace handed out in 256-byte steps from its first 256-byte boundary; with a null base it only counts.
+struct Cut {
+    uintptr_t at;
+    size_t used = 0;
+    explicit Cut(void* base) : at((reinterpret_cast<uintptr_t>(base) + 255) & ~uintptr_t(255)) {}
+    template <typename T>
+    T* take(int64_t count) {
+        T* p = reinterpret_cast<T*>(at + used);
+        used += size_t(up(count * int64_t(sizeof(T)), 256));
+        return p;
+    }
+    size_t bytes() const { return used + 256; }
+};
+
+// ---- quantising -------------------------------------------------------------------------------------------------
+
+int launch_rows(int dtype, const void* x, uint8_t* q, int64_t pitch, float* scale, int64_t M, int64_t K,
+                cudaStream_t stream, char* err, size_t err_len) {
+    RowsArgs a = {x, q, scale, M, int(K), int(blocks_of(K)), int(pitch)};
+    return by_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        constexpr int V = Elem<T>::kVec;
+        const bool wide = K % V == 0 && aligned(x, 16);
+        const int64_t tasks = M * ((K + 32 * (wide ? V : 4) - 1) / (32 * (wide ? V : 4)));
+        const dim3 grid(unsigned(std::min<int64_t>((tasks + 7) / 8, int64_t(kSms) * 8)));
+        return wide ? host::launch(err, err_len, "fp8_rows_kernel", fp8_rows_kernel<T, true>, grid, dim3(kRowsThreads),
+                                   0, stream, true, a)
+                    : host::launch(err, err_len, "fp8_rows_kernel", fp8_rows_kernel<T, false>, grid,
+                                   dim3(kRowsThreads), 0, stream, true, a);
+    });
+}
+
+template <typename T, bool TILE>
+int launch_tiles_of(const TileArgs& a, cudaStream_t stream, char* err, size_t err_len) {
+    const bool wide = a.C % 8 == 0 && aligned(a.x, sizeof(T) == 1 ? 8 : 16) && a.ld * int64_t(sizeof(T)) % 8 == 0 &&
+                      (sizeof(T) == 1 || a.ld * int64_t(sizeof(T)) % 16 == 0);
+    const unsigned y = unsigned(std::min<int64_t>(a.MB, 65535));
+    const dim3 grid(unsigned(a.CB), y, unsigned((a.MB + y - 1) / y));
+    return wide ? host::launch(err, err_len, "fp8_tile_kernel", fp8_tile_kernel<T, true, TILE>, grid,
+                               dim3(kTileThreads), 0, stream, true, a)
+                : host::launch(err, err_len, "fp8_tile_kernel", fp8_tile_kernel<T, false, TILE>, grid,
+                               dim3(kTileThreads), 0, stream, true, a);
+}
+
+int launch_tiles(int dtype, const TileArgs& a, bool tile, cudaStream_t stream, char* err, size_t err_len) {
+    if (dtype == TD_E4M3) return launch_tiles_of<E4m3, false>(a, stream, err, err_len);
+    return by_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        return tile ? launch_tiles_of<T, true>(a, stream, err, err_len)
+                    : launch_tiles_of<T, false>(a, stream, err, err_len);
+    });
+}
+
+// ---- products ---------------------------------------------------------------------------------------------------
+
+int launch_simt(const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M, int64_t N, int64_t K,
+                cudaStream_t stream, char* err, size_t err_len) {
+    const int64_t tiles = (M + kSimtRows8 - 1) / kSimtRows8 * blocks_of(N);
+    if (tiles > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "too many output tiles");
+    auto go = [&](auto zero) {
+        return host::launch(err, err_len, "fp8_product_simt_kernel", fp8_product_simt_kernel<decltype(zero)>,
+                            dim3(unsigned(tiles)), dim3(kSimtThreads8), 0, stream, true, a, b, end,
+                            static_cast<long long>(M), int(N), int(K));
+    };
+    return out_dtype == TD_E4M3 ? go(E4m3()) : by_type(out_dtype, go);
+}
+
+int launch_product(const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M, int64_t N,
+                   int64_t K, cudaStream_t stream, char* err, size_t err_len) {
+    return launch_simt(a, b, end, out_dtype, M, N, K, stream, err, err_len);
+}
+
+// What a forward call keeps in its workspace: the input in 8 bits, where it comes wider.
+struct LinearPlan {
+    uint8_t* q;
+    float* scale;
+    size_t bytes;
+};
+
+LinearPlan plan_linear(int x_dtype, int64_t M, int64_t K, int64_t N, void* workspace) {
+    LinearPlan p = {};
+    Cut cut(workspace);
+    if (x_dtype != TD_E4M3) {
+        p.q = cut.take<uint8_t>(M * up(K, 16));
+        p.scale = cut.take<float>(M * blocks_of(K));
+    }
+    p.bytes = cut.used == 0 ? 0 : cut.bytes();
+    return p;
+}
+
+// A backward call's workspace: the gradient in 1 x 128 blocks, and, transposed, in blocks of 128 rows, as is the
+// input; the transposed weight; the parts of the bias's column sums.
+struct BackwardPlan {
+    uint8_t *dy, *dyt, *xt, *wt;
+    float *dy_scale, *dyt_scale, *xt_scale, *wt_scale, *sums;
+    int64_t n_pad, k_pad;  // columns of the scales [MB, ..] of the transposed operands
+    size_t bytes;
+};
+
+BackwardPlan plan_backward(int64_t M, int64_t K, int64_t N, bool want_x, bool want_w, bool want_b, void* workspace) {
+    BackwardPlan p = {};
+    Cut cut(workspace);
+    const int64_t MB = blocks_of(M);
+    p.n_pad = up(N, 256);
+    p.k_pad = up(K, 256);
+    if (want_x) {
+        p.dy = cut.take<uint8_t>(M * up(N, 16));
+        p.dy_scale = cut.take<float>(M * blocks_of(N));
+        p.wt = cut.take<uint8_t>(K * up(N, 16));
+        p.wt_scale = cut.take<float>(blocks_of(K) * blocks_of(N));
+    }
+    if (want_w) {
+        p.dyt = cut.take<uint8_t>(N * up(M, 16));
+        p.dyt_scale = cut.take<float>(MB * p.n_pad);
+        p.xt = cut.take<uint8_t>(K * up(M, 16));
+        p.xt_scale = cut.take<float>(MB * p.k_pad);
+    }
+    if (want_b) p.sums = cut.take<float>(MB * N);
+    p.bytes = cut.bytes();
+    return p;
+}
+
+int check_workspace(const void* workspace, size_t have, size_t need, char* err, size_t err_len) {
+    if (need > 0 && (workspace == nullptr || have < need))
+        return fail(err, err_len, TD_ERR_WORKSPACE, "workspace must be of %zu bytes (got %zu)", need, have);
+    return TD_OK;
+}
+
+}  // namespace
+}  // namespace td
+
+extern "C" {
+
+int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* scale, int64_t M, int64_t K, int tiles,
+                    void* stream, char* err, size_t err_len) {
+    using namespace td;
+    if (!wide_type(dtype)) return fail(err, err_len, TD_ERR_ARG, "unsupported dtype %d", dtype);
+    if (int rc = check_sizes(M, K, 1, err, err_len)) return rc;
+    if (M == 0) return TD_OK;
+    if (x == nullptr) return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
+    if (int rc = check_written(q, q_pitch, K, scale, err, err_len)) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (!tiles) return launch_rows(dtype, x, static_cast<uint8_t*>(q), q_pitch, scale, M, K, s, err, err_len);
+    TileArgs a = {};
+    a.x = x;
+    a.ld = K;
+    a.q = static_cast<uint8_t*>(q);
+    a.scale = scale;
+    a.M = M;
+    a.q_pitch = q_pitch;
+    a.C = int(K);
+    a.CB = int(blocks_of(K));
+    a.MB = int(blocks_of(M));
+    return launch_tiles(dtype, a, true, s, err, err_len);
+}
+
+int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* scale, void* out, int64_t M, int64_t K,
+                      int tiles, void* stream, char* err, size_t err_len) {
+    using namespace td;
+    if (!wide_type(dtype)) return fail(err, err_len, TD_ERR_ARG, "unsupported dtype %d", dtype);
+    if (int rc = check_sizes(M, K, 1, err, err_len)) return rc;
+    if (M == 0) return TD_OK;
+    if (q == nullptr || scale == nullptr || out == nullptr)
+        return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
+    if (q_pitch < K) return fail(err, err_len, TD_ERR_ARG, "8-bit rows must not overlap");
+    const BackArgs a = {static_cast<const uint8_t*>(q), scale, out, M, q_pitch, int(K), int(blocks_of(K)), tiles};
+    const bool wide = K % 8 == 0 && q_pitch % 8 == 0 && aligned(q, 8) && aligned(out, 16);
+    const dim3 grid(unsigned(std::min<int64_t>((M * ((K + 7) / 8) + 255) / 256, int64_t(kSms) * 8)));
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return by_type(dtype, [&](auto zero) {
+        using T = decltype(zero);
+        return wide ? host::launch(err, err_len, "fp8_back_kernel", fp8_back_kernel<T, true>, grid, dim3(256), 0, s,
+                                   true, a)
+                    : host::launch(err, err_len, "fp8_back_kernel", fp8_back_kernel<T, false>, grid, dim3(256), 0, s,
+                                   true, a);
+    });
+}
+
+size_t td_fp8_linear_workspace_bytes(int x_dtype, int64_t M, int64_t K, int64_t N) {
+    using namespace td;
+    if ((!wide_type(x_dtype) && x_dtype != TD_E4M3) || M <= 0 || check_sizes(M, K, N, nullptr, 0) != TD_OK) return 0;
+    return plan_linear(x_dtype, M, K, N, nullptr).bytes;
+}
+
+int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_scale, const void* weight,
+                  int64_t w_pitch, const float* w_scale, int bias_dtype, const void* bias, int activation,
+                  int out_dtype, void* out, int64_t out_pitch, float* out_scale, int64_t M, int64_t K, int64_t N,
+                  void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+    using namespace td;
+    if ((!wide_type(x_dtype) && x_dtype != TD_E4M3) || (!wide_type(out_dtype) && out_dtype != TD_E4M3))
+        return fail(err, err_len, TD_ERR_ARG, "unsupported dtype");
+    if (bias != nullptr && !wide_type(bias_dtype)) return fail(err, err_len, TD_ERR_ARG, "unsupported dtype of bias");
+    if (activation < kActNone || activation > kActSilu)
+        return fail(err, err_len, TD_ERR_ARG, "unknown activation %d", activation);
+    if (int rc = check_sizes(M, K, N, err, err_len)) return rc;
+    if (M == 0) return TD_OK;
+    if (x == nullptr || weight == nullptr || w_scale == nullptr || out == nullptr)
+        return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
+    if (out_dtype == TD_E4M3) {
+        if (int rc = check_written(out, out_pitch, N, out_scale, err, err_len)) return rc;
+    }
+    if (x_dtype == TD_E4M3 && (x_scale == nullptr || x_pitch < K))
+        return fail(err, err_len, TD_ERR_ARG, "an 8-bit input has scales, and rows that do not overlap");
+    if (w_pitch < K) return fail(err, err_len, TD_ERR_ARG, "the weight's rows must not overlap");
+    const LinearPlan p = plan_linear(x_dtype, M, K, N, workspace);
+    if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const int64_t KB = blocks_of(K);
+    Operand8 a = {static_cast<const uint8_t*>(x), x_scale, x_pitch, KB, 1, 1};
+    if (x_dtype != TD_E4M3) {
+        a.q = p.q;
+        a.scale = p.scale;
+        a.pitch = up(K, 16);
+        if (int rc = launch_rows(x_dtype, x, p.q, a.pitch, p.scale, M, K, s, err, err_len)) return rc;
+    }
+    const Operand8 b = {static_cast<const uint8_t*>(weight), w_scale, w_pitch, KB, 1, kBlock8};
+    const End8 end = {bias, out, out_scale, bias_dtype, activation, int(out_pitch)};
+    return launch_product(a, b, end, out_dtype, M, N, K, s, err, err_len);
+}
+
+size_t td_fp8_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int want_input, int want_weight,
+                                              int want_bias) {
+    using namespace td;
+    if (M <= 0 || check_sizes(M, K, N, nullptr, 0) != TD_OK) return 0;
+    return plan_backward(M, K, N, want_input != 0, want_weight != 0, want_bias != 0, nullptr).bytes;
+}
+
+int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64_t x_pitch, const float* x_scale,
+                           const void* weight, void* grad_x, void* grad_weight, void* grad_bias, int64_t M, int64_t K,
+                           int64_t N, void* workspace, size_t workspace_bytes, void* stream, char* err,
+                           size_t err_len) {
+    using namespace td;
+    if (!wide_type(dtype)) return fail(err, err_len, TD_ERR_ARG, "unsupported dtype %d", dtype);
+    if (int rc = check_sizes(M, K, N, err, err_len)) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (M == 0) {
+        const size_t e = type_bytes(dtype);
+        if ((grad_weight != nullptr && cudaMemsetAsync(grad_weight, 0, e * size_t(N) * size_t(K), s) != cudaSuccess) ||
+            (grad_bias != nullptr && cudaMemsetAsync(grad_bias, 0, e * size_t(N), s) != cudaSuccess))
+            return fail(err, err_len, TD_ERR_CUDA, "memset: %s", cudaGetErrorString(cudaGetLastError()));
+        return TD_OK;
+    }
+    if (grad_out == nullptr || (grad_x != nullptr && weight == nullptr) ||
+        (grad_weight != nullptr && (x == nullptr || x_scale == nullptr)))
+        return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
+    if (grad_weight != nullptr && x_pitch < K) return fail(err, err_len, TD_ERR_ARG, "8-bit rows must not overlap");
+    const BackwardPlan p = plan_backward(M, K, N, grad_x != nullptr, grad_weight != nullptr, grad_bias != nullptr,
+                                         workspace);
+    if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
+    const int64_t KB = blocks_of(K), NB = blocks_of(N), MB = blocks_of(M);
+    TileArgs g = {};  // the gradient, read once for all that follows
+    g.x = grad_out;
+    g.ld = N;
+    g.q = p.dy;
+    g.scale = p.dy_scale;
+    g.qt = p.dyt;
+    g.scale_t = p.dyt_scale;
+    g.sums = p.sums;
+    if (grad_x == nullptr) g.q = nullptr;
+    if (grad_weight == nullptr) g.qt = nullptr;
+    if (grad_bias == nullptr) g.sums = nullptr;
+    g.M = M;
+    g.q_pitch = up(N, 16);
+    g.qt_pitch = up(M, 16);
+    g.scale_t_pitch = p.n_pad;
+    g.C = int(N);
+    g.CB = int(NB);
+    g.MB = int(MB);
+    if (int rc = launch_tiles(dtype, g, false, s, err, err_len)) return rc;
+    if (grad_bias != nullptr) {
+        const int rc = by_type(dtype, [&](auto zero) {
+            using T = decltype(zero);
+            return host::launch(err, err_len, "column_sum_kernel", column_sum_kernel<T, float>,
+                                dim3(unsigned((N + kColumnCols - 1) / kColumnCols)), dim3(kColumnCols * kColumnRows),
+                                0, s, true, static_cast<const float*>(p.sums), static_cast<T*>(grad_bias),
+                                static_cast<long long>(MB), int(N));
+        });
+        if (rc) return rc;
+    }
+    if (grad_x != nullptr) {
+        TileArgs w = {};  // the weight's blocks, as the forward's, transposed
+        w.x = weight;
+        w.ld = K;
+        w.qt = p.wt;
+        w.scale_t = p.wt_scale;
+        w.M = N;
+        w.qt_pitch = up(N, 16);
+        w.C = int(K);
+        w.CB = int(KB);
+        w.MB = int(NB);
+        if (int rc = launch_tiles(dtype, w, true, s, err, err_len)) return rc;
+        const Operand8 a = {p.dy, p.dy_scale, up(N, 16), NB, 1, 1};
+        const Operand8 b = {p.wt, p.wt_scale, up(N, 16), NB, 1, kBlock8};
+        const End8 end = {nullptr, grad_x, nullptr, dtype, kActNone, 0};
+        if (int rc = launch_product(a, b, end, dtype, M, K, N, s, err, err_len)) return rc;
+    }
+    if (grad_weight != nullptr) {
+        TileArgs x8 = {};  // the kept input, in blocks of rows
+        x8.x = x;
+        x8.x_scale = x_scale;
+        x8.ld = x_pitch;
+        x8.qt = p.xt;
+        x8.scale_t = p.xt_scale;
+        x8.M = M;
+        x8.qt_pitch = up(M, 16);
+        x8.scale_t_pitch = p.k_pad;
+        x8.C = int(K);
+        x8.CB = int(KB);
+        x8.MB = int(MB);
+        if (int rc = launch_tiles(TD_E4M3, x8, false, s, err, err_len)) return rc;
+        const Operand8 a = {p.dyt, p.dyt_scale, up(M, 16), 1, p.n_pad, 1};
+        const Operand8 b = {p.xt, p.xt_scale, up(M, 16), 1, p.k_pad, 1};
+        const End8 end = {nullptr, grad_weight, nullptr, dtype, kActNone, 0};
+        if (int rc = launch_product(a, b, end, dtype, N, K, M, s, err, err_len)) return rc;
+    }
+    return TD_OK;
+}
+
+}  // extern "C"

@@ -25,6 +25,9 @@ void count_launch();
 // cuTensorMapEncodeTiled of 16-bit elements (no interleave, 256-byte L2 promotion, zero fill outside).
 CUresult encode_tiled_u16(CUtensorMap* map, uint32_t rank, const void* base, const uint64_t* dims,
                           const uint64_t* strides, const uint32_t* box, CUtensorMapSwizzle swizzle);
+// The same of a 2-D tensor of bytes.
+CUresult encode_tiled_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
+                         uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
 // Launches `kernel` with an optional programmatic dependent launch (see launch_kernel in tinydeform.cu), counts it
 // and reports a launch error.
@@ -73,7 +76,9 @@ int allow_smem(size_t bytes, char* err, size_t err_len) {
 }  // namespace host
 
 // The device error word of td_attention_tc.cu (a translation unit has its own copy of the word td_ptx.cuh declares;
-// the kernels of the other units wait for nothing).
+// td_fp8.cu has another; the kernels of the rest wait for nothing).
 cudaError_t attention_tc_device_error(int clear, unsigned int* code);
+// That of td_fp8.cu.
+cudaError_t fp8_device_error(int clear, unsigned int* code);
 
 }  // namespace td

@@ -1117,6 +1117,14 @@ CUresult encode_tiled_u16(CUtensorMap* map, uint32_t rank, const void* base, con
     return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, rank, const_cast<void*>(base), d, st, bx, ones, swizzle);
 }
 
+CUresult encode_tiled_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
+                         uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {pitch};
+    const cuuint32_t box[2] = {box_cols, box_rows}, ones[2] = {1, 1};
+    return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, ones,
+                        swizzle);
+}
+
 }  // namespace host
 }  // namespace td
 
@@ -2046,6 +2054,8 @@ int td_device_error(int clear, unsigned int* code, char* err, size_t err_len) {
     }
     unsigned int w = 0;
     if (e == cudaSuccess) e = attention_tc_device_error(clear, &w);
+    if (e == cudaSuccess && v == 0) v = w;
+    if (e == cudaSuccess) e = fp8_device_error(clear, &w);
     if (e != cudaSuccess) return fail(err, err_len, TD_ERR_CUDA, "device error word: %s", cudaGetErrorString(e));
     if (v == 0) v = w;
     if (code != nullptr) *code = v;

@@ -124,3 +124,82 @@ def layer_norm_reference(x, weight, bias=None, residual=None, eps=1e-5):
     acc = torch.float32 if x.dtype in (torch.float16, torch.bfloat16) else x.dtype
     s = x.to(acc) if residual is None else x.to(acc) + residual.to(acc)
     return F.layer_norm(s, s.shape[-1:], weight.to(acc), None if bias is None else bias.to(acc), eps).to(x.dtype)
+
+
+def rms_norm_reference(x, weight, residual=None, eps=1e-6, return_sum=False, quantize=False):
+    """Root-mean-square norm over the last dimension with the residual added inside, with torch operators; the
+    definition ``rms_norm`` follows. float32 arithmetic for float16 / bfloat16 inputs; each result is rounded once."""
+    acc = torch.float32 if x.dtype in (torch.float16, torch.bfloat16) else x.dtype
+    s = x.to(acc) if residual is None else x.to(acc) + residual.to(acc)
+    y = s * torch.rsqrt(s.square().mean(-1, keepdim=True) + eps) * weight.to(acc)
+    y = quantize_fp8_reference(y) if quantize else y.to(x.dtype)
+    return (y, s.to(x.dtype)) if return_sum else y
+
+
+def _fp8_blocks(x, rows):
+    """x [..., R, C] in float32, zeros behind its edges, as [..., R / rows, rows, C / 128, 128]."""
+    R, C = x.shape[-2:]
+    p = F.pad(x.float(), (0, -C % 128, 0, -R % rows))
+    return p.view(*p.shape[:-2], p.shape[-2] // rows, rows, p.shape[-1] // 128, 128)
+
+
+def _fp8_quantize(x, rows):
+    """x [R, C] in blocks of rows x 128: e4m3 data [R, C], scales [R / rows, C / 128] (rounded up)."""
+    R, C = x.shape
+    p = _fp8_blocks(x, rows)
+    top = p.abs().masked_fill(~p.isfinite(), 0).amax((1, 3))
+    mantissa, exponent = torch.frexp(top)  # top = mantissa * 2^exponent, mantissa in [0.5, 1); 448 = 0.875 * 2^9
+    e = (exponent - 9 + (mantissa > 0.875).int()).clamp(min=-126).masked_fill(top == 0, -126)
+    scale = ((e + 127) << 23).int().view(torch.float32)
+    q = p * ((127 - e) << 23).int().view(torch.float32)[:, None, :, None]
+    q = q.masked_fill(~q.isfinite(), float('nan')).to(torch.float8_e4m3fn)
+    return q.view(p.shape[0] * rows, p.shape[2] * 128)[:R, :C].contiguous(), scale
+
+
+def quantize_fp8_reference(x):
+    """x [..., K] in 8 bits with torch operators; the definition ``quantize_fp8`` follows."""
+    rows = x.numel() // x.shape[-1]
+    q, scale = _fp8_quantize(x.reshape(rows, x.shape[-1]), 1)
+    return q.view(x.shape), scale.view(*x.shape[:-1], scale.shape[1])
+
+
+def quantize_weight_fp8_reference(weight):
+    """weight [N, K] in 8 bits with torch operators; the definition ``quantize_weight_fp8`` follows."""
+    return _fp8_quantize(weight, 128)
+
+
+def dequantize_fp8_reference(data, scale, dtype):
+    """What 8-bit data stands for, with torch operators; the definition ``dequantize_fp8`` follows."""
+    K = data.shape[-1]
+    per_row = scale.repeat_interleave(128, -1)[..., :K]
+    if scale.shape[:-1] != data.shape[:-1]:
+        per_row = per_row.repeat_interleave(128, 0)[:data.shape[0]]
+    return (data.float() * per_row).to(dtype)
+
+
+def linear_fp8_reference(x, weight, bias=None, activation=None, quantize=False, dtype=None):
+    """The product of two 8-bit operands (pairs) with torch operators; the definition ``linear_fp8`` follows."""
+    y = torch.matmul(dequantize_fp8_reference(*x, torch.float32), dequantize_fp8_reference(*weight, torch.float32).t())
+    if bias is not None:
+        y = y + bias.float()
+    if activation is not None:
+        y = {'relu': F.relu, 'gelu': F.gelu, 'silu': F.silu}[activation](y)
+    return quantize_fp8_reference(y) if quantize else y.to(dtype)
+
+
+def linear_fp8_backward_reference(grad_out, x8, weight, want_x, want_w, want_b):
+    """The gradients of ``linear_fp8`` with torch operators, from the input's 8-bit copy."""
+    N, K = weight.shape
+    g = grad_out.reshape(-1, N)
+    grad_x = grad_w = grad_b = None
+    if want_x:
+        w8 = dequantize_fp8_reference(*_fp8_quantize(weight, 128), torch.float32)
+        g8 = dequantize_fp8_reference(*_fp8_quantize(g, 1), torch.float32)
+        grad_x = torch.matmul(g8, w8).view(*grad_out.shape[:-1], K).to(grad_out.dtype)
+    if want_w:
+        x = dequantize_fp8_reference(*x8, torch.float32).reshape(-1, K)
+        cols = [dequantize_fp8_reference(*_fp8_quantize(t.t(), 1), torch.float32) for t in (g, x)]
+        grad_w = torch.matmul(cols[0], cols[1].t()).to(grad_out.dtype)
+    if want_b:
+        grad_b = g.float().sum(0).to(grad_out.dtype)
+    return grad_x, grad_w, grad_b
