@@ -5,6 +5,7 @@
 
 #include "td_fp8.cuh"
 #include "td_fp8_simt.cuh"
+#include "td_fp8_tc.cuh"
 #include "td_host.h"
 
 namespace td {
@@ -120,15 +121,125 @@ int launch_simt(const Operand8& a, const Operand8& b, const End8& end, int out_d
     return out_dtype == TD_E4M3 ? go(E4m3()) : by_type(out_dtype, go);
 }
 
+// How the tensor cores take a product: the tile's width, and how many parts K is split into.
+struct TcPlan {
+    int bn, splits, kb_per_split;
+    bool fits;
+};
+
+// A model of the time in microseconds: the longest CTA's blocks and tile ends, and with several parts their way
+// through memory and another launch. Its constants are B200's, from launches of one tile size each.
+TcPlan plan_tc(int64_t M, int64_t N, int64_t K) {
+    const int64_t KB = blocks_of(K);
+    TcPlan best = {0, 1, int(KB), false};
+    double least = 0;
+    for (const int bn : {256, 128}) {
+        const int64_t tiles = (M + kTc8Rows - 1) / kTc8Rows * ((N + bn - 1) / bn);
+        if (tiles > INT32_MAX / 2) continue;
+        const int64_t most = std::max<int64_t>(1, std::min<int64_t>(KB, kSms / tiles));
+        for (int64_t s = 1; s <= most; ++s) {
+            const int64_t per = (KB + s - 1) / s;
+            if (s > 1 && (KB + per - 1) / per != s) continue;  // the last part would be empty
+            const double rounds = double((tiles * s + kSms - 1) / kSms);
+            double t = rounds * (double(per) * (bn == 256 ? 0.34 : 0.22) + (bn == 256 ? 1.2 : 0.8));
+            if (s > 1) t += 2.5 + double(s) * double(M) * double(N) * 8e-6 / 4.0;
+            if (best.bn == 0 || t < least) {
+                least = t;
+                best = {bn, int(s), int(per), true};
+            }
+        }
+    }
+    return best;
+}
+
+size_t partial_floats(int64_t M, int64_t N, int64_t K) {
+    const TcPlan p = plan_tc(M, N, K);
+    return p.splits > 1 ? size_t(p.splits) * size_t(M) * size_t(N) : 0;
+}
+
+bool tc_operand(const Operand8& o) { return aligned(o.q, 16) && o.pitch % 16 == 0 && o.pitch < (1LL << 39); }
+
+int make_map8(CUtensorMap* map, const Operand8& o, int64_t rows, int64_t K, int box_rows, char* err, size_t err_len) {
+    const CUresult r = host::encode_tiled_u8(map, o.q, uint64_t(K), uint64_t(rows), uint64_t(o.pitch), kBlock8,
+                                             uint32_t(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+    if (r == CUDA_SUCCESS) return TD_OK;
+    return fail(err, err_len, TD_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit product) failed (%d)", int(r));
+}
+
+template <int BN, typename T, bool COLS>
+int launch_tc_of(const CUtensorMap& ma, const CUtensorMap& mb, const Tc8Args& t, cudaStream_t stream, char* err,
+                 size_t err_len) {
+    constexpr auto kernel = fp8_product_tc_kernel<BN, T, COLS>;
+    constexpr size_t smem = Tc8Layout<BN, COLS>::kBytes;
+    static_assert(smem <= 227 * 1024, "shared memory of a CTA");
+    if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
+    const int grid = std::min(t.tiles * t.splits, kSms);
+    return host::launch(err, err_len, "fp8_product_tc_kernel", kernel, dim3(unsigned(grid)), dim3(kTc8Threads), smem,
+                        stream, true, ma, mb, t);
+}
+
+int launch_tc(const TcPlan& p, const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M,
+              int64_t N, int64_t K, float* partial, cudaStream_t stream, char* err, size_t err_len) {
+    CUtensorMap ma, mb;
+    if (int rc = make_map8(&ma, a, M, K, kTc8Rows, err, err_len)) return rc;
+    if (int rc = make_map8(&mb, b, N, K, p.bn, err, err_len)) return rc;
+    Tc8Args t = {};
+    t.sa = a.scale;
+    t.sb = b.scale;
+    t.sa_row = a.scale_row;
+    t.sa_k = a.scale_k;
+    t.sb_row = b.scale_row;
+    t.sb_k = b.scale_k;
+    t.end = end;
+    t.partial = partial;
+    t.M = int(M);
+    t.N = int(N);
+    t.k_blocks = int(blocks_of(K));
+    t.n_tiles = int((N + p.bn - 1) / p.bn);
+    t.tiles = int((M + kTc8Rows - 1) / kTc8Rows * t.n_tiles);
+    t.splits = p.splits;
+    t.kb_per_split = p.kb_per_split;
+    if (p.splits > 1) {
+        t.end.bias = nullptr;
+        t.end.act = kActNone;
+    }
+    auto go = [&](auto zero) {
+        using T = decltype(zero);
+        if constexpr (sizeof(T) == 1)
+            return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, t, stream, err, err_len)
+                               : launch_tc_of<128, T, false>(ma, mb, t, stream, err, err_len);
+        else if (b.rows_per_scale == 1)
+            return p.bn == 256 ? launch_tc_of<256, T, true>(ma, mb, t, stream, err, err_len)
+                               : launch_tc_of<128, T, true>(ma, mb, t, stream, err, err_len);
+        else
+            return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, t, stream, err, err_len)
+                               : launch_tc_of<128, T, false>(ma, mb, t, stream, err, err_len);
+    };
+    if (p.splits == 1) return out_dtype == TD_E4M3 ? go(E4m3()) : by_type(out_dtype, go);
+    if (int rc = go(float())) return rc;
+    const dim3 grid(unsigned(std::min<int64_t>((M * blocks_of(N) + 7) / 8, int64_t(kSms) * 8)));
+    auto finish = [&](auto zero) {
+        return host::launch(err, err_len, "fp8_finish_kernel", fp8_finish_kernel<decltype(zero)>, grid, dim3(256), 0,
+                            stream, true, static_cast<const float*>(partial), p.splits, end,
+                            static_cast<long long>(M), int(N));
+    };
+    return out_dtype == TD_E4M3 ? finish(E4m3()) : by_type(out_dtype, finish);
+}
+
+// partial: partial_floats(M, N, K) of them. (Products with a scale for each row of both operands, whose b.scale_row is
+// 1, have a result in a floating type, and scales a tile's width beyond N.)
 int launch_product(const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M, int64_t N,
-                   int64_t K, cudaStream_t stream, char* err, size_t err_len) {
+                   int64_t K, float* partial, cudaStream_t stream, char* err, size_t err_len) {
+    const TcPlan p = plan_tc(M, N, K);
+    if (host::best_policy() && p.fits && tc_operand(a) && tc_operand(b))
+        return launch_tc(p, a, b, end, out_dtype, M, N, K, partial, stream, err, err_len);
     return launch_simt(a, b, end, out_dtype, M, N, K, stream, err, err_len);
 }
 
-// What a forward call keeps in its workspace: the input in 8 bits, where it comes wider.
+// What a forward call keeps in its workspace: the input in 8 bits, where it comes wider, and a split product's parts.
 struct LinearPlan {
     uint8_t* q;
-    float* scale;
+    float *scale, *partial;
     size_t bytes;
 };
 
@@ -139,15 +250,16 @@ LinearPlan plan_linear(int x_dtype, int64_t M, int64_t K, int64_t N, void* works
         p.q = cut.take<uint8_t>(M * up(K, 16));
         p.scale = cut.take<float>(M * blocks_of(K));
     }
+    p.partial = cut.take<float>(int64_t(partial_floats(M, N, K)));
     p.bytes = cut.used == 0 ? 0 : cut.bytes();
     return p;
 }
 
 // A backward call's workspace: the gradient in 1 x 128 blocks, and, transposed, in blocks of 128 rows, as is the
-// input; the transposed weight; the parts of the bias's column sums.
+// input; the transposed weight; the parts of the bias's column sums, and of split products, one after the other.
 struct BackwardPlan {
     uint8_t *dy, *dyt, *xt, *wt;
-    float *dy_scale, *dyt_scale, *xt_scale, *wt_scale, *sums;
+    float *dy_scale, *dyt_scale, *xt_scale, *wt_scale, *sums, *partial;
     int64_t n_pad, k_pad;  // columns of the scales [MB, ..] of the transposed operands
     size_t bytes;
 };
@@ -171,6 +283,8 @@ BackwardPlan plan_backward(int64_t M, int64_t K, int64_t N, bool want_x, bool wa
         p.xt_scale = cut.take<float>(MB * p.k_pad);
     }
     if (want_b) p.sums = cut.take<float>(MB * N);
+    p.partial = cut.take<float>(int64_t(std::max(want_x ? partial_floats(M, K, N) : 0,
+                                                 want_w ? partial_floats(N, K, M) : 0)));
     p.bytes = cut.bytes();
     return p;
 }
@@ -270,7 +384,7 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
     }
     const Operand8 b = {static_cast<const uint8_t*>(weight), w_scale, w_pitch, KB, 1, kBlock8};
     const End8 end = {bias, out, out_scale, bias_dtype, activation, int(out_pitch)};
-    return launch_product(a, b, end, out_dtype, M, N, K, s, err, err_len);
+    return launch_product(a, b, end, out_dtype, M, N, K, p.partial, s, err, err_len);
 }
 
 size_t td_fp8_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int want_input, int want_weight,
@@ -347,7 +461,7 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         const Operand8 a = {p.dy, p.dy_scale, up(N, 16), NB, 1, 1};
         const Operand8 b = {p.wt, p.wt_scale, up(N, 16), NB, 1, kBlock8};
         const End8 end = {nullptr, grad_x, nullptr, dtype, kActNone, 0};
-        if (int rc = launch_product(a, b, end, dtype, M, K, N, s, err, err_len)) return rc;
+        if (int rc = launch_product(a, b, end, dtype, M, K, N, p.partial, s, err, err_len)) return rc;
     }
     if (grad_weight != nullptr) {
         TileArgs x8 = {};  // the kept input, in blocks of rows
@@ -366,7 +480,7 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         const Operand8 a = {p.dyt, p.dyt_scale, up(M, 16), 1, p.n_pad, 1};
         const Operand8 b = {p.xt, p.xt_scale, up(M, 16), 1, p.k_pad, 1};
         const End8 end = {nullptr, grad_weight, nullptr, dtype, kActNone, 0};
-        if (int rc = launch_product(a, b, end, dtype, N, K, M, s, err, err_len)) return rc;
+        if (int rc = launch_product(a, b, end, dtype, N, K, M, p.partial, s, err, err_len)) return rc;
     }
     return TD_OK;
 }

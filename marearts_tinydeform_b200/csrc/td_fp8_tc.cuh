@@ -1,0 +1,392 @@
+// td_fp8_tc.cuh -- the product of two e4m3 operands on tcgen05 tensor cores, with a scale for each block of 128.
+//
+//   out[m, n] = act(sum_kb sa[m, kb] sb[n, kb] sum_{k in block kb} a[m, k] b[n, k] + bias[n])
+//
+// A block of K is one 128-byte row of a swizzled tile: four tcgen05.mma of kind::f8f6f4 (M = 128, N = BN, K = 32) sum
+// its 128 products in TMEM, from zero, and the epilogue warps add that times the scales to float32 registers while the
+// tensor cores work on the next block in another part of TMEM. The scales are so any float32 numbers, and the tensor
+// cores' own sums are never longer than 128 products, however long K is. What bounds it: a 128 x 256 block takes the
+// tensor cores 512 cycles and the 8 epilogue warps (two a scheduler) 128 packed multiply-adds each, plus the reading of
+// 128 KB from TMEM; the 16-bit results' bytes where K is short.
+//
+// Persistent, one CTA an SM, output tiles of 128 x BN (columns fastest, so that the CTAs which share rows of A run
+// together). A tile's K may be split over `splits` units whose float32 parts another kernel adds in order (a long sum
+// behind few tiles: the weight's gradient). Roles: warps 0 - 7 the epilogue (TMEM lanes 32 (w % 4) .., columns
+// w / 4 * BN / 2 ..), warp 8 the TMA producers, two lanes a slot (as in td_gemm_tc.cuh, whose notes on the waits apply
+// here), warp 9 the MMA issuer. COLS: B has a scale for each row and block, which the producers bring to shared memory.
+// In 8-bit results a block of 128 columns of a row is one thread's (BN = 256), or two threads' (BN = 128).
+#pragma once
+
+#include "td_fp8_simt.cuh"
+
+namespace td {
+
+constexpr int kTc8Threads = 320, kTc8Epi = 8, kTc8Rows = 128;
+
+struct Tc8Args {
+    const float *sa, *sb;
+    long long sa_row, sa_k, sb_row, sb_k;  // sb: of a block of 128 rows; COLS: of a row (sb_row = 1)
+    End8 end;
+    float* partial;  // splits > 1: [splits][M][N], instead of end's output
+    int M, N, k_blocks, n_tiles, tiles, splits, kb_per_split;
+};
+
+template <int BN, bool COLS>
+struct Tc8Layout {
+    static constexpr int kStages = BN == 256 ? 4 : 6;
+    static constexpr int kBufs = 512 / BN;  // of BN TMEM columns
+    static constexpr uint32_t kABytes = kTc8Rows * 128, kBBytes = BN * 128, kStageBytes = kABytes + kBBytes;
+    static constexpr size_t kScaleOffset = size_t(kStages) * kStageBytes;
+    static constexpr size_t kBiasOffset = kScaleOffset + (COLS ? size_t(kStages) * BN * 4 : 0);
+    static constexpr size_t kTopOffset = kBiasOffset + 2 * BN * 4;
+    static constexpr size_t kBarOffset = kTopOffset + 2 * kTc8Rows * 4;
+    static constexpr size_t kSlotOffset = kBarOffset + (4 * kStages + 2 * kBufs) * 8;
+    static constexpr size_t kBytes = kSlotOffset + 16 + 1024;  // + alignment of the tiles
+};
+
+__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned, completing on the mbarrier.
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+using Pair8 = uint64_t;  // two floats
+__device__ __forceinline__ Pair8 pair_of(float lo, float hi) {
+    Pair8 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ Pair8 pair_bits(uint32_t lo, uint32_t hi) {
+    Pair8 d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+    return d;
+}
+__device__ __forceinline__ float2 pair_split(Pair8 a) {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(a));
+    return f;
+}
+__device__ __forceinline__ Pair8 pair_fma(Pair8 a, Pair8 b, Pair8 c) {
+    Pair8 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ Pair8 pair_mul(Pair8 a, Pair8 b) {
+    Pair8 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ void st_global_32b_plain(void* dst, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
+// W neighbouring results (32 bytes' worth) as T
+template <typename T, int W>
+__device__ __forceinline__ void pack_results(const float* v, uint32_t* o) {
+    if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[i] = __float_as_uint(v[i]);
+    } else {
+        uint4 w;
+#pragma unroll
+        for (int i = 0; i < W; i += 8) {
+            store16<T>(reinterpret_cast<T*>(&w), v + i);
+            o[i / 2] = w.x; o[i / 2 + 1] = w.y; o[i / 2 + 2] = w.z; o[i / 2 + 3] = w.w;
+        }
+    }
+}
+
+template <int BN, typename T, bool COLS>
+__global__ void __launch_bounds__(kTc8Threads, 1)
+    fp8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                          const Tc8Args a) {
+    using Lay = Tc8Layout<BN, COLS>;
+    constexpr int S = Lay::kStages, NB = Lay::kBufs, CW = BN / 2;
+    constexpr bool kTo8 = sizeof(T) == 1;
+    constexpr bool kShare = kTo8 && CW < kBlock8;  // a block's maximum is found by two threads
+    extern __shared__ __align__(16) unsigned char smem_raw[];
+    unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
+    float* scales = reinterpret_cast<float*>(smem + Lay::kScaleOffset);
+    float* sbias = reinterpret_cast<float*>(smem + Lay::kBiasOffset);
+    float* tops = reinterpret_cast<float*>(smem + Lay::kTopOffset);
+    uint64_t* full = reinterpret_cast<uint64_t*>(smem + Lay::kBarOffset);
+    uint64_t *empty = full + S, *sfull = empty + S, *sempty = sfull + S, *tfull = sempty + S, *tempty = tfull + NB;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Lay::kSlotOffset);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < S; ++s) {
+            mbar_init(&full[s], 2);
+            mbar_init(&empty[s], 1);
+            mbar_init(&sfull[s], 1);
+            mbar_init(&sempty[s], kTc8Epi);
+        }
+        for (int i = 0; i < NB; ++i) {
+            mbar_init(&tfull[i], 1);
+            mbar_init(&tempty[i], kTc8Epi);
+        }
+        mbar_fence_init();
+        tma_prefetch_desc(&map_a);
+        tma_prefetch_desc(&map_b);
+    }
+    __syncwarp();
+    if (warp == 9) {
+        tmem_alloc(tmem_slot, 512);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    const int units = a.tiles * a.splits;
+    // unit -> its first block of K and how many it has
+    auto first_kb = [&](int unit) { return a.splits == 1 ? 0 : unit / a.tiles * a.kb_per_split; };
+    auto count_kb = [&](int unit) {
+        return a.splits == 1 ? a.k_blocks : min(a.kb_per_split, a.k_blocks - first_kb(unit));
+    };
+    auto tile_of = [&](int unit, int& m0, int& n0) {
+        const int t = a.splits == 1 ? unit : unit % a.tiles, mt = t / a.n_tiles;
+        m0 = mt * kTc8Rows;
+        n0 = (t - mt * a.n_tiles) * BN;
+    };
+    if (warp == 8) {
+        // lanes 2s, 2s + 1: the boxes of A and B of slot s; lane 2S + s (COLS): B's scales of their own ring
+        const bool scale_lane = lane >= 2 * S;
+        const int s = scale_lane ? lane - 2 * S : lane >> 1;
+        if (lane < (COLS ? 3 * S : 2 * S)) {
+            uint64_t* const free = scale_lane ? &sempty[s] : &empty[s];
+            uint64_t* const landed = scale_lane ? &sfull[s] : &full[s];
+            const uint64_t pol = l2_evict_last();
+            int unit = blockIdx.x, kb = s, round = 0;
+            long long t0 = clock64();
+            grid_dependency_wait();
+            launch_dependents();
+            // (a last pass only waits, so that nothing is still to arrive on the slot when the CTA exits)
+            for (;;) {
+                while (unit < units && kb >= count_kb(unit)) {
+                    kb -= count_kb(unit);
+                    unit += gridDim.x;
+                }
+                if (mbar_test(free, uint32_t(round & 1) ^ 1u)) {
+                    if (unit >= units) break;
+                    int m0, n0;
+                    tile_of(unit, m0, n0);
+                    const int k = first_kb(unit) + kb;
+                    if (scale_lane) {
+                        mbar_arrive_expect_tx(landed, BN * 4);
+                        bulk_load(scales + s * BN, a.sb + n0 + k * a.sb_k, BN * 4, landed);
+                    } else if ((lane & 1) == 0) {
+                        mbar_arrive_expect_tx(landed, Lay::kABytes);
+                        tma_load_2d(smem + s * Lay::kStageBytes, &map_a, landed, k * kBlock8, m0, pol);
+                    } else {
+                        mbar_arrive_expect_tx(landed, Lay::kBBytes);
+                        tma_load_2d(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k * kBlock8, n0, pol);
+                    }
+                    ++round;
+                    kb += S;
+                    t0 = clock64();
+                } else if (clock64() - t0 > kSpinLimitCycles) {
+                    record_error(kErrSlotWait);
+                    if (round > 0) mbar_wait(landed, uint32_t(round - 1) & 1u, kErrTmaWait);
+                    break;
+                } else {
+                    __nanosleep(32);
+                }
+            }
+        }
+    } else if (warp == 9) {
+        if (lane == 0) {
+            // f32 accumulator, e4m3 (format 0) by e4m3, both K-major
+            constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTc8Rows >> 4) << 24);
+            int it = 0;
+            bool ok = true;
+            for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+                for (int kb = count_kb(unit); kb > 0; --kb, ++it) {
+                    const int s = it % S, b = it % NB;
+                    ok = mbar_wait(&tempty[b], uint32_t((it / NB) & 1) ^ 1u, kErrSlotWait) &&
+                         mbar_wait(&full[s], uint32_t((it / S) & 1), kErrTmaWait);
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t da = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes));
+                    const uint64_t db = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes + Lay::kABytes));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mma_f8(tmem + uint32_t(b * BN), da + uint64_t(2 * k), db + uint64_t(2 * k), idesc, k != 0);
+                    mma_commit(&empty[s]);
+                    mma_commit(&tfull[b]);
+                }
+            }
+        }
+    } else {
+        const int quarter = warp & 3, c_lo = warp / 4 * CW;
+        const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(c_lo);
+        const bool meet = kShare || a.end.bias != nullptr;
+        const int n_blocks = (a.N + kBlock8 - 1) / kBlock8;
+        bool dead = false;  // after a wait that gave up: walk on and meet at the barriers, but wait and store no more
+        int it = 0, turn = 0;
+        grid_dependency_wait();
+        for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
+            int m0, n0;
+            tile_of(unit, m0, n0);
+            const int row = quarter * 32 + lane, m = m0 + row, n = n0 + c_lo;
+            const float* sa = a.sa + (long long)min(m, a.M - 1) * a.sa_row;
+            const float* sb = a.sb + (COLS ? 0 : (long long)min(n / kBlock8, n_blocks - 1) * a.sb_row);
+            const int kb0 = first_kb(unit), count = count_kb(unit);
+            float* const bias = sbias + turn * BN;
+            if (meet) {  // (whoever writes a half again has passed the barrier of the unit between)
+                if (a.end.bias != nullptr) {
+                    for (int i = threadIdx.x; i < BN; i += kTc8Epi * 32)
+                        bias[i] = n0 + i < a.N ? bias_at(a.end, n0 + i) : 0.f;
+                }
+                named_barrier(1, kTc8Epi * 32);
+            }
+            Pair8 acc[CW / 2];
+#pragma unroll
+            for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
+            float sa_next = __ldg(sa + kb0 * a.sa_k), sb_next = COLS ? 1.f : __ldg(sb + kb0 * a.sb_k);
+            for (int kb = 0; kb < count; ++kb, ++it) {
+                const float f = sa_next * sb_next;
+                if (kb + 1 < count) {
+                    sa_next = __ldg(sa + (kb0 + kb + 1) * a.sa_k);
+                    if (!COLS) sb_next = __ldg(sb + (kb0 + kb + 1) * a.sb_k);
+                }
+                const int b = it % NB, s = it % S;
+                bool ready = !dead && mbar_wait(&tfull[b], uint32_t((it / NB) & 1), kErrMmaWait);
+                if (COLS) ready = ready && mbar_wait(&sfull[s], uint32_t((it / S) & 1), kErrTmaWait);
+                dead = !__all_sync(0xffffffffu, ready);
+                if (dead) continue;
+                tc_fence_after();
+                const Pair8 ff = pair_of(f, f);
+#pragma unroll
+                for (int j = 0; j < CW; j += 32) {
+                    uint32_t v[32];
+                    tmem_ld_32x32b_x32(lanes + uint32_t(b * BN + j), v);
+                    tmem_ld_wait();
+                    if (j + 32 == CW) {  // all of it is in registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&tempty[b]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; i += 4) {
+                        Pair8 f0 = ff, f1 = ff;
+                        if constexpr (COLS) {
+                            const float4 c = *reinterpret_cast<const float4*>(scales + s * BN + c_lo + j + i);
+                            f0 = pair_mul(ff, pair_of(c.x, c.y));
+                            f1 = pair_mul(ff, pair_of(c.z, c.w));
+                        }
+                        Pair8 *const a0 = &acc[(j + i) / 2], *const a1 = a0 + 1;
+                        *a0 = pair_fma(pair_bits(v[i], v[i + 1]), f0, *a0);
+                        *a1 = pair_fma(pair_bits(v[i + 2], v[i + 3]), f1, *a1);
+                    }
+                }
+                if constexpr (COLS) {
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sempty[s]);
+                }
+            }
+            // the end: bias, activation, and the row's CW columns out
+            const bool bias_there = a.end.bias != nullptr;
+            float v[CW];
+#pragma unroll
+            for (int i = 0; i < CW; i += 2) {
+                const float2 p = pair_split(acc[i / 2]);
+                v[i] = p.x;
+                v[i + 1] = p.y;
+            }
+            if (bias_there) {
+#pragma unroll
+                for (int i = 0; i < CW; i += 4) {
+                    const float4 c = *reinterpret_cast<const float4*>(bias + c_lo + i);
+                    v[i] += c.x; v[i + 1] += c.y; v[i + 2] += c.z; v[i + 3] += c.w;
+                }
+            }
+            if (a.end.act == kActRelu) {
+#pragma unroll
+                for (int i = 0; i < CW; ++i) v[i] = activate(v[i], kActRelu);
+            } else if (a.end.act == kActGelu) {
+#pragma unroll
+                for (int i = 0; i < CW; ++i) v[i] = activate(v[i], kActGelu);
+            } else if (a.end.act == kActSilu) {
+#pragma unroll
+                for (int i = 0; i < CW; ++i) v[i] = activate(v[i], kActSilu);
+            }
+            const bool stores = !dead && m < a.M;
+            if constexpr (kTo8) {
+                if (n + CW > a.N) {  // (products of zeros, but for NaN in A's row or the scales)
+#pragma unroll
+                    for (int i = 0; i < CW; ++i)
+                        if (n + i >= a.N) v[i] = 0.f;
+                }
+                float top = 0.f;
+#pragma unroll
+                for (int i = 0; i < CW; ++i) top = fmaxf(top, finite_magnitude(v[i]));
+                if constexpr (kShare) {
+                    tops[(warp / 4) * kTc8Rows + row] = top;
+                    named_barrier(1, kTc8Epi * 32);
+                    top = fmaxf(top, tops[(1 - warp / 4) * kTc8Rows + row]);
+                }
+                if (stores) {
+                    const int e = scale_exponent(top);
+                    const float inv = exp2_int(-e);
+                    if (n < a.N && n % kBlock8 == 0)
+                        a.end.scale[(long long)m * n_blocks + n / kBlock8] = exp2_int(e);
+                    uint8_t* dst = static_cast<uint8_t*>(a.end.out) + (long long)m * a.end.pitch + n;
+                    const bool whole = a.end.pitch % 32 == 0;  // (16-byte steps otherwise; the base is 16-byte aligned)
+#pragma unroll
+                    for (int i = 0; i < CW; i += 32) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) w[k] = to_e4m3x4(v + i + 4 * k, inv);
+                        if (whole && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+                            if (n + i < a.end.pitch) st_global_32b_plain(dst + i, w);
+                        } else {
+                            if (n + i < a.end.pitch) *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
+                            if (n + i + 16 < a.end.pitch)
+                                *reinterpret_cast<uint4*>(dst + i + 16) = make_uint4(w[4], w[5], w[6], w[7]);
+                        }
+                    }
+                }
+            } else if (stores) {
+                constexpr int W = 32 / sizeof(T);  // results in 32 bytes
+                T* dst = a.splits == 1 ? static_cast<T*>(a.end.out)
+                                       : reinterpret_cast<T*>(a.partial + (long long)(unit / a.tiles) * a.M * a.N);
+                dst += (long long)m * a.N + n;
+                if (a.N % W == 0 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+#pragma unroll
+                    for (int i = 0; i < CW; i += W) {
+                        uint32_t w[8];
+                        pack_results<T, W>(v + i, w);
+                        if (n + i < a.N) st_global_32b_plain(dst + i, w);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < CW; ++i)
+                        if (n + i < a.N) dst[i] = from_acc<T>(v[i]);
+                }
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 9) {
+        __syncwarp();
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace td
