@@ -13,7 +13,7 @@
 // together). A tile's K may be split over `splits` units whose float32 parts another kernel adds in order (a long sum
 // behind few tiles: the weight's gradient). Roles: warps 0 - 7 the epilogue (TMEM lanes 32 (w % 4) .., columns
 // w / 4 * BN / 2 ..), warp 8 the TMA producers, two lanes a slot (as in td_gemm_tc.cuh, whose notes on the waits apply
-// here), warp 9 the MMA issuer. COLS: B has a scale for each row and block, which the producers bring to shared memory.
+// here), warp 9 the MMA issuer (10 and 11 fill its warpgroup). COLS: B has a scale for each row and block, which the producers bring to shared memory.
 // In 8-bit results a block of 128 columns of a row is one thread's (BN = 256), or two threads' (BN = 128).
 #pragma once
 
@@ -21,7 +21,7 @@
 
 namespace td {
 
-constexpr int kTc8Threads = 320, kTc8Epi = 8, kTc8Rows = 128;
+constexpr int kTc8Threads = 384, kTc8Epi = 8, kTc8Rows = 128;
 
 struct Tc8Args {
     const float *sa, *sb;
@@ -58,6 +58,18 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(smem_addr(dst)), "l"(src), "r"(bytes), "r"(smem_addr(bar))
+                 : "memory");
+}
+
+// tcgen05.wait::ld, on which the registers of an outstanding load depend.
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
                  : "memory");
 }
 
@@ -162,75 +174,81 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
         m0 = mt * kTc8Rows;
         n0 = (t - mt * a.n_tiles) * BN;
     };
-    if (warp == 8) {
-        // lanes 2s, 2s + 1: the boxes of A and B of slot s; lane 2S + s (COLS): B's scales of their own ring
-        const bool scale_lane = lane >= 2 * S;
-        const int s = scale_lane ? lane - 2 * S : lane >> 1;
-        if (lane < (COLS ? 3 * S : 2 * S)) {
-            uint64_t* const free = scale_lane ? &sempty[s] : &empty[s];
-            uint64_t* const landed = scale_lane ? &sfull[s] : &full[s];
-            const uint64_t pol = l2_evict_last();
-            int unit = blockIdx.x, kb = s, round = 0;
-            long long t0 = clock64();
-            grid_dependency_wait();
-            launch_dependents();
-            // (a last pass only waits, so that nothing is still to arrive on the slot when the CTA exits)
-            for (;;) {
-                while (unit < units && kb >= count_kb(unit)) {
-                    kb -= count_kb(unit);
-                    unit += gridDim.x;
-                }
-                if (mbar_test(free, uint32_t(round & 1) ^ 1u)) {
-                    if (unit >= units) break;
-                    int m0, n0;
-                    tile_of(unit, m0, n0);
-                    const int k = first_kb(unit) + kb;
-                    if (scale_lane) {
-                        mbar_arrive_expect_tx(landed, BN * 4);
-                        bulk_load(scales + s * BN, a.sb + n0 + k * a.sb_k, BN * 4, landed);
-                    } else if ((lane & 1) == 0) {
-                        mbar_arrive_expect_tx(landed, Lay::kABytes);
-                        tma_load_2d(smem + s * Lay::kStageBytes, &map_a, landed, k * kBlock8, m0, pol);
-                    } else {
-                        mbar_arrive_expect_tx(landed, Lay::kBBytes);
-                        tma_load_2d(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k * kBlock8, n0, pol);
+    // The epilogue's sums want more registers than an even share: 256 threads of 216 and 128 of 56 are 62464 of the
+    // 64512 that the block has at 168 each.
+    if (warp >= kTc8Epi) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+        if (warp == 8) {
+            // lanes 2s, 2s + 1: the boxes of A and B of slot s; lane 2S + s (COLS): B's scales of their own ring
+            const bool scale_lane = lane >= 2 * S;
+            const int s = scale_lane ? lane - 2 * S : lane >> 1;
+            if (lane < (COLS ? 3 * S : 2 * S)) {
+                uint64_t* const free = scale_lane ? &sempty[s] : &empty[s];
+                uint64_t* const landed = scale_lane ? &sfull[s] : &full[s];
+                const uint64_t pol = l2_evict_last();
+                int unit = blockIdx.x, kb = s, round = 0;
+                long long t0 = clock64();
+                grid_dependency_wait();
+                launch_dependents();
+                // (a last pass only waits, so that nothing is still to arrive on the slot when the CTA exits)
+                for (;;) {
+                    while (unit < units && kb >= count_kb(unit)) {
+                        kb -= count_kb(unit);
+                        unit += gridDim.x;
                     }
-                    ++round;
-                    kb += S;
-                    t0 = clock64();
-                } else if (clock64() - t0 > kSpinLimitCycles) {
-                    record_error(kErrSlotWait);
-                    if (round > 0) mbar_wait(landed, uint32_t(round - 1) & 1u, kErrTmaWait);
-                    break;
-                } else {
-                    __nanosleep(32);
+                    if (mbar_test(free, uint32_t(round & 1) ^ 1u)) {
+                        if (unit >= units) break;
+                        int m0, n0;
+                        tile_of(unit, m0, n0);
+                        const int k = first_kb(unit) + kb;
+                        if (scale_lane) {
+                            mbar_arrive_expect_tx(landed, BN * 4);
+                            bulk_load(scales + s * BN, a.sb + n0 + k * a.sb_k, BN * 4, landed);
+                        } else if ((lane & 1) == 0) {
+                            mbar_arrive_expect_tx(landed, Lay::kABytes);
+                            tma_load_2d(smem + s * Lay::kStageBytes, &map_a, landed, k * kBlock8, m0, pol);
+                        } else {
+                            mbar_arrive_expect_tx(landed, Lay::kBBytes);
+                            tma_load_2d(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k * kBlock8, n0, pol);
+                        }
+                        ++round;
+                        kb += S;
+                        t0 = clock64();
+                    } else if (clock64() - t0 > kSpinLimitCycles) {
+                        record_error(kErrSlotWait);
+                        if (round > 0) mbar_wait(landed, uint32_t(round - 1) & 1u, kErrTmaWait);
+                        break;
+                    } else {
+                        __nanosleep(32);
+                    }
                 }
             }
-        }
-    } else if (warp == 9) {
-        if (lane == 0) {
-            // f32 accumulator, e4m3 (format 0) by e4m3, both K-major
-            constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTc8Rows >> 4) << 24);
-            int it = 0;
-            bool ok = true;
-            for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
-                for (int kb = count_kb(unit); kb > 0; --kb, ++it) {
-                    const int s = it % S, b = it % NB;
-                    ok = mbar_wait(&tempty[b], uint32_t((it / NB) & 1) ^ 1u, kErrSlotWait) &&
-                         mbar_wait(&full[s], uint32_t((it / S) & 1), kErrTmaWait);
-                    if (!ok) break;
-                    tc_fence_after();
-                    const uint64_t da = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes));
-                    const uint64_t db = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes + Lay::kABytes));
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mma_f8(tmem + uint32_t(b * BN), da + uint64_t(2 * k), db + uint64_t(2 * k), idesc, k != 0);
-                    mma_commit(&empty[s]);
-                    mma_commit(&tfull[b]);
+        } else if (warp == 9) {
+            if (lane == 0) {
+                // f32 accumulator, e4m3 (format 0) by e4m3, both K-major
+                constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTc8Rows >> 4) << 24);
+                int it = 0;
+                bool ok = true;
+                for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
+                    for (int kb = count_kb(unit); kb > 0; --kb, ++it) {
+                        const int s = it % S, b = it % NB;
+                        ok = mbar_wait(&tempty[b], uint32_t((it / NB) & 1) ^ 1u, kErrSlotWait) &&
+                             mbar_wait(&full[s], uint32_t((it / S) & 1), kErrTmaWait);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint64_t da = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes));
+                        const uint64_t db = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes + Lay::kABytes));
+    #pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            mma_f8(tmem + uint32_t(b * BN), da + uint64_t(2 * k), db + uint64_t(2 * k), idesc, k != 0);
+                        mma_commit(&empty[s]);
+                        mma_commit(&tfull[b]);
+                    }
                 }
             }
         }
     } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
         const int quarter = warp & 3, c_lo = warp / 4 * CW;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(c_lo);
         const bool meet = kShare || a.end.bias != nullptr;
@@ -270,16 +288,9 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 if (dead) continue;
                 tc_fence_after();
                 const Pair8 ff = pair_of(f, f);
-#pragma unroll
-                for (int j = 0; j < CW; j += 32) {
-                    uint32_t v[32];
-                    tmem_ld_32x32b_x32(lanes + uint32_t(b * BN + j), v);
-                    tmem_ld_wait();
-                    if (j + 32 == CW) {  // all of it is in registers
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&tempty[b]);
-                    }
+// a chunk of 32 columns is on its way from TMEM while the one before it is added
+                uint32_t v0[32], v1[32];
+                auto add = [&](int j, const uint32_t(&w)[32]) {
 #pragma unroll
                     for (int i = 0; i < 32; i += 4) {
                         Pair8 f0 = ff, f1 = ff;
@@ -288,11 +299,29 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                             f0 = pair_mul(ff, pair_of(c.x, c.y));
                             f1 = pair_mul(ff, pair_of(c.z, c.w));
                         }
-                        Pair8 *const a0 = &acc[(j + i) / 2], *const a1 = a0 + 1;
-                        *a0 = pair_fma(pair_bits(v[i], v[i + 1]), f0, *a0);
-                        *a1 = pair_fma(pair_bits(v[i + 2], v[i + 3]), f1, *a1);
+                        Pair8 &a0 = acc[(j + i) / 2], &a1 = acc[(j + i) / 2 + 1];
+                        a0 = pair_fma(pair_bits(w[i], w[i + 1]), f0, a0);
+                        a1 = pair_fma(pair_bits(w[i + 2], w[i + 3]), f1, a1);
                     }
+                };
+                const uint32_t from = lanes + uint32_t(b * BN);
+                tmem_ld_32x32b_x32(from, v0);
+                tmem_ld_wait_for(v0);
+                tmem_ld_32x32b_x32(from + 32, v1);
+                add(0, v0);
+                tmem_ld_wait_for(v1);
+                if constexpr (CW == 128) {
+                    tmem_ld_32x32b_x32(from + 64, v0);
+                    add(32, v1);
+                    tmem_ld_wait_for(v0);
+                    tmem_ld_32x32b_x32(from + 96, v1);
+                    add(64, v0);
+                    tmem_ld_wait_for(v1);
                 }
+                tc_fence_before();  // all of it is in registers
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&tempty[b]);
+                add(CW - 32, v1);
                 if constexpr (COLS) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sempty[s]);
