@@ -167,7 +167,7 @@ int make_map8(CUtensorMap* map, const Operand8& o, int64_t rows, int64_t K, int 
 }
 
 template <int BN, typename T, bool COLS>
-int launch_tc_of(const CUtensorMap& ma, const CUtensorMap& mb, const Tc8Args& t, cudaStream_t stream, char* err,
+int launch_tc_of(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Tc8Args& t, cudaStream_t stream, char* err,
                  size_t err_len) {
     constexpr auto kernel = fp8_product_tc_kernel<BN, T, COLS>;
     constexpr size_t smem = Tc8Layout<BN, COLS>::kBytes;
@@ -175,7 +175,7 @@ int launch_tc_of(const CUtensorMap& ma, const CUtensorMap& mb, const Tc8Args& t,
     if (int rc = host::allow_smem<kernel>(smem, err, err_len)) return rc;
     const int grid = std::min(t.tiles * t.splits, kSms);
     return host::launch(err, err_len, "fp8_product_tc_kernel", kernel, dim3(unsigned(grid)), dim3(kTc8Threads), smem,
-                        stream, true, ma, mb, t);
+                        stream, true, ma, mb, mo, t);
 }
 
 int launch_tc(const TcPlan& p, const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M,
@@ -203,17 +203,29 @@ int launch_tc(const TcPlan& p, const Operand8& a, const Operand8& b, const End8&
         t.end.bias = nullptr;
         t.end.act = kActNone;
     }
+    // results whose rows start on 16-byte boundaries leave in boxes of 32 rows x 128 bytes
+    const int written = p.splits > 1 ? int(TD_F32) : out_dtype;
+    const void* out = p.splits > 1 ? partial : end.out;
+    const int64_t width = written == TD_E4M3 ? end.pitch : N, e = int64_t(type_bytes(written));
+    CUtensorMap mo = mb;  // (any map, where it is not used)
+    t.boxes = aligned(out, 16) && width * e % 16 == 0;
+    if (t.boxes) {
+        const CUresult r = host::encode_tiled_rows(&mo, int(e), out, uint64_t(width), uint64_t(M), uint64_t(p.splits),
+                                                   uint32_t(128 / e), 32, CU_TENSOR_MAP_SWIZZLE_128B);
+        if (r != CUDA_SUCCESS)
+            return fail(err, err_len, TD_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit product) failed (%d)", int(r));
+    }
     auto go = [&](auto zero) {
         using T = decltype(zero);
         if constexpr (sizeof(T) == 1)
-            return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, t, stream, err, err_len)
-                               : launch_tc_of<128, T, false>(ma, mb, t, stream, err, err_len);
+            return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, mo, t, stream, err, err_len)
+                               : launch_tc_of<128, T, false>(ma, mb, mo, t, stream, err, err_len);
         else if (b.rows_per_scale == 1)
-            return p.bn == 256 ? launch_tc_of<256, T, true>(ma, mb, t, stream, err, err_len)
-                               : launch_tc_of<128, T, true>(ma, mb, t, stream, err, err_len);
+            return p.bn == 256 ? launch_tc_of<256, T, true>(ma, mb, mo, t, stream, err, err_len)
+                               : launch_tc_of<128, T, true>(ma, mb, mo, t, stream, err, err_len);
         else
-            return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, t, stream, err, err_len)
-                               : launch_tc_of<128, T, false>(ma, mb, t, stream, err, err_len);
+            return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, mo, t, stream, err, err_len)
+                               : launch_tc_of<128, T, false>(ma, mb, mo, t, stream, err, err_len);
     };
     if (p.splits == 1) return out_dtype == TD_E4M3 ? go(E4m3()) : by_type(out_dtype, go);
     if (int rc = go(float())) return rc;

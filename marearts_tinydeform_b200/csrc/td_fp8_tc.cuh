@@ -22,6 +22,7 @@
 namespace td {
 
 constexpr int kTc8Threads = 384, kTc8Epi = 8, kTc8Rows = 128;
+constexpr int kTc8Ring = 8;  // blocks whose scales an epilogue thread has at hand or on their way
 
 struct Tc8Args {
     const float *sa, *sb;
@@ -29,17 +30,22 @@ struct Tc8Args {
     End8 end;
     float* partial;  // splits > 1: [splits][M][N], instead of end's output
     int M, N, k_blocks, n_tiles, tiles, splits, kb_per_split;
+    int boxes;  // the output's rows start on 16-byte boundaries: map_out (boxes of 32 rows x 128 bytes) stores it
 };
 
 template <int BN, bool COLS>
 struct Tc8Layout {
-    static constexpr int kStages = BN == 256 ? 4 : 6;
+    static constexpr int kStages = BN == 256 ? 3 : 5;
     static constexpr int kBufs = 512 / BN;  // of BN TMEM columns
     static constexpr uint32_t kABytes = kTc8Rows * 128, kBBytes = BN * 128, kStageBytes = kABytes + kBBytes;
-    static constexpr size_t kScaleOffset = size_t(kStages) * kStageBytes;
+    // bytes of results a warp stages: two boxes of 32 rows x 128 bytes, or one (and 32 x 33 floats)
+    static constexpr size_t kStageOut = BN == 256 ? 8192 : 5120;
+    static constexpr size_t kOutOffset = size_t(kStages) * kStageBytes;
+    static constexpr size_t kScaleOffset = kOutOffset + kTc8Epi * kStageOut;
     static constexpr size_t kBiasOffset = kScaleOffset + (COLS ? size_t(kStages) * BN * 4 : 0);
     static constexpr size_t kTopOffset = kBiasOffset + 2 * BN * 4;
-    static constexpr size_t kBarOffset = kTopOffset + 2 * kTc8Rows * 4;
+    static constexpr size_t kRingOffset = kTopOffset + 2 * kTc8Rows * 4;
+    static constexpr size_t kBarOffset = kRingOffset + kTc8Ring * (kTc8Epi * 32 + kTc8Epi) * 4;
     static constexpr size_t kSlotOffset = kBarOffset + (4 * kStages + 2 * kBufs) * 8;
     static constexpr size_t kBytes = kSlotOffset + 16 + 1024;  // + alignment of the tiles
 };
@@ -54,6 +60,11 @@ __device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_
         : "memory");
 }
 
+// 4 bytes from global to shared memory.
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+
 // `bytes` (a multiple of 16) from global to shared memory, both 16-byte aligned, completing on the mbarrier.
 __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
@@ -62,13 +73,11 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
 }
 
 // tcgen05.wait::ld, on which the registers of an outstanding load depend.
-__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[32]) {
+__device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
     asm volatile("tcgen05.wait::ld.sync.aligned;"
                  : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
                    "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
-                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
-                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
-                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                   "+r"(r[15])
                  :
                  : "memory");
 }
@@ -100,32 +109,18 @@ __device__ __forceinline__ Pair8 pair_mul(Pair8 a, Pair8 b) {
     return d;
 }
 
-__device__ __forceinline__ void st_global_32b_plain(void* dst, const uint32_t* w) {
-    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
-                 ::"l"(dst), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+// 3-D tiled store of the box at (x, y, z) from shared memory; what lies outside the tensor is not written. x * element
+// size is a multiple of 16 bytes, no coordinate is negative.
+__device__ __forceinline__ void tma_store_box(const CUtensorMap* map, const void* src, int x, int y, int z) {
+    asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];"
+                 ::"l"(reinterpret_cast<uint64_t>(map)), "r"(smem_addr(src)), "r"(x), "r"(y), "r"(z)
                  : "memory");
-}
-
-// W neighbouring results (32 bytes' worth) as T
-template <typename T, int W>
-__device__ __forceinline__ void pack_results(const float* v, uint32_t* o) {
-    if constexpr (sizeof(T) == 4) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) o[i] = __float_as_uint(v[i]);
-    } else {
-        uint4 w;
-#pragma unroll
-        for (int i = 0; i < W; i += 8) {
-            store16<T>(reinterpret_cast<T*>(&w), v + i);
-            o[i / 2] = w.x; o[i / 2 + 1] = w.y; o[i / 2 + 2] = w.z; o[i / 2 + 3] = w.w;
-        }
-    }
 }
 
 template <int BN, typename T, bool COLS>
 __global__ void __launch_bounds__(kTc8Threads, 1)
     fp8_product_tc_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                          const Tc8Args a) {
+                          const __grid_constant__ CUtensorMap map_out, const Tc8Args a) {
     using Lay = Tc8Layout<BN, COLS>;
     constexpr int S = Lay::kStages, NB = Lay::kBufs, CW = BN / 2;
     constexpr bool kTo8 = sizeof(T) == 1;
@@ -153,6 +148,7 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
         mbar_fence_init();
         tma_prefetch_desc(&map_a);
         tma_prefetch_desc(&map_b);
+        if (a.boxes) tma_prefetch_desc(&map_out);
     }
     __syncwarp();
     if (warp == 9) {
@@ -174,8 +170,8 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
         m0 = mt * kTc8Rows;
         n0 = (t - mt * a.n_tiles) * BN;
     };
-    // The epilogue's sums want more registers than an even share: 256 threads of 216 and 128 of 56 are 62464 of the
-    // 64512 that the block has at 168 each.
+    // The epilogue's sums want more registers than an even share: 256 threads of 224 and 128 of 56 are the
+    // 64512 that the block has at 168 each, exactly.
     if (warp >= kTc8Epi) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
         if (warp == 8) {
@@ -185,7 +181,8 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             if (lane < (COLS ? 3 * S : 2 * S)) {
                 uint64_t* const free = scale_lane ? &sempty[s] : &empty[s];
                 uint64_t* const landed = scale_lane ? &sfull[s] : &full[s];
-                const uint64_t pol = l2_evict_last();
+                // (A's rows are read by the CTAs that run together, B by all)
+                const uint64_t pol_a = l2_evict_first(), pol_b = l2_evict_last();
                 int unit = blockIdx.x, kb = s, round = 0;
                 long long t0 = clock64();
                 grid_dependency_wait();
@@ -206,10 +203,10 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                             bulk_load(scales + s * BN, a.sb + n0 + k * a.sb_k, BN * 4, landed);
                         } else if ((lane & 1) == 0) {
                             mbar_arrive_expect_tx(landed, Lay::kABytes);
-                            tma_load_2d(smem + s * Lay::kStageBytes, &map_a, landed, k * kBlock8, m0, pol);
+                            tma_load_2d(smem + s * Lay::kStageBytes, &map_a, landed, k * kBlock8, m0, pol_a);
                         } else {
                             mbar_arrive_expect_tx(landed, Lay::kBBytes);
-                            tma_load_2d(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k * kBlock8, n0, pol);
+                            tma_load_2d(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k * kBlock8, n0, pol_b);
                         }
                         ++round;
                         kb += S;
@@ -248,21 +245,48 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
         const int quarter = warp & 3, c_lo = warp / 4 * CW;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(c_lo);
+        unsigned char* const staged = smem + Lay::kOutOffset + warp * Lay::kStageOut;
         const bool meet = kShare || a.end.bias != nullptr;
         const int n_blocks = (a.N + kBlock8 - 1) / kBlock8;
         bool dead = false;  // after a wait that gave up: walk on and meet at the barriers, but wait and store no more
         int it = 0, turn = 0;
+        // The scales of the blocks ahead, over the tiles' borders: each thread copies its row's, and lane 0 the warp's
+        // of B, into rings of their own. (Read where they are used, they cost more than all else: 262 us for the 136
+        // of the same products without scales, at 8192 x 4096 x 4096.)
+        float* const ring_a = reinterpret_cast<float*>(smem + Lay::kRingOffset) + threadIdx.x;
+        float* const ring_b = reinterpret_cast<float*>(smem + Lay::kRingOffset) + kTc8Ring * kTc8Epi * 32 + warp;
+        int next_unit = blockIdx.x, next_left = 0, next_slot = 0;
+        const float *next_sa = nullptr, *next_sb = nullptr;
+        auto fetch = [&] {
+            if (next_unit < units) {
+                if (next_left == 0) {
+                    int m0, n0;
+                    tile_of(next_unit, m0, n0);
+                    const long long k0 = first_kb(next_unit);
+                    next_left = count_kb(next_unit);
+                    next_sa = a.sa + (long long)min(m0 + quarter * 32 + lane, a.M - 1) * a.sa_row + k0 * a.sa_k;
+                    if (!COLS) next_sb = a.sb + min((n0 + c_lo) / kBlock8, n_blocks - 1) * a.sb_row + k0 * a.sb_k;
+                }
+                copy4(smem_addr(ring_a + next_slot * kTc8Epi * 32), next_sa);
+                if (!COLS && lane == 0) copy4(smem_addr(ring_b + next_slot * kTc8Epi), next_sb);
+                next_sa += a.sa_k;
+                if (!COLS) next_sb += a.sb_k;
+                if (--next_left == 0) next_unit += gridDim.x;
+                next_slot = next_slot + 1 == kTc8Ring ? 0 : next_slot + 1;
+            }
+            copy_commit();
+        };
         grid_dependency_wait();
+#pragma unroll
+        for (int i = 0; i < kTc8Ring - 1; ++i) fetch();
         for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
             int m0, n0;
             tile_of(unit, m0, n0);
             const int row = quarter * 32 + lane, m = m0 + row, n = n0 + c_lo;
-            const float* sa = a.sa + (long long)min(m, a.M - 1) * a.sa_row;
-            const float* sb = a.sb + (COLS ? 0 : (long long)min(n / kBlock8, n_blocks - 1) * a.sb_row);
-            const int kb0 = first_kb(unit), count = count_kb(unit);
+            const int count = count_kb(unit);
             float* const bias = sbias + turn * BN;
             if (meet) {  // (whoever writes a half again has passed the barrier of the unit between)
                 if (a.end.bias != nullptr) {
@@ -274,13 +298,12 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             Pair8 acc[CW / 2];
 #pragma unroll
             for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
-            float sa_next = __ldg(sa + kb0 * a.sa_k), sb_next = COLS ? 1.f : __ldg(sb + kb0 * a.sb_k);
             for (int kb = 0; kb < count; ++kb, ++it) {
-                const float f = sa_next * sb_next;
-                if (kb + 1 < count) {
-                    sa_next = __ldg(sa + (kb0 + kb + 1) * a.sa_k);
-                    if (!COLS) sb_next = __ldg(sb + (kb0 + kb + 1) * a.sb_k);
-                }
+                copy_wait<kTc8Ring - 2>();
+                __syncwarp();
+                const int slot = it % kTc8Ring;
+                const float f = ring_a[slot * kTc8Epi * 32] * (COLS ? 1.f : ring_b[slot * kTc8Epi]);
+                fetch();
                 const int b = it % NB, s = it % S;
                 bool ready = !dead && mbar_wait(&tfull[b], uint32_t((it / NB) & 1), kErrMmaWait);
                 if (COLS) ready = ready && mbar_wait(&sfull[s], uint32_t((it / S) & 1), kErrTmaWait);
@@ -288,11 +311,11 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 if (dead) continue;
                 tc_fence_after();
                 const Pair8 ff = pair_of(f, f);
-// a chunk of 32 columns is on its way from TMEM while the one before it is added
-                uint32_t v0[32], v1[32];
-                auto add = [&](int j, const uint32_t(&w)[32]) {
+                // a chunk of 16 columns is on its way from TMEM while the one before it is added
+                uint32_t v0[16], v1[16];
+                auto add = [&](int j, const uint32_t(&w)[16]) {
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) {
+                    for (int i = 0; i < 16; i += 4) {
                         Pair8 f0 = ff, f1 = ff;
                         if constexpr (COLS) {
                             const float4 c = *reinterpret_cast<const float4*>(scales + s * BN + c_lo + j + i);
@@ -305,23 +328,23 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     }
                 };
                 const uint32_t from = lanes + uint32_t(b * BN);
-                tmem_ld_32x32b_x32(from, v0);
+                tmem_ld_32x32b_x16(from, v0);
                 tmem_ld_wait_for(v0);
-                tmem_ld_32x32b_x32(from + 32, v1);
-                add(0, v0);
-                tmem_ld_wait_for(v1);
-                if constexpr (CW == 128) {
-                    tmem_ld_32x32b_x32(from + 64, v0);
-                    add(32, v1);
-                    tmem_ld_wait_for(v0);
-                    tmem_ld_32x32b_x32(from + 96, v1);
-                    add(64, v0);
+#pragma unroll
+                for (int j = 0; j < CW; j += 32) {
+                    tmem_ld_32x32b_x16(from + uint32_t(j + 16), v1);
+                    add(j, v0);
                     tmem_ld_wait_for(v1);
+                    if (j + 32 < CW) {
+                        tmem_ld_32x32b_x16(from + uint32_t(j + 32), v0);
+                    } else {  // all of it is in registers
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&tempty[b]);
+                    }
+                    add(j + 16, v1);
+                    if (j + 32 < CW) tmem_ld_wait_for(v0);
                 }
-                tc_fence_before();  // all of it is in registers
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&tempty[b]);
-                add(CW - 32, v1);
                 if constexpr (COLS) {
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&sempty[s]);
@@ -368,47 +391,80 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     named_barrier(1, kTc8Epi * 32);
                     top = fmaxf(top, tops[(1 - warp / 4) * kTc8Rows + row]);
                 }
-                if (stores) {
-                    const int e = scale_exponent(top);
-                    const float inv = exp2_int(-e);
-                    if (n < a.N && n % kBlock8 == 0)
-                        a.end.scale[(long long)m * n_blocks + n / kBlock8] = exp2_int(e);
+                const int e = scale_exponent(top);
+                const float inv = exp2_int(-e);
+                if (stores && n < a.N && n % kBlock8 == 0)
+                    a.end.scale[(long long)m * n_blocks + n / kBlock8] = exp2_int(e);
+                if constexpr (CW == kBlock8) {  // a row of 128 bytes: the warp's one box
+                    if (lane == 0) bulk_wait_read();
+                    __syncwarp();
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        uint4 w;
+                        w.x = to_e4m3x4(v + 16 * i, inv);
+                        w.y = to_e4m3x4(v + 16 * i + 4, inv);
+                        w.z = to_e4m3x4(v + 16 * i + 8, inv);
+                        w.w = to_e4m3x4(v + 16 * i + 12, inv);
+                        *reinterpret_cast<uint4*>(staged + lane * 128 + ((i ^ (lane & 7)) << 4)) = w;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0 && !dead && m < a.M && n < a.end.pitch) {
+                        tma_store_box(&map_out, staged, n, m0 + quarter * 32, 0);
+                        bulk_commit();
+                    }
+                } else if (stores) {
                     uint8_t* dst = static_cast<uint8_t*>(a.end.out) + (long long)m * a.end.pitch + n;
-                    const bool whole = a.end.pitch % 32 == 0;  // (16-byte steps otherwise; the base is 16-byte aligned)
 #pragma unroll
-                    for (int i = 0; i < CW; i += 32) {
-                        uint32_t w[8];
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) w[k] = to_e4m3x4(v + i + 4 * k, inv);
-                        if (whole && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
-                            if (n + i < a.end.pitch) st_global_32b_plain(dst + i, w);
-                        } else {
-                            if (n + i < a.end.pitch) *reinterpret_cast<uint4*>(dst + i) = make_uint4(w[0], w[1], w[2], w[3]);
-                            if (n + i + 16 < a.end.pitch)
-                                *reinterpret_cast<uint4*>(dst + i + 16) = make_uint4(w[4], w[5], w[6], w[7]);
-                        }
+                    for (int i = 0; i < CW; i += 16) {
+                        const uint4 w = make_uint4(to_e4m3x4(v + i, inv), to_e4m3x4(v + i + 4, inv),
+                                                   to_e4m3x4(v + i + 8, inv), to_e4m3x4(v + i + 12, inv));
+                        if (n + i < a.end.pitch) *reinterpret_cast<uint4*>(dst + i) = w;
                     }
                 }
-            } else if (stores) {
-                constexpr int W = 32 / sizeof(T);  // results in 32 bytes
-                T* dst = a.splits == 1 ? static_cast<T*>(a.end.out)
-                                       : reinterpret_cast<T*>(a.partial + (long long)(unit / a.tiles) * a.M * a.N);
-                dst += (long long)m * a.N + n;
-                if (a.N % W == 0 && (reinterpret_cast<uintptr_t>(dst) & 31) == 0) {
+            } else if (a.boxes) {
+                constexpr int kBoxCols = 128 / sizeof(T), kBoxes = CW / kBoxCols, kOnce = BN == 256 ? 2 : 1;
 #pragma unroll
-                    for (int i = 0; i < CW; i += W) {
-                        uint32_t w[8];
-                        pack_results<T, W>(v + i, w);
-                        if (n + i < a.N) st_global_32b_plain(dst + i, w);
+                for (int h = 0; h < kBoxes; h += kOnce) {
+                    if (lane < kOnce) bulk_wait_read();
+                    __syncwarp();
+#pragma unroll
+                    for (int o = 0; o < kOnce; ++o)
+#pragma unroll
+                        for (int i = 0; i < 8; ++i)
+                            store16<T>(reinterpret_cast<T*>(staged + o * 4096 + lane * 128 + ((i ^ (lane & 7)) << 4)),
+                                       v + (h + o) * kBoxCols + i * (kBoxCols / 8));
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    const int col = n + (h + lane) * kBoxCols, first = m0 + quarter * 32;
+                    if (lane < kOnce && !dead && first < a.M && col < a.N) {
+                        tma_store_box(&map_out, staged + lane * 4096, col, first,
+                                      a.splits == 1 ? 0 : unit / a.tiles);
+                        bulk_commit();
                     }
-                } else {
+                }
+            } else {  // rows that start anywhere: 32 x 32 results at a time, turned so that a warp stores a row's 32
+                T* out = a.splits == 1 ? static_cast<T*>(a.end.out)
+                                       : reinterpret_cast<T*>(a.partial + (long long)(unit / a.tiles) * a.M * a.N);
+                float* const turned = reinterpret_cast<float*>(staged);
+                const int first = m0 + quarter * 32, rows = dead ? 0 : min(32, a.M - first);
 #pragma unroll
-                    for (int i = 0; i < CW; ++i)
-                        if (n + i < a.N) dst[i] = from_acc<T>(v[i]);
+                for (int i = 0; i < CW; i += 32) {
+                    __syncwarp();
+#pragma unroll
+                    for (int k = 0; k < 32; ++k) turned[lane * 33 + k] = v[i + k];
+                    __syncwarp();
+                    const int col = n + i + lane;
+                    if (col < a.N) {
+                        for (int r = 0; r < rows; ++r)
+                            out[(long long)(first + r) * a.N + col] = from_acc<T>(turned[r * 33 + lane]);
+                    }
                 }
             }
         }
+        bulk_wait_read();  // the CTA may exit once its stores have read the staged boxes
     }
+    copy_wait<0>();
     tc_fence_before();
     __syncthreads();
     if (warp == 9) {

@@ -28,6 +28,9 @@ CUresult encode_tiled_u16(CUtensorMap* map, uint32_t rank, const void* base, con
 // The same of a 2-D tensor of bytes.
 CUresult encode_tiled_u8(CUtensorMap* map, const void* base, uint64_t cols, uint64_t rows, uint64_t pitch,
                          uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
+// Of a dense [layers, rows, cols] tensor of 1, 2 or 4-byte elements, boxes within a layer.
+CUresult encode_tiled_rows(CUtensorMap* map, int element, const void* base, uint64_t cols, uint64_t rows,
+                           uint64_t layers, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle);
 
 // Launches `kernel` with an optional programmatic dependent launch (see launch_kernel in tinydeform.cu), counts it
 // and reports a launch error.

@@ -1125,6 +1125,16 @@ CUresult encode_tiled_u8(CUtensorMap* map, const void* base, uint64_t cols, uint
                         swizzle);
 }
 
+CUresult encode_tiled_rows(CUtensorMap* map, int element, const void* base, uint64_t cols, uint64_t rows,
+                           uint64_t layers, uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+    const cuuint64_t dims[3] = {cols, rows, layers}, strides[2] = {cols * element, cols * rows * element};
+    const cuuint32_t box[3] = {box_cols, box_rows, 1}, ones[3] = {1, 1, 1};
+    const CUtensorMapDataType type = element == 1   ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : element == 2 ? CU_TENSOR_MAP_DATA_TYPE_UINT16
+                                                    : CU_TENSOR_MAP_DATA_TYPE_UINT32;
+    return encode_tiled(map, type, 3, const_cast<void*>(base), dims, strides, box, ones, swizzle);
+}
+
 }  // namespace host
 }  // namespace td
 
