@@ -4,6 +4,7 @@
 #include <type_traits>
 
 #include "td_fp8.cuh"
+#include "td_fp8_few.cuh"
 #include "td_fp8_simt.cuh"
 #include "td_fp8_tc.cuh"
 #include "td_host.h"
@@ -248,6 +249,45 @@ int launch_product(const Operand8& a, const Operand8& b, const End8& end, int ou
     return launch_simt(a, b, end, out_dtype, M, N, K, stream, err, err_len);
 }
 
+// Products of up to 16 rows with a laid-out weight (td_fp8_few.cuh). x_dtype: what x comes in.
+constexpr int kFewMost = 16, kFewRounds = 8;  // rows, and of those that are still wider than 8 bits
+
+bool few_takes(int x_dtype, const void* x, int64_t x_pitch, const void* w, int64_t w_pitch, int64_t M) {
+    if (!host::best_policy() || M > kFewMost || !aligned(w, 16) || w_pitch % 16 != 0) return false;
+    return x_dtype == TD_E4M3 ? aligned(x, 16) && x_pitch % 16 == 0 : M <= kFewRounds;
+}
+
+int launch_few(int x_dtype, FewArgs a, int out_dtype, cudaStream_t stream, char* err, size_t err_len) {
+    const unsigned ctas = unsigned((a.N + kFewRows - 1) / kFewRows);
+    auto from = [&](auto x) {
+        using X = decltype(x);
+        if constexpr (sizeof(X) > 1) {
+            a.x_wide = a.K % Elem<X>::kVec == 0 && aligned(a.x, 16);
+        }
+        if (out_dtype == TD_E4M3) {
+            const dim3 grid((ctas + 7) / 8 * 8);
+            if constexpr (sizeof(X) == 1) {
+                if (a.M > 8)
+                    return host::launch(err, err_len, "fp8_few_to8_kernel", fp8_few_to8_kernel<X, 2>, grid,
+                                        dim3(kFewThreads), 0, stream, true, a);
+            }
+            return host::launch(err, err_len, "fp8_few_to8_kernel", fp8_few_to8_kernel<X, 1>, grid, dim3(kFewThreads),
+                                0, stream, true, a);
+        }
+        return by_type(out_dtype, [&](auto zero) {
+            using T = decltype(zero);
+            if constexpr (sizeof(X) == 1) {
+                if (a.M > 8)
+                    return host::launch(err, err_len, "fp8_few_kernel", fp8_few_kernel<X, T, 2>, dim3(ctas),
+                                        dim3(kFewThreads), 0, stream, true, a);
+            }
+            return host::launch(err, err_len, "fp8_few_kernel", fp8_few_kernel<X, T, 1>, dim3(ctas),
+                                dim3(kFewThreads), 0, stream, true, a);
+        });
+    };
+    return x_dtype == TD_E4M3 ? from(E4m3()) : by_type(x_dtype, from);
+}
+
 // What a forward call keeps in its workspace: the input in 8 bits, where it comes wider, and a split product's parts.
 struct LinearPlan {
     uint8_t* q;
@@ -387,15 +427,22 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
     if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t KB = blocks_of(K);
+    const End8 end = {bias, out, out_scale, bias_dtype, activation, int(out_pitch)};
     Operand8 a = {static_cast<const uint8_t*>(x), x_scale, x_pitch, KB, 1, 1};
+    auto few = [&](int dtype) {
+        const FewArgs f = {dtype == TD_E4M3 ? a.q : x, a.scale, static_cast<const uint8_t*>(weight), w_scale, end,
+                           a.pitch, w_pitch, int(M), int(N), int(K), int(KB), 0};
+        return launch_few(dtype, f, out_dtype, s, err, err_len);
+    };
+    if (few_takes(x_dtype, x, x_pitch, weight, w_pitch, M)) return few(x_dtype);
     if (x_dtype != TD_E4M3) {
         a.q = p.q;
         a.scale = p.scale;
         a.pitch = up(K, 16);
         if (int rc = launch_rows(x_dtype, x, p.q, a.pitch, p.scale, M, K, s, err, err_len)) return rc;
     }
+    if (few_takes(TD_E4M3, a.q, a.pitch, weight, w_pitch, M)) return few(TD_E4M3);
     const Operand8 b = {static_cast<const uint8_t*>(weight), w_scale, w_pitch, KB, 1, kBlock8};
-    const End8 end = {bias, out, out_scale, bias_dtype, activation, int(out_pitch)};
     return launch_product(a, b, end, out_dtype, M, N, K, p.partial, s, err, err_len);
 }
 

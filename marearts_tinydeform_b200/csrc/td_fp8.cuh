@@ -35,18 +35,26 @@ __device__ __forceinline__ int scale_exponent(float amax) {
 }
 __device__ __forceinline__ float exp2_int(int e) { return __uint_as_float(uint32_t(e + 127) << 23); }  // -126 .. 127
 
-// |v|, or 0 for an infinity or NaN
-__device__ __forceinline__ float finite_magnitude(float v) {
-    const float a = fabsf(v);
-    return a < __int_as_float(0x7F800000) ? a : 0.f;
+// Largest |v|: infinite where there is an infinity; a NaN counts for nothing.
+template <int N>
+__device__ __forceinline__ float largest(const float* v) {
+    float top = fabsf(v[0]) > 0.f ? fabsf(v[0]) : 0.f;
+#pragma unroll
+    for (int i = 1; i < N; ++i) top = fmaxf(top, fabsf(v[i]));
+    return top;
+}
+// Infinities to NaN, which they become in e4m3 and which counts for nothing above. The kernels look for the largest
+// magnitude first, and come here only where that is infinite.
+__device__ __forceinline__ bool infinite(float top) { return top == __int_as_float(0x7F800000); }
+template <int N>
+__device__ __forceinline__ void drop_infinities(float* v) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = fmaf(v[i], 0.f, v[i]);
 }
 
-// Two values times 2^-e as e4m3 (the first in the low byte). v * 0 is NaN for an infinity, which the conversion would
-// take to 448, and zero otherwise.
+// Two values without infinities times 2^-e as e4m3 (the first in the low byte).
 __device__ __forceinline__ uint32_t to_e4m3x2(float a, float b, float inv) {
-    a = fmaf(a, inv, a * 0.f);
-    b = fmaf(b, inv, b * 0.f);
-    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+    return __nv_cvt_float2_to_fp8x2(make_float2(a * inv, b * inv), __NV_SATFINITE, __NV_E4M3);
 }
 __device__ __forceinline__ uint32_t to_e4m3x4(const float* v, float inv) {
     return to_e4m3x2(v[0], v[1], inv) | to_e4m3x2(v[2], v[3], inv) << 16;
@@ -81,33 +89,51 @@ __global__ void __launch_bounds__(kRowsThreads) fp8_rows_kernel(const RowsArgs a
     const long long tasks = a.M * chunks, step = (long long)gridDim.x * (kRowsThreads / 32);
     grid_dependency_wait();
     launch_dependents();
-    for (long long t = (long long)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5); t < tasks; t += step) {
-        const long long row = tasks <= 0xFFFFFFFFLL ? uint32_t(t) / uint32_t(chunks) : t / chunks;
-        const int c = (int(t - row * chunks) * 32 + lane) * VEC;
-        const T* src = static_cast<const T*>(a.x) + row * a.K + c;
-        float v[VEC];
-        if constexpr (WIDE) {
-            if (c < a.K) load16<T>(src, v);
-            else {
+    constexpr int kAhead = WIDE ? 4 : 1;  // a warp's tasks whose loads are under way together
+    for (long long t = (long long)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5); t < tasks; t += kAhead * step) {
+        long long row[kAhead];
+        int col[kAhead];
+        uint4 raw[WIDE ? kAhead : 1];
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) v[i] = 0.f;
+        for (int n = 0; n < kAhead; ++n) {
+            const long long u = t + n * step;
+            row[n] = tasks <= 0x7FFFFFFFLL ? uint32_t(u) / uint32_t(chunks) : u / chunks;
+            col[n] = (int(u - row[n] * chunks) * 32 + lane) * VEC;
+            if (u >= tasks) row[n] = a.M;  // none
+            if constexpr (WIDE) {
+                raw[n] = make_uint4(0, 0, 0, 0);
+                if (row[n] < a.M && col[n] < a.K)
+                    raw[n] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row[n] * a.K + col[n]));
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) v[i] = c + i < a.K ? to_acc(src[i]) : 0.f;
         }
-        float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) top = fmaxf(top, finite_magnitude(v[i]));
+        for (int n = 0; n < kAhead; ++n) {
+            const int c = col[n];
+            float v[VEC];
+            if constexpr (WIDE) {
+                unpack16<T>(raw[n], v);
+            } else {
+                const T* src = static_cast<const T*>(a.x) + row[n] * a.K + c;
 #pragma unroll
-        for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const int e = scale_exponent(top);
-        if (c < a.K && lane % kLanes == 0) a.scale[row * a.KB + c / kBlock8] = exp2_int(e);
-        const float inv = exp2_int(-e);
-        if (c < a.pitch) {  // (the pitch is a multiple of 16)
-            uint8_t* dst = a.q + row * a.pitch + c;
-            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(v, inv), to_e4m3x4(v + 4, inv));
-            else *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(v, inv);
+                for (int i = 0; i < VEC; ++i) v[i] = row[n] < a.M && c + i < a.K ? to_acc(src[i]) : 0.f;
+            }
+            float top = largest<VEC>(v);
+            if (infinite(top)) {
+                drop_infinities<VEC>(v);
+                top = largest<VEC>(v);
+            }
+#pragma unroll
+            for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+            if (row[n] >= a.M) continue;
+            const int e = scale_exponent(top);
+            if (c < a.K && lane % kLanes == 0) a.scale[row[n] * a.KB + c / kBlock8] = exp2_int(e);
+            const float inv = exp2_int(-e);
+            if (c < a.pitch) {  // (the pitch is a multiple of 16)
+                uint8_t* dst = a.q + row[n] * a.pitch + c;
+                if constexpr (VEC == 8)
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(v, inv), to_e4m3x4(v + 4, inv));
+                else *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(v, inv);
+            }
         }
     }
 }
@@ -175,6 +201,25 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
             for (int i = 0; i < 8; ++i) v[p][i] = c0 + i < a.C ? to_acc(src[i]) : 0.f;
         }
     }
+    if (a.sums != nullptr) {  // a thread's rows in order, then the 16 groups of rows in order
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            float sum = v[0][i];
+#pragma unroll
+            for (int p = 1; p < 8; ++p) sum += v[p][i];
+            red[ty][tx * 8 + i] = sum;
+        }
+        __syncthreads();
+        const int c = cb * kBlock8 + threadIdx.x;
+        if (threadIdx.x < kBlock8 && c < a.C) {
+            float sum = red[0][threadIdx.x];
+#pragma unroll
+            for (int g = 1; g < 16; ++g) sum += red[g][threadIdx.x];
+            a.sums[mb * a.C + c] = sum;
+        }
+        __syncthreads();
+    }
+    if (infinite(largest<64>(v[0]))) drop_infinities<64>(v[0]);
     auto pack_row = [&](int p, float inv) {
         if (r0 + p >= a.M || c0 >= a.q_pitch) return;
         *reinterpret_cast<uint2*>(a.q + (r0 + p) * a.q_pitch + c0) =
@@ -182,11 +227,7 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
     };
     float tile_inv = 0.f;
     if constexpr (TILE) {
-        float top = 0.f;
-#pragma unroll
-        for (int p = 0; p < 8; ++p)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_magnitude(v[p][i]));
+        float top = largest<64>(v[0]);
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = top;
@@ -206,33 +247,13 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
     } else if (a.q != nullptr) {
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-            float top = 0.f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_magnitude(v[p][i]));
+            float top = largest<8>(v[p]);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e = scale_exponent(top);
             if (tx == 0 && r0 + p < a.M) a.scale[(r0 + p) * a.CB + cb] = exp2_int(e);
             pack_row(p, exp2_int(-e));
         }
-    }
-    if (a.sums != nullptr) {  // a thread's rows in order, then the 16 groups of rows in order
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float sum = v[0][i];
-#pragma unroll
-            for (int p = 1; p < 8; ++p) sum += v[p][i];
-            red[ty][tx * 8 + i] = sum;
-        }
-        __syncthreads();
-        const int c = cb * kBlock8 + threadIdx.x;
-        if (threadIdx.x < kBlock8 && c < a.C) {
-            float sum = red[0][threadIdx.x];
-#pragma unroll
-            for (int g = 1; g < 16; ++g) sum += red[g][threadIdx.x];
-            a.sums[mb * a.C + c] = sum;
-        }
-        __syncthreads();
     }
     if (a.qt == nullptr) return;
     float inv[8];
@@ -244,7 +265,7 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
         for (int i = 0; i < 8; ++i) {
             float top = 0.f;
 #pragma unroll
-            for (int p = 0; p < 8; ++p) top = fmaxf(top, finite_magnitude(v[p][i]));
+            for (int p = 0; p < 8; ++p) top = fmaxf(top, fabsf(v[p][i]));
             red[ty][tx * 8 + i] = top;
         }
         __syncthreads();

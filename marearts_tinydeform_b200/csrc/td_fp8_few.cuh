@@ -1,0 +1,253 @@
+// td_fp8_few.cuh -- the product of a few rows (up to 16, a serving batch's single tokens) with an e4m3 weight.
+//
+//   out[m, n] = act(sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in block kb} a[m, k] b[n, k] + bias[n])
+//
+// Bound by reading the weight, so its rows are spread over the whole GPU: a CTA takes 16 of them, and its 8 warps every
+// eighth block of K each, with the next block's bytes under way while one is multiplied. e4m3 numbers are exact in
+// float16, so the tensor cores take them as m16n8k16 fragments (16 weight rows by 8 of x) that are read straight from
+// memory: a thread's 16 bytes are four K steps' worth, in an order of K that both operands share. A block's sums start
+// from zero and enter float32 registers times its scales; the warps' sums are added in order.
+//
+// x may be wider than 8 bits (X): each warp then rounds its own blocks, four lanes to a row, instead of another launch
+// before this one. An 8-bit result's blocks of 128 columns are the work of a cluster of 8 CTAs, which exchange their
+// rows' largest magnitudes.
+#pragma once
+
+#include "td_fp8_simt.cuh"
+
+namespace td {
+
+constexpr int kFewThreads = 256, kFewWarps = 8, kFewRows = 16;  // rows of the weight
+
+struct FewArgs {
+    const void* x;         // e4m3, rows x_pitch apart (16-byte aligned), or wider and dense
+    const float* x_scale;  // [M, KB] (e4m3)
+    const uint8_t* w;      // rows w_pitch apart (16-byte aligned)
+    const float* w_scale;  // [NB, KB]
+    End8 end;
+    long long x_pitch, w_pitch;
+    int M, N, K, KB, x_wide;  // x_wide: rows of a wider x start on 16-byte boundaries
+};
+
+__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(two & 0xFFFFu), __NV_E4M3);
+    return uint32_t(h.x) | uint32_t(h.y) << 16;
+}
+// The 16 bytes at p, or those of them before `left` with zeros behind.
+__device__ __forceinline__ uint4 load_bytes(const uint8_t* p, int left) {
+    if (left <= 0) return make_uint4(0, 0, 0, 0);
+    uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+    if (left < 16) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int n = left - 4 * i;
+            w[i] &= n >= 4 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << (8 * n)) - 1;
+        }
+    }
+    return v;
+}
+
+template <typename X, typename T, int TILES>  // TILES of 8 rows of x
+__device__ __forceinline__ void few_rows(const FewArgs& a) {
+    constexpr bool kFrom8 = sizeof(X) == 1, kTo8 = sizeof(T) == 1;
+    constexpr int kVecs = kFrom8 ? 2 : 2 * int(sizeof(X));  // 16-byte vectors of a thread's 32 values
+    __shared__ float sums[kFewWarps][kFewRows][8 * TILES + 1];
+    __shared__ __align__(16) float tops[8 * TILES];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * kFewRows;
+    struct Block {
+        uint4 w[2][2];           // weight rows g, g + 8: 16-byte pieces t and t + 4 of the block
+        uint4 x[TILES][kVecs];   // row g of x: the same values
+        float sx[TILES], sw;
+    };
+    const uint8_t* w_row[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w_row[i] = a.w + (long long)min(n0 + g + 8 * i, a.N - 1) * a.w_pitch;
+    const float* w_scale = a.w_scale + (long long)(min(n0, a.N - 1) / kBlock8) * a.KB;
+    auto load_weight = [&](int kb, Block& b) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = kb * kBlock8 + (t + 4 * h) * 16;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) b.w[i][h] = load_bytes(w_row[i] + k, a.K - k);
+        }
+        b.sw = __ldg(w_scale + kb);
+    };
+    auto load_x = [&](int kb, Block& b) {
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+            const int m = n * 8 + g;
+            b.sx[n] = 0.f;
+#pragma unroll
+            for (int i = 0; i < kVecs; ++i) b.x[n][i] = make_uint4(0, 0, 0, 0);
+            if (m >= a.M) continue;
+            if constexpr (kFrom8) {
+                b.sx[n] = __ldg(a.x_scale + (long long)m * a.KB + kb);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int k = kb * kBlock8 + (t + 4 * h) * 16;
+                    b.x[n][h] = load_bytes(static_cast<const uint8_t*>(a.x) + m * a.x_pitch + k, a.K - k);
+                }
+            } else {
+                constexpr int V = Elem<X>::kVec;
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) {
+                    const int k = kb * kBlock8 + (t + 4 * (i / (kVecs / 2))) * 16 + i % (kVecs / 2) * V;
+                    const X* src = static_cast<const X*>(a.x) + (long long)m * a.K + k;
+                    if (a.x_wide) {
+                        if (k < a.K) b.x[n][i] = __ldg(reinterpret_cast<const uint4*>(src));
+                    } else {
+                        X one[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) one[j] = k + j < a.K ? src[j] : from_acc<X>(0.f);
+                        b.x[n][i] = *reinterpret_cast<const uint4*>(one);
+                    }
+                }
+            }
+        }
+    };
+    float acc[TILES][4] = {};
+    auto multiply = [&](Block& b) {
+        if constexpr (!kFrom8) {  // row g to 8 bits: its four lanes hold the whole block
+#pragma unroll
+            for (int n = 0; n < TILES; ++n) {
+                constexpr int V = Elem<X>::kVec;
+                float v[32];
+#pragma unroll
+                for (int i = 0; i < kVecs; ++i) unpack16<X>(b.x[n][i], v + i * V);
+                float top = largest<32>(v);
+                if (infinite(top)) {
+                    drop_infinities<32>(v);
+                    top = largest<32>(v);
+                }
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int e = scale_exponent(top);
+                const float inv = exp2_int(-e);
+                b.sx[n] = exp2_int(e);
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    b.x[n][h] = make_uint4(to_e4m3x4(v + 16 * h, inv), to_e4m3x4(v + 16 * h + 4, inv),
+                                           to_e4m3x4(v + 16 * h + 8, inv), to_e4m3x4(v + 16 * h + 12, inv));
+            }
+        }
+        float part[TILES][4] = {};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t w0[4] = {b.w[0][h].x, b.w[0][h].y, b.w[0][h].z, b.w[0][h].w};
+            const uint32_t w1[4] = {b.w[1][h].x, b.w[1][h].y, b.w[1][h].z, b.w[1][h].w};
+#pragma unroll
+            for (int s = 0; s < 4; ++s) {
+                const uint32_t fa[4] = {e4m3x2_to_half2(w0[s]), e4m3x2_to_half2(w1[s]), e4m3x2_to_half2(w0[s] >> 16),
+                                        e4m3x2_to_half2(w1[s] >> 16)};
+#pragma unroll
+                for (int n = 0; n < TILES; ++n) {
+                    const uint32_t x = s == 0 ? b.x[n][h].x : s == 1 ? b.x[n][h].y : s == 2 ? b.x[n][h].z : b.x[n][h].w;
+                    const uint32_t fb[2] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16)};
+                    mma_16816(part[n], fa, fb);
+                }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < TILES; ++n) {
+            // results are of rows 2t and 2t + 1 of x
+            const float s0 = __shfl_sync(0xffffffffu, b.sx[n], t * 8) * b.sw;
+            const float s1 = __shfl_sync(0xffffffffu, b.sx[n], t * 8 + 4) * b.sw;
+            acc[n][0] = fmaf(part[n][0], s0, acc[n][0]);
+            acc[n][1] = fmaf(part[n][1], s1, acc[n][1]);
+            acc[n][2] = fmaf(part[n][2], s0, acc[n][2]);
+            acc[n][3] = fmaf(part[n][3], s1, acc[n][3]);
+        }
+    };
+    grid_dependency_wait();
+    launch_dependents();
+    {
+        Block b0, b1;
+        int kb = warp;
+        if (n0 < a.N && kb < a.KB) {
+            load_weight(kb, b0);
+            load_x(kb, b0);
+            for (; kb < a.KB; kb += 2 * kFewWarps) {
+                const int k1 = kb + kFewWarps, k2 = k1 + kFewWarps;
+                if (k1 < a.KB) {
+                    load_weight(k1, b1);
+                    load_x(k1, b1);
+                }
+                multiply(b0);
+                if (k1 >= a.KB) break;
+                if (k2 < a.KB) {
+                    load_weight(k2, b0);
+                    load_x(k2, b0);
+                }
+                multiply(b1);
+            }
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < TILES; ++n) {
+        sums[warp][g][n * 8 + 2 * t] = acc[n][0];
+        sums[warp][g][n * 8 + 2 * t + 1] = acc[n][1];
+        sums[warp][g + 8][n * 8 + 2 * t] = acc[n][2];
+        sums[warp][g + 8][n * 8 + 2 * t + 1] = acc[n][3];
+    }
+    if (kTo8 && threadIdx.x < 8 * TILES) tops[threadIdx.x] = 0.f;
+    __syncthreads();
+    // 16 neighbouring threads end a row's 16 columns
+    const int r = threadIdx.x & 15, m = threadIdx.x >> 4, n = n0 + r;
+    const bool mine = m < 8 * TILES && m < a.M;
+    float v = 0.f;
+    if (mine && n < a.N) {
+#pragma unroll
+        for (int w = 0; w < kFewWarps; ++w) v += sums[w][r][m];
+        v = activate(v + bias_at(a.end, n), a.end.act);
+    }
+    if constexpr (kTo8) {
+        drop_infinities<1>(&v);
+        float top = largest<1>(&v);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (m < 8 * TILES && r == 0) tops[m] = top;
+        cluster_arrive();
+        cluster_wait();
+        float peer = 0.f;  // lane r < 8 reads CTA r's
+        if (m < 8 * TILES && r < 8) {
+            const uint32_t at = cluster_map(smem_addr(&tops[m & ~3]), uint32_t(r));
+            const uint4 four = ld_cluster_v4(at);
+            peer = __uint_as_float((m & 3) == 0 ? four.x : (m & 3) == 1 ? four.y : (m & 3) == 2 ? four.z : four.w);
+        }
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) peer = fmaxf(peer, __shfl_xor_sync(0xffffffffu, peer, o));
+        top = __shfl_sync(0xffffffffu, peer, threadIdx.x & 16);
+        cluster_arrive();
+        if (mine) {
+            const int e = scale_exponent(top);
+            if (n < a.end.pitch)
+                static_cast<uint8_t*>(a.end.out)[(long long)m * a.end.pitch + n] =
+                    uint8_t(to_e4m3x2(v, 0.f, exp2_int(-e)));
+            if (n < a.N && n % kBlock8 == 0)
+                a.end.scale[(long long)m * ((a.N + kBlock8 - 1) / kBlock8) + n / kBlock8] = exp2_int(e);
+        }
+        cluster_wait();  // (no CTA leaves while another may read its maxima)
+    } else {
+        if (mine && n < a.N) static_cast<T*>(a.end.out)[(long long)m * a.N + n] = from_acc<T>(v);
+    }
+}
+
+template <typename X, typename T, int TILES>
+__global__ void __launch_bounds__(kFewThreads) fp8_few_kernel(const FewArgs a) {
+    few_rows<X, T, TILES>(a);
+}
+template <typename X, int TILES>
+__global__ void __cluster_dims__(8, 1, 1) __launch_bounds__(kFewThreads) fp8_few_to8_kernel(const FewArgs a) {
+    few_rows<X, E4m3, TILES>(a);
+}
+
+}  // namespace td

@@ -99,14 +99,14 @@ __global__ void __launch_bounds__(kSimtThreads8)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const long long m = m0 + ty * 4 + i;
-        float top = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int n = n0 + tx + 16 * j;
             acc[i][j] = n < N ? activate(acc[i][j] + bias_at(end, n), end.act) : 0.f;
-            top = fmaxf(top, finite_magnitude(acc[i][j]));
         }
         if constexpr (sizeof(T) == 1) {
+            drop_infinities<8>(acc[i]);
+            float top = largest<8>(acc[i]);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e = scale_exponent(top);
@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[i] = n + i < N ? activate(v[i] + bias_at(end, n + i), end.act) : 0.f;
         if constexpr (sizeof(T) == 1) {
-            float top = fmaxf(fmaxf(finite_magnitude(v[0]), finite_magnitude(v[1])),
-                              fmaxf(finite_magnitude(v[2]), finite_magnitude(v[3])));
+            drop_infinities<4>(v);
+            float top = largest<4>(v);
 #pragma unroll
             for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e = scale_exponent(top);

@@ -383,9 +383,11 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     for (int i = 0; i < CW; ++i)
                         if (n + i >= a.N) v[i] = 0.f;
                 }
-                float top = 0.f;
-#pragma unroll
-                for (int i = 0; i < CW; ++i) top = fmaxf(top, finite_magnitude(v[i]));
+                float top = largest<CW>(v);
+                if (infinite(top)) {
+                    drop_infinities<CW>(v);
+                    top = largest<CW>(v);
+                }
                 if constexpr (kShare) {
                     tops[(warp / 4) * kTc8Rows + row] = top;
                     named_barrier(1, kTc8Epi * 32);

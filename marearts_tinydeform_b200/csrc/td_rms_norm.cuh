@@ -89,13 +89,12 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, false>())
         if constexpr (!Q8) {
             store_row<T, VEC, NV, G>(a.out + row * a.C, s, lane, a.C);
         } else {
-            float top[NV];
+            float top[NV], v[EPT];
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                top[i] = 0.f;
+            for (int i = 0; i < EPT; ++i) v[i] = float(s[i]);
+            if (infinite(largest<EPT>(v))) drop_infinities<EPT>(v);
 #pragma unroll
-                for (int j = 0; j < VEC; ++j) top[i] = fmaxf(top[i], finite_magnitude(float(s[i * VEC + j])));
-            }
+            for (int i = 0; i < NV; ++i) top[i] = largest<VEC>(v + i * VEC);
             if constexpr (VEC == 1 && G == 32) {
 #pragma unroll
                 for (int i = 0; i < NV; i += 4)
@@ -129,13 +128,11 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, false>())
                 if (c >= a.pitch) continue;  // (the pitch is a multiple of 16; behind C the values are zero)
                 uint8_t* dst = a.q + row * a.pitch + c;
                 const float f = exp2_int(-e);
-                float v[VEC];
-#pragma unroll
-                for (int j = 0; j < VEC; ++j) v[j] = float(s[i * VEC + j]);
+                const float* w8 = v + i * VEC;
                 if constexpr (VEC == 8)
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(v, f), to_e4m3x4(v + 4, f));
-                else if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(v, f);
-                else *dst = uint8_t(to_e4m3x2(v[0], 0.f, f));
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(w8, f), to_e4m3x4(w8 + 4, f));
+                else if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(w8, f);
+                else *dst = uint8_t(to_e4m3x2(w8[0], 0.f, f));
             }
         }
     }
