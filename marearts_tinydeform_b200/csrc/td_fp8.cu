@@ -77,6 +77,11 @@ int launch_rows(int dtype, const void* x, uint8_t* q, int64_t pitch, float* scal
     return by_type(dtype, [&](auto zero) {
         using T = decltype(zero);
         constexpr int V = Elem<T>::kVec;
+        if (K % kBlock8 == 0 && aligned(x, 32)) {
+            const dim3 flat(unsigned(std::min<int64_t>((M * (K / 16) + 255) / 256, int64_t(kSms) * 8)));
+            return host::launch(err, err_len, "fp8_flat_kernel", fp8_flat_kernel<T>, flat, dim3(kRowsThreads), 0,
+                                stream, true, a);
+        }
         const bool wide = K % V == 0 && aligned(x, 16);
         const int64_t tasks = M * ((K + 32 * (wide ? V : 4) - 1) / (32 * (wide ? V : 4)));
         const dim3 grid(unsigned(std::min<int64_t>((tasks + 7) / 8, int64_t(kSms) * 8)));
@@ -388,8 +393,12 @@ int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* sc
     const bool wide = K % 8 == 0 && q_pitch % 8 == 0 && aligned(q, 8) && aligned(out, 16);
     const dim3 grid(unsigned(std::min<int64_t>((M * ((K + 7) / 8) + 255) / 256, int64_t(kSms) * 8)));
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool flat = !tiles && K % kBlock8 == 0 && q_pitch == K && aligned(q, 16) && aligned(out, 32);
     return by_type(dtype, [&](auto zero) {
         using T = decltype(zero);
+        if (flat)
+            return host::launch(err, err_len, "fp8_flat_back_kernel", fp8_flat_back_kernel<T>, grid, dim3(256), 0, s,
+                                true, a);
         return wide ? host::launch(err, err_len, "fp8_back_kernel", fp8_back_kernel<T, true>, grid, dim3(256), 0, s,
                                    true, a)
                     : host::launch(err, err_len, "fp8_back_kernel", fp8_back_kernel<T, false>, grid, dim3(256), 0, s,

@@ -89,52 +89,80 @@ __global__ void __launch_bounds__(kRowsThreads) fp8_rows_kernel(const RowsArgs a
     const long long tasks = a.M * chunks, step = (long long)gridDim.x * (kRowsThreads / 32);
     grid_dependency_wait();
     launch_dependents();
-    constexpr int kAhead = WIDE ? 4 : 1;  // a warp's tasks whose loads are under way together
-    for (long long t = (long long)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5); t < tasks; t += kAhead * step) {
-        long long row[kAhead];
-        int col[kAhead];
-        uint4 raw[WIDE ? kAhead : 1];
+    for (long long t = (long long)blockIdx.x * (kRowsThreads / 32) + (threadIdx.x >> 5); t < tasks; t += step) {
+        const long long row = tasks <= 0x7FFFFFFFLL ? uint32_t(t) / uint32_t(chunks) : t / chunks;
+        const int c = (int(t - row * chunks) * 32 + lane) * VEC;
+        const T* src = static_cast<const T*>(a.x) + row * a.K + c;
+        float v[VEC];
+        if constexpr (WIDE) {
+            if (c < a.K) load16<T>(src, v);
+            else {
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n) {
-            const long long u = t + n * step;
-            row[n] = tasks <= 0x7FFFFFFFLL ? uint32_t(u) / uint32_t(chunks) : u / chunks;
-            col[n] = (int(u - row[n] * chunks) * 32 + lane) * VEC;
-            if (u >= tasks) row[n] = a.M;  // none
-            if constexpr (WIDE) {
-                raw[n] = make_uint4(0, 0, 0, 0);
-                if (row[n] < a.M && col[n] < a.K)
-                    raw[n] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(a.x) + row[n] * a.K + col[n]));
+                for (int i = 0; i < VEC; ++i) v[i] = 0.f;
             }
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[i] = c + i < a.K ? to_acc(src[i]) : 0.f;
+        }
+        float top = largest<VEC>(v);
+        if (infinite(top)) {
+            drop_infinities<VEC>(v);
+            top = largest<VEC>(v);
         }
 #pragma unroll
-        for (int n = 0; n < kAhead; ++n) {
-            const int c = col[n];
-            float v[VEC];
-            if constexpr (WIDE) {
-                unpack16<T>(raw[n], v);
-            } else {
-                const T* src = static_cast<const T*>(a.x) + row[n] * a.K + c;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) v[i] = row[n] < a.M && c + i < a.K ? to_acc(src[i]) : 0.f;
-            }
-            float top = largest<VEC>(v);
-            if (infinite(top)) {
-                drop_infinities<VEC>(v);
-                top = largest<VEC>(v);
-            }
-#pragma unroll
-            for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            if (row[n] >= a.M) continue;
-            const int e = scale_exponent(top);
-            if (c < a.K && lane % kLanes == 0) a.scale[row[n] * a.KB + c / kBlock8] = exp2_int(e);
-            const float inv = exp2_int(-e);
-            if (c < a.pitch) {  // (the pitch is a multiple of 16)
-                uint8_t* dst = a.q + row[n] * a.pitch + c;
-                if constexpr (VEC == 8)
-                    *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(v, inv), to_e4m3x4(v + 4, inv));
-                else *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(v, inv);
-            }
+        for (int o = kLanes / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const int e = scale_exponent(top);
+        if (c < a.K && lane % kLanes == 0) a.scale[row * a.KB + c / kBlock8] = exp2_int(e);
+        const float inv = exp2_int(-e);
+        if (c < a.pitch) {  // (the pitch is a multiple of 16)
+            uint8_t* dst = a.q + row * a.pitch + c;
+            if constexpr (VEC == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(v, inv), to_e4m3x4(v + 4, inv));
+            else *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(v, inv);
         }
+    }
+}
+
+// K a multiple of 128 (and x 32-byte aligned): blocks follow one another whatever the rows, so nothing is divided. A
+// thread takes 16 neighbouring values, eight a block, and has the next 16's loads under way.
+__device__ __forceinline__ void load_32b(const void* p, uint4& lo, uint4& hi) {
+    asm volatile("ld.global.nc.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                 : "=r"(lo.x), "=r"(lo.y), "=r"(lo.z), "=r"(lo.w), "=r"(hi.x), "=r"(hi.y), "=r"(hi.z), "=r"(hi.w)
+                 : "l"(p));
+}
+template <typename T>
+__global__ void __launch_bounds__(kRowsThreads) fp8_flat_kernel(const RowsArgs a) {
+    constexpr int kRaw = 16 * int(sizeof(T)) / 16;  // 16-byte vectors of 16 values
+    const long long total = a.M * (a.K / 16), step = (long long)gridDim.x * kRowsThreads;
+    grid_dependency_wait();
+    launch_dependents();
+    uint4 raw[kRaw];
+    auto fetch = [&](long long i) {
+        if (i < total) {
+            const char* src = static_cast<const char*>(a.x) + i * (16 * int(sizeof(T)));
+#pragma unroll
+            for (int k = 0; k < kRaw; k += 2) load_32b(src + k * 16, raw[k], raw[k + 1]);
+        }
+    };
+    long long i = (long long)blockIdx.x * kRowsThreads + threadIdx.x;
+    fetch(i);
+    for (; i < total; i += step) {  // (a block's 8 threads are all in or all out)
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < kRaw; ++k) unpack16<T>(raw[k], v + k * Elem<T>::kVec);
+        fetch(i + step);
+        float top = largest<16>(v);
+        if (infinite(top)) {
+            drop_infinities<16>(v);
+            top = largest<16>(v);
+        }
+        const uint32_t eight = 0xFFu << (threadIdx.x & 24);
+#pragma unroll
+        for (int o = 4; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(eight, top, o));
+        const int e = scale_exponent(top);
+        const float inv = exp2_int(-e);
+        if ((threadIdx.x & 7) == 0) a.scale[i >> 3] = exp2_int(e);
+        *reinterpret_cast<uint4*>(a.q + i * 16) = make_uint4(to_e4m3x4(v, inv), to_e4m3x4(v + 4, inv),
+                                                             to_e4m3x4(v + 8, inv), to_e4m3x4(v + 12, inv));
     }
 }
 
@@ -367,6 +395,46 @@ __global__ void __launch_bounds__(256) fp8_back_kernel(const BackArgs a) {
             for (int i = 0; i < 8; ++i)
                 if (c + i < a.K) dst[i] = from_acc<T>(from_e4m3(src[i]) * s);
         }
+    }
+}
+
+// The same where rows follow one another without gaps, K is a multiple of 128, q 16-byte and out 32-byte aligned: a
+// thread takes 16 neighbouring values of the blocks that follow one another (1 x 128).
+template <typename T>
+__global__ void __launch_bounds__(256) fp8_flat_back_kernel(const BackArgs a) {
+    const long long total = a.M * (a.K / 16), step = (long long)gridDim.x * 256;
+    grid_dependency_wait();
+    launch_dependents();
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    float s = 0.f;
+    auto fetch = [&](long long i) {
+        if (i < total) {
+            raw = __ldg(reinterpret_cast<const uint4*>(a.q + i * 16));
+            s = __ldg(a.scale + (i >> 3));
+        }
+    };
+    long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    fetch(i);
+    for (; i < total; i += step) {
+        const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+        float v[16];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const float2 f = from_e4m3x2(w[k / 2] >> 16 * (k % 2));
+            v[2 * k] = f.x * s;
+            v[2 * k + 1] = f.y * s;
+        }
+        fetch(i + step);
+        T* dst = static_cast<T*>(a.out) + i * 16;
+        uint4 o[16 * sizeof(T) / 16];
+#pragma unroll
+        for (int k = 0; k < int(sizeof(T)); ++k) store16<T>(reinterpret_cast<T*>(&o[k]), v + k * Elem<T>::kVec);
+#pragma unroll
+        for (int k = 0; k < int(sizeof(T)); k += 2)
+            asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                         ::"l"(reinterpret_cast<char*>(dst) + k * 16), "r"(o[k].x), "r"(o[k].y), "r"(o[k].z),
+                           "r"(o[k].w), "r"(o[k + 1].x), "r"(o[k + 1].y), "r"(o[k + 1].z), "r"(o[k + 1].w)
+                         : "memory");
     }
 }
 
