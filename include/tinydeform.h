@@ -438,9 +438,11 @@ TD_API int td_rms_norm_backward(int dtype, const void* grad_y, const void* grad_
  *   [ceil(N / 128), ceil(K / 128)]; bias [N] of bias_dtype or NULL; activation: enum td_activation;
  *   out: [M, N] of out_dtype, or TD_E4M3 as td_fp8_quantize writes it (out_pitch, out_scale [M, ceil(N / 128)]).
  *   workspace: td_fp8_linear_workspace_bytes(x_dtype, M, K, N) bytes.
- * td_fp8_linear_backward: gradients of y = Q(x) Qw(weight)^T + bias, Q and Qw the roundings to 8 bits above, whose own
- * derivative counts as 1. x (rows x_pitch apart) and x_scale: what td_fp8_quantize gave for the forward, the only copy
- * of the input that is kept. weight [N, K] of dtype.
+ * td_fp8_linear_train: the same with a floating weight [N, K] (x, weight, bias and out of dtype), x's 8-bit copy written
+ * into q and scale as td_fp8_quantize writes it: out = Q(x) Qw(weight)^T + bias, Q and Qw the roundings to 8 bits above.
+ *   workspace: td_fp8_linear_train_workspace_bytes(M, K, N) bytes.
+ * td_fp8_linear_backward: its gradients, where the roundings' own derivative counts as 1. x (rows x_pitch apart) and
+ * x_scale: the forward's 8-bit copy, the only one of the input that is kept. weight [N, K] of dtype.
  *   grad_x = Q(grad_out) Qw(weight); grad_weight = Qc(grad_out)^T Qc(x), Qc: blocks of 128 rows of one column;
  *   grad_bias = sum over rows of grad_out (not rounded before). Each may be NULL. Sums are taken in a fixed order.
  *   workspace: td_fp8_linear_backward_workspace_bytes(M, K, N, whether each is wanted) bytes.
@@ -458,6 +460,10 @@ TD_API int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const floa
                          int64_t w_pitch, const float* w_scale, int bias_dtype, const void* bias, int activation,
                          int out_dtype, void* out, int64_t out_pitch, float* out_scale, int64_t M, int64_t K,
                          int64_t N, void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
+TD_API size_t td_fp8_linear_train_workspace_bytes(int64_t M, int64_t K, int64_t N);
+TD_API int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void* bias, void* q,
+                               int64_t q_pitch, float* scale, void* out, int64_t M, int64_t K, int64_t N,
+                               void* workspace, size_t workspace_bytes, void* stream, char* err, size_t err_len);
 TD_API size_t td_fp8_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int want_input, int want_weight,
                                                      int want_bias);
 TD_API int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64_t x_pitch,

@@ -387,8 +387,7 @@ def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None
     grad_bias = the sum of g. Sums are taken in a fixed order. CUDA tensors run this library's kernels; CPU tensors
     linear_fp8_reference.
     """
-    tensors = [t for t in (x, weight, bias) if isinstance(t, torch.Tensor)]
-    grad = _wants_grad(*tensors)
+    grad = torch.is_grad_enabled() and _wants_grad(*(t for t in (x, weight, bias) if isinstance(t, torch.Tensor)))
     dtype = _native.check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad)
     cuda = (x if isinstance(x, torch.Tensor) else x[0]).is_cuda
     if cuda:

@@ -49,6 +49,8 @@ SIGNATURES = {
     'td_fp8_linear_workspace_bytes': (_sz, [_ip, _i64, _i64, _i64]),
     'td_fp8_linear': (_ip, [_ip, _vp, _i64, _vp, _vp, _i64, _vp, _ip, _vp, _ip, _ip, _vp, _i64, _vp, _i64, _i64, _i64,
                             _vp, _sz, _vp, _cp, _sz]),
+    'td_fp8_linear_train_workspace_bytes': (_sz, [_i64, _i64, _i64]),
+    'td_fp8_linear_train': (_ip, [_ip, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp, _cp, _sz]),
     'td_fp8_linear_backward_workspace_bytes': (_sz, [_i64, _i64, _i64, _ip, _ip, _ip]),
     'td_fp8_linear_backward': (_ip, [_ip, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _sz, _vp,
                                      _cp, _sz]),
@@ -1045,21 +1047,23 @@ def check_fp8_source(x, what='x'):
 def check_fp8_pair(pair, what, tiles):
     """A pair (data, scale): e4m3 data [..., K] with float32 scales [..., ceil(K / 128)], or, with tiles, data [N, K]
     with scales [ceil(N / 128), ceil(K / 128)]. Returns it."""
-    if not (isinstance(pair, (tuple, list)) and len(pair) == 2 and all(isinstance(t, torch.Tensor) for t in pair)):
+    if not isinstance(pair, (tuple, list)) or len(pair) != 2 or not isinstance(pair[0], torch.Tensor) or \
+            not isinstance(pair[1], torch.Tensor):
         raise RuntimeError(f'{what} must be a tensor, or a pair (data, scale) of tensors')
     data, scale = pair
     if data.dtype != FP8 or scale.dtype != torch.float32:
         raise RuntimeError(f'{what} in 8 bits must be float8_e4m3fn data with float32 scales')
     if data.device != scale.device:
         raise RuntimeError(f'data and scale of {what} must be on the same device')
-    if data.dim() < (2 if tiles else 1) or (tiles and data.dim() != 2):
+    shape = data.shape
+    if len(shape) != 2 if tiles else len(shape) < 1:
         raise RuntimeError(f'data of {what} must be [N, K]' if tiles else f'{what} must have at least one dimension')
-    if not 1 <= data.shape[-1] <= MAX_FP8_WIDTH or (tiles and not 1 <= data.shape[0] <= MAX_FP8_WIDTH):
+    K = shape[-1]
+    if not 1 <= K <= MAX_FP8_WIDTH or (tiles and not 1 <= shape[0] <= MAX_FP8_WIDTH):
         raise RuntimeError(f'widths of {what} must be between 1 and {MAX_FP8_WIDTH}')
-    want = tuple(data.shape[:-1]) + (-(-data.shape[-1] // FP8_BLOCK),)
-    if tiles:
-        want = (-(-data.shape[0] // FP8_BLOCK), want[1])
-    if tuple(scale.shape) != want:
+    blocks = (K + 127) // 128
+    want = ((shape[0] + 127) // 128, blocks) if tiles else (*shape[:-1], blocks)
+    if scale.shape != want:
         raise RuntimeError(f'the scales of {what} must be of shape {list(want)}, not {list(scale.shape)}')
     return data, scale
 
@@ -1068,29 +1072,26 @@ def _fp8_rows(data):
     """8-bit data [..., K] as rows an equal number of bytes apart, starting on 16-byte boundaries (a copy where they are
     not), and that distance."""
     K = data.shape[-1]
-    pitch, span = None, None
-    good = data.stride(-1) == 1 or K == 1
-    for size, stride in zip(reversed(data.shape[:-1]), reversed(data.stride()[:-1])):
-        if size == 1:
-            continue
-        if pitch is None:
-            pitch, span = stride, stride
-        good = good and stride == span
-        span *= size
-    if pitch is None:
-        pitch = -(-K // 16) * 16
-    if good and pitch >= K and pitch % 16 == 0 and data.data_ptr() % 16 == 0:
-        return data, pitch
     pitch = -(-K // 16) * 16
+    if data.data_ptr() % 16 == 0:
+        if pitch == K and data.is_contiguous():
+            return data, K
+        step = span = None
+        good = data.stride(-1) == 1 or K == 1
+        for size, stride in zip(reversed(data.shape[:-1]), reversed(data.stride()[:-1])):
+            if size == 1:
+                continue
+            if step is None:
+                step = span = stride
+            good = good and stride == span
+            span *= size
+        if step is None:
+            step = pitch
+        if good and step >= K and step % 16 == 0:
+            return data, step
     rows = data.new_zeros((*data.shape[:-1], pitch), dtype=torch.uint8)
     rows[..., :K] = data.view(torch.uint8)
     return rows, pitch
-
-
-def _fp8_weight(pair):
-    data, scale = pair
-    data, pitch = _fp8_rows(data)
-    return data, pitch, scale if scale.is_contiguous() else scale.contiguous()
 
 
 def fp8_quantize(x, tiles=False):
@@ -1173,10 +1174,29 @@ def check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad):
     return dtype
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_fp8_workspace(*sizes):
+    """td_fp8_linear_workspace_bytes (a function of the sizes alone)."""
+    return load().td_fp8_linear_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_fp8_train_workspace(*sizes):
+    """td_fp8_linear_train_workspace_bytes (a function of the sizes alone)."""
+    return load().td_fp8_linear_train_workspace_bytes(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_fp8_backward_workspace(*sizes):
+    """td_fp8_linear_backward_workspace_bytes (a function of the sizes alone)."""
+    return load().td_fp8_linear_backward_workspace_bytes(*sizes)
+
+
 def linear_fp8_forward(x, weight, bias, activation, quantize, dtype):
     """td_fp8_linear for arguments check_linear_fp8 has passed; x may be a pair, weight is one."""
     lib = load()
-    w, w_pitch, w_scale = _fp8_weight(weight)
+    w, w_pitch = _fp8_rows(weight[0])
+    w_scale = weight[1].contiguous()
     if isinstance(x, torch.Tensor):
         data, x_scale, x_pitch, code = x.contiguous(), None, 0, DTYPE_CODE[x.dtype]
         shape = x.shape
@@ -1187,10 +1207,8 @@ def linear_fp8_forward(x, weight, bias, activation, quantize, dtype):
     if not data.is_cuda:
         raise RuntimeError('inputs must be CUDA tensors')
     K, N = shape[-1], weight[0].shape[0]
-    lead = tuple(shape[:-1])
-    M = 1
-    for n in lead:
-        M *= n
+    lead = shape[:-1]
+    M = lead.numel()
     b = None if bias is None else bias.contiguous()
     if quantize:
         out, out_pitch, out_scale = _fp8_empty(data, lead, N)
@@ -1199,13 +1217,31 @@ def linear_fp8_forward(x, weight, bias, activation, quantize, dtype):
         out = result = data.new_empty((*lead, N), dtype=dtype)
         out_pitch, out_scale, out_code = 0, None, DTYPE_CODE[dtype]
     if M:
-        ws_bytes = lib.td_fp8_linear_workspace_bytes(code, M, K, N)
+        ws_bytes = _linear_fp8_workspace(code, M, K, N)
         ws = data.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         _launch(lib.td_fp8_linear, data.device, code, data.data_ptr(), x_pitch, _address(x_scale), w.data_ptr(),
                 w_pitch, w_scale.data_ptr(), 0 if b is None else DTYPE_CODE[b.dtype], _address(b),
                 ACTIVATION_CODE[activation], out_code, out.data_ptr(), out_pitch, _address(out_scale), M, K, N,
                 _address(ws), ws_bytes)
     return result
+
+
+def linear_fp8_train(x, weight, bias):
+    """(y, (data, scale)) through td_fp8_linear_train, for arguments check_linear_fp8 has passed: the product with a
+    floating weight, and x's 8-bit copy, which linear_fp8_backward takes."""
+    lib = load()
+    xs, w, b = _dense(x, weight, bias)
+    N, K = weight.shape
+    lead = x.shape[:-1]
+    M = lead.numel()
+    data, pitch, scale = _fp8_empty(xs, lead, K)
+    y = xs.new_empty((*lead, N))
+    if M:
+        ws_bytes = _linear_fp8_train_workspace(M, K, N)
+        ws = xs.new_empty((ws_bytes,), dtype=torch.uint8)
+        _launch(lib.td_fp8_linear_train, x.device, DTYPE_CODE[x.dtype], xs.data_ptr(), w.data_ptr(), _address(b),
+                data.data_ptr(), pitch, scale.data_ptr(), y.data_ptr(), M, K, N, ws.data_ptr(), ws_bytes)
+    return y, (data, scale)
 
 
 def linear_fp8_backward(grad_out, x8, weight, want_x, want_w, want_b):
@@ -1220,7 +1256,7 @@ def linear_fp8_backward(grad_out, x8, weight, want_x, want_w, want_b):
     grad_x = g.new_empty((*g.shape[:-1], K)) if want_x else None
     grad_w = g.new_empty((N, K)) if want_w else None
     grad_b = g.new_empty((N,)) if want_b else None
-    ws_bytes = lib.td_fp8_linear_backward_workspace_bytes(M, K, N, want_x, want_w, want_b)
+    ws_bytes = _linear_fp8_backward_workspace(M, K, N, want_x, want_w, want_b)
     ws = g.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
     _launch(lib.td_fp8_linear_backward, g.device, DTYPE_CODE[g.dtype], g.data_ptr(), data.data_ptr(), pitch,
             scale.data_ptr(), w.data_ptr(), _address(grad_x), _address(grad_w), _address(grad_b), M, K, N,

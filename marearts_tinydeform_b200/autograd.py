@@ -238,8 +238,7 @@ class LinearFp8Function(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias):
         if x.is_cuda:
-            x8, w8 = _native.fp8_quantize(x), _native.fp8_quantize(weight, tiles=True)
-            y = _native.linear_fp8_forward(x8, w8, bias, None, False, x.dtype)
+            y, x8 = _native.linear_fp8_train(x, weight, bias)
         else:
             x8, w8 = reference.quantize_fp8_reference(x), reference.quantize_weight_fp8_reference(weight)
             y = reference.linear_fp8_reference(x8, w8, bias, dtype=x.dtype)

@@ -92,24 +92,23 @@ int launch_rows(int dtype, const void* x, uint8_t* q, int64_t pitch, float* scal
     });
 }
 
-template <typename T, bool TILE>
-int launch_tiles_of(const TileArgs& a, cudaStream_t stream, char* err, size_t err_len) {
-    const bool wide = a.C % 8 == 0 && aligned(a.x, sizeof(T) == 1 ? 8 : 16) && a.ld * int64_t(sizeof(T)) % 8 == 0 &&
-                      (sizeof(T) == 1 || a.ld * int64_t(sizeof(T)) % 16 == 0);
-    const unsigned y = unsigned(std::min<int64_t>(a.MB, 65535));
-    const dim3 grid(unsigned(a.CB), y, unsigned((a.MB + y - 1) / y));
-    return wide ? host::launch(err, err_len, "fp8_tile_kernel", fp8_tile_kernel<T, true, TILE>, grid,
-                               dim3(kTileThreads), 0, stream, true, a)
-                : host::launch(err, err_len, "fp8_tile_kernel", fp8_tile_kernel<T, false, TILE>, grid,
-                               dim3(kTileThreads), 0, stream, true, a);
-}
-
-int launch_tiles(int dtype, const TileArgs& a, bool tile, cudaStream_t stream, char* err, size_t err_len) {
-    if (dtype == TD_E4M3) return launch_tiles_of<E4m3, false>(a, stream, err, err_len);
+// One launch of up to kTileJobs jobs; dtype: the floating type of those that read one.
+int launch_tiles(int dtype, TileJobs jobs, int count, cudaStream_t stream, char* err, size_t err_len) {
+    int64_t tiles = 0;
+    for (int j = 0; j < count; ++j) {
+        TileArgs& a = jobs.job[j];
+        const int64_t e = a.kind == kTileFrom8 ? 1 : int64_t(type_bytes(dtype)), step = a.kind == kTileFrom8 ? 8 : 16;
+        a.CB = int(blocks_of(a.C));
+        a.MB = int(blocks_of(a.M));
+        a.wide = a.C % 8 == 0 && aligned(a.x, uintptr_t(step)) && a.ld * e % step == 0;
+        tiles += int64_t(a.CB) * a.MB;
+        a.end = tiles;
+    }
+    for (int j = count; j < kTileJobs; ++j) jobs.job[j].end = tiles + 1;
+    if (tiles > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "too many tiles");
     return by_type(dtype, [&](auto zero) {
-        using T = decltype(zero);
-        return tile ? launch_tiles_of<T, true>(a, stream, err, err_len)
-                    : launch_tiles_of<T, false>(a, stream, err, err_len);
+        return host::launch(err, err_len, "fp8_tile_kernel", fp8_tile_kernel<decltype(zero)>, dim3(unsigned(tiles)),
+                            dim3(kTileThreads), 0, stream, true, jobs);
     });
 }
 
@@ -312,6 +311,23 @@ LinearPlan plan_linear(int x_dtype, int64_t M, int64_t K, int64_t N, void* works
     return p;
 }
 
+// A training forward's workspace: the weight in 8 bits, and a split product's parts.
+struct TrainPlan {
+    uint8_t* w;
+    float *w_scale, *partial;
+    size_t bytes;
+};
+
+TrainPlan plan_train(int64_t M, int64_t K, int64_t N, void* workspace) {
+    TrainPlan p = {};
+    Cut cut(workspace);
+    p.w = cut.take<uint8_t>(N * up(K, 16));
+    p.w_scale = cut.take<float>(blocks_of(N) * blocks_of(K));
+    p.partial = cut.take<float>(int64_t(partial_floats(M, N, K)));
+    p.bytes = cut.bytes();
+    return p;
+}
+
 // A backward call's workspace: the gradient in 1 x 128 blocks, and, transposed, in blocks of 128 rows, as is the
 // input; the transposed weight; the parts of the bias's column sums, and of split products, one after the other.
 struct BackwardPlan {
@@ -367,7 +383,9 @@ int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* s
     if (int rc = check_written(q, q_pitch, K, scale, err, err_len)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (!tiles) return launch_rows(dtype, x, static_cast<uint8_t*>(q), q_pitch, scale, M, K, s, err, err_len);
-    TileArgs a = {};
+    TileJobs jobs = {};
+    TileArgs& a = jobs.job[0];
+    a.kind = kTileWhole;
     a.x = x;
     a.ld = K;
     a.q = static_cast<uint8_t*>(q);
@@ -375,9 +393,7 @@ int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* s
     a.M = M;
     a.q_pitch = q_pitch;
     a.C = int(K);
-    a.CB = int(blocks_of(K));
-    a.MB = int(blocks_of(M));
-    return launch_tiles(dtype, a, true, s, err, err_len);
+    return launch_tiles(dtype, jobs, 1, s, err, err_len);
 }
 
 int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* scale, void* out, int64_t M, int64_t K,
@@ -455,6 +471,51 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
     return launch_product(a, b, end, out_dtype, M, N, K, p.partial, s, err, err_len);
 }
 
+size_t td_fp8_linear_train_workspace_bytes(int64_t M, int64_t K, int64_t N) {
+    using namespace td;
+    if (M <= 0 || check_sizes(M, K, N, nullptr, 0) != TD_OK) return 0;
+    return plan_train(M, K, N, nullptr).bytes;
+}
+
+int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void* bias, void* q, int64_t q_pitch,
+                        float* scale, void* out, int64_t M, int64_t K, int64_t N, void* workspace,
+                        size_t workspace_bytes, void* stream, char* err, size_t err_len) {
+    using namespace td;
+    if (!wide_type(dtype)) return fail(err, err_len, TD_ERR_ARG, "unsupported dtype %d", dtype);
+    if (int rc = check_sizes(M, K, N, err, err_len)) return rc;
+    if (M == 0) return TD_OK;
+    if (x == nullptr || weight == nullptr || out == nullptr)
+        return fail(err, err_len, TD_ERR_ARG, "null tensor pointer");
+    if (int rc = check_written(q, q_pitch, K, scale, err, err_len)) return rc;
+    const TrainPlan p = plan_train(M, K, N, workspace);
+    if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
+    const cudaStream_t s = static_cast<cudaStream_t>(stream);
+    TileJobs jobs = {};
+    TileArgs &xs = jobs.job[0], &w = jobs.job[1];
+    xs.kind = kTileBlocks;
+    xs.x = x;
+    xs.ld = K;
+    xs.q = static_cast<uint8_t*>(q);
+    xs.scale = scale;
+    xs.M = M;
+    xs.q_pitch = q_pitch;
+    xs.C = int(K);
+    w.kind = kTileWhole;
+    w.x = weight;
+    w.ld = K;
+    w.q = p.w;
+    w.scale = p.w_scale;
+    w.M = N;
+    w.q_pitch = up(K, 16);
+    w.C = int(K);
+    if (int rc = launch_tiles(dtype, jobs, 2, s, err, err_len)) return rc;
+    const int64_t KB = blocks_of(K);
+    const Operand8 a = {static_cast<const uint8_t*>(q), scale, q_pitch, KB, 1, 1};
+    const Operand8 b = {p.w, p.w_scale, up(K, 16), KB, 1, kBlock8};
+    const End8 end = {bias, out, nullptr, dtype, kActNone, 0};
+    return launch_product(a, b, end, dtype, M, N, K, p.partial, s, err, err_len);
+}
+
 size_t td_fp8_linear_backward_workspace_bytes(int64_t M, int64_t K, int64_t N, int want_input, int want_weight,
                                               int want_bias) {
     using namespace td;
@@ -484,26 +545,49 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
     const BackwardPlan p = plan_backward(M, K, N, grad_x != nullptr, grad_weight != nullptr, grad_bias != nullptr,
                                          workspace);
     if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
-    const int64_t KB = blocks_of(K), NB = blocks_of(N), MB = blocks_of(M);
-    TileArgs g = {};  // the gradient, read once for all that follows
+    const int64_t NB = blocks_of(N), MB = blocks_of(M);
+    // all that is laid out, in one launch: the gradient (read once for all that follows) ..
+    TileJobs jobs = {};
+    int count = 1;
+    TileArgs& g = jobs.job[0];
+    g.kind = kTileBlocks;
     g.x = grad_out;
     g.ld = N;
-    g.q = p.dy;
+    if (grad_x != nullptr) g.q = p.dy;
     g.scale = p.dy_scale;
-    g.qt = p.dyt;
+    if (grad_weight != nullptr) g.qt = p.dyt;
     g.scale_t = p.dyt_scale;
-    g.sums = p.sums;
-    if (grad_x == nullptr) g.q = nullptr;
-    if (grad_weight == nullptr) g.qt = nullptr;
-    if (grad_bias == nullptr) g.sums = nullptr;
+    if (grad_bias != nullptr) g.sums = p.sums;
     g.M = M;
     g.q_pitch = up(N, 16);
     g.qt_pitch = up(M, 16);
     g.scale_t_pitch = p.n_pad;
     g.C = int(N);
-    g.CB = int(NB);
-    g.MB = int(MB);
-    if (int rc = launch_tiles(dtype, g, false, s, err, err_len)) return rc;
+    if (grad_weight != nullptr) {  // .. the kept input, in blocks of rows
+        TileArgs& x8 = jobs.job[count++];
+        x8.kind = kTileFrom8;
+        x8.x = x;
+        x8.x_scale = x_scale;
+        x8.ld = x_pitch;
+        x8.qt = p.xt;
+        x8.scale_t = p.xt_scale;
+        x8.M = M;
+        x8.qt_pitch = up(M, 16);
+        x8.scale_t_pitch = p.k_pad;
+        x8.C = int(K);
+    }
+    if (grad_x != nullptr) {  // .. and the weight's blocks, as the forward's, transposed
+        TileArgs& w = jobs.job[count++];
+        w.kind = kTileWhole;
+        w.x = weight;
+        w.ld = K;
+        w.qt = p.wt;
+        w.scale_t = p.wt_scale;
+        w.M = N;
+        w.qt_pitch = up(N, 16);
+        w.C = int(K);
+    }
+    if (int rc = launch_tiles(dtype, jobs, count, s, err, err_len)) return rc;
     if (grad_bias != nullptr) {
         const int rc = by_type(dtype, [&](auto zero) {
             using T = decltype(zero);
@@ -515,36 +599,12 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         if (rc) return rc;
     }
     if (grad_x != nullptr) {
-        TileArgs w = {};  // the weight's blocks, as the forward's, transposed
-        w.x = weight;
-        w.ld = K;
-        w.qt = p.wt;
-        w.scale_t = p.wt_scale;
-        w.M = N;
-        w.qt_pitch = up(N, 16);
-        w.C = int(K);
-        w.CB = int(KB);
-        w.MB = int(NB);
-        if (int rc = launch_tiles(dtype, w, true, s, err, err_len)) return rc;
         const Operand8 a = {p.dy, p.dy_scale, up(N, 16), NB, 1, 1};
         const Operand8 b = {p.wt, p.wt_scale, up(N, 16), NB, 1, kBlock8};
         const End8 end = {nullptr, grad_x, nullptr, dtype, kActNone, 0};
         if (int rc = launch_product(a, b, end, dtype, M, K, N, p.partial, s, err, err_len)) return rc;
     }
     if (grad_weight != nullptr) {
-        TileArgs x8 = {};  // the kept input, in blocks of rows
-        x8.x = x;
-        x8.x_scale = x_scale;
-        x8.ld = x_pitch;
-        x8.qt = p.xt;
-        x8.scale_t = p.xt_scale;
-        x8.M = M;
-        x8.qt_pitch = up(M, 16);
-        x8.scale_t_pitch = p.k_pad;
-        x8.C = int(K);
-        x8.CB = int(KB);
-        x8.MB = int(MB);
-        if (int rc = launch_tiles(TD_E4M3, x8, false, s, err, err_len)) return rc;
         const Operand8 a = {p.dyt, p.dyt_scale, up(M, 16), 1, p.n_pad, 1};
         const Operand8 b = {p.xt, p.xt_scale, up(M, 16), 1, p.k_pad, 1};
         const End8 end = {nullptr, grad_weight, nullptr, dtype, kActNone, 0};

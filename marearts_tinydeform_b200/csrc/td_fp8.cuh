@@ -17,6 +17,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "td_common.cuh"
 #include "td_ptx.cuh"
 
@@ -168,74 +170,154 @@ __global__ void __launch_bounds__(kRowsThreads) fp8_flat_kernel(const RowsArgs a
 
 // ---- 128 x 128 tiles --------------------------------------------------------------------------------------------
 
+enum TileKind : int { kTileBlocks = 0, kTileWhole = 1, kTileFrom8 = 2 };
+
 struct TileArgs {
-    const void* x;           // [M, C], rows `ld` apart: floating, or e4m3 with
+    const void* x;           // [M, C], rows `ld` elements apart: floating, or (kTileFrom8) e4m3 with
     const float* x_scale;    //   its scales [M, CB] (1 x 128)
     long long ld;
-    uint8_t* q;              // or null: [M, q_pitch], in 1 x 128 blocks, or 128 x 128 (TILE)
+    uint8_t* q;              // or null: [M, q_pitch], in 1 x 128 blocks, or 128 x 128 (kTileWhole)
     float* scale;            //   [M, CB], or [MB, CB]
     uint8_t* qt;             // or null: the transpose [C, qt_pitch], in blocks of 128 rows of x, or 128 x 128
     float* scale_t;          //   [MB, scale_t_pitch] (one for each column), or [CB, MB]
     float* sums;             // or null: [MB, C] sums over a tile's rows
     long long M, q_pitch, qt_pitch, scale_t_pitch;
-    int C, CB, MB;
+    int C, CB, MB, kind;
+    int wide;                // rows of x start on 16-byte boundaries (8-byte ones for e4m3), C a multiple of 8
+    long long end;           // of the launch's tiles, this job's and those before it
 };
 
-constexpr int kTileThreads = 256;
+constexpr int kTileThreads = 256, kTileJobs = 3;
+struct TileJobs {  // independent jobs of one launch
+    TileArgs job[kTileJobs];
+};
 
-// A thread holds 8 rows x 8 columns of the tile: rows 8 ty .. 8 ty + 7, columns 8 tx .. 8 tx + 7 (tx < 16).
-// WIDE: rows of x start on 16-byte boundaries (8-byte ones for e4m3) and C is a multiple of 8.
-template <typename T, bool WIDE, bool TILE>
-__global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a) {
-    constexpr bool kFrom8 = sizeof(T) == 1;
-    __shared__ float red[16][kBlock8];
-    __shared__ __align__(16) uint8_t turned[kBlock8 * kBlock8];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int cb = blockIdx.x;
-    const long long mb = blockIdx.y + (long long)blockIdx.z * gridDim.y;
-    if (mb >= a.MB) return;
-    const long long r0 = mb * kBlock8 + ty * 8;
-    const int c0 = cb * kBlock8 + tx * 8;
-    grid_dependency_wait();
-    launch_dependents();
-    float v[8][8];
+// A thread's 8 rows x 8 columns of a tile, as they came from memory: fewer registers than as float32, and so more
+// tiles at once on an SM. pair(p, c): columns 2c and 2c + 1 of row p.
+template <typename T>
+struct Patch {  // 16-bit types
+    uint4 w[8];
+    static __device__ __forceinline__ uint32_t word(const uint4& v, int c) {
+        return c == 0 ? v.x : c == 1 ? v.y : c == 2 ? v.z : v.w;
+    }
+    __device__ __forceinline__ void clear(int p) { w[p] = make_uint4(0, 0, 0, 0); }
+    __device__ __forceinline__ void load(int p, const T* src, int left, bool wide) {
+        if (wide) {
+            w[p] = __ldg(reinterpret_cast<const uint4*>(src));
+        } else {
+            T one[8];
 #pragma unroll
-    for (int p = 0; p < 8; ++p) {
-        const long long row = r0 + p;
-        const T* src = static_cast<const T*>(a.x) + row * a.ld + c0;
-        if (row >= a.M || c0 >= a.C) {
+            for (int i = 0; i < 8; ++i) one[i] = i < left ? src[i] : from_acc<T>(0.f);
+            w[p] = *reinterpret_cast<const uint4*>(one);
+        }
+    }
+    __device__ __forceinline__ float2 pair(int p, int c) const {
+        const uint32_t two = word(w[p], c);
+        if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&two));
+        else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
+    }
+    // infinities to NaN (0x7FFF is one in both types)
+    __device__ __forceinline__ void drop_infinite() {
+        constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
+        uint32_t most = 0;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = 0.f;
-        } else if constexpr (kFrom8) {
-            const float s = a.x_scale[row * a.CB + cb];
-            if constexpr (WIDE) {
-                const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-                const uint32_t h[4] = {w.x, w.x >> 16, w.y, w.y >> 16};
+        for (int p = 0; p < 8; ++p)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float2 f = from_e4m3x2(h[i]);
-                    v[p][2 * i] = f.x * s;
-                    v[p][2 * i + 1] = f.y * s;
-                }
-            } else {
+            for (int c = 0; c < 4; ++c) most = __vmaxu2(most, word(w[p], c) & 0x7FFF7FFFu);
+        if ((most & 0xFFFFu) < kInf && most >> 16 < kInf) return;
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[p][i] = c0 + i < a.C ? from_e4m3(src[i].bits) * s : 0.f;
+        for (int p = 0; p < 8; ++p) {
+            uint32_t* v = reinterpret_cast<uint32_t*>(&w[p]);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if ((v[c] & 0x7FFFu) == kInf) v[c] |= 0x7FFFu;
+                if ((v[c] >> 16 & 0x7FFFu) == kInf) v[c] |= 0x7FFF0000u;
             }
-        } else if constexpr (WIDE) {
+        }
+    }
+};
+template <>
+struct Patch<float> {
+    float v[8][8];
+    __device__ __forceinline__ void clear(int p) {
 #pragma unroll
-            for (int i = 0; i < 8; i += Elem<T>::kVec) load16<T>(src + i, v[p] + i);
+        for (int i = 0; i < 8; ++i) v[p][i] = 0.f;
+    }
+    __device__ __forceinline__ void load(int p, const float* src, int left, bool wide) {
+        if (wide) {
+            load16<float>(src, v[p]);
+            load16<float>(src + 4, v[p] + 4);
         } else {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[p][i] = c0 + i < a.C ? to_acc(src[i]) : 0.f;
+            for (int i = 0; i < 8; ++i) v[p][i] = i < left ? src[i] : 0.f;
+        }
+    }
+    __device__ __forceinline__ float2 pair(int p, int c) const { return make_float2(v[p][2 * c], v[p][2 * c + 1]); }
+    __device__ __forceinline__ void drop_infinite() {
+        float top = 0.f;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) top = fmaxf(top, largest<8>(v[p]));
+        if (!infinite(top)) return;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) drop_infinities<8>(v[p]);
+    }
+};
+template <>
+struct Patch<E4m3> {
+    uint2 w[8];
+    float s[8];
+    __device__ __forceinline__ void clear(int p) {
+        w[p] = make_uint2(0, 0);
+        s[p] = 0.f;
+    }
+    __device__ __forceinline__ void load(int p, const E4m3* src, int left, bool wide) {
+        if (wide) {
+            w[p] = __ldg(reinterpret_cast<const uint2*>(src));
+        } else {
+            uint32_t two[2] = {0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (i < left) two[i / 4] |= uint32_t(src[i].bits) << 8 * (i % 4);
+            w[p] = make_uint2(two[0], two[1]);
+        }
+    }
+    __device__ __forceinline__ float2 pair(int p, int c) const {
+        const uint32_t two = c < 2 ? w[p].x : w[p].y;
+        const float2 f = from_e4m3x2(two >> 16 * (c % 2));
+        return make_float2(f.x * s[p], f.y * s[p]);
+    }
+    __device__ __forceinline__ void drop_infinite() {}
+};
+
+// A thread holds rows 8 ty .. 8 ty + 7 of the tile and columns 8 tx .. 8 tx + 7 (tx < 16).
+template <typename T, bool WHOLE>
+__device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, float (&red)[16][kBlock8],
+                                         uint8_t* turned) {
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
+    const long long mb = tile / a.CB;
+    const int cb = int(tile - mb * a.CB);
+    const long long r0 = mb * kBlock8 + ty * 8;
+    const int c0 = cb * kBlock8 + tx * 8;
+    Patch<T> v;
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        v.clear(p);
+        if (r0 + p < a.M && c0 < a.C) {
+            v.load(p, static_cast<const T*>(a.x) + (r0 + p) * a.ld + c0, a.C - c0, a.wide);
+            if constexpr (sizeof(T) == 1) v.s[p] = __ldg(a.x_scale + (r0 + p) * a.CB + cb);
         }
     }
     if (a.sums != nullptr) {  // a thread's rows in order, then the 16 groups of rows in order
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float sum = v[0][i];
+        for (int c = 0; c < 4; ++c) {
+            float2 sum = v.pair(0, c);
 #pragma unroll
-            for (int p = 1; p < 8; ++p) sum += v[p][i];
-            red[ty][tx * 8 + i] = sum;
+            for (int p = 1; p < 8; ++p) {
+                const float2 f = v.pair(p, c);
+                sum.x += f.x;
+                sum.y += f.y;
+            }
+            *reinterpret_cast<float2*>(&red[ty][tx * 8 + 2 * c]) = sum;
         }
         __syncthreads();
         const int c = cb * kBlock8 + threadIdx.x;
@@ -247,15 +329,31 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
         }
         __syncthreads();
     }
-    if (infinite(largest<64>(v[0]))) drop_infinities<64>(v[0]);
+    v.drop_infinite();
     auto pack_row = [&](int p, float inv) {
         if (r0 + p >= a.M || c0 >= a.q_pitch) return;
-        *reinterpret_cast<uint2*>(a.q + (r0 + p) * a.q_pitch + c0) =
-            make_uint2(to_e4m3x4(v[p], inv), to_e4m3x4(v[p] + 4, inv));
+        uint32_t w[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float2 f = v.pair(p, c);
+            w[c] = to_e4m3x2(f.x, f.y, inv);
+        }
+        *reinterpret_cast<uint2*>(a.q + (r0 + p) * a.q_pitch + c0) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
+    };
+    auto row_top = [&](int p) {
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float2 f = v.pair(p, c);
+            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+        return top;
     };
     float tile_inv = 0.f;
-    if constexpr (TILE) {
-        float top = largest<64>(v[0]);
+    if constexpr (WHOLE) {
+        float top = 0.f;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) top = fmaxf(top, row_top(p));
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = top;
@@ -275,7 +373,7 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
     } else if (a.q != nullptr) {
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
-            float top = largest<8>(v[p]);
+            float top = row_top(p);
 #pragma unroll
             for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
             const int e = scale_exponent(top);
@@ -284,17 +382,17 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
         }
     }
     if (a.qt == nullptr) return;
-    float inv[8];
-    if constexpr (TILE) {
+    if constexpr (!WHOLE) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) inv[i] = tile_inv;
-    } else {
+        for (int c = 0; c < 4; ++c) {
+            float2 top = make_float2(0.f, 0.f);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            float top = 0.f;
-#pragma unroll
-            for (int p = 0; p < 8; ++p) top = fmaxf(top, fabsf(v[p][i]));
-            red[ty][tx * 8 + i] = top;
+            for (int p = 0; p < 8; ++p) {
+                const float2 f = v.pair(p, c);
+                top.x = fmaxf(top.x, fabsf(f.x));
+                top.y = fmaxf(top.y, fabsf(f.y));
+            }
+            *reinterpret_cast<float2*>(&red[ty][tx * 8 + 2 * c]) = top;
         }
         __syncthreads();
         if (threadIdx.x < kBlock8) {
@@ -306,18 +404,30 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
             red[0][threadIdx.x] = exp2_int(-e);
         }
         __syncthreads();
-#pragma unroll
-        for (int i = 0; i < 8; ++i) inv[i] = red[0][tx * 8 + i];
     }
     // the transpose through shared memory: row c of `turned` is column c of the tile, its 8-byte pieces exchanged by
     // xor with (c / 8), so that the 16 threads of a group of rows write to all banks
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        float col[8];
+    for (int c = 0; c < 4; ++c) {
+        float2 inv = make_float2(tile_inv, tile_inv);
+        if constexpr (!WHOLE) inv = *reinterpret_cast<const float2*>(&red[0][tx * 8 + 2 * c]);
+        uint32_t two[8];  // of each row: column 2c in the low byte, 2c + 1 above it
 #pragma unroll
-        for (int p = 0; p < 8; ++p) col[p] = v[p][i];
-        *reinterpret_cast<uint2*>(turned + (tx * 8 + i) * kBlock8 + ((ty ^ tx) << 3)) =
-            make_uint2(to_e4m3x4(col, inv[i]), to_e4m3x4(col + 4, inv[i]));
+        for (int p = 0; p < 8; ++p) {
+            const float2 f = v.pair(p, c);
+            two[p] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv.x, f.y * inv.y), __NV_SATFINITE, __NV_E4M3);
+        }
+        uint32_t lo[2], hi[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const uint32_t a01 = __byte_perm(two[4 * h], two[4 * h + 1], 0x5140);  // bytes: c of 0, 1; c + 1 of 0, 1
+            const uint32_t a23 = __byte_perm(two[4 * h + 2], two[4 * h + 3], 0x5140);
+            lo[h] = __byte_perm(a01, a23, 0x5410);
+            hi[h] = __byte_perm(a01, a23, 0x7632);
+        }
+        uint8_t* dst = turned + (tx * 8 + 2 * c) * kBlock8 + ((ty ^ tx) << 3);
+        *reinterpret_cast<uint2*>(dst) = make_uint2(lo[0], lo[1]);
+        *reinterpret_cast<uint2*>(dst + kBlock8) = make_uint2(hi[0], hi[1]);
     }
     __syncthreads();
     for (int i = threadIdx.x; i < kBlock8 * 8; i += kTileThreads) {
@@ -328,6 +438,24 @@ __global__ void __launch_bounds__(kTileThreads) fp8_tile_kernel(const TileArgs a
         if (turn & 1) w = make_uint4(w.z, w.w, w.x, w.y);
         *reinterpret_cast<uint4*>(a.qt + (long long)(cb * kBlock8 + c) * a.qt_pitch + at) = w;
     }
+}
+
+// Tile blockIdx.x of the jobs' tiles, one job's behind the other's: what a training pass lays out is one launch.
+template <typename T>
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : 3)
+    fp8_tile_kernel(const __grid_constant__ TileJobs jobs) {
+    __shared__ __align__(16) float red[16][kBlock8];
+    __shared__ __align__(16) uint8_t turned[kBlock8 * kBlock8];
+    grid_dependency_wait();
+    launch_dependents();
+    long long tile = blockIdx.x, before = 0;
+    int j = 0;
+    while (tile >= jobs.job[j].end) before = jobs.job[j++].end;
+    const TileArgs& a = jobs.job[j];
+    tile -= before;
+    if (a.kind == kTileBlocks) tile_job<T, false>(a, tile, red, turned);
+    else if (a.kind == kTileWhole) tile_job<T, true>(a, tile, red, turned);
+    else tile_job<E4m3, false>(a, tile, red, turned);
 }
 
 // out[c] = the partial rows [parts][C] added in order: each thread adds every kColumnRows-th part of one column, then
