@@ -491,15 +491,8 @@ int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void
     if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     TileJobs jobs = {};
-    TileArgs &xs = jobs.job[0], &w = jobs.job[1];
-    xs.kind = kTileBlocks;
-    xs.x = x;
-    xs.ld = K;
-    xs.q = static_cast<uint8_t*>(q);
-    xs.scale = scale;
-    xs.M = M;
-    xs.q_pitch = q_pitch;
-    xs.C = int(K);
+    int count = 0;
+    TileArgs& w = jobs.job[count++];
     w.kind = kTileWhole;
     w.x = weight;
     w.ld = K;
@@ -508,7 +501,21 @@ int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void
     w.M = N;
     w.q_pitch = up(K, 16);
     w.C = int(K);
-    if (int rc = launch_tiles(dtype, jobs, 2, s, err, err_len)) return rc;
+    // Many rows by the kernel for rows (67200 x 256: 5.6 us for this one's 15), few with the weight in one launch.
+    if (M * K >= int64_t(4) << 20) {
+        if (int rc = launch_rows(dtype, x, static_cast<uint8_t*>(q), q_pitch, scale, M, K, s, err, err_len)) return rc;
+    } else {
+        TileArgs& xs = jobs.job[count++];
+        xs.kind = kTileBlocks;
+        xs.x = x;
+        xs.ld = K;
+        xs.q = static_cast<uint8_t*>(q);
+        xs.scale = scale;
+        xs.M = M;
+        xs.q_pitch = q_pitch;
+        xs.C = int(K);
+    }
+    if (int rc = launch_tiles(dtype, jobs, count, s, err, err_len)) return rc;
     const int64_t KB = blocks_of(K);
     const Operand8 a = {static_cast<const uint8_t*>(q), scale, q_pitch, KB, 1, 1};
     const Operand8 b = {p.w, p.w_scale, up(K, 16), KB, 1, kBlock8};

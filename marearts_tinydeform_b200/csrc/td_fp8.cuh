@@ -212,18 +212,45 @@ struct Patch {  // 16-bit types
         }
     }
     __device__ __forceinline__ float2 pair(int p, int c) const {
-        const uint32_t two = word(w[p], c);
+        return both(word(w[p], c));
+    }
+    // Maxima of packed magnitudes, of which a NaN counts for nothing.
+    static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+        using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+        const T2 m = __hmax2(*reinterpret_cast<const T2*>(&a), *reinterpret_cast<const T2*>(&b));
+        return *reinterpret_cast<const uint32_t*>(&m);
+    }
+    static __device__ __forceinline__ float2 both(uint32_t two) {
         if constexpr (std::is_same<T, __half>::value) return __half22float2(*reinterpret_cast<const __half2*>(&two));
         else return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&two));
+    }
+    __device__ __forceinline__ uint32_t row_max2(int p) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) m = max2(m, word(w[p], c) & 0x7FFF7FFFu);
+        return m;
+    }
+    // Largest magnitudes of rows 2h and 2h + 1 over the tile's columns (two rows to a shuffle).
+    __device__ __forceinline__ float2 row_tops(int h) const {
+        const uint32_t a = row_max2(2 * h), b = row_max2(2 * h + 1);
+        uint32_t m = max2(__byte_perm(a, b, 0x5410), __byte_perm(a, b, 0x7632));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) m = max2(m, __shfl_xor_sync(0xffffffffu, m, o));
+        return both(m);
+    }
+    // .. of columns 2c and 2c + 1 over the thread's rows
+    __device__ __forceinline__ float2 column_tops(int c) const {
+        uint32_t m = 0;
+#pragma unroll
+        for (int p = 0; p < 8; ++p) m = max2(m, word(w[p], c) & 0x7FFF7FFFu);
+        return both(m);
     }
     // infinities to NaN (0x7FFF is one in both types)
     __device__ __forceinline__ void drop_infinite() {
         constexpr uint32_t kInf = std::is_same<T, __half>::value ? 0x7C00u : 0x7F80u;
         uint32_t most = 0;
 #pragma unroll
-        for (int p = 0; p < 8; ++p)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) most = __vmaxu2(most, word(w[p], c) & 0x7FFF7FFFu);
+        for (int p = 0; p < 8; ++p) most = max2(most, row_max2(p));
         if ((most & 0xFFFFu) < kInf && most >> 16 < kInf) return;
 #pragma unroll
         for (int p = 0; p < 8; ++p) {
@@ -236,6 +263,34 @@ struct Patch {  // 16-bit types
         }
     }
 };
+// The same maxima through pair().
+template <typename P>
+__device__ __forceinline__ float2 patch_row_tops(const P& v, int h) {
+    float top[2];
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+        top[r] = 0.f;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const float2 f = v.pair(2 * h + r, c);
+            top[r] = fmaxf(top[r], fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], o));
+    }
+    return make_float2(top[0], top[1]);
+}
+template <typename P>
+__device__ __forceinline__ float2 patch_column_tops(const P& v, int c) {
+    float2 top = make_float2(0.f, 0.f);
+#pragma unroll
+    for (int p = 0; p < 8; ++p) {
+        const float2 f = v.pair(p, c);
+        top.x = fmaxf(top.x, fabsf(f.x));
+        top.y = fmaxf(top.y, fabsf(f.y));
+    }
+    return top;
+}
 template <>
 struct Patch<float> {
     float v[8][8];
@@ -253,6 +308,8 @@ struct Patch<float> {
         }
     }
     __device__ __forceinline__ float2 pair(int p, int c) const { return make_float2(v[p][2 * c], v[p][2 * c + 1]); }
+    __device__ __forceinline__ float2 row_tops(int h) const { return patch_row_tops(*this, h); }
+    __device__ __forceinline__ float2 column_tops(int c) const { return patch_column_tops(*this, c); }
     __device__ __forceinline__ void drop_infinite() {
         float top = 0.f;
 #pragma unroll
@@ -286,6 +343,8 @@ struct Patch<E4m3> {
         const float2 f = from_e4m3x2(two >> 16 * (c % 2));
         return make_float2(f.x * s[p], f.y * s[p]);
     }
+    __device__ __forceinline__ float2 row_tops(int h) const { return patch_row_tops(*this, h); }
+    __device__ __forceinline__ float2 column_tops(int c) const { return patch_column_tops(*this, c); }
     __device__ __forceinline__ void drop_infinite() {}
 };
 
@@ -340,20 +399,14 @@ __device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, floa
         }
         *reinterpret_cast<uint2*>(a.q + (r0 + p) * a.q_pitch + c0) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
     };
-    auto row_top = [&](int p) {
-        float top = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float2 f = v.pair(p, c);
-            top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-        return top;
-    };
     float tile_inv = 0.f;
     if constexpr (WHOLE) {
         float top = 0.f;
 #pragma unroll
-        for (int p = 0; p < 8; ++p) top = fmaxf(top, row_top(p));
+        for (int c = 0; c < 4; ++c) {
+            const float2 f = v.column_tops(c);
+            top = fmaxf(top, fmaxf(f.x, f.y));
+        }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         if ((threadIdx.x & 31) == 0) red[0][threadIdx.x >> 5] = top;
@@ -372,28 +425,18 @@ __device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, floa
         }
     } else if (a.q != nullptr) {
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-            float top = row_top(p);
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-            const int e = scale_exponent(top);
-            if (tx == 0 && r0 + p < a.M) a.scale[(r0 + p) * a.CB + cb] = exp2_int(e);
-            pack_row(p, exp2_int(-e));
+        for (int h = 0; h < 4; ++h) {
+            const float2 top = v.row_tops(h);
+            const int e0 = scale_exponent(top.x), e1 = scale_exponent(top.y);
+            if (tx < 2 && r0 + 2 * h + tx < a.M) a.scale[(r0 + 2 * h + tx) * a.CB + cb] = exp2_int(tx == 0 ? e0 : e1);
+            pack_row(2 * h, exp2_int(-e0));
+            pack_row(2 * h + 1, exp2_int(-e1));
         }
     }
     if (a.qt == nullptr) return;
     if constexpr (!WHOLE) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            float2 top = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int p = 0; p < 8; ++p) {
-                const float2 f = v.pair(p, c);
-                top.x = fmaxf(top.x, fabsf(f.x));
-                top.y = fmaxf(top.y, fabsf(f.y));
-            }
-            *reinterpret_cast<float2*>(&red[ty][tx * 8 + 2 * c]) = top;
-        }
+        for (int c = 0; c < 4; ++c) *reinterpret_cast<float2*>(&red[ty][tx * 8 + 2 * c]) = v.column_tops(c);
         __syncthreads();
         if (threadIdx.x < kBlock8) {
             float top = red[0][threadIdx.x];
@@ -442,7 +485,7 @@ __device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, floa
 
 // Tile blockIdx.x of the jobs' tiles, one job's behind the other's: what a training pass lays out is one launch.
 template <typename T>
-__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : 3)
+__global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : 4)
     fp8_tile_kernel(const __grid_constant__ TileJobs jobs) {
     __shared__ __align__(16) float red[16][kBlock8];
     __shared__ __align__(16) uint8_t turned[kBlock8 * kBlock8];

@@ -43,7 +43,7 @@ struct Tc8Layout {
     static constexpr size_t kOutOffset = size_t(kStages) * kStageBytes;
     static constexpr size_t kScaleOffset = kOutOffset + kTc8Epi * kStageOut;
     static constexpr size_t kBiasOffset = kScaleOffset + (COLS ? size_t(kStages) * BN * 4 : 0);
-    static constexpr size_t kTopOffset = kBiasOffset + 2 * BN * 4;
+    static constexpr size_t kTopOffset = kBiasOffset + kTc8Epi * (BN / 2) * 4;
     static constexpr size_t kRingOffset = kTopOffset + 2 * kTc8Rows * 4;
     static constexpr size_t kBarOffset = kRingOffset + kTc8Ring * (kTc8Epi * 32 + kTc8Epi) * 4;
     static constexpr size_t kSlotOffset = kBarOffset + (4 * kStages + 2 * kBufs) * 8;
@@ -128,7 +128,6 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
     extern __shared__ __align__(16) unsigned char smem_raw[];
     unsigned char* smem = smem_raw + ((1024 - (smem_addr(smem_raw) & 1023)) & 1023);
     float* scales = reinterpret_cast<float*>(smem + Lay::kScaleOffset);
-    float* sbias = reinterpret_cast<float*>(smem + Lay::kBiasOffset);
     float* tops = reinterpret_cast<float*>(smem + Lay::kTopOffset);
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + Lay::kBarOffset);
     uint64_t *empty = full + S, *sfull = empty + S, *sempty = sfull + S, *tfull = sempty + S, *tempty = tfull + NB;
@@ -249,10 +248,9 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
         const int quarter = warp & 3, c_lo = warp / 4 * CW;
         const uint32_t lanes = tmem + (uint32_t(quarter * 32) << 16) + uint32_t(c_lo);
         unsigned char* const staged = smem + Lay::kOutOffset + warp * Lay::kStageOut;
-        const bool meet = kShare || a.end.bias != nullptr;
         const int n_blocks = (a.N + kBlock8 - 1) / kBlock8;
         bool dead = false;  // after a wait that gave up: walk on and meet at the barriers, but wait and store no more
-        int it = 0, turn = 0;
+        int it = 0;
         // The scales of the blocks ahead, over the tiles' borders: each thread copies its row's, and lane 0 the warp's
         // of B, into rings of their own. (Read where they are used, they cost more than all else: 262 us for the 136
         // of the same products without scales, at 8192 x 4096 x 4096.)
@@ -279,22 +277,36 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             }
             copy_commit();
         };
+        // the warp's columns of the bias, as they are in memory, on their way while a unit's products are added
+        unsigned char* const raw_bias = smem + Lay::kBiasOffset + warp * CW * 4;
+        const int bias_shift = a.end.bias_dtype == 0 ? 2 : 1;  // log2 of its bytes
+        const bool bias_words = (reinterpret_cast<uintptr_t>(a.end.bias) & 3) == 0;
+        auto fetch_bias = [&](int n) {
+            const char* const src = static_cast<const char*>(a.end.bias) + ((long long)n << bias_shift);
+            const int bytes = min(CW, a.N - n) << bias_shift;  // (none behind the last column)
+            for (int i = lane * 4; i < bytes; i += 128) {
+                if (bias_words && i + 4 <= bytes) {
+                    copy4(smem_addr(raw_bias + i), src + i);
+                } else {  // (a float32 bias comes in words)
+                    *reinterpret_cast<uint16_t*>(raw_bias + i) = *reinterpret_cast<const uint16_t*>(src + i);
+                    if (i + 4 <= bytes)
+                        *reinterpret_cast<uint16_t*>(raw_bias + i + 2) =
+                            *reinterpret_cast<const uint16_t*>(src + i + 2);
+                }
+            }
+            copy_commit();
+        };
         grid_dependency_wait();
 #pragma unroll
         for (int i = 0; i < kTc8Ring - 1; ++i) fetch();
-        for (int unit = blockIdx.x; unit < units; unit += gridDim.x, turn ^= 1) {
+        for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
             int m0, n0;
             tile_of(unit, m0, n0);
             const int row = quarter * 32 + lane, m = m0 + row, n = n0 + c_lo;
             const int count = count_kb(unit);
-            float* const bias = sbias + turn * BN;
-            if (meet) {  // (whoever writes a half again has passed the barrier of the unit between)
-                if (a.end.bias != nullptr) {
-                    for (int i = threadIdx.x; i < BN; i += kTc8Epi * 32)
-                        bias[i] = n0 + i < a.N ? bias_at(a.end, n0 + i) : 0.f;
-                }
-                named_barrier(1, kTc8Epi * 32);
-            }
+            const bool biased = a.end.bias != nullptr;
+            __syncwarp();
+            if (biased) fetch_bias(n);
             Pair8 acc[CW / 2];
 #pragma unroll
             for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
@@ -351,7 +363,6 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 }
             }
             // the end: bias, activation, and the row's CW columns out
-            const bool bias_there = a.end.bias != nullptr;
             float v[CW];
 #pragma unroll
             for (int i = 0; i < CW; i += 2) {
@@ -359,12 +370,32 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 v[i] = p.x;
                 v[i + 1] = p.y;
             }
-            if (bias_there) {
+            // the boxes of the unit before have been read (they are written again from here on)
+            if (lane < 2) bulk_wait_read();
+            __syncwarp();
+            if (biased) {
+                // of the groups of copies, those behind the bias's are the blocks' scales ahead, one a block
+                if (count > 1) copy_wait<2>();
+                else copy_wait<1>();
+                __syncwarp();
+                float* const wide = reinterpret_cast<float*>(staged);
+#pragma unroll
+                for (int i = lane; i < CW; i += 32) {
+                    float f = 0.f;
+                    if (n + i < a.N) {
+                        if (a.end.bias_dtype == 0) f = reinterpret_cast<const float*>(raw_bias)[i];
+                        else if (a.end.bias_dtype == 1) f = to_acc(reinterpret_cast<const __half*>(raw_bias)[i]);
+                        else f = to_acc(reinterpret_cast<const __nv_bfloat16*>(raw_bias)[i]);
+                    }
+                    wide[i] = f;
+                }
+                __syncwarp();
 #pragma unroll
                 for (int i = 0; i < CW; i += 4) {
-                    const float4 c = *reinterpret_cast<const float4*>(bias + c_lo + i);
+                    const float4 c = *reinterpret_cast<const float4*>(wide + i);
                     v[i] += c.x; v[i + 1] += c.y; v[i + 2] += c.z; v[i + 3] += c.w;
                 }
+                __syncwarp();
             }
             if (a.end.act == kActRelu) {
 #pragma unroll
@@ -389,6 +420,7 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     top = largest<CW>(v);
                 }
                 if constexpr (kShare) {
+                    named_barrier(1, kTc8Epi * 32);  // (the unit before's are read)
                     tops[(warp / 4) * kTc8Rows + row] = top;
                     named_barrier(1, kTc8Epi * 32);
                     top = fmaxf(top, tops[(1 - warp / 4) * kTc8Rows + row]);
@@ -398,8 +430,6 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 if (stores && n < a.N && n % kBlock8 == 0)
                     a.end.scale[(long long)m * n_blocks + n / kBlock8] = exp2_int(e);
                 if constexpr (CW == kBlock8) {  // a row of 128 bytes: the warp's one box
-                    if (lane == 0) bulk_wait_read();
-                    __syncwarp();
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
                         uint4 w;
@@ -428,8 +458,10 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 constexpr int kBoxCols = 128 / sizeof(T), kBoxes = CW / kBoxCols, kOnce = BN == 256 ? 2 : 1;
 #pragma unroll
                 for (int h = 0; h < kBoxes; h += kOnce) {
-                    if (lane < kOnce) bulk_wait_read();
-                    __syncwarp();
+                    if (h > 0) {
+                        if (lane < kOnce) bulk_wait_read();
+                        __syncwarp();
+                    }
 #pragma unroll
                     for (int o = 0; o < kOnce; ++o)
 #pragma unroll
