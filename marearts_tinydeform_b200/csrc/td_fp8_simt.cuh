@@ -14,7 +14,11 @@ namespace td {
 enum Activation8 : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 
 __device__ __forceinline__ float activate(float v, int act) {
-    if (act == kActRelu) return v < 0.f ? 0.f : v;  // (a NaN stays one)
+    if (act == kActRelu) {  // a NaN stays one
+        float d;
+        asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(d) : "f"(v));
+        return d;
+    }
     if (act == kActGelu) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
     if (act == kActSilu) return __fdividef(v, 1.f + __expf(-v));  // (a few steps of float32 of |v|)
     return v;

@@ -6,7 +6,7 @@
 // its 128 products in TMEM, from zero, and the epilogue warps add that times the scales to float32 registers while the
 // tensor cores work on the next block in another part of TMEM. The scales are so any float32 numbers, and the tensor
 // cores' own sums are never longer than 128 products, however long K is. What bounds it: a 128 x 256 block takes the
-// tensor cores 512 cycles and the 8 epilogue warps (two a scheduler) 128 packed multiply-adds each, plus the reading of
+// tensor cores 512 cycles and the 8 epilogue warps (two a scheduler) 128 multiply-adds each, plus the reading of
 // 128 KB from TMEM; the 16-bit results' bytes where K is short.
 //
 // Persistent, one CTA an SM, output tiles of 128 x BN (columns fastest, so that the CTAs which share rows of A run
@@ -80,33 +80,6 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
                    "+r"(r[15])
                  :
                  : "memory");
-}
-
-using Pair8 = uint64_t;  // two floats
-__device__ __forceinline__ Pair8 pair_of(float lo, float hi) {
-    Pair8 d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
-    return d;
-}
-__device__ __forceinline__ Pair8 pair_bits(uint32_t lo, uint32_t hi) {
-    Pair8 d;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
-    return d;
-}
-__device__ __forceinline__ float2 pair_split(Pair8 a) {
-    float2 f;
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(a));
-    return f;
-}
-__device__ __forceinline__ Pair8 pair_fma(Pair8 a, Pair8 b, Pair8 c) {
-    Pair8 d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ Pair8 pair_mul(Pair8 a, Pair8 b) {
-    Pair8 d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
 }
 
 // 3-D tiled store of the box at (x, y, z) from shared memory; what lies outside the tensor is not written. x * element
@@ -307,9 +280,9 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             const bool biased = a.end.bias != nullptr;
             __syncwarp();
             if (biased) fetch_bias(n);
-            Pair8 acc[CW / 2];
+            float v[CW];
 #pragma unroll
-            for (int i = 0; i < CW / 2; ++i) acc[i] = 0;
+            for (int i = 0; i < CW; ++i) v[i] = 0.f;
             for (int kb = 0; kb < count; ++kb, ++it) {
                 copy_wait<kTc8Ring - 2>();
                 __syncwarp();
@@ -322,21 +295,21 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 dead = !__all_sync(0xffffffffu, ready);
                 if (dead) continue;
                 tc_fence_after();
-                const Pair8 ff = pair_of(f, f);
                 // a chunk of 16 columns is on its way from TMEM while the one before it is added
                 uint32_t v0[16], v1[16];
                 auto add = [&](int j, const uint32_t(&w)[16]) {
 #pragma unroll
                     for (int i = 0; i < 16; i += 4) {
-                        Pair8 f0 = ff, f1 = ff;
+                        float4 c = make_float4(f, f, f, f);
                         if constexpr (COLS) {
-                            const float4 c = *reinterpret_cast<const float4*>(scales + s * BN + c_lo + j + i);
-                            f0 = pair_mul(ff, pair_of(c.x, c.y));
-                            f1 = pair_mul(ff, pair_of(c.z, c.w));
+                            c = *reinterpret_cast<const float4*>(scales + s * BN + c_lo + j + i);
+                            c.x *= f; c.y *= f; c.z *= f; c.w *= f;
                         }
-                        Pair8 &a0 = acc[(j + i) / 2], &a1 = acc[(j + i) / 2 + 1];
-                        a0 = pair_fma(pair_bits(w[i], w[i + 1]), f0, a0);
-                        a1 = pair_fma(pair_bits(w[i + 2], w[i + 3]), f1, a1);
+                        float* const to = v + j + i;
+                        to[0] = fmaf(__uint_as_float(w[i]), c.x, to[0]);
+                        to[1] = fmaf(__uint_as_float(w[i + 1]), c.y, to[1]);
+                        to[2] = fmaf(__uint_as_float(w[i + 2]), c.z, to[2]);
+                        to[3] = fmaf(__uint_as_float(w[i + 3]), c.w, to[3]);
                     }
                 };
                 const uint32_t from = lanes + uint32_t(b * BN);
@@ -363,13 +336,6 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 }
             }
             // the end: bias, activation, and the row's CW columns out
-            float v[CW];
-#pragma unroll
-            for (int i = 0; i < CW; i += 2) {
-                const float2 p = pair_split(acc[i / 2]);
-                v[i] = p.x;
-                v[i + 1] = p.y;
-            }
             // the boxes of the unit before have been read (they are written again from here on)
             if (lane < 2) bulk_wait_read();
             __syncwarp();
