@@ -437,7 +437,8 @@ TD_API int td_rms_norm_backward(int dtype, const void* grad_y, const void* grad_
  *   x_scale [M, ceil(K / 128)]; weight [N, K] e4m3, rows w_pitch apart, in blocks of 128 x 128 with w_scale
  *   [ceil(N / 128), ceil(K / 128)]; bias [N] of bias_dtype or NULL; activation: enum td_activation;
  *   out: [M, N] of out_dtype, or TD_E4M3 as td_fp8_quantize writes it (out_pitch, out_scale [M, ceil(N / 128)]).
- *   workspace: td_fp8_linear_workspace_bytes(x_dtype, M, K, N) bytes.
+ *   workspace: td_fp8_linear_workspace_bytes(x_dtype, M, K, N, copy_x, copy_weight) bytes; copy_x (an 8-bit x),
+ *   copy_weight: its rows do not all start on 16-byte boundaries, so the call copies it to such.
  * td_fp8_linear_train: the same with a floating weight [N, K] (x, weight, bias and out of dtype), x's 8-bit copy written
  * into q and scale as td_fp8_quantize writes it: out = Q(x) Qw(weight)^T + bias, Q and Qw the roundings to 8 bits above.
  *   workspace: td_fp8_linear_train_workspace_bytes(M, K, N) bytes.
@@ -446,16 +447,18 @@ TD_API int td_rms_norm_backward(int dtype, const void* grad_y, const void* grad_
  *   grad_x = Q(grad_out) Qw(weight); grad_weight = Qc(grad_out)^T Qc(x), Qc: blocks of 128 rows of one column;
  *   grad_bias = sum over rows of grad_out (not rounded before). Each may be NULL. Sums are taken in a fixed order.
  *   workspace: td_fp8_linear_backward_workspace_bytes(M, K, N, whether each is wanted) bytes.
- * 0 <= M < 2^31, 1 <= K, N <= TD_MAX_FP8_WIDTH.
+ * 0 <= M <= TD_MAX_FP8_ROWS, 1 <= K, N <= TD_MAX_FP8_WIDTH.
  */
 #define TD_E4M3 4 /* a dtype of the td_fp8_* calls alone */
 #define TD_MAX_FP8_WIDTH 65536
+#define TD_MAX_FP8_ROWS 2147483392 /* 2^31 - 256 */
 enum td_activation { TD_ACT_NONE = 0, TD_ACT_RELU = 1, TD_ACT_GELU = 2, TD_ACT_SILU = 3 };
 TD_API int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* scale, int64_t M, int64_t K,
                            int tiles, void* stream, char* err, size_t err_len);
 TD_API int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* scale, void* out, int64_t M,
                              int64_t K, int tiles, void* stream, char* err, size_t err_len);
-TD_API size_t td_fp8_linear_workspace_bytes(int x_dtype, int64_t M, int64_t K, int64_t N);
+TD_API size_t td_fp8_linear_workspace_bytes(int x_dtype, int64_t M, int64_t K, int64_t N, int copy_x,
+                                            int copy_weight);
 TD_API int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_scale, const void* weight,
                          int64_t w_pitch, const float* w_scale, int bias_dtype, const void* bias, int activation,
                          int out_dtype, void* out, int64_t out_pitch, float* out_scale, int64_t M, int64_t K,

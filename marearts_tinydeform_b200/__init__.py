@@ -339,7 +339,7 @@ def quantize_fp8(x):
     """x [..., K] in 8 bits (e4m3), a scale for each 128 values along the last dimension: the pair (data, scale) of
     float8_e4m3fn [..., K] and float32 [..., ceil(K / 128)]; x is about data * scale.
 
-    x: float32, float16 or bfloat16, up to 65536 wide. Scales are powers of two, the smallest that bring a block's
+    x: float32, float16 or bfloat16, up to 65536 wide (and 2^31 - 256 rows). Scales are powers of two, the smallest that bring a block's
     largest finite magnitude to at most 448 (e4m3's largest); values are rounded to nearest, ties to even; infinities
     and NaN become NaN. data's rows start 16 bytes apart or a multiple of that, so it is a view where K is not one.
     """
@@ -371,6 +371,11 @@ def dequantize_fp8(data, scale, dtype):
     return _native.fp8_dequantize(data, scale, dtype, tiles)
 
 
+def _tensors(operand):
+    """An operand's tensors: itself, or a pair's."""
+    return (operand,) if isinstance(operand, torch.Tensor) else [t for t in operand if isinstance(t, torch.Tensor)]
+
+
 def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None):
     """activation(x @ weight.T + bias) with both operands in 8 bits (e4m3), over the last dimension of x; [..., N].
 
@@ -387,7 +392,7 @@ def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None
     grad_bias = the sum of g. Sums are taken in a fixed order. CUDA tensors run this library's kernels; CPU tensors
     linear_fp8_reference.
     """
-    grad = torch.is_grad_enabled() and _wants_grad(*(t for t in (x, weight, bias) if isinstance(t, torch.Tensor)))
+    grad = torch.is_grad_enabled() and _wants_grad(*_tensors(x), *_tensors(weight), bias)
     dtype = _native.check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad)
     cuda = (x if isinstance(x, torch.Tensor) else x[0]).is_cuda
     if cuda:

@@ -22,6 +22,7 @@ MAX_LEVEL_POINTS = 64
 MAX_CHANNELS = 8192
 MAX_HEAD_DIM = 128
 MAX_FP8_WIDTH = 65536
+MAX_FP8_ROWS = 2 ** 31 - 256
 FP8_BLOCK = 128  # values that share a scale, along an axis
 ACTIVATION_CODE = {None: 0, 'relu': 1, 'gelu': 2, 'silu': 3}
 ATTN_ROW_PAD = 128  # rows of the attention's lse hold Q rounded up to this
@@ -46,7 +47,7 @@ SIGNATURES = {
     'td_rms_norm_backward': (_ip, [_ip, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _vp, _sz, _vp, _cp, _sz]),
     'td_fp8_quantize': (_ip, [_ip, _vp, _vp, _i64, _vp, _i64, _i64, _ip, _vp, _cp, _sz]),
     'td_fp8_dequantize': (_ip, [_ip, _vp, _i64, _vp, _vp, _i64, _i64, _ip, _vp, _cp, _sz]),
-    'td_fp8_linear_workspace_bytes': (_sz, [_ip, _i64, _i64, _i64]),
+    'td_fp8_linear_workspace_bytes': (_sz, [_ip, _i64, _i64, _i64, _ip, _ip]),
     'td_fp8_linear': (_ip, [_ip, _vp, _i64, _vp, _vp, _i64, _vp, _ip, _vp, _ip, _ip, _vp, _i64, _vp, _i64, _i64, _i64,
                             _vp, _sz, _vp, _cp, _sz]),
     'td_fp8_linear_train_workspace_bytes': (_sz, [_i64, _i64, _i64]),
@@ -1069,29 +1070,24 @@ def check_fp8_pair(pair, what, tiles):
 
 
 def _fp8_rows(data):
-    """8-bit data [..., K] as rows an equal number of bytes apart, starting on 16-byte boundaries (a copy where they are
-    not), and that distance."""
+    """8-bit data [..., K] as rows an equal number of bytes apart (a dense copy where they are not), and that distance."""
     K = data.shape[-1]
-    pitch = -(-K // 16) * 16
-    if data.data_ptr() % 16 == 0:
-        if pitch == K and data.is_contiguous():
-            return data, K
-        step = span = None
-        good = data.stride(-1) == 1 or K == 1
-        for size, stride in zip(reversed(data.shape[:-1]), reversed(data.stride()[:-1])):
-            if size == 1:
-                continue
-            if step is None:
-                step = span = stride
-            good = good and stride == span
-            span *= size
+    if data.is_contiguous():
+        return data, K
+    step = span = None
+    good = data.stride(-1) == 1 or K == 1
+    for size, stride in zip(reversed(data.shape[:-1]), reversed(data.stride()[:-1])):
+        if size == 1:
+            continue
         if step is None:
-            step = pitch
-        if good and step >= K and step % 16 == 0:
-            return data, step
-    rows = data.new_zeros((*data.shape[:-1], pitch), dtype=torch.uint8)
-    rows[..., :K] = data.view(torch.uint8)
-    return rows, pitch
+            step = span = stride
+        good = good and stride == span
+        span *= size
+    if step is None:
+        step = -(-K // 16) * 16
+    if good and step >= K:
+        return data, step
+    return data.contiguous(), K
 
 
 def fp8_quantize(x, tiles=False):
@@ -1145,7 +1141,7 @@ def check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad):
     data, wide = (x[0] if x_pair else x), (weight[0] if w_pair else weight)
     if wide.shape[1] != data.shape[-1]:
         raise RuntimeError('weight must be [N, K] with K = the last dimension of x')
-    if data.numel() // data.shape[-1] > INT32_MAX:
+    if data.numel() // data.shape[-1] > MAX_FP8_ROWS:
         raise RuntimeError('too many rows')
     if not x_pair and not w_pair and x.dtype != weight.dtype:
         raise RuntimeError('a floating weight must have the dtype of x')
@@ -1217,7 +1213,10 @@ def linear_fp8_forward(x, weight, bias, activation, quantize, dtype):
         out = result = data.new_empty((*lead, N), dtype=dtype)
         out_pitch, out_scale, out_code = 0, None, DTYPE_CODE[dtype]
     if M:
-        ws_bytes = _linear_fp8_workspace(code, M, K, N)
+        # 8-bit operands whose rows do not start on 16-byte boundaries are copied to such by the call
+        ws_bytes = _linear_fp8_workspace(code, M, K, N,
+                                         code == TD_E4M3 and (x_pitch % 16 != 0 or data.data_ptr() % 16 != 0),
+                                         w_pitch % 16 != 0 or w.data_ptr() % 16 != 0)
         ws = data.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
         _launch(lib.td_fp8_linear, data.device, code, data.data_ptr(), x_pitch, _address(x_scale), w.data_ptr(),
                 w_pitch, w_scale.data_ptr(), 0 if b is None else DTYPE_CODE[b.dtype], _address(b),

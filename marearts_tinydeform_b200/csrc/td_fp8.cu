@@ -41,7 +41,8 @@ int by_type(int dtype, F f) {
 }
 
 int check_sizes(int64_t M, int64_t K, int64_t N, char* err, size_t err_len) {
-    if (M < 0 || M > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "rows must be between 0 and 2^31 - 1");
+    if (M < 0 || M > TD_MAX_FP8_ROWS)
+        return fail(err, err_len, TD_ERR_ARG, "rows must be between 0 and %d", TD_MAX_FP8_ROWS);
     if (K < 1 || K > TD_MAX_FP8_WIDTH || N < 1 || N > TD_MAX_FP8_WIDTH)
         return fail(err, err_len, TD_ERR_ARG, "widths must be between 1 and %d", TD_MAX_FP8_WIDTH);
     return TD_OK;
@@ -112,6 +113,16 @@ int launch_tiles(int dtype, TileJobs jobs, int count, cudaStream_t stream, char*
     });
 }
 
+// Copies rows [M, K] of 8-bit data to 16-byte boundaries; *q and *pitch are the rows' own, then the copy's.
+int launch_pitch(const uint8_t** q, long long* pitch, uint8_t* to, int64_t M, int64_t K, cudaStream_t stream,
+                 char* err, size_t err_len) {
+    const PitchArgs a = {*q, to, M, *pitch, up(K, 16), int(K)};
+    *q = to;
+    *pitch = up(K, 16);
+    const dim3 grid(unsigned(std::min<int64_t>((M * (up(K, 16) / 16) + 255) / 256, int64_t(kSms) * 8)));
+    return host::launch(err, err_len, "fp8_pitch_kernel", fp8_pitch_kernel, grid, dim3(256), 0, stream, true, a);
+}
+
 // ---- products ---------------------------------------------------------------------------------------------------
 
 int launch_simt(const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M, int64_t N, int64_t K,
@@ -162,7 +173,6 @@ size_t partial_floats(int64_t M, int64_t N, int64_t K) {
     return p.splits > 1 ? size_t(p.splits) * size_t(M) * size_t(N) : 0;
 }
 
-bool tc_operand(const Operand8& o) { return aligned(o.q, 16) && o.pitch % 16 == 0 && o.pitch < (1LL << 39); }
 
 int make_map8(CUtensorMap* map, const Operand8& o, int64_t rows, int64_t K, int box_rows, char* err, size_t err_len) {
     const CUresult r = host::encode_tiled_u8(map, o.q, uint64_t(K), uint64_t(rows), uint64_t(o.pitch), kBlock8,
@@ -243,12 +253,12 @@ int launch_tc(const TcPlan& p, const Operand8& a, const Operand8& b, const End8&
     return out_dtype == TD_E4M3 ? finish(E4m3()) : by_type(out_dtype, finish);
 }
 
-// partial: partial_floats(M, N, K) of them. (Products with a scale for each row of both operands, whose b.scale_row is
+// partial: partial_floats(M, N, K) of them. Operands start on 16-byte boundaries, as do their rows. (Products with a scale for each row of both operands, whose b.scale_row is
 // 1, have a result in a floating type, and scales a tile's width beyond N.)
 int launch_product(const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M, int64_t N,
                    int64_t K, float* partial, cudaStream_t stream, char* err, size_t err_len) {
     const TcPlan p = plan_tc(M, N, K);
-    if (host::best_policy() && p.fits && tc_operand(a) && tc_operand(b))
+    if (host::best_policy() && p.fits)
         return launch_tc(p, a, b, end, out_dtype, M, N, K, partial, stream, err, err_len);
     return launch_simt(a, b, end, out_dtype, M, N, K, stream, err, err_len);
 }
@@ -256,9 +266,8 @@ int launch_product(const Operand8& a, const Operand8& b, const End8& end, int ou
 // Products of up to 16 rows with a laid-out weight (td_fp8_few.cuh). x_dtype: what x comes in.
 constexpr int kFewMost = 16, kFewRounds = 8;  // rows, and of those that are still wider than 8 bits
 
-bool few_takes(int x_dtype, const void* x, int64_t x_pitch, const void* w, int64_t w_pitch, int64_t M) {
-    if (!host::best_policy() || M > kFewMost || !aligned(w, 16) || w_pitch % 16 != 0) return false;
-    return x_dtype == TD_E4M3 ? aligned(x, 16) && x_pitch % 16 == 0 : M <= kFewRounds;
+bool few_takes(int x_dtype, int64_t M) {
+    return host::best_policy() && M <= (x_dtype == TD_E4M3 ? kFewMost : kFewRounds);
 }
 
 int launch_few(int x_dtype, FewArgs a, int out_dtype, cudaStream_t stream, char* err, size_t err_len) {
@@ -292,20 +301,20 @@ int launch_few(int x_dtype, FewArgs a, int out_dtype, cudaStream_t stream, char*
     return x_dtype == TD_E4M3 ? from(E4m3()) : by_type(x_dtype, from);
 }
 
-// What a forward call keeps in its workspace: the input in 8 bits, where it comes wider, and a split product's parts.
+// What a forward call keeps in its workspace: the input in 8 bits, where it comes wider, 8-bit operands whose rows do
+// not start on 16-byte boundaries on such, and a split product's parts.
 struct LinearPlan {
-    uint8_t* q;
+    uint8_t *q, *w;
     float *scale, *partial;
     size_t bytes;
 };
 
-LinearPlan plan_linear(int x_dtype, int64_t M, int64_t K, int64_t N, void* workspace) {
+LinearPlan plan_linear(int x_dtype, int64_t M, int64_t K, int64_t N, bool copy_x, bool copy_w, void* workspace) {
     LinearPlan p = {};
     Cut cut(workspace);
-    if (x_dtype != TD_E4M3) {
-        p.q = cut.take<uint8_t>(M * up(K, 16));
-        p.scale = cut.take<float>(M * blocks_of(K));
-    }
+    if (x_dtype != TD_E4M3 || copy_x) p.q = cut.take<uint8_t>(M * up(K, 16));
+    if (x_dtype != TD_E4M3) p.scale = cut.take<float>(M * blocks_of(K));
+    if (copy_w) p.w = cut.take<uint8_t>(N * up(K, 16));
     p.partial = cut.take<float>(int64_t(partial_floats(M, N, K)));
     p.bytes = cut.used == 0 ? 0 : cut.bytes();
     return p;
@@ -422,10 +431,10 @@ int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* sc
     });
 }
 
-size_t td_fp8_linear_workspace_bytes(int x_dtype, int64_t M, int64_t K, int64_t N) {
+size_t td_fp8_linear_workspace_bytes(int x_dtype, int64_t M, int64_t K, int64_t N, int copy_x, int copy_weight) {
     using namespace td;
     if ((!wide_type(x_dtype) && x_dtype != TD_E4M3) || M <= 0 || check_sizes(M, K, N, nullptr, 0) != TD_OK) return 0;
-    return plan_linear(x_dtype, M, K, N, nullptr).bytes;
+    return plan_linear(x_dtype, M, K, N, copy_x != 0, copy_weight != 0, nullptr).bytes;
 }
 
 int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_scale, const void* weight,
@@ -448,26 +457,39 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
     if (x_dtype == TD_E4M3 && (x_scale == nullptr || x_pitch < K))
         return fail(err, err_len, TD_ERR_ARG, "an 8-bit input has scales, and rows that do not overlap");
     if (w_pitch < K) return fail(err, err_len, TD_ERR_ARG, "the weight's rows must not overlap");
-    const LinearPlan p = plan_linear(x_dtype, M, K, N, workspace);
+    if (std::max(w_pitch, x_dtype == TD_E4M3 ? x_pitch : 0) >= int64_t(1) << 39)
+        return fail(err, err_len, TD_ERR_ARG, "rows are too far apart");
+    const bool copy_x = x_dtype == TD_E4M3 && (!aligned(x, 16) || x_pitch % 16 != 0);
+    const bool copy_w = !aligned(weight, 16) || w_pitch % 16 != 0;
+    const LinearPlan p = plan_linear(x_dtype, M, K, N, copy_x, copy_w, workspace);
     if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t KB = blocks_of(K);
     const End8 end = {bias, out, out_scale, bias_dtype, activation, int(out_pitch)};
     Operand8 a = {static_cast<const uint8_t*>(x), x_scale, x_pitch, KB, 1, 1};
+    if (copy_x) {
+        if (int rc = launch_pitch(&a.q, &a.pitch, p.q, M, K, s, err, err_len)) return rc;
+    }
+    const uint8_t* w8 = static_cast<const uint8_t*>(weight);
+    if (copy_w) {
+        long long pitch = w_pitch;
+        if (int rc = launch_pitch(&w8, &pitch, p.w, N, K, s, err, err_len)) return rc;
+        w_pitch = pitch;
+    }
     auto few = [&](int dtype) {
-        const FewArgs f = {dtype == TD_E4M3 ? a.q : x, a.scale, static_cast<const uint8_t*>(weight), w_scale, end,
+        const FewArgs f = {dtype == TD_E4M3 ? a.q : x, a.scale, w8, w_scale, end,
                            a.pitch, w_pitch, int(M), int(N), int(K), int(KB), 0};
         return launch_few(dtype, f, out_dtype, s, err, err_len);
     };
-    if (few_takes(x_dtype, x, x_pitch, weight, w_pitch, M)) return few(x_dtype);
+    if (few_takes(x_dtype, M)) return few(x_dtype);
     if (x_dtype != TD_E4M3) {
         a.q = p.q;
         a.scale = p.scale;
         a.pitch = up(K, 16);
         if (int rc = launch_rows(x_dtype, x, p.q, a.pitch, p.scale, M, K, s, err, err_len)) return rc;
     }
-    if (few_takes(TD_E4M3, a.q, a.pitch, weight, w_pitch, M)) return few(TD_E4M3);
-    const Operand8 b = {static_cast<const uint8_t*>(weight), w_scale, w_pitch, KB, 1, kBlock8};
+    if (few_takes(TD_E4M3, M)) return few(TD_E4M3);
+    const Operand8 b = {w8, w_scale, w_pitch, KB, 1, kBlock8};
     return launch_product(a, b, end, out_dtype, M, N, K, p.partial, s, err, err_len);
 }
 

@@ -181,4 +181,30 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// ---- rows to 16-byte boundaries -----------------------------------------------------------------------------------
+
+struct PitchArgs {
+    const uint8_t* from;  // [M, from_pitch], anywhere
+    uint8_t* to;          // [M, to_pitch], 16-byte aligned, the pitch a multiple of 16; zeros behind K
+    long long M, from_pitch, to_pitch;
+    int K;
+};
+// A thread takes 16 bytes of a row.
+__global__ void __launch_bounds__(256) fp8_pitch_kernel(const PitchArgs a) {
+    const int per_row = int(a.to_pitch / 16);
+    const long long total = a.M * per_row, step = (long long)gridDim.x * 256;
+    grid_dependency_wait();
+    launch_dependents();
+    for (long long t = (long long)blockIdx.x * 256 + threadIdx.x; t < total; t += step) {
+        const long long row = t / per_row;
+        const int c = int(t - row * per_row) * 16;
+        const uint8_t* src = a.from + row * a.from_pitch + c;
+        uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            if (c + i < a.K) w[i / 4] |= uint32_t(__ldg(src + i)) << 8 * (i % 4);
+        *reinterpret_cast<uint4*>(a.to + row * a.to_pitch + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+}
+
 }  // namespace td

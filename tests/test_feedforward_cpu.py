@@ -133,6 +133,7 @@ def test_linear_refusals():
             (dict(quantize=True, dtype=torch.float32), 'no dtype'), (dict(dtype=torch.float64), 'dtype must be'),
             (dict(x=x.clone().requires_grad_()), 'gradients need'), (dict(x=x8, weight=wg, dtype=x.dtype),
                                                                     'gradients need'),
+            (dict(x=(x8[0], x8[1].clone().requires_grad_()), dtype=x.dtype), 'gradients need'),
             (dict(weight=wg, activation='relu'), 'plain product'), (dict(weight=wg, quantize=True), 'plain product'),
             (dict(weight=wg, dtype=torch.float16), 'plain product'), (dict(weight=wg, bias=b.half()), 'bias must'),
             (dict(x=x.to('meta')), 'same device')]:
@@ -177,12 +178,14 @@ def test_fp8_abi_refuses_before_any_launch(lib):
                                  out_pitch, out_scale, M, K, N, ws, ws_bytes, None, err, 256)
 
     for kw in (dict(x_dtype=3), dict(out_dtype=3), dict(bias=p, bias_dtype=4), dict(act=4), dict(act=-1), dict(M=-1),
-               dict(M=2 ** 31), dict(K=0), dict(N=0), dict(K=65537), dict(x=None), dict(w_pitch=127), dict(out=None),
+               dict(M=2 ** 31 - 255), dict(K=0), dict(N=0), dict(K=65537), dict(x=None), dict(w_pitch=127), dict(out=None),
                dict(x_dtype=4, x_pitch=128), dict(x_dtype=4, x_pitch=127, x_scale=p),
                dict(out_dtype=4, out_pitch=80, out_scale=p), dict(out_dtype=4, out_pitch=64)):
         assert linear(**kw) == 1, (kw, err.value)
     assert linear(M=0, x=None) == 0 and linear(ws=None) == 3 and linear(ws_bytes=8) == 3
-    assert lib.td_fp8_linear_workspace_bytes(3, 4, 128, 64) == 0
+    assert lib.td_fp8_linear_workspace_bytes(3, 4, 128, 64, 0, 0) == 0
+    assert lib.td_fp8_linear_workspace_bytes(4, 4, 128, 64, 0, 0) == 0
+    assert linear(w_pitch=136, ws=None) == 3 and linear(w_pitch=1 << 40) == 1
 
     def backward(dtype=0, g=p, x=p, x_pitch=128, w=p, M=4, K=128, N=64, ws=p, ws_bytes=big):
         return lib.td_fp8_linear_backward(dtype, g, x, x_pitch, p, w, p, p, p, M, K, N, ws, ws_bytes, None, err, 256)

@@ -174,6 +174,27 @@ def test_strides_and_shapes(policy):
     assert gx.shape == (0, 10, 264) and not gw.any()
 
 
+@pytest.mark.parametrize('M', (1, 3, 14, 40, 200))
+def test_operands_that_start_anywhere(policy, M):
+    """x, weight and bias one element behind a boundary, in wide and in 8-bit types."""
+    def shifted(t):
+        return torch.cat([t.new_zeros(1), t.reshape(-1)])[1:].view(t.shape)
+
+    def shifted8(t):
+        return shifted(t.contiguous().view(torch.uint8)).view(E4M3)
+
+    for dtype, K in ((torch.bfloat16, 256), (torch.float32, 136), (torch.float16, 131)):
+        x, w = normal(M, K, dtype=dtype), normal(200, K, dtype=dtype, seed=1)
+        b = normal(200, dtype=dtype, seed=2)
+        x8, w8 = quantize_fp8(x), quantize_weight_fp8(w)
+        want, want8 = linear_fp8(x8, w8, b, 'relu', dtype=dtype), linear_fp8(x8, w8, b, quantize=True)
+        for a in (x, shifted(x), x8, (shifted8(x8[0]), x8[1]), (x8[0].contiguous(), x8[1])):
+            for v in (w8, (shifted8(w8[0]), w8[1]), (w8[0].contiguous(), w8[1])):
+                assert torch.equal(linear_fp8(a, v, shifted(b), 'relu', dtype=dtype), want)
+                got8 = linear_fp8(a, v, shifted(b), quantize=True)
+                assert torch.equal(got8[0].float(), want8[0].float()) and torch.equal(got8[1], want8[1])
+
+
 @pytest.mark.parametrize('M', (1, 5, 200))
 def test_infinities_and_nan_stay_in_their_rows(policy, M):
     x, w = normal(M + 2, 300), normal(140, 300, seed=1)
@@ -190,7 +211,7 @@ def test_rows_behind_the_last_are_left_alone(policy):
     for M, N in ((5, 130), (130, 264), (300, 1024)):
         x, w8 = normal(M, 256, dtype=torch.bfloat16), quantize_weight_fp8(normal(N, 256, dtype=torch.bfloat16, seed=1))
         lib, big = _native.load(), torch.full((M + 140, N), 7.0, dtype=torch.bfloat16, device='cuda')
-        ws_bytes = lib.td_fp8_linear_workspace_bytes(_native.TD_BF16, M, 256, N)
+        ws_bytes = lib.td_fp8_linear_workspace_bytes(_native.TD_BF16, M, 256, N, 0, 0)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device='cuda')
         _native._launch(lib.td_fp8_linear, x.device, _native.TD_BF16, x.data_ptr(), 0, None, w8[0].data_ptr(),
                         256, w8[1].data_ptr(), 0, None, 0, _native.TD_BF16, big.data_ptr(), 0, None, M, 256, N,
