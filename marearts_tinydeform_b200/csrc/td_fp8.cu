@@ -270,33 +270,35 @@ bool few_takes(int x_dtype, int64_t M) {
     return host::best_policy() && M <= (x_dtype == TD_E4M3 ? kFewMost : kFewRounds);
 }
 
-int launch_few(int x_dtype, FewArgs a, int out_dtype, cudaStream_t stream, char* err, size_t err_len) {
+template <typename X, typename T, int TILES>
+int launch_few_of(const FewArgs& a, cudaStream_t stream, char* err, size_t err_len) {
     const unsigned ctas = unsigned((a.N + kFewRows - 1) / kFewRows);
+    constexpr size_t smem = few_smem<X, TILES>();
+    if constexpr (sizeof(T) == 1) {
+        constexpr auto kernel = fp8_few_to8_kernel<X, TILES>;
+        if (int rc = host::allow_smem<kernel>(smem + 16384, err, err_len)) return rc;
+        return host::launch(err, err_len, "fp8_few_to8_kernel", kernel, dim3((ctas + 7) / 8 * 8), dim3(kFewThreads), smem,
+                            stream, true, a);
+    } else {
+        constexpr auto kernel = fp8_few_kernel<X, T, TILES>;
+        if (int rc = host::allow_smem<kernel>(smem + 16384, err, err_len)) return rc;
+        return host::launch(err, err_len, "fp8_few_kernel", kernel, dim3(ctas), dim3(kFewThreads), smem, stream, true,
+                            a);
+    }
+}
+
+int launch_few(int x_dtype, FewArgs a, int out_dtype, cudaStream_t stream, char* err, size_t err_len) {
     auto from = [&](auto x) {
         using X = decltype(x);
-        if constexpr (sizeof(X) > 1) {
-            a.x_wide = a.K % Elem<X>::kVec == 0 && aligned(a.x, 16);
-        }
-        if (out_dtype == TD_E4M3) {
-            const dim3 grid((ctas + 7) / 8 * 8);
-            if constexpr (sizeof(X) == 1) {
-                if (a.M > 8)
-                    return host::launch(err, err_len, "fp8_few_to8_kernel", fp8_few_to8_kernel<X, 2>, grid,
-                                        dim3(kFewThreads), 0, stream, true, a);
-            }
-            return host::launch(err, err_len, "fp8_few_to8_kernel", fp8_few_to8_kernel<X, 1>, grid, dim3(kFewThreads),
-                                0, stream, true, a);
-        }
-        return by_type(out_dtype, [&](auto zero) {
+        if constexpr (sizeof(X) > 1) a.x_wide = a.K % Elem<X>::kVec == 0 && aligned(a.x, 16);
+        auto to = [&](auto zero) {
             using T = decltype(zero);
             if constexpr (sizeof(X) == 1) {
-                if (a.M > 8)
-                    return host::launch(err, err_len, "fp8_few_kernel", fp8_few_kernel<X, T, 2>, dim3(ctas),
-                                        dim3(kFewThreads), 0, stream, true, a);
+                if (a.M > 8) return launch_few_of<X, T, 2>(a, stream, err, err_len);
             }
-            return host::launch(err, err_len, "fp8_few_kernel", fp8_few_kernel<X, T, 1>, dim3(ctas),
-                                dim3(kFewThreads), 0, stream, true, a);
-        });
+            return launch_few_of<X, T, 1>(a, stream, err, err_len);
+        };
+        return out_dtype == TD_E4M3 ? to(E4m3()) : by_type(out_dtype, to);
     };
     return x_dtype == TD_E4M3 ? from(E4m3()) : by_type(x_dtype, from);
 }

@@ -3,7 +3,7 @@
 //   out[m, n] = act(sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in block kb} a[m, k] b[n, k] + bias[n])
 //
 // Bound by reading the weight, so its rows are spread over the whole GPU: a CTA takes 16 of them, and its 8 warps every
-// eighth block of K each, with the next block's bytes under way while one is multiplied. e4m3 numbers are exact in
+// eighth block of K each, with three blocks' bytes under way while one is multiplied. e4m3 numbers are exact in
 // float16, so the tensor cores take them as m16n8k16 fragments (16 weight rows by 8 of x) that are read straight from
 // memory: a thread's 16 bytes are four K steps' worth, in an order of K that both operands share. A block's sums start
 // from zero and enter float32 registers times its scales; the warps' sums are added in order.
@@ -40,19 +40,21 @@ __device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
     const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(two & 0xFFFFu), __NV_E4M3);
     return uint32_t(h.x) | uint32_t(h.y) << 16;
 }
-// The 16 bytes at p, or those of them before `left` with zeros behind.
-__device__ __forceinline__ uint4 load_bytes(const uint8_t* p, int left) {
-    if (left <= 0) return make_uint4(0, 0, 0, 0);
-    uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
-    if (left < 16) {
-        uint32_t* w = reinterpret_cast<uint32_t*>(&v);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int n = left - 4 * i;
-            w[i] &= n >= 4 ? 0xFFFFFFFFu : n <= 0 ? 0u : (1u << (8 * n)) - 1;
-        }
-    }
-    return v;
+// The 16 bytes at p to shared memory, or those of them before `left` with zeros behind.
+__device__ __forceinline__ void copy_bytes(uint32_t dst, const void* p, int left) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(p), "r"(min(max(left, 0), 16))
+                 : "memory");
+}
+
+// Pieces of 16 bytes a thread has of a block: 4 of the weight, 2 of each 8 rows of an 8-bit x.
+template <typename X, int TILES>
+constexpr int few_pieces() {
+    return 4 + (sizeof(X) == 1 ? 2 * TILES : 0);
+}
+constexpr int kFewStages = 4;
+template <typename X, int TILES>
+constexpr size_t few_smem() {
+    return size_t(kFewStages) * few_pieces<X, TILES>() * kFewThreads * 16;
 }
 
 template <typename X, typename T, int TILES>  // TILES of 8 rows of x
@@ -63,45 +65,64 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
     __shared__ __align__(16) float tops[8 * TILES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const int n0 = blockIdx.x * kFewRows;
-    struct Block {
-        uint4 w[2][2];           // weight rows g, g + 8: 16-byte pieces t and t + 4 of the block
-        uint4 x[TILES][kVecs];   // row g of x: the same values
-        float sx[TILES], sw;
-    };
+    const int blocks = n0 < a.N && warp < a.KB ? (a.KB - 1 - warp) / kFewWarps + 1 : 0;  // this warp's
     const uint8_t* w_row[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) w_row[i] = a.w + (long long)min(n0 + g + 8 * i, a.N - 1) * a.w_pitch;
     const float* w_scale = a.w_scale + (long long)(min(n0, a.N - 1) / kBlock8) * a.KB;
-    auto load_weight = [&](int kb, Block& b) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int k = kb * kBlock8 + (t + 4 * h) * 16;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) b.w[i][h] = load_bytes(w_row[i] + k, a.K - k);
-        }
-        b.sw = __ldg(w_scale + kb);
+    // Bytes go through shared memory, three blocks ahead: each thread copies its own pieces there (weight rows g and
+    // g + 8, pieces t and t + 4 of the block's 8; row g of an 8-bit x likewise) and reads them back, so no barrier is
+    // needed.
+    extern __shared__ __align__(16) unsigned char smem[];
+    constexpr int P = few_pieces<X, TILES>();
+    auto place = [&](int stage, int piece) {
+        return smem + ((stage * P + piece) * kFewThreads + threadIdx.x) * 16;
     };
-    auto load_x = [&](int kb, Block& b) {
+    auto issue = [&](int i) {
+        if (i < blocks) {
+            const int stage = i % kFewStages, kb = warp + i * kFewWarps;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int k = kb * kBlock8 + (t + 4 * h) * 16, left = a.K - k;
+#pragma unroll
+                for (int r = 0; r < 2; ++r)
+                    copy_bytes(smem_addr(place(stage, 2 * r + h)), left > 0 ? w_row[r] + k : w_row[r], left);
+                if constexpr (kFrom8) {
+#pragma unroll
+                    for (int n = 0; n < TILES; ++n) {
+                        const int m = n * 8 + g;
+                        const bool there = m < a.M && left > 0;
+                        const uint8_t* x = static_cast<const uint8_t*>(a.x);
+                        copy_bytes(smem_addr(place(stage, 4 + 2 * n + h)), there ? x + m * a.x_pitch + k : x,
+                                   there ? left : 0);
+                    }
+                }
+            }
+        }
+        copy_commit();
+    };
+    // scales and a wider x one block ahead, in registers
+    struct Ahead {
+        uint4 x[kFrom8 ? 1 : TILES][kFrom8 ? 1 : kVecs];
+        float sx[TILES], sw;
+    };
+    auto load = [&](int i, Ahead& b) {
+        if (i >= blocks) return;
+        const int kb = warp + i * kFewWarps;
+        b.sw = __ldg(w_scale + kb);
 #pragma unroll
         for (int n = 0; n < TILES; ++n) {
             const int m = n * 8 + g;
-            b.sx[n] = 0.f;
-#pragma unroll
-            for (int i = 0; i < kVecs; ++i) b.x[n][i] = make_uint4(0, 0, 0, 0);
-            if (m >= a.M) continue;
             if constexpr (kFrom8) {
-                b.sx[n] = __ldg(a.x_scale + (long long)m * a.KB + kb);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int k = kb * kBlock8 + (t + 4 * h) * 16;
-                    b.x[n][h] = load_bytes(static_cast<const uint8_t*>(a.x) + m * a.x_pitch + k, a.K - k);
-                }
+                b.sx[n] = m < a.M ? __ldg(a.x_scale + (long long)m * a.KB + kb) : 0.f;
             } else {
                 constexpr int V = Elem<X>::kVec;
 #pragma unroll
                 for (int i = 0; i < kVecs; ++i) {
                     const int k = kb * kBlock8 + (t + 4 * (i / (kVecs / 2))) * 16 + i % (kVecs / 2) * V;
                     const X* src = static_cast<const X*>(a.x) + (long long)m * a.K + k;
+                    b.x[n][i] = make_uint4(0, 0, 0, 0);
+                    if (m >= a.M) continue;
                     if (a.x_wide) {
                         if (k < a.K) b.x[n][i] = __ldg(reinterpret_cast<const uint4*>(src));
                     } else {
@@ -115,8 +136,14 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
         }
     };
     float acc[TILES][4] = {};
-    auto multiply = [&](Block& b) {
-        if constexpr (!kFrom8) {  // row g to 8 bits: its four lanes hold the whole block
+    auto multiply = [&](int stage, Ahead& b) {
+        uint4 x[TILES][2];
+        if constexpr (kFrom8) {
+#pragma unroll
+            for (int n = 0; n < TILES; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) x[n][h] = *reinterpret_cast<const uint4*>(place(stage, 4 + 2 * n + h));
+        } else {  // row g to 8 bits: its four lanes hold the whole block
 #pragma unroll
             for (int n = 0; n < TILES; ++n) {
                 constexpr int V = Elem<X>::kVec;
@@ -135,23 +162,25 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
                 b.sx[n] = exp2_int(e);
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
-                    b.x[n][h] = make_uint4(to_e4m3x4(v + 16 * h, inv), to_e4m3x4(v + 16 * h + 4, inv),
-                                           to_e4m3x4(v + 16 * h + 8, inv), to_e4m3x4(v + 16 * h + 12, inv));
+                    x[n][h] = make_uint4(to_e4m3x4(v + 16 * h, inv), to_e4m3x4(v + 16 * h + 4, inv),
+                                         to_e4m3x4(v + 16 * h + 8, inv), to_e4m3x4(v + 16 * h + 12, inv));
             }
         }
         float part[TILES][4] = {};
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-            const uint32_t w0[4] = {b.w[0][h].x, b.w[0][h].y, b.w[0][h].z, b.w[0][h].w};
-            const uint32_t w1[4] = {b.w[1][h].x, b.w[1][h].y, b.w[1][h].z, b.w[1][h].w};
+            const uint4 a0 = *reinterpret_cast<const uint4*>(place(stage, h));
+            const uint4 a1 = *reinterpret_cast<const uint4*>(place(stage, 2 + h));
+            const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
             for (int s = 0; s < 4; ++s) {
                 const uint32_t fa[4] = {e4m3x2_to_half2(w0[s]), e4m3x2_to_half2(w1[s]), e4m3x2_to_half2(w0[s] >> 16),
                                         e4m3x2_to_half2(w1[s] >> 16)};
 #pragma unroll
                 for (int n = 0; n < TILES; ++n) {
-                    const uint32_t x = s == 0 ? b.x[n][h].x : s == 1 ? b.x[n][h].y : s == 2 ? b.x[n][h].z : b.x[n][h].w;
-                    const uint32_t fb[2] = {e4m3x2_to_half2(x), e4m3x2_to_half2(x >> 16)};
+                    const uint4& q = x[n][h];
+                    const uint32_t four = s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w;
+                    const uint32_t fb[2] = {e4m3x2_to_half2(four), e4m3x2_to_half2(four >> 16)};
                     mma_16816(part[n], fa, fb);
                 }
             }
@@ -170,26 +199,22 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
     grid_dependency_wait();
     launch_dependents();
     {
-        Block b0, b1;
-        int kb = warp;
-        if (n0 < a.N && kb < a.KB) {
-            load_weight(kb, b0);
-            load_x(kb, b0);
-            for (; kb < a.KB; kb += 2 * kFewWarps) {
-                const int k1 = kb + kFewWarps, k2 = k1 + kFewWarps;
-                if (k1 < a.KB) {
-                    load_weight(k1, b1);
-                    load_x(k1, b1);
-                }
-                multiply(b0);
-                if (k1 >= a.KB) break;
-                if (k2 < a.KB) {
-                    load_weight(k2, b0);
-                    load_x(k2, b0);
-                }
-                multiply(b1);
-            }
+#pragma unroll
+        for (int i = 0; i < kFewStages - 1; ++i) issue(i);
+        Ahead b0, b1;
+        load(0, b0);
+        for (int i = 0; i < blocks; i += 2) {
+            copy_wait<kFewStages - 2>();
+            issue(i + kFewStages - 1);
+            load(i + 1, b1);
+            multiply(i % kFewStages, b0);
+            if (i + 1 >= blocks) break;
+            copy_wait<kFewStages - 2>();
+            issue(i + kFewStages);
+            load(i + 2, b0);
+            multiply((i + 1) % kFewStages, b1);
         }
+        copy_wait<0>();
     }
 #pragma unroll
     for (int n = 0; n < TILES; ++n) {
