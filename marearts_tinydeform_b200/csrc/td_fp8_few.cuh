@@ -29,16 +29,13 @@ struct FewArgs {
     int M, N, K, KB, x_wide;  // x_wide: rows of a wider x start on 16-byte boundaries
 };
 
-__device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], const uint32_t (&b)[2]) {
+__device__ __forceinline__ void mma_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                          uint32_t b0, uint32_t b1) {
     asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
         "{%0, %1, %2, %3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
-}
-__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two) {
-    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(__nv_fp8x2_storage_t(two & 0xFFFFu), __NV_E4M3);
-    return uint32_t(h.x) | uint32_t(h.y) << 16;
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 // The 16 bytes at p to shared memory, or those of them before `left` with zeros behind.
 __device__ __forceinline__ void copy_bytes(uint32_t dst, const void* p, int left) {
@@ -171,18 +168,11 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
         for (int h = 0; h < 2; ++h) {
             const uint4 a0 = *reinterpret_cast<const uint4*>(place(stage, h));
             const uint4 a1 = *reinterpret_cast<const uint4*>(place(stage, 2 + h));
-            const uint32_t w0[4] = {a0.x, a0.y, a0.z, a0.w}, w1[4] = {a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
-            for (int s = 0; s < 4; ++s) {
-                const uint32_t fa[4] = {e4m3x2_to_half2(w0[s]), e4m3x2_to_half2(w1[s]), e4m3x2_to_half2(w0[s] >> 16),
-                                        e4m3x2_to_half2(w1[s] >> 16)};
-#pragma unroll
-                for (int n = 0; n < TILES; ++n) {
-                    const uint4& q = x[n][h];
-                    const uint32_t four = s == 0 ? q.x : s == 1 ? q.y : s == 2 ? q.z : q.w;
-                    const uint32_t fb[2] = {e4m3x2_to_half2(four), e4m3x2_to_half2(four >> 16)};
-                    mma_16816(part[n], fa, fb);
-                }
+            for (int n = 0; n < TILES; ++n) {
+                const uint4& q = x[n][h];
+                mma_16832(part[n], a0.x, a1.x, a0.y, a1.y, q.x, q.y);
+                mma_16832(part[n], a0.z, a1.z, a0.w, a1.w, q.z, q.w);
             }
         }
 #pragma unroll
