@@ -263,11 +263,13 @@ int launch_product(const Operand8& a, const Operand8& b, const End8& end, int ou
     return launch_simt(a, b, end, out_dtype, M, N, K, stream, err, err_len);
 }
 
-// Products of up to 16 rows with a laid-out weight (td_fp8_few.cuh). x_dtype: what x comes in.
-constexpr int kFewMost = 16, kFewRounds = 8;  // rows, and of those that are still wider than 8 bits
-
-bool few_takes(int x_dtype, int64_t M) {
-    return host::best_policy() && M <= (x_dtype == TD_E4M3 ? kFewMost : kFewRounds);
+// Whether a product of M rows that come in x_dtype is one of few (td_fp8_few.cuh). Rows wider than 8 bits are rounded
+// there as long as they are short: every CTA does that again, at 0.5 us a row and 1024 of K, where a launch of its own
+// is 1.2 us on the GPU and 2.5 us of the host's time (1 x 1024 x 256: 1.75 us against 3.0; 1 x 4096 x 4096: 7.7 against
+// 6.9, 18 against 20 with the host; 4 x 4096 x 1024: 7.1 against 4.9).
+bool few_takes(int x_dtype, int64_t M, int64_t K) {
+    if (!host::best_policy()) return false;
+    return x_dtype == TD_E4M3 ? M <= kFewMost : M <= kFewWide && M * K <= 4096;
 }
 
 template <typename X, typename T, int TILES>
@@ -290,7 +292,7 @@ int launch_few_of(const FewArgs& a, cudaStream_t stream, char* err, size_t err_l
 int launch_few(int x_dtype, FewArgs a, int out_dtype, cudaStream_t stream, char* err, size_t err_len) {
     auto from = [&](auto x) {
         using X = decltype(x);
-        if constexpr (sizeof(X) > 1) a.x_wide = a.K % Elem<X>::kVec == 0 && aligned(a.x, 16);
+        a.x_wide = a.K % 4 == 0 && aligned(a.x, 4 * sizeof(X));
         auto to = [&](auto zero) {
             using T = decltype(zero);
             if constexpr (sizeof(X) == 1) {
@@ -483,14 +485,14 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
                            a.pitch, w_pitch, int(M), int(N), int(K), int(KB), 0};
         return launch_few(dtype, f, out_dtype, s, err, err_len);
     };
-    if (few_takes(x_dtype, M)) return few(x_dtype);
+    if (few_takes(x_dtype, M, K)) return few(x_dtype);
     if (x_dtype != TD_E4M3) {
         a.q = p.q;
         a.scale = p.scale;
         a.pitch = up(K, 16);
         if (int rc = launch_rows(x_dtype, x, p.q, a.pitch, p.scale, M, K, s, err, err_len)) return rc;
     }
-    if (few_takes(TD_E4M3, M)) return few(TD_E4M3);
+    if (few_takes(TD_E4M3, M, K)) return few(TD_E4M3);
     const Operand8 b = {w8, w_scale, w_pitch, KB, 1, kBlock8};
     return launch_product(a, b, end, out_dtype, M, N, K, p.partial, s, err, err_len);
 }

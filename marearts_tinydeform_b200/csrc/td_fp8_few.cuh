@@ -3,14 +3,16 @@
 //   out[m, n] = act(sum_kb sa[m, kb] sb[n / 128, kb] sum_{k in block kb} a[m, k] b[n, k] + bias[n])
 //
 // Bound by reading the weight, so its rows are spread over the whole GPU: a CTA takes 16 of them, and its 8 warps every
-// eighth block of K each, with three blocks' bytes under way while one is multiplied. e4m3 numbers are exact in
-// float16, so the tensor cores take them as m16n8k16 fragments (16 weight rows by 8 of x) that are read straight from
-// memory: a thread's 16 bytes are four K steps' worth, in an order of K that both operands share. A block's sums start
-// from zero and enter float32 registers times its scales; the warps' sums are added in order.
+// eighth block of K each, with three blocks' bytes under way while one is multiplied. The tensor cores take e4m3
+// fragments of m16n8k32 (16 weight rows by 8 of x): a thread's 16 bytes of a row are two K steps' worth, in an order of
+// K that both operands share, so fragments are what memory holds. (As float16 they would be converted, 48 numbers a
+// thread and block: 20.8 us for the 16.2 below.) A block's sums start from zero and enter float32 registers times its
+// scales; the warps' sums are added in order.
 //
-// x may be wider than 8 bits (X): each warp then rounds its own blocks, four lanes to a row, instead of another launch
-// before this one. An 8-bit result's blocks of 128 columns are the work of a cluster of 8 CTAs, which exchange their
-// rows' largest magnitudes.
+// Up to four short rows of x may be wider than 8 bits (X): each warp then rounds its own blocks instead of another
+// launch before this one. An 8-bit result's blocks of 128 columns are the work of a cluster of 8 CTAs, which exchange
+// their rows' largest magnitudes. One row, the weight from memory: 4096 x 4096 5.6 us (3.0 TB/s), 8192 x 8192 16.2
+// (4.1 TB/s); a weight in the L2, 1024 x 256, 1.7 us. 16 rows, 4096 x 4096: 9.1.
 #pragma once
 
 #include "td_fp8_simt.cuh"
@@ -18,6 +20,7 @@
 namespace td {
 
 constexpr int kFewThreads = 256, kFewWarps = 8, kFewRows = 16;  // rows of the weight
+constexpr int kFewMost = 16, kFewWide = 4;  // rows of x: in 8 bits, and wider
 
 struct FewArgs {
     const void* x;         // e4m3, rows x_pitch apart (16-byte aligned), or wider and dense
@@ -26,7 +29,7 @@ struct FewArgs {
     const float* w_scale;  // [NB, KB]
     End8 end;
     long long x_pitch, w_pitch;
-    int M, N, K, KB, x_wide;  // x_wide: rows of a wider x start on 16-byte boundaries
+    int M, N, K, KB, x_wide;  // x_wide: four values of a wider x are one aligned word
 };
 
 __device__ __forceinline__ void mma_16832(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -57,7 +60,7 @@ constexpr size_t few_smem() {
 template <typename X, typename T, int TILES>  // TILES of 8 rows of x
 __device__ __forceinline__ void few_rows(const FewArgs& a) {
     constexpr bool kFrom8 = sizeof(X) == 1, kTo8 = sizeof(T) == 1;
-    constexpr int kVecs = kFrom8 ? 2 : 2 * int(sizeof(X));  // 16-byte vectors of a thread's 32 values
+    constexpr int kWideRows = kFrom8 ? 1 : kFewWide;
     __shared__ float sums[kFewWarps][kFewRows][8 * TILES + 1];
     __shared__ __align__(16) float tops[8 * TILES];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -98,36 +101,33 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
         }
         copy_commit();
     };
-    // scales and a wider x one block ahead, in registers
+    // scales and a wider x (four neighbouring values of each row a lane) one block ahead, in registers
     struct Ahead {
-        uint4 x[kFrom8 ? 1 : TILES][kFrom8 ? 1 : kVecs];
+        X x[kWideRows][4];
         float sx[TILES], sw;
     };
     auto load = [&](int i, Ahead& b) {
         if (i >= blocks) return;
         const int kb = warp + i * kFewWarps;
         b.sw = __ldg(w_scale + kb);
+        if constexpr (kFrom8) {
 #pragma unroll
-        for (int n = 0; n < TILES; ++n) {
-            const int m = n * 8 + g;
-            if constexpr (kFrom8) {
+            for (int n = 0; n < TILES; ++n) {
+                const int m = n * 8 + g;
                 b.sx[n] = m < a.M ? __ldg(a.x_scale + (long long)m * a.KB + kb) : 0.f;
-            } else {
-                constexpr int V = Elem<X>::kVec;
+            }
+        } else {
+            const int k = kb * kBlock8 + lane * 4;
 #pragma unroll
-                for (int i = 0; i < kVecs; ++i) {
-                    const int k = kb * kBlock8 + (t + 4 * (i / (kVecs / 2))) * 16 + i % (kVecs / 2) * V;
-                    const X* src = static_cast<const X*>(a.x) + (long long)m * a.K + k;
-                    b.x[n][i] = make_uint4(0, 0, 0, 0);
-                    if (m >= a.M) continue;
-                    if (a.x_wide) {
-                        if (k < a.K) b.x[n][i] = __ldg(reinterpret_cast<const uint4*>(src));
-                    } else {
-                        X one[V];
+            for (int m = 0; m < kWideRows; ++m) {
+                if (m >= a.M) break;
+                const X* src = static_cast<const X*>(a.x) + (long long)m * a.K + k;
+                using Four = typename std::conditional<sizeof(X) == 4, uint4, uint2>::type;
+                if (a.x_wide && k < a.K) {
+                    *reinterpret_cast<Four*>(b.x[m]) = __ldg(reinterpret_cast<const Four*>(src));
+                } else {
 #pragma unroll
-                        for (int j = 0; j < V; ++j) one[j] = k + j < a.K ? src[j] : from_acc<X>(0.f);
-                        b.x[n][i] = *reinterpret_cast<const uint4*>(one);
-                    }
+                    for (int j = 0; j < 4; ++j) b.x[m][j] = !a.x_wide && k + j < a.K ? src[j] : from_acc<X>(0.f);
                 }
             }
         }
@@ -140,27 +140,29 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
             for (int n = 0; n < TILES; ++n)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) x[n][h] = *reinterpret_cast<const uint4*>(place(stage, 4 + 2 * n + h));
-        } else {  // row g to 8 bits: its four lanes hold the whole block
+        } else {  // a row at a time to 8 bits by the whole warp, and its pieces to the lanes that multiply them
+            x[0][0] = x[0][1] = make_uint4(0, 0, 0, 0);
+            b.sx[0] = 0.f;
 #pragma unroll
-            for (int n = 0; n < TILES; ++n) {
-                constexpr int V = Elem<X>::kVec;
-                float v[32];
+            for (int m = 0; m < kWideRows; ++m) {
+                if (m >= a.M) break;
+                float v[4];
 #pragma unroll
-                for (int i = 0; i < kVecs; ++i) unpack16<X>(b.x[n][i], v + i * V);
-                float top = largest<32>(v);
-                if (infinite(top)) {
-                    drop_infinities<32>(v);
-                    top = largest<32>(v);
-                }
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                for (int j = 0; j < 4; ++j) v[j] = to_acc(b.x[m][j]);
+                drop_infinities<4>(v);
+                float top = largest<4>(v);
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
                 const int e = scale_exponent(top);
-                const float inv = exp2_int(-e);
-                b.sx[n] = exp2_int(e);
+                const uint32_t four = to_e4m3x4(v, exp2_int(-e));
+                uint32_t w[8];
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-                    x[n][h] = make_uint4(to_e4m3x4(v + 16 * h, inv), to_e4m3x4(v + 16 * h + 4, inv),
-                                         to_e4m3x4(v + 16 * h + 8, inv), to_e4m3x4(v + 16 * h + 12, inv));
+                for (int j = 0; j < 8; ++j) w[j] = __shfl_sync(0xffffffffu, four, (j / 4) * 16 + 4 * t + j % 4);
+                if (g == m) {
+                    x[0][0] = make_uint4(w[0], w[1], w[2], w[3]);
+                    x[0][1] = make_uint4(w[4], w[5], w[6], w[7]);
+                    b.sx[0] = exp2_int(e);
+                }
             }
         }
         float part[TILES][4] = {};
