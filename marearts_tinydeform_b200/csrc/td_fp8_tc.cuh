@@ -50,13 +50,53 @@ struct Tc8Layout {
     static constexpr size_t kBytes = kSlotOffset + 16 + 1024;  // + alignment of the tiles
 };
 
-__device__ __forceinline__ void mma_f8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                       uint32_t accumulate) {
+// The issuing thread and the epilogue's warps go around once a block of K, and each instruction on the issuing thread's
+// way costs about six cycles: barriers are plain addresses here, descriptors a changing low and a constant high word.
+__device__ __forceinline__ bool mbar_try_at(uint32_t bar, uint32_t parity) {
+    uint32_t done;
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(done)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+// Wait for the phase with the given parity; false (and the error word set) after about a second.
+__device__ __forceinline__ bool mbar_wait_at(uint32_t bar, uint32_t parity, unsigned int err_code) {
+    if (mbar_try_at(bar, parity)) return true;
+    const long long t0 = clock64();
+    while (!mbar_try_at(bar, parity)) {
+        if (clock64() - t0 > kSpinLimitCycles) {
+            record_error(err_code);
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_commit_at(uint32_t bar) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// D[tmem] = (the first: , the others: +=) A B^T of the 4 K steps of a block; a_lo, b_lo: the low words of the tiles'
+// descriptors, whose K steps are 32 bytes apart.
+__device__ __forceinline__ void mma_f8_block(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi,
+                                             uint32_t idesc) {
+    asm volatile(
+        "{\n\t.reg .pred no, yes;\n\t.reg .b64 a, b;\n\t.reg .b32 x, y;\n\t"
+        "setp.ne.b32 no, %3, %3;\n\tsetp.eq.b32 yes, %3, %3;\n\t"
+        "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, no;\n\t"
+        "add.u32 x, %1, 2;\n\tadd.u32 y, %2, 2;\n\tmov.b64 a, {x, %3};\n\tmov.b64 b, {y, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, yes;\n\t"
+        "add.u32 x, %1, 4;\n\tadd.u32 y, %2, 4;\n\tmov.b64 a, {x, %3};\n\tmov.b64 b, {y, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, yes;\n\t"
+        "add.u32 x, %1, 6;\n\tadd.u32 y, %2, 6;\n\tmov.b64 a, {x, %3};\n\tmov.b64 b, {y, %3};\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %4, yes;\n\t}"
+        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc)
         : "memory");
 }
 
@@ -196,22 +236,30 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             if (lane == 0) {
                 // f32 accumulator, e4m3 (format 0) by e4m3, both K-major
                 constexpr uint32_t idesc = (1u << 4) | (uint32_t(BN >> 3) << 17) | (uint32_t(kTc8Rows >> 4) << 24);
-                int it = 0;
+                const uint64_t first = sdesc_sw128(smem_addr(smem));
+                const uint32_t hi = uint32_t(first >> 32), lo = uint32_t(first);
+                const uint32_t full0 = smem_addr(full), empty0 = smem_addr(empty), tfull0 = smem_addr(tfull),
+                               tempty0 = smem_addr(tempty);
+                uint32_t s = 0, b = 0, s_phase = 0, b_phase = 1;
                 bool ok = true;
                 for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
-                    for (int kb = count_kb(unit); kb > 0; --kb, ++it) {
-                        const int s = it % S, b = it % NB;
-                        ok = mbar_wait(&tempty[b], uint32_t((it / NB) & 1) ^ 1u, kErrSlotWait) &&
-                             mbar_wait(&full[s], uint32_t((it / S) & 1), kErrTmaWait);
+                    for (int kb = count_kb(unit); kb > 0; --kb) {
+                        ok = mbar_wait_at(tempty0 + 8 * b, b_phase, kErrSlotWait) &&
+                             mbar_wait_at(full0 + 8 * s, s_phase, kErrTmaWait);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint64_t da = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes));
-                        const uint64_t db = sdesc_sw128(smem_addr(smem + s * Lay::kStageBytes + Lay::kABytes));
-    #pragma unroll
-                        for (int k = 0; k < 4; ++k)
-                            mma_f8(tmem + uint32_t(b * BN), da + uint64_t(2 * k), db + uint64_t(2 * k), idesc, k != 0);
-                        mma_commit(&empty[s]);
-                        mma_commit(&tfull[b]);
+                        const uint32_t a_lo = lo + s * (Lay::kStageBytes >> 4);
+                        mma_f8_block(tmem + b * BN, a_lo, a_lo + (Lay::kABytes >> 4), hi, idesc);
+                        mma_commit_at(empty0 + 8 * s);
+                        mma_commit_at(tfull0 + 8 * b);
+                        if (++s == S) {
+                            s = 0;
+                            s_phase ^= 1;
+                        }
+                        if (++b == NB) {
+                            b = 0;
+                            b_phase ^= 1;
+                        }
                     }
                 }
             }
@@ -223,7 +271,9 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
         unsigned char* const staged = smem + Lay::kOutOffset + warp * Lay::kStageOut;
         const int n_blocks = (a.N + kBlock8 - 1) / kBlock8;
         bool dead = false;  // after a wait that gave up: walk on and meet at the barriers, but wait and store no more
-        int it = 0;
+        const uint32_t tfull0 = smem_addr(tfull), tempty0 = smem_addr(tempty), sfull0 = smem_addr(sfull),
+                       sempty0 = smem_addr(sempty);
+        uint32_t at_b = 0, b_phase = 0, at_s = 0, s_phase = 0, slot = 0;
         // The scales of the blocks ahead, over the tiles' borders: each thread copies its row's, and lane 0 the warp's
         // of B, into rings of their own. (Read where they are used, they cost more than all else: 262 us for the 136
         // of the same products without scales, at 8192 x 4096 x 4096.)
@@ -283,16 +333,24 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             float v[CW];
 #pragma unroll
             for (int i = 0; i < CW; ++i) v[i] = 0.f;
-            for (int kb = 0; kb < count; ++kb, ++it) {
+            for (int kb = 0; kb < count; ++kb) {
                 copy_wait<kTc8Ring - 2>();
                 __syncwarp();
-                const int slot = it % kTc8Ring;
                 const float f = ring_a[slot * kTc8Epi * 32] * (COLS ? 1.f : ring_b[slot * kTc8Epi]);
                 fetch();
-                const int b = it % NB, s = it % S;
-                bool ready = !dead && mbar_wait(&tfull[b], uint32_t((it / NB) & 1), kErrMmaWait);
-                if (COLS) ready = ready && mbar_wait(&sfull[s], uint32_t((it / S) & 1), kErrTmaWait);
+                const uint32_t b = at_b, s = at_s;  // TMEM buffer, slot of B's scales
+                bool ready = !dead && mbar_wait_at(tfull0 + 8 * b, b_phase, kErrMmaWait);
+                if (COLS) ready = ready && mbar_wait_at(sfull0 + 8 * s, s_phase, kErrTmaWait);
                 dead = !__all_sync(0xffffffffu, ready);
+                slot = (slot + 1) % kTc8Ring;
+                if (++at_b == NB) {
+                    at_b = 0;
+                    b_phase ^= 1;
+                }
+                if (COLS && ++at_s == S) {
+                    at_s = 0;
+                    s_phase ^= 1;
+                }
                 if (dead) continue;
                 tc_fence_after();
                 // a chunk of 16 columns is on its way from TMEM while the one before it is added
@@ -325,14 +383,14 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     } else {  // all of it is in registers
                         tc_fence_before();
                         __syncwarp();
-                        if (lane == 0) mbar_arrive(&tempty[b]);
+                        if (lane == 0) mbar_arrive_at(tempty0 + 8 * b);
                     }
                     add(j + 16, v1);
                     if (j + 32 < CW) tmem_ld_wait_for(v0);
                 }
                 if constexpr (COLS) {
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&sempty[s]);
+                    if (lane == 0) mbar_arrive_at(sempty0 + 8 * s);
                 }
             }
             // the end: bias, activation, and the row's CW columns out
