@@ -93,19 +93,18 @@ int launch_rows(int dtype, const void* x, uint8_t* q, int64_t pitch, float* scal
     });
 }
 
-// One launch of up to kTileJobs jobs; dtype: the floating type of those that read one.
-int launch_tiles(int dtype, TileJobs jobs, int count, cudaStream_t stream, char* err, size_t err_len) {
+// One launch of up to kTileJobs jobs (those with M > 0); dtype: the floating type of those that read one.
+int launch_tiles(int dtype, TileJobs jobs, cudaStream_t stream, char* err, size_t err_len) {
     int64_t tiles = 0;
-    for (int j = 0; j < count; ++j) {
-        TileArgs& a = jobs.job[j];
-        const int64_t e = a.kind == kTileFrom8 ? 1 : int64_t(type_bytes(dtype)), step = a.kind == kTileFrom8 ? 8 : 16;
+    for (int kind = 0; kind < kTileJobs; ++kind) {
+        TileArgs& a = jobs.job[kind];
+        const int64_t e = kind == kTileFrom8 ? 1 : int64_t(type_bytes(dtype)), step = kind == kTileFrom8 ? 8 : 16;
         a.CB = int(blocks_of(a.C));
         a.MB = int(blocks_of(a.M));
         a.wide = a.C % 8 == 0 && aligned(a.x, uintptr_t(step)) && a.ld * e % step == 0;
         tiles += int64_t(a.CB) * a.MB;
         a.end = tiles;
     }
-    for (int j = count; j < kTileJobs; ++j) jobs.job[j].end = tiles + 1;
     if (tiles > INT32_MAX) return fail(err, err_len, TD_ERR_ARG, "too many tiles");
     return by_type(dtype, [&](auto zero) {
         return host::launch(err, err_len, "fp8_tile_kernel", fp8_tile_kernel<decltype(zero)>, dim3(unsigned(tiles)),
@@ -400,8 +399,7 @@ int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* s
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (!tiles) return launch_rows(dtype, x, static_cast<uint8_t*>(q), q_pitch, scale, M, K, s, err, err_len);
     TileJobs jobs = {};
-    TileArgs& a = jobs.job[0];
-    a.kind = kTileWhole;
+    TileArgs& a = jobs.job[kTileWhole];
     a.x = x;
     a.ld = K;
     a.q = static_cast<uint8_t*>(q);
@@ -409,7 +407,7 @@ int td_fp8_quantize(int dtype, const void* x, void* q, int64_t q_pitch, float* s
     a.M = M;
     a.q_pitch = q_pitch;
     a.C = int(K);
-    return launch_tiles(dtype, jobs, 1, s, err, err_len);
+    return launch_tiles(dtype, jobs, s, err, err_len);
 }
 
 int td_fp8_dequantize(int dtype, const void* q, int64_t q_pitch, const float* scale, void* out, int64_t M, int64_t K,
@@ -520,9 +518,7 @@ int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void
     if (int rc = check_workspace(workspace, workspace_bytes, p.bytes, err, err_len)) return rc;
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     TileJobs jobs = {};
-    int count = 0;
-    TileArgs& w = jobs.job[count++];
-    w.kind = kTileWhole;
+    TileArgs& w = jobs.job[kTileWhole];
     w.x = weight;
     w.ld = K;
     w.q = p.w;
@@ -534,8 +530,7 @@ int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void
     if (M * K >= int64_t(4) << 20) {
         if (int rc = launch_rows(dtype, x, static_cast<uint8_t*>(q), q_pitch, scale, M, K, s, err, err_len)) return rc;
     } else {
-        TileArgs& xs = jobs.job[count++];
-        xs.kind = kTileBlocks;
+        TileArgs& xs = jobs.job[kTileBlocks];
         xs.x = x;
         xs.ld = K;
         xs.q = static_cast<uint8_t*>(q);
@@ -544,7 +539,7 @@ int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void
         xs.q_pitch = q_pitch;
         xs.C = int(K);
     }
-    if (int rc = launch_tiles(dtype, jobs, count, s, err, err_len)) return rc;
+    if (int rc = launch_tiles(dtype, jobs, s, err, err_len)) return rc;
     const int64_t KB = blocks_of(K);
     const Operand8 a = {static_cast<const uint8_t*>(q), scale, q_pitch, KB, 1, 1};
     const Operand8 b = {p.w, p.w_scale, up(K, 16), KB, 1, kBlock8};
@@ -584,9 +579,7 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
     const int64_t NB = blocks_of(N), MB = blocks_of(M);
     // all that is laid out, in one launch: the gradient (read once for all that follows) ..
     TileJobs jobs = {};
-    int count = 1;
-    TileArgs& g = jobs.job[0];
-    g.kind = kTileBlocks;
+    TileArgs& g = jobs.job[kTileBlocks];
     g.x = grad_out;
     g.ld = N;
     if (grad_x != nullptr) g.q = p.dy;
@@ -600,8 +593,7 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
     g.scale_t_pitch = p.n_pad;
     g.C = int(N);
     if (grad_weight != nullptr) {  // .. the kept input, in blocks of rows
-        TileArgs& x8 = jobs.job[count++];
-        x8.kind = kTileFrom8;
+        TileArgs& x8 = jobs.job[kTileFrom8];
         x8.x = x;
         x8.x_scale = x_scale;
         x8.ld = x_pitch;
@@ -613,8 +605,7 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         x8.C = int(K);
     }
     if (grad_x != nullptr) {  // .. and the weight's blocks, as the forward's, transposed
-        TileArgs& w = jobs.job[count++];
-        w.kind = kTileWhole;
+        TileArgs& w = jobs.job[kTileWhole];
         w.x = weight;
         w.ld = K;
         w.qt = p.wt;
@@ -623,7 +614,7 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         w.qt_pitch = up(N, 16);
         w.C = int(K);
     }
-    if (int rc = launch_tiles(dtype, jobs, count, s, err, err_len)) return rc;
+    if (int rc = launch_tiles(dtype, jobs, s, err, err_len)) return rc;
     if (grad_bias != nullptr) {
         const int rc = by_type(dtype, [&](auto zero) {
             using T = decltype(zero);

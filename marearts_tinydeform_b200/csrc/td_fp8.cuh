@@ -182,13 +182,13 @@ struct TileArgs {
     float* scale_t;          //   [MB, scale_t_pitch] (one for each column), or [CB, MB]
     float* sums;             // or null: [MB, C] sums over a tile's rows
     long long M, q_pitch, qt_pitch, scale_t_pitch;
-    int C, CB, MB, kind;
+    int C, CB, MB;
     int wide;                // rows of x start on 16-byte boundaries (8-byte ones for e4m3), C a multiple of 8
     long long end;           // of the launch's tiles, this job's and those before it
 };
 
 constexpr int kTileThreads = 256, kTileJobs = 3;
-struct TileJobs {  // independent jobs of one launch
+struct TileJobs {  // independent jobs of one launch, each kind's in its place (their arguments are then constants)
     TileArgs job[kTileJobs];
 };
 
@@ -213,6 +213,26 @@ struct Patch {  // 16-bit types
     }
     __device__ __forceinline__ float2 pair(int p, int c) const {
         return both(word(w[p], c));
+    }
+    // Columns 2c and 2c + 1 of row p times a pair of scales, as e4m3. bfloat16 has the exponents for the product, which
+    // is exact but for what e4m3 rounds to zero anyway; float16 goes through float32.
+    static constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+    using Scales = typename std::conditional<kBf16, __nv_bfloat162, float2>::type;
+    static __device__ __forceinline__ Scales scales(float x, float y) {
+        if constexpr (kBf16) return __floats2bfloat162_rn(x, y);
+        else return make_float2(x, y);
+    }
+    __device__ __forceinline__ uint32_t e4m3x2(int p, int c, const Scales& f) const {
+        const uint32_t two = word(w[p], c);
+        float2 v;
+        if constexpr (kBf16) {
+            v = __bfloat1622float2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&two), f));
+        } else {
+            v = both(two);
+            v.x *= f.x;
+            v.y *= f.y;
+        }
+        return __nv_cvt_float2_to_fp8x2(v, __NV_SATFINITE, __NV_E4M3);
     }
     // Maxima of packed magnitudes, of which a NaN counts for nothing.
     static __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
@@ -263,7 +283,16 @@ struct Patch {  // 16-bit types
         }
     }
 };
-// The same maxima through pair().
+// The same conversion and maxima through pair().
+struct PatchScales {
+    using Scales = float2;
+    static __device__ __forceinline__ float2 scales(float x, float y) { return make_float2(x, y); }
+};
+template <typename P>
+__device__ __forceinline__ uint32_t patch_e4m3x2(const P& v, int p, int c, float2 f) {
+    const float2 two = v.pair(p, c);
+    return __nv_cvt_float2_to_fp8x2(make_float2(two.x * f.x, two.y * f.y), __NV_SATFINITE, __NV_E4M3);
+}
 template <typename P>
 __device__ __forceinline__ float2 patch_row_tops(const P& v, int h) {
     float top[2];
@@ -292,7 +321,7 @@ __device__ __forceinline__ float2 patch_column_tops(const P& v, int c) {
     return top;
 }
 template <>
-struct Patch<float> {
+struct Patch<float> : PatchScales {
     float v[8][8];
     __device__ __forceinline__ void clear(int p) {
 #pragma unroll
@@ -308,6 +337,7 @@ struct Patch<float> {
         }
     }
     __device__ __forceinline__ float2 pair(int p, int c) const { return make_float2(v[p][2 * c], v[p][2 * c + 1]); }
+    __device__ __forceinline__ uint32_t e4m3x2(int p, int c, float2 f) const { return patch_e4m3x2(*this, p, c, f); }
     __device__ __forceinline__ float2 row_tops(int h) const { return patch_row_tops(*this, h); }
     __device__ __forceinline__ float2 column_tops(int c) const { return patch_column_tops(*this, c); }
     __device__ __forceinline__ void drop_infinite() {
@@ -320,7 +350,7 @@ struct Patch<float> {
     }
 };
 template <>
-struct Patch<E4m3> {
+struct Patch<E4m3> : PatchScales {
     uint2 w[8];
     float s[8];
     __device__ __forceinline__ void clear(int p) {
@@ -343,6 +373,7 @@ struct Patch<E4m3> {
         const float2 f = from_e4m3x2(two >> 16 * (c % 2));
         return make_float2(f.x * s[p], f.y * s[p]);
     }
+    __device__ __forceinline__ uint32_t e4m3x2(int p, int c, float2 f) const { return patch_e4m3x2(*this, p, c, f); }
     __device__ __forceinline__ float2 row_tops(int h) const { return patch_row_tops(*this, h); }
     __device__ __forceinline__ float2 column_tops(int c) const { return patch_column_tops(*this, c); }
     __device__ __forceinline__ void drop_infinite() {}
@@ -392,11 +423,9 @@ __device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, floa
     auto pack_row = [&](int p, float inv) {
         if (r0 + p >= a.M || c0 >= a.q_pitch) return;
         uint32_t w[4];
+        const auto f = v.scales(inv, inv);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-            const float2 f = v.pair(p, c);
-            w[c] = to_e4m3x2(f.x, f.y, inv);
-        }
+        for (int c = 0; c < 4; ++c) w[c] = v.e4m3x2(p, c, f);
         *reinterpret_cast<uint2*>(a.q + (r0 + p) * a.q_pitch + c0) = make_uint2(w[0] | w[1] << 16, w[2] | w[3] << 16);
     };
     float tile_inv = 0.f;
@@ -455,11 +484,9 @@ __device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, floa
         float2 inv = make_float2(tile_inv, tile_inv);
         if constexpr (!WHOLE) inv = *reinterpret_cast<const float2*>(&red[0][tx * 8 + 2 * c]);
         uint32_t two[8];  // of each row: column 2c in the low byte, 2c + 1 above it
+        const auto f = v.scales(inv.x, inv.y);
 #pragma unroll
-        for (int p = 0; p < 8; ++p) {
-            const float2 f = v.pair(p, c);
-            two[p] = __nv_cvt_float2_to_fp8x2(make_float2(f.x * inv.x, f.y * inv.y), __NV_SATFINITE, __NV_E4M3);
-        }
+        for (int p = 0; p < 8; ++p) two[p] = v.e4m3x2(p, c, f);
         uint32_t lo[2], hi[2];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -491,14 +518,13 @@ __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : 4)
     __shared__ __align__(16) uint8_t turned[kBlock8 * kBlock8];
     grid_dependency_wait();
     launch_dependents();
-    long long tile = blockIdx.x, before = 0;
-    int j = 0;
-    while (tile >= jobs.job[j].end) before = jobs.job[j++].end;
-    const TileArgs& a = jobs.job[j];
-    tile -= before;
-    if (a.kind == kTileBlocks) tile_job<T, false>(a, tile, red, turned);
-    else if (a.kind == kTileWhole) tile_job<T, true>(a, tile, red, turned);
-    else tile_job<E4m3, false>(a, tile, red, turned);
+    const long long tile = blockIdx.x;
+    if (tile < jobs.job[kTileBlocks].end)
+        tile_job<T, false>(jobs.job[kTileBlocks], tile, red, turned);
+    else if (tile < jobs.job[kTileWhole].end)
+        tile_job<T, true>(jobs.job[kTileWhole], tile - jobs.job[kTileBlocks].end, red, turned);
+    else
+        tile_job<E4m3, false>(jobs.job[kTileFrom8], tile - jobs.job[kTileWhole].end, red, turned);
 }
 
 // out[c] = the partial rows [parts][C] added in order: each thread adds every kColumnRows-th part of one column, then
