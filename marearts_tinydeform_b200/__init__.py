@@ -317,7 +317,8 @@ def rms_norm(x, weight, residual=None, eps=1e-6, return_sum=False, quantize=Fals
     * weight, in x's shape and dtype.
 
     weight and residual have x's dtype and device. s is not rounded before the norm, and the mean is float32 (float64
-    for float64). return_sum: the pair (result, s), s being what the next layer adds to. quantize: the result in 8 bits,
+    for float64), so squares have to stay in its range. return_sum: the pair (result, s), s being what the next layer
+    adds to. quantize: the result in 8 bits,
     as a pair (data, scale) like quantize_fp8's, rounded once; for calls without gradients, not for float64. CUDA
     tensors run this library's kernels, forward and backward (the weight's gradient summed in a fixed order); CPU
     tensors run rms_norm_reference.
@@ -390,7 +391,8 @@ def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None
     for it only in 8 bits; no activation, quantize or other dtype then. With Q the roundings to 8 bits, whose own
     derivative counts as 1: grad_x = Q(g) Q(weight), grad_weight = Q(g)^T Q(Q(x)), the last two in blocks of 128 rows,
     grad_bias = the sum of g. Sums are taken in a fixed order. CUDA tensors run this library's kernels; CPU tensors
-    linear_fp8_reference.
+    linear_fp8_reference. The backward can be captured in a CUDA graph with the forward; as with every autograd backward
+    under capture, no graph of the same leaves that was built outside the capture may be alive then.
     """
     grad = torch.is_grad_enabled() and _wants_grad(*_tensors(x), *_tensors(weight), bias)
     dtype = _native.check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad)

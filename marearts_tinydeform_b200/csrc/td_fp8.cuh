@@ -10,9 +10,13 @@
 // anywhere in the range. Blocks are 1 x 128 (activations: along the contraction), 128 x 1 (the same tensors when rows
 // are contracted, as in the weight's gradient) or 128 x 128 (weights, whose blocks stay blocks when transposed).
 //
-// fp8_rows_kernel (1 x 128 alone) reads a row in 16-byte vectors, 128 / VEC lanes to a block. fp8_tile_kernel takes
-// 128 x 128 values into registers, once, for any of: the 1 x 128 form, the 128 x 1 form transposed, the 128 x 128 form
-// or its transpose, and column sums. Both are bound by memory.
+// Rows alone (1 x 128) are bound by memory: fp8_flat_kernel, where blocks follow one another (K a multiple of 128),
+// takes 32 bytes a thread and runs at the copy rate (177784 x 1024 bfloat16 88 us, 6.2 TB/s; 177784 x 256 22.8; with
+// one 16-byte vector a thread and a division a task 143), fp8_rows_kernel any other rows (8800 x 515 float32 8 us).
+// fp8_tile_kernel takes 128 x 128 values into registers, once, for any of: the 1 x 128 form, the 128 x 1 form
+// transposed, the 128 x 128 form or its transpose, and column sums. It is bound by instructions (76 % of the issue
+// slots): what a training backward lays out at 67200 x 1024 and 67200 x 256, 309 MB, takes 79 us (3.9 TB/s; 103 from
+// float32 registers, in three launches).
 #pragma once
 
 #include <cuda_fp8.h>

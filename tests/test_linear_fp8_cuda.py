@@ -219,6 +219,28 @@ def test_rows_behind_the_last_are_left_alone(policy):
         assert (big[M:] == 7).all() and torch.equal(big[:M], linear_fp8(x, w8))
 
 
+def test_offsets_past_31_bits(cuda):
+    """Results and gradients of more than 2^31 values: the last rows, and a weight's gradient that only they feed."""
+    M, K, N, last = 530000, 128, 4096, 700
+    x, w = normal(M, K, dtype=torch.bfloat16), normal(N, K, dtype=torch.bfloat16, seed=1, std=K ** -0.5)
+    end = slice(M - last, M)
+    xd, wd = through(x[end], 1, 128), through(w, 128, 128)
+    y8, scale = linear_fp8(x, quantize_weight_fp8(w), quantize=True)
+    check_quantized((y8[end], scale[end]), product_exact(xd, wd, torch.bfloat16), '8-bit result')
+    del y8, scale
+    leaves = [x.requires_grad_(), w.requires_grad_()]
+    y = linear_fp8(*leaves)
+    check(y.detach()[end], product_exact(xd, wd, torch.bfloat16), 'y')
+    g = torch.zeros(M, N, dtype=torch.bfloat16, device='cuda')
+    first = M // 128 * 128 - 512  # from the beginning of a block of rows
+    g[first:] = normal(M - first, N, dtype=torch.bfloat16, seed=2)
+    gx, gw = torch.autograd.grad(y, leaves, g)
+    del y
+    check(gx[first:], product_exact(through(g[first:], 1, 128), wd.t(), torch.bfloat16), 'grad_x')
+    cols = through(g[first:], 128, 1).t(), through(through(x.detach()[first:], 1, 128), 128, 1).t()
+    check(gw, product_exact(*cols, torch.bfloat16), 'grad_weight')
+
+
 def test_same_bits_every_time(cuda):
     x, w, b = spread(2400, 256, torch.float16), normal(1024, 256, dtype=torch.float16, seed=1), \
         normal(1024, dtype=torch.float16, seed=2)

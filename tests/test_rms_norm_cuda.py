@@ -110,6 +110,23 @@ def test_either_output_alone(cuda):
         rms_norm(x8, w, quantize=True)
 
 
+def test_offsets_past_31_bits(cuda):
+    """More than 2^31 values: the last rows are the same rows' alone."""
+    rows, C = 2100000, 1024
+    x, w = torch.randn(rows, C, dtype=torch.bfloat16, device='cuda'), inputs(1, C, torch.bfloat16)[1]
+    part = x[-300:].clone()
+    with torch.inference_mode():
+        (data, scale), s = rms_norm(x, w, quantize=True, return_sum=True)
+        want = rms_norm(part, w, quantize=True)
+        assert torch.equal(data[-300:].float(), want[0].float()) and torch.equal(scale[-300:], want[1])
+        assert torch.equal(s[-300:], part)
+        del data, s
+    leaf = x.requires_grad_()
+    grad = torch.autograd.grad(rms_norm(leaf, w), leaf, x.detach())[0]
+    alone = part.requires_grad_()
+    assert torch.equal(grad[-300:], torch.autograd.grad(rms_norm(alone, w), alone, part.detach())[0])
+
+
 def test_same_bits_every_time(cuda):
     x, w, r, dy, ds = inputs(9000, 256, torch.float16, 3)
     first = run(x, w, r, dy, ds)
