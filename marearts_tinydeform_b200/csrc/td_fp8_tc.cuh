@@ -45,7 +45,8 @@ struct Tc8Layout {
     static constexpr size_t kOutOffset = size_t(kStages) * kStageBytes;
     static constexpr size_t kScaleOffset = kOutOffset + kTc8Epi * kStageOut;
     static constexpr size_t kBiasOffset = kScaleOffset + (COLS ? size_t(kStages) * BN * 4 : 0);
-    static constexpr size_t kTopOffset = kBiasOffset + kTc8Epi * (BN / 2) * 4;
+    // a warp's columns of the bias, as they come and as float32 (COLS: products without one)
+    static constexpr size_t kTopOffset = kBiasOffset + (COLS ? 0 : 2 * kTc8Epi * (BN / 2) * 4);
     static constexpr size_t kRingOffset = kTopOffset + 2 * kTc8Rows * 4;
     static constexpr size_t kBarOffset = kRingOffset + kTc8Ring * (kTc8Epi * 32 + kTc8Epi) * 4;
     static constexpr size_t kSlotOffset = kBarOffset + (4 * kStages + 2 * kBufs) * 8;
@@ -302,39 +303,70 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             }
             copy_commit();
         };
-        // the warp's columns of the bias, as they are in memory, on their way while a unit's products are added
+        // the warp's columns of the next unit's bias, as they are in memory, on their way while a unit's products are
+        // added; a unit's sums begin with them
+        const bool biased = !COLS && a.end.bias != nullptr;
         unsigned char* const raw_bias = smem + Lay::kBiasOffset + warp * CW * 4;
+        float* const wide_bias = reinterpret_cast<float*>(raw_bias + kTc8Epi * CW * 4);
         const int bias_shift = a.end.bias_dtype == 0 ? 2 : 1;  // log2 of its bytes
         const bool bias_words = (reinterpret_cast<uintptr_t>(a.end.bias) & 3) == 0;
-        auto fetch_bias = [&](int n) {
-            const char* const src = static_cast<const char*>(a.end.bias) + ((long long)n << bias_shift);
-            const int bytes = min(CW, a.N - n) << bias_shift;  // (none behind the last column)
-            for (int i = lane * 4; i < bytes; i += 128) {
-                if (bias_words && i + 4 <= bytes) {
-                    copy4(smem_addr(raw_bias + i), src + i);
-                } else {  // (a float32 bias comes in words)
-                    *reinterpret_cast<uint16_t*>(raw_bias + i) = *reinterpret_cast<const uint16_t*>(src + i);
-                    if (i + 4 <= bytes)
-                        *reinterpret_cast<uint16_t*>(raw_bias + i + 2) =
-                            *reinterpret_cast<const uint16_t*>(src + i + 2);
+        auto fetch_bias = [&](int next) {
+            if (next < units) {
+                int m0, n0;
+                tile_of(next, m0, n0);
+                const int n = n0 + c_lo;
+                const char* const src = static_cast<const char*>(a.end.bias) + ((long long)n << bias_shift);
+                const int bytes = min(CW, a.N - n) << bias_shift;  // (none behind the last column)
+                for (int i = lane * 4; i < bytes; i += 128) {
+                    if (bias_words && i + 4 <= bytes) {
+                        copy4(smem_addr(raw_bias + i), src + i);
+                    } else {  // (a float32 bias comes in words)
+                        *reinterpret_cast<uint16_t*>(raw_bias + i) = *reinterpret_cast<const uint16_t*>(src + i);
+                        if (i + 4 <= bytes)
+                            *reinterpret_cast<uint16_t*>(raw_bias + i + 2) =
+                                *reinterpret_cast<const uint16_t*>(src + i + 2);
+                    }
                 }
             }
             copy_commit();
         };
         grid_dependency_wait();
+        if (biased) fetch_bias(blockIdx.x);
 #pragma unroll
         for (int i = 0; i < kTc8Ring - 1; ++i) fetch();
+        int behind = kTc8Ring - 1;  // groups of copies behind the bias's
         for (int unit = blockIdx.x; unit < units; unit += gridDim.x) {
             int m0, n0;
             tile_of(unit, m0, n0);
             const int row = quarter * 32 + lane, m = m0 + row, n = n0 + c_lo;
             const int count = count_kb(unit);
-            const bool biased = a.end.bias != nullptr;
-            __syncwarp();
-            if (biased) fetch_bias(n);
             float v[CW];
+            if (biased) {
+                if (behind > 1) copy_wait<2>();
+                else copy_wait<1>();
+                __syncwarp();
 #pragma unroll
-            for (int i = 0; i < CW; ++i) v[i] = 0.f;
+                for (int i = lane; i < CW; i += 32) {
+                    float f = 0.f;
+                    if (n + i < a.N) {
+                        if (a.end.bias_dtype == 0) f = reinterpret_cast<const float*>(raw_bias)[i];
+                        else if (a.end.bias_dtype == 1) f = to_acc(reinterpret_cast<const __half*>(raw_bias)[i]);
+                        else f = to_acc(reinterpret_cast<const __nv_bfloat16*>(raw_bias)[i]);
+                    }
+                    wide_bias[i] = f;
+                }
+                __syncwarp();
+                fetch_bias(unit + gridDim.x);
+                behind = count;
+#pragma unroll
+                for (int i = 0; i < CW; i += 4) {
+                    const float4 c = *reinterpret_cast<const float4*>(wide_bias + i);
+                    v[i] = c.x; v[i + 1] = c.y; v[i + 2] = c.z; v[i + 3] = c.w;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < CW; ++i) v[i] = 0.f;
+            }
             for (int kb = 0; kb < count; ++kb) {
                 copy_wait<kTc8Ring - 2>();
                 __syncwarp();
@@ -395,34 +427,10 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     if (lane == 0) mbar_arrive_at(sempty0 + 8 * s);
                 }
             }
-            // the end: bias, activation, and the row's CW columns out
+            // the end: activation, and the row's CW columns out
             // the boxes of the unit before have been read (they are written again from here on)
             if (lane < 2) bulk_wait_read();
             __syncwarp();
-            if (biased) {
-                // of the groups of copies, those behind the bias's are the blocks' scales ahead, one a block
-                if (count > 1) copy_wait<2>();
-                else copy_wait<1>();
-                __syncwarp();
-                float* const wide = reinterpret_cast<float*>(staged);
-#pragma unroll
-                for (int i = lane; i < CW; i += 32) {
-                    float f = 0.f;
-                    if (n + i < a.N) {
-                        if (a.end.bias_dtype == 0) f = reinterpret_cast<const float*>(raw_bias)[i];
-                        else if (a.end.bias_dtype == 1) f = to_acc(reinterpret_cast<const __half*>(raw_bias)[i]);
-                        else f = to_acc(reinterpret_cast<const __nv_bfloat16*>(raw_bias)[i]);
-                    }
-                    wide[i] = f;
-                }
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < CW; i += 4) {
-                    const float4 c = *reinterpret_cast<const float4*>(wide + i);
-                    v[i] += c.x; v[i + 1] += c.y; v[i + 2] += c.z; v[i + 3] += c.w;
-                }
-                __syncwarp();
-            }
             if (a.end.act == kActRelu) {
 #pragma unroll
                 for (int i = 0; i < CW; ++i) v[i] = activate(v[i], kActRelu);
