@@ -177,8 +177,12 @@ size_t partial_floats(int64_t M, int64_t N, int64_t K) {
 
 
 int make_map8(CUtensorMap* map, const Operand8& o, int64_t rows, int64_t K, int box_rows, char* err, size_t err_len) {
-    const CUresult r = host::encode_tiled_u8(map, o.q, uint64_t(K), uint64_t(rows), uint64_t(o.pitch), kBlock8,
-                                             uint32_t(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
+    const CUresult r =
+        !o.blocks
+            ? host::encode_tiled_u8(map, o.q, uint64_t(K), uint64_t(rows), uint64_t(o.pitch), kBlock8,
+                                    uint32_t(box_rows), CU_TENSOR_MAP_SWIZZLE_128B)
+            : host::encode_tiled_rows(map, 1, o.q, kBlock8, uint64_t(rows), uint64_t(blocks_of(K)), kBlock8,
+                                      uint32_t(box_rows), CU_TENSOR_MAP_SWIZZLE_128B);
     if (r == CUDA_SUCCESS) return TD_OK;
     return fail(err, err_len, TD_ERR_CUDA, "cuTensorMapEncodeTiled (8-bit product) failed (%d)", int(r));
 }
@@ -237,7 +241,7 @@ int launch_tc(const TcPlan& p, const Operand8& a, const Operand8& b, const End8&
         if constexpr (sizeof(T) == 1)
             return p.bn == 256 ? launch_tc_of<256, T, false>(ma, mb, mo, t, stream, err, err_len)
                                : launch_tc_of<128, T, false>(ma, mb, mo, t, stream, err, err_len);
-        else if (b.rows_per_scale == 1)
+        else if (b.blocks)  // (as a is, and with a scale for each row)
             return p.bn == 256 ? launch_tc_of<256, T, true>(ma, mb, mo, t, stream, err, err_len)
                                : launch_tc_of<128, T, true>(ma, mb, mo, t, stream, err, err_len);
         else
@@ -343,8 +347,8 @@ TrainPlan plan_train(int64_t M, int64_t K, int64_t N, void* workspace) {
     return p;
 }
 
-// A backward call's workspace: the gradient in 1 x 128 blocks, and, transposed, in blocks of 128 rows, as is the
-// input; the transposed weight; the parts of the bias's column sums, and of split products, one after the other.
+// A backward call's workspace: the gradient in 1 x 128 blocks, and, transposed, in blocks of 128 rows ([MB, N, 128]),
+// as is the input ([MB, K, 128]); the transposed weight; the parts of the bias's column sums, and of split products, one after the other.
 struct BackwardPlan {
     uint8_t *dy, *dyt, *xt, *wt;
     float *dy_scale, *dyt_scale, *xt_scale, *wt_scale, *sums, *partial;
@@ -365,9 +369,9 @@ BackwardPlan plan_backward(int64_t M, int64_t K, int64_t N, bool want_x, bool wa
         p.wt_scale = cut.take<float>(blocks_of(K) * blocks_of(N));
     }
     if (want_w) {
-        p.dyt = cut.take<uint8_t>(N * up(M, 16));
+        p.dyt = cut.take<uint8_t>(N * MB * kBlock8);
         p.dyt_scale = cut.take<float>(MB * p.n_pad);
-        p.xt = cut.take<uint8_t>(K * up(M, 16));
+        p.xt = cut.take<uint8_t>(K * MB * kBlock8);
         p.xt_scale = cut.take<float>(MB * p.k_pad);
     }
     if (want_b) p.sums = cut.take<float>(MB * N);
@@ -471,7 +475,7 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     const int64_t KB = blocks_of(K);
     const End8 end = {bias, out, out_scale, bias_dtype, activation, int(out_pitch)};
-    Operand8 a = {static_cast<const uint8_t*>(x), x_scale, x_pitch, KB, 1, 1};
+    Operand8 a = {static_cast<const uint8_t*>(x), x_scale, x_pitch, KB, 1, 1, false, kBlock8};
     if (copy_x) {
         if (int rc = launch_pitch(&a.q, &a.pitch, p.q, M, K, s, err, err_len)) return rc;
     }
@@ -494,7 +498,7 @@ int td_fp8_linear(int x_dtype, const void* x, int64_t x_pitch, const float* x_sc
         if (int rc = launch_rows(x_dtype, x, p.q, a.pitch, p.scale, M, K, s, err, err_len)) return rc;
     }
     if (few_takes(TD_E4M3, M, K)) return few(TD_E4M3);
-    const Operand8 b = {w8, w_scale, w_pitch, KB, 1, kBlock8};
+    const Operand8 b = {w8, w_scale, w_pitch, KB, 1, kBlock8, false, kBlock8};
     return launch_product(a, b, end, out_dtype, M, N, K, p.partial, s, err, err_len);
 }
 
@@ -541,8 +545,8 @@ int td_fp8_linear_train(int dtype, const void* x, const void* weight, const void
     }
     if (int rc = launch_tiles(dtype, jobs, s, err, err_len)) return rc;
     const int64_t KB = blocks_of(K);
-    const Operand8 a = {static_cast<const uint8_t*>(q), scale, q_pitch, KB, 1, 1};
-    const Operand8 b = {p.w, p.w_scale, up(K, 16), KB, 1, kBlock8};
+    const Operand8 a = {static_cast<const uint8_t*>(q), scale, q_pitch, KB, 1, 1, false, kBlock8};
+    const Operand8 b = {p.w, p.w_scale, up(K, 16), KB, 1, kBlock8, false, kBlock8};
     const End8 end = {bias, out, nullptr, dtype, kActNone, 0};
     return launch_product(a, b, end, dtype, M, N, K, p.partial, s, err, err_len);
 }
@@ -589,7 +593,6 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
     if (grad_bias != nullptr) g.sums = p.sums;
     g.M = M;
     g.q_pitch = up(N, 16);
-    g.qt_pitch = up(M, 16);
     g.scale_t_pitch = p.n_pad;
     g.C = int(N);
     if (grad_weight != nullptr) {  // .. the kept input, in blocks of rows
@@ -600,7 +603,6 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         x8.qt = p.xt;
         x8.scale_t = p.xt_scale;
         x8.M = M;
-        x8.qt_pitch = up(M, 16);
         x8.scale_t_pitch = p.k_pad;
         x8.C = int(K);
     }
@@ -626,14 +628,14 @@ int td_fp8_linear_backward(int dtype, const void* grad_out, const void* x, int64
         if (rc) return rc;
     }
     if (grad_x != nullptr) {
-        const Operand8 a = {p.dy, p.dy_scale, up(N, 16), NB, 1, 1};
-        const Operand8 b = {p.wt, p.wt_scale, up(N, 16), NB, 1, kBlock8};
+        const Operand8 a = {p.dy, p.dy_scale, up(N, 16), NB, 1, 1, false, kBlock8};
+        const Operand8 b = {p.wt, p.wt_scale, up(N, 16), NB, 1, kBlock8, false, kBlock8};
         const End8 end = {nullptr, grad_x, nullptr, dtype, kActNone, 0};
         if (int rc = launch_product(a, b, end, dtype, M, K, N, p.partial, s, err, err_len)) return rc;
     }
     if (grad_weight != nullptr) {
-        const Operand8 a = {p.dyt, p.dyt_scale, up(M, 16), 1, p.n_pad, 1};
-        const Operand8 b = {p.xt, p.xt_scale, up(M, 16), 1, p.k_pad, 1};
+        const Operand8 a = {p.dyt, p.dyt_scale, kBlock8, 1, p.n_pad, 1, true, N * kBlock8};
+        const Operand8 b = {p.xt, p.xt_scale, kBlock8, 1, p.k_pad, 1, true, K * kBlock8};
         const End8 end = {nullptr, grad_weight, nullptr, dtype, kActNone, 0};
         if (int rc = launch_product(a, b, end, dtype, N, K, M, p.partial, s, err, err_len)) return rc;
     }

@@ -182,7 +182,8 @@ struct TileArgs {
     long long ld;
     uint8_t* q;              // or null: [M, q_pitch], in 1 x 128 blocks, or 128 x 128 (kTileWhole)
     float* scale;            //   [M, CB], or [MB, CB]
-    uint8_t* qt;             // or null: the transpose [C, qt_pitch], in blocks of 128 rows of x, or 128 x 128
+    uint8_t* qt;             // or null: the transpose, [C, qt_pitch] in blocks of 128 x 128 (kTileWhole), or
+                             //   [MB, C, 128], a block of 128 rows of x a column: a tile is 16 KB that follow one another
     float* scale_t;          //   [MB, scale_t_pitch] (one for each column), or [CB, MB]
     float* sums;             // or null: [MB, C] sums over a tile's rows
     long long M, q_pitch, qt_pitch, scale_t_pitch;
@@ -506,11 +507,12 @@ __device__ __forceinline__ void tile_job(const TileArgs& a, long long tile, floa
     __syncthreads();
     for (int i = threadIdx.x; i < kBlock8 * 8; i += kTileThreads) {
         const int c = i >> 3, piece = i & 7, turn = c >> 3;
-        const long long at = mb * kBlock8 + piece * 16;
-        if (cb * kBlock8 + c >= a.C || at >= a.qt_pitch) continue;  // (the pitch is a multiple of 16)
+        const long long col = cb * kBlock8 + c, at = mb * kBlock8 + piece * 16;
+        if (col >= a.C || (WHOLE && at >= a.qt_pitch)) continue;  // (the pitch is a multiple of 16)
         uint4 w = *reinterpret_cast<const uint4*>(turned + c * kBlock8 + ((piece ^ (turn >> 1)) << 4));
         if (turn & 1) w = make_uint4(w.z, w.w, w.x, w.y);
-        *reinterpret_cast<uint4*>(a.qt + (long long)(cb * kBlock8 + c) * a.qt_pitch + at) = w;
+        uint8_t* to = WHOLE ? a.qt + col * a.qt_pitch + at : a.qt + (mb * a.C + col) * kBlock8 + piece * 16;
+        *reinterpret_cast<uint4*>(to) = w;
     }
 }
 

@@ -24,12 +24,15 @@ __device__ __forceinline__ float activate(float v, int act) {
     return v;
 }
 
-// One operand [rows, K] of a product, K innermost, rows `pitch` bytes apart.
+// One operand [rows, K] of a product: rows along K, `pitch` bytes apart, or (blocks) [K / 128, rows, 128], laid out a
+// block of K at a time. Value k of row r is at q[r * pitch + k / 128 * block + k % 128] in both.
 struct Operand8 {
     const uint8_t* q;
     const float* scale;  // of row r and block kb: scale[r / rows_per_scale * scale_row + kb * scale_k]
     long long pitch, scale_row, scale_k;
     int rows_per_scale;  // 1 or 128
+    bool blocks;
+    long long block;
 };
 
 // How a product ends: bias, activation, and the type it is written in.
@@ -68,8 +71,8 @@ __global__ void __launch_bounds__(kSimtThreads8)
         for (int k1 = k0; k1 < k0 + kBlock8 && k1 < K; k1 += kSimtStep8) {
             for (int i = threadIdx.x; i < (kSimtRows8 + kBlock8) * kSimtStep8; i += kSimtThreads8) {
                 const int r = i / kSimtStep8, c = i % kSimtStep8, k = k1 + c, n = n0 + r - kSimtRows8;
-                if (r < kSimtRows8) sa[c][r] = m0 + r < M && k < K ? from_e4m3(a.q[(m0 + r) * a.pitch + k]) : 0.f;
-                else sb[c][r - kSimtRows8] = n < N && k < K ? from_e4m3(b.q[n * b.pitch + k]) : 0.f;
+                if (r < kSimtRows8) sa[c][r] = m0 + r < M && k < K ? from_e4m3(a.q[(m0 + r) * a.pitch + k / kBlock8 * a.block + k % kBlock8]) : 0.f;
+                else sb[c][r - kSimtRows8] = n < N && k < K ? from_e4m3(b.q[n * b.pitch + k / kBlock8 * b.block + k % kBlock8]) : 0.f;
             }
             __syncthreads();
 #pragma unroll 4

@@ -15,7 +15,9 @@
 // together). A tile's K may be split over `splits` units whose float32 parts another kernel adds in order (a long sum
 // behind few tiles: the weight's gradient). Roles: warps 0 - 7 the epilogue (TMEM lanes 32 (w % 4) .., columns
 // w / 4 * BN / 2 ..), warp 8 the TMA producers, two lanes a slot (as in td_gemm_tc.cuh, whose notes on the waits apply
-// here), warp 9 the MMA issuer (10 and 11 fill its warpgroup). COLS: B has a scale for each row and block, which the producers bring to shared memory.
+// here), warp 9 the MMA issuer (10 and 11 fill its warpgroup).
+// COLS (the weight's gradient): both operands are laid out a block of K at a time, so that a tile is bytes that follow one
+// another in memory, and B has a scale for each row and block, which the producers bring to shared memory.
 // In 8-bit results a block of 128 columns of a row is one thread's (BN = 256), or two threads' (BN = 128).
 #pragma once
 
@@ -125,6 +127,14 @@ __device__ __forceinline__ void tmem_ld_wait_for(uint32_t (&r)[16]) {
                  : "memory");
 }
 
+// Block k of the rows from `row` on, of rows along K or (BLOCKS) of a tensor laid out a block at a time.
+template <bool BLOCKS>
+__device__ __forceinline__ void load_box(void* dst, const CUtensorMap* map, uint64_t* bar, int k, int row,
+                                         uint64_t pol) {
+    if constexpr (BLOCKS) tma_load_3d(dst, map, bar, 0, row, k, pol);
+    else tma_load_2d(dst, map, bar, k * kBlock8, row, pol);
+}
+
 // 3-D tiled store of the box at (x, y, z) from shared memory; what lies outside the tensor is not written. x * element
 // size is a multiple of 16 bytes, no coordinate is negative.
 __device__ __forceinline__ void tma_store_box(const CUtensorMap* map, const void* src, int x, int y, int z) {
@@ -218,10 +228,10 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                             bulk_load(scales + s * BN, a.sb + n0 + k * a.sb_k, BN * 4, landed);
                         } else if ((lane & 1) == 0) {
                             mbar_arrive_expect_tx(landed, Lay::kABytes);
-                            tma_load_2d(smem + s * Lay::kStageBytes, &map_a, landed, k * kBlock8, m0, pol_a);
+                            load_box<COLS>(smem + s * Lay::kStageBytes, &map_a, landed, k, m0, pol_a);
                         } else {
                             mbar_arrive_expect_tx(landed, Lay::kBBytes);
-                            tma_load_2d(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k * kBlock8, n0, pol_b);
+                            load_box<COLS>(smem + s * Lay::kStageBytes + Lay::kABytes, &map_b, landed, k, n0, pol_b);
                         }
                         ++round;
                         kb += S;

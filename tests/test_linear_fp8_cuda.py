@@ -96,7 +96,7 @@ def test_linear(policy, dtype, shape):
     assert _native.device_error() == 0
 
 
-@pytest.mark.parametrize('shape', [s for s in SHAPES if s[0] * s[1] * s[2] > 1], ids=str)
+@pytest.mark.parametrize('shape', SHAPES + [(1, 1, 200), (300, 1, 7), (300, 9, 1), (300, 1, 1), (129, 128, 1)], ids=str)
 @pytest.mark.parametrize('dtype', DTYPES, ids=str)
 def test_training(policy, dtype, shape):
     M, K, N = shape
