@@ -535,7 +535,7 @@ __global__ void __launch_bounds__(kTileThreads, sizeof(T) == 4 ? 2 : 4)
 
 // out[c] = the partial rows [parts][C] added in order: each thread adds every kColumnRows-th part of one column, then
 // the threads of a column are added in order.
-constexpr int kColumnCols = 32, kColumnRows = 16;
+constexpr int kColumnCols = 32, kColumnRows = 32;
 template <typename T, typename A>
 __global__ void __launch_bounds__(kColumnCols* kColumnRows)
     column_sum_kernel(const A* __restrict__ partial, T* out, long long parts, int C) {
@@ -546,7 +546,7 @@ __global__ void __launch_bounds__(kColumnCols* kColumnRows)
     launch_dependents();
     A sum = 0;
     if (col < C) {
-#pragma unroll 4
+#pragma unroll 8
         for (long long p = ty; p < parts; p += kColumnRows) sum += partial[p * C + col];
     }
     sums[ty][tx] = sum;
