@@ -6,10 +6,10 @@
 // its 128 products in TMEM, from zero, and the epilogue warps add that times the scales to float32 registers while the
 // tensor cores work on the next block in another part of TMEM. The scales are so any float32 numbers, and the tensor
 // cores' own sums are never longer than 128 products, however long K is. What bounds it: a 128 x 256 block takes the
-// tensor cores 512 cycles, shared memory 768 (48 KB written and 48 KB read at 128 bytes a cycle) and the 8 epilogue warps
+// tensor cores 512 cycles, shared memory 768 by count (48 KB in, 48 KB out, 128 bytes a cycle) and the 8 epilogue warps
 // about 890 each (128 multiply-adds, 128 columns from TMEM, waits); with two TMEM buffers between them it goes around in
-// 1100. 8192 x 4096 x 4096 in 142 us (1.94 PFLOP/s), 177784 x 1024 x 256 75, 177784 x 256 x 1024 106, 2400 x 256 x 1024
-// 5.2, 300 x 256 x 1024 4.0; 16-bit results. Where K is short a tile's end counts as much as its blocks.
+// 1100. 8192 x 4096 x 4096 in 143 us (1.92 PFLOP/s), 177784 x 1024 x 256 71, 177784 x 256 x 1024 93, 2400 x 256 x 1024
+// 5.1, 300 x 256 x 1024 3.9; 16-bit results. Where K is short a tile's end counts as much as its blocks.
 //
 // Persistent, one CTA an SM, output tiles of 128 x BN (columns fastest, so that the CTAs which share rows of A run
 // together). A tile's K may be split over `splits` units whose float32 parts another kernel adds in order (a long sum
