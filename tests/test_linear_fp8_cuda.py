@@ -206,6 +206,78 @@ def test_infinities_and_nan_stay_in_their_rows(policy, M):
     assert data[[0, M + 1]].float().isnan().all() and data[1:M + 1].float().isfinite().all()
 
 
+@pytest.mark.parametrize('M', (1, 9, 200))
+def test_nan_in_a_weight_or_bias_stays_in_its_column(policy, M):
+    x, w, b = normal(M, 300), normal(270, 300, seed=1), normal(270, seed=2)
+    clean = linear_fp8(x, quantize_weight_fp8(w), b)
+    rest = [n for n in range(270) if n not in (5, 140, 269)]
+    w[5, 299], w[140, 0], b[269] = float('nan'), float('inf'), float('nan')
+    got = linear_fp8(x, quantize_weight_fp8(w), b)
+    assert got[:, [5, 140, 269]].isnan().all() and torch.equal(got[:, rest], clean[:, rest])
+    data, scale = linear_fp8(x, quantize_weight_fp8(w), b, activation='relu', quantize=True)
+    assert data[:, [5, 140, 269]].float().isnan().all() and data[:, rest].float().isfinite().all()
+    assert scale.isfinite().all()
+
+
+def test_infinities_and_nan_in_a_gradient(policy):
+    """A row of grad_x and a row of grad_weight go, the rest stays; the bias's sum is the sum, infinity and all."""
+    x, w, b, g = normal(300, 200), normal(140, 200, seed=1), normal(140, seed=2), normal(300, 140, seed=3)
+
+    def grads(g):
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        return torch.autograd.grad(linear_fp8(*leaves), leaves, g)
+
+    clean = grads(g)
+    g[7, 3], g[250, 139] = float('inf'), float('nan')
+    gx, gw, gb = grads(g)
+    for got, want, bad in ((gx, clean[0], [7, 250]), (gw, clean[1], [3, 139])):
+        rest = torch.ones(got.shape[0], dtype=torch.bool, device='cuda')
+        rest[bad] = False
+        assert got[bad].isnan().all() and torch.isfinite(got[rest]).all()
+    keep = [n for n in range(140) if n not in (3, 139)]
+    assert gb[3] == float('inf') and gb[139].isnan() and torch.equal(gb[keep], clean[2][keep])
+
+
+@pytest.mark.parametrize('M', (2, 40))
+def test_activations_at_their_ends(policy, M):
+    """Arguments from -1000 to 1000 (exact products of powers of two), where exponentials leave float32's range."""
+    x = torch.zeros(M, 128, device='cuda')
+    x[:, 0] = 1
+    v = torch.tensor([-1000., -128, -96, -88, -64, -32, -16, -8, -1, -2.0 ** -6, 0, 2.0 ** -6, 1, 8, 88, 128, 1000],
+                     device='cuda')
+    w8 = quantize_weight_fp8(torch.zeros(v.numel(), 128, device='cuda'))
+    for act in ('relu', 'gelu', 'silu'):
+        check(linear_fp8(x, w8, v, act), product_exact(x, torch.zeros(v.numel(), 128, device='cuda'), torch.float32, v,
+                                                       act), act)
+
+
+def test_two_threads_at_once(cuda):
+    """Calls from two host threads, each on a stream of its own, give what they give alone."""
+    import threading
+    w8 = quantize_weight_fp8(normal(512, 256, dtype=torch.bfloat16, seed=1))
+    xs = [normal(M, 256, dtype=torch.bfloat16, seed=M) for M in (3, 300)]
+    want = [linear_fp8(x, w8, activation='relu') for x in xs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(x, e):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                outs = [linear_fp8(x, w8, activation='relu') for _ in range(50)]
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(o, e) for o in outs):
+                wrong.append('results differ')
+        except Exception as exc:  # a thread's own exception would be lost
+            wrong.append(repr(exc))
+
+    threads = [threading.Thread(target=work, args=a) for a in zip(xs, want)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_rows_behind_the_last_are_left_alone(policy):
     """Results of a smaller call into the front of a larger allocation's neighbours: what lies behind stays."""
     for M, N in ((5, 130), (130, 264), (300, 1024)):
