@@ -13,14 +13,47 @@ namespace td {
 
 enum Activation8 : int { kActNone = 0, kActRelu = 1, kActGelu = 2, kActSilu = 3 };
 
+// 1 / x for 1 <= x, to a step of float32.
+__device__ __forceinline__ float reciprocal(float x) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+
+// GELU, v Phi(v), by the upper tail h = 1 - Phi(|v|) = exp(-v^2 / 2) R, which keeps the digits of a lower tail that
+// 1 + erf loses (a tenth of the value at -5, all of it below -5.6). R = erfcx(|v| / sqrt 2) / 2 is smooth, in
+// t = 1 / (1 + 0.35 |v|) a polynomial times t, fitted to |v| < 15 (beyond, the tail is less than float32 holds) for the
+// least relative error, 3e-8. 177784 x 256 x 1024 with 8-bit results: 302 us, by erfcf 768, by 1 + erff 336.
+__device__ __forceinline__ float gelu(float v) {
+    const float a = fabsf(v), t = reciprocal(fmaf(0.35f, a, 1.f));
+    float p = -0.029163928f;
+    p = fmaf(p, t, 0.14406084f);
+    p = fmaf(p, t, -0.25590193f);
+    p = fmaf(p, t, 0.15939298f);
+    p = fmaf(p, t, -0.023263887f);
+    p = fmaf(p, t, 0.10557482f);
+    p = fmaf(p, t, 0.11981549f);
+    p = fmaf(p, t, 0.13986434f);
+    p = fmaf(p, t, 0.13962126f);
+    const float h = exp2f(v * v * -0.72134752f) * (p * t);  // -log2(e) / 2
+    return v * (v < 0.f ? h : 1.f - h);
+}
+
+// SiLU, v / (1 + exp(-v)), with the exponential at most 1, so that neither it nor the denominator leaves the range. The
+// same call 225 us; 206 with __expf(-v) and __fdividef, which is zero below -87.
+__device__ __forceinline__ float silu(float v) {
+    const float e = expf(-fabsf(v));
+    return (v < 0.f ? v * e : v) * reciprocal(1.f + e);
+}
+
 __device__ __forceinline__ float activate(float v, int act) {
     if (act == kActRelu) {  // a NaN stays one
         float d;
         asm("max.NaN.f32 %0, %1, 0f00000000;" : "=f"(d) : "f"(v));
         return d;
     }
-    if (act == kActGelu) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-    if (act == kActSilu) return __fdividef(v, 1.f + __expf(-v));  // (a few steps of float32 of |v|)
+    if (act == kActGelu) return gelu(v);
+    if (act == kActSilu) return silu(v);
     return v;
 }
 

@@ -182,8 +182,11 @@ def linear_fp8_reference(x, weight, bias=None, activation=None, quantize=False, 
     y = torch.matmul(dequantize_fp8_reference(*x, torch.float32), dequantize_fp8_reference(*weight, torch.float32).t())
     if bias is not None:
         y = y + bias.float()
-    if activation is not None:
-        y = {'relu': F.relu, 'gelu': F.gelu, 'silu': F.silu}[activation](y)
+    if activation == 'relu':
+        y = F.relu(y)
+    elif activation is not None:  # in 64 bits: float32 loses the lower tails' digits
+        d = y.double()
+        y = (0.5 * d * torch.special.erfc(d * -0.5 ** 0.5) if activation == 'gelu' else F.silu(d)).float()
     return quantize_fp8_reference(y) if quantize else y.to(dtype)
 
 

@@ -1,0 +1,35 @@
+"""The feed-forward operators where roundings add up or digits cancel: results that are exact, or held to a count of the
+roundings that the kernels make."""
+
+import pytest
+import torch
+
+from marearts_tinydeform_b200 import linear_fp8, quantize_weight_fp8
+
+pytestmark = pytest.mark.gpu
+
+E = 2.0 ** -24  # half a step of float32, relative
+
+
+@pytest.mark.parametrize('M, K', [(2, 128), (40, 128), (40, 4096), (2400, 128)])
+def test_activations_keep_their_digits(policy, M, K):
+    """GELU and SiLU relative to their own values, where those are far smaller than the argument too.
+
+    E is half a step of float32. GELU, v (1 - Phi(|v|)) below zero: the tail's smooth factor is good to 7 E (its fit 1,
+    nine fused steps and a reciprocal good to a step the rest), its exponential to 2 steps (4 E), whose argument, rounded
+    twice behind a rounded constant, adds at most 1.5 v^2 E; a product, and 1 - tail or v times it: (14 + 2 v^2) E. SiLU,
+    v exp(-|v|) / (1 + exp(-|v|)) below zero: an exponential good to 2 steps (4 E, and no more again through the sum), a
+    product, a sum, a reciprocal good to a step and its product: 14 E. Below float32's normal numbers each of these steps
+    may be off by 2^-149, times up to |v| + 1."""
+    N = 1024 if M > 1000 else 270
+    v = torch.linspace(-14, 14, N, device='cuda')
+    v[:9] = torch.tensor([-110., -100, -96, -90, -88.5, -88, -87, -40, -20], device='cuda')
+    x = torch.ones(M, K, device='cuda')
+    w8 = quantize_weight_fp8(torch.zeros(N, K, device='cuda'))
+    d = v.double()
+    exact = {'gelu': (0.5 * d * torch.erfc(-d / 2 ** 0.5), (14 + 2 * d * d) * E), 'silu': (d * torch.sigmoid(d), 14 * E)}
+    for act, (want, bound) in exact.items():
+        got = linear_fp8(x, w8, v, act)
+        off = (got.double() - want).abs()
+        allowed = bound * want.abs() + (d.abs() + 1) * 2.0 ** -148
+        assert (off <= allowed).all(), f'{act}: {(off / allowed).max().item()} of what it may be off'

@@ -87,6 +87,16 @@ def test_linear_reference(dtype):
         check(a, e, 'training')
 
 
+def test_activations_keep_their_digits():
+    """The lower tails of GELU and SiLU, to two roundings of float32 (computed in 64 bits, rounded once, compared)."""
+    v = torch.cat([torch.linspace(-13, 13, 200), torch.tensor([-100., -90, -88.5, -40, -20])])
+    w8 = quantize_weight_fp8(torch.zeros(v.numel(), 128))
+    d = v.double()
+    for act, want in (('gelu', 0.5 * d * torch.erfc(-d / 2 ** 0.5)), ('silu', d * torch.sigmoid(d))):
+        off = (linear_fp8(torch.ones(1, 128), w8, v, act)[0].double() - want).abs()
+        assert (off <= 2.0 ** -23 * want.abs() + 2.0 ** -149).all(), act
+
+
 def test_linear_gradients_against_differences():
     """Small whole numbers survive the rounding to 8 bits, so the product is its own formula and linear in each
     operand: differences over a step of 1 are its gradients, exactly."""
