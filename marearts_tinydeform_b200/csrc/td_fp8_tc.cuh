@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             copy_commit();
         };
         // the warp's columns of the next unit's bias, as they are in memory, on their way while a unit's products are
-        // added; a unit's sums begin with them
+        // added; they are added behind the products, so that a large one is rounded once and not with every block
         const bool biased = !COLS && a.end.bias != nullptr;
         unsigned char* const raw_bias = smem + Lay::kBiasOffset + warp * CW * 4;
         float* const wide_bias = reinterpret_cast<float*>(raw_bias + kTc8Epi * CW * 4);
@@ -351,6 +351,8 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
             const int row = quarter * 32 + lane, m = m0 + row, n = n0 + c_lo;
             const int count = count_kb(unit);
             float v[CW];
+#pragma unroll
+            for (int i = 0; i < CW; ++i) v[i] = 0.f;
             if (biased) {
                 if (behind > 1) copy_wait<2>();
                 else copy_wait<1>();
@@ -368,14 +370,6 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 __syncwarp();
                 fetch_bias(unit + gridDim.x);
                 behind = count;
-#pragma unroll
-                for (int i = 0; i < CW; i += 4) {
-                    const float4 c = *reinterpret_cast<const float4*>(wide_bias + i);
-                    v[i] = c.x; v[i + 1] = c.y; v[i + 2] = c.z; v[i + 3] = c.w;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < CW; ++i) v[i] = 0.f;
             }
             for (int kb = 0; kb < count; ++kb) {
                 copy_wait<kTc8Ring - 2>();
@@ -437,7 +431,14 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                     if (lane == 0) mbar_arrive_at(sempty0 + 8 * s);
                 }
             }
-            // the end: activation, and the row's CW columns out
+            // the end: bias, activation, and the row's CW columns out
+            if (biased) {
+#pragma unroll
+                for (int i = 0; i < CW; i += 4) {
+                    const float4 c = *reinterpret_cast<const float4*>(wide_bias + i);
+                    v[i] += c.x; v[i + 1] += c.y; v[i + 2] += c.z; v[i + 3] += c.w;
+                }
+            }
             // the boxes of the unit before have been read (they are written again from here on)
             if (lane < 2) bulk_wait_read();
             __syncwarp();

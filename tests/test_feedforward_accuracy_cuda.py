@@ -33,3 +33,15 @@ def test_activations_keep_their_digits(policy, M, K):
         off = (got.double() - want).abs()
         allowed = bound * want.abs() + (d.abs() + 1) * 2.0 ** -148
         assert (off <= allowed).all(), f'{act}: {(off / allowed).max().item()} of what it may be off'
+
+
+@pytest.mark.parametrize('M, K, N', [(1, 2048, 260), (16, 2048, 260), (40, 2048, 260), (2400, 2048, 1024),
+                                     (300, 2048, 4100)])
+def test_a_large_bias_is_rounded_once(policy, M, K, N):
+    """Each block of 128 adds 1/4 to a bias of 2^23, whose neighbours are 1 away: with the products first the result is
+    the exact sum, 2^23 + 4."""
+    x, w = torch.ones(M, K, device='cuda'), torch.full((N, K), 2.0 ** -9, device='cuda')
+    got = linear_fp8(x, quantize_weight_fp8(w), torch.full((N,), 2.0 ** 23, device='cuda'))
+    assert (got == 2.0 ** 23 + K / 512).all()
+    leaves = [t.requires_grad_() for t in (x, w)]
+    assert (linear_fp8(*leaves, torch.full((N,), 2.0 ** 23, device='cuda')) == 2.0 ** 23 + K / 512).all()
