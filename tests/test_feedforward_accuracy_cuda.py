@@ -4,7 +4,7 @@ roundings that the kernels make."""
 import pytest
 import torch
 
-from marearts_tinydeform_b200 import linear_fp8, quantize_weight_fp8
+from marearts_tinydeform_b200 import linear_fp8, quantize_weight_fp8, rms_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -45,3 +45,19 @@ def test_a_large_bias_is_rounded_once(policy, M, K, N):
     assert (got == 2.0 ** 23 + K / 512).all()
     leaves = [t.requires_grad_() for t in (x, w)]
     assert (linear_fp8(*leaves, torch.full((N,), 2.0 ** 23, device='cuda')) == 2.0 ** 23 + K / 512).all()
+
+
+def test_column_sums_that_cancel(cuda):
+    """Gradients summed over rows, where the first and the last rows' 2^26 cancel and ones lie between: what CTAs have
+    added is joined in float64, so the ones are all there."""
+    g = torch.zeros(100 * 128, 40, device='cuda')  # 100 blocks of 128 rows
+    g[::128] = 1
+    g[0], g[99 * 128] = 2.0 ** 26, -2.0 ** 26
+    leaves = [torch.ones(s, device='cuda', requires_grad=True) for s in ((g.shape[0], 8), (40, 8), (40,))]
+    assert (torch.autograd.grad(linear_fp8(*leaves), leaves[2], g)[0] == 98).all()
+    rows, C = 148 * 8, 256  # a row for each of a CTA's warps
+    g = torch.ones(rows, C, device='cuda')
+    g[:8] = g[-8:] = 0
+    g[0], g[-1] = 2.0 ** 26, -2.0 ** 26
+    x, w = (torch.ones(s, device='cuda', requires_grad=True) for s in ((rows, C), (C,)))
+    assert (torch.autograd.grad(rms_norm(x, w, eps=0.0), w, g)[0] == rows - 16).all()
