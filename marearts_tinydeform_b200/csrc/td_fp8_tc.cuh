@@ -209,9 +209,9 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                 // (A's rows are read by the CTAs that run together, B by all)
                 const uint64_t pol_a = l2_evict_first(), pol_b = l2_evict_last();
                 int unit = blockIdx.x, kb = s, round = 0;
-                long long t0 = clock64();
                 grid_dependency_wait();
                 launch_dependents();
+                long long t0 = clock64();  // (the time that the kernel before this one takes does not count)
                 // (a last pass only waits, so that nothing is still to arrive on the slot when the CTA exits)
                 for (;;) {
                     while (unit < units && kb >= count_kb(unit)) {
@@ -255,6 +255,8 @@ __global__ void __launch_bounds__(kTc8Threads, 1)
                                tempty0 = smem_addr(tempty);
                 uint32_t s = 0, b = 0, s_phase = 0, b_phase = 1;
                 bool ok = true;
+                // its waits give up after a second of their own, not of the kernel's before this one
+                grid_dependency_wait();
                 for (int unit = blockIdx.x; ok && unit < units; unit += gridDim.x) {
                     for (int kb = count_kb(unit); kb > 0; --kb) {
                         ok = mbar_wait_at(tempty0 + 8 * b, b_phase, kErrSlotWait) &&

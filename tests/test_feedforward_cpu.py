@@ -2,6 +2,7 @@
 argument checks."""
 
 import ctypes
+import os
 
 import pytest
 import torch
@@ -212,3 +213,21 @@ def test_fp8_abi_refuses_before_any_launch(lib):
         assert quantize(**kw) == 1, kw
     assert quantize(M=0, x=None) == 0
     assert lib.td_fp8_dequantize(0, p, 127, p, p, 4, 128, 0, None, err, 256) == 1
+
+
+def role(file, start):
+    """The source of a warp's role, from `start` on."""
+    text = open(os.path.join(build.CSRC, file)).read()
+    return text[text.index(start):]
+
+
+def test_bounded_waits_begin_behind_the_kernel_before():
+    """A product's CTA may start while the kernel before it in the stream still runs, for longer than its own waits last:
+    the issuing thread and the producers count from behind their dependency wait. (Read from the source: a kernel that
+    runs for a second after it let the next one start would be needed to see it.)"""
+    issuer = role('td_fp8_tc.cuh', 'else if (warp == 9) {')
+    assert 0 < issuer.index('grid_dependency_wait()') < issuer.index('mbar_wait_at(')
+    producer = role('td_fp8_tc.cuh', 'if (warp == 8) {')
+    assert producer.index('grid_dependency_wait()') < producer.index('t0 = clock64()') < producer.index('mbar_test(')
+    epilogue = role('td_fp8_tc.cuh', 'setmaxnreg.inc')
+    assert epilogue.index('grid_dependency_wait()') < epilogue.index('mbar_wait_at(')
