@@ -231,3 +231,7 @@ def test_bounded_waits_begin_behind_the_kernel_before():
     assert producer.index('grid_dependency_wait()') < producer.index('t0 = clock64()') < producer.index('mbar_test(')
     epilogue = role('td_fp8_tc.cuh', 'setmaxnreg.inc')
     assert epilogue.index('grid_dependency_wait()') < epilogue.index('mbar_wait_at(')
+    issuer = role('td_gemm_tc.cuh', '// MMA issuer.')
+    assert 0 < issuer.index('grid_dependency_wait()') < issuer.index('mbar_wait(')
+    splitter = role('td_gemm_tc.cuh', '// float32: split every landed slot')
+    assert 0 < splitter.index('grid_dependency_wait()') < splitter.index('mbar_wait(')
