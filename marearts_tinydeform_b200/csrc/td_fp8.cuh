@@ -210,10 +210,13 @@ struct Patch {  // 16-bit types
         if (wide) {
             w[p] = __ldg(reinterpret_cast<const uint4*>(src));
         } else {
-            T one[8];
+            struct __align__(16) Eight {
+                T v[8];
+            } one;
+            static_assert(alignof(Eight) >= alignof(uint4), "one word of eight values");
 #pragma unroll
-            for (int i = 0; i < 8; ++i) one[i] = i < left ? src[i] : from_acc<T>(0.f);
-            w[p] = *reinterpret_cast<const uint4*>(one);
+            for (int i = 0; i < 8; ++i) one.v[i] = i < left ? src[i] : from_acc<T>(0.f);
+            w[p] = *reinterpret_cast<const uint4*>(one.v);
         }
     }
     __device__ __forceinline__ float2 pair(int p, int c) const {

@@ -103,9 +103,10 @@ __device__ __forceinline__ void few_rows(const FewArgs& a) {
     };
     // scales and a wider x (four neighbouring values of each row a lane) one block ahead, in registers
     struct Ahead {
-        X x[kWideRows][4];
+        __align__(4 * sizeof(X)) X x[kWideRows][4];  // (a row's four are read as one word)
         float sx[TILES], sw;
     };
+    static_assert(alignof(Ahead) >= 4 * sizeof(X), "words of four values");
     auto load = [&](int i, Ahead& b) {
         if (i >= blocks) return;
         const int kb = warp + i * kFewWarps;
