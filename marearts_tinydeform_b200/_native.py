@@ -1245,19 +1245,19 @@ def linear_fp8_train(x, weight, bias):
 
 def linear_fp8_backward(grad_out, x8, weight, want_x, want_w, want_b):
     """(grad_x, grad_weight, grad_bias), None where not wanted, through td_fp8_linear_backward; x8: the pair that the
-    forward's input was quantised to."""
+    forward's input was quantised to, read for grad_weight alone; weight: read for grad_x alone."""
     lib = load()
-    g, w = _dense(grad_out, weight)
-    data, pitch = _fp8_rows(x8[0])
-    scale = x8[1]
-    N, K = weight.shape
+    g, w = _dense(grad_out, weight if want_x else None)
+    (data, pitch), scale = (_fp8_rows(x8[0]), x8[1]) if want_w else ((None, 0), None)
+    N = g.shape[-1]
+    K = w.shape[1] if want_x else data.shape[-1] if want_w else 1  # (the bias's gradient has no K)
     M = g.numel() // N
     grad_x = g.new_empty((*g.shape[:-1], K)) if want_x else None
     grad_w = g.new_empty((N, K)) if want_w else None
     grad_b = g.new_empty((N,)) if want_b else None
     ws_bytes = _linear_fp8_backward_workspace(M, K, N, want_x, want_w, want_b)
     ws = g.new_empty((ws_bytes,), dtype=torch.uint8) if ws_bytes else None
-    _launch(lib.td_fp8_linear_backward, g.device, DTYPE_CODE[g.dtype], g.data_ptr(), data.data_ptr(), pitch,
-            scale.data_ptr(), w.data_ptr(), _address(grad_x), _address(grad_w), _address(grad_b), M, K, N,
+    _launch(lib.td_fp8_linear_backward, g.device, DTYPE_CODE[g.dtype], g.data_ptr(), _address(data), pitch,
+            _address(scale), _address(w), _address(grad_x), _address(grad_w), _address(grad_b), M, K, N,
             _address(ws), ws_bytes)
     return grad_x, grad_w, grad_b

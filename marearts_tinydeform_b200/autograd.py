@@ -233,7 +233,8 @@ class RmsNormFunction(torch.autograd.Function):
 
 class LinearFp8Function(torch.autograd.Function):
     """The 8-bit product, differentiable in x, weight and bias, on CUDA and (with torch operators) on the CPU. The
-    input is kept as its 8-bit copy alone; the weight, which the caller keeps anyway, is laid out again."""
+    input is kept as its 8-bit copy alone, and only where the weight's gradient will read it; the weight, which the
+    caller keeps anyway and which is laid out again, only for the input's."""
 
     @staticmethod
     def forward(ctx, x, weight, bias):
@@ -242,12 +243,14 @@ class LinearFp8Function(torch.autograd.Function):
         else:
             x8, w8 = reference.quantize_fp8_reference(x), reference.quantize_weight_fp8_reference(weight)
             y = reference.linear_fp8_reference(x8, w8, bias, dtype=x.dtype)
-        ctx.save_for_backward(*x8, weight)
+        need = ctx.needs_input_grad
+        ctx.save_for_backward(*(x8 if need[1] else (None, None)), weight if need[0] else None)
+        ctx.dtype = x.dtype
         return y
 
     @staticmethod
     @_first_order
     def backward(ctx, grad_y):
         data, scale, weight = ctx.saved_tensors
-        run = _native.linear_fp8_backward if data.is_cuda else reference.linear_fp8_backward_reference
-        return run(grad_y.to(weight.dtype), (data, scale), weight, *ctx.needs_input_grad)
+        run = _native.linear_fp8_backward if grad_y.is_cuda else reference.linear_fp8_backward_reference
+        return run(grad_y.to(ctx.dtype), (data, scale), weight, *ctx.needs_input_grad)

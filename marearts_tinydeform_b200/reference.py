@@ -191,16 +191,16 @@ def linear_fp8_reference(x, weight, bias=None, activation=None, quantize=False, 
 
 
 def linear_fp8_backward_reference(grad_out, x8, weight, want_x, want_w, want_b):
-    """The gradients of ``linear_fp8`` with torch operators, from the input's 8-bit copy."""
-    N, K = weight.shape
-    g = grad_out.reshape(-1, N)
+    """The gradients of ``linear_fp8`` with torch operators: grad_x from the weight, grad_weight from the input's 8-bit
+    copy."""
+    g = grad_out.reshape(-1, grad_out.shape[-1])
     grad_x = grad_w = grad_b = None
     if want_x:
         w8 = dequantize_fp8_reference(*_fp8_quantize(weight, 128), torch.float32)
         g8 = dequantize_fp8_reference(*_fp8_quantize(g, 1), torch.float32)
-        grad_x = torch.matmul(g8, w8).view(*grad_out.shape[:-1], K).to(grad_out.dtype)
+        grad_x = torch.matmul(g8, w8).view(*grad_out.shape[:-1], weight.shape[1]).to(grad_out.dtype)
     if want_w:
-        x = dequantize_fp8_reference(*x8, torch.float32).reshape(-1, K)
+        x = dequantize_fp8_reference(*x8, torch.float32).reshape(-1, x8[0].shape[-1])
         cols = [dequantize_fp8_reference(*_fp8_quantize(t.t(), 1), torch.float32) for t in (g, x)]
         grad_w = torch.matmul(cols[0], cols[1].t()).to(grad_out.dtype)
     if want_b:

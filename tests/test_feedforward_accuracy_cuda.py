@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from marearts_tinydeform_b200 import linear_fp8, quantize_weight_fp8, rms_norm
+from test_feedforward_cpu import keeps_what_its_gradients_read
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +62,13 @@ def test_column_sums_that_cancel(cuda):
     g[0], g[-1] = 2.0 ** 26, -2.0 ** 26
     x, w = (torch.ones(s, device='cuda', requires_grad=True) for s in ((rows, C), (C,)))
     assert (torch.autograd.grad(rms_norm(x, w, eps=0.0), w, g)[0] == rows - 16).all()
+
+
+def test_the_graph_keeps_what_its_gradients_read(policy):
+    keeps_what_its_gradients_read('cuda')
+    x = torch.randn(4096, 1024, device='cuda', dtype=torch.bfloat16, requires_grad=True)
+    w = torch.randn(128, 1024, device='cuda', dtype=torch.bfloat16)
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    y = linear_fp8(x, w)
+    assert torch.cuda.memory_allocated() - before == y.numel() * 2  # a frozen weight: nothing of the input is kept

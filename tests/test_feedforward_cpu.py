@@ -114,6 +114,28 @@ def test_linear_gradients_against_differences():
             assert slope == grads[k].reshape(-1)[i]
 
 
+def keeps_what_its_gradients_read(device):
+    """Each gradient alone: what the graph holds until the backward, and that the operand which the gradient does not
+    read may change in between."""
+    gen = torch.Generator().manual_seed(3)
+    x, w, b, g = (torch.randint(-4, 5, s, generator=gen).float().to(device) for s in ((6, 20), (7, 20), (7,), (6, 7)))
+    leaves = [t.clone().requires_grad_() for t in (x, w, b)]
+    want = torch.autograd.grad(linear_fp8(*leaves), leaves, g)
+    for k, held in enumerate(([torch.float32], [E4M3, torch.float32], [])):
+        only = [t.clone().requires_grad_(i == k) for i, t in enumerate((x, w, b))]
+        y = linear_fp8(*only)
+        assert [t.dtype for t in y.grad_fn.saved_tensors if t is not None] == held
+        with torch.no_grad():
+            for i, t in enumerate(only):
+                if i != 1 or k != 0:
+                    t.zero_()
+        assert torch.equal(torch.autograd.grad(y, only[k], g)[0], want[k])
+
+
+def test_the_graph_keeps_what_its_gradients_read():
+    keeps_what_its_gradients_read('cpu')
+
+
 def test_rms_norm_refusals():
     x, w = torch.zeros(3, 8), torch.ones(8)
     for args, kw, message in [((x, w[:7]), {}, 'weight'), ((x, w, x[:2]), {}, 'residual'),
