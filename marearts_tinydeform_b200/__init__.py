@@ -342,16 +342,20 @@ def quantize_fp8(x):
 
     x: float32, float16 or bfloat16, up to 65536 wide (and 2^31 - 256 rows). Scales are powers of two, the smallest that bring a block's
     largest finite magnitude to at most 448 (e4m3's largest); values are rounded to nearest, ties to even; infinities
-    and NaN become NaN. data's rows start 16 bytes apart or a multiple of that, so it is a view where K is not one.
+    and NaN become NaN. data's rows start 16 bytes apart or a multiple of that, so it is a view where K is not one. What
+    is in 8 bits has no gradient, so an x that requires grad is refused (linear_fp8 takes it as it is).
     """
     _native.check_fp8_source(x)
+    if _wants_grad(x):
+        raise RuntimeError('what is in 8 bits has no gradient: detach x, or run under torch.no_grad()')
     x = x.detach()
     return _native.fp8_quantize(x) if x.is_cuda else quantize_fp8_reference(x)
 
 
 def quantize_weight_fp8(weight):
     """A weight [N, K] in 8 bits as linear_fp8 takes it, to be laid out once: (data, scale) as quantize_fp8's, with a
-    scale for each block of 128 x 128, float32 [ceil(N / 128), ceil(K / 128)]."""
+    scale for each block of 128 x 128, float32 [ceil(N / 128), ceil(K / 128)]. The pair is the weight's values alone, a
+    parameter's too: no gradient goes back through it (training takes the weight itself)."""
     _native.check_fp8_source(weight, 'weight')
     if weight.dim() != 2 or not 1 <= weight.shape[0] <= _native.MAX_FP8_WIDTH:
         raise RuntimeError(f'weight must be [N, K], both between 1 and {_native.MAX_FP8_WIDTH}')

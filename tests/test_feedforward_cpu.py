@@ -182,6 +182,18 @@ def test_linear_refusals():
         dequantize_fp8(*x8, torch.float64)
 
 
+def test_quantising_refuses_to_cut_a_graph():
+    """A result that looks differentiable and is not would train nothing."""
+    x = torch.randn(3, 200, requires_grad=True)
+    w8 = quantize_weight_fp8(torch.nn.Parameter(torch.randn(150, 200)))  # laid out once, from a module's parameter
+    for make in (quantize_fp8, lambda t: linear_fp8(quantize_fp8(t), w8, dtype=t.dtype), lambda t: quantize_fp8(t * 2)):
+        with pytest.raises(RuntimeError, match='no gradient'):
+            make(x)
+    with torch.no_grad():
+        kept = quantize_fp8(x)
+    assert torch.equal(kept[0].float(), quantize_fp8(x.detach())[0].float())
+
+
 def test_rms_norm_abi_refuses_before_any_launch(lib):
     err = ctypes.create_string_buffer(256)
     p = ctypes.c_void_p(16)
