@@ -365,12 +365,15 @@ def quantize_weight_fp8(weight):
 
 def dequantize_fp8(data, scale, dtype):
     """data * scale in `dtype` (float32, float16 or bfloat16): what quantize_fp8's pair, or quantize_weight_fp8's, stands
-    for. bfloat16 and float32 hold the values of this package's own pairs exactly."""
+    for. bfloat16 and float32 hold the values of this package's own pairs exactly. Scales that require grad are refused:
+    a pair has no gradient."""
     tiles = isinstance(data, torch.Tensor) and isinstance(scale, torch.Tensor) and data.dim() == 2 and \
         scale.dim() == 2 and scale.shape[0] != data.shape[0]
     _native.check_fp8_pair((data, scale), 'the input', tiles)
     if dtype not in (torch.float32, torch.float16, torch.bfloat16):
         raise RuntimeError('dtype must be float32, float16 or bfloat16')
+    if _wants_grad(data, scale):
+        raise RuntimeError('what is in 8 bits has no gradient: detach the scales, or run under torch.no_grad()')
     if not data.is_cuda:
         return dequantize_fp8_reference(data, scale, dtype)
     return _native.fp8_dequantize(data, scale, dtype, tiles)

@@ -192,6 +192,8 @@ def test_quantising_refuses_to_cut_a_graph():
     with torch.no_grad():
         kept = quantize_fp8(x)
     assert torch.equal(kept[0].float(), quantize_fp8(x.detach())[0].float())
+    with pytest.raises(RuntimeError, match='no gradient'):
+        dequantize_fp8(kept[0], kept[1].requires_grad_(), torch.float32)
 
 
 def test_rms_norm_abi_refuses_before_any_launch(lib):
