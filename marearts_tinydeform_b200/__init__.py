@@ -44,6 +44,7 @@ inputs that require grad: the forward runs the same kernels and the backward run
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from .autograd import (AttentionFunction, LayerNormFunction, LinearFp8Function, RmsNormFunction, linear_train,
@@ -182,6 +183,11 @@ def ma_deform_attn(memory, value_weight, value_bias, spatial_shapes, level_start
 
 
 def _wants_grad(*ts):
+    """Whether a call of these operands is differentiated. Forward-mode tangents, which the kernels would drop without a
+    word, are refused (the CPU path carries them)."""
+    if forward_ad._current_level >= 0 and any(
+            t is not None and t.is_cuda and forward_ad.unpack_dual(t).tangent is not None for t in ts):
+        raise RuntimeError('no forward-mode derivative on CUDA: differentiate in reverse mode')
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 

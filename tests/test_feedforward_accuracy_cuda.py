@@ -3,8 +3,10 @@ roundings that the kernels make."""
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
-from marearts_tinydeform_b200 import linear_fp8, quantize_weight_fp8, rms_norm
+from marearts_tinydeform_b200 import (attention, deform_attn_layer, layer_norm, linear_fp8, ma_deform_attn, quantize_fp8,
+                                      quantize_weight_fp8, rms_norm, sampling_producer)
 from test_feedforward_cpu import keeps_what_its_gradients_read
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +74,24 @@ def test_the_graph_keeps_what_its_gradients_read(policy):
     before = torch.cuda.memory_allocated()
     y = linear_fp8(x, w)
     assert torch.cuda.memory_allocated() - before == y.numel() * 2  # a frozen weight: nothing of the input is kept
+
+
+def test_forward_mode_tangents_are_refused(cuda):
+    """An operator that dropped its operand's tangent would give a constant."""
+    x, w, q = (torch.randn(s, device='cuda') for s in ((6, 64), (64, 64), (1, 6, 2, 32)))
+    shapes, start = torch.tensor([[4, 4]], device='cuda'), torch.tensor([0], device='cuda')
+    loc, attn = torch.rand(1, 5, 2, 1, 4, 2, device='cuda'), torch.rand(1, 5, 2, 1, 4, device='cuda')
+    memory, query, ref = (torch.randn(s, device='cuda') for s in ((1, 16, 64), (1, 5, 64), (1, 5, 1, 2)))
+    sw = torch.randn(2 * 4 * 3, 64, device='cuda')
+    calls = [(x, lambda t: rms_norm(t, w[0])), (w, lambda t: linear_fp8(x, t)),
+             (x, lambda t: linear_fp8(t, quantize_weight_fp8(w))), (x, quantize_fp8), (x, lambda t: layer_norm(t, w[0])),
+             (q, lambda t: attention(t, q, q)),
+             (memory, lambda t: ma_deform_attn(t, w, None, shapes, start, loc, attn)),
+             (query, lambda t: sampling_producer(t, ref, shapes, 2, 4, sw, None)),
+             (memory, lambda t: deform_attn_layer(query, ref, t, shapes, start, 2, 4, sw, None, w, None))]
+    for operand, call in calls:
+        call(operand)
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match='forward-mode'):
+                call(forward_ad.make_dual(operand, torch.ones_like(operand)))
+            call(operand)
