@@ -387,7 +387,9 @@ def dequantize_fp8(data, scale, dtype):
 
 def _tensors(operand):
     """An operand's tensors: itself, or a pair's."""
-    return (operand,) if isinstance(operand, torch.Tensor) else [t for t in operand if isinstance(t, torch.Tensor)]
+    if isinstance(operand, torch.Tensor):
+        return (operand,)
+    return [t for t in operand if isinstance(t, torch.Tensor)] if isinstance(operand, (tuple, list)) else ()
 
 
 def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None):
@@ -407,7 +409,8 @@ def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None
     linear_fp8_reference. The backward can be captured in a CUDA graph with the forward; as with every autograd backward
     under capture, no graph of the same leaves that was built outside the capture may be alive then.
     """
-    grad = torch.is_grad_enabled() and _wants_grad(*_tensors(x), *_tensors(weight), bias)
+    grad = (torch.is_grad_enabled() or forward_ad._current_level >= 0) and \
+        _wants_grad(*_tensors(x), *_tensors(weight), bias)
     dtype = _native.check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad)
     cuda = (x if isinstance(x, torch.Tensor) else x[0]).is_cuda
     if cuda:

@@ -92,6 +92,9 @@ def test_forward_mode_tangents_are_refused(cuda):
     for operand, call in calls:
         call(operand)
         with forward_ad.dual_level():
+            dual = forward_ad.make_dual(operand, torch.ones_like(operand))
             with pytest.raises(RuntimeError, match='forward-mode'):
-                call(forward_ad.make_dual(operand, torch.ones_like(operand)))
+                call(dual)
+            with pytest.raises(RuntimeError, match='forward-mode'), torch.no_grad():  # (of reverse mode alone)
+                call(dual)
             call(operand)

@@ -182,6 +182,14 @@ def test_linear_refusals():
         dequantize_fp8(*x8, torch.float64)
 
 
+def test_linear_refuses_what_is_no_operand():
+    for bad in (None, 3.0):
+        with pytest.raises(RuntimeError, match='pair'):
+            linear_fp8(bad, torch.zeros(4, 8))
+        with pytest.raises(RuntimeError, match='pair'):
+            linear_fp8(torch.zeros(4, 8), bad)
+
+
 def test_quantising_refuses_to_cut_a_graph():
     """A result that looks differentiable and is not would train nothing."""
     x = torch.randn(3, 200, requires_grad=True)
