@@ -127,10 +127,14 @@ __global__ void __launch_bounds__(kNormThreads, norm_ctas<T, VEC, EPT, false>())
             for (int i = 0; i < NV; ++i) {
                 const int c = (lane + i * G) * VEC, e = scale_exponent(top[i]);
                 if (c < a.C && c % kBlock8 == 0) a.scale[row * blocks + c / kBlock8] = exp2_int(e);
-                if (c >= a.pitch) continue;  // (the pitch is a multiple of 16; behind C the values are zero)
+                if (c >= a.pitch) continue;  // (the pitch is a multiple of 16)
                 uint8_t* dst = a.q + row * a.pitch + c;
                 const float f = exp2_int(-e);
-                const float* w8 = v + i * VEC;
+                float* w8 = v + i * VEC;
+                if (c >= a.C) {  // zeros, where a NaN as the row's norm has made the products of zeros NaN
+#pragma unroll
+                    for (int k = 0; k < VEC; ++k) w8[k] = 0.f;
+                }
                 if constexpr (VEC == 8)
                     *reinterpret_cast<uint2*>(dst) = make_uint2(to_e4m3x4(w8, f), to_e4m3x4(w8 + 4, f));
                 else if constexpr (VEC == 4) *reinterpret_cast<uint32_t*>(dst) = to_e4m3x4(w8, f);

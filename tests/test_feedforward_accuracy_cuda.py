@@ -5,6 +5,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from fp8_oracle import behind_rows
 from marearts_tinydeform_b200 import (attention, deform_attn_layer, layer_norm, linear_fp8, ma_deform_attn, quantize_fp8,
                                       quantize_weight_fp8, rms_norm, sampling_producer)
 from test_feedforward_cpu import keeps_what_its_gradients_read
@@ -98,3 +99,18 @@ def test_forward_mode_tangents_are_refused(cuda):
             with pytest.raises(RuntimeError, match='forward-mode'), torch.no_grad():  # (of reverse mode alone)
                 call(dual)
             call(operand)
+
+
+def test_zeros_behind_rows_of_nan(policy):
+    """What lies behind an 8-bit row is zero, whatever the row holds: an infinity or a NaN in it, or (without eps) none
+    but zeros."""
+    for C in (129, 130, 136, 520, 521, 1030, 2057, 4099, 8190):
+        x = torch.randn(5, C, device='cuda')
+        x[0, 3], x[1, C - 1], x[2] = float('nan'), float('inf'), 0
+        w8 = quantize_weight_fp8(torch.randn(C, C if C < 2000 else 300, device='cuda'))
+        for x in (x, x.half(), x.repeat(60, 1)):
+            y = rms_norm(x, x.new_ones(C), eps=0.0, quantize=True)[0]
+            assert y[:3].float().isnan().any(1).all() and not behind_rows(y).any()
+            assert not behind_rows(quantize_fp8(x)[0]).any()
+            y = linear_fp8(x[:, :w8[0].shape[1]], w8, quantize=True)[0]
+            assert y[0].float().isnan().all() and not behind_rows(y).any()
