@@ -5,10 +5,11 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from fp8_oracle import behind_rows
+from fp8_oracle import behind_rows, through
 from marearts_tinydeform_b200 import (attention, deform_attn_layer, layer_norm, linear_fp8, ma_deform_attn, quantize_fp8,
                                       quantize_weight_fp8, rms_norm, sampling_producer)
 from test_feedforward_cpu import keeps_what_its_gradients_read
+from test_linear_fp8_cuda import ACTS, DTYPES, SHAPES, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -114,3 +115,96 @@ def test_zeros_behind_rows_of_nan(policy):
             assert not behind_rows(quantize_fp8(x)[0]).any()
             y = linear_fp8(x[:, :w8[0].shape[1]], w8, quantize=True)[0]
             assert y[0].float().isnan().all() and not behind_rows(y).any()
+
+
+def whole(*shape, seed, wide=None):
+    """Whole numbers from -15 to 15 (four bits, which survive any of the roundings to 8 bits), every 61st index along
+    the dimension `wide` times 8."""
+    gen = torch.Generator(device='cuda').manual_seed(seed)
+    v = torch.randint(-15, 16, shape, generator=gen, device='cuda').float()
+    if wide is not None:
+        v.select(wide, 0).mul_(8) if shape[wide] < 61 else v.movedim(wide, 0)[::61].mul_(8)
+    return v
+
+
+@pytest.mark.parametrize('shape', SHAPES, ids=str)
+@pytest.mark.parametrize('dtype', DTYPES, ids=str)
+def test_whole_numbers_are_exact(policy, dtype, shape):
+    """Products and all three gradients of whole numbers whose sums stay below 2^24 (at most 8200 * 225 + 135 * 64 * 225):
+    every partial sum is one, so the results are the exact ones, rounded once."""
+    M, K, N = shape
+    x, w = whole(M, K, seed=1, wide=1).to(dtype), whole(N, K, seed=2, wide=1).to(dtype)
+    b, g = whole(N, seed=3).to(dtype), whole(M, N, seed=4).to(dtype)
+    xd, wd, gd = x.double(), w.double(), g.double()
+    want = xd @ wd.t() + b.double()
+    w8 = quantize_weight_fp8(w)
+    assert torch.equal(linear_fp8(x, w8, b), want.to(dtype))
+    assert torch.equal(linear_fp8(quantize_fp8(x), w8, b, dtype=torch.float32).double(), want)
+    leaves = [t.requires_grad_() for t in (x, w, b)]
+    y = linear_fp8(*leaves)
+    assert torch.equal(y, want.to(dtype))
+    for got, exact in zip(torch.autograd.grad(y, leaves, g), (gd @ wd, gd.t() @ xd, gd.sum(0))):
+        assert torch.equal(got, exact.to(dtype))
+
+
+def test_a_bad_gradient_leaves_the_other_rows(policy):
+    """An infinity and a NaN in the incoming gradient take their row of grad_x and of grad_weight; the others keep their
+    bits."""
+    x, w, g = normal(300, 200), normal(140, 200, seed=1), normal(300, 140, seed=3)
+
+    def grads():
+        leaves = [t.detach().requires_grad_() for t in (x, w)]
+        return torch.autograd.grad(linear_fp8(*leaves), leaves, g)
+
+    clean = grads()
+    g[7, 3], g[250, 139] = float('inf'), float('nan')
+    for got, want, bad in zip(grads(), clean, ([7, 250], [3, 139])):
+        rest = [i for i in range(got.shape[0]) if i not in bad]
+        assert got[bad].isnan().all() and torch.equal(got[rest], want[rest])
+
+
+@pytest.mark.parametrize('act', ACTS, ids=str)
+@pytest.mark.parametrize('M', (1, 9, 200))
+def test_bad_columns_leave_an_8_bit_block_its_rounding(policy, M, act):
+    """NaN in columns of a block: the others are the float32 results rounded with the scale that these call for, to half a
+    step (2^-4 of the value, 2^-10 of the scale; 2^-20 for the sums' own roundings)."""
+    x, w, b = normal(M, 300), normal(270, 300, seed=1), normal(270, seed=2)
+    bad = [5, 140, 269]
+    w[5, 299], w[140, 0], b[269] = float('nan'), float('inf'), float('nan')
+    w8 = quantize_weight_fp8(w)
+    v = linear_fp8(x, w8, b, act).double()
+    data, scale = (t.double() for t in linear_fp8(x, w8, b, act, quantize=True))
+    assert data[:, bad].isnan().all()
+    for block in range(3):
+        cols = [n for n in range(128 * block, min(270, 128 * block + 128)) if n not in bad]
+        s, top = scale[:, block], v[:, cols].abs().amax(1)
+        assert (top <= 448 * s * (1 + 2.0 ** -20)).all() and (top > 224 * s * (1 - 2.0 ** -20)).all()
+        off = (data[:, cols] * s[:, None] - v[:, cols]).abs()
+        assert (off <= (2.0 ** -4 + 2.0 ** -20) * v[:, cols].abs() + 2.0 ** -10 * s[:, None]).all()
+
+
+def held_to_blocks(got, a, b):
+    """got = a b^T in float32: a block's 128 exact products are added in float32 (128 roundings or cuts), the blocks of K
+    in turn, and perhaps the parts of a split sum, no more than there are blocks; 16 more for the scales and the rest."""
+    a, b = a.double(), b.double()
+    mag, blocks = a.abs() @ b.abs().t(), -(-a.shape[1] // 128)
+    off, allowed = (got.double() - a @ b.t()).abs(), (128 + 2 * blocks + 16) * 2 * E * mag + 2.0 ** -149
+    assert (off <= allowed).all(), f'{(off / allowed).max().item()} of what it may be off'
+
+
+@pytest.mark.parametrize('shape', [(1, 4096, 700), (16, 4100, 512), (33, 4099, 40), (130, 8200, 130), (5000, 384, 1000),
+                                   (40, 300, 20000), (20000, 100, 60)], ids=str)
+def test_long_sums_are_held_to_float32(policy, shape):
+    """Sums over many blocks, in the product and in both gradients, to roundings that count blocks and not values."""
+    M, K, N = shape
+    x, w, g = normal(M, K), normal(N, K, seed=1), normal(M, N, seed=2)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    y = linear_fp8(*leaves)
+    gx, gw = torch.autograd.grad(y, leaves, g)
+    x, w, y = x.detach(), w.detach(), y.detach()
+    x8, w8 = through(x, 1, 128), through(w, 128, 128)
+    held_to_blocks(y, x8, w8)
+    with torch.no_grad():
+        held_to_blocks(linear_fp8(x, quantize_weight_fp8(w)), x8, w8)
+    held_to_blocks(gx, through(g, 1, 128), w8.t())
+    held_to_blocks(gw, through(g, 128, 1).t(), through(x8, 128, 1).t())
