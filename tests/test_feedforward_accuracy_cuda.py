@@ -8,7 +8,7 @@ from torch.autograd import forward_ad
 from fp8_oracle import behind_rows, through
 from marearts_tinydeform_b200 import (attention, deform_attn_layer, layer_norm, linear_fp8, ma_deform_attn, quantize_fp8,
                                       quantize_weight_fp8, rms_norm, sampling_producer)
-from test_feedforward_cpu import keeps_what_its_gradients_read
+from test_feedforward_cpu import check_feed_forward, keeps_what_its_gradients_read
 from test_linear_fp8_cuda import ACTS, DTYPES, SHAPES, normal
 
 pytestmark = pytest.mark.gpu
@@ -208,3 +208,7 @@ def test_long_sums_are_held_to_float32(policy, shape):
         held_to_blocks(linear_fp8(x, quantize_weight_fp8(w)), x8, w8)
     held_to_blocks(gx, through(g, 1, 128), w8.t())
     held_to_blocks(gw, through(g, 128, 1).t(), through(x8, 128, 1).t())
+
+
+def test_a_models_feed_forward_half_in_serving(policy):
+    check_feed_forward('cuda')

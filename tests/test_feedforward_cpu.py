@@ -182,6 +182,38 @@ def test_linear_refusals():
         dequantize_fp8(*x8, torch.float64)
 
 
+def feed_forward(linear1, linear2, gain, out, tgt):
+    """A serving layer's feed-forward half from a model's parameters, as a user writes it."""
+    w1, w2 = quantize_weight_fp8(linear1.weight), quantize_weight_fp8(linear2.weight)
+    with torch.no_grad():
+        h, tgt = rms_norm(out, gain, residual=tgt, return_sum=True, quantize=True)
+        a = linear_fp8(h, w1, linear1.bias, activation='relu', quantize=True)
+        return linear_fp8(a, w2, linear2.bias, dtype=tgt.dtype), tgt
+
+
+def check_feed_forward(device):
+    torch.manual_seed(0)
+    layers = [torch.nn.Linear(*s, device=device) for s in ((256, 512), (512, 256))]
+    gain = torch.nn.Parameter(torch.rand(256, device=device) + 0.5)
+    out, tgt = (torch.randn(3, 20, 256, device=device) for _ in range(2))
+    y, s = feed_forward(*layers, gain, out, tgt)
+    assert torch.equal(s, out + tgt) and not y.requires_grad
+    with torch.no_grad():
+        h = s * torch.rsqrt(s.square().mean(-1, keepdim=True) + 1e-6) * gain
+        want = layers[1](torch.relu(layers[0](h)))
+    # the operands' roundings to 8 bits, 2^-4 at most each: about 3 % of independent terms
+    assert (y - want).norm() <= 0.1 * want.norm()
+    h8 = rms_norm(out, gain.detach(), residual=tgt, quantize=True)
+    with pytest.raises(RuntimeError, match='gradients need'):  # a bias that requires grad, outside no_grad
+        linear_fp8(h8, quantize_weight_fp8(layers[0].weight), layers[0].bias, activation='relu', quantize=True)
+    with pytest.raises(RuntimeError, match='no gradient'):
+        rms_norm(out, gain, residual=tgt, quantize=True)
+
+
+def test_a_models_feed_forward_half_in_serving():
+    check_feed_forward('cpu')
+
+
 def test_linear_refuses_what_is_no_operand():
     for bad in (None, 3.0):
         with pytest.raises(RuntimeError, match='pair'):
