@@ -26,14 +26,12 @@ The rest of a decoder layer's attention half, forward and backward:
     attention(query, key, value, key_padding_mask, attn_mask, causal, scale)   -> [B, Q, H * D]
     layer_norm(x, weight, bias, residual, eps)                                -> x's shape
 
-and its feed-forward half, with products in 8-bit floating point (e4m3, a scale for each block of 128), forward and
-backward:
+the self attention among the queries, and the norm over a sublayer's result plus its residual. Its feed-forward half,
+with products in 8-bit floating point (e4m3, a scale for each block of 128), forward and backward:
 
     rms_norm(x, weight, residual, eps, return_sum, quantize)                   -> x's shape, or 8-bit (data, scale)
     linear_fp8(x, weight, bias, activation, quantize, dtype)                   -> [..., N], or 8-bit (data, scale)
     quantize_fp8(x), quantize_weight_fp8(weight), dequantize_fp8(data, scale, dtype)
-
-the self attention among the queries, and the norm over a sublayer's result plus its residual.
 
 CPU tensors run ``ma_deform_attn_reference`` (as upstream does). CUDA tensors run only the native library; if it is
 missing, the call raises. Unlike upstream (inference only), this package's ``ma_deform_attn`` differentiates CUDA
@@ -324,10 +322,9 @@ def rms_norm(x, weight, residual=None, eps=1e-6, return_sum=False, quantize=Fals
 
     weight and residual have x's dtype and device. s is not rounded before the norm, and the mean is float32 (float64
     for float64), so squares have to stay in its range. return_sum: the pair (result, s), s being what the next layer
-    adds to. quantize: the result in 8 bits,
-    as a pair (data, scale) like quantize_fp8's, rounded once; for calls without gradients, not for float64. CUDA
-    tensors run this library's kernels, forward and backward (the weight's gradient summed in a fixed order); CPU
-    tensors run rms_norm_reference.
+    adds to. quantize: the result in 8 bits, as a pair (data, scale) like quantize_fp8's, rounded once; for calls without
+    gradients, not for float64. CUDA tensors run this library's kernels, forward and backward (the weight's gradient
+    summed in a fixed order); CPU tensors run rms_norm_reference.
     """
     _native.check_rms_norm(x, weight, residual, eps, quantize)
     grad = _wants_grad(x, weight, residual)
@@ -346,10 +343,10 @@ def quantize_fp8(x):
     """x [..., K] in 8 bits (e4m3), a scale for each 128 values along the last dimension: the pair (data, scale) of
     float8_e4m3fn [..., K] and float32 [..., ceil(K / 128)]; x is about data * scale.
 
-    x: float32, float16 or bfloat16, up to 65536 wide (and 2^31 - 256 rows). Scales are powers of two, the smallest that bring a block's
-    largest finite magnitude to at most 448 (e4m3's largest); values are rounded to nearest, ties to even; infinities
-    and NaN become NaN. data's rows start 16 bytes apart or a multiple of that, so it is a view where K is not one. What
-    is in 8 bits has no gradient, so an x that requires grad is refused (linear_fp8 takes it as it is).
+    x: float32, float16 or bfloat16, up to 65536 wide (and 2^31 - 256 rows). Scales are powers of two, the smallest that
+    bring a block's largest finite magnitude to at most 448 (e4m3's largest); values are rounded to nearest, ties to
+    even; infinities and NaN become NaN. data's rows start 16 bytes apart or a multiple of that, so it is a view where K
+    is not one. What is in 8 bits has no gradient, so an x that requires grad is refused (linear_fp8 takes it as it is).
     """
     _native.check_fp8_source(x)
     if _wants_grad(x):
@@ -371,8 +368,8 @@ def quantize_weight_fp8(weight):
 
 def dequantize_fp8(data, scale, dtype):
     """data * scale in `dtype` (float32, float16 or bfloat16): what quantize_fp8's pair, or quantize_weight_fp8's, stands
-    for. bfloat16 and float32 hold the values of this package's own pairs exactly. Scales that require grad are refused:
-    a pair has no gradient."""
+    for. float32 holds the values of this package's own pairs exactly, bfloat16 those from 2^-126 on (below, its numbers
+    are further apart than theirs). Scales that require grad are refused: a pair has no gradient."""
     tiles = isinstance(data, torch.Tensor) and isinstance(scale, torch.Tensor) and data.dim() == 2 and \
         scale.dim() == 2 and scale.shape[0] != data.shape[0]
     _native.check_fp8_pair((data, scale), 'the input', tiles)

@@ -5,8 +5,8 @@
 //   q = e4m3(v 2^-e), to nearest, ties to even; an infinity or NaN becomes NaN (e4m3 has no infinity)
 //
 // Scales are powers of two: a product with one is exact, so a value is rounded once, a quantised value is exact in
-// bfloat16, and values kept in 8 bits are quantised again along the other axis without a second rounding (but for those
-// below the other block's smallest step). Floating-point codes lose nothing by it: their relative step is the same
+// float32 (and from 2^-126 on in bfloat16), and values kept in 8 bits are quantised again along the other axis without a
+// second rounding (but for those below the other block's smallest step). Floating-point codes lose nothing by it: their relative step is the same
 // anywhere in the range. Blocks are 1 x 128 (activations: along the contraction), 128 x 1 (the same tensors when rows
 // are contracted, as in the weight's gradient) or 128 x 128 (weights, whose blocks stay blocks when transposed).
 //

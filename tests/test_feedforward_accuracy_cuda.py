@@ -5,9 +5,9 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
-from fp8_oracle import behind_rows, through
-from marearts_tinydeform_b200 import (attention, deform_attn_layer, layer_norm, linear_fp8, ma_deform_attn, quantize_fp8,
-                                      quantize_weight_fp8, rms_norm, sampling_producer)
+from fp8_oracle import behind_rows, quantized, through, worth
+from marearts_tinydeform_b200 import (attention, deform_attn_layer, dequantize_fp8, layer_norm, linear_fp8, ma_deform_attn,
+                                      quantize_fp8, quantize_weight_fp8, rms_norm, sampling_producer)
 from test_feedforward_cpu import check_feed_forward, keeps_what_its_gradients_read
 from test_linear_fp8_cuda import ACTS, DTYPES, SHAPES, normal
 
@@ -181,6 +181,26 @@ def test_bad_columns_leave_an_8_bit_block_its_rounding(policy, M, act):
         assert (top <= 448 * s * (1 + 2.0 ** -20)).all() and (top > 224 * s * (1 - 2.0 ** -20)).all()
         off = (data[:, cols] * s[:, None] - v[:, cols]).abs()
         assert (off <= (2.0 ** -4 + 2.0 ** -20) * v[:, cols].abs() + 2.0 ** -10 * s[:, None]).all()
+
+
+@pytest.mark.parametrize('dtype', (torch.float32, torch.bfloat16), ids=str)
+def test_tiny_values_go_to_8_bits_and_back(cuda, dtype):
+    """Below float32's normal numbers, where the scale cannot be smaller: data as by definition, from each kernel that
+    rounds, and back exactly."""
+    for C in (128, 136, 130):
+        x = whole(40, C, seed=9).double() * 2.0 ** -torch.arange(108, 148, device='cuda').double()[:, None]
+        x = x.float().to(dtype)
+        for make, rows in ((quantize_fp8, 1), (quantize_weight_fp8, 128)):
+            for part in (x, x[20:].contiguous()):
+                q, s = quantized(part, rows, 128)
+                data, scale = make(part)
+                assert torch.equal(scale.double(), s) and torch.equal(data.double(), q)
+                assert torch.equal(dequantize_fp8(data, scale, torch.float32).double(), worth(q, s, rows, 128))
+        leaves = [t.requires_grad_() for t in (x, x[:30].clone())]
+        y = linear_fp8(*leaves)
+        data, scale, _ = y.grad_fn.saved_tensors  # a training call's copy of its input
+        q, s = quantized(x.detach(), 1, 128)
+        assert torch.equal(scale.double(), s) and torch.equal(data.double(), q)
 
 
 def held_to_blocks(got, a, b):
