@@ -175,7 +175,6 @@ size_t partial_floats(int64_t M, int64_t N, int64_t K) {
     return p.splits > 1 ? size_t(p.splits) * size_t(M) * size_t(N) : 0;
 }
 
-
 int make_map8(CUtensorMap* map, const Operand8& o, int64_t rows, int64_t K, int box_rows, char* err, size_t err_len) {
     const CUresult r =
         !o.blocks
@@ -188,8 +187,8 @@ int make_map8(CUtensorMap* map, const Operand8& o, int64_t rows, int64_t K, int 
 }
 
 template <int BN, typename T, bool COLS>
-int launch_tc_of(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Tc8Args& t, cudaStream_t stream, char* err,
-                 size_t err_len) {
+int launch_tc_of(const CUtensorMap& ma, const CUtensorMap& mb, const CUtensorMap& mo, const Tc8Args& t,
+                 cudaStream_t stream, char* err, size_t err_len) {
     constexpr auto kernel = fp8_product_tc_kernel<BN, T, COLS>;
     constexpr size_t smem = Tc8Layout<BN, COLS>::kBytes;
     static_assert(smem <= 227 * 1024, "shared memory of a CTA");
@@ -259,8 +258,9 @@ int launch_tc(const TcPlan& p, const Operand8& a, const Operand8& b, const End8&
     return out_dtype == TD_E4M3 ? finish(E4m3()) : by_type(out_dtype, finish);
 }
 
-// partial: partial_floats(M, N, K) of them. Operands start on 16-byte boundaries, as do their rows. (Products with a scale for each row of both operands, whose b.scale_row is
-// 1, have a result in a floating type, and scales a tile's width beyond N.)
+// partial: partial_floats(M, N, K) of them. Operands start on 16-byte boundaries, as do their rows. (Products with a
+// scale for each row of both operands, whose b.scale_row is 1, have a result in a floating type, and scales a tile's
+// width beyond N.)
 int launch_product(const Operand8& a, const Operand8& b, const End8& end, int out_dtype, int64_t M, int64_t N,
                    int64_t K, float* partial, cudaStream_t stream, char* err, size_t err_len) {
     const TcPlan p = plan_tc(M, N, K);
@@ -272,7 +272,9 @@ int launch_product(const Operand8& a, const Operand8& b, const End8& end, int ou
 // Whether a product of M rows that come in x_dtype is one of few (td_fp8_few.cuh). Rows wider than 8 bits are rounded
 // there as long as they are short: every CTA does that again, at 0.5 us a row and 1024 of K, where a launch of its own
 // is 1.2 us on the GPU and 2.5 us of the host's time (1 x 1024 x 256: 1.75 us against 3.0; 1 x 4096 x 4096: 7.7 against
-// 6.9, 18 against 20 with the host; 4 x 4096 x 1024: 7.1 against 4.9).
+// 6.9, 18 against 20 with the host; 4 x 4096 x 1024: 7.1 against 4.9). By these costs the GPU alone would change over
+// at about 2500 values and the whole call at about 7600; the limit lies between, so a captured graph pays up to 0.8 us
+// for what a call gains.
 bool few_takes(int x_dtype, int64_t M, int64_t K) {
     if (!host::best_policy()) return false;
     return x_dtype == TD_E4M3 ? M <= kFewMost : M <= kFewWide && M * K <= 4096;
@@ -285,8 +287,8 @@ int launch_few_of(const FewArgs& a, cudaStream_t stream, char* err, size_t err_l
     if constexpr (sizeof(T) == 1) {
         constexpr auto kernel = fp8_few_to8_kernel<X, TILES>;
         if (int rc = host::allow_smem<kernel>(smem + 16384, err, err_len)) return rc;
-        return host::launch(err, err_len, "fp8_few_to8_kernel", kernel, dim3((ctas + 7) / 8 * 8), dim3(kFewThreads), smem,
-                            stream, true, a);
+        return host::launch(err, err_len, "fp8_few_to8_kernel", kernel, dim3((ctas + 7) / 8 * 8), dim3(kFewThreads),
+                            smem, stream, true, a);
     } else {
         constexpr auto kernel = fp8_few_kernel<X, T, TILES>;
         if (int rc = host::allow_smem<kernel>(smem + 16384, err, err_len)) return rc;
@@ -348,7 +350,8 @@ TrainPlan plan_train(int64_t M, int64_t K, int64_t N, void* workspace) {
 }
 
 // A backward call's workspace: the gradient in 1 x 128 blocks, and, transposed, in blocks of 128 rows ([MB, N, 128]),
-// as is the input ([MB, K, 128]); the transposed weight; the parts of the bias's column sums, and of split products, one after the other.
+// as is the input ([MB, K, 128]); the transposed weight; the parts of the bias's column sums, and of split products,
+// one after the other.
 struct BackwardPlan {
     uint8_t *dy, *dyt, *xt, *wt;
     float *dy_scale, *dyt_scale, *xt_scale, *wt_scale, *sums, *partial;

@@ -23,7 +23,7 @@ __device__ __forceinline__ float reciprocal(float x) {
 // GELU, v Phi(v), by the upper tail h = 1 - Phi(|v|) = exp(-v^2 / 2) R, which keeps the digits of a lower tail that
 // 1 + erf loses (a tenth of the value at -5, all of it below -5.6). R = erfcx(|v| / sqrt 2) / 2 is smooth, in
 // t = 1 / (1 + 0.35 |v|) a polynomial times t, fitted to |v| < 15 (beyond, the tail is less than float32 holds) for the
-// least relative error, 3e-8. 177784 x 256 x 1024 with 8-bit results: 302 us, by erfcf 768, by 1 + erff 336.
+// least relative error, 3e-8. 177784 x 256 x 1024 with 8-bit results: 306 us, by erfcf 768, by 1 + erff 336.
 __device__ __forceinline__ float gelu(float v) {
     const float a = fabsf(v), t = reciprocal(fmaf(0.35f, a, 1.f));
     float p = -0.029163928f;
@@ -40,7 +40,7 @@ __device__ __forceinline__ float gelu(float v) {
 }
 
 // SiLU, v / (1 + exp(-v)), with the exponential at most 1, so that neither it nor the denominator leaves the range. The
-// same call 225 us; 206 with __expf(-v) and __fdividef, which is zero below -87.
+// same call 226 us; 206 with __expf(-v) and __fdividef, which is zero below -87.
 __device__ __forceinline__ float silu(float v) {
     const float e = expf(-fabsf(v));
     return (v < 0.f ? v * e : v) * reciprocal(1.f + e);
@@ -104,8 +104,11 @@ __global__ void __launch_bounds__(kSimtThreads8)
         for (int k1 = k0; k1 < k0 + kBlock8 && k1 < K; k1 += kSimtStep8) {
             for (int i = threadIdx.x; i < (kSimtRows8 + kBlock8) * kSimtStep8; i += kSimtThreads8) {
                 const int r = i / kSimtStep8, c = i % kSimtStep8, k = k1 + c, n = n0 + r - kSimtRows8;
-                if (r < kSimtRows8) sa[c][r] = m0 + r < M && k < K ? from_e4m3(a.q[(m0 + r) * a.pitch + k / kBlock8 * a.block + k % kBlock8]) : 0.f;
-                else sb[c][r - kSimtRows8] = n < N && k < K ? from_e4m3(b.q[n * b.pitch + k / kBlock8 * b.block + k % kBlock8]) : 0.f;
+                const int kb = k / kBlock8, at = k % kBlock8;
+                if (r < kSimtRows8)
+                    sa[c][r] = m0 + r < M && k < K ? from_e4m3(a.q[(m0 + r) * a.pitch + kb * a.block + at]) : 0.f;
+                else
+                    sb[c][r - kSimtRows8] = n < N && k < K ? from_e4m3(b.q[n * b.pitch + kb * b.block + at]) : 0.f;
             }
             __syncthreads();
 #pragma unroll 4

@@ -7,17 +7,19 @@
 // tensor cores work on the next block in another part of TMEM. The scales are so any float32 numbers, and the tensor
 // cores' own sums are never longer than 128 products, however long K is. What bounds it: a 128 x 256 block takes the
 // tensor cores 512 cycles, shared memory 768 by count (48 KB in, 48 KB out, 128 bytes a cycle) and the 8 epilogue warps
-// about 890 each (128 multiply-adds, 128 columns from TMEM, waits); with two TMEM buffers between them it goes around in
-// 1100. 8192 x 4096 x 4096 in 143 us (1.92 PFLOP/s), 177784 x 1024 x 256 71, 177784 x 256 x 1024 93, 2400 x 256 x 1024
-// 5.1, 300 x 256 x 1024 3.9; 16-bit results. Where K is short a tile's end counts as much as its blocks.
+// about 890 each (128 multiply-adds, 128 columns from TMEM, waits); with two TMEM buffers between them it goes around
+// in 1100. Three sets of operands in turn, 16-bit results: 8192 x 4096 x 4096 in 145 us (1.90 PFLOP/s), 177784 x 1024
+// x 256 72, 177784 x 256 x 1024 97, 2400 x 256 x 1024 5.6, 300 x 256 x 1024 4.3. Where K is short a tile's end counts
+// as much as its blocks: 67200 x 256 x 1024 38.5, with a bias 44; 177784 rows of it with 8-bit results 100, with a bias
+// 123, GELU as well 306.
 //
 // Persistent, one CTA an SM, output tiles of 128 x BN (columns fastest, so that the CTAs which share rows of A run
 // together). A tile's K may be split over `splits` units whose float32 parts another kernel adds in order (a long sum
 // behind few tiles: the weight's gradient). Roles: warps 0 - 7 the epilogue (TMEM lanes 32 (w % 4) .., columns
 // w / 4 * BN / 2 ..), warp 8 the TMA producers, two lanes a slot (as in td_gemm_tc.cuh, whose notes on the waits apply
 // here), warp 9 the MMA issuer (10 and 11 fill its warpgroup).
-// COLS (the weight's gradient): both operands are laid out a block of K at a time, so that a tile is bytes that follow one
-// another in memory, and B has a scale for each row and block, which the producers bring to shared memory.
+// COLS (the weight's gradient): both operands are laid out a block of K at a time, so that a tile is bytes that follow
+// one another in memory, and B has a scale for each row and block, which the producers bring to shared memory.
 // In 8-bit results a block of 128 columns of a row is one thread's (BN = 256), or two threads' (BN = 128).
 #pragma once
 

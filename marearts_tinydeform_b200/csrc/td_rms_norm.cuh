@@ -13,9 +13,9 @@
 //
 // A block of 128 channels is 128 / VEC neighbouring lanes of one vector, so its largest magnitude is a few shuffles;
 // without vectors (rows that start anywhere) it is 128 / G vectors of a warp's lanes, or four warps of one, which meet
-// in shared memory. 177784 x 256 bfloat16 with the residual: in 8 bits 41.5 us (5.5 TB/s), with the sum
-// 55 (6.6 TB/s), backward with the sum's gradient 79 (5.8 TB/s, with its column sums); 8800 x 515 float32, whose
-// rows start anywhere, 19 and 21.
+// in shared memory. 177784 x 256 bfloat16 with the residual: in 8 bits 42 us (5.4 TB/s), with the sum 57.5 (6.3 TB/s),
+// backward with the sum's gradient 78 (5.8 TB/s, with its column sums); 8800 x 515 float32, whose rows start anywhere,
+// forward and backward together 44.
 #pragma once
 
 #include "td_fp8.cuh"
