@@ -445,7 +445,8 @@ TD_API int td_rms_norm_backward(int dtype, const void* grad_y, const void* grad_
  * td_fp8_linear_backward: its gradients, where the roundings' own derivative counts as 1. x (rows x_pitch apart) and
  * x_scale: the forward's 8-bit copy, the only one of the input that is kept. weight [N, K] of dtype.
  *   grad_x = Q(grad_out) Qw(weight); grad_weight = Qc(grad_out)^T Qc(x), Qc: blocks of 128 rows of one column;
- *   grad_bias = sum over rows of grad_out (not rounded before). Each may be NULL. Sums are taken in a fixed order.
+ *   grad_bias = sum over rows of grad_out (not rounded before). Each may be NULL; weight is read for grad_x alone, x and
+ *   x_scale for grad_weight alone, and may be NULL without it. Sums are taken in a fixed order.
  *   workspace: td_fp8_linear_backward_workspace_bytes(M, K, N, whether each is wanted) bytes.
  * 0 <= M <= TD_MAX_FP8_ROWS, 1 <= K, N <= TD_MAX_FP8_WIDTH.
  */

@@ -180,10 +180,15 @@ def ma_deform_attn(memory, value_weight, value_bias, spatial_shapes, level_start
     return out if output_weight is None else _native.linear(out, output_weight, output_bias)
 
 
+def _in_dual_level():
+    """Whether forward-mode differentiation is under way (without torch's own name for it: its tensors are asked)."""
+    return getattr(forward_ad, '_current_level', 0) >= 0
+
+
 def _wants_grad(*ts):
     """Whether a call of these operands is differentiated. Forward-mode tangents, which the kernels would drop without a
     word, are refused (the CPU path carries them)."""
-    if forward_ad._current_level >= 0 and any(
+    if _in_dual_level() and any(
             t is not None and t.is_cuda and forward_ad.unpack_dual(t).tangent is not None for t in ts):
         raise RuntimeError('no forward-mode derivative on CUDA: differentiate in reverse mode')
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
@@ -406,7 +411,7 @@ def linear_fp8(x, weight, bias=None, activation=None, quantize=False, dtype=None
     linear_fp8_reference. The backward can be captured in a CUDA graph with the forward; as with every autograd backward
     under capture, no graph of the same leaves that was built outside the capture may be alive then.
     """
-    grad = (torch.is_grad_enabled() or forward_ad._current_level >= 0) and \
+    grad = (torch.is_grad_enabled() or _in_dual_level()) and \
         _wants_grad(*_tensors(x), *_tensors(weight), bias)
     dtype = _native.check_linear_fp8(x, weight, bias, activation, quantize, dtype, grad)
     cuda = (x if isinstance(x, torch.Tensor) else x[0]).is_cuda
