@@ -260,10 +260,10 @@ __device__ __forceinline__ void proj_tc_tiles(const CUtensorMap& map_a0, const C
     // Under programmatic dependent launch everything up to a thread's first global access overlaps the previous
     // kernel in the stream: each role waits for it (grid_dependency_wait) right before its first global read or
     // write, after the set-up work and the first pass through its code. The MMA and split warps touch only shared
-    // memory and TMEM, behind the producers; they wait for it too, so that their bounded waits give up after a second
-    // of their own and not of the previous kernel's. Dependents are released only after that wait (by the producer lanes):
-    // the sampler that follows in the project order reads this call's locations and weights before its own wait,
-    // so the kernels that wrote them must have completed.
+    // memory and TMEM, behind the producers (mbar_wait_behind: their bounded waits do not count the previous kernel's
+    // time). Dependents are released only after that wait (by the producer lanes): the sampler that follows in the
+    // project order reads this call's locations and weights before its own wait, so the kernels that wrote them must
+    // have completed.
 
     if (warp < Lay::kMmaWarp) {
         if (RES && warp == 0 && lane >= S && lane < S + KB) {
@@ -323,9 +323,8 @@ __device__ __forceinline__ void proj_tc_tiles(const CUtensorMap& map_a0, const C
             constexpr uint32_t idesc = (1u << 4) | (GemmKind<T>::kFormat << 7) | (GemmKind<T>::kFormat << 10) |
                                        (uint32_t(BN >> 3) << 17) | (uint32_t(kTcBM >> 4) << 24);
             int it = 0;
-            grid_dependency_wait();
             // resident weights: the slice has landed before the first MMA
-            bool ok = !RES || my_tiles == 0 || mbar_wait(wfull, 0u, kErrTmaWait);
+            bool ok = !RES || my_tiles == 0 || mbar_wait_behind(wfull, 0u, kErrTmaWait);
             for (int tc = 0; ok && tc < my_tiles; ++tc) {
                 const int acc = tc & 1;
                 if (!mbar_wait(&tempty[acc], uint32_t((tc >> 1) & 1) ^ 1u, kErrSlotWait)) break;
@@ -333,7 +332,7 @@ __device__ __forceinline__ void proj_tc_tiles(const CUtensorMap& map_a0, const C
                 const uint32_t d = tmem + uint32_t(acc * BN);
                 for (int kb = 0; kb < KB; ++kb, ++it) {
                     const int s = it % S;
-                    if (!mbar_wait(kSplit ? &split[s] : &full[s], uint32_t((it / S) & 1), kErrTmaWait)) {
+                    if (!mbar_wait_behind(kSplit ? &split[s] : &full[s], uint32_t((it / S) & 1), kErrTmaWait)) {
                         ok = false;
                         break;
                     }
@@ -492,10 +491,9 @@ __device__ __forceinline__ void proj_tc_tiles(const CUtensorMap& map_a0, const C
         // float32: split every landed slot into hi (in place) and lo
         const int tid = (warp - Lay::kSplitWarp0) * 32 + lane;  // 128 threads
         const int total = my_tiles * KB;
-        grid_dependency_wait();
         for (int it = 0; it < total; ++it) {
             const int s = it % S;
-            const bool landed = mbar_wait(&full[s], uint32_t((it / S) & 1), kErrTmaWait);
+            const bool landed = mbar_wait_behind(&full[s], uint32_t((it / S) & 1), kErrTmaWait);
             if (!__all_sync(0xffffffffu, landed)) break;  // warp-uniform, for the __syncwarp below
             float4* x = reinterpret_cast<float4*>(slot_a(s));
             float4* xl = reinterpret_cast<float4*>(slot_alo(s));

@@ -307,7 +307,10 @@ def test_bounded_waits_begin_behind_the_kernel_before():
     assert producer.index('grid_dependency_wait()') < producer.index('t0 = clock64()') < producer.index('mbar_test(')
     epilogue = role('td_fp8_tc.cuh', 'setmaxnreg.inc')
     assert epilogue.index('grid_dependency_wait()') < epilogue.index('mbar_wait_at(')
-    issuer = role('td_gemm_tc.cuh', '// MMA issuer.')
-    assert 0 < issuer.index('grid_dependency_wait()') < issuer.index('mbar_wait(')
-    splitter = role('td_gemm_tc.cuh', '// float32: split every landed slot')
-    assert 0 < splitter.index('grid_dependency_wait()') < splitter.index('mbar_wait(')
+    # the projection's roles wait for the kernel before where their time for a tile runs out, and then once more
+    for start, end in (('// MMA issuer.', 'mma_issue<T>'), ('// float32: split every landed slot', 'float4* x')):
+        text = role('td_gemm_tc.cuh', start)
+        text = text[:text.index(end)]
+        assert 'mbar_wait_behind(' in text and 'mbar_wait(&full' not in text and 'mbar_wait(wfull' not in text
+    patient = role('td_ptx.cuh', 'bool mbar_wait_behind(')
+    assert 0 < patient.index('grid_dependency_wait()') < patient.index('mbar_wait(bar, parity, err_code)')
